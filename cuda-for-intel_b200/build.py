@@ -26,8 +26,8 @@ CXXFLAGS = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-ffp-contract=
 
 def _deps(src):
     deps = [src] + [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".h", ".hpp", ".cuh"))]
-    deps.append(os.path.join(HERE, "..", "include", "cfi_subst.h"))
-    deps.append(os.path.join(HERE, "..", "include", "cfi_cublas.h"))
+    inc = os.path.join(HERE, "..", "include")
+    deps += [os.path.join(inc, f) for f in os.listdir(inc) if f.endswith(".h")]
     return [d for d in deps if os.path.exists(d)]
 
 

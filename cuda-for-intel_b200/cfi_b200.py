@@ -16,6 +16,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libcfi_b200.so")
 
 # ---- ggml types ----
+T_F32, T_F16 = 0, 1
 Q4_0, Q5_0, Q8_0, Q4_K, Q5_K, Q6_K = 2, 6, 8, 12, 13, 14
 BLOCK_BYTES = {Q4_0: 18, Q5_0: 22, Q8_0: 34, Q4_K: 144, Q5_K: 176, Q6_K: 210}
 QK = {Q4_0: 32, Q5_0: 32, Q8_0: 32, Q4_K: 256, Q5_K: 256, Q6_K: 256}
@@ -139,6 +140,14 @@ def lib():
     L.cfi_fused_mmvq_add_rmsnorm_q8_1.argtypes = [vp, vp, vp, i, i, vp, vp, vp, f, vp]
     L.cfi_fused_mmvq_swiglu_q8_1.argtypes = [vp, vp, vp, i, i, vp, vp]
     L.cfi_fused_mmvq_qkv_rope_store.argtypes = [vp, vp, vp, i, vp, vp, vp, vp, vp, i, i, i, i, f, vp]
+    cp = C.POINTER(PagedCache)
+    L.cfi_paged_page_bytes.argtypes = [cp]
+    L.cfi_paged_page_bytes.restype = C.c_size_t
+    L.cfi_paged_kv_store.argtypes = [cp, vp, vp, i, ll, ll, vp, i, vp]
+    L.cfi_paged_kv_load.argtypes = [cp, vp, vp, vp, ll, ll, i, vp]
+    L.cfi_paged_attention.argtypes = [cp, vp, i, ll, vp, i, ll, vp, i, vp, i, i, f, vp]
+    L.cfi_packed_attention.argtypes = [C.POINTER(PackedAttention), vp]
+    L.cfi_sample.argtypes = [vp, ll, i, i, vp, vp, vp, vp, vp, vp, vp, vp]
     _lib = L
     return L
 
@@ -310,6 +319,20 @@ class DecodeStep(C.Structure):
                 [("eps", C.c_float), ("theta", C.c_float)] +
                 [(n, C.c_void_p) for n in ("embd", "head", "out_norm", "x", "qkv", "qr", "o", "gu", "dn", "logits", "hq", "aq",
                                            "gq", "token", "pos")])
+
+
+class PagedCache(C.Structure):
+    """CfiPagedCache (include/cfi_serve.h)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p)] + [(n, C.c_int) for n in ("type", "n_pages", "page_size", "n_kv_head",
+                                                                                "head_dim")]
+
+
+class PackedAttention(C.Structure):
+    """CfiPackedAttention (include/cfi_serve.h)."""
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "k", "v", "out", "cu_q", "cu_kv")] +
+                [(n, C.c_longlong) for n in ("q_stride", "k_stride", "v_stride", "out_stride")] +
+                [(n, C.c_int) for n in ("n_seq", "n_q", "n_kv", "n_head", "n_kv_head", "head_dim", "out_type", "causal")] +
+                [("scale", C.c_float)])
 
 
 class Ctx:
@@ -594,6 +617,73 @@ def mmq_skinny_group(ty, xs, y, dsts, nrows, k, ncols, ncols_y=None, stride_row_
     rc = lib().cfi_mmq_skinny_group(ty, n, P(*xs), C.c_void_p(y), P(*dsts), U(*nrows), U(*srx), U(*scd), k, ncols,
                                     ncols_y or ncols, C.c_void_p(stream))
     check(rc, "cfi_mmq_skinny_group")
+
+
+# ---------------------------------------------------------------------------------------------
+# serving operators (include/cfi_serve.h); pointers are device addresses, strides in values
+# ---------------------------------------------------------------------------------------------
+def paged_cache(ty, k, v, n_pages, page_size, n_kv_head, head_dim):
+    """The description of a paged cache (F16 or Q8_0) whose pools lie at k and v; raises when the
+    library does not serve such a cache."""
+    c = PagedCache(k, v, ty, n_pages, page_size, n_kv_head, head_dim)
+    if lib().cfi_paged_page_bytes(C.byref(c)) == 0:
+        raise ValueError("no paged cache of type %d, %d pages of %d, %d heads of %d" % (ty, n_pages, page_size, n_kv_head, head_dim))
+    return c
+
+
+def paged_page_bytes(ty, page_size, n_kv_head, head_dim):
+    """Bytes of one page of a K or V pool (0 for a cache that is not served)."""
+    c = PagedCache(None, None, ty, 1, page_size, n_kv_head, head_dim)
+    return lib().cfi_paged_page_bytes(C.byref(c))
+
+
+def paged_kv_store(cache, k, v, slots, n_tokens, src_type=T_F32, k_stride=0, v_stride=0, stream=0):
+    """cfi_paged_kv_store: n_tokens rows of k and v (F32 or F16; strides 0: packed) into the cache's
+    int64 slots."""
+    w = cache.n_kv_head * cache.head_dim
+    rc = lib().cfi_paged_kv_store(cache, k, v, src_type, k_stride or w, v_stride or w, slots, n_tokens, stream)
+    if rc:
+        check(rc, "cfi_paged_kv_store")
+
+
+def paged_kv_load(cache, slots, k, v, n_tokens, k_stride=0, v_stride=0, stream=0):
+    """cfi_paged_kv_load: the cache's int64 slots as n_tokens f16 rows of k and v (strides 0: packed)."""
+    w = cache.n_kv_head * cache.head_dim
+    rc = lib().cfi_paged_kv_load(cache, slots, k, v, k_stride or w, v_stride or w, n_tokens, stream)
+    if rc:
+        check(rc, "cfi_paged_kv_load")
+
+
+def paged_attention(cache, q, out, table, lens, n_seq, n_head, max_pages, scale, q_type=T_F32, out_type=T_F32, q_stride=0,
+                    out_stride=0, stream=0):
+    """cfi_paged_attention: one new token for each of n_seq sequences (int32 page table of max_pages
+    a row, int32 lens) over the cache; q and out F32 or F16 (strides 0: packed)."""
+    w = n_head * cache.head_dim
+    rc = lib().cfi_paged_attention(cache, q, q_type, q_stride or w, out, out_type, out_stride or w, table, max_pages, lens,
+                                   n_seq, n_head, scale, stream)
+    if rc:
+        check(rc, "cfi_paged_attention")
+
+
+def packed_attention(q, k, v, out, cu_q, cu_kv, n_seq, n_q, n_kv, n_head, n_kv_head, head_dim, scale, causal=True,
+                     out_type=T_F32, q_stride=0, k_stride=0, v_stride=0, out_stride=0, stream=0):
+    """cfi_packed_attention: f16 q, k, v of n_seq packed sequences bounded by the int32 cu_q and cu_kv;
+    out F32 or F16 (strides 0: packed)."""
+    wq, wk = n_head * head_dim, n_kv_head * head_dim
+    a = PackedAttention(q, k, v, out, cu_q, cu_kv, q_stride or wq, k_stride or wk, v_stride or wk, out_stride or wq, n_seq,
+                        n_q, n_kv, n_head, n_kv_head, head_dim, out_type, causal, scale)
+    rc = lib().cfi_packed_attention(a, stream)
+    if rc:
+        check(rc, "cfi_packed_attention")
+
+
+def sample(logits, u, token, n_rows, n_vocab, temperature=0, top_k=0, top_p=0, min_p=0, logprob=0, row_stride=0, stream=0):
+    """cfi_sample: int32 token[row] from n_rows rows of f32 logits and the uniform numbers u; the
+    settings are device arrays of n_rows (0: off)."""
+    rc = lib().cfi_sample(logits, row_stride or n_vocab, n_rows, n_vocab, temperature or None, top_k or None, top_p or None,
+                          min_p or None, u, token, logprob or None, stream)
+    if rc:
+        check(rc, "cfi_sample")
 
 
 PEER_HANDLE_BYTES = 64

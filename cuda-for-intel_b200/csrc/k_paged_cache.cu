@@ -1,0 +1,207 @@
+// k_paged_cache.cu -- writing rows of K and V into the pages of a serving cache (quantised to Q8_0
+// where the cache is) and reading them back as f16.  include/cfi_serve.h gives the layout.
+//
+// Per block of 32 values x: d = max|x| / 127, q = rn(x * (1/d)), stored scale f16(d); read back as
+// f16(q * scale).  One thread moves 8 values (16 bytes of f16), four neighbours make a block.
+#include "paged_cache.cuh"
+#include "sm100_ptx.cuh"
+#include "cfi_kernels.h"
+
+#include <stdlib.h>
+#include <string.h>
+
+namespace {
+
+constexpr int PC_THREADS = 256;
+
+struct PcArgs {
+    uint8_t *k, *v;          // pools
+    const int64_t* slots;
+    const uint8_t *src_k, *src_v;  // store: rows in
+    uint8_t *dst_k, *dst_v;        // load: rows out
+    long long k_stride, v_stride;  // values
+    long long n_slots;
+    uint32_t n_items;        // tokens x kv heads x D / 8
+    int page_shift, n_kv_head;
+};
+
+CFI_DEV uint4 ldg_stream(const void* p) {  // read once: do not keep it in L1
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+template <int D, bool Q8, bool SRC_F16>
+__global__ void __launch_bounds__(PC_THREADS) paged_kv_store(const PcArgs a) {
+    sm100::pdl_launch_dependents();
+    sm100::pdl_wait();
+    constexpr int G = D / 8;  // threads a (token, head) row takes
+    const uint32_t i = blockIdx.x * PC_THREADS + threadIdx.x;
+    const bool in = i < a.n_items;
+    const uint32_t row = (in ? i : a.n_items - 1) / G, g = i % G;
+    const uint32_t t = row / a.n_kv_head, h = row - t * a.n_kv_head;
+    const long long slot = a.slots[t];
+    const bool ok = in && slot >= 0 && slot < a.n_slots;
+    const bool is_v = blockIdx.y;
+    const long long at = (long long)t * (is_v ? a.v_stride : a.k_stride) + h * D + g * 8;
+    float x[8];
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    if (SRC_F16) {
+        raw = ldg_stream((is_v ? a.src_v : a.src_k) + at * 2);
+        const __half2* p = reinterpret_cast<const __half2*>(&raw);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float2 f = __half22float2(p[j]);
+            x[2 * j] = f.x;
+            x[2 * j + 1] = f.y;
+        }
+    } else {
+        const uint8_t* p = (is_v ? a.src_v : a.src_k) + at * 4;
+        const uint4 lo = ldg_stream(p), hi = ldg_stream(p + 16);
+        const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = __uint_as_float(w[j]);
+        __half2* q = reinterpret_cast<__half2*>(&raw);
+#pragma unroll
+        for (int j = 0; j < 4; j++) q[j] = __floats2half2_rn(x[2 * j], x[2 * j + 1]);
+    }
+    const long long page = slot >> a.page_shift;
+    const int off = (int)(slot & ((1 << a.page_shift) - 1));
+    uint8_t* region = (is_v ? a.v : a.k) + (page * a.n_kv_head + h) * paged_region_bytes<D, Q8>(1 << a.page_shift);
+    if (!Q8) {
+        if (ok) *reinterpret_cast<uint4*>(region + ((size_t)off * D + g * 8) * 2) = raw;
+        return;
+    }
+    float m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) m = fmaxf(m, fabsf(x[j]));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    const float d = m / 127.0f, id = d > 0.0f ? 1.0f / d : 0.0f;
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const int q = max(-127, min(127, __float2int_rn(x[j] * id)));
+        w[j >> 2] |= (uint32_t)(q & 0xff) << (8 * (j & 3));
+    }
+    // fmaxf drops a NaN: a block that has one gets a NaN scale
+    uint32_t nan = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) nan |= (uint32_t)(x[j] != x[j]);
+    nan |= __shfl_xor_sync(0xffffffffu, nan, 1);
+    nan |= __shfl_xor_sync(0xffffffffu, nan, 2);
+    if (!ok) return;
+    *reinterpret_cast<uint2*>(region + (size_t)off * D + g * 8) = make_uint2(w[0], w[1]);
+    if ((g & 3) == 0)
+        *reinterpret_cast<uint16_t*>(region + (size_t)(D << a.page_shift) + ((size_t)off * (D / 32) + g / 4) * 2) =
+            nan ? (uint16_t)0x7fff : f2h_bits(d);
+}
+
+template <int D, bool Q8>
+__global__ void __launch_bounds__(PC_THREADS) paged_kv_load(const PcArgs a) {
+    sm100::pdl_launch_dependents();
+    sm100::pdl_wait();
+    constexpr int G = D / 8;
+    const uint32_t i = blockIdx.x * PC_THREADS + threadIdx.x;
+    if (i >= a.n_items) return;
+    const uint32_t row = i / G, g = i % G;
+    const uint32_t t = row / a.n_kv_head, h = row - t * a.n_kv_head;
+    const long long slot = a.slots[t];
+    const bool is_v = blockIdx.y;
+    uint4 out = make_uint4(0, 0, 0, 0);
+    if (slot >= 0 && slot < a.n_slots) {
+        const long long page = slot >> a.page_shift;
+        const int off = (int)(slot & ((1 << a.page_shift) - 1));
+        const uint8_t* region = (is_v ? a.v : a.k) + (page * a.n_kv_head + h) * paged_region_bytes<D, Q8>(1 << a.page_shift);
+        if (!Q8) {
+            out = ldg_stream(region + ((size_t)off * D + g * 8) * 2);
+        } else {
+            const uint2 q = *reinterpret_cast<const uint2*>(region + (size_t)off * D + g * 8);
+            const float d = h2f_bits(*reinterpret_cast<const uint16_t*>(region + (size_t)(D << a.page_shift) +
+                                                                        ((size_t)off * (D / 32) + g / 4) * 2));
+            __half2* o = reinterpret_cast<__half2*>(&out);
+            const uint32_t w[2] = {q.x, q.y};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t b = w[j >> 1] >> (16 * (j & 1));
+                o[j] = __floats2half2_rn(d * (float)(int8_t)(b & 0xff), d * (float)(int8_t)((b >> 8) & 0xff));
+            }
+        }
+    }
+    const long long at = (long long)t * (is_v ? a.v_stride : a.k_stride) + h * D + g * 8;
+    *reinterpret_cast<uint4*>((is_v ? a.dst_v : a.dst_k) + at * 2) = out;
+}
+
+int go(const void* fn, const PcArgs& a, cudaStream_t stream) {
+    const char* ep = getenv("CFI_PDL");
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3((a.n_items + PC_THREADS - 1) / PC_THREADS, 2, 1);
+    c.blockDim = dim3(PC_THREADS, 1, 1);
+    c.stream = stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = at;
+    c.numAttrs = (ep && strcmp(ep, "0") == 0) ? 0 : 1;
+    void* args[1] = {const_cast<PcArgs*>(&a)};
+    return (int)cudaLaunchKernelExC(&c, fn, args);
+}
+
+bool rows_ok(const void* k, const void* v, long long ks, long long vs, long long width, const void* slots, int n) {
+    return n >= 0 && k && v && slots && !(((uintptr_t)k | (uintptr_t)v) & 15) && !((uintptr_t)slots & 7) && ks % 8 == 0 &&
+           vs % 8 == 0 && ks >= width && vs >= width;
+}
+
+bool args_of(const CfiPagedCache* c, long long ks, long long vs, const int64_t* slots, int n, PcArgs* a) {
+    const long long items = (long long)n * c->n_kv_head * (c->head_dim / 8);
+    if (items > 0x7fffffffLL) return false;
+    a->k = static_cast<uint8_t*>(c->k);
+    a->v = static_cast<uint8_t*>(c->v);
+    a->slots = slots;
+    a->k_stride = ks;
+    a->v_stride = vs;
+    a->n_slots = (long long)c->n_pages * c->page_size;
+    a->n_items = (uint32_t)items;
+    a->page_shift = __builtin_ctz((unsigned)c->page_size);
+    a->n_kv_head = c->n_kv_head;
+    return true;
+}
+
+}  // namespace
+
+extern "C" size_t cfi_paged_page_bytes(const CfiPagedCache* c) {
+    if (!c || !cfi_paged_shape_ok(c)) return 0;
+    return (size_t)c->n_kv_head * c->page_size * (c->type == 1 ? (size_t)c->head_dim * 2 : (size_t)c->head_dim / 32 * 34);
+}
+
+extern "C" int cfi_paged_kv_store(const CfiPagedCache* c, const void* k, const void* v, int src_type, long long k_stride,
+                                  long long v_stride, const int64_t* slots, int n_tokens, void* stream) {
+    PcArgs a = {};
+    if (!cfi_paged_ok(c) || (src_type != 0 && src_type != 1) ||
+        !rows_ok(k, v, k_stride, v_stride, (long long)c->n_kv_head * c->head_dim, slots, n_tokens) ||
+        !args_of(c, k_stride, v_stride, slots, n_tokens, &a))
+        return (int)cudaErrorInvalidValue;
+    if (n_tokens == 0) return 0;
+    a.src_k = static_cast<const uint8_t*>(k);
+    a.src_v = static_cast<const uint8_t*>(v);
+    static const void* const fns[8] = {
+        (const void*)paged_kv_store<64, false, false>,  (const void*)paged_kv_store<64, false, true>,
+        (const void*)paged_kv_store<64, true, false>,   (const void*)paged_kv_store<64, true, true>,
+        (const void*)paged_kv_store<128, false, false>, (const void*)paged_kv_store<128, false, true>,
+        (const void*)paged_kv_store<128, true, false>,  (const void*)paged_kv_store<128, true, true>};
+    return go(fns[(c->head_dim == 128) * 4 + (c->type == 8) * 2 + src_type], a, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int cfi_paged_kv_load(const CfiPagedCache* c, const int64_t* slots, void* k, void* v, long long k_stride,
+                                 long long v_stride, int n_tokens, void* stream) {
+    PcArgs a = {};
+    if (!cfi_paged_ok(c) || !rows_ok(k, v, k_stride, v_stride, (long long)c->n_kv_head * c->head_dim, slots, n_tokens) ||
+        !args_of(c, k_stride, v_stride, slots, n_tokens, &a))
+        return (int)cudaErrorInvalidValue;
+    if (n_tokens == 0) return 0;
+    a.dst_k = static_cast<uint8_t*>(k);
+    a.dst_v = static_cast<uint8_t*>(v);
+    static const void* const fns[4] = {(const void*)paged_kv_load<64, false>, (const void*)paged_kv_load<64, true>,
+                                       (const void*)paged_kv_load<128, false>, (const void*)paged_kv_load<128, true>};
+    return go(fns[(c->head_dim == 128) * 2 + (c->type == 8)], a, static_cast<cudaStream_t>(stream));
+}
