@@ -1,65 +1,432 @@
-// k_packed_attn_sm100.cu -- causal attention of packed sequences (include/cfi_serve.h).
+// k_packed_attn_sm100.cu -- causal attention of packed sequences (include/cfi_serve.h) on the
+// 5th-generation tensor cores: O = softmax(scale Q K') V by blocks of 128 keys, with a running row
+// maximum and sum, so that no score leaves the SM.
 //
-// One warp per (query, head) walks the keys it sees with a running maximum and sum.
+// Rows are (token, head) pairs of one kv head's group: a tile is floor(128 / G) tokens times the G query
+// heads that share the kv head, one TMA box in token-major order.  That fills the 128 rows of an MMA
+// for any group (126 for 7, 126 for 6, 128 for 4), keeps a tile's tokens close together (few keys past
+// the diagonal), and reads K and V once for the whole group.
+//
+// A CTA of 384 threads has two tiles, A and B, of neighbouring tokens, over the same keys:
+//   * warps 0-3 run the softmax of tile A, warps 4-7 that of B, a thread for each row (TMEM lane): the
+//     128 scores of a block come from tensor memory into registers, the weights go back over them
+//     as f16, the A operand of the product with V.  The rows of O are rescaled only when a row's maximum
+//     has grown by more than 2^8 since the last time (weights stay far inside f16);
+//   * warp 8 issues the MMAs: O_A += P_A V_j, S_A = Q_A K_j+1', then the same for B, so that the tensor
+//     pipe works on one tile while the other is in its softmax;
+//   * warp 9 brings Q and the ring of K and V blocks by TMA.  V rows past the sequence's end are zeroed
+//     in shared memory (the next sequence's rows are there, and 0 x NaN would reach this one).
+//
+// Tensor memory: S_A, S_B (128 columns each; P over the first 64), O_A, O_B (D columns each).
 #include "../../include/cfi_serve.h"
 #include "sm100_ptx.cuh"
 #include "cfi_kernels.h"
 
+#include <math.h>
 #include <stdlib.h>
 #include <string.h>
 
 namespace {
 
-constexpr int KA_WARPS = 4;
+using namespace sm100;
+
+constexpr int KA_MMA_WARP = 8, KA_TMA_WARP = 9, KA_THREADS = 384;
+// Registers: 384 threads start with 168 each; the softmax warps take 208 (a row's 128 scores stay in
+// them) and the other four give up theirs: 256 x 208 + 128 x 88 = 384 x 168.
+constexpr int KA_REGS_SOFTMAX = 208, KA_REGS_OTHER = 88;
+constexpr int KA_M = 128, KA_N = 128;       // rows of a tile, keys of a block
+constexpr uint32_t KA_TMEM_COLS = 512;
+constexpr float KA_RESCALE_LOG2 = 8.0f;
+template <int D> constexpr int ka_slots() { return D == 64 ? 8 : 5; }  // K and V blocks in flight
+template <int D> constexpr uint32_t ka_tile_bytes() { return KA_M * D * 2; }
+template <int D> constexpr size_t ka_smem() { return 1024 + (2 + ka_slots<D>()) * (size_t)ka_tile_bytes<D>() + 256; }
+
+struct KaArgs {
+    void* out;
+    const int32_t *cu_q, *cu_kv;
+    long long out_stride;
+    int n_seq, n_q, n_kv, group, tokens;  // tokens a tile has
+    int out_f16, causal;
+    float scale_log2;
+    unsigned int* err;
+};
+
+CFI_DEV float ex2(float x) {  // 2^x (PTX ex2.approx; -inf -> +0)
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 template <int D>
-__global__ void __launch_bounds__(KA_WARPS * 32) packed_attn(const CfiPackedAttention a) {
-    sm100::pdl_launch_dependents();
-    sm100::pdl_wait();
-    constexpr int E = D / 32;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int t = blockIdx.x * KA_WARPS + warp, head = blockIdx.y, kvh = head / (a.n_head / a.n_kv_head);
-    if (t >= min(a.n_q, a.cu_q[a.n_seq])) return;
-    int lo = 0, hi = a.n_seq;  // the sequence: cu_q[lo] <= t < cu_q[lo + 1]
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (a.cu_q[mid] <= t)
-            lo = mid;
+__global__ void __launch_bounds__(KA_THREADS, 1)
+    packed_attn(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                const __grid_constant__ CUtensorMap tv, const KaArgs a) {
+    constexpr int DB = D / 64;  // 64-value blocks of a row: one 128-byte swizzle atom column each
+    constexpr int NS = ka_slots<D>();
+    constexpr uint32_t TILE = ka_tile_bytes<D>(), BLK = KA_M * 128;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t* sQ = smem;             // tiles A, B
+    uint8_t* ring = smem + 2 * TILE;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(ring + NS * TILE);
+    uint64_t* full = bars;          // [NS] a block's TMA bytes
+    uint64_t* empty = bars + NS;    // [NS] the MMAs that read it are done
+    uint64_t* s_full = bars + 2 * NS;      // [2] scores of a block (and O up to the block before)
+    uint64_t* p_full = bars + 2 * NS + 2;  // [2] its weights (a warp each arrives)
+    uint64_t* o_full = bars + 2 * NS + 4;  // [2] O complete
+    uint64_t* q_full = bars + 2 * NS + 6;
+    uint64_t* v_clean = bars + 2 * NS + 7;  // V rows past the end are zeroed
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * NS + 8);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kvh = blockIdx.y;
+    pdl_launch_dependents();
+    pdl_wait();  // lengths, q, k and v may come from the kernel before
+
+    // ---- which pair of tiles: sequence s, its pair number from the last (the longest) to the first ----
+    const int span = 2 * a.tokens;
+    int s = -1, pair = 0, q0 = 0, nq = 0;
+    for (int base = 0, acc = 0; base < a.n_seq && s < 0; base += 32) {
+        int b0 = 0, n = 0;
+        if (base + lane < a.n_seq) {
+            b0 = min(max(a.cu_q[base + lane], 0), a.n_q);
+            n = min(a.cu_q[base + lane + 1], a.n_q) - b0;
+        }
+        const int c = n > 0 ? (n + span - 1) / span : 0;
+        int incl = c;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += x;
+        }
+        const uint32_t hit = __ballot_sync(0xffffffffu, acc + incl > (int)blockIdx.x);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            s = base + l;
+            q0 = __shfl_sync(0xffffffffu, b0, l);
+            nq = __shfl_sync(0xffffffffu, n, l);
+            pair = acc + __shfl_sync(0xffffffffu, incl, l) - 1 - (int)blockIdx.x;
+        }
+        acc += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (s < 0) return;
+    const int k0 = min(max(a.cu_kv[s], 0), a.n_kv), nk = max(min(a.cu_kv[s + 1], a.n_kv) - k0, 0);
+    // keys that token t sees, and blocks that a tile needs (its last token sees the most)
+    auto seen = [&](int t) { return a.causal ? max(0, min(nk, t + nk - nq + 1)) : nk; };
+    auto first_token = [&](int x) { return pair * span + x * a.tokens; };
+    auto blocks = [&](int x) {
+        const int t = first_token(x);
+        return t < nq ? (seen(min(nq, t + a.tokens) - 1) + KA_N - 1) / KA_N : 0;
+    };
+    const int nb0 = blocks(0), nb1 = blocks(1), nmax = max(nb0, nb1);
+    const bool cut = nmax * KA_N > nk;  // the last block runs past the sequence
+
+    if (tid == 0) {
+        for (int i = 0; i < NS; i++) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        for (int x = 0; x < 2; x++) {
+            mbar_init(&s_full[x], 1);
+            mbar_init(&p_full[x], 4);
+            mbar_init(&o_full[x], 1);
+        }
+        mbar_init(q_full, 1);
+        mbar_init(v_clean, 1);
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == KA_MMA_WARP) {
+        tmem_alloc(tmem_slot, KA_TMEM_COLS);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    auto fail = [&](unsigned code) {
+        cfi_set_error(a.err, code);
+        *abort_flag = 1;
+    };
+
+    if (warp >= KA_MMA_WARP) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KA_REGS_OTHER));
+      if (warp == KA_TMA_WARP) {
+        bool ok = true;
+        if (lane == 0 && nmax > 0) {
+            const uint32_t rows = (uint32_t)(a.tokens * a.group);
+            mbar_arrive_expect_tx(q_full, 2 * DB * rows * 128);
+            for (int x = 0; x < 2; x++)
+                for (int b = 0; b < DB; b++)  // a tile past the sequence loads rows that nothing uses
+                    tma_load_3d(sQ + x * TILE + b * BLK, &tq, 64 * b, kvh * a.group, q0 + first_token(x), q_full);
+            for (int i = 0; ok && i < 2 * nmax; i++) {
+                const int st = i % NS;
+                ok = mbar_wait(&empty[st], ((uint32_t)(i / NS) & 1) ^ 1, abort_flag);
+                if (!ok) break;
+                mbar_arrive_expect_tx(&full[st], TILE);
+                for (int b = 0; b < DB; b++)
+                    tma_load_3d(ring + st * TILE + b * BLK, (i & 1) ? &tv : &tk, 64 * b, kvh, k0 + (i >> 1) * KA_N, &full[st]);
+            }
+            if (!ok) fail(0xfb100);
+        }
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+        if (ok && cut) {
+            const int i = 2 * nmax - 1, st = i % NS;
+            if (__all_sync(0xffffffffu, mbar_wait(&full[st], (uint32_t)(i / NS) & 1, abort_flag))) {
+                const int r0 = nk - (nmax - 1) * KA_N;  // first row past the end
+                uint4* v = reinterpret_cast<uint4*>(ring + st * TILE);
+                for (int c = lane; c < (KA_N - r0) * 8; c += 32)
+                    for (int b = 0; b < DB; b++) v[b * (BLK / 16) + r0 * 8 + c] = make_uint4(0, 0, 0, 0);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(v_clean);
+            } else if (lane == 0) {
+                fail(0xfb110);
+            }
+        }
+      } else if (warp == KA_MMA_WARP) {
+        if (lane == 0 && nmax > 0) {
+            const uint32_t id_s = idesc_f16(KA_M, KA_N, 0);
+            const uint32_t id_o = idesc_f16(KA_M, D, 0) | (1u << 16);  // B (V) MN-major
+            // descriptors of Q and the first slot; an offset of n bytes adds n / 16
+            const uint64_t dq = sw128_kmajor_desc(smem_u32(sQ)), dk = sw128_kmajor_desc(smem_u32(ring)),
+                           dv = sw128_mnmajor_desc(smem_u32(ring), BLK);
+            auto scores = [&](int x, int st) {  // S_x = Q_x K'
+#pragma unroll
+                for (int kk = 0; kk < D / 16; kk++) {
+                    const uint32_t off = (kk >> 2) * BLK + (kk & 3) * 32;
+                    mma_f16(tmem + x * KA_N, dq + ((x * TILE + off) >> 4), dk + st * (TILE >> 4) + (off >> 4), id_s, kk > 0 ? 1u : 0u);
+                }
+                mma_commit(&s_full[x]);
+            };
+            auto values = [&](int x, int st, bool first) {  // O_x += P_x V
+#pragma unroll
+                for (int kk = 0; kk < KA_N / 16; kk++)
+                    mma_f16_ts(tmem + 256 + x * D, tmem + x * KA_N + kk * 8, dv + st * (TILE >> 4) + kk * (16 * 128 >> 4), id_o,
+                               (!first || kk > 0) ? 1u : 0u);
+            };
+            bool ok = mbar_wait(q_full, 0, abort_flag) && mbar_wait(&full[0], 0, abort_flag);
+            if (ok) {
+                tc_fence_after();
+#pragma unroll
+                for (int x = 0; x < 2; x++)
+                    if ((x ? nb1 : nb0) > 0) scores(x, 0);
+                mma_commit(&empty[0]);
+            }
+            for (int j = 0; ok && j < nmax; j++) {
+                const int iv = 2 * j + 1, ik = 2 * j + 2, sv = iv % NS, sk = ik % NS;
+                ok = mbar_wait(&full[sv], (uint32_t)(iv / NS) & 1, abort_flag);
+                if (ok && cut && j == nmax - 1) ok = mbar_wait(v_clean, 0, abort_flag);
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const int n = x ? nb1 : nb0;
+                    if (ok && j < n) {
+                        ok = mbar_wait(&p_full[x], (uint32_t)j & 1, abort_flag);
+                        if (!ok) break;
+                        tc_fence_after();
+                        values(x, sv, j == 0);
+                        if (j == n - 1) mma_commit(&o_full[x]);
+                    }
+                    if (x == 1) mma_commit(&empty[sv]);
+                    if (j + 1 < n) {
+                        ok = mbar_wait(&full[sk], (uint32_t)(ik / NS) & 1, abort_flag);
+                        if (!ok) break;
+                        scores(x, sk);
+                    }
+                    if (x == 1 && j + 1 < nmax) mma_commit(&empty[sk]);
+                }
+            }
+            if (!ok) fail(0xfb200);
+        }
+      }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(KA_REGS_SOFTMAX));
+        // ---- softmax: row r of tile x ----
+        const int x = warp >> 2, r = 32 * (warp & 3) + lane;
+        const int t = first_token(x) + r / a.group, n_blocks = x ? nb1 : nb0;
+        const bool valid = r < a.tokens * a.group && t < nq;
+        const int limit = valid ? seen(t) : 0;
+        const uint32_t trow = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+        const uint32_t ts = trow + x * KA_N, to = trow + 256 + x * D;
+        // blocks below this one are seen whole by every row of the tile
+        const int n_whole = seen(first_token(x)) / KA_N;
+        float m_used = -INFINITY, l = 0.0f;
+        bool ok = true;
+        for (int j = 0; j < n_blocks; j++) {
+            if (!__all_sync(0xffffffffu, mbar_wait(&s_full[x], (uint32_t)j & 1, abort_flag))) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            uint32_t sv[4][32];
+#pragma unroll
+            for (int c = 0; c < 4; c++) tmem_ld32(ts + 32 * c, sv[c]);
+            tmem_ld_wait();
+            if (j >= n_whole) {
+                const int left = limit - j * KA_N;
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+#pragma unroll
+                    for (int i = 0; i < 32; i++)
+                        if (32 * c + i >= left) sv[c][i] = 0xff800000u;
+            }
+            float mx4[4];
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                mx4[c] = __uint_as_float(sv[c][0]);
+#pragma unroll
+                for (int i = 1; i < 32; i++) mx4[c] = fmaxf(mx4[c], __uint_as_float(sv[c][i]));
+            }
+            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * a.scale_log2;
+            const bool grow = valid && (mx > m_used + KA_RESCALE_LOG2 || (m_used == -INFINITY && mx > -INFINITY));
+            if (__any_sync(0xffffffffu, grow)) {
+                const float alpha = !grow ? 1.0f : m_used == -INFINITY ? 0.0f : ex2(m_used - mx);
+                if (grow) m_used = mx;
+                l *= alpha;
+                if (j > 0) {  // the product before is complete: its MMAs were committed before these scores
+#pragma unroll
+                    for (int c = 0; c < D / 32; c++) {
+                        uint32_t v[32];
+                        tmem_ld32(to + 32 * c, v);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
+                        tmem_st32(to + 32 * c, v);
+                    }
+                }
+            }
+            const float sub = m_used == -INFINITY ? 0.0f : m_used;  // nothing seen yet: every score is -inf
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                uint32_t p[16];
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const float e0 = ex2(fmaf(__uint_as_float(sv[c][2 * i]), a.scale_log2, -sub));
+                    const float e1 = ex2(fmaf(__uint_as_float(sv[c][2 * i + 1]), a.scale_log2, -sub));
+                    sum[i & 3] += e0 + e1;
+                    const __half2 h = __floats2half2_rn(e0, e1);
+                    p[i] = *reinterpret_cast<const uint32_t*>(&h);
+                }
+                tmem_st16(ts + 16 * c, p);
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[x]);
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        }
+        if (ok && n_blocks > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[x], 0, abort_flag));
+        tc_fence_after();
+        if (!ok) {
+            if (lane == 0) fail(0xfb300 + warp);
+        } else {
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            const long long at = (long long)(q0 + t) * a.out_stride + (long long)(kvh * a.group + r % a.group) * D;
+#pragma unroll
+            for (int c = 0; c < D / 32; c++) {
+                uint32_t v[32];
+                if (n_blocks > 0) tmem_ld32(to + 32 * c, v);
+                tmem_ld_wait();
+                if (l == 0.0f)
+#pragma unroll
+                    for (int i = 0; i < 32; i++) v[i] = 0u;
+                if (!valid) continue;
+                if (a.out_f16) {
+                    __half* o = static_cast<__half*>(a.out) + at + 32 * c;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const __half2 h = __floats2half2_rn(__uint_as_float(v[i + 2 * e]) * inv, __uint_as_float(v[i + 2 * e + 1]) * inv);
+                            w[e] = *reinterpret_cast<const uint32_t*>(&h);
+                        }
+                        *reinterpret_cast<uint4*>(o + i) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                } else {
+                    float* o = static_cast<float*>(a.out) + at + 32 * c;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        *reinterpret_cast<float4*>(o + i) = make_float4(__uint_as_float(v[i]) * inv, __uint_as_float(v[i + 1]) * inv,
+                                                                        __uint_as_float(v[i + 2]) * inv, __uint_as_float(v[i + 3]) * inv);
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == KA_MMA_WARP) {
+        tc_fence_after();
+        tmem_dealloc(tmem, KA_TMEM_COLS);
+    }
+}
+
+typedef CUresult (*PFN_encodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+PFN_encodeTiled encode_fn() {
+    static PFN_encodeTiled fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_encodeTiled>(p);
         else
-            hi = mid;
-    }
-    const int q0 = a.cu_q[lo], nq = min(a.cu_q[lo + 1], a.n_q) - q0;
-    const int k0 = max(a.cu_kv[lo], 0), k1 = min(a.cu_kv[lo + 1], a.n_kv), nk = k1 - k0;
-    const int seen = a.causal ? min(nk, t - q0 + nk - nq + 1) : nk;
-    const __half* qp = static_cast<const __half*>(a.q) + t * a.q_stride + head * D;
-    float q[E], o[E], m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        q[e] = __half2float(qp[e * 32 + lane]);
-        o[e] = 0.0f;
-    }
-    for (int j = 0; j < seen; j++) {
-        const __half* kp = static_cast<const __half*>(a.k) + (k0 + j) * a.k_stride + kvh * D;
-        const __half* vp = static_cast<const __half*>(a.v) + (k0 + j) * a.v_stride + kvh * D;
-        float s = 0.0f;
-#pragma unroll
-        for (int e = 0; e < E; e++) s += q[e] * __half2float(kp[e * 32 + lane]);
-        s = warp_sum(s) * a.scale;
-        const float mn = fmaxf(m, s), c = m == -INFINITY ? 0.0f : expf(m - mn), p = s == -INFINITY ? 0.0f : expf(s - mn);
-        l = l * c + p;
-#pragma unroll
-        for (int e = 0; e < E; e++) o[e] = o[e] * c + p * __half2float(vp[e * 32 + lane]);
-        m = mn;
-    }
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        const float r = l > 0.0f ? o[e] / l : o[e];
-        const long long at = t * a.out_stride + head * D + e * 32 + lane;
-        if (a.out_type == 1)
-            static_cast<__half*>(a.out)[at] = __float2half_rn(r);
-        else
-            static_cast<float*>(a.out)[at] = r;
-    }
+            cudaGetLastError();
+    });
+    return fn;
+}
+
+// [token][head][D] f16 with a token stride, loaded in boxes of 64 values x heads x tokens.
+bool map_rows(CUtensorMap* m, const void* p, int d, int heads, long long stride, int n, int box_heads, int box_tokens) {
+    const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)n};
+    const cuuint64_t str[2] = {(cuuint64_t)d * 2, (cuuint64_t)stride * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens}, es[3] = {1, 1, 1};
+    return encode_fn()(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(p), dims, str, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D> int launch(const CfiPackedAttention* p, cudaStream_t stream) {
+    if (!encode_fn()) return (int)cudaErrorNotSupported;
+    KaArgs a;
+    a.out = p->out;
+    a.cu_q = p->cu_q;
+    a.cu_kv = p->cu_kv;
+    a.out_stride = p->out_stride;
+    a.n_seq = p->n_seq;
+    a.n_q = p->n_q;
+    a.n_kv = p->n_kv;
+    a.group = p->n_head / p->n_kv_head;
+    a.tokens = KA_M / a.group;
+    a.out_f16 = p->out_type;
+    a.causal = p->causal;
+    a.scale_log2 = p->scale * 1.4426950408889634f;
+    a.err = cfi_device_error_word();
+    CUtensorMap tq, tk, tv;
+    // no keys at all: the maps still need an extent, and nothing is loaded
+    if (!map_rows(&tq, p->q, D, p->n_head, p->q_stride, p->n_q, a.group, a.tokens) ||
+        !map_rows(&tk, p->k, D, p->n_kv_head, p->k_stride, p->n_kv > 0 ? p->n_kv : 1, 1, KA_N) ||
+        !map_rows(&tv, p->v, D, p->n_kv_head, p->v_stride, p->n_kv > 0 ? p->n_kv : 1, 1, KA_N))
+        return (int)cudaErrorInvalidValue;
+    static CfiPerDeviceOnce attr;
+    cfi_once_per_device(attr, [] { cudaFuncSetAttribute(packed_attn<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ka_smem<D>()); });
+    const char* ep = getenv("CFI_PDL");
+    cudaLaunchConfig_t lc = {};
+    // every sequence adds at most one pair of tiles that is not full
+    lc.gridDim = dim3((unsigned)(p->n_q / (2 * a.tokens) + (p->n_seq < p->n_q ? p->n_seq : p->n_q)), (unsigned)p->n_kv_head, 1);
+    lc.blockDim = dim3(KA_THREADS, 1, 1);
+    lc.dynamicSmemBytes = ka_smem<D>();
+    lc.stream = stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    lc.attrs = at;
+    lc.numAttrs = (ep && strcmp(ep, "0") == 0) ? 0 : 1;
+    return (int)cudaLaunchKernelEx(&lc, packed_attn<D>, tq, tk, tv, a);
 }
 
 }  // namespace
@@ -67,7 +434,8 @@ __global__ void __launch_bounds__(KA_WARPS * 32) packed_attn(const CfiPackedAtte
 extern "C" int cfi_packed_attention(const CfiPackedAttention* a, void* stream) {
     if (!a || !a->q || !a->k || !a->v || !a->out || !a->cu_q || !a->cu_kv || a->n_seq < 0 || a->n_seq > 65535 || a->n_q < 0 ||
         a->n_kv < 0 || a->n_head <= 0 || a->n_kv_head <= 0 || a->n_head % a->n_kv_head || a->n_head / a->n_kv_head > 128 ||
-        a->n_head > 65535 || (a->head_dim != 64 && a->head_dim != 128) || (a->out_type != 0 && a->out_type != 1))
+        a->n_head > 65535 || (a->head_dim != 64 && a->head_dim != 128) || (a->out_type != 0 && a->out_type != 1) ||
+        !(a->scale > 0.0f) || isinf(a->scale))
         return (int)cudaErrorInvalidValue;
     const long long wq = (long long)a->n_head * a->head_dim, wk = (long long)a->n_kv_head * a->head_dim;
     if ((((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->out) & 15) ||
@@ -75,16 +443,6 @@ extern "C" int cfi_packed_attention(const CfiPackedAttention* a, void* stream) {
         a->q_stride < wq || a->out_stride < wq || a->k_stride < wk || a->v_stride < wk)
         return (int)cudaErrorInvalidValue;
     if (a->n_seq == 0 || a->n_q == 0) return 0;
-    const char* ep = getenv("CFI_PDL");
-    cudaLaunchConfig_t lc = {};
-    lc.gridDim = dim3((a->n_q + KA_WARPS - 1) / KA_WARPS, a->n_head, 1);
-    lc.blockDim = dim3(KA_WARPS * 32, 1, 1);
-    lc.stream = static_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    lc.attrs = at;
-    lc.numAttrs = (ep && strcmp(ep, "0") == 0) ? 0 : 1;
-    void* args[1] = {const_cast<CfiPackedAttention*>(a)};
-    return (int)cudaLaunchKernelExC(&lc, a->head_dim == 64 ? (const void*)packed_attn<64> : (const void*)packed_attn<128>, args);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return a->head_dim == 64 ? launch<64>(a, s) : launch<128>(a, s);
 }
