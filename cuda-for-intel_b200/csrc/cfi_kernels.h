@@ -122,7 +122,8 @@ int cfi_glue_slot(cudaStream_t stream, CfiGlueSlot* out);
 // A buffer of at least `bytes` for (current device, stream, kind), grown outside stream capture
 // only (*err = cudaErrorStreamCaptureUnsupported when it would have to grow under capture).
 // (CFI_BUF_COUNTERS buffers are zeroed when allocated; their kernels leave them at zero)
-enum { CFI_BUF_SPLITK = 1, CFI_BUF_MMQ_SCRATCH = 2, CFI_BUF_SKINNY_WS = 3, CFI_BUF_COUNTERS = 4, CFI_BUF_DECODE_SYNC = 5 };
+enum { CFI_BUF_SPLITK = 1, CFI_BUF_MMQ_SCRATCH = 2, CFI_BUF_SKINNY_WS = 3, CFI_BUF_COUNTERS = 4, CFI_BUF_DECODE_SYNC = 5,
+       CFI_BUF_PAGED_PARTS = 6 };
 void* cfi_stream_buffer(int kind, size_t bytes, cudaStream_t stream, int* err);
 
 // The library's device error word (k_mmq_sm100.cu; read and cleared by cfi_device_error).

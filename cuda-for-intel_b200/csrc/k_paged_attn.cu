@@ -1,86 +1,478 @@
 // k_paged_attn.cu -- attention of one new token per sequence over a paged key-value cache
 // (include/cfi_serve.h): out = sum_j softmax_j(scale q.K_j) V_j over the sequence's positions.
 //
-// One warp walks every fourth position of a (sequence, head) with a running maximum and sum; the four
-// meet in shared memory.
+// Bound by HBM: every cached row is read once for the query heads that share it.  The list of all
+// 16-position tiles of all (sequence, kv head) pairs is cut into equal runs, one per CTA, whatever the
+// lengths: no CTA waits for the longest sequence.  The lengths are read on the device, so every CTA
+// works out the same cuts.  A pair whose tiles lie in several CTAs leaves partial sums (row maximum,
+// sum, weighted values) in the stream's workspace; the last of its CTAs to finish joins them in CTA order,
+// so that the result does not depend on which one that was.
+//
+// Each of a CTA's four warps walks every fourth tile with its own ring of cp.async stages (rows past the
+// length are filled with zeros, so what a page holds there never matters) and a running maximum.
+// The products run on mma.sync m16n8k16 with at most 8 query heads: rows 0-7 of A are the heads'
+// f16 values and rows 8-15 what f16 rounding left of them, so one MMA multiplies operands of 22 bits
+// and the two halves of its result are added.  The same holds for the weights.  A group of more than 8
+// heads is cut into chunks that read the rows again (from L2).
+//
+// Q8_0: int8 values are exact in f16, so K enters the MMA as whole numbers, one block of 32 dims at
+// a time, and each block's sum is multiplied by its scale in 32 bits; V's scales are multiplied into the
+// weights before these are split (times 2^8, so that small scales stay clear of f16's subnormals).
 #include "paged_cache.cuh"
 #include "sm100_ptx.cuh"
+#include "mma_sync.cuh"
 #include "cfi_kernels.h"
 
+#include <math.h>
 #include <stdlib.h>
 #include <string.h>
 
 namespace {
 
-constexpr int PA_WARPS = 4;
+using namespace sm100;
+
+constexpr int PA_WARPS = 4, PA_THREADS = PA_WARPS * 32;
+constexpr int PA_HEADS = 8;        // query heads of a chunk
+constexpr int PA_TILE = 16;        // positions; a page is a multiple of it
+constexpr float PA_V_UNIT = 256.0f;
+
+template <int D, bool Q8> struct PaShape {
+    static constexpr int ROW = Q8 ? D : 2 * D;            // bytes of a row
+    static constexpr int ROWS = PA_TILE * ROW;            // of a tile of K or V
+    static constexpr int SCALES = Q8 ? PA_TILE * D / 16 : 0;
+    static constexpr int STAGE = 2 * (ROWS + SCALES);
+    static constexpr int STAGES = Q8 ? (D == 64 ? 6 : 4) : (D == 64 ? 4 : 3);
+    static constexpr int CTAS = Q8 ? 3 : (D == 64 ? 3 : 2);  // per SM
+    static constexpr int RING = STAGES * STAGE;           // a warp's
+    static constexpr int SMEM = PA_WARPS * RING;
+    static constexpr int PART = PA_HEADS * (D + 2);       // floats of a partial result
+    static_assert(SMEM >= PA_WARPS * PART * 4, "the warps meet in the stages' memory");
+};
 
 struct PaArgs {
     const uint8_t *k, *v, *q;
     uint8_t* out;
     const int32_t *table, *lens;
+    float* parts;           // [2 x CTAs][PART]
+    unsigned int* counters;  // [sequence][kv head x chunk], zero between calls
     long long q_stride, out_stride;
-    int n_pages, page_shift, n_kv_head, group, max_pages, q_f16, out_f16;
-    float scale;
+    int n_pages, page_shift, n_kv_head, group, chunks, max_pages, n_seq, q_f16, out_f16;
+    float scale_log2;
 };
 
-template <int D, bool Q8> CFI_DEV float cached(const uint8_t* region, int page_size, int off, int d) {
-    if (!Q8) return h2f_bits(*reinterpret_cast<const uint16_t*>(region + ((size_t)off * D + d) * 2));
-    const float s = h2f_bits(*reinterpret_cast<const uint16_t*>(region + (size_t)D * page_size + ((size_t)off * (D / 32) + d / 32) * 2));
-    return s * (float)*reinterpret_cast<const int8_t*>(region + (size_t)off * D + d);
+CFI_DEV float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+CFI_DEV void cp16z(uint32_t dst, const void* src, bool take) {  // 16 bytes, or 16 zeros
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+CFI_DEV void cp8z(uint32_t dst, const void* src, bool take) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(take ? 8 : 0) : "memory");
+}
+CFI_DEV void cp4z(uint32_t dst, const void* src, bool take) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(take ? 4 : 0) : "memory");
+}
+CFI_DEV void ldsm_x4_trans(uint32_t a, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(a));
+}
+CFI_DEV void mma_f16f32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+CFI_DEV uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+// (x, y) as f16 and what the rounding left, as f16: 22 bits together
+CFI_DEV void split(float x, float y, uint32_t* hi, uint32_t* lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    *hi = h2_bits(h);
+    *lo = h2_bits(__floats2half2_rn(x - f.x, y - f.y));
+}
+// bytes `sel` of w (int8 with its sign bit flipped) as two f16: 0x6400 + u is 1024 + u, less 1152
+CFI_DEV uint32_t s8_to_h2(uint32_t w, uint32_t sel) {
+    const uint32_t u = __byte_perm(w, 0x64646464u, sel);
+    return h2_bits(__hsub2(*reinterpret_cast<const __half2*>(&u), __half2half2(__ushort_as_half(0x6480))));
+}
+
+// Byte offset of 16-byte chunk c of row r in a tile: chunks are exchanged so that the reads below
+// take every bank once.
+template <int D, bool Q8, bool V> CFI_DEV uint32_t chunk_at(int r, int c) {
+    if (!Q8) return r * (2 * D) + ((c ^ (r & 7)) << 4);                    // ldmatrix: 8 rows, one chunk each
+    if (D == 128) return r * 128 + ((c ^ (((V ? r >> 1 : r) & 3) << 1)) << 4);  // 4 rows, two chunks each
+    // 64-byte rows, two to a line of banks
+    const int half = V ? r >> 2 & 1 : r & 1, line = V ? (r & 3) | (r >> 3) << 2 : r >> 1;
+    return line * 128 + half * 64 + ((c ^ ((r >> 1 & 1) << 1)) << 4);
 }
 
 template <int D, bool Q8>
-__global__ void __launch_bounds__(PA_WARPS * 32) paged_attn(const PaArgs a) {
-    sm100::pdl_launch_dependents();
-    sm100::pdl_wait();
-    constexpr int E = D / 32;
-    __shared__ float sm[PA_WARPS], sl[PA_WARPS], so[PA_WARPS][D];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int head = blockIdx.x, seq = blockIdx.y, kvh = head / a.group;
-    const int page_size = 1 << a.page_shift;
-    const int len = min(a.lens[seq], (int)min((long long)a.max_pages << a.page_shift, 0x7fffffffLL));
-    float q[E], o[E], m = -INFINITY, l = 0.0f;
+__global__ void __launch_bounds__(PA_THREADS, (PaShape<D, Q8>::CTAS)) paged_attn(const PaArgs a) {
+    using S = PaShape<D, Q8>;
+    constexpr int NB = D / 32, NT = D / 8, KK = D / 16;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ unsigned int s_last;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+    const int page_size = 1 << a.page_shift, hc = a.n_kv_head * a.chunks;
+    pdl_launch_dependents();
+    pdl_wait();
+
+    const int most = (int)min((long long)a.max_pages << a.page_shift, 0x7fffff00LL);
+    auto length = [&](int s) { return max(0, min(a.lens[s], most)); };
+    auto tiles_of = [&](int len) { return max(1, (len + PA_TILE - 1) / PA_TILE); };  // an empty sequence still has its zeros to write
+    // ---- this CTA's run of tiles ----
+    long long total = 0;
+    for (int s = lane; s < a.n_seq; s += 32) total += tiles_of(length(s));
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-        const long long at = seq * a.q_stride + head * D + e * 32 + lane;
-        q[e] = a.q_f16 ? h2f_bits(reinterpret_cast<const uint16_t*>(a.q)[at]) : reinterpret_cast<const float*>(a.q)[at];
-        o[e] = 0.0f;
-    }
-    for (int j = warp; j < len; j += PA_WARPS) {
-        const int page = min(max(a.table[(long long)seq * a.max_pages + (j >> a.page_shift)], 0), a.n_pages - 1);
-        const long long region = ((long long)page * a.n_kv_head + kvh) * paged_region_bytes<D, Q8>(page_size);
-        float s = 0.0f;
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    total *= hc;
+    const long long quota = max((total + gridDim.x - 1) / gridDim.x, (long long)PA_WARPS);
+    long long at = blockIdx.x * quota;
+    const long long end = min(at + quota, total);
+    if (at >= end) return;
+    int seq = 0;
+    long long seq_start = 0;  // the sequence's first tile
+    for (int base = 0;; base += 32) {
+        const long long n = base + lane < a.n_seq ? (long long)tiles_of(length(base + lane)) * hc : 0;
+        long long incl = n;
 #pragma unroll
-        for (int e = 0; e < E; e++) s += q[e] * cached<D, Q8>(a.k + region, page_size, j & (page_size - 1), e * 32 + lane);
-        s = warp_sum(s) * a.scale;
-        const float mn = fmaxf(m, s), c = m == -INFINITY ? 0.0f : expf(m - mn), p = s == -INFINITY ? 0.0f : expf(s - mn);
-        l = l * c + p;
-#pragma unroll
-        for (int e = 0; e < E; e++) o[e] = o[e] * c + p * cached<D, Q8>(a.v + region, page_size, j & (page_size - 1), e * 32 + lane);
-        m = mn;
-    }
-    if (lane == 0) {
-        sm[warp] = m;
-        sl[warp] = l;
-    }
-#pragma unroll
-    for (int e = 0; e < E; e++) so[warp][e * 32 + lane] = o[e];
-    __syncthreads();
-    for (int d = threadIdx.x; d < D; d += PA_WARPS * 32) {
-        float mm = -INFINITY, ll = 0.0f, oo = 0.0f;
-        for (int w = 0; w < PA_WARPS; w++) mm = fmaxf(mm, sm[w]);
-        for (int w = 0; w < PA_WARPS; w++) {
-            const float c = sm[w] == -INFINITY ? 0.0f : expf(sm[w] - mm);
-            ll += c * sl[w];
-            oo += c * so[w][d];
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += x;
         }
-        const float r = ll > 0.0f ? oo / ll : oo;
-        const long long at = seq * a.out_stride + head * D + d;
-        if (a.out_f16)
-            reinterpret_cast<uint16_t*>(a.out)[at] = f2h_bits(r);
-        else
-            reinterpret_cast<float*>(a.out)[at] = r;
+        const uint32_t hit = __ballot_sync(0xffffffffu, seq_start + incl > at);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            seq = base + l;
+            seq_start += __shfl_sync(0xffffffffu, incl - n, l);
+            break;
+        }
+        seq_start += __shfl_sync(0xffffffffu, incl, 31);
     }
+
+    const uint32_t ring = smem_u32(smem) + warp * S::RING;
+    while (at < end) {
+        // ---- one (sequence, kv head, chunk): its tiles [t0, t1) of n_tiles ----
+        const int len = length(seq), n_tiles = tiles_of(len);
+        const int pair = (int)((at - seq_start) / n_tiles);
+        const long long pair_start = seq_start + (long long)pair * n_tiles;
+        const int t0 = (int)(at - pair_start), t1 = (int)min((long long)n_tiles, end - pair_start);
+        const int kvh = pair / a.chunks, h0 = (pair - kvh * a.chunks) * PA_HEADS, nh = min(PA_HEADS, a.group - h0);
+        const int head0 = kvh * a.group + h0;
+
+        // page ids of this warp's next 32 tiles, one a lane
+        const int32_t* trow = a.table + (long long)seq * a.max_pages;
+        const int mine = t1 - t0 > warp ? (t1 - t0 - warp + PA_WARPS - 1) / PA_WARPS : 0;  // tiles of this warp
+        auto load_ids = [&](int i) {
+            const int t = t0 + warp + (i + lane) * PA_WARPS;
+            return t < t1 && t * PA_TILE < len ? min(max(trow[t * PA_TILE >> a.page_shift], 0), a.n_pages - 1) : 0;
+        };
+        int ids = load_ids(0);
+
+        // ---- the queries: scaled to log2 units, split ----
+        uint32_t qf[KK][4];
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++)
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                // A's k = 2c, 2c+1 (x 0) and 2c+8, 2c+9 (x 1), in the order that K's fragments have
+                const int d = Q8 ? 32 * (kk >> 1) + 8 * c + 4 * (kk & 1) + 2 * x : 16 * kk + 2 * c + 8 * x;
+                float2 f = make_float2(0.0f, 0.0f);
+                if (g < nh) {
+                    const long long o = seq * a.q_stride + (long long)(head0 + g) * D + d;
+                    f = a.q_f16 ? __half22float2(*reinterpret_cast<const __half2*>(a.q + o * 2)) : *reinterpret_cast<const float2*>(a.q + o * 4);
+                }
+                split(f.x * a.scale_log2, f.y * a.scale_log2, &qf[kk][2 * x], &qf[kk][2 * x + 1]);
+            }
+
+        auto fetch = [&](int i) {  // tile i of this warp into its stage
+            if (i < mine) {
+                const int t = t0 + warp + i * PA_WARPS, p0 = t * PA_TILE;
+                const int page = __shfl_sync(0xffffffffu, ids, i & 31), off = p0 & (page_size - 1);
+                const long long region = ((long long)page * a.n_kv_head + kvh) * paged_region_bytes<D, Q8>(page_size);
+                const uint32_t st = ring + (i % S::STAGES) * S::STAGE;
+                const int left = len - p0;
+#pragma unroll
+                for (int e = 0; e < S::ROWS / 512; e++) {
+                    constexpr int CH = S::ROW / 16;
+                    const int r = (e * 32 + lane) / CH, ch = (e * 32 + lane) % CH;
+                    const long long src = region + (long long)(off + r) * S::ROW + ch * 16;
+                    cp16z(st + chunk_at<D, Q8, false>(r, ch), a.k + src, r < left);
+                    cp16z(st + S::ROWS + chunk_at<D, Q8, true>(r, ch), a.v + src, r < left);
+                }
+                if (Q8) {  // lanes 0-15 bring K's scales, 16-31 V's
+                    const int r = lane & 15;
+                    const uint8_t* src = (lane < 16 ? a.k : a.v) + region + (long long)page_size * D + (off + r) * (D / 16);
+                    const uint32_t dst = st + 2 * S::ROWS + (lane < 16 ? 0 : S::SCALES) + r * (D / 16);
+                    if (D == 128) cp8z(dst, src, r < left); else cp4z(dst, src, r < left);
+                }
+            }
+            cp_async_commit();
+        };
+
+        float o[NT][4], m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[j][e] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < S::STAGES - 1; i++) fetch(i);
+        for (int i = 0; i < mine; i++) {
+            if ((i + S::STAGES - 1) % 32 == 0) ids = load_ids(i + S::STAGES - 1);
+            fetch(i + S::STAGES - 1);
+            cp_async_wait<S::STAGES - 1>();
+            __syncwarp();
+            const uint32_t sk = ring + (i % S::STAGES) * S::STAGE, sv = sk + S::ROWS, ss = sk + 2 * S::ROWS;
+            // ---- scores of positions 2c, 2c+1 and 8+2c, 9+2c for head g ----
+            float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (!Q8) {
+                float acc[2][4] = {};
+#pragma unroll
+                for (int kk = 0; kk < KK; kk++) {
+                    uint32_t b[4];
+                    ldsm_x4(sk + chunk_at<D, Q8, false>((lane >> 4) * 8 + (lane & 7), 2 * kk + (lane >> 3 & 1)), b);
+                    mma_f16f32(acc[0], qf[kk], b[0], b[1]);
+                    mma_f16f32(acc[1], qf[kk], b[2], b[3]);
+                }
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    s[2 * n] = acc[n][0] + acc[n][2];
+                    s[2 * n + 1] = acc[n][1] + acc[n][3];
+                }
+            } else {
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    uint32_t sc[NB];  // scales of positions 2c and 2c+1
+                    if (D == 128) {
+                        const uint4 w = lds128(ss + (8 * n + 2 * c) * 8);
+                        sc[0] = w.x, sc[1] = w.y, sc[NB - 2] = w.z, sc[NB - 1] = w.w;
+                    } else {
+                        const uint2 w = lds64(ss + (8 * n + 2 * c) * 4);
+                        sc[0] = w.x, sc[1] = w.y;
+                    }
+#pragma unroll
+                    for (int b = 0; b < NB; b++) {
+                        const uint2 w = lds64(sk + chunk_at<D, Q8, false>(8 * n + g, 2 * b + (c >> 1)) + 8 * (c & 1));
+                        const uint32_t w0 = w.x ^ 0x80808080u, w1 = w.y ^ 0x80808080u;
+                        float acc[4] = {};
+                        mma_f16f32(acc, qf[2 * b], s8_to_h2(w0, 0x4140), s8_to_h2(w0, 0x4342));
+                        mma_f16f32(acc, qf[2 * b + 1], s8_to_h2(w1, 0x4140), s8_to_h2(w1, 0x4342));
+                        const float d0 = h2f_bits((uint16_t)(sc[b >> 1] >> (16 * (b & 1)))),
+                                    d1 = h2f_bits((uint16_t)(sc[NB / 2 + (b >> 1)] >> (16 * (b & 1))));
+                        s[2 * n] = fmaf(acc[0] + acc[2], d0, s[2 * n]);
+                        s[2 * n + 1] = fmaf(acc[1] + acc[3], d1, s[2 * n + 1]);
+                    }
+                }
+            }
+            const int left = len - (t0 + warp + i * PA_WARPS) * PA_TILE;
+            if (left < PA_TILE) {
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if ((e >> 1) * 8 + 2 * c + (e & 1) >= left) s[e] = -INFINITY;
+            }
+            float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            if (__any_sync(0xffffffffu, mx > m)) {
+                const float mn = fmaxf(m, mx), alpha = m == -INFINITY ? 0.0f : ex2(m - mn);
+                l *= alpha;
+#pragma unroll
+                for (int j = 0; j < NT; j++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[j][e] *= alpha;
+                m = mn;
+            }
+            const float sub = m == -INFINITY ? 0.0f : m;
+            float p[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) p[e] = ex2(s[e] - sub);
+            l += (p[0] + p[1]) + (p[2] + p[3]);
+            // ---- weighted values ----
+            if (!Q8) {
+                uint32_t pf[4];
+                split(p[0], p[1], &pf[0], &pf[1]);
+                split(p[2], p[3], &pf[2], &pf[3]);
+#pragma unroll
+                for (int j = 0; j < NT; j += 2) {
+                    uint32_t b[4];
+                    ldsm_x4_trans(sv + chunk_at<D, Q8, true>(lane & 15, j + (lane >> 4)), b);
+                    mma_f16f32(o[j], pf, b[0], b[1]);
+                    mma_f16f32(o[j + 1], pf, b[2], b[3]);
+                }
+            } else {
+                uint32_t sc[2][NB];  // scales of positions 2c, 2c+1 and 8+2c, 9+2c
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    if (D == 128) {
+                        const uint4 w = lds128(ss + S::SCALES + (8 * n + 2 * c) * 8);
+                        sc[n][0] = w.x, sc[n][1] = w.y, sc[n][NB - 2] = w.z, sc[n][NB - 1] = w.w;
+                    } else {
+                        const uint2 w = lds64(ss + S::SCALES + (8 * n + 2 * c) * 4);
+                        sc[n][0] = w.x, sc[n][1] = w.y;
+                    }
+                }
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    uint32_t pf[4], bw[2][4];
+#pragma unroll
+                    for (int n = 0; n < 2; n++) {
+                        const float d0 = h2f_bits((uint16_t)(sc[n][b >> 1] >> (16 * (b & 1)))),
+                                    d1 = h2f_bits((uint16_t)(sc[n][NB / 2 + (b >> 1)] >> (16 * (b & 1))));
+                        split(p[2 * n] * PA_V_UNIT * d0, p[2 * n + 1] * PA_V_UNIT * d1, &pf[2 * n], &pf[2 * n + 1]);
+                        // dims 32 b + 4 g .. + 3 of two positions, interleaved: column g of MMA e is dim 32 b + 4 g + e
+                        const uint32_t wa = lds32(sv + chunk_at<D, Q8, true>(8 * n + 2 * c, 2 * b + (g >> 2)) + 4 * (g & 3)) ^ 0x80808080u;
+                        const uint32_t wb = lds32(sv + chunk_at<D, Q8, true>(8 * n + 2 * c + 1, 2 * b + (g >> 2)) + 4 * (g & 3)) ^ 0x80808080u;
+                        const uint32_t x = __byte_perm(wa, wb, 0x5140), y = __byte_perm(wa, wb, 0x7362);
+                        bw[n][0] = s8_to_h2(x, 0x4140);
+                        bw[n][1] = s8_to_h2(x, 0x4342);
+                        bw[n][2] = s8_to_h2(y, 0x4140);
+                        bw[n][3] = s8_to_h2(y, 0x4342);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) mma_f16f32(o[4 * b + e], pf, bw[0][e], bw[1][e]);
+                }
+            }
+            __syncwarp();  // the stage is free
+        }
+        // ---- the warps meet: [warp][head]: D values, maximum, sum ----
+        cp_async_wait<0>();
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        __syncthreads();  // every warp is done with its stages
+        float* meet = reinterpret_cast<float*>(smem);
+        float* wp = meet + warp * S::PART + g * (D + 2);
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int d = Q8 ? 32 * (j >> 2) + 4 * (2 * c + e) + (j & 3) : 8 * j + 2 * c + e;
+                wp[d] = (o[j][e] + o[j][e + 2]) * (Q8 ? 1.0f / PA_V_UNIT : 1.0f);
+            }
+        if (c == 0) {
+            wp[D] = m;
+            wp[D + 1] = l;
+        }
+        __syncthreads();
+        // joins n partial results (stride `step` floats) for head h, dim d
+        auto join = [&](const float* part, int n, long long step, int h, int d, float* om, float* ol) {
+            float mm = -INFINITY;
+            for (int i = 0; i < n; i++) mm = fmaxf(mm, __ldcg(part + i * step + h * (D + 2) + D));
+            float ll = 0.0f, oo = 0.0f;
+            for (int i = 0; i < n; i++) {
+                const float* p = part + i * step + h * (D + 2);
+                const float mi = __ldcg(p + D), f = mi == -INFINITY ? 0.0f : ex2(mi - mm);
+                ll = fmaf(f, __ldcg(p + D + 1), ll);
+                oo = fmaf(f, __ldcg(p + d), oo);
+            }
+            *om = mm;
+            *ol = ll;
+            return oo;
+        };
+        auto join_warps = [&](int h, int d, float* om, float* ol) {
+            const float* p = meet + h * (D + 2);
+            float mm = -INFINITY, ll = 0.0f, oo = 0.0f;
+#pragma unroll
+            for (int w = 0; w < PA_WARPS; w++) mm = fmaxf(mm, p[w * S::PART + D]);
+#pragma unroll
+            for (int w = 0; w < PA_WARPS; w++) {
+                const float mi = p[w * S::PART + D], f = mi == -INFINITY ? 0.0f : ex2(mi - mm);
+                ll = fmaf(f, p[w * S::PART + D + 1], ll);
+                oo = fmaf(f, p[w * S::PART + d], oo);
+            }
+            *om = mm;
+            *ol = ll;
+            return oo;
+        };
+        auto write = [&](int h, int d, float v, float sum) {
+            const float r = sum == 0.0f ? 0.0f : v / sum;
+            const long long w = seq * a.out_stride + (long long)(head0 + h) * D + d;
+            if (a.out_f16)
+                reinterpret_cast<uint16_t*>(a.out)[w] = f2h_bits(r);
+            else
+                reinterpret_cast<float*>(a.out)[w] = r;
+        };
+        const bool whole = t0 == 0 && t1 == n_tiles;
+        // a CTA leaves at most two partial results: of the pair that its run begins in, and of the last
+        float* part = a.parts + (2LL * blockIdx.x + (pair_start > blockIdx.x * quota ? 1 : 0)) * S::PART;
+        for (int i = tid; i < nh * D; i += PA_THREADS) {
+            const int h = i / D, d = i % D;
+            float mm, ll;
+            const float oo = join_warps(h, d, &mm, &ll);
+            if (whole) {
+                write(h, d, oo, ll);
+            } else {
+                __stcg(part + h * (D + 2) + d, oo);
+                if (d == 0) {
+                    __stcg(part + h * (D + 2) + D, mm);
+                    __stcg(part + h * (D + 2) + D + 1, ll);
+                }
+            }
+        }
+        if (!whole) {
+            const long long b0 = pair_start / quota, b1 = (pair_start + n_tiles - 1) / quota;  // its CTAs
+            __threadfence();
+            __syncthreads();
+            unsigned int* count = a.counters + (long long)seq * hc + pair;
+            if (tid == 0) s_last = atomicAdd(count, 1u) == (unsigned)(b1 - b0);
+            __syncthreads();
+            if (s_last) {
+                __threadfence();
+                if (tid == 0) *count = 0u;
+                // CTA b0's result is in its second place unless the pair begins its run
+                const float* first = a.parts + (2 * b0 + (pair_start > b0 * quota ? 1 : 0)) * S::PART;
+                for (int i = tid; i < nh * D; i += PA_THREADS) {
+                    const int h = i / D, d = i % D;
+                    float m0, l0, m1, l1;
+                    const float o0 = join(first, 1, 0, h, d, &m0, &l0);
+                    const float o1 = join(a.parts + 2 * (b0 + 1) * S::PART, (int)(b1 - b0), 2 * S::PART, h, d, &m1, &l1);
+                    const float mm = fmaxf(m0, m1), f0 = m0 == -INFINITY ? 0.0f : ex2(m0 - mm), f1 = m1 == -INFINITY ? 0.0f : ex2(m1 - mm);
+                    write(h, d, o0 * f0 + o1 * f1, l0 * f0 + l1 * f1);
+                }
+            }
+        }
+        __syncthreads();  // the meeting place is free for the next pair's stages
+        at = pair_start + t1;
+        if (pair == hc - 1 && t1 == n_tiles) {
+            seq_start = at;
+            seq++;
+        }
+    }
+}
+
+template <int D, bool Q8> int launch(PaArgs& a, long long pairs, long long most_tiles, cudaStream_t stream) {
+    using S = PaShape<D, Q8>;
+    static CfiPerDeviceOnce once;
+    static int sms[CFI_MAX_DEVICES + 1];
+    const int dev = cfi_device_index();
+    int* n = &sms[dev < 0 ? CFI_MAX_DEVICES : dev];
+    cfi_once_per_device(once, [n] {
+        int d = 0;
+        cudaGetDevice(&d);
+        cudaDeviceGetAttribute(n, cudaDevAttrMultiProcessorCount, d);
+        cudaFuncSetAttribute(paged_attn<D, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    });
+    const long long ctas = (long long)(*n > 0 ? *n : 148) * S::CTAS;
+    // no CTA has fewer tiles than warps
+    const long long grid = most_tiles / PA_WARPS + 1 < ctas ? most_tiles / PA_WARPS + 1 : ctas;
+    int err = 0;
+    a.parts = static_cast<float*>(cfi_stream_buffer(CFI_BUF_PAGED_PARTS, (size_t)ctas * 2 * S::PART * 4, stream, &err));
+    if (!a.parts) return err;
+    a.counters = static_cast<unsigned int*>(cfi_stream_buffer(CFI_BUF_COUNTERS, (size_t)pairs * 4, stream, &err));
+    if (!a.counters) return err;
+    const char* ep = getenv("CFI_PDL");
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3((unsigned)grid, 1, 1);
+    lc.blockDim = dim3(PA_THREADS, 1, 1);
+    lc.dynamicSmemBytes = S::SMEM;
+    lc.stream = stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    lc.attrs = at;
+    lc.numAttrs = (ep && strcmp(ep, "0") == 0) ? 0 : 1;
+    return (int)cudaLaunchKernelEx(&lc, paged_attn<D, Q8>, (const PaArgs)a);
 }
 
 }  // namespace
@@ -89,12 +481,12 @@ extern "C" int cfi_paged_attention(const CfiPagedCache* c, const void* q, int q_
                                    int out_type, long long out_stride, const int32_t* table, int max_pages,
                                    const int32_t* lens, int n_seq, int n_head, float scale, void* stream) {
     if (!cfi_paged_ok(c) || !q || !out || !table || !lens || (q_type != 0 && q_type != 1) || (out_type != 0 && out_type != 1) ||
-        n_seq < 0 || n_seq > 65535 || max_pages <= 0 || n_head <= 0 || n_head % c->n_kv_head ||
+        n_seq < 0 || n_seq > 65535 || max_pages <= 0 || n_head <= 0 || n_head > 65535 || n_head % c->n_kv_head ||
         (((uintptr_t)q | (uintptr_t)out) & 15) || (((uintptr_t)table | (uintptr_t)lens) & 3) || q_stride % 8 || out_stride % 8 ||
-        q_stride < (long long)n_head * c->head_dim || out_stride < (long long)n_head * c->head_dim)
+        q_stride < (long long)n_head * c->head_dim || out_stride < (long long)n_head * c->head_dim || !(scale > 0.0f) || isinf(scale))
         return (int)cudaErrorInvalidValue;
     if (n_seq == 0) return 0;
-    PaArgs a;
+    PaArgs a = {};
     a.k = static_cast<const uint8_t*>(c->k);
     a.v = static_cast<const uint8_t*>(c->v);
     a.q = static_cast<const uint8_t*>(q);
@@ -107,22 +499,15 @@ extern "C" int cfi_paged_attention(const CfiPagedCache* c, const void* q, int q_
     a.page_shift = __builtin_ctz((unsigned)c->page_size);
     a.n_kv_head = c->n_kv_head;
     a.group = n_head / c->n_kv_head;
+    a.chunks = (a.group + PA_HEADS - 1) / PA_HEADS;
     a.max_pages = max_pages;
+    a.n_seq = n_seq;
     a.q_f16 = q_type;
     a.out_f16 = out_type;
-    a.scale = scale;
-    const char* ep = getenv("CFI_PDL");
-    cudaLaunchConfig_t lc = {};
-    lc.gridDim = dim3(n_head, n_seq, 1);
-    lc.blockDim = dim3(PA_WARPS * 32, 1, 1);
-    lc.stream = static_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    lc.attrs = at;
-    lc.numAttrs = (ep && strcmp(ep, "0") == 0) ? 0 : 1;
-    const void* fn = c->head_dim == 64 ? (c->type == 1 ? (const void*)paged_attn<64, false> : (const void*)paged_attn<64, true>)
-                                       : (c->type == 1 ? (const void*)paged_attn<128, false> : (const void*)paged_attn<128, true>);
-    void* args[1] = {&a};
-    return (int)cudaLaunchKernelExC(&lc, fn, args);
+    a.scale_log2 = scale * 1.4426950408889634f;
+    const long long pairs = (long long)n_seq * c->n_kv_head * a.chunks;
+    const long long most_tiles = pairs * ((long long)max_pages * (c->page_size / PA_TILE));
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (c->head_dim == 64) return c->type == 1 ? launch<64, false>(a, pairs, most_tiles, s) : launch<64, true>(a, pairs, most_tiles, s);
+    return c->type == 1 ? launch<128, false>(a, pairs, most_tiles, s) : launch<128, true>(a, pairs, most_tiles, s);
 }

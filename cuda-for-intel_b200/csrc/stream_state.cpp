@@ -143,7 +143,8 @@ void* cfi_stream_buffer(int kind, size_t bytes, cudaStream_t stream, int* err) {
             *err = (int)cudaErrorMemoryAllocation;
             return nullptr;
         }
-        if (kind == CFI_BUF_COUNTERS && cudaMemset(b.p, 0, want) != cudaSuccess) {
+        // on the buffer's own stream: a non-blocking one would not wait for the legacy stream
+        if (kind == CFI_BUF_COUNTERS && cudaMemsetAsync(b.p, 0, want, stream) != cudaSuccess) {
             cudaGetLastError();
             cudaFree(b.p);
             b.p = nullptr;

@@ -69,8 +69,10 @@ CFI_API int cfi_paged_kv_load(const CfiPagedCache *cache, const int64_t *slots, 
  * zero or less gives zeros.  A page id outside the pool is read as the nearest page inside.  What
  * lies in a page past the length never matters, whatever it holds.
  * q and out: [sequence][head][dim], types 0 F32 or 1 F16, row strides in values (q's a multiple of
- * 8), 16-byte aligned.  Sums, maxima and the products with K and V carry 22 bits or more: the
- * results are those of 32-bit arithmetic on the cached values.
+ * 8), 16-byte aligned; scale > 0.  Sums and maxima are in 32 bits and the operands of the products with
+ * K and V carry 22 bits: the results are those of 32-bit arithmetic on the cached values, as long as
+ * |q| * scale stays below 45000 and a Q8_0 block of V below 32000.  An infinity or a NaN within a
+ * sequence's length makes that sequence's results NaN.
  */
 CFI_API int cfi_paged_attention(const CfiPagedCache *cache, const void *q, int q_type, long long q_stride, void *out,
                                 int out_type, long long out_stride, const int32_t *table, int max_pages,
@@ -85,7 +87,7 @@ CFI_API int cfi_paged_attention(const CfiPagedCache *cache, const void *q, int q
  * query sees all the sequence's keys.  Rows of out past cu_q[n_seq] are left as they are.
  * q, out: [token][head][dim], k, v: [token][kv head][dim]; q, k, v f16, out F32 or F16; row strides
  * in values, multiples of 8, heads contiguous, 16-byte aligned; n_head / n_kv_head at most 128;
- * head_dim 64 or 128.  Products are of f16 values (the softmax weights rounded to f16 too) with
+ * head_dim 64 or 128; scale > 0.  Products are of f16 values (the softmax weights rounded to f16 too) with
  * 32-bit sums.  A NaN or an infinity in V reaches the queries of its own sequence only.
  */
 typedef struct {

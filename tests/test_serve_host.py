@@ -54,7 +54,8 @@ def test_load_refusals(at, value):
 
 
 @pytest.mark.parametrize("at,value", [(1, None), (1, P + 8), (2, 8), (3, 192), (3, 260), (4, None), (5, 14), (6, 128), (7, None),
-                                      (8, 0), (9, None), (9, P + 2), (10, -1), (11, 0), (11, 3)])
+                                      (8, 0), (9, None), (9, P + 2), (10, -1), (11, 0), (11, 3), (12, 0.0), (12, -1.0),
+                                      (12, float("nan")), (12, float("inf"))])
 def test_paged_attention_refusals(at, value):
     a = [cache(), P, 0, 256, P, 0, 256, P, 4, P, 1, 4, 0.125, None]
     a[at] = value
@@ -64,7 +65,8 @@ def test_paged_attention_refusals(at, value):
 @pytest.mark.parametrize("bad", [dict(q=None), dict(k=P + 8), dict(v=None), dict(out=P + 4), dict(cu_q=None), dict(cu_kv=P + 1),
                                  dict(q_stride=192), dict(k_stride=132), dict(v_stride=64), dict(out_stride=250), dict(n_seq=-1),
                                  dict(n_q=-1), dict(n_kv=-1), dict(n_head=3), dict(n_head=0), dict(n_kv_head=0), dict(head_dim=80),
-                                 dict(out_type=8), dict(n_head=258, n_kv_head=2, q_stride=1 << 15, out_stride=1 << 15)])
+                                 dict(out_type=8), dict(scale=0.0), dict(scale=-0.5), dict(scale=float("nan")), dict(scale=float("inf")),
+                                 dict(n_head=258, n_kv_head=2, q_stride=1 << 15, out_stride=1 << 15)])
 def test_packed_attention_refusals(bad):
     a = dict(q=P, k=P, v=P, out=P, cu_q=P, cu_kv=P, q_stride=256, k_stride=128, v_stride=128, out_stride=256, n_seq=1, n_q=5,
              n_kv=5, n_head=4, n_kv_head=2, head_dim=64, out_type=0, causal=1, scale=0.125)
