@@ -5,8 +5,7 @@
 // 16-position tiles of all (sequence, kv head) pairs is cut into equal runs, one per CTA, whatever the
 // lengths: no CTA waits for the longest sequence.  The lengths are read on the device, so every CTA
 // works out the same cuts.  A pair whose tiles lie in several CTAs leaves partial sums (row maximum,
-// sum, weighted values) in the stream's workspace; the last of its CTAs to finish joins them in CTA order,
-// so that the result does not depend on which one that was.
+// sum, weighted values) in the stream's workspace, and a second kernel joins them in CTA order.
 //
 // Each of a CTA's four warps walks every fourth tile with its own ring of cp.async stages (rows past the
 // length are filled with zeros, so what a page holds there never matters) and a running maximum.
@@ -23,6 +22,7 @@
 #include "mma_sync.cuh"
 #include "cfi_kernels.h"
 
+#include <algorithm>
 #include <math.h>
 #include <stdlib.h>
 #include <string.h>
@@ -35,6 +35,13 @@ constexpr int PA_WARPS = 4, PA_THREADS = PA_WARPS * 32;
 constexpr int PA_HEADS = 8;        // query heads of a chunk
 constexpr int PA_TILE = 16;        // positions; a page is a multiple of it
 constexpr float PA_V_UNIT = 256.0f;
+constexpr int PA_MAX_SMS = 256;
+// What beginning and ending a pair costs, in tiles: a run's share of the list counts it, so that CTAs with
+// many short sequences get fewer tiles.
+#ifndef PA_FIXED_TILES
+#define PA_FIXED_TILES 5
+#endif
+constexpr int PA_FIXED = PA_FIXED_TILES;
 
 template <int D, bool Q8> struct PaShape {
     static constexpr int ROW = Q8 ? D : 2 * D;            // bytes of a row
@@ -45,8 +52,10 @@ template <int D, bool Q8> struct PaShape {
     static constexpr int CTAS = Q8 ? 3 : (D == 64 ? 3 : 2);  // per SM
     static constexpr int RING = STAGES * STAGE;           // a warp's
     static constexpr int SMEM = PA_WARPS * RING;
-    static constexpr int PART = PA_HEADS * (D + 2);       // floats of a partial result
-    static_assert(SMEM >= PA_WARPS * PART * 4, "the warps meet in the stages' memory");
+    static constexpr int PART = PA_HEADS * (D + 2);       // floats of a partial result: values, then maximum and sum of each head
+    // where the warps meet: a row is a head's values, maximum and sum (stores of the fragments meet no bank twice)
+    static constexpr int MEET_ROW = D + (Q8 ? 4 : 8), MEET = PA_HEADS * MEET_ROW;
+    static_assert(SMEM >= PA_WARPS * MEET * 4, "the warps meet in the stages' memory");
 };
 
 struct PaArgs {
@@ -54,7 +63,6 @@ struct PaArgs {
     uint8_t* out;
     const int32_t *table, *lens;
     float* parts;           // [2 x CTAs][PART]
-    unsigned int* counters;  // [sequence][kv head x chunk], zero between calls
     long long q_stride, out_stride;
     int n_pages, page_shift, n_kv_head, group, chunks, max_pages, n_seq, q_f16, out_f16;
     float scale_log2;
@@ -108,38 +116,68 @@ template <int D, bool Q8, bool V> CFI_DEV uint32_t chunk_at(int r, int c) {
     return line * 128 + half * 64 + ((c ^ ((r >> 1 & 1) << 1)) << 4);
 }
 
+CFI_DEV void add_to(float4& x, float f, const float4& y) {
+    x.x = fmaf(f, y.x, x.x);
+    x.y = fmaf(f, y.y, x.y);
+    x.z = fmaf(f, y.z, x.z);
+    x.w = fmaf(f, y.w, x.w);
+}
+// Four values of a head's row, over the sum of its weights.
+CFI_DEV void write_out(const PaArgs& a, int seq, int head, int dim, int d, float4 v, float sum) {
+    const float r = sum == 0.0f ? 0.0f : 1.0f / sum;
+    if (sum == 0.0f) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const long long w = seq * a.out_stride + (long long)head * dim + d;
+    if (a.out_f16)
+        *reinterpret_cast<uint2*>(a.out + w * 2) =
+            make_uint2(h2_bits(__floats2half2_rn(v.x * r, v.y * r)), h2_bits(__floats2half2_rn(v.z * r, v.w * r)));
+    else
+        *reinterpret_cast<float4*>(a.out + w * 4) = make_float4(v.x * r, v.y * r, v.z * r, v.w * r);
+}
+
+// How the work is cut: a pair (kv head, chunk) of a sequence is PA_FIXED units and then one for each tile,
+// the pairs of all sequences follow one another, and CTA b has the units b * quota .. (b + 1) * quota.
+// There are less than 2^31.
+struct PaCut {
+    const int32_t* lens;
+    int most, first, total, quota;
+    CFI_DEV int length(int s) const { return max(0, min(lens[s], most)); }
+    // an empty sequence still has its zeros to write
+    static CFI_DEV int tiles_of(int len) { return max(1, (len + PA_TILE - 1) / PA_TILE); }
+    CFI_DEV int units_of(int s) const { return PA_FIXED + tiles_of(length(s)); }
+    // Called by whole warps.  `first`: the units of the sequence that is this lane's, of the first 32.
+    CFI_DEV PaCut(const PaArgs& a, int ctas) : lens(a.lens) {
+        const int lane = threadIdx.x & 31, hc = a.n_kv_head * a.chunks;
+        most = (int)min((long long)a.max_pages << a.page_shift, 0x7fffff00LL);
+        first = lane < a.n_seq ? units_of(lane) * hc : 0;
+        int n = first;
+        for (int s = lane + 32; s < a.n_seq; s += 32) n += units_of(s) * hc;
+        total = __reduce_add_sync(0xffffffffu, n);
+        quota = max((total + ctas - 1) / ctas, PA_FIXED + PA_WARPS);
+    }
+};
+
 template <int D, bool Q8>
 __global__ void __launch_bounds__(PA_THREADS, (PaShape<D, Q8>::CTAS)) paged_attn(const PaArgs a) {
     using S = PaShape<D, Q8>;
     constexpr int NB = D / 32, NT = D / 8, KK = D / 16;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ unsigned int s_last;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
     const int page_size = 1 << a.page_shift, hc = a.n_kv_head * a.chunks;
     pdl_launch_dependents();
     pdl_wait();
 
-    const int most = (int)min((long long)a.max_pages << a.page_shift, 0x7fffff00LL);
-    auto length = [&](int s) { return max(0, min(a.lens[s], most)); };
-    auto tiles_of = [&](int len) { return max(1, (len + PA_TILE - 1) / PA_TILE); };  // an empty sequence still has its zeros to write
-    // ---- this CTA's run of tiles ----
-    long long total = 0;
-    for (int s = lane; s < a.n_seq; s += 32) total += tiles_of(length(s));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    total *= hc;
-    const long long quota = max((total + gridDim.x - 1) / gridDim.x, (long long)PA_WARPS);
-    long long at = blockIdx.x * quota;
-    const long long end = min(at + quota, total);
-    if (at >= end) return;
-    int seq = 0;
-    long long seq_start = 0;  // the sequence's first tile
+    // ---- this CTA's run ----
+    const PaCut cut(a, gridDim.x);
+    const int quota = cut.quota;
+    if ((int)blockIdx.x > (cut.total - 1) / quota) return;
+    const int begin = blockIdx.x * quota, end = min(begin + quota, cut.total);
+    int at = begin, seq = 0, seq_start = 0;  // seq_start: the sequence's first unit
     for (int base = 0;; base += 32) {
-        const long long n = base + lane < a.n_seq ? (long long)tiles_of(length(base + lane)) * hc : 0;
-        long long incl = n;
+        const int n = base == 0 ? cut.first : base + lane < a.n_seq ? cut.units_of(base + lane) * hc : 0;
+        int incl = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long x = __shfl_up_sync(0xffffffffu, incl, o);
+            const int x = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += x;
         }
         const uint32_t hit = __ballot_sync(0xffffffffu, seq_start + incl > at);
@@ -155,10 +193,11 @@ __global__ void __launch_bounds__(PA_THREADS, (PaShape<D, Q8>::CTAS)) paged_attn
     const uint32_t ring = smem_u32(smem) + warp * S::RING;
     while (at < end) {
         // ---- one (sequence, kv head, chunk): its tiles [t0, t1) of n_tiles ----
-        const int len = length(seq), n_tiles = tiles_of(len);
-        const int pair = (int)((at - seq_start) / n_tiles);
-        const long long pair_start = seq_start + (long long)pair * n_tiles;
-        const int t0 = (int)(at - pair_start), t1 = (int)min((long long)n_tiles, end - pair_start);
+        const int len = cut.length(seq), n_tiles = PaCut::tiles_of(len);
+        const int units = PA_FIXED + n_tiles, pair = (at - seq_start) / units, first = seq_start + pair * units + PA_FIXED;
+        const int t0 = max(0, at - first), t1 = min(n_tiles, end - first);
+        at = first + n_tiles;
+        if (t1 <= 0) break;  // the run ends before the pair's first tile
         const int kvh = pair / a.chunks, h0 = (pair - kvh * a.chunks) * PA_HEADS, nh = min(PA_HEADS, a.group - h0);
         const int head0 = kvh * a.group + h0;
 
@@ -171,20 +210,22 @@ __global__ void __launch_bounds__(PA_THREADS, (PaShape<D, Q8>::CTAS)) paged_attn
         };
         int ids = load_ids(0);
 
-        // ---- the queries: scaled to log2 units, split ----
-        uint32_t qf[KK][4];
+        // the queries: loaded here, converted when the first tiles are on their way.  A's k = 2c, 2c+1
+        // (x 0) and 2c+8, 2c+9 (x 1) are dims in the order that K's fragments have
+        float2 qv[KK][2];
 #pragma unroll
         for (int kk = 0; kk < KK; kk++)
 #pragma unroll
             for (int x = 0; x < 2; x++) {
-                // A's k = 2c, 2c+1 (x 0) and 2c+8, 2c+9 (x 1), in the order that K's fragments have
                 const int d = Q8 ? 32 * (kk >> 1) + 8 * c + 4 * (kk & 1) + 2 * x : 16 * kk + 2 * c + 8 * x;
-                float2 f = make_float2(0.0f, 0.0f);
+                qv[kk][x] = make_float2(0.0f, 0.0f);
                 if (g < nh) {
                     const long long o = seq * a.q_stride + (long long)(head0 + g) * D + d;
-                    f = a.q_f16 ? __half22float2(*reinterpret_cast<const __half2*>(a.q + o * 2)) : *reinterpret_cast<const float2*>(a.q + o * 4);
+                    if (a.q_f16)
+                        qv[kk][x].x = __uint_as_float(*reinterpret_cast<const uint32_t*>(a.q + o * 2));
+                    else
+                        qv[kk][x] = *reinterpret_cast<const float2*>(a.q + o * 4);
                 }
-                split(f.x * a.scale_log2, f.y * a.scale_log2, &qf[kk][2 * x], &qf[kk][2 * x + 1]);
             }
 
         auto fetch = [&](int i) {  // tile i of this warp into its stage
@@ -219,6 +260,15 @@ __global__ void __launch_bounds__(PA_THREADS, (PaShape<D, Q8>::CTAS)) paged_attn
             for (int e = 0; e < 4; e++) o[j][e] = 0.0f;
 #pragma unroll
         for (int i = 0; i < S::STAGES - 1; i++) fetch(i);
+        uint32_t qf[KK][4];  // in log2 units, split
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++)
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const uint32_t raw = __float_as_uint(qv[kk][x].x);
+                const float2 f = a.q_f16 ? __half22float2(*reinterpret_cast<const __half2*>(&raw)) : qv[kk][x];
+                split(f.x * a.scale_log2, f.y * a.scale_log2, &qf[kk][2 * x], &qf[kk][2 * x + 1]);
+            }
         for (int i = 0; i < mine; i++) {
             if ((i + S::STAGES - 1) % 32 == 0) ids = load_ids(i + S::STAGES - 1);
             fetch(i + S::STAGES - 1);
@@ -342,106 +392,112 @@ __global__ void __launch_bounds__(PA_THREADS, (PaShape<D, Q8>::CTAS)) paged_attn
         l += __shfl_xor_sync(0xffffffffu, l, 2);
         __syncthreads();  // every warp is done with its stages
         float* meet = reinterpret_cast<float*>(smem);
-        float* wp = meet + warp * S::PART + g * (D + 2);
+        float* mine_o = meet + warp * S::MEET + g * S::MEET_ROW;
+        if (Q8) {
 #pragma unroll
-        for (int j = 0; j < NT; j++)
+            for (int b = 0; b < NB; b++)
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const int d = Q8 ? 32 * (j >> 2) + 4 * (2 * c + e) + (j & 3) : 8 * j + 2 * c + e;
-                wp[d] = (o[j][e] + o[j][e + 2]) * (Q8 ? 1.0f / PA_V_UNIT : 1.0f);
-            }
-        if (c == 0) {
-            wp[D] = m;
-            wp[D + 1] = l;
+                for (int e = 0; e < 2; e++) {
+                    float f[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) f[i] = (o[4 * b + i][e] + o[4 * b + i][e + 2]) * (1.0f / PA_V_UNIT);
+                    *reinterpret_cast<float4*>(mine_o + 32 * b + 8 * c + 4 * e) = make_float4(f[0], f[1], f[2], f[3]);
+                }
+        } else {
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+                *reinterpret_cast<float2*>(mine_o + 8 * j + 2 * c) = make_float2(o[j][0] + o[j][2], o[j][1] + o[j][3]);
         }
+        if (c == 0) *reinterpret_cast<float2*>(mine_o + D) = make_float2(m, l);
         __syncthreads();
-        // joins n partial results (stride `step` floats) for head h, dim d
-        auto join = [&](const float* part, int n, long long step, int h, int d, float* om, float* ol) {
-            float mm = -INFINITY;
-            for (int i = 0; i < n; i++) mm = fmaxf(mm, __ldcg(part + i * step + h * (D + 2) + D));
-            float ll = 0.0f, oo = 0.0f;
-            for (int i = 0; i < n; i++) {
-                const float* p = part + i * step + h * (D + 2);
-                const float mi = __ldcg(p + D), f = mi == -INFINITY ? 0.0f : ex2(mi - mm);
-                ll = fmaf(f, __ldcg(p + D + 1), ll);
-                oo = fmaf(f, __ldcg(p + d), oo);
-            }
-            *om = mm;
-            *ol = ll;
-            return oo;
-        };
-        auto join_warps = [&](int h, int d, float* om, float* ol) {
-            const float* p = meet + h * (D + 2);
-            float mm = -INFINITY, ll = 0.0f, oo = 0.0f;
+        const bool whole = t0 == 0 && t1 == n_tiles;
+        // a CTA leaves at most two partial results: of a pair that it goes on with, and of one that it leaves unfinished
+        float* part = a.parts + (2LL * blockIdx.x + (t0 == 0 ? 1 : 0)) * S::PART;
+        for (int i = tid; i < nh * (D / 4); i += PA_THREADS) {
+            const int h = i / (D / 4), d = i % (D / 4) * 4;
+            const float* p = meet + h * S::MEET_ROW;
+            float mm = -INFINITY, ll = 0.0f;
+            float4 oo = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-            for (int w = 0; w < PA_WARPS; w++) mm = fmaxf(mm, p[w * S::PART + D]);
+            for (int w = 0; w < PA_WARPS; w++) mm = fmaxf(mm, p[w * S::MEET + D]);
 #pragma unroll
             for (int w = 0; w < PA_WARPS; w++) {
-                const float mi = p[w * S::PART + D], f = mi == -INFINITY ? 0.0f : ex2(mi - mm);
-                ll = fmaf(f, p[w * S::PART + D + 1], ll);
-                oo = fmaf(f, p[w * S::PART + d], oo);
+                const float2 ml = *reinterpret_cast<const float2*>(p + w * S::MEET + D);
+                const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - mm);
+                ll = fmaf(f, ml.y, ll);
+                add_to(oo, f, *reinterpret_cast<const float4*>(p + w * S::MEET + d));
             }
-            *om = mm;
-            *ol = ll;
-            return oo;
-        };
-        auto write = [&](int h, int d, float v, float sum) {
-            const float r = sum == 0.0f ? 0.0f : v / sum;
-            const long long w = seq * a.out_stride + (long long)(head0 + h) * D + d;
-            if (a.out_f16)
-                reinterpret_cast<uint16_t*>(a.out)[w] = f2h_bits(r);
-            else
-                reinterpret_cast<float*>(a.out)[w] = r;
-        };
-        const bool whole = t0 == 0 && t1 == n_tiles;
-        // a CTA leaves at most two partial results: of the pair that its run begins in, and of the last
-        float* part = a.parts + (2LL * blockIdx.x + (pair_start > blockIdx.x * quota ? 1 : 0)) * S::PART;
-        for (int i = tid; i < nh * D; i += PA_THREADS) {
-            const int h = i / D, d = i % D;
-            float mm, ll;
-            const float oo = join_warps(h, d, &mm, &ll);
             if (whole) {
-                write(h, d, oo, ll);
+                write_out(a, seq, head0 + h, D, d, oo, ll);
             } else {
-                __stcg(part + h * (D + 2) + d, oo);
-                if (d == 0) {
-                    __stcg(part + h * (D + 2) + D, mm);
-                    __stcg(part + h * (D + 2) + D + 1, ll);
-                }
-            }
-        }
-        if (!whole) {
-            const long long b0 = pair_start / quota, b1 = (pair_start + n_tiles - 1) / quota;  // its CTAs
-            __threadfence();
-            __syncthreads();
-            unsigned int* count = a.counters + (long long)seq * hc + pair;
-            if (tid == 0) s_last = atomicAdd(count, 1u) == (unsigned)(b1 - b0);
-            __syncthreads();
-            if (s_last) {
-                __threadfence();
-                if (tid == 0) *count = 0u;
-                // CTA b0's result is in its second place unless the pair begins its run
-                const float* first = a.parts + (2 * b0 + (pair_start > b0 * quota ? 1 : 0)) * S::PART;
-                for (int i = tid; i < nh * D; i += PA_THREADS) {
-                    const int h = i / D, d = i % D;
-                    float m0, l0, m1, l1;
-                    const float o0 = join(first, 1, 0, h, d, &m0, &l0);
-                    const float o1 = join(a.parts + 2 * (b0 + 1) * S::PART, (int)(b1 - b0), 2 * S::PART, h, d, &m1, &l1);
-                    const float mm = fmaxf(m0, m1), f0 = m0 == -INFINITY ? 0.0f : ex2(m0 - mm), f1 = m1 == -INFINITY ? 0.0f : ex2(m1 - mm);
-                    write(h, d, o0 * f0 + o1 * f1, l0 * f0 + l1 * f1);
-                }
+                __stcg(reinterpret_cast<float4*>(part + h * D + d), oo);
+                if (d == 0) __stcg(reinterpret_cast<float2*>(part + PA_HEADS * D + 2 * h), make_float2(mm, ll));
             }
         }
         __syncthreads();  // the meeting place is free for the next pair's stages
-        at = pair_start + t1;
-        if (pair == hc - 1 && t1 == n_tiles) {
+        if (pair == hc - 1) {
             seq_start = at;
             seq++;
         }
     }
 }
 
-template <int D, bool Q8> int launch(PaArgs& a, long long pairs, long long most_tiles, cudaStream_t stream) {
+// Joins the results of a pair's CTAs, in their order; a pair that one CTA did whole is already written.
+// Grid: (pair, sequence).  Thread (x, d): results x, x + PJ_WAYS, ... of the four dims d of a head in turn.
+template <int D, bool Q8>
+__global__ void __launch_bounds__(PA_THREADS) paged_join(const PaArgs a, int ctas) {
+    using S = PaShape<D, Q8>;
+    extern __shared__ __align__(16) float2 ml[];  // [result][head]: maximum and sum
+    __shared__ float peak[PA_WARPS][PA_HEADS];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hc = a.n_kv_head * a.chunks;
+    const int pair = blockIdx.x, seq = blockIdx.y;
+    pdl_launch_dependents();
+    pdl_wait();
+    const PaCut cut(a, ctas);
+    int before = 0;
+    for (int s = lane; s < seq; s += 32) before += s < 32 ? cut.first : cut.units_of(s) * hc;
+    before = __reduce_add_sync(0xffffffffu, before);
+    const int n_tiles = PaCut::tiles_of(cut.length(seq)), first = before + pair * (PA_FIXED + n_tiles) + PA_FIXED;
+    const int b0 = first / cut.quota, n = (first + n_tiles - 1) / cut.quota - b0 + 1;  // the CTAs that have its tiles
+    if (n == 1) return;
+    const int kvh = pair / a.chunks, h0 = (pair - kvh * a.chunks) * PA_HEADS, nh = min(PA_HEADS, a.group - h0);
+    auto result = [&](int i) { return a.parts + (2LL * (b0 + i) + (i == 0 ? 1 : 0)) * S::PART; };
+    float top = -INFINITY;
+    for (int i = tid; i < n * PA_HEADS; i += PA_THREADS) {  // this thread's head: tid % 8
+        const float2 x = i % PA_HEADS < nh ? __ldcg(reinterpret_cast<const float2*>(result(i / PA_HEADS) + PA_HEADS * D) + i % PA_HEADS)
+                                           : make_float2(-INFINITY, 0.0f);
+        ml[i] = x;
+        top = fmaxf(top, x.x);
+    }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+    if (lane < PA_HEADS) peak[warp][lane] = top;
+    __syncthreads();
+    for (int i = tid; i < nh * (D / 4); i += PA_THREADS) {
+        const int h = i / (D / 4), d = i % (D / 4) * 4;
+        float mm = peak[0][h], ll = 0.0f;
+#pragma unroll
+        for (int w = 1; w < PA_WARPS; w++) mm = fmaxf(mm, peak[w][h]);
+        float4 oo = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int x0 = 0; x0 < n; x0 += 8) {
+            float4 v[8];
+#pragma unroll
+            for (int x = 0; x < 8; x++)
+                if (x0 + x < n) v[x] = __ldcg(reinterpret_cast<const float4*>(result(x0 + x) + h * D + d));
+#pragma unroll
+            for (int x = 0; x < 8; x++)
+                if (x0 + x < n) {
+                    const float2 y = ml[(x0 + x) * PA_HEADS + h];
+                    const float f = y.x == -INFINITY ? 0.0f : ex2(y.x - mm);
+                    ll = fmaf(f, y.y, ll);
+                    add_to(oo, f, v[x]);
+                }
+        }
+        write_out(a, seq, kvh * a.group + h0 + h, D, d, oo, ll);
+    }
+}
+
+template <int D, bool Q8> int launch(PaArgs& a, long long most_units, cudaStream_t stream) {
     using S = PaShape<D, Q8>;
     static CfiPerDeviceOnce once;
     static int sms[CFI_MAX_DEVICES + 1];
@@ -452,15 +508,14 @@ template <int D, bool Q8> int launch(PaArgs& a, long long pairs, long long most_
         cudaGetDevice(&d);
         cudaDeviceGetAttribute(n, cudaDevAttrMultiProcessorCount, d);
         cudaFuncSetAttribute(paged_attn<D, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+        cudaFuncSetAttribute(paged_join<D, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::CTAS * PA_MAX_SMS * PA_HEADS * 8);
     });
-    const long long ctas = (long long)(*n > 0 ? *n : 148) * S::CTAS;
-    // no CTA has fewer tiles than warps
-    const long long grid = most_tiles / PA_WARPS + 1 < ctas ? most_tiles / PA_WARPS + 1 : ctas;
+    const long long ctas = (long long)(*n > 0 && *n <= PA_MAX_SMS ? *n : 148) * S::CTAS;
+    // no CTA has fewer units than this
+    const long long grid = std::min(ctas, most_units / (PA_FIXED + PA_WARPS) + 1);
     int err = 0;
     a.parts = static_cast<float*>(cfi_stream_buffer(CFI_BUF_PAGED_PARTS, (size_t)ctas * 2 * S::PART * 4, stream, &err));
     if (!a.parts) return err;
-    a.counters = static_cast<unsigned int*>(cfi_stream_buffer(CFI_BUF_COUNTERS, (size_t)pairs * 4, stream, &err));
-    if (!a.counters) return err;
     const char* ep = getenv("CFI_PDL");
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3((unsigned)grid, 1, 1);
@@ -472,7 +527,11 @@ template <int D, bool Q8> int launch(PaArgs& a, long long pairs, long long most_
     at[0].val.programmaticStreamSerializationAllowed = 1;
     lc.attrs = at;
     lc.numAttrs = (ep && strcmp(ep, "0") == 0) ? 0 : 1;
-    return (int)cudaLaunchKernelEx(&lc, paged_attn<D, Q8>, (const PaArgs)a);
+    err = (int)cudaLaunchKernelEx(&lc, paged_attn<D, Q8>, (const PaArgs)a);
+    if (err || grid == 1) return err;
+    lc.gridDim = dim3((unsigned)(a.n_kv_head * a.chunks), (unsigned)a.n_seq, 1);
+    lc.dynamicSmemBytes = (size_t)grid * PA_HEADS * sizeof(float2);
+    return (int)cudaLaunchKernelEx(&lc, paged_join<D, Q8>, (const PaArgs)a, (int)grid);
 }
 
 }  // namespace
@@ -506,8 +565,9 @@ extern "C" int cfi_paged_attention(const CfiPagedCache* c, const void* q, int q_
     a.out_f16 = out_type;
     a.scale_log2 = scale * 1.4426950408889634f;
     const long long pairs = (long long)n_seq * c->n_kv_head * a.chunks;
-    const long long most_tiles = pairs * ((long long)max_pages * (c->page_size / PA_TILE));
+    const long long most_units = pairs * (PA_FIXED + (long long)max_pages * (c->page_size / PA_TILE));
+    if (most_units > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (c->head_dim == 64) return c->type == 1 ? launch<64, false>(a, pairs, most_tiles, s) : launch<64, true>(a, pairs, most_tiles, s);
-    return c->type == 1 ? launch<128, false>(a, pairs, most_tiles, s) : launch<128, true>(a, pairs, most_tiles, s);
+    if (c->head_dim == 64) return c->type == 1 ? launch<64, false>(a, most_units, s) : launch<64, true>(a, most_units, s);
+    return c->type == 1 ? launch<128, false>(a, most_units, s) : launch<128, true>(a, most_units, s);
 }
