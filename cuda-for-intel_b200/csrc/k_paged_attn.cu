@@ -35,7 +35,6 @@ constexpr int PA_WARPS = 4, PA_THREADS = PA_WARPS * 32;
 constexpr int PA_HEADS = 8;        // query heads of a chunk
 constexpr int PA_TILE = 16;        // positions; a page is a multiple of it
 constexpr float PA_V_UNIT = 256.0f;
-constexpr int PA_MAX_SMS = 256;
 // What beginning and ending a pair costs, in tiles: a run's share of the list counts it, so that CTAs with
 // many short sequences get fewer tiles.
 #ifndef PA_FIXED_TILES
@@ -442,15 +441,17 @@ __global__ void __launch_bounds__(PA_THREADS, (PaShape<D, Q8>::CTAS)) paged_attn
     }
 }
 
-// Joins the results of a pair's CTAs, in their order; a pair that one CTA did whole is already written.
-// Grid: (pair, sequence).  Thread (x, d): results x, x + PJ_WAYS, ... of the four dims d of a head in turn.
+// Joins the results of a pair's CTAs, one head a CTA; a pair that one CTA did whole is already written.  Thread
+// (way, d) takes results way, way + WAYS, ... of four dims, all loads of a round before the first use.
 template <int D, bool Q8>
 __global__ void __launch_bounds__(PA_THREADS) paged_join(const PaArgs a, int ctas) {
     using S = PaShape<D, Q8>;
-    extern __shared__ __align__(16) float2 ml[];  // [result][head]: maximum and sum
-    __shared__ float peak[PA_WARPS][PA_HEADS];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, hc = a.n_kv_head * a.chunks;
-    const int pair = blockIdx.x, seq = blockIdx.y;
+    constexpr int QUADS = D / 4, WAYS = PA_THREADS / QUADS, ROUND = 4;
+    __shared__ float4 so[WAYS][QUADS];
+    __shared__ float2 sm[WAYS];
+    const int tid = threadIdx.x, lane = tid & 31, way = tid / QUADS, d = tid % QUADS * 4, hc = a.n_kv_head * a.chunks;
+    const int head = blockIdx.x, seq = blockIdx.y, h = head % a.group % PA_HEADS;
+    const int pair = head / a.group * a.chunks + head % a.group / PA_HEADS;
     pdl_launch_dependents();
     pdl_wait();
     const PaCut cut(a, ctas);
@@ -460,40 +461,49 @@ __global__ void __launch_bounds__(PA_THREADS) paged_join(const PaArgs a, int cta
     const int n_tiles = PaCut::tiles_of(cut.length(seq)), first = before + pair * (PA_FIXED + n_tiles) + PA_FIXED;
     const int b0 = first / cut.quota, n = (first + n_tiles - 1) / cut.quota - b0 + 1;  // the CTAs that have its tiles
     if (n == 1) return;
-    const int kvh = pair / a.chunks, h0 = (pair - kvh * a.chunks) * PA_HEADS, nh = min(PA_HEADS, a.group - h0);
-    auto result = [&](int i) { return a.parts + (2LL * (b0 + i) + (i == 0 ? 1 : 0)) * S::PART; };
-    float top = -INFINITY;
-    for (int i = tid; i < n * PA_HEADS; i += PA_THREADS) {  // this thread's head: tid % 8
-        const float2 x = i % PA_HEADS < nh ? __ldcg(reinterpret_cast<const float2*>(result(i / PA_HEADS) + PA_HEADS * D) + i % PA_HEADS)
-                                           : make_float2(-INFINITY, 0.0f);
-        ml[i] = x;
-        top = fmaxf(top, x.x);
-    }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-    if (lane < PA_HEADS) peak[warp][lane] = top;
-    __syncthreads();
-    for (int i = tid; i < nh * (D / 4); i += PA_THREADS) {
-        const int h = i / (D / 4), d = i % (D / 4) * 4;
-        float mm = peak[0][h], ll = 0.0f;
+    const float* parts = a.parts + 2LL * b0 * S::PART;
+    float m = -INFINITY, l = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int x0 = way; x0 < n; x0 += WAYS * ROUND) {
+        float4 v[ROUND];
+        float2 ml[ROUND];
 #pragma unroll
-        for (int w = 1; w < PA_WARPS; w++) mm = fmaxf(mm, peak[w][h]);
-        float4 oo = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int x0 = 0; x0 < n; x0 += 8) {
-            float4 v[8];
-#pragma unroll
-            for (int x = 0; x < 8; x++)
-                if (x0 + x < n) v[x] = __ldcg(reinterpret_cast<const float4*>(result(x0 + x) + h * D + d));
-#pragma unroll
-            for (int x = 0; x < 8; x++)
-                if (x0 + x < n) {
-                    const float2 y = ml[(x0 + x) * PA_HEADS + h];
-                    const float f = y.x == -INFINITY ? 0.0f : ex2(y.x - mm);
-                    ll = fmaf(f, y.y, ll);
-                    add_to(oo, f, v[x]);
-                }
+        for (int i = 0; i < ROUND; i++) {
+            const int x = x0 + i * WAYS;
+            // the first CTA's result is in its second place: it leaves the pair unfinished
+            const float* p = parts + (2LL * x + (x == 0 ? 1 : 0)) * S::PART;
+            ml[i] = x < n ? __ldcg(reinterpret_cast<const float2*>(p + PA_HEADS * D) + h) : make_float2(-INFINITY, 0.0f);
+            v[i] = x < n ? __ldcg(reinterpret_cast<const float4*>(p + h * D + d)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
-        write_out(a, seq, kvh * a.group + h0 + h, D, d, oo, ll);
+        float mm = m;
+#pragma unroll
+        for (int i = 0; i < ROUND; i++) mm = fmaxf(mm, ml[i].x);
+        const float keep = m == -INFINITY ? 0.0f : ex2(m - mm);
+        l *= keep;
+        o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
+        m = mm;
+#pragma unroll
+        for (int i = 0; i < ROUND; i++) {
+            const float f = ml[i].x == -INFINITY ? 0.0f : ex2(ml[i].x - mm);
+            l = fmaf(f, ml[i].y, l);
+            add_to(o, f, v[i]);
+        }
+    }
+    so[way][d / 4] = o;
+    if (d == 0) sm[way] = make_float2(m, l);
+    __syncthreads();
+    if (way == 0) {
+        float mm = m, ll = 0.0f;
+#pragma unroll
+        for (int w = 1; w < WAYS; w++) mm = fmaxf(mm, sm[w].x);
+        o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < WAYS; w++) {
+            const float f = sm[w].x == -INFINITY ? 0.0f : ex2(sm[w].x - mm);
+            ll = fmaf(f, sm[w].y, ll);
+            add_to(o, f, so[w][d / 4]);
+        }
+        write_out(a, seq, head, D, d, o, ll);
     }
 }
 
@@ -508,9 +518,8 @@ template <int D, bool Q8> int launch(PaArgs& a, long long most_units, cudaStream
         cudaGetDevice(&d);
         cudaDeviceGetAttribute(n, cudaDevAttrMultiProcessorCount, d);
         cudaFuncSetAttribute(paged_attn<D, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
-        cudaFuncSetAttribute(paged_join<D, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::CTAS * PA_MAX_SMS * PA_HEADS * 8);
     });
-    const long long ctas = (long long)(*n > 0 && *n <= PA_MAX_SMS ? *n : 148) * S::CTAS;
+    const long long ctas = (long long)(*n > 0 ? *n : 148) * S::CTAS;
     // no CTA has fewer units than this
     const long long grid = std::min(ctas, most_units / (PA_FIXED + PA_WARPS) + 1);
     int err = 0;
@@ -529,8 +538,8 @@ template <int D, bool Q8> int launch(PaArgs& a, long long most_units, cudaStream
     lc.numAttrs = (ep && strcmp(ep, "0") == 0) ? 0 : 1;
     err = (int)cudaLaunchKernelEx(&lc, paged_attn<D, Q8>, (const PaArgs)a);
     if (err || grid == 1) return err;
-    lc.gridDim = dim3((unsigned)(a.n_kv_head * a.chunks), (unsigned)a.n_seq, 1);
-    lc.dynamicSmemBytes = (size_t)grid * PA_HEADS * sizeof(float2);
+    lc.gridDim = dim3((unsigned)(a.n_kv_head * a.group), (unsigned)a.n_seq, 1);
+    lc.dynamicSmemBytes = 0;
     return (int)cudaLaunchKernelEx(&lc, paged_join<D, Q8>, (const PaArgs)a, (int)grid);
 }
 
