@@ -1,16 +1,22 @@
 // k_sample.cu -- one token per row of logits: temperature, top-k, top-p, min-p and a given uniform
 // number (include/cfi_serve.h gives the definition).
 //
-// A cluster of CTAs takes a row.  The logits are read once: each CTA keeps its slice of z = logit /
-// temperature in shared memory, the later passes walk it there and meet through distributed shared memory.
-// Everything that is summed is a whole number (a weight is exp(z - max) in units of 2^-40), so no sum
-// depends on its order and every CTA of a cluster reaches the same decisions from the same histograms.
+// A cluster of CTAs takes a row.  The logits are read once, by bulk copies: each CTA keeps its slice in
+// shared memory, the later passes walk it there and meet through distributed shared memory.  Everything
+// that is summed is a whole number (a weight is exp(z - max) in units of 2^-40), so no sum depends on its order
+// and every CTA of a cluster reaches the same decisions from the same histograms.
 //
-// All three filters keep a run from the top of the order (larger z first, then lower index), so each
-// is a cut: the last element that stays.  A cut is found without sorting: a histogram over 512 bins of
-// max - z finds the bin that the cut falls in; the at most SA_LIST elements of that bin are listed and each
-// one's rank is counted against the others.  A fuller bin is divided again: first by the next bits of
-// max - z, then by the bits of z itself, after which all that is left is equal and the index decides.
+// All three filters keep a run from the top of the order (larger z first, then lower index).  Where that run
+// is short -- it is, when a top-k or a nucleus of a language model's logits is asked for -- the bins of a
+// histogram of max - z say down to which depth it can reach, the few elements above that depth are gathered in
+// the cluster's first CTA, and that CTA sorts them and finishes alone.  The gathering needs no exact z: bins
+// of (max logit - logit) / T are 1/64 wide, far above the rounding of z, and one bin more is taken.
+//
+// Where it is long (more than SA_CAP elements) each filter is a cut, the last element that stays, found
+// without sorting: a histogram over 512 bins finds the bin that the cut falls in; the at most SA_LIST
+// elements of that bin are listed and each one's rank is counted against the others.  A fuller bin is divided
+// again: first by the next bits of max - z, then by the bits of z itself, after which all that is left is
+// equal and the index decides.
 #include "../../include/cfi_serve.h"
 #include "sm100_ptx.cuh"
 #include "cfi_kernels.h"
@@ -24,7 +30,8 @@ using namespace sm100;
 
 constexpr int SA_THREADS = 512, SA_WARPS = SA_THREADS / 32;
 constexpr int SA_BINS = SA_THREADS;   // a thread holds a bin's total
-constexpr int SA_LIST = 256;          // boundary-bin elements of one CTA that are listed
+constexpr int SA_LIST = 256;          // boundary-bin elements that are listed
+constexpr int SA_CAP = 1024;          // elements that the first CTA sorts (two a thread)
 constexpr int SA_MAX_CTAS = 8;
 constexpr int SA_MAX_SLICE = 50000;   // floats of a row that one CTA holds
 constexpr int SA_MAX_VOCAB = SA_MAX_CTAS * SA_MAX_SLICE;
@@ -37,6 +44,7 @@ struct SaArgs {
     int32_t* token;
     float* logprob;
     int n_vocab, slice;
+    unsigned int* err;
 };
 
 struct SaItem {
@@ -44,23 +52,31 @@ struct SaItem {
     int idx;
     unsigned long long w;
 };
+static_assert(SA_MAX_SLICE <= 65536, "a slice's indexes take 16 bits");
 
 struct SaShared {
     uint32_t cnt[2][SA_BINS];
-    unsigned long long wt[2][SA_BINS];
-    SaItem list[2][SA_LIST];
-    unsigned long long sums[SA_WARPS];
-    uint32_t ties[SA_WARPS];
+    unsigned long long wt[2][SA_BINS];  // in the end: the sorted elements' weights
+    union {
+        SaItem list[2][SA_LIST];           // long runs: the boundary bin's elements
+        unsigned long long order[SA_CAP];  // short runs: index and rank of the kept ones
+    };
+    unsigned long long cand[SA_CAP];    // gathered elements: logit's bits, index
+    uint16_t own[SA_CAP];               // this CTA's share of them
+    uint64_t bar;
     unsigned long long scan[SA_WARPS];
-    uint32_t scan_n[SA_WARPS];
+    unsigned long long cta_sum, kept_sum;
+    uint32_t ties[SA_WARPS];
     float wmax[SA_WARPS];
     float cta_max;
-    int n_list[2];
+    int n_list[2], n_own, n_cand, base;
+    int abort;
     int found_bin;
     unsigned long long found_before;
     uint32_t found_n, cut_key;
     int cut_idx;
 };
+static_assert(sizeof(unsigned long long) * 2 * SA_BINS >= sizeof(unsigned long long) * SA_CAP, "the weights take the histogram's place");
 
 // The same variable of CTA `rank` of the cluster.
 template <class T> CFI_DEV const T* peer(const T* p, uint32_t rank) {
@@ -74,9 +90,11 @@ CFI_DEV uint32_t key_of(float z) {
     const uint32_t b = __float_as_uint(z);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+CFI_DEV float z_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
+constexpr double SA_UNIT = 1099511627776.0;  // 2^40
 // exp(z - max) in units of 2^-40: 24 bits of expf, scaled without rounding, cut to whole units
 CFI_DEV float exp_of(float z, float zmax) { return z == zmax ? 1.0f : expf(z - zmax); }
-CFI_DEV unsigned long long weight_of(float e) { return (unsigned long long)(e * 1099511627776.0f); }
+CFI_DEV unsigned long long weight_of(float e) { return (unsigned long long)(e * (float)SA_UNIT); }
 // max - z in units of 2^-22, 27 bits: a weight is zero from 27.8 on
 CFI_DEV uint32_t depth_of(float z, float zmax) { return z == zmax ? 0u : (uint32_t)fminf((zmax - z) * 4194304.0f, 134217727.0f); }
 
@@ -121,50 +139,304 @@ struct SaPrefix {
     }
 };
 
+// Inclusive sum over the block's threads, and the whole sum.  Ends with every thread past its reads of `scan`.
+CFI_DEV unsigned long long block_incl(unsigned long long v, unsigned long long* scan, unsigned long long* total) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    unsigned long long incl = warp_incl(v, lane);
+    if (lane == 31) scan[warp] = incl;
+    __syncthreads();
+    unsigned long long prev = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < SA_WARPS; w++) {
+        const unsigned long long x = scan[w];
+        if (w < warp) prev += x;
+        all += x;
+    }
+    __syncthreads();
+    *total = all;
+    return incl + prev;
+}
+
+// The sum of v over the block (ties: a word for each warp).
+CFI_DEV int block_count(int v, uint32_t* words) {
+    v = __reduce_add_sync(0xffffffffu, v);
+    if ((threadIdx.x & 31) == 0) words[threadIdx.x >> 5] = (uint32_t)v;
+    __syncthreads();
+    int n = 0;
+#pragma unroll
+    for (int w = 0; w < SA_WARPS; w++) n += (int)words[w];
+    __syncthreads();
+    return n;
+}
+
+// Sorts n (a power of two, at most SA_CAP) numbers in rising order.
+CFI_DEV void block_sort(unsigned long long* v, int n) {
+    for (int k = 2; k <= n; k <<= 1)
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            __syncthreads();
+            const int t = threadIdx.x;
+            if (t < n / 2) {
+                const int i = (t / j) * 2 * j + t % j;  // j is a power of two
+                const unsigned long long x = v[i], y = v[i + j];
+                if ((x > y) == ((i & k) == 0)) {
+                    v[i] = y;
+                    v[i + j] = x;
+                }
+            }
+        }
+    __syncthreads();
+}
+CFI_DEV int power_of_two(int n) { return n <= 2 ? 2 : 1 << (32 - __clz(n - 1)); }
+
 __global__ void __launch_bounds__(SA_THREADS) sample_rows(const SaArgs a) {
-    extern __shared__ float z[];
+    extern __shared__ __align__(16) float slice[];
     __shared__ SaShared s;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = cluster_ctarank(), ctas = cluster_nctarank();
     const int row = blockIdx.x / ctas;
     const int base = rank * a.slice, n = max(0, min(a.slice, a.n_vocab - base));
-    const int chunk = ((n + SA_WARPS - 1) / SA_WARPS + 31) & ~31;  // each warp's run of the slice
-    const int w0 = min(n, warp * chunk), w1 = min(n, w0 + chunk);
+    if (tid == 0) {
+        mbar_init(&s.bar, 1);
+        s.abort = s.n_own = s.n_cand = 0;
+        s.kept_sum = 0;
+        fence_mbar_init();
+    }
+    for (int b = tid; b < SA_BINS; b += SA_THREADS) {
+        s.cnt[0][b] = 0;
+        s.wt[0][b] = 0;
+    }
+    __syncthreads();
     pdl_launch_dependents();
     pdl_wait();
 
+    // ---- the one read of the row: 16-byte pieces by bulk copies, the ragged ends by loads ----
+    const float* src = a.logits + row * a.stride + base;
+    const int shift = (int)(reinterpret_cast<uintptr_t>(src) >> 2 & 3), head = min(n, (4 - shift) & 3), body = (n - head) & ~3;
+    float* z = slice + shift;  // logit i of the slice is z[i], 16-byte aligned where it is in memory
+    if (tid == 0 && body > 0) {
+        mbar_arrive_expect_tx(&s.bar, (uint32_t)body * 4);
+        for (int i = 0; i < body; i += 8192)
+            bulk_g2s(z + head + i, src + head + i, (uint32_t)min(8192, body - i) * 4, &s.bar);
+    }
+    if (tid < head) z[tid] = src[tid];
+    if (tid >= 32 && tid < 32 + n - head - body) z[head + body + tid - 32] = src[head + body + tid - 32];
     const float t = a.temperature ? a.temperature[row] : 1.0f;
     const bool greedy = t <= 0.0f;
     const float div = greedy ? 1.0f : t;
     int k = a.top_k ? a.top_k[row] : 0;
     if (greedy) k = 1;
+    if (k >= a.n_vocab) k = 0;
     const float p = a.top_p ? a.top_p[row] : 1.0f;
     const float minp = a.min_p ? a.min_p[row] : 0.0f;
-
-    // ---- the one read of the row ----
-    const float* src = a.logits + row * a.stride + base;
-    float mx = -INFINITY;
-    for (int i = w0 + lane; i < w1; i += 32) {
-        float v = src[i] / div + 0.0f;
-        v = v == v ? v : -INFINITY;
-        z[i] = v;
-        mx = fmaxf(mx, v);
+    if (body > 0 && !mbar_wait(&s.bar, 0, &s.abort)) {
+        cfi_set_error(a.err, 0xfc100);
+        s.abort = 1;
     }
+    __syncthreads();
+
+    // element i's z: never -0, and -inf for a NaN
+    auto scaled = [&](float l) {
+        const float v = (div == 1.0f ? l : l / div) + 0.0f;
+        return v == v ? v : -INFINITY;
+    };
+    const int chunk = ((n + SA_WARPS - 1) / SA_WARPS + 31) & ~31;  // each warp's run of the slice
+    const int w0 = min(n, warp * chunk), w1 = min(n, w0 + chunk);
+    const int run = ((n + SA_THREADS - 1) / SA_THREADS) | 1;  // each thread's run: odd, so that 32 of them meet no bank twice
+    const int r0 = min(n, tid * run), r1 = min(n, r0 + run);
+    float mx = -INFINITY;
+#pragma unroll 4
+    for (int i = tid; i < n; i += SA_THREADS) mx = fmaxf(mx, z[i]);  // a NaN is passed over
     mx = warp_max(mx);
     if (lane == 0) s.wmax[warp] = mx;
     __syncthreads();
-    if (tid == 0) {
-        for (int w = 1; w < SA_WARPS; w++) mx = fmaxf(mx, s.wmax[w]);
-        s.cta_max = mx;
+    if (warp == 0) {
+        mx = warp_max(lane < SA_WARPS ? s.wmax[lane] : -INFINITY);
+        if (lane == 0) s.cta_max = mx;
     }
     cluster_sync();
-    float zmax = -INFINITY;
-    for (uint32_t r = 0; r < ctas; r++) zmax = fmaxf(zmax, *peer(&s.cta_max, r));
+    float lmax = lane < (int)ctas ? *peer(&s.cta_max, lane) : -INFINITY;
+    lmax = warp_max(lmax);
+    const float zmax = scaled(lmax);  // division by a positive number keeps the order
+    const bool empty = zmax == -INFINITY;
+
+    auto logprob_of = [&](float v, unsigned long long total) {
+        return (v == zmax ? 0.0f : v - zmax) - logf((float)((double)total / SA_UNIT));
+    };
+    auto target_of = [&](unsigned long long total) {
+        const double ud = (double)a.u[row] * (double)total;
+        const unsigned long long target = ud > 0.0 ? (unsigned long long)ud : 0ull;
+        return target < total ? target : total - 1;  // u outside [0, 1)
+    };
+
+    // ---- no top-k: every weight counts.  Each thread sums its run; with a top-p, the top of the order by bins ----
+    unsigned long long run_sum = 0, whole = 0;
+    const float near = 1.0f / div;
+    const bool bins_hold = fabsf(zmax) < 8192.0f && near < 1e30f;  // z is exact to far less than a bin
+    if (!empty && k <= 0) {
+        const bool binned = p < 1.0f;
+        for (int i = r0; i < r1; i++) {
+            const float v = scaled(z[i]);
+            const unsigned long long w = weight_of(exp_of(v, zmax));
+            run_sum += w;
+            if (binned && bins_hold) {
+                const float d = (zmax - v) * 64.0f;
+                if (d < (float)SA_BINS) {
+                    atomicAdd(&s.cnt[0][(int)d], 1u);
+                    atomicAdd(&s.wt[0][(int)d], w);
+                }
+            }
+        }
+        unsigned long long sum;
+        block_incl(run_sum, s.scan, &sum);
+        if (tid == 0) s.cta_sum = sum;
+        cluster_sync();
+        for (uint32_t r = 0; r < ctas; r++) whole += *peer(&s.cta_sum, r);
+    }
+    uint32_t level = 1;  // histogram 0 has been used
+    // ---- a short run: down to which depth? ----
+    float depth = -1.0f;  // gather what lies less deep (in units of z)
+    if (!empty && bins_hold && (k > 0 || p < 1.0f)) {
+        float scale = 64.0f;
+        for (int turn = 0;; turn++) {
+            const uint32_t b = turn & 1;
+            if (k > 0) {
+                if (turn > 0) {
+                    s.cnt[b][tid] = 0;
+                    __syncthreads();
+                }
+                for (int i = w0 + lane; i < w1; i += 32) {
+                    const float d = (lmax - z[i]) * near * scale;  // a NaN compares false
+                    if (d < (float)SA_BINS) atomicAdd(&s.cnt[b][(int)d], 1u);
+                }
+                cluster_sync();
+            }
+            uint32_t c = 0;
+            unsigned long long m = 0;
+            for (uint32_t r = 0; r < ctas; r++) {
+                c += *peer(&s.cnt[b][tid], r);
+                if (k <= 0) m += *peer(&s.wt[b][tid], r);
+            }
+            unsigned long long all;
+            // counts in the upper bits would not leave room for the weights: two sums where both are needed
+            const unsigned long long upto = block_incl(c, s.scan, &all);
+            bool reached = upto >= (unsigned long long)k;
+            if (k <= 0) {
+                unsigned long long ignore;
+                reached = !((double)block_incl(m, s.scan, &ignore) < (double)p * (double)whole);
+            }
+            // the first bin whose end lies past the run's; with the next one, and one more for the rounding
+            if (tid == 0) s.found_bin = SA_BINS;
+            __syncthreads();
+            if (reached) atomicMin(&s.found_bin, tid);
+            __syncthreads();
+            const int bin = s.found_bin;
+            if (bin + 2 < SA_BINS) {
+                if (tid == bin + 2) s.found_n = (uint32_t)upto;
+                __syncthreads();
+                if (s.found_n <= SA_CAP) depth = (float)(bin + 2) / scale;
+                __syncthreads();
+                break;
+            }
+            __syncthreads();
+            if (k <= 0 || turn == 1) {
+                // fewer than k elements have any weight: all of them are gathered
+                if (k > 0 && bin == SA_BINS && all <= SA_CAP) depth = (float)SA_BINS / scale;
+                break;
+            }
+            scale = 16.0f;  // down to 32: no weight is left below 27.8
+            level = 2;
+        }
+    }
+    if (depth > 0.0f) {
+        // ---- gather, in the first CTA ----
+        for (int i = w0 + lane; i < w1; i += 32) {
+            const float l = z[i];
+            if ((lmax - l) * near < depth) s.own[atomicAdd(&s.n_own, 1)] = (uint16_t)i;
+        }
+        __syncthreads();
+        const int mine = s.n_own;
+        if (tid == 0 && mine > 0) s.base = atomicAdd(const_cast<int*>(peer(&s.n_cand, 0)), mine);
+        __syncthreads();
+        unsigned long long* to = const_cast<unsigned long long*>(peer(&s.cand[0], 0));
+        for (int e = tid; e < mine; e += SA_THREADS)
+            to[s.base + e] = (unsigned long long)__float_as_uint(z[s.own[e]]) << 32 | (uint32_t)(base + s.own[e]);
+        cluster_sync();
+        if (rank != 0) return;
+        // ---- order: larger z, then lower index ----
+        const int nc = s.n_cand, size = power_of_two(nc);
+        for (int e = tid; e < size; e += SA_THREADS) {
+            unsigned long long v = ~0ull;
+            if (e < nc) {
+                const unsigned long long x = s.cand[e];
+                v = (unsigned long long)~key_of(scaled(__uint_as_float((uint32_t)(x >> 32)))) << 32 | (uint32_t)x;
+            }
+            s.cand[e] = v;
+        }
+        block_sort(s.cand, size);
+        unsigned long long* weight = s.wt[0];
+        unsigned long long w[2] = {0, 0};
+        float e[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int r = 2 * tid + i;
+            if (r < nc) {
+                e[i] = exp_of(z_of(~(uint32_t)(s.cand[r] >> 32)), zmax);
+                w[i] = k > 0 && r >= k ? 0ull : weight_of(e[i]);
+                weight[r] = w[i];
+            }
+        }
+        unsigned long long among;
+        const unsigned long long incl = block_incl(w[0] + w[1], s.scan, &among);
+        const double limit = (double)p * (double)(k > 0 ? among : whole);
+        int stays = 0;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int r = 2 * tid + i;
+            const unsigned long long upto = i ? incl : incl - w[1], before = upto - w[i];
+            if (w[i] > 0 && (r == 0 || ((!(p < 1.0f) || (double)before < limit) && !(e[i] < minp)))) {
+                stays++;
+                atomicMax(&s.kept_sum, upto);
+            }
+        }
+        const int kept = block_count(stays, s.ties);
+        const unsigned long long total = s.kept_sum, target = target_of(total);
+        // ---- the draw, in index order ----
+        const int size2 = power_of_two(kept);
+        for (int i = 0; i < 2; i++) {  // (index, rank); both passes read cand before either writes: the ranks are a thread's own
+            const int r = 2 * tid + i;
+            if (r < size2) s.order[r] = r < kept ? (unsigned long long)(uint32_t)s.cand[r] << 32 | (uint32_t)r : ~0ull;
+        }
+        block_sort(s.order, size2);
+        int rk[2] = {0, 0};
+        w[0] = w[1] = 0;
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            if (2 * tid + i < kept) {
+                rk[i] = (int)(uint32_t)s.order[2 * tid + i];
+                w[i] = weight[rk[i]];
+            }
+        unsigned long long ignore;
+        const unsigned long long drawn = block_incl(w[0] + w[1], s.scan, &ignore);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const unsigned long long upto = i ? drawn : drawn - w[1];
+            if (w[i] > 0 && upto > target && upto - w[i] <= target) {
+                const unsigned long long x = s.cand[rk[i]];
+                a.token[row] = (int)(uint32_t)x;
+                if (a.logprob) a.logprob[row] = logprob_of(z_of(~(uint32_t)(x >> 32)), total);
+            }
+        }
+        return;
+    }
+
+    // ---- a long run, or none: z in place of the logits ----
+    for (int i = w0 + lane; i < w1; i += 32) z[i] = scaled(z[i]);
+    __syncthreads();
 
     // what stays: key > cut_key, or key == cut_key and index <= cut_idx
     uint32_t cut_key = 0;
     int cut_idx = -1;
-    uint32_t level = 0, lists = 0;
+    uint32_t lists = 0;
     auto kept = [&](uint32_t key, int idx) { return key > cut_key || (key == cut_key && idx <= cut_idx); };
 
     // Lowers the cut to the last element with less than `limit` before it (count or weight).
@@ -302,8 +574,7 @@ __global__ void __launch_bounds__(SA_THREADS) sample_rows(const SaArgs a) {
                 if (lane == 0) s.ties[warp] = mine;
                 cluster_sync();
                 // how many of them stay: before + i * w < limit for the i-th; w from the bin's total
-                const float zq = __uint_as_float(eq & 0x80000000u ? eq & 0x7fffffffu : ~eq);
-                const unsigned long long w = by_weight ? weight_of(exp_of(zq, zmax)) : 1ull;
+                const unsigned long long w = by_weight ? weight_of(exp_of(z_of(eq), zmax)) : 1ull;
                 uint32_t lo = 0, hi = in_bin - 1;  // the last i that stays
                 while (lo < hi) {
                     const uint32_t mid = (lo + hi + 1) / 2;
@@ -334,9 +605,8 @@ __global__ void __launch_bounds__(SA_THREADS) sample_rows(const SaArgs a) {
         }
     };
 
-    const bool empty = zmax == -INFINITY;
     if (!empty) {
-        if (k > 0 && k < a.n_vocab) select(false, (double)k);
+        if (k > 0) select(false, (double)k);
         if (p < 1.0f) select(true, (double)p);
     }
     // ---- the draw: kept weights in index order ----
@@ -344,46 +614,38 @@ __global__ void __launch_bounds__(SA_THREADS) sample_rows(const SaArgs a) {
         const float v = z[i];
         if (!kept(key_of(v), base + i)) return 0ull;
         const float e = exp_of(v, zmax);
-        return v == zmax || e >= minp ? weight_of(e) : 0ull;
+        return v == zmax || !(e < minp) ? weight_of(e) : 0ull;
     };
-    unsigned long long sum = 0;
-    if (!empty)
-        for (int i = w0 + lane; i < w1; i += 32) sum += weight_at(i);
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) s.sums[warp] = sum;
+    if (!empty && (k > 0 || p < 1.0f || minp > 0.0f)) {
+        run_sum = 0;
+        for (int i = r0; i < r1; i++) run_sum += weight_at(i);
+    }
+    unsigned long long sum;
+    const unsigned long long upto = block_incl(run_sum, s.scan, &sum);
+    if (tid == 0) s.kept_sum = sum;
     cluster_sync();
     unsigned long long total = 0, ahead = 0;
-    for (uint32_t r = 0; r < ctas; r++)
-        for (int q = 0; q < SA_WARPS; q++) {
-            const unsigned long long x = *peer(&s.sums[q], r);
-            if (r < rank || (r == rank && q < warp)) ahead += x;
-            total += x;
-        }
+    for (uint32_t r = 0; r < ctas; r++) {
+        const unsigned long long x = *peer(&s.kept_sum, r);
+        if (r < rank) ahead += x;
+        total += x;
+    }
     if (total == 0) {
         if (rank == 0 && tid == 0) {
             a.token[row] = -1;
             if (a.logprob) a.logprob[row] = -INFINITY;
         }
     } else {
-        const double ud = (double)a.u[row] * (double)total;
-        unsigned long long target = ud > 0.0 ? (unsigned long long)ud : 0ull;
-        if (target >= total) target = total - 1;  // u outside [0, 1)
-        if (target >= ahead && target < ahead + sum) {
-            for (int i = w0; i < w1; i += 32) {
-                const unsigned long long w = i + lane < w1 ? weight_at(i + lane) : 0ull;
-                const unsigned long long incl = ahead + warp_incl(w, lane);
-                const uint32_t over = __ballot_sync(0xffffffffu, incl > target);
-                if (over) {
-                    if (lane == __ffs(over) - 1) {
-                        a.token[row] = base + i + lane;
-                        if (a.logprob) {
-                            const float d = z[i + lane] == zmax ? 0.0f : z[i + lane] - zmax;
-                            a.logprob[row] = d - logf((float)((double)total / 1099511627776.0));
-                        }
-                    }
+        const unsigned long long target = target_of(total);
+        ahead += upto - run_sum;
+        if (target >= ahead && target < ahead + run_sum) {
+            for (int i = r0; i < r1; i++) {
+                ahead += weight_at(i);
+                if (ahead > target) {
+                    a.token[row] = base + i;
+                    if (a.logprob) a.logprob[row] = logprob_of(z[i], total);
                     break;
                 }
-                ahead = __shfl_sync(0xffffffffu, incl, 31);
             }
         }
     }
@@ -402,10 +664,10 @@ extern "C" int cfi_sample(const float* logits, long long row_stride, int n_rows,
         return (int)cudaErrorInvalidValue;
     if (n_rows == 0) return 0;
     if (n_rows > 0x7fffffff / SA_MAX_CTAS) return (int)cudaErrorInvalidValue;
-    SaArgs a = {logits, row_stride, temperature, top_p, min_p, u, top_k, token, logprob, n_vocab, 0};
+    SaArgs a = {logits, row_stride, temperature, top_p, min_p, u, top_k, token, logprob, n_vocab, 0, cfi_device_error_word()};
     unsigned ctas = SA_MAX_CTAS;
     a.slice = (int)(((n_vocab + ctas - 1) / ctas + 3) / 4 * 4);
-    const size_t smem = (size_t)a.slice * 4;
+    const size_t smem = (size_t)a.slice * 4 + 16;  // a row's slice keeps its place within 16 bytes
     static CfiPerDeviceOnce attr;
     cfi_once_per_device(attr, [] {
         cudaFuncSetAttribute(sample_rows, cudaFuncAttributeMaxDynamicSharedMemorySize, SA_MAX_SLICE * 4 + 64);
