@@ -21,6 +21,7 @@
 #include "sm100_ptx.cuh"
 #include "cfi_kernels.h"
 
+#include <algorithm>
 #include <stdlib.h>
 #include <string.h>
 
@@ -30,11 +31,11 @@ using namespace sm100;
 
 constexpr int SA_THREADS = 512, SA_WARPS = SA_THREADS / 32;
 constexpr int SA_BINS = SA_THREADS;   // a thread holds a bin's total
-constexpr int SA_LIST = 256;          // boundary-bin elements that are listed
-constexpr int SA_CAP = 1024;          // elements that the first CTA sorts (two a thread)
-constexpr int SA_MAX_CTAS = 8;
+constexpr int SA_LIST = 128;          // boundary-bin elements that are listed
+constexpr int SA_CAP = 2048, SA_EACH = SA_CAP / SA_THREADS;  // elements that the first CTA sorts, and a thread's of them
+constexpr int SA_CTAS = 8;            // of a cluster: the portable size, two CTAs to an SM at a vocabulary of 150,000
 constexpr int SA_MAX_SLICE = 50000;   // floats of a row that one CTA holds
-constexpr int SA_MAX_VOCAB = SA_MAX_CTAS * SA_MAX_SLICE;
+constexpr int SA_AHEAD = 8;           // loads of a pass that are in flight together
 
 struct SaArgs {
     const float* logits;
@@ -56,27 +57,22 @@ static_assert(SA_MAX_SLICE <= 65536, "a slice's indexes take 16 bits");
 
 struct SaShared {
     uint32_t cnt[2][SA_BINS];
-    unsigned long long wt[2][SA_BINS];  // in the end: the sorted elements' weights
-    union {
-        SaItem list[2][SA_LIST];           // long runs: the boundary bin's elements
-        unsigned long long order[SA_CAP];  // short runs: index and rank of the kept ones
-    };
-    unsigned long long cand[SA_CAP];    // gathered elements: logit's bits, index
-    uint16_t own[SA_CAP];               // this CTA's share of them
+    unsigned long long wt[2][SA_BINS];
+    SaItem list[2][SA_LIST];   // long runs: the boundary bin's elements
+    uint32_t cand[SA_CAP];     // short runs: the gathered elements' indexes
+    uint16_t own[SA_CAP];      // this CTA's share of them, from its slice's start
     uint64_t bar;
     unsigned long long scan[SA_WARPS];
     unsigned long long cta_sum, kept_sum;
     uint32_t ties[SA_WARPS];
     float wmax[SA_WARPS];
     float cta_max;
-    int n_list[2], n_own, n_cand, base;
-    int abort;
+    int n_list[2], n_own, n_cand, base, abort;
     int found_bin;
     unsigned long long found_before;
     uint32_t found_n, cut_key;
     int cut_idx;
 };
-static_assert(sizeof(unsigned long long) * 2 * SA_BINS >= sizeof(unsigned long long) * SA_CAP, "the weights take the histogram's place");
 
 // The same variable of CTA `rank` of the cluster.
 template <class T> CFI_DEV const T* peer(const T* p, uint32_t rank) {
@@ -174,9 +170,8 @@ CFI_DEV void block_sort(unsigned long long* v, int n) {
     for (int k = 2; k <= n; k <<= 1)
         for (int j = k >> 1; j > 0; j >>= 1) {
             __syncthreads();
-            const int t = threadIdx.x;
-            if (t < n / 2) {
-                const int i = (t / j) * 2 * j + t % j;  // j is a power of two
+            for (int t = threadIdx.x; t < n / 2; t += SA_THREADS) {
+                const int i = (t & -j) * 2 + (t & (j - 1));  // j is a power of two
                 const unsigned long long x = v[i], y = v[i + j];
                 if ((x > y) == ((i & k) == 0)) {
                     v[i] = y;
@@ -192,8 +187,8 @@ __global__ void __launch_bounds__(SA_THREADS) sample_rows(const SaArgs a) {
     extern __shared__ __align__(16) float slice[];
     __shared__ SaShared s;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t rank = cluster_ctarank(), ctas = cluster_nctarank();
-    const int row = blockIdx.x / ctas;
+    const uint32_t rank = cluster_ctarank();
+    const int row = blockIdx.x / SA_CTAS;
     const int base = rank * a.slice, n = max(0, min(a.slice, a.n_vocab - base));
     if (tid == 0) {
         mbar_init(&s.bar, 1);
@@ -243,9 +238,19 @@ __global__ void __launch_bounds__(SA_THREADS) sample_rows(const SaArgs a) {
     const int w0 = min(n, warp * chunk), w1 = min(n, w0 + chunk);
     const int run = ((n + SA_THREADS - 1) / SA_THREADS) | 1;  // each thread's run: odd, so that 32 of them meet no bank twice
     const int r0 = min(n, tid * run), r1 = min(n, r0 + run);
+    // f(i, z[i]) for this warp's run, or this thread's, SA_AHEAD loads at a time
+    auto walk = [&](int i0, int i1, int step, auto&& f) {
+        for (int i = i0; i < i1; i += step * SA_AHEAD) {
+            float v[SA_AHEAD];
+#pragma unroll
+            for (int e = 0; e < SA_AHEAD; e++) v[e] = i + step * e < i1 ? z[i + step * e] : -INFINITY;
+#pragma unroll
+            for (int e = 0; e < SA_AHEAD; e++)
+                if (i + step * e < i1) f(i + step * e, v[e]);
+        }
+    };
     float mx = -INFINITY;
-#pragma unroll 4
-    for (int i = tid; i < n; i += SA_THREADS) mx = fmaxf(mx, z[i]);  // a NaN is passed over
+    walk(w0 + lane, w1, 32, [&](int, float v) { mx = fmaxf(mx, v); });  // a NaN is passed over
     mx = warp_max(mx);
     if (lane == 0) s.wmax[warp] = mx;
     __syncthreads();
@@ -254,7 +259,7 @@ __global__ void __launch_bounds__(SA_THREADS) sample_rows(const SaArgs a) {
         if (lane == 0) s.cta_max = mx;
     }
     cluster_sync();
-    float lmax = lane < (int)ctas ? *peer(&s.cta_max, lane) : -INFINITY;
+    float lmax = lane < SA_CTAS ? *peer(&s.cta_max, lane) : -INFINITY;
     lmax = warp_max(lmax);
     const float zmax = scaled(lmax);  // division by a positive number keeps the order
     const bool empty = zmax == -INFINITY;
@@ -272,31 +277,33 @@ __global__ void __launch_bounds__(SA_THREADS) sample_rows(const SaArgs a) {
     unsigned long long run_sum = 0, whole = 0;
     const float near = 1.0f / div;
     const bool bins_hold = fabsf(zmax) < 8192.0f && near < 1e30f;  // z is exact to far less than a bin
-    if (!empty && k <= 0) {
-        const bool binned = p < 1.0f;
-        for (int i = r0; i < r1; i++) {
-            const float v = scaled(z[i]);
+    if (!empty && k <= 0 && bins_hold) {
+        const bool binned = p < 1.0f && bins_hold;
+        walk(r0, r1, 1, [&](int, float l) {
+            if (!((lmax - l) * near < 28.0f)) return;  // no weight (or a NaN)
+            const float v = scaled(l);
             const unsigned long long w = weight_of(exp_of(v, zmax));
             run_sum += w;
-            if (binned && bins_hold) {
-                const float d = (zmax - v) * 64.0f;
-                if (d < (float)SA_BINS) {
-                    atomicAdd(&s.cnt[0][(int)d], 1u);
-                    atomicAdd(&s.wt[0][(int)d], w);
-                }
+            const float d = (zmax - v) * 64.0f;
+            if (binned && d < (float)SA_BINS) {
+                atomicAdd(&s.cnt[0][(int)d], 1u);
+                atomicAdd(&s.wt[0][(int)d], w);
             }
-        }
+        });
         unsigned long long sum;
         block_incl(run_sum, s.scan, &sum);
         if (tid == 0) s.cta_sum = sum;
         cluster_sync();
-        for (uint32_t r = 0; r < ctas; r++) whole += *peer(&s.cta_sum, r);
+#pragma unroll
+        for (uint32_t r = 0; r < SA_CTAS; r++) whole += *peer(&s.cta_sum, r);
     }
     uint32_t level = 1;  // histogram 0 has been used
     // ---- a short run: down to which depth? ----
     float depth = -1.0f;  // gather what lies less deep (in units of z)
     if (!empty && bins_hold && (k > 0 || p < 1.0f)) {
-        float scale = 64.0f;
+        // bins down to a depth of 8, or 16 where more than a few are asked for; the second turn reaches 32, where no
+        // weight is left
+        float scale = k > 8 ? 32.0f : 64.0f;
         for (int turn = 0;; turn++) {
             const uint32_t b = turn & 1;
             if (k > 0) {
@@ -304,30 +311,31 @@ __global__ void __launch_bounds__(SA_THREADS) sample_rows(const SaArgs a) {
                     s.cnt[b][tid] = 0;
                     __syncthreads();
                 }
-                for (int i = w0 + lane; i < w1; i += 32) {
-                    const float d = (lmax - z[i]) * near * scale;  // a NaN compares false
+                walk(w0 + lane, w1, 32, [&](int, float l) {
+                    const float d = (lmax - l) * near * scale;  // a NaN compares false
                     if (d < (float)SA_BINS) atomicAdd(&s.cnt[b][(int)d], 1u);
-                }
+                });
                 cluster_sync();
             }
             uint32_t c = 0;
             unsigned long long m = 0;
-            for (uint32_t r = 0; r < ctas; r++) {
+#pragma unroll
+            for (uint32_t r = 0; r < SA_CTAS; r++) {
                 c += *peer(&s.cnt[b][tid], r);
                 if (k <= 0) m += *peer(&s.wt[b][tid], r);
             }
-            unsigned long long all;
-            // counts in the upper bits would not leave room for the weights: two sums where both are needed
-            const unsigned long long upto = block_incl(c, s.scan, &all);
-            bool reached = upto >= (unsigned long long)k;
-            if (k <= 0) {
-                unsigned long long ignore;
-                reached = !((double)block_incl(m, s.scan, &ignore) < (double)p * (double)whole);
-            }
             // the first bin whose end lies past the run's; with the next one, and one more for the rounding
+            unsigned long long all, ignore;
+            const unsigned long long upto = block_incl(c, s.scan, &all);
             if (tid == 0) s.found_bin = SA_BINS;
             __syncthreads();
-            if (reached) atomicMin(&s.found_bin, tid);
+            if (k > 0) {
+                if (upto >= (unsigned long long)k && upto - c < (unsigned long long)k) s.found_bin = tid;
+            } else {
+                const unsigned long long w = block_incl(m, s.scan, &ignore);
+                const double limit = (double)p * (double)whole;
+                if (!((double)w < limit) && (double)(w - m) < limit) s.found_bin = tid;
+            }
             __syncthreads();
             const int bin = s.found_bin;
             if (bin + 2 < SA_BINS) {
@@ -343,88 +351,94 @@ __global__ void __launch_bounds__(SA_THREADS) sample_rows(const SaArgs a) {
                 if (k > 0 && bin == SA_BINS && all <= SA_CAP) depth = (float)SA_BINS / scale;
                 break;
             }
-            scale = 16.0f;  // down to 32: no weight is left below 27.8
+            scale = 16.0f;
             level = 2;
         }
     }
     if (depth > 0.0f) {
         // ---- gather, in the first CTA ----
-        for (int i = w0 + lane; i < w1; i += 32) {
-            const float l = z[i];
+        walk(w0 + lane, w1, 32, [&](int i, float l) {
             if ((lmax - l) * near < depth) s.own[atomicAdd(&s.n_own, 1)] = (uint16_t)i;
-        }
+        });
         __syncthreads();
         const int mine = s.n_own;
         if (tid == 0 && mine > 0) s.base = atomicAdd(const_cast<int*>(peer(&s.n_cand, 0)), mine);
         __syncthreads();
-        unsigned long long* to = const_cast<unsigned long long*>(peer(&s.cand[0], 0));
-        for (int e = tid; e < mine; e += SA_THREADS)
-            to[s.base + e] = (unsigned long long)__float_as_uint(z[s.own[e]]) << 32 | (uint32_t)(base + s.own[e]);
+        uint32_t* to = const_cast<uint32_t*>(peer(&s.cand[0], 0));
+        for (int e = tid; e < mine; e += SA_THREADS) to[s.base + e] = (uint32_t)(base + s.own[e]);
         cluster_sync();
         if (rank != 0) return;
-        // ---- order: larger z, then lower index ----
+        // ---- order: larger z, then lower index.  The slice's place is free for what is sorted ----
+        unsigned long long *order = reinterpret_cast<unsigned long long*>(slice), *weight = order + SA_CAP;
         const int nc = s.n_cand, size = power_of_two(nc);
         for (int e = tid; e < size; e += SA_THREADS) {
             unsigned long long v = ~0ull;
             if (e < nc) {
-                const unsigned long long x = s.cand[e];
-                v = (unsigned long long)~key_of(scaled(__uint_as_float((uint32_t)(x >> 32)))) << 32 | (uint32_t)x;
+                const uint32_t i = s.cand[e];
+                v = (unsigned long long)~key_of(scaled(a.logits[row * a.stride + i])) << 32 | i;
             }
-            s.cand[e] = v;
+            order[e] = v;
         }
-        block_sort(s.cand, size);
-        unsigned long long* weight = s.wt[0];
-        unsigned long long w[2] = {0, 0};
-        float e[2] = {0.0f, 0.0f};
+        block_sort(order, size);
+        unsigned long long w[SA_EACH], part = 0;
+        float e[SA_EACH];
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const int r = 2 * tid + i;
+        for (int i = 0; i < SA_EACH; i++) {
+            const int r = SA_EACH * tid + i;
+            w[i] = 0;
+            e[i] = 0.0f;
             if (r < nc) {
-                e[i] = exp_of(z_of(~(uint32_t)(s.cand[r] >> 32)), zmax);
+                e[i] = exp_of(z_of(~(uint32_t)(order[r] >> 32)), zmax);
                 w[i] = k > 0 && r >= k ? 0ull : weight_of(e[i]);
                 weight[r] = w[i];
             }
+            part += w[i];
         }
         unsigned long long among;
-        const unsigned long long incl = block_incl(w[0] + w[1], s.scan, &among);
+        unsigned long long before = block_incl(part, s.scan, &among) - part;
         const double limit = (double)p * (double)(k > 0 ? among : whole);
         int stays = 0;
+        unsigned long long upto = 0;  // up to the last of this thread's that stays
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const int r = 2 * tid + i;
-            const unsigned long long upto = i ? incl : incl - w[1], before = upto - w[i];
-            if (w[i] > 0 && (r == 0 || ((!(p < 1.0f) || (double)before < limit) && !(e[i] < minp)))) {
+        for (int i = 0; i < SA_EACH; i++) {
+            if (w[i] > 0 && (tid + i == 0 || ((!(p < 1.0f) || (double)before < limit) && !(e[i] < minp)))) {
                 stays++;
-                atomicMax(&s.kept_sum, upto);
+                upto = before + w[i];
             }
+            before += w[i];
         }
         const int kept = block_count(stays, s.ties);
-        const unsigned long long total = s.kept_sum, target = target_of(total);
-        // ---- the draw, in index order ----
+        if (stays > 0 && SA_EACH * tid + stays == kept) s.kept_sum = upto;
+        // ---- the draw, in index order: index and rank are sorted again ----
+        uint32_t idx[SA_EACH];
         const int size2 = power_of_two(kept);
-        for (int i = 0; i < 2; i++) {  // (index, rank); both passes read cand before either writes: the ranks are a thread's own
-            const int r = 2 * tid + i;
-            if (r < size2) s.order[r] = r < kept ? (unsigned long long)(uint32_t)s.cand[r] << 32 | (uint32_t)r : ~0ull;
+#pragma unroll
+        for (int i = 0; i < SA_EACH; i++) idx[i] = SA_EACH * tid + i < kept ? (uint32_t)order[SA_EACH * tid + i] : ~0u;
+        unsigned long long* again = weight + SA_CAP;
+#pragma unroll
+        for (int i = 0; i < SA_EACH; i++)
+            if (SA_EACH * tid + i < size2) again[SA_EACH * tid + i] = (unsigned long long)idx[i] << 32 | (uint32_t)(SA_EACH * tid + i);
+        block_sort(again, size2);
+        const unsigned long long total = s.kept_sum, target = target_of(total);
+        int rk[SA_EACH];
+        part = 0;
+#pragma unroll
+        for (int i = 0; i < SA_EACH; i++) {
+            const int r = SA_EACH * tid + i;
+            rk[i] = r < kept ? (int)(uint32_t)again[r] : 0;
+            w[i] = r < kept ? weight[rk[i]] : 0ull;
+            part += w[i];
         }
-        block_sort(s.order, size2);
-        int rk[2] = {0, 0};
-        w[0] = w[1] = 0;
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-            if (2 * tid + i < kept) {
-                rk[i] = (int)(uint32_t)s.order[2 * tid + i];
-                w[i] = weight[rk[i]];
-            }
         unsigned long long ignore;
-        const unsigned long long drawn = block_incl(w[0] + w[1], s.scan, &ignore);
+        before = block_incl(part, s.scan, &ignore) - part;
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const unsigned long long upto = i ? drawn : drawn - w[1];
-            if (w[i] > 0 && upto > target && upto - w[i] <= target) {
-                const unsigned long long x = s.cand[rk[i]];
+        for (int i = 0; i < SA_EACH; i++) {
+            if (w[i] > 0 && before <= target && before + w[i] > target) {
+                const unsigned long long x = order[rk[i]];
                 a.token[row] = (int)(uint32_t)x;
                 if (a.logprob) a.logprob[row] = logprob_of(z_of(~(uint32_t)(x >> 32)), total);
             }
+            before += w[i];
         }
         return;
     }
@@ -462,7 +476,8 @@ __global__ void __launch_bounds__(SA_THREADS) sample_rows(const SaArgs a) {
             cluster_sync();
             uint32_t c = 0;
             unsigned long long m = 0;
-            for (uint32_t r = 0; r < ctas; r++) {
+#pragma unroll
+            for (uint32_t r = 0; r < SA_CTAS; r++) {
                 c += *peer(&s.cnt[b][tid], r);
                 if (by_weight) m += *peer(&s.wt[b][tid], r);
             }
@@ -519,7 +534,8 @@ __global__ void __launch_bounds__(SA_THREADS) sample_rows(const SaArgs a) {
                 SaItem me = {};
                 bool have = false;
                 int e = tid;
-                for (uint32_t r = 0; r < ctas; r++) {
+#pragma unroll
+                for (uint32_t r = 0; r < SA_CTAS; r++) {
                     const int nr = *peer(&s.n_list[lb], r);
                     if (!have && e < nr) {
                         me = *peer(&s.list[lb][e], r);
@@ -530,7 +546,8 @@ __global__ void __launch_bounds__(SA_THREADS) sample_rows(const SaArgs a) {
                 if (have) {
                     unsigned long long mine = before;
                     bool last = true;  // no element behind this one stays
-                    for (uint32_t r = 0; r < ctas; r++) {
+#pragma unroll
+                    for (uint32_t r = 0; r < SA_CTAS; r++) {
                         const int nr = *peer(&s.n_list[lb], r);
                         const SaItem* l = peer(&s.list[lb][0], r);
                         for (int j = 0; j < nr; j++) {
@@ -542,7 +559,7 @@ __global__ void __launch_bounds__(SA_THREADS) sample_rows(const SaArgs a) {
                     // the last of the bin has no other behind it, whatever the limit
                     if ((double)mine < limit && !last) {
                         bool behind = false;
-                        for (uint32_t r = 0; r < ctas && !behind; r++) {
+                        for (uint32_t r = 0; r < SA_CTAS && !behind; r++) {
                             const int nr = *peer(&s.n_list[lb], r);
                             const SaItem* l = peer(&s.list[lb][0], r);
                             for (int j = 0; j < nr && !behind; j++) {
@@ -584,7 +601,8 @@ __global__ void __launch_bounds__(SA_THREADS) sample_rows(const SaArgs a) {
                         hi = mid - 1;
                 }
                 uint32_t ahead = 0;
-                for (uint32_t r = 0; r < ctas; r++)
+#pragma unroll
+                for (uint32_t r = 0; r < SA_CTAS; r++)
                     for (int q = 0; q < SA_WARPS; q++)
                         if (r < rank || (r == rank && q < warp)) ahead += *peer(&s.ties[q], r);
                 if (lo >= ahead && lo < ahead + mine) {  // the warp that has it
@@ -592,7 +610,8 @@ __global__ void __launch_bounds__(SA_THREADS) sample_rows(const SaArgs a) {
                         const bool is = i + lane < w1 && key_of(z[i + lane]) == eq && kept(eq, base + i + lane);
                         const uint32_t bal = __ballot_sync(0xffffffffu, is);
                         if (is && ahead + __popc(bal & ((1u << lane) - 1)) == lo)
-                            for (uint32_t r = 0; r < ctas; r++) *const_cast<int*>(peer(&s.cut_idx, r)) = base + i + lane;
+#pragma unroll
+                            for (uint32_t r = 0; r < SA_CTAS; r++) *const_cast<int*>(peer(&s.cut_idx, r)) = base + i + lane;
                         ahead += __popc(bal);
                     }
                 }
@@ -616,7 +635,7 @@ __global__ void __launch_bounds__(SA_THREADS) sample_rows(const SaArgs a) {
         const float e = exp_of(v, zmax);
         return v == zmax || !(e < minp) ? weight_of(e) : 0ull;
     };
-    if (!empty && (k > 0 || p < 1.0f || minp > 0.0f)) {
+    if (!empty && (k > 0 || p < 1.0f || minp > 0.0f || !bins_hold)) {
         run_sum = 0;
         for (int i = r0; i < r1; i++) run_sum += weight_at(i);
     }
@@ -625,7 +644,8 @@ __global__ void __launch_bounds__(SA_THREADS) sample_rows(const SaArgs a) {
     if (tid == 0) s.kept_sum = sum;
     cluster_sync();
     unsigned long long total = 0, ahead = 0;
-    for (uint32_t r = 0; r < ctas; r++) {
+#pragma unroll
+    for (uint32_t r = 0; r < SA_CTAS; r++) {
         const unsigned long long x = *peer(&s.kept_sum, r);
         if (r < rank) ahead += x;
         total += x;
@@ -657,30 +677,30 @@ __global__ void __launch_bounds__(SA_THREADS) sample_rows(const SaArgs a) {
 extern "C" int cfi_sample(const float* logits, long long row_stride, int n_rows, int n_vocab, const float* temperature,
                           const int32_t* top_k, const float* top_p, const float* min_p, const float* u, int32_t* token,
                           float* logprob, void* stream) {
-    if (!logits || !u || !token || n_rows < 0 || n_vocab <= 0 || n_vocab > SA_MAX_VOCAB || row_stride < n_vocab ||
+    if (!logits || !u || !token || n_rows < 0 || n_vocab <= 0 || n_vocab > SA_CTAS * SA_MAX_SLICE || row_stride < n_vocab ||
         (((uintptr_t)logits | (uintptr_t)temperature | (uintptr_t)top_k | (uintptr_t)top_p | (uintptr_t)min_p | (uintptr_t)u |
           (uintptr_t)token | (uintptr_t)logprob) &
          3))
         return (int)cudaErrorInvalidValue;
     if (n_rows == 0) return 0;
-    if (n_rows > 0x7fffffff / SA_MAX_CTAS) return (int)cudaErrorInvalidValue;
+    if (n_rows > 0x7fffffff / SA_CTAS) return (int)cudaErrorInvalidValue;
     SaArgs a = {logits, row_stride, temperature, top_p, min_p, u, top_k, token, logprob, n_vocab, 0, cfi_device_error_word()};
-    unsigned ctas = SA_MAX_CTAS;
-    a.slice = (int)(((n_vocab + ctas - 1) / ctas + 3) / 4 * 4);
-    const size_t smem = (size_t)a.slice * 4 + 16;  // a row's slice keeps its place within 16 bytes
+    a.slice = (int)(((n_vocab + SA_CTAS - 1) / SA_CTAS + 3) / 4 * 4);
+    // a row's slice keeps its place within 16 bytes; three arrays of SA_CAP numbers take its place later
+    const size_t smem = std::max((size_t)a.slice * 4 + 16, (size_t)SA_CAP * 3 * 8);
     static CfiPerDeviceOnce attr;
     cfi_once_per_device(attr, [] {
         cudaFuncSetAttribute(sample_rows, cudaFuncAttributeMaxDynamicSharedMemorySize, SA_MAX_SLICE * 4 + 64);
     });
     const char* ep = getenv("CFI_PDL");
     cudaLaunchConfig_t lc = {};
-    lc.gridDim = dim3((unsigned)n_rows * ctas, 1, 1);
+    lc.gridDim = dim3((unsigned)n_rows * SA_CTAS, 1, 1);
     lc.blockDim = dim3(SA_THREADS, 1, 1);
     lc.dynamicSmemBytes = smem;
     lc.stream = static_cast<cudaStream_t>(stream);
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = ctas;
+    at[0].val.clusterDim.x = SA_CTAS;
     at[0].val.clusterDim.y = 1;
     at[0].val.clusterDim.z = 1;
     at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
