@@ -9,11 +9,11 @@
 // All three filters keep a run from the top of the order (larger z first, then lower index).  Where that run
 // is short -- it is, when a top-k or a nucleus of a language model's logits is asked for -- the bins of a
 // histogram of max - z say down to which depth it can reach, the few elements above that depth are gathered in
-// the cluster's first CTA, and that CTA sorts them and finishes alone.  The gathering needs no exact z: bins
+// the cluster's first CTA, and that CTA finishes alone with them in registers.  The gathering needs no exact z: bins
 // of (max logit - logit) / T are 1/64 wide, far above the rounding of z, and one bin more is taken.
 //
-// Where it is long (more than SA_CAP elements) each filter is a cut, the last element that stays, found
-// without sorting: a histogram over 512 bins finds the bin that the cut falls in; the at most SA_LIST
+// Each filter is a cut, the last element that stays, found
+// without sorting, in one CTA or in the whole cluster (more than SA_CAP elements): a histogram over 512 bins finds the bin that the cut falls in; the at most SA_LIST
 // elements of that bin are listed and each one's rank is counted against the others.  A fuller bin is divided
 // again: first by the next bits of max - z, then by the bits of z itself, after which all that is left is
 // equal and the index decides.
@@ -21,9 +21,9 @@
 #include "sm100_ptx.cuh"
 #include "cfi_kernels.h"
 
-#include <algorithm>
 #include <stdlib.h>
 #include <string.h>
+#include <type_traits>
 
 namespace {
 
@@ -53,21 +53,19 @@ struct SaItem {
     int idx;
     unsigned long long w;
 };
-static_assert(SA_MAX_SLICE <= 65536, "a slice's indexes take 16 bits");
+static_assert((SA_MAX_SLICE / SA_THREADS | 1) + 1 <= 128, "a thread's run is a mask of 128 bits");
 
 struct SaShared {
     uint32_t cnt[2][SA_BINS];
     unsigned long long wt[2][SA_BINS];
-    SaItem list[2][SA_LIST];   // long runs: the boundary bin's elements
-    uint32_t cand[SA_CAP];     // short runs: the gathered elements' indexes
-    uint16_t own[SA_CAP];      // this CTA's share of them, from its slice's start
+    SaItem list[2][SA_LIST];   // the boundary bin's elements: this CTA's, and all
+    uint32_t cand[SA_CAP];     // a short run's elements: their indexes, rising
     uint64_t bar;
     unsigned long long scan[SA_WARPS];
     unsigned long long cta_sum, kept_sum;
-    uint32_t ties[SA_WARPS];
     float wmax[SA_WARPS];
     float cta_max;
-    int n_list[2], n_own, n_cand, base, abort;
+    int n_list, n_own, n_ties, abort;
     int found_bin;
     unsigned long long found_before;
     uint32_t found_n, cut_key;
@@ -153,37 +151,7 @@ CFI_DEV unsigned long long block_incl(unsigned long long v, unsigned long long* 
     return incl + prev;
 }
 
-// The sum of v over the block (ties: a word for each warp).
-CFI_DEV int block_count(int v, uint32_t* words) {
-    v = __reduce_add_sync(0xffffffffu, v);
-    if ((threadIdx.x & 31) == 0) words[threadIdx.x >> 5] = (uint32_t)v;
-    __syncthreads();
-    int n = 0;
-#pragma unroll
-    for (int w = 0; w < SA_WARPS; w++) n += (int)words[w];
-    __syncthreads();
-    return n;
-}
-
-// Sorts n (a power of two, at most SA_CAP) numbers in rising order.
-CFI_DEV void block_sort(unsigned long long* v, int n) {
-    for (int k = 2; k <= n; k <<= 1)
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            __syncthreads();
-            for (int t = threadIdx.x; t < n / 2; t += SA_THREADS) {
-                const int i = (t & -j) * 2 + (t & (j - 1));  // j is a power of two
-                const unsigned long long x = v[i], y = v[i + j];
-                if ((x > y) == ((i & k) == 0)) {
-                    v[i] = y;
-                    v[i + j] = x;
-                }
-            }
-        }
-    __syncthreads();
-}
-CFI_DEV int power_of_two(int n) { return n <= 2 ? 2 : 1 << (32 - __clz(n - 1)); }
-
-__global__ void __launch_bounds__(SA_THREADS) sample_rows(const SaArgs a) {
+__global__ void __launch_bounds__(SA_THREADS, 2) sample_rows(const SaArgs a) {
     extern __shared__ __align__(16) float slice[];
     __shared__ SaShared s;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -192,8 +160,7 @@ __global__ void __launch_bounds__(SA_THREADS) sample_rows(const SaArgs a) {
     const int base = rank * a.slice, n = max(0, min(a.slice, a.n_vocab - base));
     if (tid == 0) {
         mbar_init(&s.bar, 1);
-        s.abort = s.n_own = s.n_cand = 0;
-        s.kept_sum = 0;
+        s.abort = 0;
         fence_mbar_init();
     }
     for (int b = tid; b < SA_BINS; b += SA_THREADS) {
@@ -263,15 +230,6 @@ __global__ void __launch_bounds__(SA_THREADS) sample_rows(const SaArgs a) {
     lmax = warp_max(lmax);
     const float zmax = scaled(lmax);  // division by a positive number keeps the order
     const bool empty = zmax == -INFINITY;
-
-    auto logprob_of = [&](float v, unsigned long long total) {
-        return (v == zmax ? 0.0f : v - zmax) - logf((float)((double)total / SA_UNIT));
-    };
-    auto target_of = [&](unsigned long long total) {
-        const double ud = (double)a.u[row] * (double)total;
-        const unsigned long long target = ud > 0.0 ? (unsigned long long)ud : 0ull;
-        return target < total ? target : total - 1;  // u outside [0, 1)
-    };
 
     // ---- no top-k: every weight counts.  Each thread sums its run; with a top-p, the top of the order by bins ----
     unsigned long long run_sum = 0, whole = 0;
@@ -355,242 +313,131 @@ __global__ void __launch_bounds__(SA_THREADS) sample_rows(const SaArgs a) {
             level = 2;
         }
     }
-    if (depth > 0.0f) {
-        // ---- gather, in the first CTA ----
-        walk(w0 + lane, w1, 32, [&](int i, float l) {
-            if ((lmax - l) * near < depth) s.own[atomicAdd(&s.n_own, 1)] = (uint16_t)i;
-        });
-        __syncthreads();
-        const int mine = s.n_own;
-        if (tid == 0 && mine > 0) s.base = atomicAdd(const_cast<int*>(peer(&s.n_cand, 0)), mine);
-        __syncthreads();
-        uint32_t* to = const_cast<uint32_t*>(peer(&s.cand[0], 0));
-        for (int e = tid; e < mine; e += SA_THREADS) to[s.base + e] = (uint32_t)(base + s.own[e]);
-        cluster_sync();
-        if (rank != 0) return;
-        // ---- order: larger z, then lower index.  The slice's place is free for what is sorted ----
-        unsigned long long *order = reinterpret_cast<unsigned long long*>(slice), *weight = order + SA_CAP;
-        const int nc = s.n_cand, size = power_of_two(nc);
-        for (int e = tid; e < size; e += SA_THREADS) {
-            unsigned long long v = ~0ull;
-            if (e < nc) {
-                const uint32_t i = s.cand[e];
-                v = (unsigned long long)~key_of(scaled(a.logits[row * a.stride + i])) << 32 | i;
-            }
-            order[e] = v;
-        }
-        block_sort(order, size);
-        unsigned long long w[SA_EACH], part = 0;
-        float e[SA_EACH];
-#pragma unroll
-        for (int i = 0; i < SA_EACH; i++) {
-            const int r = SA_EACH * tid + i;
-            w[i] = 0;
-            e[i] = 0.0f;
-            if (r < nc) {
-                e[i] = exp_of(z_of(~(uint32_t)(order[r] >> 32)), zmax);
-                w[i] = k > 0 && r >= k ? 0ull : weight_of(e[i]);
-                weight[r] = w[i];
-            }
-            part += w[i];
-        }
-        unsigned long long among;
-        unsigned long long before = block_incl(part, s.scan, &among) - part;
-        const double limit = (double)p * (double)(k > 0 ? among : whole);
-        int stays = 0;
-        unsigned long long upto = 0;  // up to the last of this thread's that stays
-#pragma unroll
-        for (int i = 0; i < SA_EACH; i++) {
-            if (w[i] > 0 && (tid + i == 0 || ((!(p < 1.0f) || (double)before < limit) && !(e[i] < minp)))) {
-                stays++;
-                upto = before + w[i];
-            }
-            before += w[i];
-        }
-        const int kept = block_count(stays, s.ties);
-        if (stays > 0 && SA_EACH * tid + stays == kept) s.kept_sum = upto;
-        // ---- the draw, in index order: index and rank are sorted again ----
-        uint32_t idx[SA_EACH];
-        const int size2 = power_of_two(kept);
-#pragma unroll
-        for (int i = 0; i < SA_EACH; i++) idx[i] = SA_EACH * tid + i < kept ? (uint32_t)order[SA_EACH * tid + i] : ~0u;
-        unsigned long long* again = weight + SA_CAP;
-#pragma unroll
-        for (int i = 0; i < SA_EACH; i++)
-            if (SA_EACH * tid + i < size2) again[SA_EACH * tid + i] = (unsigned long long)idx[i] << 32 | (uint32_t)(SA_EACH * tid + i);
-        block_sort(again, size2);
-        const unsigned long long total = s.kept_sum, target = target_of(total);
-        int rk[SA_EACH];
-        part = 0;
-#pragma unroll
-        for (int i = 0; i < SA_EACH; i++) {
-            const int r = SA_EACH * tid + i;
-            rk[i] = r < kept ? (int)(uint32_t)again[r] : 0;
-            w[i] = r < kept ? weight[rk[i]] : 0ull;
-            part += w[i];
-        }
-        unsigned long long ignore;
-        before = block_incl(part, s.scan, &ignore) - part;
-#pragma unroll
-        for (int i = 0; i < SA_EACH; i++) {
-            if (w[i] > 0 && before <= target && before + w[i] > target) {
-                const unsigned long long x = order[rk[i]];
-                a.token[row] = (int)(uint32_t)x;
-                if (a.logprob) a.logprob[row] = logprob_of(z_of(~(uint32_t)(x >> 32)), total);
-            }
-            before += w[i];
-        }
-        return;
-    }
 
-    // ---- a long run, or none: z in place of the logits ----
-    for (int i = w0 + lane; i < w1; i += 32) z[i] = scaled(z[i]);
-    __syncthreads();
-
-    // what stays: key > cut_key, or key == cut_key and index <= cut_idx
+    // ---- cuts.  What stays: key > cut_key, or key == cut_key and index <= cut_idx ----
     uint32_t cut_key = 0;
     int cut_idx = -1;
-    uint32_t lists = 0;
     auto kept = [&](uint32_t key, int idx) { return key > cut_key || (key == cut_key && idx <= cut_idx); };
-
-    // Lowers the cut to the last element with less than `limit` before it (count or weight).
-    auto select = [&](bool by_weight, double limit_in) {
+    // Lowers the cut to the last element with less than `limit` before it: a count, or a share of the weight.
+    // `each` calls its argument with z and index of this thread's elements, threads and elements in index order.
+    // ALONE: the elements are this CTA's, at most `count`; else the whole cluster's.
+    auto select = [&](auto alone, auto&& each, int count, bool by_weight, double limit, unsigned long long all_weight) {
+        constexpr bool ALONE = decltype(alone)::value;
+        constexpr uint32_t PEERS = ALONE ? 1 : SA_CTAS;
+        auto meet = [] {
+            if (ALONE) __syncthreads(); else cluster_sync();
+        };
+        auto of = [](auto* v, uint32_t r) { return ALONE ? (const std::remove_pointer_t<decltype(v)>*)v : peer(v, r); };
         SaPrefix pre;
-        double limit = limit_in;
         unsigned long long before = 0;
+        uint32_t in_bin = (uint32_t)count;
+        if (by_weight && all_weight > 0) limit *= (double)all_weight;
+        bool scaled_limit = !by_weight || all_weight > 0;
         for (;;) {
-            const uint32_t b = level++ & 1;
-            s.cnt[b][tid] = 0;
-            s.wt[b][tid] = 0;
-            __syncthreads();
-            for (int i = w0 + lane; i < w1; i += 32) {
-                const float v = z[i];
-                const uint32_t key = key_of(v);
-                uint32_t bin;
-                if (!kept(key, base + i) || !pre.digit(depth_of(v, zmax), key, &bin)) continue;
-                const unsigned long long w = weight_of(exp_of(v, zmax));
-                if (w == 0) continue;
-                atomicAdd(&s.cnt[b][bin], 1u);
-                if (by_weight) atomicAdd(&s.wt[b][bin], w);
-            }
-            cluster_sync();
-            uint32_t c = 0;
-            unsigned long long m = 0;
-#pragma unroll
-            for (uint32_t r = 0; r < SA_CTAS; r++) {
-                c += *peer(&s.cnt[b][tid], r);
-                if (by_weight) m += *peer(&s.wt[b][tid], r);
-            }
-            if (!by_weight) m = c;
-            unsigned long long incl = warp_incl(m, lane);
-            if (lane == 31) s.scan[warp] = incl;
-            __syncthreads();
-            unsigned long long prev = 0, total = 0;
-            for (int w = 0; w < SA_WARPS; w++) {
-                const unsigned long long x = s.scan[w];
-                if (w < warp) prev += x;
-                total += x;
-            }
-            if (pre.stage == 0) {
-                if (by_weight)
-                    limit = limit_in * (double)total;
-                else if (total <= (unsigned long long)limit_in) {
-                    __syncthreads();
-                    return;  // nothing to cut
-                }
-                if (!(limit > 0.0)) limit = 0.5;  // the largest always stays
-            }
-            incl += prev + before;
-            // the bin of the cut: the last that has less than the limit before it (a later one has weight)
-            if (tid == 0) s.found_bin = -1;
-            __syncthreads();
-            if (m > 0 && (double)(incl - m) < limit) atomicMax(&s.found_bin, tid);
-            __syncthreads();
-            if (tid == s.found_bin) {
-                s.found_before = incl - m;
-                s.found_n = c;
-            }
-            __syncthreads();
-            const int bin = s.found_bin;
-            before = s.found_before;
-            const uint32_t in_bin = s.found_n;
-            if (bin < 0) return;  // no element has weight: a row of -inf
-            pre.take((uint32_t)bin);
-            if (in_bin <= SA_LIST) {
-                const uint32_t lb = lists++ & 1;
-                if (tid == 0) s.n_list[lb] = 0;
+            if (!ALONE || in_bin > SA_LIST) {
+                const uint32_t b = level++ & 1;
+                s.cnt[b][tid] = 0;
+                s.wt[b][tid] = 0;
+                if (tid == 0) s.found_bin = -1;
                 __syncthreads();
-                for (int i = w0 + lane; i < w1; i += 32) {
-                    const float v = z[i];
+                each([&](float v, int idx) {
                     const uint32_t key = key_of(v);
-                    if (!kept(key, base + i) || !pre.holds(depth_of(v, zmax), key)) continue;
+                    uint32_t bin;
+                    if (!kept(key, idx) || !pre.digit(depth_of(v, zmax), key, &bin)) return;
                     const unsigned long long w = weight_of(exp_of(v, zmax));
-                    if (w == 0) continue;
-                    const int at = atomicAdd(&s.n_list[lb], 1);
-                    s.list[lb][at] = SaItem{key, base + i, by_weight ? w : 1ull};
+                    if (w == 0) return;
+                    atomicAdd(&s.cnt[b][bin], 1u);
+                    if (by_weight) atomicAdd(&s.wt[b][bin], w);
+                });
+                meet();
+                uint32_t c = 0;
+                unsigned long long m = 0;
+#pragma unroll
+                for (uint32_t r = 0; r < PEERS; r++) {
+                    c += *of(&s.cnt[b][tid], r);
+                    if (by_weight) m += *of(&s.wt[b][tid], r);
                 }
-                cluster_sync();
-                // every CTA ranks every element: thread e's is the e-th of the lists one behind another
+                if (!by_weight) m = c;
+                unsigned long long total;
+                const unsigned long long incl = block_incl(m, s.scan, &total) + before;
+                if (pre.stage == 0) {
+                    if (!scaled_limit) limit *= (double)total;
+                    if (!by_weight && total <= (unsigned long long)limit) return;  // nothing to cut
+                    if (!(limit > 0.0)) limit = 0.5;                               // the largest always stays
+                }
+                // the bin of the cut: the last that has less than the limit before it (a later one has weight)
+                if (m > 0 && (double)(incl - m) < limit) atomicMax(&s.found_bin, tid);
+                __syncthreads();
+                if (tid == s.found_bin) {
+                    s.found_before = incl - m;
+                    s.found_n = c;
+                }
+                __syncthreads();
+                pre.take((uint32_t)s.found_bin);
+                before = s.found_before;
+                in_bin = s.found_n;
+            } else if (pre.stage == 0) {
+                if (!(limit > 0.0)) limit = 0.5;
+            }
+            if (in_bin <= SA_LIST) {
+                if (tid == 0) s.n_list = 0;
+                __syncthreads();
+                each([&](float v, int idx) {
+                    const uint32_t key = key_of(v);
+                    if (!kept(key, idx) || !pre.holds(depth_of(v, zmax), key)) return;
+                    const unsigned long long w = weight_of(exp_of(v, zmax));
+                    if (w != 0) s.list[0][atomicAdd(&s.n_list, 1)] = SaItem{key, idx, by_weight ? w : 1ull};
+                });
+                meet();
+                int n_all = 0;
+#pragma unroll
+                for (uint32_t r = 0; r < PEERS; r++) {
+                    const int nr = *of(&s.n_list, r);
+                    for (int e = tid; e < nr; e += SA_THREADS) s.list[1][n_all + e] = *of(&s.list[0][e], r);
+                    n_all += nr;
+                }
+                __syncthreads();
+                // four threads rank an element: what is before it, and whether one is behind it
+                const int e = tid / 4;
+                const bool have = e < n_all;
+                unsigned long long mine = 0;
+                int behind = 0;
                 SaItem me = {};
-                bool have = false;
-                int e = tid;
-#pragma unroll
-                for (uint32_t r = 0; r < SA_CTAS; r++) {
-                    const int nr = *peer(&s.n_list[lb], r);
-                    if (!have && e < nr) {
-                        me = *peer(&s.list[lb][e], r);
-                        have = true;
-                    }
-                    if (!have) e -= nr;
-                }
                 if (have) {
-                    unsigned long long mine = before;
-                    bool last = true;  // no element behind this one stays
+                    me = s.list[1][e];
+                    for (int j = tid & 3; j < n_all; j += 4) {
+                        const SaItem o = s.list[1][j];
+                        if (o.key > me.key || (o.key == me.key && o.idx < me.idx)) mine += o.w;
+                        if (o.key < me.key || (o.key == me.key && o.idx > me.idx)) behind = 1;
+                    }
+                }
 #pragma unroll
-                    for (uint32_t r = 0; r < SA_CTAS; r++) {
-                        const int nr = *peer(&s.n_list[lb], r);
-                        const SaItem* l = peer(&s.list[lb][0], r);
-                        for (int j = 0; j < nr; j++) {
-                            const SaItem o = l[j];
-                            if (o.key > me.key || (o.key == me.key && o.idx < me.idx)) mine += o.w;
-                        }
-                    }
-                    last = (double)mine < limit && !((double)(mine + me.w) < limit);
-                    // the last of the bin has no other behind it, whatever the limit
-                    if ((double)mine < limit && !last) {
-                        bool behind = false;
-                        for (uint32_t r = 0; r < SA_CTAS && !behind; r++) {
-                            const int nr = *peer(&s.n_list[lb], r);
-                            const SaItem* l = peer(&s.list[lb][0], r);
-                            for (int j = 0; j < nr && !behind; j++) {
-                                const SaItem o = l[j];
-                                behind = o.key < me.key || (o.key == me.key && o.idx > me.idx);
-                            }
-                        }
-                        last = !behind;
-                    }
-                    if (last) {
-                        s.cut_key = me.key;
-                        s.cut_idx = me.idx;
-                    }
+                for (int x = 1; x < 4; x <<= 1) {
+                    mine += __shfl_xor_sync(0xffffffffu, mine, x);
+                    behind |= __shfl_xor_sync(0xffffffffu, behind, x);
+                }
+                mine += before;
+                // the last that stays: the one behind it has the limit before it, or there is none
+                if (have && (double)mine < limit && (!behind || !((double)(mine + me.w) < limit))) {
+                    s.cut_key = me.key;
+                    s.cut_idx = me.idx;
                 }
                 __syncthreads();
                 cut_key = s.cut_key;
                 cut_idx = s.cut_idx;
-                __syncthreads();
                 return;
             }
             if (pre.stage == 7) {  // equal elements: each has the same weight, the index decides
                 const uint32_t eq = ~pre.key;
-                uint32_t mine = 0;
-                for (int i = w0 + lane; i < w1; i += 32) {
-                    const uint32_t key = key_of(z[i]);
-                    mine += (uint32_t)(key == eq && kept(key, base + i));
-                }
-                for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-                if (lane == 0) s.ties[warp] = mine;
-                cluster_sync();
-                // how many of them stay: before + i * w < limit for the i-th; w from the bin's total
+                unsigned long long mine = 0, ties;
+                each([&](float v, int idx) { mine += (unsigned long long)(key_of(v) == eq && kept(eq, idx)); });
+                unsigned long long ahead = block_incl(mine, s.scan, &ties) - mine;
+                if (tid == 0) s.n_ties = (int)ties;
+                meet();
+#pragma unroll
+                for (uint32_t r = 0; r < PEERS; r++)
+                    if (!ALONE && r < rank) ahead += (unsigned long long)*of(&s.n_ties, r);
+                // how many of them stay: before + i * w < limit for the i-th
                 const unsigned long long w = by_weight ? weight_of(exp_of(z_of(eq), zmax)) : 1ull;
                 uint32_t lo = 0, hi = in_bin - 1;  // the last i that stays
                 while (lo < hi) {
@@ -600,44 +447,114 @@ __global__ void __launch_bounds__(SA_THREADS) sample_rows(const SaArgs a) {
                     else
                         hi = mid - 1;
                 }
-                uint32_t ahead = 0;
-#pragma unroll
-                for (uint32_t r = 0; r < SA_CTAS; r++)
-                    for (int q = 0; q < SA_WARPS; q++)
-                        if (r < rank || (r == rank && q < warp)) ahead += *peer(&s.ties[q], r);
-                if (lo >= ahead && lo < ahead + mine) {  // the warp that has it
-                    for (int i = w0; i < w1; i += 32) {
-                        const bool is = i + lane < w1 && key_of(z[i + lane]) == eq && kept(eq, base + i + lane);
-                        const uint32_t bal = __ballot_sync(0xffffffffu, is);
-                        if (is && ahead + __popc(bal & ((1u << lane) - 1)) == lo)
-#pragma unroll
-                            for (uint32_t r = 0; r < SA_CTAS; r++) *const_cast<int*>(peer(&s.cut_idx, r)) = base + i + lane;
-                        ahead += __popc(bal);
-                    }
-                }
-                cluster_sync();
+                if (lo >= ahead && lo < ahead + mine)
+                    each([&](float v, int idx) {
+                        if (key_of(v) != eq || !kept(eq, idx)) return;
+                        if (ahead++ == lo)
+                            for (uint32_t r = 0; r < PEERS; r++) *const_cast<int*>(of(&s.cut_idx, r)) = idx;
+                    });
+                meet();
                 cut_key = eq;
                 cut_idx = s.cut_idx;
-                __syncthreads();
                 return;
             }
         }
     };
-
-    if (!empty) {
-        if (k > 0) select(false, (double)k);
-        if (p < 1.0f) select(true, (double)p);
-    }
-    // ---- the draw: kept weights in index order ----
-    auto weight_at = [&](int i) -> unsigned long long {
-        const float v = z[i];
-        if (!kept(key_of(v), base + i)) return 0ull;
-        const float e = exp_of(v, zmax);
-        return v == zmax || !(e < minp) ? weight_of(e) : 0ull;
+    // The draw: kept weights in index order.  `ahead`: what the CTAs before this one have.
+    auto draw = [&](auto&& each, unsigned long long own, unsigned long long ahead, unsigned long long total) {
+        const double ud = (double)a.u[row] * (double)total;
+        unsigned long long target = ud > 0.0 ? (unsigned long long)ud : 0ull;
+        if (target >= total) target = total - 1;  // u outside [0, 1)
+        if (target < ahead || target >= ahead + own) return;
+        each([&](float v, int idx) {
+            if (!kept(key_of(v), idx)) return;
+            const float e = exp_of(v, zmax);
+            if (v != zmax && e < minp) return;
+            const unsigned long long w = weight_of(e);
+            if (ahead <= target && ahead + w > target) {
+                a.token[row] = idx;
+                if (a.logprob) a.logprob[row] = (v == zmax ? 0.0f : v - zmax) - logf((float)((double)total / SA_UNIT));
+            }
+            ahead += w;
+        });
     };
-    if (!empty && (k > 0 || p < 1.0f || minp > 0.0f || !bins_hold)) {
-        run_sum = 0;
-        for (int i = r0; i < r1; i++) run_sum += weight_at(i);
+    auto weight_of_kept = [&](auto&& each) {
+        unsigned long long sum = 0;
+        each([&](float v, int idx) {
+            if (!kept(key_of(v), idx)) return;
+            const float e = exp_of(v, zmax);
+            if (v == zmax || !(e < minp)) sum += weight_of(e);
+        });
+        return sum;
+    };
+
+    if (depth > 0.0f) {
+        // ---- a short run: gathered in index order by the first CTA, which goes on alone ----
+        unsigned long long hit[2] = {0, 0};
+        walk(r0, r1, 1, [&](int i, float l) {
+            if ((lmax - l) * near < depth) {
+                if (i - r0 < 64) hit[0] |= 1ull << (i - r0); else hit[1] |= 1ull << (i - r0 - 64);
+            }
+        });
+        const int mine = __popcll(hit[0]) + __popcll(hit[1]);
+        unsigned long long own;
+        int at = (int)block_incl((unsigned long long)mine, s.scan, &own) - mine;
+        if (tid == 0) s.n_own = (int)own;
+        cluster_sync();
+        int nc = 0;
+#pragma unroll
+        for (uint32_t r = 0; r < SA_CTAS; r++) {
+            const int x = *peer(&s.n_own, r);
+            if (r < rank) at += x;
+            nc += x;
+        }
+        uint32_t* to = const_cast<uint32_t*>(peer(&s.cand[0], 0));
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+            for (unsigned long long h = hit[x]; h; h &= h - 1) to[at++] = (uint32_t)(base + r0 + 64 * x + __ffsll((long long)h) - 1);
+        cluster_sync();
+        if (rank != 0) return;
+        float v[SA_EACH];
+        int idx[SA_EACH];
+        const int each_n = (nc + SA_THREADS - 1) / SA_THREADS;  // a thread's elements, in index order
+#pragma unroll
+        for (int e = 0; e < SA_EACH; e++) {
+            const int x = tid * each_n + e;
+            idx[e] = e < each_n && x < nc ? (int)s.cand[x] : -1;
+            v[e] = idx[e] >= 0 ? scaled(a.logits[row * a.stride + idx[e]]) : -INFINITY;
+        }
+        auto each = [&](auto&& f) {
+#pragma unroll
+            for (int e = 0; e < SA_EACH; e++)
+                if (idx[e] >= 0) f(v[e], idx[e]);
+        };
+        if (k > 0 && k < nc) select(std::true_type{}, each, nc, false, (double)k, 0ull);
+        if (p < 1.0f) {
+            unsigned long long among = whole;
+            if (k > 0) {
+                unsigned long long sum = 0;
+                each([&](float x, int i) {
+                    if (kept(key_of(x), i)) sum += weight_of(exp_of(x, zmax));
+                });
+                block_incl(sum, s.scan, &among);
+            }
+            select(std::true_type{}, each, nc, true, (double)p, among);
+        }
+        const unsigned long long sum = weight_of_kept(each);
+        unsigned long long total;
+        const unsigned long long upto = block_incl(sum, s.scan, &total);
+        draw(each, sum, upto - sum, total);
+        return;
+    }
+
+    // ---- a long run, or no filter: z in place of the logits ----
+    for (int i = w0 + lane; i < w1; i += 32) z[i] = scaled(z[i]);
+    __syncthreads();
+    auto each = [&](auto&& f) { walk(r0, r1, 1, [&](int i, float v) { f(v, base + i); }); };
+    if (!empty) {
+        if (k > 0) select(std::false_type{}, each, a.n_vocab, false, (double)k, 0ull);
+        if (p < 1.0f) select(std::false_type{}, each, a.n_vocab, true, (double)p, 0ull);
+        if (k > 0 || p < 1.0f || minp > 0.0f || !bins_hold) run_sum = weight_of_kept(each);
     }
     unsigned long long sum;
     const unsigned long long upto = block_incl(run_sum, s.scan, &sum);
@@ -650,24 +567,11 @@ __global__ void __launch_bounds__(SA_THREADS) sample_rows(const SaArgs a) {
         if (r < rank) ahead += x;
         total += x;
     }
-    if (total == 0) {
-        if (rank == 0 && tid == 0) {
-            a.token[row] = -1;
-            if (a.logprob) a.logprob[row] = -INFINITY;
-        }
-    } else {
-        const unsigned long long target = target_of(total);
-        ahead += upto - run_sum;
-        if (target >= ahead && target < ahead + run_sum) {
-            for (int i = r0; i < r1; i++) {
-                ahead += weight_at(i);
-                if (ahead > target) {
-                    a.token[row] = base + i;
-                    if (a.logprob) a.logprob[row] = logprob_of(z[i], total);
-                    break;
-                }
-            }
-        }
+    if (total > 0) {
+        draw(each, run_sum, ahead + upto - run_sum, total);
+    } else if (rank == 0 && tid == 0) {
+        a.token[row] = -1;
+        if (a.logprob) a.logprob[row] = -INFINITY;
     }
     cluster_sync();  // no CTA leaves while another may read its shared memory
 }
@@ -686,8 +590,7 @@ extern "C" int cfi_sample(const float* logits, long long row_stride, int n_rows,
     if (n_rows > 0x7fffffff / SA_CTAS) return (int)cudaErrorInvalidValue;
     SaArgs a = {logits, row_stride, temperature, top_p, min_p, u, top_k, token, logprob, n_vocab, 0, cfi_device_error_word()};
     a.slice = (int)(((n_vocab + SA_CTAS - 1) / SA_CTAS + 3) / 4 * 4);
-    // a row's slice keeps its place within 16 bytes; three arrays of SA_CAP numbers take its place later
-    const size_t smem = std::max((size_t)a.slice * 4 + 16, (size_t)SA_CAP * 3 * 8);
+    const size_t smem = (size_t)a.slice * 4 + 16;  // a row's slice keeps its place within 16 bytes
     static CfiPerDeviceOnce attr;
     cfi_once_per_device(attr, [] {
         cudaFuncSetAttribute(sample_rows, cudaFuncAttributeMaxDynamicSharedMemorySize, SA_MAX_SLICE * 4 + 64);
