@@ -53,7 +53,7 @@ struct SaItem {
     int idx;
     unsigned long long w;
 };
-static_assert((SA_MAX_SLICE / SA_THREADS | 1) + 1 <= 128, "a thread's run is a mask of 128 bits");
+static_assert((((SA_MAX_SLICE + 6) / 4 / SA_THREADS + 1) | 1) <= 32, "a thread's groups of four are a mask of 128 bits");
 
 struct SaShared {
     uint32_t cnt[2][SA_BINS];
@@ -175,6 +175,11 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows(const SaArgs a) {
     const float* src = a.logits + row * a.stride + base;
     const int shift = (int)(reinterpret_cast<uintptr_t>(src) >> 2 & 3), head = min(n, (4 - shift) & 3), body = (n - head) & ~3;
     float* z = slice + shift;  // logit i of the slice is z[i], 16-byte aligned where it is in memory
+    // the slice in groups of four: what lies before and behind it in the first and the last never counts
+    const int groups = (shift + n + 3) / 4;
+    const float4* z4 = reinterpret_cast<const float4*>(slice);
+    if (tid >= 64 && tid < 64 + shift) slice[tid - 64] = -INFINITY;
+    if (tid >= 96 && tid < 96 + 4 * groups - shift - n) z[n + tid - 96] = -INFINITY;
     if (tid == 0 && body > 0) {
         mbar_arrive_expect_tx(&s.bar, (uint32_t)body * 4);
         for (int i = 0; i < body; i += 8192)
@@ -201,23 +206,35 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows(const SaArgs a) {
         const float v = (div == 1.0f ? l : l / div) + 0.0f;
         return v == v ? v : -INFINITY;
     };
-    const int chunk = ((n + SA_WARPS - 1) / SA_WARPS + 31) & ~31;  // each warp's run of the slice
-    const int w0 = min(n, warp * chunk), w1 = min(n, w0 + chunk);
     const int run = ((n + SA_THREADS - 1) / SA_THREADS) | 1;  // each thread's run: odd, so that 32 of them meet no bank twice
     const int r0 = min(n, tid * run), r1 = min(n, r0 + run);
-    // f(i, z[i]) for this warp's run, or this thread's, SA_AHEAD loads at a time
-    auto walk = [&](int i0, int i1, int step, auto&& f) {
-        for (int i = i0; i < i1; i += step * SA_AHEAD) {
+    // f(i, z[i]) for this thread's run, SA_AHEAD loads at a time
+    auto walk = [&](auto&& f) {
+        int i = r0;
+        for (; i + SA_AHEAD <= r1; i += SA_AHEAD) {
             float v[SA_AHEAD];
 #pragma unroll
-            for (int e = 0; e < SA_AHEAD; e++) v[e] = i + step * e < i1 ? z[i + step * e] : -INFINITY;
+            for (int e = 0; e < SA_AHEAD; e++) v[e] = z[i + e];
 #pragma unroll
-            for (int e = 0; e < SA_AHEAD; e++)
-                if (i + step * e < i1) f(i + step * e, v[e]);
+            for (int e = 0; e < SA_AHEAD; e++) f(i + e, v[e]);
         }
+        for (; i < r1; i++) f(i, z[i]);
     };
+    // f(g, z4[g]) for groups of four: g0, g0 + step, ... below g1
+    auto by_four = [&](int g0, int g1, int step, auto&& f) {
+        int g = g0;
+        for (; g + 3 * step < g1; g += 4 * step) {
+            float4 v[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = z4[g + e * step];
+#pragma unroll
+            for (int e = 0; e < 4; e++) f(g + e * step, v[e]);
+        }
+        for (; g < g1; g += step) f(g, z4[g]);
+    };
+    auto max4 = [](const float4& v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); };  // a NaN is passed over
     float mx = -INFINITY;
-    walk(w0 + lane, w1, 32, [&](int, float v) { mx = fmaxf(mx, v); });  // a NaN is passed over
+    by_four(tid, groups, SA_THREADS, [&](int, const float4& v) { mx = fmaxf(mx, max4(v)); });
     mx = warp_max(mx);
     if (lane == 0) s.wmax[warp] = mx;
     __syncthreads();
@@ -236,18 +253,25 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows(const SaArgs a) {
     const float near = 1.0f / div;
     const bool bins_hold = fabsf(zmax) < 8192.0f && near < 1e30f;  // z is exact to far less than a bin
     if (!empty && k <= 0 && bins_hold) {
-        const bool binned = p < 1.0f && bins_hold;
-        walk(r0, r1, 1, [&](int, float l) {
-            if (!((lmax - l) * near < 28.0f)) return;  // no weight (or a NaN)
-            const float v = scaled(l);
-            const unsigned long long w = weight_of(exp_of(v, zmax));
+        const bool binned = p < 1.0f;
+        const float floor = lmax - 28.0f * div * 1.0001f;  // no weight at or below this
+        auto weigh = [&](float v) {  // zmax is finite: expf(0) is 1
+            const unsigned long long w = weight_of(expf(v - zmax));
             run_sum += w;
             const float d = (zmax - v) * 64.0f;
             if (binned && d < (float)SA_BINS) {
                 atomicAdd(&s.cnt[0][(int)d], 1u);
                 atomicAdd(&s.wt[0][(int)d], w);
             }
-        });
+        };
+        if (div == 1.0f)
+            walk([&](int, float l) {
+                if (l > floor) weigh(l + 0.0f);
+            });
+        else
+            walk([&](int, float l) {
+                if (l > floor) weigh(l / div + 0.0f);
+            });
         unsigned long long sum;
         block_incl(run_sum, s.scan, &sum);
         if (tid == 0) s.cta_sum = sum;
@@ -257,7 +281,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows(const SaArgs a) {
     }
     uint32_t level = 1;  // histogram 0 has been used
     // ---- a short run: down to which depth? ----
-    float depth = -1.0f;  // gather what lies less deep (in units of z)
+    float floor = INFINITY;  // gather what is larger
     if (!empty && bins_hold && (k > 0 || p < 1.0f)) {
         // bins down to a depth of 8, or 16 where more than a few are asked for; the second turn reaches 32, where no
         // weight is left
@@ -269,9 +293,15 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows(const SaArgs a) {
                     s.cnt[b][tid] = 0;
                     __syncthreads();
                 }
-                walk(w0 + lane, w1, 32, [&](int, float l) {
-                    const float d = (lmax - l) * near * scale;  // a NaN compares false
-                    if (d < (float)SA_BINS) atomicAdd(&s.cnt[b][(int)d], 1u);
+                const float unit = near * scale, floor = lmax - (float)SA_BINS / unit * 1.0001f;
+                by_four(tid, groups, SA_THREADS, [&](int, const float4& v) {
+                    if (!(max4(v) > floor)) return;
+                    const float l[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float d = (lmax - l[e]) * unit;  // a NaN compares false
+                        if (d < (float)SA_BINS) atomicAdd(&s.cnt[b][(int)d], 1u);
+                    }
                 });
                 cluster_sync();
             }
@@ -299,14 +329,14 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows(const SaArgs a) {
             if (bin + 2 < SA_BINS) {
                 if (tid == bin + 2) s.found_n = (uint32_t)upto;
                 __syncthreads();
-                if (s.found_n <= SA_CAP) depth = (float)(bin + 2) / scale;
+                if (s.found_n <= SA_CAP) floor = lmax - (float)(bin + 2) / scale * div * 1.00001f;
                 __syncthreads();
                 break;
             }
             __syncthreads();
             if (k <= 0 || turn == 1) {
                 // fewer than k elements have any weight: all of them are gathered
-                if (k > 0 && bin == SA_BINS && all <= SA_CAP) depth = (float)SA_BINS / scale;
+                if (k > 0 && bin == SA_BINS && all <= SA_CAP) floor = lmax - (float)SA_BINS / scale * div * 1.00001f;
                 break;
             }
             scale = 16.0f;
@@ -488,30 +518,38 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows(const SaArgs a) {
         return sum;
     };
 
-    if (depth > 0.0f) {
+    int nc = SA_CAP + 1;
+    if (floor < INFINITY) {
         // ---- a short run: gathered in index order by the first CTA, which goes on alone ----
+        const int q = ((groups + SA_THREADS - 1) / SA_THREADS) | 1;  // odd: eight threads' groups take every bank once
+        const int g0 = min(groups, tid * q), g1 = min(groups, g0 + q);
         unsigned long long hit[2] = {0, 0};
-        walk(r0, r1, 1, [&](int i, float l) {
-            if ((lmax - l) * near < depth) {
-                if (i - r0 < 64) hit[0] |= 1ull << (i - r0); else hit[1] |= 1ull << (i - r0 - 64);
-            }
+        by_four(g0, g1, 1, [&](int g, const float4& v) {
+            if (!(max4(v) > floor)) return;
+            const unsigned long long bits = (v.x > floor) | (v.y > floor) << 1 | (v.z > floor) << 2 | (v.w > floor) << 3;
+            if (g - g0 < 16) hit[0] |= bits << 4 * (g - g0); else hit[1] |= bits << 4 * (g - g0 - 16);
         });
         const int mine = __popcll(hit[0]) + __popcll(hit[1]);
         unsigned long long own;
         int at = (int)block_incl((unsigned long long)mine, s.scan, &own) - mine;
         if (tid == 0) s.n_own = (int)own;
         cluster_sync();
-        int nc = 0;
+        nc = 0;
 #pragma unroll
         for (uint32_t r = 0; r < SA_CTAS; r++) {
             const int x = *peer(&s.n_own, r);
             if (r < rank) at += x;
             nc += x;
         }
-        uint32_t* to = const_cast<uint32_t*>(peer(&s.cand[0], 0));
+        if (nc <= SA_CAP) {  // as counted, but for what rounding brings in at the edge
+            uint32_t* to = const_cast<uint32_t*>(peer(&s.cand[0], 0));
 #pragma unroll
-        for (int x = 0; x < 2; x++)
-            for (unsigned long long h = hit[x]; h; h &= h - 1) to[at++] = (uint32_t)(base + r0 + 64 * x + __ffsll((long long)h) - 1);
+            for (int x = 0; x < 2; x++)
+                for (unsigned long long h = hit[x]; h; h &= h - 1)
+                    to[at++] = (uint32_t)(base + 4 * g0 - shift + 64 * x + __ffsll((long long)h) - 1);
+        }
+    }
+    if (nc <= SA_CAP) {
         cluster_sync();
         if (rank != 0) return;
         float v[SA_EACH];
@@ -548,9 +586,9 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows(const SaArgs a) {
     }
 
     // ---- a long run, or no filter: z in place of the logits ----
-    for (int i = w0 + lane; i < w1; i += 32) z[i] = scaled(z[i]);
+    for (int i = tid; i < n; i += SA_THREADS) z[i] = scaled(z[i]);
     __syncthreads();
-    auto each = [&](auto&& f) { walk(r0, r1, 1, [&](int i, float v) { f(v, base + i); }); };
+    auto each = [&](auto&& f) { walk([&](int i, float v) { f(v, base + i); }); };
     if (!empty) {
         if (k > 0) select(std::false_type{}, each, a.n_vocab, false, (double)k, 0ull);
         if (p < 1.0f) select(std::false_type{}, each, a.n_vocab, true, (double)p, 0ull);
@@ -590,7 +628,7 @@ extern "C" int cfi_sample(const float* logits, long long row_stride, int n_rows,
     if (n_rows > 0x7fffffff / SA_CTAS) return (int)cudaErrorInvalidValue;
     SaArgs a = {logits, row_stride, temperature, top_p, min_p, u, top_k, token, logprob, n_vocab, 0, cfi_device_error_word()};
     a.slice = (int)(((n_vocab + SA_CTAS - 1) / SA_CTAS + 3) / 4 * 4);
-    const size_t smem = (size_t)a.slice * 4 + 16;  // a row's slice keeps its place within 16 bytes
+    const size_t smem = (size_t)a.slice * 4 + 32;  // a row's slice keeps its place within 16 bytes
     static CfiPerDeviceOnce attr;
     cfi_once_per_device(attr, [] {
         cudaFuncSetAttribute(sample_rows, cudaFuncAttributeMaxDynamicSharedMemorySize, SA_MAX_SLICE * 4 + 64);
