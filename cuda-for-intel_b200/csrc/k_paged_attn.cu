@@ -5,7 +5,8 @@
 // 16-position tiles of all (sequence, kv head) pairs is cut into equal runs, one per CTA, whatever the
 // lengths: no CTA waits for the longest sequence.  The lengths are read on the device, so every CTA
 // works out the same cuts.  A pair whose tiles lie in several CTAs leaves partial sums (row maximum,
-// sum, weighted values) in the stream's workspace, and a second kernel joins them in CTA order.
+// sum, weighted values) in the stream's workspace; the last of its CTAs to finish joins them in CTA order,
+// so that the result does not depend on which one that was.
 //
 // Each of a CTA's four warps walks every fourth tile with its own ring of cp.async stages (rows past the
 // length are filled with zeros, so what a page holds there never matters) and a running maximum.
@@ -31,39 +32,38 @@ namespace {
 
 using namespace sm100;
 
-constexpr int PA_WARPS = 4, PA_THREADS = PA_WARPS * 32;
+constexpr int PA_WARPS = 4;        // of a CTA; twice as many where a CTA has a pair and an SM to itself
 constexpr int PA_HEADS = 8;        // query heads of a chunk
 constexpr int PA_TILE = 16;        // positions; a page is a multiple of it
 constexpr float PA_V_UNIT = 256.0f;
 // What beginning and ending a pair costs, in tiles: a run's share of the list counts it, so that CTAs with
 // many short sequences get fewer tiles.
-#ifndef PA_FIXED_TILES
-#define PA_FIXED_TILES 5
-#endif
-constexpr int PA_FIXED = PA_FIXED_TILES;
+constexpr int PA_FIXED = 5;
 
-template <int D, bool Q8> struct PaShape {
+template <int D, bool Q8, int W = PA_WARPS> struct PaShape {
     static constexpr int ROW = Q8 ? D : 2 * D;            // bytes of a row
     static constexpr int ROWS = PA_TILE * ROW;            // of a tile of K or V
     static constexpr int SCALES = Q8 ? PA_TILE * D / 16 : 0;
     static constexpr int STAGE = 2 * (ROWS + SCALES);
     static constexpr int STAGES = Q8 ? (D == 64 ? 6 : 4) : (D == 64 ? 4 : 3);
-    static constexpr int CTAS = Q8 ? 3 : (D == 64 ? 3 : 2);  // per SM
+    static constexpr int CTAS = W > PA_WARPS ? 1 : Q8 ? 3 : (D == 64 ? 3 : 2);  // per SM
     static constexpr int RING = STAGES * STAGE;           // a warp's
-    static constexpr int SMEM = PA_WARPS * RING;
+    static constexpr int SMEM = W * RING;
     static constexpr int PART = PA_HEADS * (D + 2);       // floats of a partial result: values, then maximum and sum of each head
     // where the warps meet: a row is a head's values, maximum and sum (stores of the fragments meet no bank twice)
     static constexpr int MEET_ROW = D + (Q8 ? 4 : 8), MEET = PA_HEADS * MEET_ROW;
-    static_assert(SMEM >= PA_WARPS * MEET * 4, "the warps meet in the stages' memory");
+    static_assert(SMEM >= W * MEET * 4, "the warps meet in the stages' memory");
 };
 
 struct PaArgs {
     const uint8_t *k, *v, *q;
     uint8_t* out;
     const int32_t *table, *lens;
-    float* parts;           // [2 x CTAs][PART]
+    float* parts;            // [2 x CTAs][PART]
+    unsigned int* counters;  // [sequence][pair]: zero between calls
     long long q_stride, out_stride;
     int n_pages, page_shift, n_kv_head, group, chunks, max_pages, n_seq, q_f16, out_f16;
+    int whole;  // a CTA to a pair
     float scale_log2;
 };
 
@@ -143,10 +143,11 @@ struct PaCut {
     // an empty sequence still has its zeros to write
     static CFI_DEV int tiles_of(int len) { return max(1, (len + PA_TILE - 1) / PA_TILE); }
     CFI_DEV int units_of(int s) const { return PA_FIXED + tiles_of(length(s)); }
+    CFI_DEV explicit PaCut(const PaArgs& a)
+        : lens(a.lens), most((int)min((long long)a.max_pages << a.page_shift, 0x7fffff00LL)) {}
     // Called by whole warps.  `first`: the units of the sequence that is this lane's, of the first 32.
-    CFI_DEV PaCut(const PaArgs& a, int ctas) : lens(a.lens) {
+    CFI_DEV void read(const PaArgs& a, int ctas) {
         const int lane = threadIdx.x & 31, hc = a.n_kv_head * a.chunks;
-        most = (int)min((long long)a.max_pages << a.page_shift, 0x7fffff00LL);
         first = lane < a.n_seq ? units_of(lane) * hc : 0;
         int n = first;
         for (int s = lane + 32; s < a.n_seq; s += 32) n += units_of(s) * hc;
@@ -155,56 +156,115 @@ struct PaCut {
     }
 };
 
-template <int D, bool Q8>
-__global__ void __launch_bounds__(PA_THREADS, (PaShape<D, Q8>::CTAS)) paged_attn(const PaArgs a) {
-    using S = PaShape<D, Q8>;
+// A pair that this CTA has a part of, and what it takes to join all of them.
+struct PaShared {
+    int id = -1, seq, head0, nh, b0, n;  // place of its counter; CTAs b0 .. b0 + n - 1 have its tiles
+};
+
+// Joins the results of a pair's CTAs in their order.  A thread takes four dims of a head; a round's loads are
+// in flight together.
+template <class S, int D, int THREADS> CFI_DEV void join_parts(const PaArgs& a, const PaShared& p) {
+    constexpr int ROUND = 16;
+    const float* parts = a.parts + 2LL * p.b0 * S::PART;
+    for (int i = threadIdx.x; i < p.nh * (D / 4); i += THREADS) {
+        const int h = i / (D / 4), d = i % (D / 4) * 4;
+        float m = -INFINITY, l = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int x0 = 0; x0 < p.n; x0 += ROUND) {
+            float4 v[ROUND];
+            float2 ml[ROUND];
+#pragma unroll
+            for (int e = 0; e < ROUND; e++) {
+                const int x = x0 + e;
+                // the first CTA's result is in its second place: it leaves the pair unfinished
+                const float* q = parts + (2LL * x + (x == 0 ? 1 : 0)) * S::PART;
+                ml[e] = x < p.n ? __ldcg(reinterpret_cast<const float2*>(q + PA_HEADS * D) + h) : make_float2(-INFINITY, 0.0f);
+                v[e] = x < p.n ? __ldcg(reinterpret_cast<const float4*>(q + h * D + d)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+            float mm = m;
+#pragma unroll
+            for (int e = 0; e < ROUND; e++) mm = fmaxf(mm, ml[e].x);
+            const float keep = m == -INFINITY ? 0.0f : ex2(m - mm);
+            l *= keep;
+            o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
+            m = mm;
+#pragma unroll
+            for (int e = 0; e < ROUND; e++) {
+                const float f = ml[e].x == -INFINITY ? 0.0f : ex2(ml[e].x - mm);
+                l = fmaf(f, ml[e].y, l);
+                add_to(o, f, v[e]);
+            }
+        }
+        write_out(a, p.seq, p.head0 + h, D, d, o, l);
+    }
+}
+
+template <int D, bool Q8, int W>
+__global__ void __launch_bounds__(W * 32, (PaShape<D, Q8, W>::CTAS)) paged_attn(const PaArgs a) {
+    using S = PaShape<D, Q8, W>;
     constexpr int NB = D / 32, NT = D / 8, KK = D / 16;
     extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int s_last[2];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
     const int page_size = 1 << a.page_shift, hc = a.n_kv_head * a.chunks;
     pdl_launch_dependents();
     pdl_wait();
 
-    // ---- this CTA's run ----
-    const PaCut cut(a, gridDim.x);
-    const int quota = cut.quota;
-    if ((int)blockIdx.x > (cut.total - 1) / quota) return;
-    const int begin = blockIdx.x * quota, end = min(begin + quota, cut.total);
-    int at = begin, seq = 0, seq_start = 0;  // seq_start: the sequence's first unit
-    for (int base = 0;; base += 32) {
-        const int n = base == 0 ? cut.first : base + lane < a.n_seq ? cut.units_of(base + lane) * hc : 0;
-        int incl = n;
+    PaCut cut(a);
+    int begin = 0, end = 1, at = 0, seq = 0, seq_start = 0, pair = 0;  // seq_start: the sequence's first unit
+    if (a.whole) {
+        seq = blockIdx.x / hc;
+        pair = blockIdx.x - seq * hc;
+    } else {
+        // ---- this CTA's run ----
+        cut.read(a, gridDim.x);
+        if ((int)blockIdx.x > (cut.total - 1) / cut.quota) return;
+        begin = at = blockIdx.x * cut.quota;
+        end = min(begin + cut.quota, cut.total);
+        for (int base = 0;; base += 32) {
+            const int n = base == 0 ? cut.first : base + lane < a.n_seq ? cut.units_of(base + lane) * hc : 0;
+            int incl = n;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += x;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += x;
+            }
+            const uint32_t hit = __ballot_sync(0xffffffffu, seq_start + incl > at);
+            if (hit) {
+                const int l = __ffs(hit) - 1;
+                seq = base + l;
+                seq_start += __shfl_sync(0xffffffffu, incl - n, l);
+                break;
+            }
+            seq_start += __shfl_sync(0xffffffffu, incl, 31);
         }
-        const uint32_t hit = __ballot_sync(0xffffffffu, seq_start + incl > at);
-        if (hit) {
-            const int l = __ffs(hit) - 1;
-            seq = base + l;
-            seq_start += __shfl_sync(0xffffffffu, incl - n, l);
-            break;
-        }
-        seq_start += __shfl_sync(0xffffffffu, incl, 31);
     }
 
     const uint32_t ring = smem_u32(smem) + warp * S::RING;
+    PaShared shared[2];  // of the pairs that it goes on with, and leaves unfinished
     while (at < end) {
         // ---- one (sequence, kv head, chunk): its tiles [t0, t1) of n_tiles ----
         const int len = cut.length(seq), n_tiles = PaCut::tiles_of(len);
-        const int units = PA_FIXED + n_tiles, pair = (at - seq_start) / units, first = seq_start + pair * units + PA_FIXED;
-        const int t0 = max(0, at - first), t1 = min(n_tiles, end - first);
-        at = first + n_tiles;
-        if (t1 <= 0) break;  // the run ends before the pair's first tile
+        int t0 = 0, t1 = n_tiles;
+        if (!a.whole) {
+            const int units = PA_FIXED + n_tiles;
+            pair = (at - seq_start) / units;
+            const int first = seq_start + pair * units + PA_FIXED;
+            t0 = max(0, at - first);
+            t1 = min(n_tiles, end - first);
+            at = first + n_tiles;
+            if (t1 <= 0) break;  // the run ends before the pair's first tile
+        } else {
+            at = end;
+        }
         const int kvh = pair / a.chunks, h0 = (pair - kvh * a.chunks) * PA_HEADS, nh = min(PA_HEADS, a.group - h0);
         const int head0 = kvh * a.group + h0;
 
         // page ids of this warp's next 32 tiles, one a lane
         const int32_t* trow = a.table + (long long)seq * a.max_pages;
-        const int mine = t1 - t0 > warp ? (t1 - t0 - warp + PA_WARPS - 1) / PA_WARPS : 0;  // tiles of this warp
+        const int mine = t1 - t0 > warp ? (t1 - t0 - warp + W - 1) / W : 0;  // tiles of this warp
         auto load_ids = [&](int i) {
-            const int t = t0 + warp + (i + lane) * PA_WARPS;
+            const int t = t0 + warp + (i + lane) * W;
             return t < t1 && t * PA_TILE < len ? min(max(trow[t * PA_TILE >> a.page_shift], 0), a.n_pages - 1) : 0;
         };
         int ids = load_ids(0);
@@ -229,7 +289,7 @@ __global__ void __launch_bounds__(PA_THREADS, (PaShape<D, Q8>::CTAS)) paged_attn
 
         auto fetch = [&](int i) {  // tile i of this warp into its stage
             if (i < mine) {
-                const int t = t0 + warp + i * PA_WARPS, p0 = t * PA_TILE;
+                const int t = t0 + warp + i * W, p0 = t * PA_TILE;
                 const int page = __shfl_sync(0xffffffffu, ids, i & 31), off = p0 & (page_size - 1);
                 const long long region = ((long long)page * a.n_kv_head + kvh) * paged_region_bytes<D, Q8>(page_size);
                 const uint32_t st = ring + (i % S::STAGES) * S::STAGE;
@@ -315,7 +375,7 @@ __global__ void __launch_bounds__(PA_THREADS, (PaShape<D, Q8>::CTAS)) paged_attn
                     }
                 }
             }
-            const int left = len - (t0 + warp + i * PA_WARPS) * PA_TILE;
+            const int left = len - (t0 + warp + i * W) * PA_TILE;
             if (left < PA_TILE) {
 #pragma unroll
                 for (int e = 0; e < 4; e++)
@@ -409,24 +469,28 @@ __global__ void __launch_bounds__(PA_THREADS, (PaShape<D, Q8>::CTAS)) paged_attn
         }
         if (c == 0) *reinterpret_cast<float2*>(mine_o + D) = make_float2(m, l);
         __syncthreads();
-        const bool whole = t0 == 0 && t1 == n_tiles;
-        // a CTA leaves at most two partial results: of a pair that it goes on with, and of one that it leaves unfinished
+        const bool done = t0 == 0 && t1 == n_tiles;
+        if (!done) {
+            const int start = at - n_tiles, b0 = start / cut.quota, n = (at - 1) / cut.quota - b0 + 1;
+            const PaShared p = {seq * hc + pair, seq, head0, nh, b0, n};
+            if (t0 == 0) shared[1] = p; else shared[0] = p;
+        }
         float* part = a.parts + (2LL * blockIdx.x + (t0 == 0 ? 1 : 0)) * S::PART;
-        for (int i = tid; i < nh * (D / 4); i += PA_THREADS) {
+        for (int i = tid; i < nh * (D / 4); i += W * 32) {
             const int h = i / (D / 4), d = i % (D / 4) * 4;
             const float* p = meet + h * S::MEET_ROW;
             float mm = -INFINITY, ll = 0.0f;
             float4 oo = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-            for (int w = 0; w < PA_WARPS; w++) mm = fmaxf(mm, p[w * S::MEET + D]);
+            for (int w = 0; w < W; w++) mm = fmaxf(mm, p[w * S::MEET + D]);
 #pragma unroll
-            for (int w = 0; w < PA_WARPS; w++) {
+            for (int w = 0; w < W; w++) {
                 const float2 ml = *reinterpret_cast<const float2*>(p + w * S::MEET + D);
                 const float f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - mm);
                 ll = fmaf(f, ml.y, ll);
                 add_to(oo, f, *reinterpret_cast<const float4*>(p + w * S::MEET + d));
             }
-            if (whole) {
+            if (done) {
                 write_out(a, seq, head0 + h, D, d, oo, ll);
             } else {
                 __stcg(reinterpret_cast<float4*>(part + h * D + d), oo);
@@ -439,96 +503,58 @@ __global__ void __launch_bounds__(PA_THREADS, (PaShape<D, Q8>::CTAS)) paged_attn
             seq++;
         }
     }
-}
-
-// Joins the results of a pair's CTAs, one head a CTA; a pair that one CTA did whole is already written.  Thread
-// (way, d) takes results way, way + WAYS, ... of four dims, all loads of a round before the first use.
-template <int D, bool Q8>
-__global__ void __launch_bounds__(PA_THREADS) paged_join(const PaArgs a, int ctas) {
-    using S = PaShape<D, Q8>;
-    constexpr int QUADS = D / 4, WAYS = PA_THREADS / QUADS, ROUND = 4;
-    __shared__ float4 so[WAYS][QUADS];
-    __shared__ float2 sm[WAYS];
-    const int tid = threadIdx.x, lane = tid & 31, way = tid / QUADS, d = tid % QUADS * 4, hc = a.n_kv_head * a.chunks;
-    const int head = blockIdx.x, seq = blockIdx.y, h = head % a.group % PA_HEADS;
-    const int pair = head / a.group * a.chunks + head % a.group / PA_HEADS;
-    pdl_launch_dependents();
-    pdl_wait();
-    const PaCut cut(a, ctas);
-    int before = 0;
-    for (int s = lane; s < seq; s += 32) before += s < 32 ? cut.first : cut.units_of(s) * hc;
-    before = __reduce_add_sync(0xffffffffu, before);
-    const int n_tiles = PaCut::tiles_of(cut.length(seq)), first = before + pair * (PA_FIXED + n_tiles) + PA_FIXED;
-    const int b0 = first / cut.quota, n = (first + n_tiles - 1) / cut.quota - b0 + 1;  // the CTAs that have its tiles
-    if (n == 1) return;
-    const float* parts = a.parts + 2LL * b0 * S::PART;
-    float m = -INFINITY, l = 0.0f;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int x0 = way; x0 < n; x0 += WAYS * ROUND) {
-        float4 v[ROUND];
-        float2 ml[ROUND];
-#pragma unroll
-        for (int i = 0; i < ROUND; i++) {
-            const int x = x0 + i * WAYS;
-            // the first CTA's result is in its second place: it leaves the pair unfinished
-            const float* p = parts + (2LL * x + (x == 0 ? 1 : 0)) * S::PART;
-            ml[i] = x < n ? __ldcg(reinterpret_cast<const float2*>(p + PA_HEADS * D) + h) : make_float2(-INFINITY, 0.0f);
-            v[i] = x < n ? __ldcg(reinterpret_cast<const float4*>(p + h * D + d)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    // ---- the results that are parts: the last of a pair's CTAs to come here joins them ----
+    if (a.whole || (shared[0].id < 0 && shared[1].id < 0)) return;
+    if (lane == 0 && warp < 2) {  // one thread for each
+        const PaShared p = warp == 0 ? shared[0] : shared[1];
+        bool last = false;
+        if (p.id >= 0) {
+            __threadfence();  // after a barrier: covers the stores of the whole CTA
+            last = atomicAdd(&a.counters[p.id], 1u) == (unsigned)(p.n - 1);
+            if (last) {
+                __threadfence();
+                a.counters[p.id] = 0u;
+            }
         }
-        float mm = m;
-#pragma unroll
-        for (int i = 0; i < ROUND; i++) mm = fmaxf(mm, ml[i].x);
-        const float keep = m == -INFINITY ? 0.0f : ex2(m - mm);
-        l *= keep;
-        o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
-        m = mm;
-#pragma unroll
-        for (int i = 0; i < ROUND; i++) {
-            const float f = ml[i].x == -INFINITY ? 0.0f : ex2(ml[i].x - mm);
-            l = fmaf(f, ml[i].y, l);
-            add_to(o, f, v[i]);
-        }
+        s_last[warp] = last;
     }
-    so[way][d / 4] = o;
-    if (d == 0) sm[way] = make_float2(m, l);
     __syncthreads();
-    if (way == 0) {
-        float mm = m, ll = 0.0f;
 #pragma unroll
-        for (int w = 1; w < WAYS; w++) mm = fmaxf(mm, sm[w].x);
-        o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int w = 0; w < WAYS; w++) {
-            const float f = sm[w].x == -INFINITY ? 0.0f : ex2(sm[w].x - mm);
-            ll = fmaf(f, sm[w].y, ll);
-            add_to(o, f, so[w][d / 4]);
-        }
-        write_out(a, seq, head, D, d, o, ll);
-    }
+    for (int x = 0; x < 2; x++)
+        if (s_last[x]) join_parts<S, D, W * 32>(a, shared[x]);
 }
 
-template <int D, bool Q8> int launch(PaArgs& a, long long most_units, cudaStream_t stream) {
-    using S = PaShape<D, Q8>;
+int sm_count() {
     static CfiPerDeviceOnce once;
     static int sms[CFI_MAX_DEVICES + 1];
     const int dev = cfi_device_index();
     int* n = &sms[dev < 0 ? CFI_MAX_DEVICES : dev];
     cfi_once_per_device(once, [n] {
         int d = 0;
-        cudaGetDevice(&d);
-        cudaDeviceGetAttribute(n, cudaDevAttrMultiProcessorCount, d);
-        cudaFuncSetAttribute(paged_attn<D, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+        if (cudaGetDevice(&d) != cudaSuccess || cudaDeviceGetAttribute(n, cudaDevAttrMultiProcessorCount, d) != cudaSuccess) cudaGetLastError();
     });
-    const long long ctas = (long long)(*n > 0 ? *n : 148) * S::CTAS;
-    // no CTA has fewer units than this
-    const long long grid = std::min(ctas, most_units / (PA_FIXED + PA_WARPS) + 1);
-    int err = 0;
-    a.parts = static_cast<float*>(cfi_stream_buffer(CFI_BUF_PAGED_PARTS, (size_t)ctas * 2 * S::PART * 4, stream, &err));
-    if (!a.parts) return err;
+    return *n > 0 ? *n : 148;
+}
+
+template <int D, bool Q8, int W> int launch(PaArgs& a, long long pairs, long long most_units, cudaStream_t stream) {
+    using S = PaShape<D, Q8, W>;
+    static CfiPerDeviceOnce once;
+    cfi_once_per_device(once, [] { cudaFuncSetAttribute(paged_attn<D, Q8, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM); });
+    long long grid = pairs;
+    if (!a.whole) {
+        // no CTA has fewer units than this
+        const long long ctas = (long long)sm_count() * S::CTAS;
+        grid = std::min(ctas, most_units / (PA_FIXED + PA_WARPS) + 1);
+        int err = 0;
+        a.parts = static_cast<float*>(cfi_stream_buffer(CFI_BUF_PAGED_PARTS, (size_t)ctas * 2 * S::PART * 4, stream, &err));
+        if (!a.parts) return err;
+        a.counters = static_cast<unsigned int*>(cfi_stream_buffer(CFI_BUF_COUNTERS, (size_t)pairs * 4, stream, &err));
+        if (!a.counters) return err;
+    }
     const char* ep = getenv("CFI_PDL");
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3((unsigned)grid, 1, 1);
-    lc.blockDim = dim3(PA_THREADS, 1, 1);
+    lc.blockDim = dim3(W * 32, 1, 1);
     lc.dynamicSmemBytes = S::SMEM;
     lc.stream = stream;
     cudaLaunchAttribute at[1];
@@ -536,11 +562,7 @@ template <int D, bool Q8> int launch(PaArgs& a, long long most_units, cudaStream
     at[0].val.programmaticStreamSerializationAllowed = 1;
     lc.attrs = at;
     lc.numAttrs = (ep && strcmp(ep, "0") == 0) ? 0 : 1;
-    err = (int)cudaLaunchKernelEx(&lc, paged_attn<D, Q8>, (const PaArgs)a);
-    if (err || grid == 1) return err;
-    lc.gridDim = dim3((unsigned)(a.n_kv_head * a.group), (unsigned)a.n_seq, 1);
-    lc.dynamicSmemBytes = 0;
-    return (int)cudaLaunchKernelEx(&lc, paged_join<D, Q8>, (const PaArgs)a, (int)grid);
+    return (int)cudaLaunchKernelEx(&lc, paged_attn<D, Q8, W>, (const PaArgs)a);
 }
 
 }  // namespace
@@ -577,6 +599,23 @@ extern "C" int cfi_paged_attention(const CfiPagedCache* c, const void* q, int q_
     const long long most_units = pairs * (PA_FIXED + (long long)max_pages * (c->page_size / PA_TILE));
     if (most_units > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (c->head_dim == 64) return c->type == 1 ? launch<64, false>(a, most_units, s) : launch<64, true>(a, most_units, s);
-    return c->type == 1 ? launch<128, false>(a, most_units, s) : launch<128, true>(a, most_units, s);
+    const long long positions = (long long)max_pages * c->page_size;
+    // Short tables: a CTA to a pair, which neither reads all lengths nor joins anything.  Measured against the equal
+    // runs (us, every sequence but one up to four times shorter than the longest; 14/2 heads of 64 in f16, then 12/2 of
+    // 128 in Q8_0): eight warps, 1 sequence of 768 5.1 to 6.0 and 9.0 to 8.0, of 2048 9.6 to 6.3 and 19 to 9.6; 64
+    // sequences of 1536 8.2 to 11 and 15 to 16, of 2048 10 to 11 and 19 to 19; four warps, three CTAs to an SM, 128
+    // sequences of 768 9.1 to 13 and 19 to 18.
+    const int sms = sm_count();
+    const int w = pairs <= sms ? (positions <= (2 * pairs > sms ? 1536 : 768) ? 8 : 0) : positions <= 768 ? 4 : 0;
+    a.whole = w > 0;
+    const int variant = (c->head_dim == 128) * 2 + (c->type == 8);
+    if (w == 8)
+        return variant == 0   ? launch<64, false, 8>(a, pairs, most_units, s)
+               : variant == 1 ? launch<64, true, 8>(a, pairs, most_units, s)
+               : variant == 2 ? launch<128, false, 8>(a, pairs, most_units, s)
+                              : launch<128, true, 8>(a, pairs, most_units, s);
+    return variant == 0   ? launch<64, false, PA_WARPS>(a, pairs, most_units, s)
+           : variant == 1 ? launch<64, true, PA_WARPS>(a, pairs, most_units, s)
+           : variant == 2 ? launch<128, false, PA_WARPS>(a, pairs, most_units, s)
+                          : launch<128, true, PA_WARPS>(a, pairs, most_units, s);
 }
