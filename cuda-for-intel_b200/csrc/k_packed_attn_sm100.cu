@@ -57,6 +57,12 @@ CFI_DEV float ex2(float x) {  // 2^x (PTX ex2.approx; -inf -> +0)
     return y;
 }
 
+CFI_DEV bool elect_one() {  // true in one lane of a converged warp
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+
 template <int D>
 __global__ void __launch_bounds__(KA_THREADS, 1)
     packed_attn(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
@@ -143,7 +149,9 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    // all 512 columns: they begin at 0, and the MMAs' operands are constants
+    constexpr uint32_t TM = 0;
+    const uint32_t tmem = TM;
     auto fail = [&](unsigned code) {
         cfi_set_error(a.err, code);
         *abort_flag = 1;
@@ -185,7 +193,7 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
             }
         }
       } else if (warp == KA_MMA_WARP) {
-        if (lane == 0 && nmax > 0) {
+        if (nmax > 0) {
             const uint32_t id_s = idesc_f16(KA_M, KA_N, 0);
             const uint32_t id_o = idesc_f16(KA_M, D, 0) | (1u << 16);  // B (V) MN-major
             // descriptors of Q and the first slot; an offset of n bytes adds n / 16
@@ -195,48 +203,51 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
 #pragma unroll
                 for (int kk = 0; kk < D / 16; kk++) {
                     const uint32_t off = (kk >> 2) * BLK + (kk & 3) * 32;
-                    mma_f16(tmem + x * KA_N, dq + ((x * TILE + off) >> 4), dk + st * (TILE >> 4) + (off >> 4), id_s, kk > 0 ? 1u : 0u);
+                    mma_f16(TM + x * KA_N, dq + ((x * TILE + off) >> 4), dk + st * (TILE >> 4) + (off >> 4), id_s, kk > 0 ? 1u : 0u);
                 }
                 mma_commit(&s_full[x]);
             };
             auto values = [&](int x, int st, bool first) {  // O_x += P_x V
 #pragma unroll
                 for (int kk = 0; kk < KA_N / 16; kk++)
-                    mma_f16_ts(tmem + 256 + x * D, tmem + x * KA_N + kk * 8, dv + st * (TILE >> 4) + kk * (16 * 128 >> 4), id_o,
-                               (!first || kk > 0) ? 1u : 0u);
+                    mma_f16_ts(TM + 256 + x * D, TM + x * KA_N + kk * 8, dv + st * (TILE >> 4) + kk * (16 * 128 >> 4), id_o,
+                              (!first || kk > 0) ? 1u : 0u);
             };
-            bool ok = mbar_wait(q_full, 0, abort_flag) && mbar_wait(&full[0], 0, abort_flag);
+            auto ready = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)) != 0; };
+            bool ok = ready(q_full, 0) && ready(&full[0], 0);
             if (ok) {
                 tc_fence_after();
 #pragma unroll
                 for (int x = 0; x < 2; x++)
-                    if ((x ? nb1 : nb0) > 0) scores(x, 0);
-                mma_commit(&empty[0]);
+                    if ((x ? nb1 : nb0) > 0 && elect_one()) scores(x, 0);
+                if (elect_one()) mma_commit(&empty[0]);
             }
             for (int j = 0; ok && j < nmax; j++) {
                 const int iv = 2 * j + 1, ik = 2 * j + 2, sv = iv % NS, sk = ik % NS;
-                ok = mbar_wait(&full[sv], (uint32_t)(iv / NS) & 1, abort_flag);
-                if (ok && cut && j == nmax - 1) ok = mbar_wait(v_clean, 0, abort_flag);
+                ok = ready(&full[sv], (uint32_t)(iv / NS) & 1);
+                if (ok && cut && j == nmax - 1) ok = ready(v_clean, 0);
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
                     const int n = x ? nb1 : nb0;
                     if (ok && j < n) {
-                        ok = mbar_wait(&p_full[x], (uint32_t)j & 1, abort_flag);
+                        ok = ready(&p_full[x], (uint32_t)j & 1);
                         if (!ok) break;
                         tc_fence_after();
-                        values(x, sv, j == 0);
-                        if (j == n - 1) mma_commit(&o_full[x]);
+                        if (elect_one()) {
+                            values(x, sv, j == 0);
+                            if (j == n - 1) mma_commit(&o_full[x]);
+                        }
                     }
-                    if (x == 1) mma_commit(&empty[sv]);
+                    if (x == 1 && elect_one()) mma_commit(&empty[sv]);
                     if (j + 1 < n) {
-                        ok = mbar_wait(&full[sk], (uint32_t)(ik / NS) & 1, abort_flag);
+                        ok = ready(&full[sk], (uint32_t)(ik / NS) & 1);
                         if (!ok) break;
-                        scores(x, sk);
+                        if (elect_one()) scores(x, sk);
                     }
-                    if (x == 1 && j + 1 < nmax) mma_commit(&empty[sk]);
+                    if (x == 1 && j + 1 < nmax && elect_one()) mma_commit(&empty[sk]);
                 }
             }
-            if (!ok) fail(0xfb200);
+            if (!ok && lane == 0) fail(0xfb200);
         }
       }
     } else {
@@ -270,14 +281,15 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
                     for (int i = 0; i < 32; i++)
                         if (32 * c + i >= left) sv[c][i] = 0xff800000u;
             }
-            float mx4[4];
+            float mx8[8];  // chains that do not wait on one another
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                mx4[c] = __uint_as_float(sv[c][0]);
+            for (int e = 0; e < 8; e++) mx8[e] = fmaxf(__uint_as_float(sv[e >> 1][16 * (e & 1)]), __uint_as_float(sv[e >> 1][16 * (e & 1) + 1]));
 #pragma unroll
-                for (int i = 1; i < 32; i++) mx4[c] = fmaxf(mx4[c], __uint_as_float(sv[c][i]));
-            }
-            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * a.scale_log2;
+            for (int i = 2; i < 16; i += 2)
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    mx8[e] = fmaxf(fmaxf(mx8[e], __uint_as_float(sv[e >> 1][16 * (e & 1) + i])), __uint_as_float(sv[e >> 1][16 * (e & 1) + i + 1]));
+            const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])), fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]))) * a.scale_log2;
             const bool grow = valid && (mx > m_used + KA_RESCALE_LOG2 || (m_used == -INFINITY && mx > -INFINITY));
             if (__any_sync(0xffffffffu, grow)) {
                 const float alpha = !grow ? 1.0f : m_used == -INFINITY ? 0.0f : ex2(m_used - mx);
