@@ -126,6 +126,9 @@ enum { CFI_BUF_SPLITK = 1, CFI_BUF_MMQ_SCRATCH = 2, CFI_BUF_SKINNY_WS = 3, CFI_B
        CFI_BUF_PAGED_PARTS = 6 };
 void* cfi_stream_buffer(int kind, size_t bytes, cudaStream_t stream, int* err);
 
+// SMs of the current device (148 when it cannot be asked).
+int cfi_sm_count();
+
 // The library's device error word (k_mmq_sm100.cu; read and cleared by cfi_device_error).
 unsigned int* cfi_device_error_word();
 

@@ -524,18 +524,6 @@ __global__ void __launch_bounds__(W * 32, (PaShape<D, Q8, W>::CTAS)) paged_attn(
         if (s_last[x]) join_parts<S, D, W * 32>(a, shared[x]);
 }
 
-int sm_count() {
-    static CfiPerDeviceOnce once;
-    static int sms[CFI_MAX_DEVICES + 1];
-    const int dev = cfi_device_index();
-    int* n = &sms[dev < 0 ? CFI_MAX_DEVICES : dev];
-    cfi_once_per_device(once, [n] {
-        int d = 0;
-        if (cudaGetDevice(&d) != cudaSuccess || cudaDeviceGetAttribute(n, cudaDevAttrMultiProcessorCount, d) != cudaSuccess) cudaGetLastError();
-    });
-    return *n > 0 ? *n : 148;
-}
-
 template <int D, bool Q8, int W> int launch(PaArgs& a, long long pairs, long long most_units, cudaStream_t stream) {
     using S = PaShape<D, Q8, W>;
     static CfiPerDeviceOnce once;
@@ -543,7 +531,7 @@ template <int D, bool Q8, int W> int launch(PaArgs& a, long long pairs, long lon
     long long grid = pairs;
     if (!a.whole) {
         // no CTA has fewer units than this
-        const long long ctas = (long long)sm_count() * S::CTAS;
+        const long long ctas = (long long)cfi_sm_count() * S::CTAS;
         grid = std::min(ctas, most_units / (PA_FIXED + PA_WARPS) + 1);
         int err = 0;
         a.parts = static_cast<float*>(cfi_stream_buffer(CFI_BUF_PAGED_PARTS, (size_t)ctas * 2 * S::PART * 4, stream, &err));
@@ -605,7 +593,7 @@ extern "C" int cfi_paged_attention(const CfiPagedCache* c, const void* q, int q_
     // 128 in Q8_0): eight warps, 1 sequence of 768 5.1 to 6.0 and 9.0 to 8.0, of 2048 9.6 to 6.3 and 19 to 9.6; 64
     // sequences of 1536 8.2 to 11 and 15 to 16, of 2048 10 to 11 and 19 to 19; four warps, three CTAs to an SM, 128
     // sequences of 768 9.1 to 13 and 19 to 18.
-    const int sms = sm_count();
+    const int sms = cfi_sm_count();
     const int w = pairs <= sms ? (positions <= (2 * pairs > sms ? 1536 : 768) ? 8 : 0) : positions <= 768 ? 4 : 0;
     a.whole = w > 0;
     const int variant = (c->head_dim == 128) * 2 + (c->type == 8);

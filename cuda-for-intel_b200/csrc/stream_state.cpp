@@ -80,6 +80,25 @@ std::vector<void*> g_retired;
 
 }  // namespace
 
+int cfi_sm_count() {
+    static std::mutex mu;
+    static std::map<int, int> sms;
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) {
+        cudaGetLastError();
+        return 148;
+    }
+    std::lock_guard<std::mutex> g(mu);
+    auto it = sms.find(dev);
+    if (it != sms.end()) return it->second;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) {
+        cudaGetLastError();
+        return 148;
+    }
+    sms[dev] = n;
+    return n;
+}
+
 int cfi_glue_slot(cudaStream_t stream, CfiGlueSlot* out) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) {
