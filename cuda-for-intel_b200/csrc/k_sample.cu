@@ -1,10 +1,13 @@
 // k_sample.cu -- one token per row of logits: temperature, top-k, top-p, min-p and a given uniform
 // number (include/cfi_serve.h gives the definition).
 //
-// A cluster of CTAs takes a row.  The logits are read once, by bulk copies: each CTA keeps its slice in
-// shared memory, the later passes walk it there and meet through distributed shared memory.  Everything
-// that is summed is a whole number (a weight is exp(z - max) in units of 2^-40), so no sum depends on its order
-// and every CTA of a cluster reaches the same decisions from the same histograms.
+// The logits are one read of memory; what bounds a call is the chain of passes behind it, each of which needs the
+// last one's answer.  Few rows: a cluster of CTAs takes a row, each keeps its slice in shared memory,
+// walks it there and meets the others through distributed shared memory (one row of 151936 with a nucleus among the
+// first 50: 13.9 us).  Many: a CTA takes a row and streams it from memory, as many rows at once as fit (256 rows, top-k 50: 44 us, 3.5 TB/s;
+// greedy: 34 us, 4.6 TB/s; without a filter, two reads and an exponential of everything: 81 us).
+// Everything that is summed is a whole number (a weight is exp(z - max) in units of 2^-40), so no sum depends on its
+// order and every CTA of a cluster reaches the same decisions from the same histograms.
 //
 // All three filters keep a run from the top of the order (larger z first, then lower index).  Where that run
 // is short -- it is, when a top-k or a nucleus of a language model's logits is asked for -- the bins of a
@@ -12,8 +15,10 @@
 // the cluster's first CTA, and that CTA finishes alone with them in registers.  The gathering needs no exact z: bins
 // of (max logit - logit) / T are 1/64 wide, far above the rounding of z, and one bin more is taken.
 //
-// Each filter is a cut, the last element that stays, found
-// without sorting, in one CTA or in the whole cluster (more than SA_CAP elements): a histogram over 512 bins finds the bin that the cut falls in; the at most SA_LIST
+// A long nucleus: the bin that its end falls in is gathered and ranked alone, and the kept weights are summed over the row.
+//
+// Each filter is a cut, the last element that stays, found without sorting, in one CTA or in the whole cluster
+// (more than SA_CAP elements): a histogram over 512 bins finds the bin that the cut falls in; the at most SA_LIST
 // elements of that bin are listed and each one's rank is counted against the others.  A fuller bin is divided
 // again: first by the next bits of max - z, then by the bits of z itself, after which all that is left is
 // equal and the index decides.
@@ -23,6 +28,7 @@
 
 #include <stdlib.h>
 #include <string.h>
+#include <algorithm>
 #include <type_traits>
 
 namespace {
@@ -35,6 +41,7 @@ constexpr int SA_LIST = 128;          // boundary-bin elements that are listed
 constexpr int SA_CAP = 2048, SA_EACH = SA_CAP / SA_THREADS;  // elements that the first CTA sorts, and a thread's of them
 constexpr int SA_CTAS = 8;            // of a cluster: the portable size, two CTAs to an SM at a vocabulary of 150,000
 constexpr int SA_MAX_SLICE = 50000;   // floats of a row that one CTA holds
+constexpr int SA_BLOCK4 = 256;         // float4 of a block: 32 lanes' groups of eight
 constexpr int SA_AHEAD = 8;           // loads of a pass that are in flight together
 
 struct SaArgs {
@@ -45,7 +52,27 @@ struct SaArgs {
     int32_t* token;
     float* logprob;
     int n_vocab, slice;
+    int n_rows;
+    int spare;  // of many rows: how many whole() ones clusters take, 0 for all rows
     unsigned int* err;
+};
+
+// A row's parameters as they act
+struct SaRow {
+    bool greedy;
+    float div, p, minp;
+    int k;  // 0: no top-k
+    CFI_DEV SaRow(const SaArgs& a, int row) {
+        const float t = a.temperature ? __ldcg(a.temperature + row) : 1.0f;
+        greedy = t <= 0.0f;
+        div = greedy ? 1.0f : t;
+        k = greedy ? 1 : a.top_k ? __ldcg(a.top_k + row) : 0;
+        if (k < 0 || k >= a.n_vocab) k = 0;
+        p = a.top_p ? __ldcg(a.top_p + row) : 1.0f;
+        minp = a.min_p ? __ldcg(a.min_p + row) : 0.0f;
+    }
+    // rows that are long work for one CTA: a nucleus of the whole row, and what more than a few are kept of
+    CFI_DEV bool whole(int n_vocab) const { return n_vocab > SA_CAP && (k > SA_CAP / 2 || (k == 0 && p < 1.0f)); }
 };
 
 struct SaItem {
@@ -53,11 +80,13 @@ struct SaItem {
     int idx;
     unsigned long long w;
 };
+constexpr int SA_MAX_BLOCKS = (SA_CTAS * SA_MAX_SLICE + 6) / 4 / SA_BLOCK4 + 1;
+static_assert(SA_MAX_BLOCKS <= SA_THREADS, "a thread holds a block's sum");
 static_assert((((SA_MAX_SLICE + 6) / 4 / SA_THREADS + 1) | 1) <= 32, "a thread's groups of four are a mask of 128 bits");
 
 struct SaShared {
     uint32_t cnt[2][SA_BINS];
-    unsigned long long wt[2][SA_BINS];
+    uint32_t wlo[2][SA_BINS], whi[2][SA_BINS];  // sums of weights in two words
     SaItem list[2][SA_LIST];   // the boundary bin's elements: this CTA's, and all
     uint32_t cand[SA_CAP];     // a short run's elements: their indexes, rising
     uint64_t bar;
@@ -66,9 +95,10 @@ struct SaShared {
     float wmax[SA_WARPS];
     float cta_max;
     int n_list, n_own, n_ties, abort;
+    int row;
     int found_bin;
     unsigned long long found_before;
-    uint32_t found_n, cut_key;
+    uint32_t found_n, cta_n, cut_key;
     int cut_idx;
 };
 
@@ -89,6 +119,19 @@ constexpr double SA_UNIT = 1099511627776.0;  // 2^40
 // exp(z - max) in units of 2^-40: 24 bits of expf, scaled without rounding, cut to whole units
 CFI_DEV float exp_of(float z, float zmax) { return z == zmax ? 1.0f : expf(z - zmax); }
 CFI_DEV unsigned long long weight_of(float e) { return (unsigned long long)(e * (float)SA_UNIT); }
+// The same in two halves of 20 bits, by roundings to zero at 2^23: a conversion to 64 bits takes eight times as long, and a
+// thread adds a few thousand halves in 32 bits
+CFI_DEV void weight_of(float e, uint32_t* hi, uint32_t* lo) {
+    const float h = __fmaf_rz(e, 1048576.0f, 8388608.0f), rest = fmaf(e, 1048576.0f, 8388608.0f - h);
+    *hi = __float_as_uint(h) - 0x4b000000u;
+    *lo = __float_as_uint(__fmaf_rz(rest, 1048576.0f, 8388608.0f)) - 0x4b000000u;
+}
+// A sum in two words: what passes the lower one is carried.  An addition of 64 bits in shared memory is a loop that waits
+// for every other thread of its bin: 782 of one bin took 28 us, in two words 2.
+CFI_DEV void sum_add(uint32_t* lo, uint32_t* hi, unsigned long long w) {
+    const uint32_t low = (uint32_t)w, old = atomicAdd(lo, low), high = (uint32_t)(w >> 32) + (old + low < old);
+    if (high) atomicAdd(hi, high);
+}
 // max - z in units of 2^-22, 27 bits: a weight is zero from 27.8 on
 CFI_DEV uint32_t depth_of(float z, float zmax) { return z == zmax ? 0u : (uint32_t)fminf((zmax - z) * 4194304.0f, 134217727.0f); }
 
@@ -151,215 +194,67 @@ CFI_DEV unsigned long long block_incl(unsigned long long v, unsigned long long* 
     return incl + prev;
 }
 
-__global__ void __launch_bounds__(SA_THREADS, 2) sample_rows(const SaArgs a) {
-    extern __shared__ __align__(16) float slice[];
-    __shared__ SaShared s;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t rank = cluster_ctarank();
-    const int row = blockIdx.x / SA_CTAS;
-    const int base = rank * a.slice, n = max(0, min(a.slice, a.n_vocab - base));
-    if (tid == 0) {
-        mbar_init(&s.bar, 1);
-        s.abort = 0;
-        fence_mbar_init();
-    }
-    for (int b = tid; b < SA_BINS; b += SA_THREADS) {
-        s.cnt[0][b] = 0;
-        s.wt[0][b] = 0;
-    }
-    __syncthreads();
-    pdl_launch_dependents();
-    pdl_wait();
+// Element z of a logit: never -0, and -inf for a NaN
+CFI_DEV float scaled_of(float l, float div) {
+    const float v = (div == 1.0f ? l : l / div) + 0.0f;
+    return v == v ? v : -INFINITY;
+}
 
-    // ---- the one read of the row: 16-byte pieces by bulk copies, the ragged ends by loads ----
-    const float* src = a.logits + row * a.stride + base;
-    const int shift = (int)(reinterpret_cast<uintptr_t>(src) >> 2 & 3), head = min(n, (4 - shift) & 3), body = (n - head) & ~3;
-    float* z = slice + shift;  // logit i of the slice is z[i], 16-byte aligned where it is in memory
-    // the slice in groups of four: what lies before and behind it in the first and the last never counts
-    const int groups = (shift + n + 3) / 4;
-    const float4* z4 = reinterpret_cast<const float4*>(slice);
-    if (tid >= 64 && tid < 64 + shift) slice[tid - 64] = -INFINITY;
-    if (tid >= 96 && tid < 96 + 4 * groups - shift - n) z[n + tid - 96] = -INFINITY;
-    if (tid == 0 && body > 0) {
-        mbar_arrive_expect_tx(&s.bar, (uint32_t)body * 4);
-        for (int i = 0; i < body; i += 8192)
-            bulk_g2s(z + head + i, src + head + i, (uint32_t)min(8192, body - i) * 4, &s.bar);
-    }
-    if (tid < head) z[tid] = src[tid];
-    if (tid >= 32 && tid < 32 + n - head - body) z[head + body + tid - 32] = src[head + body + tid - 32];
-    const float t = a.temperature ? a.temperature[row] : 1.0f;
-    const bool greedy = t <= 0.0f;
-    const float div = greedy ? 1.0f : t;
-    int k = a.top_k ? a.top_k[row] : 0;
-    if (greedy) k = 1;
-    if (k >= a.n_vocab) k = 0;
-    const float p = a.top_p ? a.top_p[row] : 1.0f;
-    const float minp = a.min_p ? a.min_p[row] : 0.0f;
-    if (body > 0 && !mbar_wait(&s.bar, 0, &s.abort)) {
-        cfi_set_error(a.err, 0xfc100);
-        s.abort = 1;
-    }
-    __syncthreads();
-
-    // element i's z: never -0, and -inf for a NaN
-    auto scaled = [&](float l) {
-        const float v = (div == 1.0f ? l : l / div) + 0.0f;
-        return v == v ? v : -INFINITY;
-    };
-    const int run = ((n + SA_THREADS - 1) / SA_THREADS) | 1;  // each thread's run: odd, so that 32 of them meet no bank twice
-    const int r0 = min(n, tid * run), r1 = min(n, r0 + run);
-    // f(i, z[i]) for this thread's run, SA_AHEAD loads at a time
-    auto walk = [&](auto&& f) {
-        int i = r0;
-        for (; i + SA_AHEAD <= r1; i += SA_AHEAD) {
-            float v[SA_AHEAD];
-#pragma unroll
-            for (int e = 0; e < SA_AHEAD; e++) v[e] = z[i + e];
-#pragma unroll
-            for (int e = 0; e < SA_AHEAD; e++) f(i + e, v[e]);
-        }
-        for (; i < r1; i++) f(i, z[i]);
-    };
-    // f(g, z4[g]) for groups of four: g0, g0 + step, ... below g1
-    auto by_four = [&](int g0, int g1, int step, auto&& f) {
-        int g = g0;
-        for (; g + 3 * step < g1; g += 4 * step) {
-            float4 v[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = z4[g + e * step];
-#pragma unroll
-            for (int e = 0; e < 4; e++) f(g + e * step, v[e]);
-        }
-        for (; g < g1; g += step) f(g, z4[g]);
-    };
-    auto max4 = [](const float4& v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); };  // a NaN is passed over
-    float mx = -INFINITY;
-    by_four(tid, groups, SA_THREADS, [&](int, const float4& v) { mx = fmaxf(mx, max4(v)); });
-    mx = warp_max(mx);
-    if (lane == 0) s.wmax[warp] = mx;
-    __syncthreads();
-    if (warp == 0) {
-        mx = warp_max(lane < SA_WARPS ? s.wmax[lane] : -INFINITY);
-        if (lane == 0) s.cta_max = mx;
-    }
-    cluster_sync();
-    float lmax = lane < SA_CTAS ? *peer(&s.cta_max, lane) : -INFINITY;
-    lmax = warp_max(lmax);
-    const float zmax = scaled(lmax);  // division by a positive number keeps the order
-    const bool empty = zmax == -INFINITY;
-
-    // ---- no top-k: every weight counts.  Each thread sums its run; with a top-p, the top of the order by bins ----
-    unsigned long long run_sum = 0, whole = 0;
-    const float near = 1.0f / div;
-    const bool bins_hold = fabsf(zmax) < 8192.0f && near < 1e30f;  // z is exact to far less than a bin
-    if (!empty && k <= 0 && bins_hold) {
-        const bool binned = p < 1.0f;
-        const float floor = lmax - 28.0f * div * 1.0001f;  // no weight at or below this
-        auto weigh = [&](float v) {  // zmax is finite: expf(0) is 1
-            const unsigned long long w = weight_of(expf(v - zmax));
-            run_sum += w;
-            const float d = (zmax - v) * 64.0f;
-            if (binned && d < (float)SA_BINS) {
-                atomicAdd(&s.cnt[0][(int)d], 1u);
-                atomicAdd(&s.wt[0][(int)d], w);
-            }
-        };
-        if (div == 1.0f)
-            walk([&](int, float l) {
-                if (l > floor) weigh(l + 0.0f);
-            });
-        else
-            walk([&](int, float l) {
-                if (l > floor) weigh(l / div + 0.0f);
-            });
-        unsigned long long sum;
-        block_incl(run_sum, s.scan, &sum);
-        if (tid == 0) s.cta_sum = sum;
-        cluster_sync();
-#pragma unroll
-        for (uint32_t r = 0; r < SA_CTAS; r++) whole += *peer(&s.cta_sum, r);
-    }
-    uint32_t level = 1;  // histogram 0 has been used
-    // ---- a short run: down to which depth? ----
-    float floor = INFINITY;  // gather what is larger
-    if (!empty && bins_hold && (k > 0 || p < 1.0f)) {
-        // bins down to a depth of 8, or 16 where more than a few are asked for; the second turn reaches 32, where no
-        // weight is left
-        float scale = k > 8 ? 32.0f : 64.0f;
-        for (int turn = 0;; turn++) {
-            const uint32_t b = turn & 1;
-            if (k > 0) {
-                if (turn > 0) {
-                    s.cnt[b][tid] = 0;
-                    __syncthreads();
-                }
-                const float unit = near * scale, floor = lmax - (float)SA_BINS / unit * 1.0001f;
-                by_four(tid, groups, SA_THREADS, [&](int, const float4& v) {
-                    if (!(max4(v) > floor)) return;
-                    const float l[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float d = (lmax - l[e]) * unit;  // a NaN compares false
-                        if (d < (float)SA_BINS) atomicAdd(&s.cnt[b][(int)d], 1u);
-                    }
-                });
-                cluster_sync();
-            }
-            uint32_t c = 0;
-            unsigned long long m = 0;
-#pragma unroll
-            for (uint32_t r = 0; r < SA_CTAS; r++) {
-                c += *peer(&s.cnt[b][tid], r);
-                if (k <= 0) m += *peer(&s.wt[b][tid], r);
-            }
-            // the first bin whose end lies past the run's; with the next one, and one more for the rounding
-            unsigned long long all, ignore;
-            const unsigned long long upto = block_incl(c, s.scan, &all);
-            if (tid == 0) s.found_bin = SA_BINS;
-            __syncthreads();
-            if (k > 0) {
-                if (upto >= (unsigned long long)k && upto - c < (unsigned long long)k) s.found_bin = tid;
-            } else {
-                const unsigned long long w = block_incl(m, s.scan, &ignore);
-                const double limit = (double)p * (double)whole;
-                if (!((double)w < limit) && (double)(w - m) < limit) s.found_bin = tid;
-            }
-            __syncthreads();
-            const int bin = s.found_bin;
-            if (bin + 2 < SA_BINS) {
-                if (tid == bin + 2) s.found_n = (uint32_t)upto;
-                __syncthreads();
-                if (s.found_n <= SA_CAP) floor = lmax - (float)(bin + 2) / scale * div * 1.00001f;
-                __syncthreads();
-                break;
-            }
-            __syncthreads();
-            if (k <= 0 || turn == 1) {
-                // fewer than k elements have any weight: all of them are gathered
-                if (k > 0 && bin == SA_BINS && all <= SA_CAP) floor = lmax - (float)SA_BINS / scale * div * 1.00001f;
-                break;
-            }
-            scale = 16.0f;
-            level = 2;
-        }
-    }
-
-    // ---- cuts.  What stays: key > cut_key, or key == cut_key and index <= cut_idx ----
+// The cut of a row.  What stays: key > cut_key, or key == cut_key and index <= cut_idx.  `each` calls its argument
+// with z and index of this thread's elements; of `in_order`, threads and elements are in index order.
+struct SaCut {
+    SaShared& s;
+    const SaArgs& a;
+    const int row;
+    const uint32_t rank;
+    const float zmax, minp;
+    uint32_t level = 1;  // the histogram that is used next: 0 is used before the first select
     uint32_t cut_key = 0;
     int cut_idx = -1;
-    auto kept = [&](uint32_t key, int idx) { return key > cut_key || (key == cut_key && idx <= cut_idx); };
-    // Lowers the cut to the last element with less than `limit` before it: a count, or a share of the weight.
-    // `each` calls its argument with z and index of this thread's elements, threads and elements in index order.
-    // ALONE: the elements are this CTA's, at most `count`; else the whole cluster's.
-    auto select = [&](auto alone, auto&& each, int count, bool by_weight, double limit, unsigned long long all_weight) {
-        constexpr bool ALONE = decltype(alone)::value;
+
+    CFI_DEV bool kept(uint32_t key, int idx) const { return key > cut_key || (key == cut_key && idx <= cut_idx); }
+    CFI_DEV unsigned long long weight_kept(float v, int idx) const {
+        if (!kept(key_of(v), idx)) return 0;
+        const float e = exp_of(v, zmax);
+        return v == zmax || !(e < minp) ? weight_of(e) : 0;
+    }
+    template <class E> CFI_DEV unsigned long long weight_of_kept(E&& each) const {
+        unsigned long long sum = 0;
+        each([&](float v, int idx) { sum += weight_kept(v, idx); });
+        return sum;
+    }
+    // The uniform number's place among `total` units
+    CFI_DEV unsigned long long target_of(unsigned long long total) const {
+        const double ud = (double)__ldcg(a.u + row) * (double)total;
+        const unsigned long long target = ud > 0.0 ? (unsigned long long)ud : 0ull;
+        return target < total ? target : total - 1;  // u outside [0, 1)
+    }
+    CFI_DEV void drawn(float v, int idx, unsigned long long total) const {
+        a.token[row] = idx;
+        if (a.logprob) a.logprob[row] = (v == zmax ? 0.0f : v - zmax) - logf((float)((double)total / SA_UNIT));
+    }
+    // The draw: kept weights in index order.  `own`: this thread's, `ahead`: those of the threads before it.
+    template <class E> CFI_DEV void draw(E&& in_order, unsigned long long own, unsigned long long ahead, unsigned long long total) const {
+        const unsigned long long target = target_of(total);
+        if (target < ahead || target >= ahead + own) return;
+        in_order([&](float v, int idx) {
+            const unsigned long long w = weight_kept(v, idx);
+            if (ahead <= target && ahead + w > target) drawn(v, idx, total);
+            ahead += w;
+        });
+    }
+    // Lowers the cut to the last element with less than `limit` before it: a count, or a share of the weight;
+    // `before`: of what lies above all elements.  ALONE: the elements are this CTA's, at most `count`; else the
+    // whole cluster's.
+    template <bool ALONE, class E, class O>
+    CFI_DEV void select(E&& each, O&& in_order, int count, bool by_weight, double limit, unsigned long long all_weight,
+                        unsigned long long before = 0, SaPrefix pre = {}) {
+        const int tid = threadIdx.x;
         constexpr uint32_t PEERS = ALONE ? 1 : SA_CTAS;
         auto meet = [] {
             if (ALONE) __syncthreads(); else cluster_sync();
         };
         auto of = [](auto* v, uint32_t r) { return ALONE ? (const std::remove_pointer_t<decltype(v)>*)v : peer(v, r); };
-        SaPrefix pre;
-        unsigned long long before = 0;
         uint32_t in_bin = (uint32_t)count;
         if (by_weight && all_weight > 0) limit *= (double)all_weight;
         bool scaled_limit = !by_weight || all_weight > 0;
@@ -367,7 +262,8 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows(const SaArgs a) {
             if (!ALONE || in_bin > SA_LIST) {
                 const uint32_t b = level++ & 1;
                 s.cnt[b][tid] = 0;
-                s.wt[b][tid] = 0;
+                s.wlo[b][tid] = 0;
+                s.whi[b][tid] = 0;
                 if (tid == 0) s.found_bin = -1;
                 __syncthreads();
                 each([&](float v, int idx) {
@@ -377,7 +273,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows(const SaArgs a) {
                     const unsigned long long w = weight_of(exp_of(v, zmax));
                     if (w == 0) return;
                     atomicAdd(&s.cnt[b][bin], 1u);
-                    if (by_weight) atomicAdd(&s.wt[b][bin], w);
+                    if (by_weight) sum_add(&s.wlo[b][bin], &s.whi[b][bin], w);
                 });
                 meet();
                 uint32_t c = 0;
@@ -385,7 +281,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows(const SaArgs a) {
 #pragma unroll
                 for (uint32_t r = 0; r < PEERS; r++) {
                     c += *of(&s.cnt[b][tid], r);
-                    if (by_weight) m += *of(&s.wt[b][tid], r);
+                    if (by_weight) m += (unsigned long long)*of(&s.whi[b][tid], r) << 32 | *of(&s.wlo[b][tid], r);
                 }
                 if (!by_weight) m = c;
                 unsigned long long total;
@@ -460,7 +356,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows(const SaArgs a) {
             if (pre.stage == 7) {  // equal elements: each has the same weight, the index decides
                 const uint32_t eq = ~pre.key;
                 unsigned long long mine = 0, ties;
-                each([&](float v, int idx) { mine += (unsigned long long)(key_of(v) == eq && kept(eq, idx)); });
+                in_order([&](float v, int idx) { mine += (unsigned long long)(key_of(v) == eq && kept(eq, idx)); });
                 unsigned long long ahead = block_incl(mine, s.scan, &ties) - mine;
                 if (tid == 0) s.n_ties = (int)ties;
                 meet();
@@ -478,7 +374,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows(const SaArgs a) {
                         hi = mid - 1;
                 }
                 if (lo >= ahead && lo < ahead + mine)
-                    each([&](float v, int idx) {
+                    in_order([&](float v, int idx) {
                         if (key_of(v) != eq || !kept(eq, idx)) return;
                         if (ahead++ == lo)
                             for (uint32_t r = 0; r < PEERS; r++) *const_cast<int*>(of(&s.cut_idx, r)) = idx;
@@ -489,35 +385,246 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows(const SaArgs a) {
                 return;
             }
         }
-    };
-    // The draw: kept weights in index order.  `ahead`: what the CTAs before this one have.
-    auto draw = [&](auto&& each, unsigned long long own, unsigned long long ahead, unsigned long long total) {
-        const double ud = (double)a.u[row] * (double)total;
-        unsigned long long target = ud > 0.0 ? (unsigned long long)ud : 0ull;
-        if (target >= total) target = total - 1;  // u outside [0, 1)
-        if (target < ahead || target >= ahead + own) return;
-        each([&](float v, int idx) {
-            if (!kept(key_of(v), idx)) return;
-            const float e = exp_of(v, zmax);
-            if (v != zmax && e < minp) return;
-            const unsigned long long w = weight_of(e);
-            if (ahead <= target && ahead + w > target) {
-                a.token[row] = idx;
-                if (a.logprob) a.logprob[row] = (v == zmax ? 0.0f : v - zmax) - logf((float)((double)total / SA_UNIT));
-            }
-            ahead += w;
-        });
-    };
-    auto weight_of_kept = [&](auto&& each) {
-        unsigned long long sum = 0;
-        each([&](float v, int idx) {
-            if (!kept(key_of(v), idx)) return;
-            const float e = exp_of(v, zmax);
-            if (v == zmax || !(e < minp)) sum += weight_of(e);
-        });
-        return sum;
-    };
+    }
+};
 
+// Elements in the registers of one CTA, a thread's in index order: those whose indexes s.cand holds, rising.
+struct SaHeld {
+    float v[SA_EACH];
+    int idx[SA_EACH];
+    CFI_DEV SaHeld(const SaCut& cut, int nc, float div) {
+        const int each_n = (nc + SA_THREADS - 1) / SA_THREADS;
+#pragma unroll
+        for (int e = 0; e < SA_EACH; e++) {
+            const int x = threadIdx.x * each_n + e;
+            idx[e] = e < each_n && x < nc ? (int)cut.s.cand[x] : -1;
+            v[e] = idx[e] >= 0 ? scaled_of(__ldcg(cut.a.logits + cut.row * cut.a.stride + idx[e]), div) : -INFINITY;
+        }
+    }
+    template <class F> CFI_DEV void operator()(F&& f) const {
+#pragma unroll
+        for (int e = 0; e < SA_EACH; e++)
+            if (idx[e] >= 0) f(v[e], idx[e]);
+    }
+};
+
+// The cut among those of the nc elements of s.cand that are in(z), which have `before` units above them.
+template <class F> CFI_DEV void rank_edge(SaCut& cut, int nc, float div, double limit, unsigned long long before, int bin, F&& in) {
+    SaHeld each(cut, nc, div);
+#pragma unroll
+    for (int e = 0; e < SA_EACH; e++)
+        if (!in(each.v[e])) each.idx[e] = -1;
+    // a bin of 1/32 lies in one of the first histogram's
+    SaPrefix pre;
+    pre.take((uint32_t)bin >> 1);
+    cut.select<true>(each, each, nc, true, limit, 1ull, before, pre);
+}
+
+// A short run, alone: s.cand holds the indexes of nc elements, rising, with all that can stay among them.  `whole`: the weight
+// that a top-p is a share of, 0 where it is that of these elements as the top-k leaves them.
+CFI_DEV void finish_short(SaCut& cut, int nc, float div, int k, float p, unsigned long long whole) {
+    const SaHeld each(cut, nc, div);
+    if (k > 0 && k < nc) cut.select<true>(each, each, nc, false, (double)k, 0ull);
+    if (p < 1.0f) {
+        unsigned long long among = whole;
+        if (among == 0) {
+            unsigned long long sum = 0;
+            each([&](float x, int i) {
+                if (cut.kept(key_of(x), i)) sum += weight_of(exp_of(x, cut.zmax));
+            });
+            block_incl(sum, cut.s.scan, &among);
+        }
+        cut.select<true>(each, each, nc, true, (double)p, among);
+    }
+    const unsigned long long sum = cut.weight_of_kept(each);
+    unsigned long long total;
+    const unsigned long long upto = block_incl(sum, cut.s.scan, &total);
+    cut.draw(each, sum, upto - sum, total);
+}
+
+// One row, by a cluster: this CTA has the n logits from `base`.
+CFI_DEV void sample_row(const SaArgs& a, SaShared& s, float* slice, uint32_t rank, int row) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int base = rank * a.slice, n = max(0, min(a.slice, a.n_vocab - base));
+
+    // ---- the one read of the row: 16-byte pieces by bulk copies, the ragged ends by loads ----
+    const float* src = a.logits + row * a.stride + base;
+    const int shift = (int)(reinterpret_cast<uintptr_t>(src) >> 2 & 3), head = min(n, (4 - shift) & 3), body = (n - head) & ~3;
+    float* z = slice + shift;  // logit i of the slice is z[i], 16-byte aligned where it is in memory
+    // the slice in groups of four: what lies before and behind it in the first and the last never counts
+    const int groups = (shift + n + 3) / 4;
+    const float4* z4 = reinterpret_cast<const float4*>(slice);
+    if (tid >= 64 && tid < 64 + shift) slice[tid - 64] = -INFINITY;
+    if (tid >= 96 && tid < 96 + 4 * groups - shift - n) z[n + tid - 96] = -INFINITY;
+    if (tid == 0 && body > 0) {
+        mbar_arrive_expect_tx(&s.bar, (uint32_t)body * 4);
+        for (int i = 0; i < body; i += 8192)
+            bulk_g2s(z + head + i, src + head + i, (uint32_t)min(8192, body - i) * 4, &s.bar);
+    }
+    if (tid < head) z[tid] = __ldcg(src + tid);
+    if (tid >= 32 && tid < 32 + n - head - body) z[head + body + tid - 32] = __ldcg(src + head + body + tid - 32);
+    const SaRow par(a, row);
+    const float div = par.div, p = par.p, minp = par.minp;
+    const int k = par.k;
+    if (body > 0 && !mbar_wait(&s.bar, 0, &s.abort)) {
+        cfi_set_error(a.err, 0xfc100);
+        s.abort = 1;
+    }
+    __syncthreads();
+
+    auto scaled = [&](float l) { return scaled_of(l, div); };
+    const int run = ((n + SA_THREADS - 1) / SA_THREADS) | 1;  // each thread's run: odd, so that 32 of them meet no bank twice
+    const int r0 = min(n, tid * run), r1 = min(n, r0 + run);
+    // f(i, z[i]) for this thread's run, SA_AHEAD loads at a time
+    auto walk = [&](auto&& f) {
+        int i = r0;
+        for (; i + SA_AHEAD <= r1; i += SA_AHEAD) {
+            float v[SA_AHEAD];
+#pragma unroll
+            for (int e = 0; e < SA_AHEAD; e++) v[e] = z[i + e];
+#pragma unroll
+            for (int e = 0; e < SA_AHEAD; e++) f(i + e, v[e]);
+        }
+        for (; i < r1; i++) f(i, z[i]);
+    };
+    // f(g, z4[g]) for groups of four: g0, g0 + step, ... below g1
+    auto by_four = [&](int g0, int g1, int step, auto&& f) {
+        int g = g0;
+        for (; g + 3 * step < g1; g += 4 * step) {
+            float4 v[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = z4[g + e * step];
+#pragma unroll
+            for (int e = 0; e < 4; e++) f(g + e * step, v[e]);
+        }
+        for (; g < g1; g += step) f(g, z4[g]);
+    };
+    auto max4 = [](const float4& v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); };  // a NaN is passed over
+    float mx = -INFINITY;
+    by_four(tid, groups, SA_THREADS, [&](int, const float4& v) { mx = fmaxf(mx, max4(v)); });
+    mx = warp_max(mx);
+    if (lane == 0) s.wmax[warp] = mx;
+    __syncthreads();
+    if (warp == 0) {
+        mx = warp_max(lane < SA_WARPS ? s.wmax[lane] : -INFINITY);
+        if (lane == 0) s.cta_max = mx;
+    }
+    cluster_sync();
+    float lmax = lane < SA_CTAS ? *peer(&s.cta_max, lane) : -INFINITY;
+    lmax = warp_max(lmax);
+    const float zmax = scaled(lmax);  // division by a positive number keeps the order
+    const bool empty = zmax == -INFINITY;
+
+    // ---- no top-k: every weight counts.  Each thread sums its run; with a top-p, the top of the order by bins ----
+    unsigned long long run_sum = 0, whole = 0;
+    const float near = 1.0f / div;
+    const bool bins_hold = fabsf(zmax) < 8192.0f && near < 1e30f;  // z is exact to far less than a bin
+    if (!empty && k <= 0 && bins_hold) {
+        const bool binned = p < 1.0f;
+        const float floor = lmax - 28.0f * div * 1.0001f;  // no weight at or below this
+        auto weigh = [&](float v) {  // zmax is finite: expf(0) is 1
+            const unsigned long long w = weight_of(expf(v - zmax));
+            run_sum += w;
+            const float d = (zmax - v) * 32.0f;
+            if (binned && d < (float)SA_BINS) {
+                atomicAdd(&s.cnt[0][(int)d], 1u);
+                sum_add(&s.wlo[0][(int)d], &s.whi[0][(int)d], w);
+            }
+        };
+        if (div == 1.0f)
+            walk([&](int, float l) {
+                if (l > floor) weigh(l + 0.0f);
+            });
+        else
+            walk([&](int, float l) {
+                if (l > floor) weigh(l / div + 0.0f);
+            });
+        unsigned long long sum;
+        block_incl(run_sum, s.scan, &sum);
+        if (tid == 0) s.cta_sum = sum;
+        cluster_sync();
+#pragma unroll
+        for (uint32_t r = 0; r < SA_CTAS; r++) whole += *peer(&s.cta_sum, r);
+    }
+    uint32_t level = 1;  // histogram 0 has been used
+    // ---- a short run: down to which depth? ----
+    float floor = INFINITY, top = INFINITY;  // gather what is larger than the one and not than the other
+    int edge = -1;                          // or a long run's end: the bin that it lies in
+    double limit = 0.0;
+    if (!empty && bins_hold && (k > 0 || p < 1.0f)) {
+        // bins down to a depth of 8, or 16 where more than a few are asked for; the second turn reaches 32, where no
+        // weight is left
+        float scale = k > 8 || k <= 0 ? 32.0f : 64.0f;
+        for (int turn = 0;; turn++) {
+            const uint32_t b = turn & 1;
+            if (k > 0) {
+                if (turn > 0) {
+                    s.cnt[b][tid] = 0;
+                    __syncthreads();
+                }
+                const float unit = near * scale, floor = lmax - (float)SA_BINS / unit * 1.0001f;
+                by_four(tid, groups, SA_THREADS, [&](int, const float4& v) {
+                    if (!(max4(v) > floor)) return;
+                    const float l[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float d = (lmax - l[e]) * unit;  // a NaN compares false
+                        if (d < (float)SA_BINS) atomicAdd(&s.cnt[b][(int)d], 1u);
+                    }
+                });
+                cluster_sync();
+            }
+            uint32_t c = 0;
+            unsigned long long m = 0;
+#pragma unroll
+            for (uint32_t r = 0; r < SA_CTAS; r++) {
+                c += *peer(&s.cnt[b][tid], r);
+                if (k <= 0) m += (unsigned long long)*peer(&s.whi[b][tid], r) << 32 | *peer(&s.wlo[b][tid], r);
+            }
+            // the first bin whose end lies past the run's; with the next one, and one more for the rounding
+            unsigned long long all, ignore;
+            const unsigned long long upto = block_incl(c, s.scan, &all);
+            if (tid == 0) s.found_bin = SA_BINS;
+            __syncthreads();
+            if (k > 0) {
+                if (upto >= (unsigned long long)k && upto - c < (unsigned long long)k) s.found_bin = tid;
+            } else {
+                const unsigned long long w = block_incl(m, s.scan, &ignore);
+                limit = fmax((double)p * (double)whole, 0.5);  // the largest always stays
+                if (!((double)w < limit) && (double)(w - m) < limit) {
+                    s.found_bin = tid;
+                    s.found_before = w - m;
+                    s.cta_n = c;
+                }
+            }
+            __syncthreads();
+            const int bin = s.found_bin;
+            if (bin + 2 < SA_BINS) {
+                if (tid == bin + 2) s.found_n = (uint32_t)upto;
+                __syncthreads();
+                if (s.found_n <= SA_CAP) {
+                    floor = lmax - (float)(bin + 2) / scale * div * 1.00001f;
+                } else if (k <= 0 && s.cta_n <= SA_CAP / 2) {
+                    edge = bin;  // a bin and the rounding on both sides
+                    floor = lmax - ((float)bin + 1.1f) / scale * div * 1.00001f;
+                    if (bin > 0) top = lmax - ((float)bin - 0.1f) / scale * div * 0.99999f;
+                }
+                __syncthreads();
+                break;
+            }
+            __syncthreads();
+            if (k <= 0 || turn == 1) {
+                // fewer than k elements have any weight: all of them are gathered
+                if (k > 0 && bin == SA_BINS && all <= SA_CAP) floor = lmax - (float)SA_BINS / scale * div * 1.00001f;
+                break;
+            }
+            scale = 16.0f;
+            level = 2;
+        }
+    }
+
+    SaCut cut = {s, a, row, rank, zmax, minp, level};
+    bool ranked = false;
     int nc = SA_CAP + 1;
     if (floor < INFINITY) {
         // ---- a short run: gathered in index order by the first CTA, which goes on alone ----
@@ -526,7 +633,8 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows(const SaArgs a) {
         unsigned long long hit[2] = {0, 0};
         by_four(g0, g1, 1, [&](int g, const float4& v) {
             if (!(max4(v) > floor)) return;
-            const unsigned long long bits = (v.x > floor) | (v.y > floor) << 1 | (v.z > floor) << 2 | (v.w > floor) << 3;
+            auto in = [&](float l) { return (unsigned long long)(l > floor && l <= top); };
+            const unsigned long long bits = in(v.x) | in(v.y) << 1 | in(v.z) << 2 | in(v.w) << 3;
             if (g - g0 < 16) hit[0] |= bits << 4 * (g - g0); else hit[1] |= bits << 4 * (g - g0 - 16);
         });
         const int mine = __popcll(hit[0]) + __popcll(hit[1]);
@@ -551,38 +659,21 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows(const SaArgs a) {
     }
     if (nc <= SA_CAP) {
         cluster_sync();
-        if (rank != 0) return;
-        float v[SA_EACH];
-        int idx[SA_EACH];
-        const int each_n = (nc + SA_THREADS - 1) / SA_THREADS;  // a thread's elements, in index order
-#pragma unroll
-        for (int e = 0; e < SA_EACH; e++) {
-            const int x = tid * each_n + e;
-            idx[e] = e < each_n && x < nc ? (int)s.cand[x] : -1;
-            v[e] = idx[e] >= 0 ? scaled(a.logits[row * a.stride + idx[e]]) : -INFINITY;
+        if (edge < 0) {
+            if (rank == 0) finish_short(cut, nc, div, k, p, whole);
+            return;
         }
-        auto each = [&](auto&& f) {
-#pragma unroll
-            for (int e = 0; e < SA_EACH; e++)
-                if (idx[e] >= 0) f(v[e], idx[e]);
-        };
-        if (k > 0 && k < nc) select(std::true_type{}, each, nc, false, (double)k, 0ull);
-        if (p < 1.0f) {
-            unsigned long long among = whole;
-            if (k > 0) {
-                unsigned long long sum = 0;
-                each([&](float x, int i) {
-                    if (kept(key_of(x), i)) sum += weight_of(exp_of(x, zmax));
-                });
-                block_incl(sum, s.scan, &among);
+        if (rank == 0) {
+            rank_edge(cut, nc, div, limit, s.found_before, edge, [&](float v) { return (int)((zmax - v) * 32.0f) == edge; });
+            if (tid == 0) {
+                s.cut_key = cut.cut_key;
+                s.cut_idx = cut.cut_idx;
             }
-            select(std::true_type{}, each, nc, true, (double)p, among);
         }
-        const unsigned long long sum = weight_of_kept(each);
-        unsigned long long total;
-        const unsigned long long upto = block_incl(sum, s.scan, &total);
-        draw(each, sum, upto - sum, total);
-        return;
+        cluster_sync();
+        cut.cut_key = *peer(&s.cut_key, 0);
+        cut.cut_idx = *peer(&s.cut_idx, 0);
+        ranked = true;
     }
 
     // ---- a long run, or no filter: z in place of the logits ----
@@ -590,9 +681,9 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows(const SaArgs a) {
     __syncthreads();
     auto each = [&](auto&& f) { walk([&](int i, float v) { f(v, base + i); }); };
     if (!empty) {
-        if (k > 0) select(std::false_type{}, each, a.n_vocab, false, (double)k, 0ull);
-        if (p < 1.0f) select(std::false_type{}, each, a.n_vocab, true, (double)p, 0ull);
-        if (k > 0 || p < 1.0f || minp > 0.0f || !bins_hold) run_sum = weight_of_kept(each);
+        if (k > 0) cut.select<false>(each, each, a.n_vocab, false, (double)k, 0ull);
+        if (p < 1.0f && !ranked) cut.select<false>(each, each, a.n_vocab, true, (double)p, 0ull);
+        if (k > 0 || p < 1.0f || minp > 0.0f || !bins_hold) run_sum = cut.weight_of_kept(each);
     }
     unsigned long long sum;
     const unsigned long long upto = block_incl(run_sum, s.scan, &sum);
@@ -606,12 +697,497 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows(const SaArgs a) {
         total += x;
     }
     if (total > 0) {
-        draw(each, run_sum, ahead + upto - run_sum, total);
+        cut.draw(each, run_sum, ahead + upto - run_sum, total);
     } else if (rank == 0 && tid == 0) {
         a.token[row] = -1;
         if (a.logprob) a.logprob[row] = -INFINITY;
     }
     cluster_sync();  // no CTA leaves while another may read its shared memory
+}
+
+// Which is the row with `wanted` whole() ones before it?  -1: none; `count`: how many there are in all, as far as it was
+// looked for.
+CFI_DEV int whole_row(const SaArgs& a, SaShared& s, int wanted, int* count) {
+    const int tid = threadIdx.x;
+    if (tid == 0) s.row = -1;
+    int before = 0;
+    for (int first = 0; first < a.n_rows && before <= max(wanted, a.spare); first += SA_THREADS) {
+        const bool mine = first + tid < a.n_rows && SaRow(a, first + tid).whole(a.n_vocab);
+        unsigned long long here;
+        const int upto = before + (int)block_incl(mine, s.scan, &here);
+        if (mine && upto - 1 == wanted) s.row = first + tid;
+        before += (int)here;
+    }
+    __syncthreads();
+    *count = before;
+    return s.row;
+}
+
+// SPARE: behind stream_rows, cluster i takes the i-th of the whole() rows where they are few.
+template <bool SPARE> __global__ void __launch_bounds__(SA_THREADS, 2) sample_rows(const SaArgs a) {
+    extern __shared__ __align__(16) float slice[];
+    __shared__ SaShared s;
+    const int tid = threadIdx.x;
+    if (tid == 0) {
+        mbar_init(&s.bar, 1);
+        s.abort = 0;
+        fence_mbar_init();
+    }
+    s.cnt[0][tid] = 0;
+    s.wlo[0][tid] = 0;
+    s.whi[0][tid] = 0;
+    __syncthreads();
+    pdl_launch_dependents();
+    if (!SPARE) {
+        pdl_wait();
+        sample_row(a, s, slice, cluster_ctarank(), blockIdx.x / SA_CTAS);
+        return;
+    }
+    // stream_rows lets this kernel start after its own wait: what that waited for is complete, and is read past L1.
+    // The end waits for stream_rows itself, so that the next kernel's wait is for both.
+    int count;
+    const int row = whole_row(a, s, blockIdx.x / SA_CTAS, &count);
+    if (row >= 0 && count <= a.spare) sample_row(a, s, slice, cluster_ctarank(), row);
+    pdl_wait();
+}
+
+// l / T in three forms.  The second, for ordinary T and l only, is Markstein's (Computation of elementary functions on the IBM RISC
+// System/6000, 1990): from the reciprocal rounded to nearest, corrections by the exact remainder end at
+// the quotient rounded to nearest, the first within an ulp of it.  The same value as the division's, without its branch.
+struct SaByOne {
+    CFI_DEV float operator()(float l) const { return l; }
+};
+struct SaByDivision {
+    float t;
+    CFI_DEV float operator()(float l) const { return l / t; }
+};
+struct SaByReciprocal {
+    float t, r;
+    CFI_DEV float operator()(float l) const {
+        const float q0 = l * r, q1 = fmaf(fmaf(-q0, t, l), r, q0);
+        return fmaf(fmaf(-q1, t, l), r, q1);
+    }
+};
+
+// ---- many rows: a CTA takes one ----
+// The row is streamed past registers, and of each group of 32 logits the largest is kept.  A block is 1024 logits,
+// and a lane's eight float4 of it, 128 logits apart, are its group: no lane waits for another.  The group maxima say
+// almost all: the row's maximum; a depth that k elements reach at least, namely k groups' largest; and where the few
+// elements above a depth are, so that only their groups are read again.
+struct SaStream {
+    const float4* z4;  // logit i is element shift + i
+    int shift, n, groups, blocks;
+
+    CFI_DEV int index(int b, int j, int lane, int c) const { return 4 * (SA_BLOCK4 * b + 32 * j + lane) + c - shift; }
+    // the row's first and last float4 hold what is not the row's: it is not read
+    CFI_DEV float4 edge(int g) const {
+        float v[4];
+        const float* z = reinterpret_cast<const float*>(z4);
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            const int i = 4 * g + c;
+            v[c] = i >= shift && i < shift + n ? __ldcg(z + i) : -INFINITY;
+        }
+        return make_float4(v[0], v[1], v[2], v[3]);
+    }
+    CFI_DEV bool inner(int b) const { return b > 0 && SA_BLOCK4 * (b + 1) < groups; }
+    CFI_DEV float4 at(int b, int j, int lane) const {
+        const int g = SA_BLOCK4 * b + 32 * j + lane;
+        return g > 0 && g < groups - 1 ? __ldcg(z4 + g) : edge(g);
+    }
+    // four float4 of a lane, in eights
+    static CFI_DEV constexpr int step(int e) { return 128 * (e / 4) + e % 4; }
+    CFI_DEV void load(int b, int j0, int lane, float (&l)[2][8]) const {
+        float4 v[4];
+        if (inner(b)) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = __ldcg(z4 + SA_BLOCK4 * b + 32 * (j0 + j) + lane);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = at(b, j0 + j, lane);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            l[j / 2][j % 2 * 4] = v[j].x;
+            l[j / 2][j % 2 * 4 + 1] = v[j].y;
+            l[j / 2][j % 2 * 4 + 2] = v[j].z;
+            l[j / 2][j % 2 * 4 + 3] = v[j].w;
+        }
+    }
+    CFI_DEV void load(int b, int lane, float4 (&v)[8]) const {
+        if (inner(b)) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = __ldcg(z4 + SA_BLOCK4 * b + 32 * j + lane);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = at(b, j, lane);
+        }
+    }
+};
+
+CFI_DEV float max_of(const float4& v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }  // a NaN is passed over
+
+// One row, by this CTA alone.
+CFI_DEV void stream_row(const SaArgs& a, SaShared& s, float* slice, int row) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const SaRow par(a, row);
+    if (a.spare > 0 && par.whole(a.n_vocab)) {
+        int count;
+        whole_row(a, s, 0, &count);
+        if (count <= a.spare) return;
+    }
+    const float div = par.div, p = par.p, minp = par.minp;
+    const int k = par.k;
+    s.cnt[0][tid] = 0;
+    s.cnt[1][tid] = 0;
+    s.wlo[0][tid] = 0;
+    s.whi[0][tid] = 0;
+    const float* src = a.logits + row * a.stride;
+    SaStream in;
+    in.shift = (int)(reinterpret_cast<uintptr_t>(src) >> 2 & 3);
+    in.z4 = reinterpret_cast<const float4*>(src - in.shift);
+    in.n = a.n_vocab;
+    in.groups = (in.shift + in.n + 3) / 4;
+    in.blocks = (in.groups + SA_BLOCK4 - 1) / SA_BLOCK4;
+    unsigned long long* part = reinterpret_cast<unsigned long long*>(slice);  // of each block, what is summed or counted
+    float* gm = slice + 2 * in.blocks;                                        // of each group, the largest,
+    uint32_t* hits = reinterpret_cast<uint32_t*>(gm + 32 * in.blocks);        // and which are gathered
+
+    // ---- the read from memory ----
+    float mx = -INFINITY;
+    for (int b = warp; b < in.blocks; b += SA_WARPS) {
+        float4 v[8];
+        in.load(b, lane, v);
+        float m = max_of(v[0]);
+#pragma unroll
+        for (int j = 1; j < 8; j++) m = fmaxf(m, max_of(v[j]));
+        m = fmaxf(m, -INFINITY);  // NaN in all of them
+        gm[32 * b + lane] = m;
+        mx = fmaxf(mx, m);
+    }
+    mx = warp_max(mx);
+    if (lane == 0) s.wmax[warp] = mx;
+    __syncthreads();
+    const float lmax = warp_max(lane < SA_WARPS ? s.wmax[lane] : -INFINITY);
+    const float zmax = scaled_of(lmax, div);
+    if (zmax == -INFINITY) {
+        if (tid == 0) {
+            a.token[row] = -1;
+            if (a.logprob) a.logprob[row] = -INFINITY;
+        }
+        return;
+    }
+    const float near = 1.0f / div;
+    const bool bins_hold = fabsf(zmax) < 8192.0f && near < 1e30f;
+    const float nothing = bins_hold ? lmax - 28.0f * div * 1.0001f : -INFINITY;  // no weight at or below this
+    const bool few = a.n_vocab <= SA_CAP;
+    SaCut cut = {s, a, row, 0, zmax, minp};
+
+    // f(divided by, eight logits, first) for this thread's elements of groups that reach above `floor`, the e-th with index
+    // first + SaStream::step(e), and g(block) after each block
+    const bool ordinary = bins_hold && div > 0x1p-60f && div < 0x1p60f;
+    auto walk = [&](float floor, auto&& f, auto&& g) {
+        for (int b = warp; b < in.blocks; b += SA_WARPS) {
+            if (gm[32 * b + lane] > floor) {
+#pragma unroll 1
+                for (int j0 = 0; j0 < 8; j0 += 4) {
+                    float l[2][8];
+                    in.load(b, j0, lane, l);
+                    const int first = in.index(b, j0, lane, 0);
+                    if (div == 1.0f) {
+                        f(SaByOne{}, l[0], first);
+                        f(SaByOne{}, l[1], first + 256);
+                        continue;
+                    }
+                    float least_abs = INFINITY;
+#pragma unroll
+                    for (int e = 0; e < 16; e++) least_abs = fminf(least_abs, fabsf(l[e / 8][e % 8]));
+                    if (ordinary && least_abs > 0x1p-60f) {
+                        const SaByReciprocal by = {div, near};
+                        f(by, l[0], first);
+                        f(by, l[1], first + 256);
+                    } else {
+                        f(SaByDivision{div}, l[0], first);
+                        f(SaByDivision{div}, l[1], first + 256);
+                    }
+                }
+            }
+            g(b);
+        }
+    };
+    // f(value, index) for this thread's elements that have weight, in no order
+    auto each = [&](auto&& f) {
+        for (int b = warp; b < in.blocks; b += SA_WARPS)
+            if (gm[32 * b + lane] > nothing)
+#pragma unroll 1
+                for (int j0 = 0; j0 < 8; j0 += 4) {
+                    float l[2][8];
+                    in.load(b, j0, lane, l);
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        if (l[e / 8][e % 8] > nothing)
+                            f(scaled_of(l[e / 8][e % 8], div), in.index(b, j0, lane, 0) + 256 * (e / 8) + SaStream::step(e % 8));
+                }
+    };
+    const int run = (a.n_vocab + SA_THREADS - 1) / SA_THREADS, r0 = min(a.n_vocab, tid * run), r1 = min(a.n_vocab, r0 + run);
+    auto in_order = [&](auto&& f) {
+        for (int i = r0; i < r1; i++) f(scaled_of(__ldcg(src + i), div), i);
+    };
+    // The elements above `floor` and up to `top` to s.cand in index order; how many.
+    auto gather = [&](float floor, float top) {
+        if (tid == 0) s.n_list = 0;
+        __syncthreads();
+        for (int i = tid; i < 32 * in.blocks; i += SA_THREADS) {
+            hits[i] = 0;
+            if (gm[i] > floor) {
+                const int at = atomicAdd(&s.n_list, 1);
+                if (at < SA_CAP) s.cand[at] = (uint32_t)i;
+            }
+        }
+        __syncthreads();
+        const int listed = s.n_list;
+        if (listed > SA_CAP && top == INFINITY) return SA_CAP + 1;
+        auto look = [&](int i) {  // a thread a group: its eight loads are in flight together
+            float4 v[8];
+            in.load(i >> 5, i & 31, v);
+            uint32_t mask = 0;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float l[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+                for (int c = 0; c < 4; c++) mask |= (uint32_t)(l[c] > floor && l[c] <= top) << (4 * j + c);
+            }
+            hits[i] = mask;
+        };
+        if (listed <= SA_CAP) {
+            for (int x = tid; x < listed; x += SA_THREADS) look((int)s.cand[x]);
+        } else {
+            for (int i = tid; i < 32 * in.blocks; i += SA_THREADS)
+                if (gm[i] > floor) look(i);
+        }
+        __syncthreads();
+        for (int b = warp; b < in.blocks; b += SA_WARPS) {
+            const uint32_t count = __reduce_add_sync(0xffffffffu, __popc(hits[32 * b + lane]));
+            if (lane == 0) part[b] = count;
+        }
+        __syncthreads();
+        unsigned long long all;
+        const unsigned long long mine = tid < in.blocks ? part[tid] : 0, upto = block_incl(mine, s.scan, &all);
+        if (tid < in.blocks) part[tid] = upto - mine;
+        __syncthreads();
+        if (all > SA_CAP) return SA_CAP + 1;
+        for (int b = warp; b < in.blocks; b += SA_WARPS) {
+            const uint32_t mask = hits[32 * b + lane];
+            if (!__any_sync(0xffffffffu, mask)) continue;
+            int at = (int)part[b];
+#pragma unroll 1
+            for (int j = 0; j < 8; j++) {
+                const uint32_t four = mask >> (4 * j) & 15u;
+                if (!__any_sync(0xffffffffu, four)) continue;
+                int below = 0, all_four = 0;
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const uint32_t lanes = __ballot_sync(0xffffffffu, four >> c & 1u);
+                    below += __popc(lanes & ((1u << lane) - 1u));
+                    all_four += __popc(lanes);
+                }
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+                    if (four >> c & 1u) s.cand[at + below++] = (uint32_t)in.index(b, j, lane, c);
+                at += all_four;
+            }
+        }
+        __syncthreads();
+        return (int)all;
+    };
+
+    // ---- a short run: all elements that can stay, in s.cand ----
+    int nc = SA_CAP + 1;
+    bool decided = k == 0 && !(p < 1.0f);  // the cut is known
+    float least = nothing;                 // nothing stays at or below this
+    if (few && (k > 0 || p < 1.0f)) {
+        nc = gather(-INFINITY, INFINITY);
+    } else if (bins_hold && k > 0) {
+        // bins down to a depth of 8, or 16 where more than a few are asked for; the second turn reaches 32
+        for (int turn = 0; turn < 2; turn++) {
+            const float unit = near * (turn ? 16.0f : k > 8 ? 32.0f : 64.0f), window = lmax - (float)SA_BINS / unit * 1.0001f;
+            if (turn) {
+                __syncthreads();
+                s.cnt[0][tid] = 0;
+                s.cnt[1][tid] = 0;
+            }
+            if (tid == 0) s.found_bin = SA_BINS;
+            __syncthreads();
+            auto bin = [&](float l, uint32_t* into) {
+                const float d = (lmax - l) * unit;  // a NaN compares false
+                if (d < (float)SA_BINS) atomicAdd(into + (int)d, 1u);
+            };
+            for (int i = tid; i < 32 * in.blocks; i += SA_THREADS)
+                if (gm[i] > window) bin(gm[i], s.cnt[0]);
+            __syncthreads();
+            // the bin in which the k-th largest group maximum lies: the k-th element is no deeper
+            const uint32_t g = s.cnt[0][tid];
+            unsigned long long all, upto = block_incl(g, s.scan, &all);
+            if (upto >= (unsigned long long)k && upto - g < (unsigned long long)k) s.found_bin = tid;
+            __syncthreads();
+            const int reach = s.found_bin + 2;  // one bin more for the rounding
+            if (reach < SA_BINS) {
+                nc = gather(lmax - (float)reach / unit * 1.00001f, INFINITY);
+                if (nc <= SA_CAP) break;
+            }
+            // too many, or fewer such groups: the elements themselves are counted
+            __syncthreads();
+            if (tid == 0) s.found_bin = SA_BINS;
+            const float floor = reach + 2 < SA_BINS ? lmax - (float)(reach + 2) / unit * 1.0001f : window;
+            for (int b = warp; b < in.blocks; b += SA_WARPS)
+                if (gm[32 * b + lane] > floor) {
+                    float4 v[8];
+                    in.load(b, lane, v);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        if (v[j].x > floor) bin(v[j].x, s.cnt[1]);
+                        if (v[j].y > floor) bin(v[j].y, s.cnt[1]);
+                        if (v[j].z > floor) bin(v[j].z, s.cnt[1]);
+                        if (v[j].w > floor) bin(v[j].w, s.cnt[1]);
+                    }
+                }
+            __syncthreads();
+            const uint32_t c = s.cnt[1][tid];
+            upto = block_incl(c, s.scan, &all);
+            if (upto >= (unsigned long long)k && upto - c < (unsigned long long)k) s.found_bin = tid;
+            __syncthreads();
+            const int found = s.found_bin;
+            if (found + 2 < SA_BINS) {
+                nc = gather(lmax - (float)(found + 2) / unit * 1.00001f, INFINITY);
+                break;
+            }
+            if (turn == 1 && all <= SA_CAP) nc = gather(window, INFINITY);  // fewer than k have any weight
+        }
+    } else if (bins_hold && p < 1.0f) {
+        // the whole sum, and the weights by bins of 1/32 down to a depth of 16: what lies deeper is a small share of the
+        // largest's weight for each 1e5 elements
+        uint32_t hi = 0, lo = 0;
+        auto depth_bin = [&](float v) { return (zmax - v) * 32.0f; };
+        walk(nothing, [&](auto by, const float (&l)[8], int) {
+            float d[8];
+            uint32_t h[8], w[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float v = by(l[e]) + 0.0f;
+                d[e] = depth_bin(v);
+                weight_of(l[e] > nothing ? expf(v - zmax) : 0.0f, &h[e], &w[e]);
+                hi += h[e];
+                lo += w[e];
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (d[e] < (float)SA_BINS) sum_add(&s.wlo[0][(int)d[e]], &s.whi[0][(int)d[e]], ((unsigned long long)h[e] << 20) + w[e]);
+        }, [](int) {});
+        if (tid == 0) s.found_bin = SA_BINS;
+        unsigned long long whole, ignore;
+        block_incl(((unsigned long long)hi << 20) + lo, s.scan, &whole);
+        const double limit = fmax((double)p * (double)whole, 0.5);  // the largest always stays
+        const unsigned long long m = (unsigned long long)s.whi[0][tid] << 32 | s.wlo[0][tid], w = block_incl(m, s.scan, &ignore);
+        if (!((double)w < limit) && (double)(w - m) < limit) {
+            s.found_bin = tid;
+            s.found_before = w - m;
+        }
+        __syncthreads();
+        const int found = s.found_bin;
+        if (found < SA_BINS) {
+            // the run's end lies in one bin: only that is ranked, gathered with the rounding on both sides
+            const unsigned long long before = s.found_before;
+            const float unit = near * 32.0f, floor = lmax - ((float)found + 1.1f) / unit * 1.00001f;
+            const int edge = gather(floor, found > 0 ? lmax - ((float)found - 0.1f) / unit * 0.99999f : INFINITY);
+            if (edge <= SA_CAP) {
+                rank_edge(cut, edge, div, limit, before, found, [&](float v) { return (int)depth_bin(v) == found; });
+                least = floor;
+                decided = true;
+            }
+        }
+    }
+    if (nc <= SA_CAP) {
+        finish_short(cut, nc, div, k, p, 0ull);
+        return;
+    }
+
+    // ---- a long run, or no filter ----
+    if (!decided) {
+        if (k > 0) cut.select<true>(each, in_order, a.n_vocab, false, (double)k, 0ull);
+        if (p < 1.0f) {
+            unsigned long long sum = 0, among;
+            each([&](float v, int idx) {
+                if (cut.kept(key_of(v), idx)) sum += weight_of(exp_of(v, zmax));
+            });
+            block_incl(sum, s.scan, &among);
+            cut.select<true>(each, in_order, a.n_vocab, true, (double)p, among);
+        }
+    }
+    const float v_cut = cut.cut_key == 0 ? -INFINITY : z_of(cut.cut_key);
+    // without branches: all that a warp has in flight is wanted
+    auto weigh = [&](auto by, float l, int first, int step, uint32_t* hi, uint32_t* lo) {
+        const float v = by(l) + 0.0f, e = expf(v == zmax ? 0.0f : v - zmax);
+        const bool stays = (l > least) & ((v == zmax) | !(e < minp)) & ((v > v_cut) | ((v == v_cut) & (step <= cut.cut_idx - first)));
+        weight_of(stays ? e : 0.0f, hi, lo);
+    };
+    uint32_t hi = 0, lo = 0;
+    walk(least, [&](auto by, const float (&l)[8], int first) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            uint32_t h, w;
+            weigh(by, l[e], first, SaStream::step(e), &h, &w);
+            hi += h;
+            lo += w;
+        }
+    }, [&](int b) {
+        const uint32_t h = __reduce_add_sync(0xffffffffu, hi), w = __reduce_add_sync(0xffffffffu, lo);
+        if (lane == 0) part[b] = ((unsigned long long)h << 20) + w;
+        hi = lo = 0;
+    });
+    __syncthreads();
+    unsigned long long total;
+    const unsigned long long mine = tid < in.blocks ? part[tid] : 0, upto = block_incl(mine, s.scan, &total);
+    const unsigned long long target = cut.target_of(total);
+    if (target >= upto - mine && target < upto) {  // one thread: the block that the number falls in
+        s.found_bin = tid;
+        s.found_before = upto - mine;
+    }
+    __syncthreads();
+    if (warp != 0) return;
+    const int b = s.found_bin;
+    unsigned long long ahead = s.found_before;
+#pragma unroll 1
+    for (int j = 0; j < 8; j++) {
+        const float4 v = in.at(b, j, lane);
+        const float l[4] = {v.x, v.y, v.z, v.w};
+        unsigned long long w[4], own = 0;
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            uint32_t h, x;
+            weigh(SaByDivision{div}, l[c], in.index(b, j, lane, c), 0, &h, &x);
+            own += w[c] = ((unsigned long long)h << 20) + x;
+        }
+        unsigned long long at = ahead + warp_incl(own, lane) - own;
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            if (at <= target && at + w[c] > target) cut.drawn(scaled_of(l[c], div), in.index(b, j, lane, c), total);
+            at += w[c];
+        }
+        ahead = __shfl_sync(0xffffffffu, at, 31);
+    }
+}
+
+__global__ void __launch_bounds__(SA_THREADS, 2) stream_rows(const SaArgs a) {
+    extern __shared__ __align__(16) float slice[];
+    __shared__ SaShared s;
+    if (a.spare > 0) {
+        pdl_wait();
+        pdl_launch_dependents();  // sample_rows reads what this one waited for
+    } else {
+        pdl_launch_dependents();
+        pdl_wait();
+    }
+    stream_row(a, s, slice, blockIdx.x);
 }
 
 }  // namespace
@@ -626,27 +1202,43 @@ extern "C" int cfi_sample(const float* logits, long long row_stride, int n_rows,
         return (int)cudaErrorInvalidValue;
     if (n_rows == 0) return 0;
     if (n_rows > 0x7fffffff / SA_CTAS) return (int)cudaErrorInvalidValue;
-    SaArgs a = {logits, row_stride, temperature, top_p, min_p, u, top_k, token, logprob, n_vocab, 0, cfi_device_error_word()};
+    SaArgs a = {logits, row_stride, temperature, top_p, min_p, u, top_k, token, logprob, n_vocab, 0, n_rows, 0, cfi_device_error_word()};
     a.slice = (int)(((n_vocab + SA_CTAS - 1) / SA_CTAS + 3) / 4 * 4);
-    const size_t smem = (size_t)a.slice * 4 + 32;  // a row's slice keeps its place within 16 bytes
+    const int blocks = (n_vocab + 6) / 4 / SA_BLOCK4 + 1;
     static CfiPerDeviceOnce attr;
     cfi_once_per_device(attr, [] {
-        cudaFuncSetAttribute(sample_rows, cudaFuncAttributeMaxDynamicSharedMemorySize, SA_MAX_SLICE * 4 + 64);
+        cudaFuncSetAttribute(sample_rows<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, SA_MAX_SLICE * 4 + 64);
+        cudaFuncSetAttribute(sample_rows<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SA_MAX_SLICE * 4 + 64);
+        cudaFuncSetAttribute(stream_rows, cudaFuncAttributeMaxDynamicSharedMemorySize, SA_MAX_BLOCKS * 264);
     });
     const char* ep = getenv("CFI_PDL");
-    cudaLaunchConfig_t lc = {};
-    lc.gridDim = dim3((unsigned)n_rows * SA_CTAS, 1, 1);
-    lc.blockDim = dim3(SA_THREADS, 1, 1);
-    lc.dynamicSmemBytes = smem;
-    lc.stream = static_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = SA_CTAS;
-    at[0].val.clusterDim.y = 1;
-    at[0].val.clusterDim.z = 1;
-    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[1].val.programmaticStreamSerializationAllowed = 1;
-    lc.attrs = at;
-    lc.numAttrs = (ep && strcmp(ep, "0") == 0) ? 1 : 2;
-    return (int)cudaLaunchKernelEx(&lc, sample_rows, a);
+    const int pdl = ep && strcmp(ep, "0") == 0 ? 0 : 1;
+    auto launch = [&](void (*kernel)(SaArgs), int ctas, size_t smem, bool cluster) {
+        cudaLaunchConfig_t lc = {};
+        lc.gridDim = dim3((unsigned)ctas, 1, 1);
+        lc.blockDim = dim3(SA_THREADS, 1, 1);
+        lc.dynamicSmemBytes = smem;
+        lc.stream = static_cast<cudaStream_t>(stream);
+        cudaLaunchAttribute at[2];
+        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[0].val.programmaticStreamSerializationAllowed = pdl;
+        at[1].id = cudaLaunchAttributeClusterDimension;
+        at[1].val.clusterDim.x = SA_CTAS;
+        at[1].val.clusterDim.y = 1;
+        at[1].val.clusterDim.z = 1;
+        lc.attrs = at;
+        lc.numAttrs = cluster ? 2 : 1;
+        return cudaLaunchKernelEx(&lc, kernel, a);
+    };
+    // Clusters while all run together: 37 rows of 151936 with all kinds of parameters take 30 us, a CTA a row 49; 74 rows
+    // 58 and 51, 256 rows 144 and 104.  Then rows that are long work for one CTA are left to clusters behind, where
+    // these are no more than run together and the rows are long: 256 rows of 151936 157 -> 104 us, of 32000 44 and
+    // 45; where no row is such that launch costs 10 us.
+    const int at_once = 2 * cfi_sm_count() / SA_CTAS;
+    const size_t slice_bytes = (size_t)a.slice * 4 + 32;  // a row's slice keeps its place within 16 bytes
+    if (n_rows <= at_once) return (int)launch(sample_rows<false>, n_rows * SA_CTAS, slice_bytes, true);
+    a.spare = top_p && n_vocab >= 65536 ? at_once : 0;
+    const cudaError_t e = launch(stream_rows, n_rows, (size_t)blocks * 264, false);
+    if (e != cudaSuccess || a.spare == 0) return (int)e;
+    return (int)launch(sample_rows<true>, at_once * SA_CTAS, slice_bytes, true);
 }

@@ -487,6 +487,46 @@ def test_sample_top_p_zero_and_top_k_one():
     assert (token == z.argmax(1).cpu().numpy()).all() and (lp == 0).all()
 
 
+@pytest.mark.parametrize("vocab", [1, 33, 1000, 2049, 5001, 65536, 151936, 400000])
+@pytest.mark.parametrize("whole", [2, 60])
+def test_sample_many_rows(vocab, whole):
+    """Many rows in one call, of which few or most have a nucleus of the whole row or a long top-k, give what each
+    row gives in a small call: every sum is a whole number, so token and log probability are the same."""
+    rng = np.random.default_rng(vocab + whole)
+    rows, wide = 76, vocab + 5
+    z = (rng.normal(size=(rows, wide)) * 2.5).astype(np.float32)
+    z[:, 3:][np.arange(rows), rng.integers(0, vocab, rows)] += 12
+    z[3] = 0.0
+    z[4] = np.round(z[4] * 2) / 2   # long runs of equal logits
+    z[5, ::2] = -np.inf
+    z[6] = -np.inf
+    z[7, :vocab // 2] = np.nan
+    z[8, 3] = np.inf
+    z[9] = np.finfo(np.float32).min
+    z[10] *= 1e-3                   # flat
+    z[11] *= np.float32(1e-38)      # products that underflow
+    z[12] *= 1000.0
+    t = np.array([0.7, 1.0, 0.0, 1.3, 2.5, 1e-3, 1e20], np.float32)[np.arange(rows) % 7]
+    k = np.array([40, 1000, 5, 1, 1024, 300], np.int32)[np.arange(rows) % 6]
+    k[20:30] = 0
+    p = np.array([1.0, 0.9, 0.5, 0.999], np.float32)[np.arange(rows) % 4]
+    m = np.array([0.0, 0.0, 0.05], np.float32)[np.arange(rows) % 3]
+    p[20:30] = 1.0                  # no filter
+    for r in range(30 if whole > 2 else 74, 76):
+        k[r], p[r] = (0, [0.95, 0.3, 0.9999][r % 3]) if r % 4 else (min(vocab, 3000), 0.9)
+    k[3:13], p[3:13] = (0, 0.9) if whole > 2 else (50, 0.8)
+    u = rng.random(rows).astype(np.float32)
+    d = torch.from_numpy(z).to(DEV)[:, 3:3 + vocab]
+    token, lp = sample(d, u, t, k, p, m)
+    for at in range(0, rows, 30):
+        one = slice(at, at + 30)
+        alone, lp2 = sample(d[one], u[one], t[one], k[one], p[one], m[one])
+        assert (token[one] == alone).all(), (at, token[one], alone)
+        assert ((lp[one] == lp2) | ((lp[one] != lp[one]) & (lp2 != lp2))).all()
+    for r in (0, 1, 13, 21, 40, 41, 75):
+        assert fits(z[r, 3:3 + vocab], u[r], token[r], lp[r], t[r], k[r], p[r], m[r]), r
+
+
 # ---- streams ----
 def test_two_streams_do_not_share():
     """The operators on two streams at once give what each gives alone."""
