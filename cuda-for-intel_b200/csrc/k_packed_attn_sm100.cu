@@ -18,6 +18,12 @@
 //     in shared memory (the next sequence's rows are there, and 0 x NaN would reach this one).
 //
 // Tensor memory: S_A, S_B (128 columns each; P over the first 64), O_A, O_B (D columns each).
+//
+// Bound by the softmax: a block of a tile takes 16384 exponentials, 1024 cycles of an SM's exponential unit, and with
+// the maxima, the fp16 packing and two trips through tensor memory about 2000, half of it beside the other
+// tile's; its MMAs take 512 (heads of 64) or 1024.  One document of 16384 tokens, 12/2 heads of 128: 0.83 ms under the
+// power cap, 995 TFLOP/s (0.70 ms in short bursts); sixteen prompts of 1 to 2048 tokens 60 us, 530 TFLOP/s (the longest
+// tile's 17 blocks and the CTAs behind it); four chunks after 7000 tokens, 14/2 heads of 64, 91 us, 480 TFLOP/s.
 #include "../../include/cfi_serve.h"
 #include "sm100_ptx.cuh"
 #include "cfi_kernels.h"
