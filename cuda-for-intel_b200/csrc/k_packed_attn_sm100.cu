@@ -28,6 +28,7 @@
 #include "sm100_ptx.cuh"
 #include "cfi_kernels.h"
 
+#include <algorithm>
 #include <math.h>
 #include <stdlib.h>
 #include <string.h>
@@ -119,47 +120,11 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kvh = blockIdx.y;
     pdl_launch_dependents();
-    pdl_wait();  // lengths, q, k and v may come from the kernel before
-
-    // ---- which pair of tiles: sequence s, its pair number from the last (the longest) to the first ----
-    const int span = a.tiles * a.tokens;
-    int s = -1, pair = 0, q0 = 0, nq = 0;
-    for (int base = 0, acc = 0; base < a.n_seq && s < 0; base += 32) {
-        int b0 = 0, n = 0;
-        if (base + lane < a.n_seq) {
-            b0 = min(max(a.cu_q[base + lane], 0), a.n_q);
-            n = min(a.cu_q[base + lane + 1], a.n_q) - b0;
-        }
-        const int c = n > 0 ? (n + span - 1) / span : 0;
-        int incl = c;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += x;
-        }
-        const uint32_t hit = __ballot_sync(0xffffffffu, acc + incl > (int)blockIdx.x);
-        if (hit) {
-            const int l = __ffs(hit) - 1;
-            s = base + l;
-            q0 = __shfl_sync(0xffffffffu, b0, l);
-            nq = __shfl_sync(0xffffffffu, n, l);
-            pair = acc + __shfl_sync(0xffffffffu, incl, l) - 1 - (int)blockIdx.x;
-        }
-        acc += __shfl_sync(0xffffffffu, incl, 31);
-    }
-    if (s < 0) return;
-    const int k0 = min(max(a.cu_kv[s], 0), a.n_kv), nk = max(min(a.cu_kv[s + 1], a.n_kv) - k0, 0);
-    // keys that token t sees, and blocks that a tile needs (its last token sees the most)
-    auto seen = [&](int t) { return a.causal ? max(0, min(nk, t + nk - nq + 1)) : nk; };
-    auto first_token = [&](int x) { return pair * span + x * a.tokens; };
-    auto blocks = [&](int x) {
-        const int t = first_token(x);
-        return x < a.tiles && t < nq ? (seen(min(nq, t + a.tokens) - 1) + KA_N - 1) / KA_N : 0;
-    };
-    const int nb0 = blocks(0), nb1 = blocks(1), nmax = max(nb0, nb1);
-    const bool cut = nmax * KA_N > nk;  // the last block runs past the sequence
-
+    // all that needs no input: it runs beside the end of the kernel before
     if (tid == 0) {
+        prefetch_tmap(&tq);
+        prefetch_tmap(&tk);
+        prefetch_tmap(&tv);
         for (int i = 0; i < NS; i++) {
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
@@ -178,6 +143,53 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
         tmem_alloc(tmem_slot, KA_TMEM_COLS);
         tmem_relinquish();
     }
+    pdl_wait();  // lengths, q, k and v may come from the kernel before
+
+    // ---- which pair of tiles: sequence s, its pair number from the last (the longest) to the first ----
+    const int span = a.tiles * a.tokens;
+    int s = -1, pair = 0, q0 = 0, nq = 0, k_from = 0, k_to = 0;
+    for (int base = 0, acc = 0; base < a.n_seq && s < 0; base += 32) {
+        int b0 = 0, n = 0, kb0 = 0, kb1 = 0;
+        if (base + lane < a.n_seq) {
+            kb0 = a.cu_kv[base + lane];
+            kb1 = a.cu_kv[base + lane + 1];
+            b0 = min(max(a.cu_q[base + lane], 0), a.n_q);
+            n = min(a.cu_q[base + lane + 1], a.n_q) - b0;
+        }
+        const int c = n > 0 ? (n + span - 1) / span : 0;
+        int incl = c;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += x;
+        }
+        const uint32_t hit = __ballot_sync(0xffffffffu, acc + incl > (int)blockIdx.x);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            s = base + l;
+            q0 = __shfl_sync(0xffffffffu, b0, l);
+            nq = __shfl_sync(0xffffffffu, n, l);
+            k_from = __shfl_sync(0xffffffffu, kb0, l);
+            k_to = __shfl_sync(0xffffffffu, kb1, l);
+            pair = acc + __shfl_sync(0xffffffffu, incl, l) - 1 - (int)blockIdx.x;
+        }
+        acc += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (s < 0) {
+        if (warp == KA_MMA_WARP) tmem_dealloc(0, KA_TMEM_COLS);
+        return;
+    }
+    const int k0 = min(max(k_from, 0), a.n_kv), nk = max(min(k_to, a.n_kv) - k0, 0);
+    // keys that token t sees, and blocks that a tile needs (its last token sees the most)
+    auto seen = [&](int t) { return a.causal ? max(0, min(nk, t + nk - nq + 1)) : nk; };
+    auto first_token = [&](int x) { return pair * span + x * a.tokens; };
+    auto blocks = [&](int x) {
+        const int t = first_token(x);
+        return x < a.tiles && t < nq ? (seen(min(nq, t + a.tokens) - 1) + KA_N - 1) / KA_N : 0;
+    };
+    const int nb0 = blocks(0), nb1 = blocks(1), nmax = max(nb0, nb1);
+    const bool cut = nmax * KA_N > nk;  // the last block runs past the sequence
+
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -286,7 +298,7 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
         // ---- softmax: row r of tile x ----
         const int x = warp >> 2, r = 32 * (warp & 3) + lane;
         const int t = first_token(x) + r / a.group, n_blocks = x ? nb1 : nb0;
-        const bool valid = r < a.tokens * a.group && t < nq;
+        const bool valid = x < a.tiles && r < a.tokens * a.group && t < nq;
         const int limit = valid ? seen(t) : 0;
         const uint32_t trow = TM + ((uint32_t)(32 * (warp & 3)) << 16);
         const uint32_t ts = trow + x * KA_N, to = trow + 256 + x * D;
@@ -451,10 +463,14 @@ template <int D> int launch(const CfiPackedAttention* p, cudaStream_t stream) {
     a.causal = p->causal;
     a.scale_log2 = p->scale * 1.4426950408889634f;
     a.err = cfi_device_error_word();
-    // Every sequence adds at most one pair that is not full.  Where pairs would leave half the SMs idle, a CTA takes a
-    // single tile, and a block of keys takes it 2/3 of the time (one prompt of 631, 14/2 heads of 64: 14.8 to 12.5 us).
+    // Every sequence adds at most one pair that is not full.  A CTA takes a single tile, and is faster through its keys,
+    // where the SMs have room for all of them within the longest's time.  `share`: how long a tile is on the average,
+    // with sequences of one length (a prompt without a context: half).  Single tiles against pairs, us: one prompt of
+    // 631, 14/2 heads of 64, 12.1 and 14.8; of 2048, 12/2 heads of 128, 33 and 37; of 3000, 51 and 52; of 4096, 97 and
+    // 67; of 1024 with 32/8 heads 32 and 22; four of 100 to 1000 after 2000, 14/2 heads of 64, 53 and 35.
     auto pairs = [&](int tiles) { return p->n_q / (tiles * a.tokens) + (p->n_seq < p->n_q ? p->n_seq : p->n_q); };
-    a.tiles = 2LL * pairs(2) * p->n_kv_head <= cfi_sm_count() ? 1 : 2;
+    const double share = p->causal && p->n_kv > 0 ? 1.0 - 0.5 * std::min(p->n_q, p->n_kv) / p->n_kv : 1.0;
+    a.tiles = 2.2 * pairs(2) * p->n_kv_head * share <= cfi_sm_count() ? 1 : 2;
     CUtensorMap tq, tk, tv;
     // no keys at all: the maps still need an extent, and nothing is loaded
     if (!map_rows(&tq, p->q, D, p->n_head, p->q_stride, p->n_q, a.group, a.tokens) ||

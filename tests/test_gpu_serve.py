@@ -337,6 +337,15 @@ def test_packed_attention_bad_neighbour():
         packed_case(heads, kv, dim, [200, 3, 130], [333, 3, 140], poison=True)
 
 
+@pytest.mark.parametrize("heads,kv,dim,n", [(12, 2, 128, 2048), (14, 2, 64, 1500), (2, 2, 64, 9000)])
+def test_packed_attention_every_tile_writes_its_own_rows(heads, kv, dim, n):
+    """More single tiles than SMs, of which the short ones end long before their neighbours: each row is written by
+    its own tile only, in both output types, with and without the mask."""
+    for causal in (True, False):
+        for ot in (cfi.T_F32, cfi.T_F16):
+            packed_case(heads, kv, dim, [n], [n] if causal else [130], causal, ot=ot, seed=n)
+
+
 def test_packed_attention_ranges_are_cut():
     """Ends past the tensors are cut to them: nothing outside is read or written."""
     heads, kv, dim, n = 4, 2, 64, 100
