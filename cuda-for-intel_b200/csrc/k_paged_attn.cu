@@ -20,7 +20,7 @@
 // weights before these are split (times 2^8, so that small scales stay clear of f16's subnormals).
 //
 // Measured: 8 sequences of 9000 to 65000 positions, 32/8 heads of 128 in f16, 146 us, 6.2 TB/s; 64 of 16 to 4096, 12/2 heads
-// of 128 in Q8_0, 20.6 us (36 MB; the work of a tile, some 870 instructions of a warp, is what it waits for:
+// of 128 in Q8_0, 20.0 us (36 MB; the work of a tile, some 870 instructions of a warp, is what it waits for:
 // the warps of three CTAs issue in 45 % of the cycles); one of 672, 14/2 heads of 64 in f16, 6.3 us, 5.1 of them on the device:
 // launch, table, one round of loads and the join.
 #include "paged_cache.cuh"
@@ -44,6 +44,7 @@ constexpr float PA_V_UNIT = 256.0f;
 // What beginning and ending a pair costs, in tiles: a run's share of the list counts it, so that CTAs with
 // many short sequences get fewer tiles.
 constexpr int PA_FIXED = 5;
+constexpr int PA_KEPT = 4;
 
 template <int D, bool Q8, int W = PA_WARPS> struct PaShape {
     static constexpr int ROW = Q8 ? D : 2 * D;            // bytes of a row
@@ -143,19 +144,23 @@ CFI_DEV void write_out(const PaArgs& a, int seq, int head, int dim, int d, float
 // There are less than 2^31.
 struct PaCut {
     const int32_t* lens;
-    int most, first, total, quota;
+    int most, total, quota;
+    int units[PA_KEPT];  // of the sequences that are this lane's, of the first 32 PA_KEPT, all loaded together
     CFI_DEV int length(int s) const { return max(0, min(lens[s], most)); }
     // an empty sequence still has its zeros to write
     static CFI_DEV int tiles_of(int len) { return max(1, (len + PA_TILE - 1) / PA_TILE); }
     CFI_DEV int units_of(int s) const { return PA_FIXED + tiles_of(length(s)); }
     CFI_DEV explicit PaCut(const PaArgs& a)
         : lens(a.lens), most((int)min((long long)a.max_pages << a.page_shift, 0x7fffff00LL)) {}
-    // Called by whole warps.  `first`: the units of the sequence that is this lane's, of the first 32.
+    // Called by whole warps.
     CFI_DEV void read(const PaArgs& a, int ctas) {
         const int lane = threadIdx.x & 31, hc = a.n_kv_head * a.chunks;
-        first = lane < a.n_seq ? units_of(lane) * hc : 0;
-        int n = first;
-        for (int s = lane + 32; s < a.n_seq; s += 32) n += units_of(s) * hc;
+        int n = 0;
+#pragma unroll
+        for (int e = 0; e < PA_KEPT; e++) units[e] = lane + 32 * e < a.n_seq ? units_of(lane + 32 * e) * hc : 0;
+#pragma unroll
+        for (int e = 0; e < PA_KEPT; e++) n += units[e];
+        for (int s = lane + 32 * PA_KEPT; s < a.n_seq; s += 32) n += units_of(s) * hc;
         total = __reduce_add_sync(0xffffffffu, n);
         quota = max((total + ctas - 1) / ctas, PA_FIXED + PA_WARPS);
     }
@@ -226,8 +231,7 @@ __global__ void __launch_bounds__(W * 32, (PaShape<D, Q8, W>::CTAS)) paged_attn(
         if ((int)blockIdx.x > (cut.total - 1) / cut.quota) return;
         begin = at = blockIdx.x * cut.quota;
         end = min(begin + cut.quota, cut.total);
-        for (int base = 0;; base += 32) {
-            const int n = base == 0 ? cut.first : base + lane < a.n_seq ? cut.units_of(base + lane) * hc : 0;
+        auto among = [&](int base, int n) {  // is it one of the 32 sequences from `base` on, this lane's with n units?
             int incl = n;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -235,14 +239,17 @@ __global__ void __launch_bounds__(W * 32, (PaShape<D, Q8, W>::CTAS)) paged_attn(
                 if (lane >= o) incl += x;
             }
             const uint32_t hit = __ballot_sync(0xffffffffu, seq_start + incl > at);
-            if (hit) {
-                const int l = __ffs(hit) - 1;
-                seq = base + l;
-                seq_start += __shfl_sync(0xffffffffu, incl - n, l);
-                break;
-            }
-            seq_start += __shfl_sync(0xffffffffu, incl, 31);
-        }
+            const int l = hit ? __ffs(hit) - 1 : 31;
+            seq = base + l;
+            seq_start += __shfl_sync(0xffffffffu, hit ? incl - n : incl, l);
+            return hit != 0;
+        };
+        bool found = false;
+#pragma unroll
+        for (int e = 0; e < PA_KEPT; e++)
+            if (!found) found = among(32 * e, cut.units[e]);
+        for (int base = 32 * PA_KEPT; !found && base < a.n_seq; base += 32)
+            found = among(base, base + lane < a.n_seq ? cut.units_of(base + lane) * hc : 0);
     }
 
     const uint32_t ring = smem_u32(smem) + warp * S::RING;
