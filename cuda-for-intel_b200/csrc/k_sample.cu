@@ -4,8 +4,8 @@
 // The logits are one read of memory; what bounds a call is the chain of passes behind it, each of which needs the
 // last one's answer.  Few rows: a cluster of CTAs takes a row, each keeps its slice in shared memory,
 // walks it there and meets the others through distributed shared memory (one row of 151936 with a nucleus among the
-// first 50: 13.9 us).  Many: a CTA takes a row and streams it from memory, as many rows at once as fit (256 rows, top-k 50: 44 us, 3.5 TB/s;
-// greedy: 34 us, 4.6 TB/s; without a filter, two reads and an exponential of everything: 81 us).
+// first 50: 12.6 us).  Many: a CTA takes a row and streams it from memory, as many rows at once as fit (256 rows, top-k
+// 50: 44 us, 3.5 TB/s; greedy: 34 us, 4.6 TB/s; without a filter, two reads and an exponential of everything: 81 us).
 // Everything that is summed is a whole number (a weight is exp(z - max) in units of 2^-40), so no sum depends on its
 // order and every CTA of a cluster reaches the same decisions from the same histograms.
 //
@@ -86,7 +86,12 @@ static_assert((((SA_MAX_SLICE + 6) / 4 / SA_THREADS + 1) | 1) <= 32, "a thread's
 
 struct SaShared {
     uint32_t cnt[2][SA_BINS];
-    uint32_t wlo[2][SA_BINS], whi[2][SA_BINS];  // sums of weights in two words
+    union {
+        struct {
+            uint32_t wlo[2][SA_BINS], whi[2][SA_BINS];  // sums of weights in two words
+        };
+        float logit[SA_CAP];  // from sample_row, the logits of cand, until SaHeld has them
+    };
     SaItem list[2][SA_LIST];   // the boundary bin's elements: this CTA's, and all
     uint32_t cand[SA_CAP];     // a short run's elements: their indexes, rising
     uint64_t bar;
@@ -234,7 +239,8 @@ struct SaCut {
         if (a.logprob) a.logprob[row] = (v == zmax ? 0.0f : v - zmax) - logf((float)((double)total / SA_UNIT));
     }
     // The draw: kept weights in index order.  `own`: this thread's, `ahead`: those of the threads before it.
-    template <class E> CFI_DEV void draw(E&& in_order, unsigned long long own, unsigned long long ahead, unsigned long long total) const {
+    template <class E>
+    CFI_DEV void draw(E&& in_order, unsigned long long own, unsigned long long ahead, unsigned long long total) const {
         const unsigned long long target = target_of(total);
         if (target < ahead || target >= ahead + own) return;
         in_order([&](float v, int idx) {
@@ -392,14 +398,17 @@ struct SaCut {
 struct SaHeld {
     float v[SA_EACH];
     int idx[SA_EACH];
-    CFI_DEV SaHeld(const SaCut& cut, int nc, float div) {
+    // `logits`: theirs in the same order, or null to read them again
+    CFI_DEV SaHeld(const SaCut& cut, int nc, const float* logits, float div) {
         const int each_n = (nc + SA_THREADS - 1) / SA_THREADS;
 #pragma unroll
         for (int e = 0; e < SA_EACH; e++) {
             const int x = threadIdx.x * each_n + e;
             idx[e] = e < each_n && x < nc ? (int)cut.s.cand[x] : -1;
-            v[e] = idx[e] >= 0 ? scaled_of(__ldcg(cut.a.logits + cut.row * cut.a.stride + idx[e]), div) : -INFINITY;
+            v[e] = -INFINITY;
+            if (idx[e] >= 0) v[e] = scaled_of(logits ? logits[x] : __ldcg(cut.a.logits + cut.row * cut.a.stride + idx[e]), div);
         }
+        if (logits) __syncthreads();  // their place is free
     }
     template <class F> CFI_DEV void operator()(F&& f) const {
 #pragma unroll
@@ -409,8 +418,10 @@ struct SaHeld {
 };
 
 // The cut among those of the nc elements of s.cand that are in(z), which have `before` units above them.
-template <class F> CFI_DEV void rank_edge(SaCut& cut, int nc, float div, double limit, unsigned long long before, int bin, F&& in) {
-    SaHeld each(cut, nc, div);
+template <class F>
+CFI_DEV void rank_edge(SaCut& cut, int nc, const float* logits, float div, double limit, unsigned long long before, int bin,
+                       F&& in) {
+    SaHeld each(cut, nc, logits, div);
 #pragma unroll
     for (int e = 0; e < SA_EACH; e++)
         if (!in(each.v[e])) each.idx[e] = -1;
@@ -422,8 +433,8 @@ template <class F> CFI_DEV void rank_edge(SaCut& cut, int nc, float div, double 
 
 // A short run, alone: s.cand holds the indexes of nc elements, rising, with all that can stay among them.  `whole`: the weight
 // that a top-p is a share of, 0 where it is that of these elements as the top-k leaves them.
-CFI_DEV void finish_short(SaCut& cut, int nc, float div, int k, float p, unsigned long long whole) {
-    const SaHeld each(cut, nc, div);
+CFI_DEV void finish_short(SaCut& cut, int nc, const float* logits, float div, int k, float p, unsigned long long whole) {
+    const SaHeld each(cut, nc, logits, div);
     if (k > 0 && k < nc) cut.select<true>(each, each, nc, false, (double)k, 0ull);
     if (p < 1.0f) {
         unsigned long long among = whole;
@@ -500,9 +511,11 @@ CFI_DEV void sample_row(const SaArgs& a, SaShared& s, float* slice, uint32_t ran
         for (; g < g1; g += step) f(g, z4[g]);
     };
     auto max4 = [](const float4& v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); };  // a NaN is passed over
-    float mx = -INFINITY;
-    by_four(tid, groups, SA_THREADS, [&](int, const float4& v) { mx = fmaxf(mx, max4(v)); });
-    mx = warp_max(mx);
+    // this thread's groups, in index order; an odd number: eight threads' groups take every bank once
+    const int q = ((groups + SA_THREADS - 1) / SA_THREADS) | 1, g0 = min(groups, tid * q), g1 = min(groups, g0 + q);
+    float largest = -INFINITY;  // of them
+    by_four(g0, g1, 1, [&](int, const float4& v) { largest = fmaxf(largest, max4(v)); });
+    float mx = warp_max(largest);
     if (lane == 0) s.wmax[warp] = mx;
     __syncthreads();
     if (warp == 0) {
@@ -546,32 +559,42 @@ CFI_DEV void sample_row(const SaArgs& a, SaShared& s, float* slice, uint32_t ran
 #pragma unroll
         for (uint32_t r = 0; r < SA_CTAS; r++) whole += *peer(&s.cta_sum, r);
     }
-    uint32_t level = 1;  // histogram 0 has been used
-    // ---- a short run: down to which depth? ----
-    float floor = INFINITY, top = INFINITY;  // gather what is larger than the one and not than the other
-    int edge = -1;                          // or a long run's end: the bin that it lies in
+    // ---- a short run: down to which depth?  What is above is gathered in index order by the first CTA ----
+    uint32_t level = 0;  // the next histogram; the first is zero, or has the sums above
+    int edge = -1;       // a long run's end: the bin that it lies in
     double limit = 0.0;
+    int nc = SA_CAP + 1;
     if (!empty && bins_hold && (k > 0 || p < 1.0f)) {
-        // bins down to a depth of 8, or 16 where more than a few are asked for; the second turn reaches 32, where no
-        // weight is left
-        float scale = k > 8 || k <= 0 ? 32.0f : 64.0f;
-        for (int turn = 0;; turn++) {
-            const uint32_t b = turn & 1;
+        // A top-k: bins of the threads' largest first, down to a depth of 8, or 16 where more than a few are asked for: as
+        // many elements reach as deep as the k-th of these, and few more where k is a small share of them (one row of
+        // 151936, k 50: 13.9 -> 12.6 us; 1000 of 5000 would fail so and take 2 us longer).  Else, or where that is too
+        // many or there are fewer, bins of all elements, and then down to 32, where no weight is left.
+        const bool small_share = 4LL * k <= SA_CTAS * (a.slice / 4 / (((a.slice / 4 + SA_THREADS - 1) / SA_THREADS) | 1));
+#pragma unroll 1
+        for (int turn = k > 0 && small_share ? 0 : 1; turn < 3; turn++) {
+            const float scale = turn == 2 ? 16.0f : k > 8 || k <= 0 ? 32.0f : 64.0f;
+            const uint32_t b = level++ & 1;
             if (k > 0) {
-                if (turn > 0) {
+                if (level > 1) {
                     s.cnt[b][tid] = 0;
                     __syncthreads();
                 }
-                const float unit = near * scale, floor = lmax - (float)SA_BINS / unit * 1.0001f;
-                by_four(tid, groups, SA_THREADS, [&](int, const float4& v) {
-                    if (!(max4(v) > floor)) return;
-                    const float l[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float d = (lmax - l[e]) * unit;  // a NaN compares false
-                        if (d < (float)SA_BINS) atomicAdd(&s.cnt[b][(int)d], 1u);
-                    }
-                });
+                const float unit = near * scale, window = lmax - (float)SA_BINS / unit * 1.0001f;
+                auto bin = [&](float l) {
+                    const float d = (lmax - l) * unit;  // a NaN compares false
+                    if (d < (float)SA_BINS) atomicAdd(&s.cnt[b][(int)d], 1u);
+                };
+                if (turn == 0) {
+                    if (largest > window) bin(largest);
+                } else {
+                    by_four(g0, g1, 1, [&](int, const float4& v) {
+                        if (!(max4(v) > window)) return;
+                        bin(v.x);
+                        bin(v.y);
+                        bin(v.z);
+                        bin(v.w);
+                    });
+                }
                 cluster_sync();
             }
             uint32_t c = 0;
@@ -583,9 +606,8 @@ CFI_DEV void sample_row(const SaArgs& a, SaShared& s, float* slice, uint32_t ran
             }
             // the first bin whose end lies past the run's; with the next one, and one more for the rounding
             unsigned long long all, ignore;
-            const unsigned long long upto = block_incl(c, s.scan, &all);
             if (tid == 0) s.found_bin = SA_BINS;
-            __syncthreads();
+            const unsigned long long upto = block_incl(c, s.scan, &all);
             if (k > 0) {
                 if (upto >= (unsigned long long)k && upto - c < (unsigned long long)k) s.found_bin = tid;
             } else {
@@ -598,73 +620,72 @@ CFI_DEV void sample_row(const SaArgs& a, SaShared& s, float* slice, uint32_t ran
                 }
             }
             __syncthreads();
-            const int bin = s.found_bin;
-            if (bin + 2 < SA_BINS) {
-                if (tid == bin + 2) s.found_n = (uint32_t)upto;
+            const int found = s.found_bin;
+            float floor = INFINITY, top = INFINITY;  // gather what is larger than the one and not than the other
+            if (found + 2 < SA_BINS) {
+                if (tid == found + 2) s.found_n = (uint32_t)upto;
                 __syncthreads();
-                if (s.found_n <= SA_CAP) {
-                    floor = lmax - (float)(bin + 2) / scale * div * 1.00001f;
+                if (turn == 0 || s.found_n <= SA_CAP) {
+                    floor = lmax - (float)(found + 2) / scale * div * 1.00001f;
                 } else if (k <= 0 && s.cta_n <= SA_CAP / 2) {
-                    edge = bin;  // a bin and the rounding on both sides
-                    floor = lmax - ((float)bin + 1.1f) / scale * div * 1.00001f;
-                    if (bin > 0) top = lmax - ((float)bin - 0.1f) / scale * div * 0.99999f;
+                    edge = found;  // a bin and the rounding on both sides
+                    floor = lmax - ((float)found + 1.1f) / scale * div * 1.00001f;
+                    if (found > 0) top = lmax - ((float)found - 0.1f) / scale * div * 0.99999f;
                 }
-                __syncthreads();
-                break;
+            } else if (turn == 2 && found == SA_BINS && all <= SA_CAP) {
+                floor = lmax - (float)SA_BINS / scale * div * 1.00001f;  // fewer than k elements have any weight
             }
             __syncthreads();
-            if (k <= 0 || turn == 1) {
-                // fewer than k elements have any weight: all of them are gathered
-                if (k > 0 && bin == SA_BINS && all <= SA_CAP) floor = lmax - (float)SA_BINS / scale * div * 1.00001f;
-                break;
+            if (floor < INFINITY) {
+                unsigned long long hit[2] = {0, 0};
+                if (largest > floor)
+                    by_four(g0, g1, 1, [&](int g, const float4& v) {
+                        if (!(max4(v) > floor)) return;
+                        auto in = [&](float l) { return (unsigned long long)(l > floor && l <= top); };
+                        const unsigned long long bits = in(v.x) | in(v.y) << 1 | in(v.z) << 2 | in(v.w) << 3;
+                        if (g - g0 < 16) hit[0] |= bits << 4 * (g - g0); else hit[1] |= bits << 4 * (g - g0 - 16);
+                    });
+                const int mine = __popcll(hit[0]) + __popcll(hit[1]);
+                unsigned long long own;
+                int at = (int)block_incl((unsigned long long)mine, s.scan, &own) - mine;
+                if (tid == 0) s.n_own = (int)own;
+                cluster_sync();
+                nc = 0;
+#pragma unroll
+                for (uint32_t r = 0; r < SA_CTAS; r++) {
+                    const int x = *peer(&s.n_own, r);
+                    if (r < rank) at += x;
+                    nc += x;
+                }
+                if (nc <= SA_CAP) {  // as counted, but for what rounding brings in at the edge
+                    uint32_t* to = const_cast<uint32_t*>(peer(&s.cand[0], 0));
+                    float* to_logit = const_cast<float*>(peer(&s.logit[0], 0));
+#pragma unroll
+                    for (int x = 0; x < 2; x++)
+                        for (unsigned long long h = hit[x]; h; h &= h - 1) {
+                            const int i = 4 * g0 - shift + 64 * x + __ffsll((long long)h) - 1;
+                            to_logit[at] = z[i];
+                            to[at++] = (uint32_t)(base + i);
+                        }
+                    break;
+                }
+                edge = -1;
             }
-            scale = 16.0f;
-            level = 2;
+            if (k <= 0 || (turn == 1 && found + 2 < SA_BINS)) break;  // a long run
         }
     }
 
     SaCut cut = {s, a, row, rank, zmax, minp, level};
     bool ranked = false;
-    int nc = SA_CAP + 1;
-    if (floor < INFINITY) {
-        // ---- a short run: gathered in index order by the first CTA, which goes on alone ----
-        const int q = ((groups + SA_THREADS - 1) / SA_THREADS) | 1;  // odd: eight threads' groups take every bank once
-        const int g0 = min(groups, tid * q), g1 = min(groups, g0 + q);
-        unsigned long long hit[2] = {0, 0};
-        by_four(g0, g1, 1, [&](int g, const float4& v) {
-            if (!(max4(v) > floor)) return;
-            auto in = [&](float l) { return (unsigned long long)(l > floor && l <= top); };
-            const unsigned long long bits = in(v.x) | in(v.y) << 1 | in(v.z) << 2 | in(v.w) << 3;
-            if (g - g0 < 16) hit[0] |= bits << 4 * (g - g0); else hit[1] |= bits << 4 * (g - g0 - 16);
-        });
-        const int mine = __popcll(hit[0]) + __popcll(hit[1]);
-        unsigned long long own;
-        int at = (int)block_incl((unsigned long long)mine, s.scan, &own) - mine;
-        if (tid == 0) s.n_own = (int)own;
-        cluster_sync();
-        nc = 0;
-#pragma unroll
-        for (uint32_t r = 0; r < SA_CTAS; r++) {
-            const int x = *peer(&s.n_own, r);
-            if (r < rank) at += x;
-            nc += x;
-        }
-        if (nc <= SA_CAP) {  // as counted, but for what rounding brings in at the edge
-            uint32_t* to = const_cast<uint32_t*>(peer(&s.cand[0], 0));
-#pragma unroll
-            for (int x = 0; x < 2; x++)
-                for (unsigned long long h = hit[x]; h; h &= h - 1)
-                    to[at++] = (uint32_t)(base + 4 * g0 - shift + 64 * x + __ffsll((long long)h) - 1);
-        }
-    }
     if (nc <= SA_CAP) {
         cluster_sync();
         if (edge < 0) {
-            if (rank == 0) finish_short(cut, nc, div, k, p, whole);
+            if (rank == 0) finish_short(cut, nc, s.logit, div, k, p, whole);
             return;
         }
         if (rank == 0) {
-            rank_edge(cut, nc, div, limit, s.found_before, edge, [&](float v) { return (int)((zmax - v) * 32.0f) == edge; });
+            rank_edge(cut, nc, s.logit, div, limit, s.found_before, edge,
+                      [&](float v) { return (int)((zmax - v) * 32.0f) == edge; });
             if (tid == 0) {
                 s.cut_key = cut.cut_key;
                 s.cut_idx = cut.cut_idx;
@@ -1100,14 +1121,14 @@ CFI_DEV void stream_row(const SaArgs& a, SaShared& s, float* slice, int row) {
             const float unit = near * 32.0f, floor = lmax - ((float)found + 1.1f) / unit * 1.00001f;
             const int edge = gather(floor, found > 0 ? lmax - ((float)found - 0.1f) / unit * 0.99999f : INFINITY);
             if (edge <= SA_CAP) {
-                rank_edge(cut, edge, div, limit, before, found, [&](float v) { return (int)depth_bin(v) == found; });
+                rank_edge(cut, edge, nullptr, div, limit, before, found, [&](float v) { return (int)depth_bin(v) == found; });
                 least = floor;
                 decided = true;
             }
         }
     }
     if (nc <= SA_CAP) {
-        finish_short(cut, nc, div, k, p, 0ull);
+        finish_short(cut, nc, nullptr, div, k, p, 0ull);
         return;
     }
 
