@@ -453,6 +453,24 @@ CFI_DEV void finish_short(SaCut& cut, int nc, const float* logits, float div, in
     cut.draw(each, sum, upto - sum, total);
 }
 
+// l / T in three forms.  The second, for ordinary T and l only, is Markstein's (Computation of elementary functions on the IBM RISC
+// System/6000, 1990): from the reciprocal rounded to nearest, corrections by the exact remainder end at
+// the quotient rounded to nearest, the first within an ulp of it.  The same value as the division's, without its branch.
+struct SaByOne {
+    CFI_DEV float operator()(float l) const { return l; }
+};
+struct SaByDivision {
+    float t;
+    CFI_DEV float operator()(float l) const { return l / t; }
+};
+struct SaByReciprocal {
+    float t, r;
+    CFI_DEV float operator()(float l) const {
+        const float q0 = l * r, q1 = fmaf(fmaf(-q0, t, l), r, q0);
+        return fmaf(fmaf(-q1, t, l), r, q1);
+    }
+};
+
 // One row, by a cluster: this CTA has the n logits from `base`.
 CFI_DEV void sample_row(const SaArgs& a, SaShared& s, float* slice, uint32_t rank, int row) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -528,18 +546,18 @@ CFI_DEV void sample_row(const SaArgs& a, SaShared& s, float* slice, uint32_t ran
     const float zmax = scaled(lmax);  // division by a positive number keeps the order
     const bool empty = zmax == -INFINITY;
 
-    // ---- no top-k: every weight counts.  Each thread sums its run; with a top-p, the top of the order by bins ----
-    unsigned long long run_sum = 0, whole = 0;
+    // ---- a top-p of the whole row: the sum of all weights, and the top of the order by bins ----
+    unsigned long long whole = 0;
     const float near = 1.0f / div;
     const bool bins_hold = fabsf(zmax) < 8192.0f && near < 1e30f;  // z is exact to far less than a bin
-    if (!empty && k <= 0 && bins_hold) {
-        const bool binned = p < 1.0f;
+    if (!empty && k <= 0 && p < 1.0f && bins_hold) {
         const float floor = lmax - 28.0f * div * 1.0001f;  // no weight at or below this
+        unsigned long long run_sum = 0;
         auto weigh = [&](float v) {  // zmax is finite: expf(0) is 1
             const unsigned long long w = weight_of(expf(v - zmax));
             run_sum += w;
             const float d = (zmax - v) * 32.0f;
-            if (binned && d < (float)SA_BINS) {
+            if (d < (float)SA_BINS) {
                 atomicAdd(&s.cnt[0][(int)d], 1u);
                 sum_add(&s.wlo[0][(int)d], &s.whi[0][(int)d], w);
             }
@@ -627,7 +645,7 @@ CFI_DEV void sample_row(const SaArgs& a, SaShared& s, float* slice, uint32_t ran
                 __syncthreads();
                 if (turn == 0 || s.found_n <= SA_CAP) {
                     floor = lmax - (float)(found + 2) / scale * div * 1.00001f;
-                } else if (k <= 0 && s.cta_n <= SA_CAP / 2) {
+                } else if (k <= 0 && s.cta_n <= SA_CAP * 3 / 4) {
                     edge = found;  // a bin and the rounding on both sides
                     floor = lmax - ((float)found + 1.1f) / scale * div * 1.00001f;
                     if (found > 0) top = lmax - ((float)found - 0.1f) / scale * div * 0.99999f;
@@ -697,15 +715,32 @@ CFI_DEV void sample_row(const SaArgs& a, SaShared& s, float* slice, uint32_t ran
         ranked = true;
     }
 
-    // ---- a long run, or no filter: z in place of the logits ----
-    for (int i = tid; i < n; i += SA_THREADS) z[i] = scaled(z[i]);
-    __syncthreads();
-    auto each = [&](auto&& f) { walk([&](int i, float v) { f(v, base + i); }); };
-    if (!empty) {
+    // ---- a long run, or no filter ----
+    const bool filter = !empty && !ranked && (k > 0 || p < 1.0f);
+    auto each = [&](auto&& f) { walk([&](int i, float v) { f(filter ? v : scaled(v), base + i); }); };
+    if (filter) {  // z in place of the logits: many passes
+        for (int i = tid; i < n; i += SA_THREADS) z[i] = scaled(z[i]);
+        __syncthreads();
         if (k > 0) cut.select<false>(each, each, a.n_vocab, false, (double)k, 0ull);
-        if (p < 1.0f && !ranked) cut.select<false>(each, each, a.n_vocab, true, (double)p, 0ull);
-        if (k > 0 || p < 1.0f || minp > 0.0f || !bins_hold) run_sum = cut.weight_of_kept(each);
+        if (p < 1.0f) cut.select<false>(each, each, a.n_vocab, true, (double)p, 0ull);
     }
+    // the kept weights of this thread's run, without branches: the exponentials of a batch are in flight together
+    const float v_cut = cut.cut_key == 0 ? -INFINITY : z_of(cut.cut_key);
+    auto sum_of_kept = [&](auto by) {
+        uint32_t hi = 0, lo = 0;
+        walk([&](int i, float l) {
+            float v = by(l) + 0.0f;
+            v = v == v ? v : -INFINITY;
+            const float e = expf(v == zmax ? 0.0f : v - zmax);
+            const bool stays = ((v == zmax) | !(e < minp)) & ((v > v_cut) | ((v == v_cut) & (base + i <= cut.cut_idx)));
+            uint32_t h, w;
+            weight_of(stays ? e : 0.0f, &h, &w);
+            hi += h;
+            lo += w;
+        });
+        return ((unsigned long long)hi << 20) + lo;
+    };
+    const unsigned long long run_sum = empty ? 0 : filter || div == 1.0f ? sum_of_kept(SaByOne{}) : sum_of_kept(SaByDivision{div});
     unsigned long long sum;
     const unsigned long long upto = block_incl(run_sum, s.scan, &sum);
     if (tid == 0) s.kept_sum = sum;
@@ -771,24 +806,6 @@ template <bool SPARE> __global__ void __launch_bounds__(SA_THREADS, 2) sample_ro
     if (row >= 0 && count <= a.spare) sample_row(a, s, slice, cluster_ctarank(), row);
     pdl_wait();
 }
-
-// l / T in three forms.  The second, for ordinary T and l only, is Markstein's (Computation of elementary functions on the IBM RISC
-// System/6000, 1990): from the reciprocal rounded to nearest, corrections by the exact remainder end at
-// the quotient rounded to nearest, the first within an ulp of it.  The same value as the division's, without its branch.
-struct SaByOne {
-    CFI_DEV float operator()(float l) const { return l; }
-};
-struct SaByDivision {
-    float t;
-    CFI_DEV float operator()(float l) const { return l / t; }
-};
-struct SaByReciprocal {
-    float t, r;
-    CFI_DEV float operator()(float l) const {
-        const float q0 = l * r, q1 = fmaf(fmaf(-q0, t, l), r, q0);
-        return fmaf(fmaf(-q1, t, l), r, q1);
-    }
-};
 
 // ---- many rows: a CTA takes one ----
 // The row is streamed past registers, and of each group of 32 logits the largest is kept.  A block is 1024 logits,
