@@ -1017,22 +1017,31 @@ CFI_DEV void stream_row(const SaArgs& a, SaShared& s, float* slice, int row) {
         for (int b = warp; b < in.blocks; b += SA_WARPS) {
             const uint32_t mask = hits[32 * b + lane];
             if (!__any_sync(0xffffffffu, mask)) continue;
-            int at = (int)part[b];
-#pragma unroll 1
-            for (int j = 0; j < 8; j++) {
-                const uint32_t four = mask >> (4 * j) & 15u;
-                if (!__any_sync(0xffffffffu, four)) continue;
-                int below = 0, all_four = 0;
+            // how many of each eighth lie in the lanes up to this one: eight counts of at most 128 in two words
+            uint32_t upto[2], eighths[2];
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const uint32_t lanes = __ballot_sync(0xffffffffu, four >> c & 1u);
-                    below += __popc(lanes & ((1u << lane) - 1u));
-                    all_four += __popc(lanes);
+            for (int w = 0; w < 2; w++) {
+                uint32_t n = mask >> 16 * w & 0xffffu;  // four masks of four bits, then their counts, a byte each
+                n = (n & 0xfu) | (n & 0xf0u) << 4 | (n & 0xf00u) << 8 | (n & 0xf000u) << 12;
+                n = (n & 0x05050505u) + (n >> 1 & 0x05050505u);
+                n = (n & 0x03030303u) + (n >> 2 & 0x03030303u);
+                eighths[w] = n;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t x = __shfl_up_sync(0xffffffffu, n, o);
+                    if (lane >= o) n += x;
                 }
+                upto[w] = n;
+            }
+            int at = (int)part[b];
 #pragma unroll
-                for (int c = 0; c < 4; c++)
-                    if (four >> c & 1u) s.cand[at + below++] = (uint32_t)in.index(b, j, lane, c);
-                at += all_four;
+            for (int j = 0; j < 8; j++) {
+                const int sh = 8 * (j & 3);
+                const int mine = eighths[j >> 2] >> sh & 0xff, incl = upto[j >> 2] >> sh & 0xff;
+                int to = at + incl - mine;
+                for (uint32_t four = mask >> 4 * j & 15u; four; four &= four - 1)
+                    s.cand[to++] = (uint32_t)in.index(b, j, lane, __ffs((int)four) - 1);
+                at += (int)(__shfl_sync(0xffffffffu, upto[j >> 2], 31) >> sh & 0xff);
             }
         }
         __syncthreads();
