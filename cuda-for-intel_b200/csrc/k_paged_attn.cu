@@ -20,7 +20,7 @@
 // weights before these are split (times 2^8, so that small scales stay clear of f16's subnormals).
 //
 // Measured: 8 sequences of 9000 to 65000 positions, 32/8 heads of 128 in f16, 146 us, 6.2 TB/s; 64 of 16 to 4096, 12/2 heads
-// of 128 in Q8_0, 20.0 us (36 MB; the work of a tile, some 870 instructions of a warp, is what it waits for:
+// of 128 in Q8_0, 20.0 us (36 MB; the work of a tile, some 600 instructions of a warp, is what it waits for:
 // the warps of three CTAs issue in 45 % of the cycles); one of 672, 14/2 heads of 64 in f16, 6.3 us, 5.1 of them on the device:
 // launch, table, one round of loads and the join.
 #include "paged_cache.cuh"

@@ -1277,10 +1277,11 @@ extern "C" int cfi_sample(const float* logits, long long row_stride, int n_rows,
         lc.numAttrs = cluster ? 2 : 1;
         return cudaLaunchKernelEx(&lc, kernel, a);
     };
-    // Clusters while all run together: 37 rows of 151936 with all kinds of parameters take 30 us, a CTA a row 49; 74 rows
-    // 58 and 51, 256 rows 144 and 104.  Then rows that are long work for one CTA are left to clusters behind, where
-    // these are no more than run together and the rows are long: 256 rows of 151936 157 -> 104 us, of 32000 44 and
-    // 45; where no row is such that launch costs 10 us.
+    // Clusters while all run together: 37 rows of 151936 with all kinds of parameters take 30 us, a CTA a row 43; 74
+    // rows 55 and 46, 256 rows 136 and 100; one row of 1500 without a filter 5.2 and 10, 16 with all kinds 20 and 14.  Then
+    // rows that are long work for one CTA are left to clusters behind, where these are no more than run together and the
+    // rows are long: 256 rows of 151936 152 -> 100 us, of 65536 70 -> 60, of 32000 43 and 43; where no row is such that
+    // launch costs 9 us.
     const int at_once = 2 * cfi_sm_count() / SA_CTAS;
     const size_t slice_bytes = (size_t)a.slice * 4 + 32;  // a row's slice keeps its place within 16 bytes
     if (n_rows <= at_once) return (int)launch(sample_rows<false>, n_rows * SA_CTAS, slice_bytes, true);
