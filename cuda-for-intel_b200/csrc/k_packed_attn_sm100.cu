@@ -21,9 +21,9 @@
 //
 // Bound by the softmax: a block of a tile takes 16384 exponentials, 1024 cycles of an SM's exponential unit, and with
 // the maxima, the fp16 packing and two trips through tensor memory about 2000, half of it beside the other
-// tile's; its MMAs take 512 (heads of 64) or 1024.  One document of 16384 tokens, 12/2 heads of 128: 0.83 ms under the
-// power cap, 995 TFLOP/s (0.70 ms in short bursts); sixteen prompts of 1 to 2048 tokens 60 us, 530 TFLOP/s (the longest
-// tile's 17 blocks and the CTAs behind it); four chunks after 7000 tokens, 14/2 heads of 64, 91 us, 480 TFLOP/s.
+// tile's; its MMAs take 512 (heads of 64) or 1024.  One document of 16384 tokens, 12/2 heads of 128: 0.81 ms under the
+// power cap, 1017 TFLOP/s (0.69 ms in short bursts); sixteen prompts of 1 to 2048 tokens 53 us, 600 TFLOP/s (the longest
+// tile's 16 blocks and the CTAs behind it); four chunks after 7000 tokens, 14/2 heads of 64, 91 us, 480 TFLOP/s.
 #include "../../include/cfi_serve.h"
 #include "sm100_ptx.cuh"
 #include "cfi_kernels.h"
@@ -52,7 +52,7 @@ struct KaArgs {
     void* out;
     const int32_t *cu_q, *cu_kv;
     long long out_stride;
-    int n_seq, n_q, n_kv, group, tokens, tiles;  // tokens a tile has, tiles a CTA has
+    int n_seq, n_q, n_kv, n_kv_head, group, tokens, tiles;  // tokens a tile has, tiles a CTA has
     int out_f16, causal;
     float scale_log2;
     unsigned int* err;
@@ -96,6 +96,38 @@ CFI_DEV bool elect_one() {  // true in one lane of a converged warp
     return r != 0;
 }
 
+// The `index`-th pair of tiles (of `span` tokens) in the order in which they are begun.  No long one is left for the end: of
+// each 32 sequences that with the most keys first, a sequence's last pair, which sees the most, before the others, and the kv
+// heads of a pair together (sixteen prompts of 1 to 2048 tokens, 12/2 heads of 128: 58 us by sequences and heads as they
+// come, 53 so, 56 by the pairs' own lengths, which take longer to find; one of 2048, 32/8 heads of 128: 61 and 44).
+// Called by a warp; out: the pair's number in its sequence, or -1 where there are fewer pairs, and the sequence's
+// first query, queries, first key and keys.
+CFI_DEV void find_pair(const KaArgs& a, int span, int index, int* out) {
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) out[0] = -1;
+    __syncwarp();
+    for (int base = 0, acc = 0; base < a.n_seq && acc <= index; base += 32) {
+        const int s = base + lane;
+        int q0 = 0, nq = 0, k0 = 0, nk = 0;
+        if (s < a.n_seq) {
+            q0 = min(max(a.cu_q[s], 0), a.n_q);
+            nq = max(min(a.cu_q[s + 1], a.n_q) - q0, 0);
+            k0 = min(max(a.cu_kv[s], 0), a.n_kv);
+            nk = max(min(a.cu_kv[s + 1], a.n_kv) - k0, 0);
+        }
+        const int n = (nq + span - 1) / span;
+        int before = acc;
+        for (int l = 0; l < min(32, a.n_seq - base); l++) {
+            const int other = __shfl_sync(0xffffffffu, nk, l), pairs = __shfl_sync(0xffffffffu, n, l);
+            if (other > nk || (other == nk && l < lane)) before += pairs;
+        }
+        if (index >= before && index < before + n)
+            out[0] = n - 1 - (index - before), out[1] = q0, out[2] = nq, out[3] = k0, out[4] = nk;
+        acc += (int)__reduce_add_sync(0xffffffffu, n);
+    }
+    __syncwarp();
+}
+
 template <int D>
 __global__ void __launch_bounds__(KA_THREADS, 1)
     packed_attn(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
@@ -117,8 +149,9 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
     uint64_t* v_clean = bars + 2 * NS + 7;  // V rows past the end are zeroed
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * NS + 8);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    int* place = reinterpret_cast<int*>(tmem_slot + 2);  // what find_pair found
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kvh = blockIdx.y;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kvh = blockIdx.x % a.n_kv_head;
     pdl_launch_dependents();
     // all that needs no input: it runs beside the end of the kernel before
     if (tid == 0) {
@@ -145,41 +178,17 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
     }
     pdl_wait();  // lengths, q, k and v may come from the kernel before
 
-    // ---- which pair of tiles: sequence s, its pair number from the last (the longest) to the first ----
+    // ---- which pair of tiles ----
     const int span = a.tiles * a.tokens;
-    int s = -1, pair = 0, q0 = 0, nq = 0, k_from = 0, k_to = 0;
-    for (int base = 0, acc = 0; base < a.n_seq && s < 0; base += 32) {
-        int b0 = 0, n = 0, kb0 = 0, kb1 = 0;
-        if (base + lane < a.n_seq) {
-            kb0 = a.cu_kv[base + lane];
-            kb1 = a.cu_kv[base + lane + 1];
-            b0 = min(max(a.cu_q[base + lane], 0), a.n_q);
-            n = min(a.cu_q[base + lane + 1], a.n_q) - b0;
-        }
-        const int c = n > 0 ? (n + span - 1) / span : 0;
-        int incl = c;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += x;
-        }
-        const uint32_t hit = __ballot_sync(0xffffffffu, acc + incl > (int)blockIdx.x);
-        if (hit) {
-            const int l = __ffs(hit) - 1;
-            s = base + l;
-            q0 = __shfl_sync(0xffffffffu, b0, l);
-            nq = __shfl_sync(0xffffffffu, n, l);
-            k_from = __shfl_sync(0xffffffffu, kb0, l);
-            k_to = __shfl_sync(0xffffffffu, kb1, l);
-            pair = acc + __shfl_sync(0xffffffffu, incl, l) - 1 - (int)blockIdx.x;
-        }
-        acc += __shfl_sync(0xffffffffu, incl, 31);
-    }
-    if (s < 0) {
+    if (warp == 0) find_pair(a, span, blockIdx.x / a.n_kv_head, place);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const int pair = place[0], q0 = place[1], nq = place[2], k0 = place[3], nk = place[4];
+    if (pair < 0) {
         if (warp == KA_MMA_WARP) tmem_dealloc(0, KA_TMEM_COLS);
         return;
     }
-    const int k0 = min(max(k_from, 0), a.n_kv), nk = max(min(k_to, a.n_kv) - k0, 0);
     // keys that token t sees, and blocks that a tile needs (its last token sees the most)
     auto seen = [&](int t) { return a.causal ? max(0, min(nk, t + nk - nq + 1)) : nk; };
     auto first_token = [&](int x) { return pair * span + x * a.tokens; };
@@ -190,9 +199,6 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
     const int nb0 = blocks(0), nb1 = blocks(1), nmax = max(nb0, nb1);
     const bool cut = nmax * KA_N > nk;  // the last block runs past the sequence
 
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
     // all 512 columns: they begin at 0, and the MMAs' operands are constants
     constexpr uint32_t TM = 0;
     auto fail = [&](unsigned code) {
@@ -457,6 +463,7 @@ template <int D> int launch(const CfiPackedAttention* p, cudaStream_t stream) {
     a.n_seq = p->n_seq;
     a.n_q = p->n_q;
     a.n_kv = p->n_kv;
+    a.n_kv_head = p->n_kv_head;
     a.group = p->n_head / p->n_kv_head;
     a.tokens = KA_M / a.group;
     a.out_f16 = p->out_type;
@@ -471,6 +478,8 @@ template <int D> int launch(const CfiPackedAttention* p, cudaStream_t stream) {
     auto pairs = [&](int tiles) { return p->n_q / (tiles * a.tokens) + (p->n_seq < p->n_q ? p->n_seq : p->n_q); };
     const double share = p->causal && p->n_kv > 0 ? 1.0 - 0.5 * std::min(p->n_q, p->n_kv) / p->n_kv : 1.0;
     a.tiles = 2.2 * pairs(2) * p->n_kv_head * share <= cfi_sm_count() ? 1 : 2;
+    const long long grid = (long long)pairs(a.tiles) * p->n_kv_head;
+    if (grid > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
     CUtensorMap tq, tk, tv;
     // no keys at all: the maps still need an extent, and nothing is loaded
     if (!map_rows(&tq, p->q, D, p->n_head, p->q_stride, p->n_q, a.group, a.tokens) ||
@@ -481,7 +490,7 @@ template <int D> int launch(const CfiPackedAttention* p, cudaStream_t stream) {
     cfi_once_per_device(attr, [] { cudaFuncSetAttribute(packed_attn<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ka_smem<D>()); });
     const char* ep = getenv("CFI_PDL");
     cudaLaunchConfig_t lc = {};
-    lc.gridDim = dim3((unsigned)pairs(a.tiles), (unsigned)p->n_kv_head, 1);
+    lc.gridDim = dim3((unsigned)grid, 1, 1);
     lc.blockDim = dim3(KA_THREADS, 1, 1);
     lc.dynamicSmemBytes = ka_smem<D>();
     lc.stream = stream;
