@@ -22,7 +22,7 @@
 // Bound by the softmax: a block of a tile takes 16384 exponentials, 1024 cycles of an SM's exponential unit, and with
 // the maxima, the fp16 packing and two trips through tensor memory about 2000, half of it beside the other
 // tile's; its MMAs take 512 (heads of 64) or 1024.  One document of 16384 tokens, 12/2 heads of 128: 0.81 ms under the
-// power cap, 1017 TFLOP/s (0.69 ms in short bursts); sixteen prompts of 1 to 2048 tokens 53 us, 600 TFLOP/s (the longest
+// power cap, 1019 TFLOP/s (0.68 ms in short bursts); sixteen prompts of 1 to 2048 tokens 51 us, 620 TFLOP/s (the longest
 // tile's 16 blocks and the CTAs behind it); four chunks after 7000 tokens, 14/2 heads of 64, 91 us, 480 TFLOP/s.
 #include "../../include/cfi_serve.h"
 #include "sm100_ptx.cuh"
@@ -145,9 +145,9 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
     uint64_t* s_full = bars + 2 * NS;      // [2] scores of a block (and O up to the block before)
     uint64_t* p_full = bars + 2 * NS + 2;  // [2] its weights (a warp each arrives)
     uint64_t* o_full = bars + 2 * NS + 4;  // [2] O complete
-    uint64_t* q_full = bars + 2 * NS + 6;
-    uint64_t* v_clean = bars + 2 * NS + 7;  // V rows past the end are zeroed
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * NS + 8);
+    uint64_t* q_full = bars + 2 * NS + 6;   // [2]
+    uint64_t* v_clean = bars + 2 * NS + 8;  // V rows past the end are zeroed
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * NS + 9);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* place = reinterpret_cast<int*>(tmem_slot + 2);  // what find_pair found
 
@@ -166,8 +166,8 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
             mbar_init(&s_full[x], 1);
             mbar_init(&p_full[x], 4);
             mbar_init(&o_full[x], 1);
+            mbar_init(&q_full[x], 1);
         }
-        mbar_init(q_full, 1);
         mbar_init(v_clean, 1);
         *abort_flag = 0;
         fence_mbar_init();
@@ -212,10 +212,12 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
         bool ok = true;
         if (lane == 0 && nmax > 0) {
             const uint32_t rows = (uint32_t)(a.tokens * a.group);
-            mbar_arrive_expect_tx(q_full, a.tiles * DB * rows * 128);
-            for (int x = 0; x < a.tiles; x++)
-                for (int b = 0; b < DB; b++)  // a tile past the sequence loads rows that nothing uses
-                    tma_load_3d(sQ + x * TILE + b * BLK, &tq, 64 * b, kvh * a.group, q0 + first_token(x), q_full);
+            // only for a tile that sees keys: another's warps use the place at once
+            auto load_q = [&](int x) {
+                mbar_arrive_expect_tx(&q_full[x], DB * rows * 128);
+                for (int b = 0; b < DB; b++) tma_load_3d(sQ + x * TILE + b * BLK, &tq, 64 * b, kvh * a.group, q0 + first_token(x), &q_full[x]);
+            };
+            if (nb0 > 0) load_q(0);
             for (int i = 0; ok && i < 2 * nmax; i++) {
                 const int st = i % NS;
                 ok = mbar_wait(&empty[st], ((uint32_t)(i / NS) & 1) ^ 1, abort_flag);
@@ -223,6 +225,7 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
                 mbar_arrive_expect_tx(&full[st], TILE);
                 for (int b = 0; b < DB; b++)
                     tma_load_3d(ring + st * TILE + b * BLK, (i & 1) ? &tv : &tk, 64 * b, kvh, k0 + (i >> 1) * KA_N, &full[st]);
+                if (i == 0 && nb1 > 0) load_q(1);  // behind the first keys: tile A begins with these
             }
             if (!ok) fail(0xfb100);
         }
@@ -263,14 +266,15 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
                               (!first || kk > 0) ? 1u : 0u);
             };
             auto ready = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)) != 0; };
-            bool ok = ready(q_full, 0) && ready(&full[0], 0);
-            if (ok) {
-                tc_fence_after();
+            bool ok = ready(&full[0], 0);
 #pragma unroll
-                for (int x = 0; x < 2; x++)
-                    if ((x ? nb1 : nb0) > 0 && elect_one()) scores(x, 0);
-                if (elect_one()) mma_commit(&empty[0]);
-            }
+            for (int x = 0; x < 2; x++)
+                if (ok && (x ? nb1 : nb0) > 0) {
+                    ok = ready(&q_full[x], 0);
+                    tc_fence_after();
+                    if (ok && elect_one()) scores(x, 0);
+                }
+            if (ok && elect_one()) mma_commit(&empty[0]);
             for (int j = 0; ok && j < nmax; j++) {
                 const int iv = 2 * j + 1, ik = 2 * j + 2, sv = iv % NS, sk = ik % NS;
                 ok = ready(&full[sv], (uint32_t)(iv / NS) & 1);
@@ -385,7 +389,25 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
             if (lane == 0) fail(0xfb300 + warp);
         } else {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            const long long at = (long long)(q0 + t) * a.out_stride + (long long)(kvh * a.group + r % a.group) * D;
+            const long long at = valid ? (long long)(q0 + t) * a.out_stride + (long long)(kvh * a.group + r % a.group) * D : -1;
+            // The warp's 32 rows go through the shared memory of its rows of Q, which nothing reads any more, so that its stores
+            // are of whole rows (sixteen prompts of 100 to 1000 tokens, 12/2 heads of 128: 32.7 us with a lane storing its
+            // own row in pieces of 16 bytes, 31.0 so; a prompt of 631 in single tiles 11.7 and 11.8).
+            uint8_t* rows = sQ + x * TILE + (warp & 3) * (TILE / 4);
+            auto put = [&](int chunk, int chunks, uint4 v) {
+                *reinterpret_cast<uint4*>(rows + (lane * chunks + (chunk ^ (lane & 7))) * 16) = v;
+            };
+            auto store = [&](int chunks, int size, int first) {  // pieces of 16 bytes a row, bytes of a value, first value
+                __syncwarp();
+#pragma unroll 4
+                for (int i = lane; i < 32 * chunks; i += 32) {
+                    const int row = i / chunks, chunk = i % chunks;
+                    const long long to = __shfl_sync(0xffffffffu, at, row);
+                    const uint4 v = *reinterpret_cast<const uint4*>(rows + (row * chunks + (chunk ^ (row & 7))) * 16);
+                    if (to >= 0) *reinterpret_cast<uint4*>(static_cast<uint8_t*>(a.out) + (to + first) * size + 16 * chunk) = v;
+                }
+                __syncwarp();
+            };
 #pragma unroll
             for (int c = 0; c < D / 32; c++) {
                 uint32_t v[32];
@@ -394,9 +416,7 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
                 if (l == 0.0f)
 #pragma unroll
                     for (int i = 0; i < 32; i++) v[i] = 0u;
-                if (!valid) continue;
                 if (a.out_f16) {
-                    __half* o = static_cast<__half*>(a.out) + at + 32 * c;
 #pragma unroll
                     for (int i = 0; i < 32; i += 8) {
                         uint32_t w[4];
@@ -405,14 +425,19 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
                             const __half2 h = __floats2half2_rn(__uint_as_float(v[i + 2 * e]) * inv, __uint_as_float(v[i + 2 * e + 1]) * inv);
                             w[e] = *reinterpret_cast<const uint32_t*>(&h);
                         }
-                        *reinterpret_cast<uint4*>(o + i) = make_uint4(w[0], w[1], w[2], w[3]);
+                        put(4 * c + i / 8, D / 8, make_uint4(w[0], w[1], w[2], w[3]));
                     }
-                } else {
-                    float* o = static_cast<float*>(a.out) + at + 32 * c;
+                    if (c == D / 32 - 1) store(D / 8, 2, 0);
+                } else {  // half a row at a time
+                    constexpr int HALF = D / 64;
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4)
-                        *reinterpret_cast<float4*>(o + i) = make_float4(__uint_as_float(v[i]) * inv, __uint_as_float(v[i + 1]) * inv,
-                                                                        __uint_as_float(v[i + 2]) * inv, __uint_as_float(v[i + 3]) * inv);
+                    for (int i = 0; i < 32; i += 4) {
+                        float f[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) f[e] = __uint_as_float(v[i + e]) * inv;
+                        put(8 * (c % HALF) + i / 4, D / 8, make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])));
+                    }
+                    if (c % HALF == HALF - 1) store(D / 8, 4, 32 * (c - HALF + 1));
                 }
             }
         }

@@ -346,6 +346,15 @@ def test_packed_attention_every_tile_writes_its_own_rows(heads, kv, dim, n):
             packed_case(heads, kv, dim, [n], [n] if causal else [130], causal, ot=ot, seed=n)
 
 
+@pytest.mark.parametrize("heads,kv,dim", [(12, 2, 128), (14, 2, 64), (40, 2, 64)])
+@pytest.mark.parametrize("n", [400, 2000])
+def test_packed_attention_tiles_without_a_key(heads, kv, dim, n):
+    """Far more queries than keys: tiles that see none, alone and beside one that sees some, are zeros, on every run."""
+    for m in (1, 10, 45, 130):
+        for ot in (cfi.T_F32, cfi.T_F16):
+            packed_case(heads, kv, dim, [n, 5, n], [m, 9, m + 3], True, ot=ot, seed=m)
+
+
 def test_packed_attention_ranges_are_cut():
     """Ends past the tensors are cut to them: nothing outside is read or written."""
     heads, kv, dim, n = 4, 2, 64, 100
