@@ -16,6 +16,8 @@
 //     pipe works on one tile while the other is in its softmax;
 //   * warp 9 brings Q and the ring of K and V blocks by TMA.  V rows past the sequence's end are zeroed
 //     in shared memory (the next sequence's rows are there, and 0 x NaN would reach this one).
+// Where there are few tiles a CTA takes one: A and B are then the same rows over every other block of keys, and are joined at
+// the end by their maxima and sums, through shared memory.
 //
 // Tensor memory: S_A, S_B (128 columns each; P over the first 64), O_A, O_B (D columns each).
 //
@@ -23,12 +25,11 @@
 // the maxima, the fp16 packing and two trips through tensor memory about 2000, half of it beside the other
 // tile's; its MMAs take 512 (heads of 64) or 1024.  One document of 16384 tokens, 12/2 heads of 128: 0.81 ms under the
 // power cap, 1019 TFLOP/s (0.68 ms in short bursts); sixteen prompts of 1 to 2048 tokens 51 us, 620 TFLOP/s (the longest
-// tile's 16 blocks and the CTAs behind it); four chunks after 7000 tokens, 14/2 heads of 64, 91 us, 480 TFLOP/s.
+// tile's 16 blocks and the CTAs behind it); four chunks after 7000 tokens, 14/2 heads of 64, 81 us, 540 TFLOP/s.
 #include "../../include/cfi_serve.h"
 #include "sm100_ptx.cuh"
 #include "cfi_kernels.h"
 
-#include <algorithm>
 #include <math.h>
 #include <stdlib.h>
 #include <string.h>
@@ -197,6 +198,9 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
         return x < a.tiles && t < nq ? (seen(min(nq, t + a.tokens) - 1) + KA_N - 1) / KA_N : 0;
     };
     const int nb0 = blocks(0), nb1 = blocks(1), nmax = max(nb0, nb1);
+    // One tile: both halves of the CTA work on it, the first with every other block of keys, the second with those between
+    const bool split = a.tiles == 1;
+    const int n0 = split ? (nb0 + 1) / 2 : nb0, n1 = split ? nb0 / 2 : nb1;  // blocks of each half
     const bool cut = nmax * KA_N > nk;  // the last block runs past the sequence
 
     // all 512 columns: they begin at 0, and the MMAs' operands are constants
@@ -251,11 +255,11 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
             // descriptors of Q and the first slot; an offset of n bytes adds n / 16
             const uint64_t dq = sw128_kmajor_desc(smem_u32(sQ)), dk = sw128_kmajor_desc(smem_u32(ring)),
                            dv = sw128_mnmajor_desc(smem_u32(ring), BLK);
-            auto scores = [&](int x, int st) {  // S_x = Q_x K'
+            auto scores = [&](int x, int st, int q) {  // S_x = Q_q K'
 #pragma unroll
                 for (int kk = 0; kk < D / 16; kk++) {
                     const uint32_t off = (kk >> 2) * BLK + (kk & 3) * 32;
-                    mma_f16(TM + x * KA_N, dq + ((x * TILE + off) >> 4), dk + st * (TILE >> 4) + (off >> 4), id_s, kk > 0 ? 1u : 0u);
+                    mma_f16(TM + x * KA_N, dq + ((q * TILE + off) >> 4), dk + st * (TILE >> 4) + (off >> 4), id_s, kk > 0 ? 1u : 0u);
                 }
                 mma_commit(&s_full[x]);
             };
@@ -266,22 +270,62 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
                               (!first || kk > 0) ? 1u : 0u);
             };
             auto ready = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag)) != 0; };
-            bool ok = ready(&full[0], 0);
+            bool ok = true;
+            if (split) {
+                ok = ready(&q_full[0], 0);
 #pragma unroll
-            for (int x = 0; x < 2; x++)
-                if (ok && (x ? nb1 : nb0) > 0) {
-                    ok = ready(&q_full[x], 0);
-                    tc_fence_after();
-                    if (ok && elect_one()) scores(x, 0);
+                for (int x = 0; x < 2; x++)
+                    if (ok && (x ? n1 : n0) > 0) {
+                        ok = ready(&full[2 * x], 0);
+                        tc_fence_after();
+                        if (ok && elect_one()) {
+                            scores(x, 2 * x, 0);
+                            mma_commit(&empty[2 * x]);
+                        }
+                    }
+                for (int j = 0; ok && j < n0; j++) {
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        const int n = x ? n1 : n0, b = 2 * j + x, iv = 2 * b + 1, ik = iv + 3, sv = iv % NS, sk = ik % NS;
+                        if (j >= n) continue;
+                        ok = ready(&full[sv], (uint32_t)(iv / NS) & 1);
+                        if (ok && cut && b == nmax - 1) ok = ready(v_clean, 0);
+                        ok = ok && ready(&p_full[x], (uint32_t)j & 1);
+                        if (!ok) break;
+                        tc_fence_after();
+                        if (elect_one()) {
+                            values(x, sv, j == 0);
+                            mma_commit(&empty[sv]);
+                            if (j == n - 1) mma_commit(&o_full[x]);
+                        }
+                        if (j + 1 < n) {
+                            ok = ready(&full[sk], (uint32_t)(ik / NS) & 1);
+                            if (!ok) break;
+                            if (elect_one()) {
+                                scores(x, sk, 0);
+                                mma_commit(&empty[sk]);
+                            }
+                        }
+                    }
                 }
-            if (ok && elect_one()) mma_commit(&empty[0]);
-            for (int j = 0; ok && j < nmax; j++) {
+            } else {
+                ok = ready(&full[0], 0);
+#pragma unroll
+                for (int x = 0; x < 2; x++)
+                    if (ok && (x ? n1 : n0) > 0) {
+                        ok = ready(&q_full[x], 0);
+                        tc_fence_after();
+                        if (ok && elect_one()) scores(x, 0, x);
+                    }
+                if (ok && elect_one()) mma_commit(&empty[0]);
+            }
+            for (int j = 0; ok && !split && j < nmax; j++) {
                 const int iv = 2 * j + 1, ik = 2 * j + 2, sv = iv % NS, sk = ik % NS;
                 ok = ready(&full[sv], (uint32_t)(iv / NS) & 1);
                 if (ok && cut && j == nmax - 1) ok = ready(v_clean, 0);
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
-                    const int n = x ? nb1 : nb0;
+                    const int n = x ? n1 : n0;
                     if (ok && j < n) {
                         ok = ready(&p_full[x], (uint32_t)j & 1);
                         if (!ok) break;
@@ -295,7 +339,7 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
                     if (j + 1 < n) {
                         ok = ready(&full[sk], (uint32_t)(ik / NS) & 1);
                         if (!ok) break;
-                        if (elect_one()) scores(x, sk);
+                        if (elect_one()) scores(x, sk, x);
                     }
                     if (x == 1 && j + 1 < nmax && elect_one()) mma_commit(&empty[sk]);
                 }
@@ -305,15 +349,15 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
       }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(KA_REGS_SOFTMAX));
-        // ---- softmax: row r of tile x ----
-        const int x = warp >> 2, r = 32 * (warp & 3) + lane;
-        const int t = first_token(x) + r / a.group, n_blocks = x ? nb1 : nb0;
-        const bool valid = x < a.tiles && r < a.tokens * a.group && t < nq;
+        // ---- softmax: row r of tile x, or of the one tile ----
+        const int x = warp >> 2, r = 32 * (warp & 3) + lane, tile = split ? 0 : x;
+        const int t = first_token(tile) + r / a.group, n_blocks = x ? n1 : n0;
+        const bool valid = r < a.tokens * a.group && t < nq;
         const int limit = valid ? seen(t) : 0;
         const uint32_t trow = TM + ((uint32_t)(32 * (warp & 3)) << 16);
         const uint32_t ts = trow + x * KA_N, to = trow + 256 + x * D;
         // blocks below this one are seen whole by every row of the tile
-        const int n_whole = seen(first_token(x)) / KA_N;
+        const int n_whole = seen(first_token(tile)) / KA_N;
         float m_used = -INFINITY, l = 0.0f;
         bool ok = true;
         for (int j = 0; j < n_blocks; j++) {
@@ -326,8 +370,9 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
 #pragma unroll
             for (int c = 0; c < 4; c++) tmem_ld32(ts + 32 * c, sv[c]);
             tmem_ld_wait();
-            if (j >= n_whole) {
-                const int left = limit - j * KA_N;
+            const int block = split ? 2 * j + x : j;
+            if (block >= n_whole) {
+                const int left = limit - block * KA_N;
 #pragma unroll
                 for (int c = 0; c < 4; c++)
 #pragma unroll
@@ -383,17 +428,48 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
             if (lane == 0) mbar_arrive(&p_full[x]);
             l += both.x + both.y;
         }
-        if (ok && n_blocks > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[x], 0, abort_flag));
+        if (ok && (n_blocks > 0)) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[x], 0, abort_flag));
+        float keep = 1.0f, other = 0.0f;  // what the halves of a split tile count for
+        // the second half's values by four, [dims / 4][row of the warp], in Q's place; its maxima and sums in the ring's
+        float4* half_o = reinterpret_cast<float4*>(sQ + (warp & 3) * (TILE / 2)) + lane;
+        float2* half_ml = reinterpret_cast<float2*>(ring + TILE) + r;
+        if (split) {
+            // everything that was issued is done before anything is written over it
+            if (ok && (x ? n0 : n1) > 0) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[x ^ 1], 0, abort_flag));
+            tc_fence_after();
+            if (x == 1 && ok) {
+                *half_ml = make_float2(m_used, l);
+                if (n_blocks > 0)
+#pragma unroll
+                    for (int c = 0; c < D / 32; c++) {
+                        uint32_t v[32];
+                        tmem_ld32(to + 32 * c, v);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            half_o[(8 * c + i) * 32] = make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]),
+                                                                   __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
+                    }
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");  // the softmax warps, after a failed wait too
+            if (x == 0 && ok) {
+                const float2 ml = *half_ml;
+                const float m = fmaxf(m_used, ml.x);
+                keep = m_used == -INFINITY ? 0.0f : ex2(m_used - m);
+                other = ml.x == -INFINITY ? 0.0f : ex2(ml.x - m);
+                l = l * keep + ml.y * other;
+            }
+        }
         tc_fence_after();
         if (!ok) {
             if (lane == 0) fail(0xfb300 + warp);
-        } else {
+        } else if (!split || x == 0) {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             const long long at = valid ? (long long)(q0 + t) * a.out_stride + (long long)(kvh * a.group + r % a.group) * D : -1;
             // The warp's 32 rows go through the shared memory of its rows of Q, which nothing reads any more, so that its stores
             // are of whole rows (sixteen prompts of 100 to 1000 tokens, 12/2 heads of 128: 32.7 us with a lane storing its
             // own row in pieces of 16 bytes, 31.0 so; a prompt of 631 in single tiles 11.7 and 11.8).
-            uint8_t* rows = sQ + x * TILE + (warp & 3) * (TILE / 4);
+            uint8_t* rows = (split ? ring : sQ + x * TILE) + (warp & 3) * (TILE / 4);
             auto put = [&](int chunk, int chunks, uint4 v) {
                 *reinterpret_cast<uint4*>(rows + (lane * chunks + (chunk ^ (lane & 7))) * 16) = v;
             };
@@ -413,6 +489,15 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
                 uint32_t v[32];
                 if (n_blocks > 0) tmem_ld32(to + 32 * c, v);
                 tmem_ld_wait();
+                if (split && n1 > 0)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float4 h = half_o[(8 * c + i) * 32];
+                        v[4 * i] = __float_as_uint(fmaf(__uint_as_float(v[4 * i]), keep, h.x * other));
+                        v[4 * i + 1] = __float_as_uint(fmaf(__uint_as_float(v[4 * i + 1]), keep, h.y * other));
+                        v[4 * i + 2] = __float_as_uint(fmaf(__uint_as_float(v[4 * i + 2]), keep, h.z * other));
+                        v[4 * i + 3] = __float_as_uint(fmaf(__uint_as_float(v[4 * i + 3]), keep, h.w * other));
+                    }
                 if (l == 0.0f)
 #pragma unroll
                     for (int i = 0; i < 32; i++) v[i] = 0u;
@@ -495,14 +580,13 @@ template <int D> int launch(const CfiPackedAttention* p, cudaStream_t stream) {
     a.causal = p->causal;
     a.scale_log2 = p->scale * 1.4426950408889634f;
     a.err = cfi_device_error_word();
-    // Every sequence adds at most one pair that is not full.  A CTA takes a single tile, and is faster through its keys,
-    // where the SMs have room for all of them within the longest's time.  `share`: how long a tile is on the average,
-    // with sequences of one length (a prompt without a context: half).  Single tiles against pairs, us: one prompt of
-    // 631, 14/2 heads of 64, 12.1 and 14.8; of 2048, 12/2 heads of 128, 33 and 37; of 3000, 51 and 52; of 4096, 97 and
-    // 67; of 1024 with 32/8 heads 32 and 22; four of 100 to 1000 after 2000, 14/2 heads of 64, 53 and 35.
+    // Every sequence adds at most one pair that is not full.  Up to 5/4 pairs an SM a CTA takes a single tile, which halves the
+    // chain of the longest; more share the reads of K and V and the CTAs' beginnings and ends.  Single tiles against
+    // pairs, us: one prompt of 1024, 12/2 heads of 128, 15 and 22; of 3000 (145 pairs) 39 and 54; of 4096 (196) 67 and
+    // 69; of 5000 (240) 90 and 85; four chunks of 300 to 800 after 7000, 14/2 heads of 64 (134), 81 and 91; eight of 100 to
+    // 1000 after 2000 (244) 48 and 48; one of 2048, 32/8 heads of 128 (264), 58 and 43.
     auto pairs = [&](int tiles) { return p->n_q / (tiles * a.tokens) + (p->n_seq < p->n_q ? p->n_seq : p->n_q); };
-    const double share = p->causal && p->n_kv > 0 ? 1.0 - 0.5 * std::min(p->n_q, p->n_kv) / p->n_kv : 1.0;
-    a.tiles = 2.2 * pairs(2) * p->n_kv_head * share <= cfi_sm_count() ? 1 : 2;
+    a.tiles = 4LL * pairs(2) * p->n_kv_head <= 5LL * cfi_sm_count() ? 1 : 2;
     const long long grid = (long long)pairs(a.tiles) * p->n_kv_head;
     if (grid > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
     CUtensorMap tq, tk, tv;
