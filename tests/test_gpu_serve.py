@@ -337,13 +337,25 @@ def test_packed_attention_bad_neighbour():
         packed_case(heads, kv, dim, [200, 3, 130], [333, 3, 140], poison=True)
 
 
-@pytest.mark.parametrize("heads,kv,dim,n", [(12, 2, 128, 2048), (14, 2, 64, 1500), (2, 2, 64, 9000)])
+@pytest.mark.parametrize("heads,kv,dim,n", [(12, 2, 128, 2048), (14, 2, 64, 1500), (2, 2, 64, 9000), (16, 16, 64, 3000),
+                                             (40, 2, 64, 1500), (32, 8, 128, 1500)])
 def test_packed_attention_every_tile_writes_its_own_rows(heads, kv, dim, n):
     """More single tiles than SMs, of which the short ones end long before their neighbours: each row is written by
     its own tile only, in both output types, with and without the mask."""
     for causal in (True, False):
         for ot in (cfi.T_F32, cfi.T_F16):
             packed_case(heads, kv, dim, [n], [n] if causal else [130], causal, ot=ot, seed=n)
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(12, 2, 128), (14, 2, 64), (8, 8, 128), (64, 1, 64)])
+@pytest.mark.parametrize("n", [3, 40, 130])
+def test_packed_attention_many_sequences(heads, kv, dim, n):
+    """Sequences of all lengths in no order, empty ones, contexts, more queries than keys: few tiles and many."""
+    rng = np.random.default_rng(n + heads)
+    nq = [int(x) for x in rng.integers(0, 260, n)]
+    nk = [max(0, q + int(x)) for q, x in zip(nq, rng.choice([0, 0, 0, 500, -60], n))]
+    for causal in (True, False):
+        packed_case(heads, kv, dim, nq, nk, causal, ot=cfi.T_F16, seed=n)
 
 
 @pytest.mark.parametrize("heads,kv,dim", [(12, 2, 128), (14, 2, 64), (40, 2, 64)])
