@@ -13,7 +13,8 @@
 namespace {
 
 // Items of a thread.  Measured with 1, 2 and 4 (f16 rows of 8 x 128, Q8_0 pages): reading back 65537 rows 78, 65.9
-// (6.2 TB/s of reads and writes) and 80 us; storing 8192 rows 12.7, 12.7 and 13.8 us, a step's 48 rows 1.2, 1.5 and 1.9.
+// (6.2 TB/s of reads and writes) and 80 us; storing 8192 rows 12.7, 12.7 and 13.8 us (10.3, 5 TB/s, since the maximum of f16
+// rows is taken in f16 and the bytes come from one conversion: it is bound by issue), a step's 48 rows 1.2, 1.5 and 1.9.
 constexpr int PC_THREADS = 256, PC_STORE_ITEMS = 1, PC_LOAD_ITEMS = 2;
 
 struct PcArgs {
@@ -60,6 +61,19 @@ template <int D> struct PcPlace {
     CFI_DEV int off(const PcArgs& a) const { return (int)(slot & ((1 << a.page_shift) - 1)); }
     CFI_DEV long long value(long long stride) const { return (long long)t * stride + h * D + g * 8; }
 };
+
+CFI_DEV __half2 abs_h2(uint32_t w) {
+    w &= 0x7fff7fffu;
+    return *reinterpret_cast<const __half2*>(&w);
+}
+CFI_DEV int to_s8(float x) {  // to the nearest, ties to even; the ends at +-128, a NaN 0
+    int q;
+    asm("cvt.rni.sat.s8.f32 %0, %1;" : "=r"(q) : "f"(x));
+    return q;
+}
+CFI_DEV uint32_t bytes_of(int a, int b, int c, int d) {
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
 
 template <int D, bool Q8, bool SRC_F16>
 __global__ void __launch_bounds__(PC_THREADS) paged_kv_store(const PcArgs a) {
@@ -108,30 +122,39 @@ __global__ void __launch_bounds__(PC_THREADS) paged_kv_store(const PcArgs a) {
                 if (ok) *reinterpret_cast<uint4*>(region + ((size_t)off * D + p[e].g * 8) * 2) = raw;
                 continue;
             }
-            float m = 0.0f;
-            uint32_t nan = 0;  // fmaxf drops a NaN: a block that has one gets a NaN scale
+            float m;  // of a block that has a NaN: NaN, and so its scale
+            if (SRC_F16) {
+                __half2 h = abs_h2(raw.x);
+                h = __hmax2_nan(__hmax2_nan(h, abs_h2(raw.y)), __hmax2_nan(abs_h2(raw.z), abs_h2(raw.w)));
+                h = __hmax2_nan(h, __lowhigh2highlow(h));
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                m = fmaxf(m, fabsf(x[j]));
-                nan |= (uint32_t)(x[j] != x[j]);
-            }
+                for (int o = 1; o < 4; o <<= 1) h = __hmax2_nan(h, __shfl_xor_sync(0xffffffffu, h, o));
+                m = __low2float(h);
+            } else {
+                m = 0.0f;
+                uint32_t nan = 0;
 #pragma unroll
-            for (int o = 1; o < 4; o <<= 1) {
-                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                nan |= __shfl_xor_sync(0xffffffffu, nan, o);
+                for (int j = 0; j < 8; j++) {
+                    m = fmaxf(m, fabsf(x[j]));  // drops a NaN
+                    nan |= (uint32_t)(x[j] != x[j]);
+                }
+                if (nan) m = __uint_as_float(0x7fffffffu);
+#pragma unroll
+                for (int o = 1; o < 4; o <<= 1) {
+                    const float other = __shfl_xor_sync(0xffffffffu, m, o);
+                    m = other != other ? other : m != m ? m : fmaxf(m, other);
+                }
             }
             const float d = m / 127.0f, id = d > 0.0f ? 1.0f / d : 0.0f;
-            uint32_t w[2] = {0, 0};
+            int q[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int q = max(-127, min(127, __float2int_rn(x[j] * id)));
-                w[j >> 2] |= (uint32_t)(q & 0xff) << (8 * (j & 3));
-            }
+            for (int j = 0; j < 8; j++) q[j] = to_s8(x[j] * id);
+            const uint32_t w[2] = {bytes_of(q[0], q[1], q[2], q[3]), bytes_of(q[4], q[5], q[6], q[7])};
             if (!ok) continue;
             *reinterpret_cast<uint2*>(region + (size_t)off * D + p[e].g * 8) = make_uint2(w[0], w[1]);
             if ((p[e].g & 3) == 0)
                 *reinterpret_cast<uint16_t*>(region + (size_t)(D << a.page_shift) + ((size_t)off * (D / 32) + p[e].g / 4) * 2) =
-                    nan ? (uint16_t)0x7fff : f2h_bits(d);
+                    d != d ? (uint16_t)0x7fff : f2h_bits(d);
         }
 }
 
