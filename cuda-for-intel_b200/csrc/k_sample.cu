@@ -11,9 +11,10 @@
 //
 // All three filters keep a run from the top of the order (larger z first, then lower index).  Where that run
 // is short -- it is, when a top-k or a nucleus of a language model's logits is asked for -- the bins of a
-// histogram of max - z say down to which depth it can reach, the few elements above that depth are gathered in
-// the cluster's first CTA, and that CTA finishes alone with them in registers.  The gathering needs no exact z: bins
-// of (max logit - logit) / T are 1/64 wide, far above the rounding of z, and one bin more is taken.
+// histogram of max - z, of the largest of each group of elements or of all, say down to which depth it can reach, the
+// few elements above that depth are gathered in one CTA, and that CTA finishes alone with them in registers.  The
+// gathering needs no exact z: bins of (max logit - logit) / T are at least 1/64 wide, far above the rounding of z, and
+// one bin more is taken.
 //
 // A long nucleus: the bin that its end falls in is gathered and ranked alone, and the kept weights are summed over the row.
 //
