@@ -15,9 +15,13 @@
 // and the two halves of its result are added.  The same holds for the weights.  A group of more than 8
 // heads is cut into chunks that read the rows again (from L2).
 //
+// A weight is split at 2^15 times its size: what f16 leaves of it ends at 2^-39 of the largest, and a long tail of small
+// weights stays as large as the sum of them that the result is divided by.
+//
 // Q8_0: int8 values are exact in f16, so K enters the MMA as whole numbers, one block of 32 dims at
 // a time, and each block's sum is multiplied by its scale in 32 bits; V's scales are multiplied into the
-// weights before these are split (times 2^8, so that small scales stay clear of f16's subnormals).
+// weights before these are split, in units of the power of two above the largest scale so far (the sums are rescaled where
+// that grows, as they are where the maximum does).
 //
 // Measured: 8 sequences of 9000 to 65000 positions, 32/8 heads of 128 in f16, 146 us, 6.2 TB/s; 64 of 16 to 4096, 12/2 heads
 // of 128 in Q8_0, 20.0 us (36 MB; the work of a tile, some 600 instructions of a warp, is what it waits for:
@@ -40,7 +44,8 @@ using namespace sm100;
 constexpr int PA_WARPS = 4;        // of a CTA; twice as many where a CTA has a pair and an SM to itself
 constexpr int PA_HEADS = 8;        // query heads of a chunk
 constexpr int PA_TILE = 16;        // positions; a page is a multiple of it
-constexpr float PA_V_UNIT = 256.0f;
+constexpr float PA_TOP = 15.0f;    // log2 of the largest weight as it is split: f16 ends at 65504
+constexpr float PA_LEAST_V = -23.0f, PA_MOST_V = 16.0f;  // f16 scales are below 2^these
 // What beginning and ending a pair costs, in tiles: a run's share of the list counts it, so that CTAs with
 // many short sequences get fewer tiles.
 constexpr int PA_FIXED = 5;
@@ -98,6 +103,10 @@ CFI_DEV void mma_f16f32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 CFI_DEV uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+CFI_DEV __half2 abs_h2(uint32_t w) {
+    w &= 0x7fff7fffu;
+    return *reinterpret_cast<const __half2*>(&w);
+}
 // (x, y) as f16 and what the rounding left, as f16: 22 bits together
 CFI_DEV void split(float x, float y, uint32_t* hi, uint32_t* lo) {
     const __half2 h = __floats2half2_rn(x, y);
@@ -324,7 +333,9 @@ __global__ void __launch_bounds__(W * 32, (PaShape<D, Q8, W>::CTAS)) paged_attn(
             cp_async_commit();
         };
 
-        float o[NT][4], m = -INFINITY, l = 0.0f;
+        // Q8_0: V's scales have been below 2^top_v; weights, l and o have 2^-top_v in them
+        float o[NT][4], m = -INFINITY, l = 0.0f, top_v = Q8 ? PA_LEAST_V : 0.0f;
+        __half2 limit_v = __float2half2_rn(ex2(top_v));
 #pragma unroll
         for (int j = 0; j < NT; j++)
 #pragma unroll
@@ -405,7 +416,7 @@ __global__ void __launch_bounds__(W * 32, (PaShape<D, Q8, W>::CTAS)) paged_attn(
                     for (int e = 0; e < 4; e++) o[j][e] *= alpha;
                 m = mn;
             }
-            const float sub = m == -INFINITY ? 0.0f : m;
+            const float sub = (m == -INFINITY ? 0.0f : m) + (top_v - PA_TOP);
             float p[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) p[e] = ex2(s[e] - sub);
@@ -434,6 +445,23 @@ __global__ void __launch_bounds__(W * 32, (PaShape<D, Q8, W>::CTAS)) paged_attn(
                         sc[n][0] = w.x, sc[n][1] = w.y;
                     }
                 }
+                // a lane looks at two of the tile's scales
+                const __half2 d = abs_h2(lds32(ss + S::SCALES + (lane * 4 & (D - 1))));
+                if (__any_sync(0xffffffffu, !__hblt2(d, limit_v))) {
+                    // the exponent of the largest, cut where that is an infinity or a NaN
+                    const uint32_t exponent = __float_as_uint(fmaxf(__low2float(d), __high2float(d))) >> 23;
+                    const float grown = fmaxf(top_v, fminf((float)__reduce_max_sync(0xffffffffu, exponent) - 126.0f, PA_MOST_V));
+                    const float f = ex2(top_v - grown);
+                    l *= f;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) p[e] *= f;
+#pragma unroll
+                    for (int j = 0; j < NT; j++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) o[j][e] *= f;
+                    top_v = grown;
+                    limit_v = __float2half2_rn(ex2(grown));
+                }
 #pragma unroll
                 for (int b = 0; b < NB; b++) {
                     uint32_t pf[4], bw[2][4];
@@ -441,7 +469,7 @@ __global__ void __launch_bounds__(W * 32, (PaShape<D, Q8, W>::CTAS)) paged_attn(
                     for (int n = 0; n < 2; n++) {
                         const float d0 = h2f_bits((uint16_t)(sc[n][b >> 1] >> (16 * (b & 1)))),
                                     d1 = h2f_bits((uint16_t)(sc[n][NB / 2 + (b >> 1)] >> (16 * (b & 1))));
-                        split(p[2 * n] * PA_V_UNIT * d0, p[2 * n + 1] * PA_V_UNIT * d1, &pf[2 * n], &pf[2 * n + 1]);
+                        split(p[2 * n] * d0, p[2 * n + 1] * d1, &pf[2 * n], &pf[2 * n + 1]);
                         // dims 32 b + 4 g .. + 3 of two positions, interleaved: column g of MMA e is dim 32 b + 4 g + e
                         const uint32_t wa = lds32(sv + chunk_at<D, Q8, true>(8 * n + 2 * c, 2 * b + (g >> 2)) + 4 * (g & 3)) ^ 0x80808080u;
                         const uint32_t wb = lds32(sv + chunk_at<D, Q8, true>(8 * n + 2 * c + 1, 2 * b + (g >> 2)) + 4 * (g & 3)) ^ 0x80808080u;
@@ -471,7 +499,7 @@ __global__ void __launch_bounds__(W * 32, (PaShape<D, Q8, W>::CTAS)) paged_attn(
                 for (int e = 0; e < 2; e++) {
                     float f[4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) f[i] = (o[4 * b + i][e] + o[4 * b + i][e + 2]) * (1.0f / PA_V_UNIT);
+                    for (int i = 0; i < 4; i++) f[i] = o[4 * b + i][e] + o[4 * b + i][e + 2];
                     *reinterpret_cast<float4*>(mine_o + 32 * b + 8 * c + 4 * e) = make_float4(f[0], f[1], f[2], f[3]);
                 }
         } else {
@@ -479,7 +507,7 @@ __global__ void __launch_bounds__(W * 32, (PaShape<D, Q8, W>::CTAS)) paged_attn(
             for (int j = 0; j < NT; j++)
                 *reinterpret_cast<float2*>(mine_o + 8 * j + 2 * c) = make_float2(o[j][0] + o[j][2], o[j][1] + o[j][3]);
         }
-        if (c == 0) *reinterpret_cast<float2*>(mine_o + D) = make_float2(m, l);
+        if (c == 0) *reinterpret_cast<float2*>(mine_o + D) = make_float2(m + top_v, l);
         __syncthreads();
         const bool done = t0 == 0 && t1 == n_tiles;
         if (!done) {

@@ -1,0 +1,116 @@
+"""The serving operators at the ends of their ranges: one key that outweighs a long flat tail, small and large
+values of Q8_0 blocks.
+
+Bounds, as in test_gpu_serve.py: a score is off by at most EPS_S times the sum of its products' magnitudes times
+the scale, a weight by that much twice (numerator and sum) and 2^-20 twice for the exponential.  Three more terms count
+here.  A weight is held to 22 bits or to 2^-40 of the largest, whichever is coarser.  A sum of n positions is n / 16
+additions in 32 bits one after another, each off by an ulp of 2^-23 at most.  An output is compared with its own
+size where the largest value has no part in it."""
+import math
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+import cfi_b200 as cfi  # noqa: E402
+from test_gpu_serve import DEV, EPS_S, attend, garbage_pool, pool_rows, stream  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+F16, F32, Q8 = cfi.T_F16, cfi.T_F32, cfi.Q8_0
+
+
+def filled(ty, kv, dim, page, k, v):
+    """Pools that hold the rows k and v [position, kv * dim] at slots 0, 1, ..."""
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(1)
+    pages = -(-k.shape[0] // page)
+    pools = [garbage_pool(ty, pages, kv, page, dim, gen) for _ in "kv"]
+    cache = cfi.paged_cache(ty, pools[0].data_ptr(), pools[1].data_ptr(), pages, page, kv, dim)
+    slots = torch.arange(k.shape[0], device=DEV)
+    cfi.paged_kv_store(cache, k.data_ptr(), v.data_ptr(), slots.data_ptr(), k.shape[0], stream=stream())
+    rows = [pool_rows(p, ty, pages, kv, page, dim)[:k.shape[0]] for p in pools]
+    return cache, pools, rows
+
+
+def attention(cache, q, table, lens, scale):
+    batch, width = q.shape
+    out = torch.full_like(q, 7.0)
+    cfi.paged_attention(cache, q.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(), batch, width // cache.head_dim,
+                        table.shape[1], scale, stream=stream())
+    torch.cuda.synchronize()
+    return out.double().cpu().numpy().reshape(batch, -1, cache.head_dim)
+
+
+# ---- weights ----
+@pytest.mark.parametrize("ty", [F16, Q8])
+@pytest.mark.parametrize("heads,kv,dim,batch,n", [(14, 2, 64, 64, 65536), (32, 8, 128, 8, 65000), (12, 2, 128, 1, 700)])
+@pytest.mark.parametrize("gap", [10.0, 14.3, 17.0, 17.5, 18.7])
+def test_one_key_over_a_long_flat_tail(ty, heads, kv, dim, batch, n, gap):
+    """The first key outweighs each of the others by e^gap and has no value; the others are equal and share one page."""
+    page = 16
+    scale = 1.0 / math.sqrt(dim)
+    k = torch.zeros(2 * page, kv * dim, device=DEV)
+    k[0] = 1.0
+    v = torch.ones(2 * page, kv * dim, device=DEV)
+    v[0] = 0.0
+    cache, pools, (K, V) = filled(ty, kv, dim, page, k, v)
+    width = -(-n // page)
+    table = torch.ones(batch, width, dtype=torch.int32, device=DEV)
+    table[:, 0] = 0
+    lens = torch.full((batch,), n, dtype=torch.int32, device=DEV)
+    q = torch.full((batch, heads * dim), gap / (dim * scale), device=DEV)
+    got = attention(cache, q, table, lens, scale)
+    score = float(q[0, 0].double()) * scale * K[0, 0].sum()
+    tail = (n - 1) * math.exp(-score)
+    want = tail / (1 + tail) * float(V[1, 0, 0])
+    tol = want * (2 * EPS_S * score + 2 * 2.0 ** -20 + -(-n // 16) * 2.0 ** -23) + n * 2.0 ** -40
+    assert np.abs(got - want).max() <= tol, (float(np.abs(got - want).max()) / want, tol / want)
+
+
+def values_case(ty, heads, kv, dim, n, amplitude, seed=0):
+    """Random scores over n positions of values of the given amplitude [position, 1 or dim]; compared block by block of 32 dims."""
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(seed + n)
+    page = 32
+    k = torch.randn(n, kv * dim, generator=gen, device=DEV)
+    v = torch.randn(n, kv, dim, generator=gen, device=DEV).clamp(-3, 3) * amplitude.to(DEV)[:, None]
+    cache, pools, (K, V) = filled(ty, kv, dim, page, k, v.reshape(n, -1).contiguous())
+    q = torch.randn(1, heads * dim, generator=gen, device=DEV)
+    table = torch.arange(-(-n // page), dtype=torch.int32, device=DEV)[None].contiguous()
+    lens = torch.tensor([n], dtype=torch.int32, device=DEV)
+    scale = 1.0 / math.sqrt(dim)
+    got = attention(cache, q, table, lens, scale)[0]
+    Q = q.double().cpu().numpy().reshape(heads, dim)
+    g = heads // kv
+    for h in range(kv):
+        qq = Q[h * g:(h + 1) * g]
+        want = attend(qq, K[:, h], V[:, h], scale)
+        S = float((np.abs(qq) @ np.abs(K[:, h]).T).max() * scale)
+        largest = np.abs(V[:, h]).max()
+        for b in range(0, dim, 32):
+            tol = (2 * EPS_S * S + 2 * 2.0 ** -20 + -(-n // 16) * 2.0 ** -23) * np.abs(V[:, h, b:b + 32]).max() + n * 2.0 ** -40 * largest
+            err = np.abs(got[h * g:(h + 1) * g, b:b + 32] - want[:, b:b + 32])
+            assert (err <= tol).all(), (h, b, float((err / tol).max()))
+
+
+@pytest.mark.parametrize("ty", [F16, Q8])
+@pytest.mark.parametrize("heads,kv,dim", [(14, 2, 64), (12, 2, 128)])
+@pytest.mark.parametrize("n", [5, 600, 9000])
+def test_values_of_all_sizes(ty, heads, kv, dim, n):
+    """Values from f16's smallest normal ones to its largest, the same everywhere, growing and falling along the positions, and
+    of another size in each block of 32 dims."""
+    one = torch.ones(n, 1)
+    for size in (1.0, 1.3e-3, 1.3e-4, 2e4):
+        values_case(ty, heads, kv, dim, n, one * size)
+    steps = torch.linspace(0, 1, n)[:, None]
+    values_case(ty, heads, kv, dim, n, 1e-3 * 1e7 ** steps)
+    values_case(ty, heads, kv, dim, n, 1e4 * 1e-7 ** steps)
+    blocks = torch.tensor([1e-3, 30.0, 1.0, 1e3])[torch.arange(dim) // 32 % 4][None].expand(n, dim)
+    values_case(ty, heads, kv, dim, n, blocks)
+    values_case(ty, heads, kv, dim, n, blocks.roll(32, 1))
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(14, 2, 64), (12, 2, 128)])
+def test_values_of_q8_0_past_f16(heads, kv, dim):
+    """A block's scale may be any f16, its values then pass f16's range."""
+    values_case(Q8, heads, kv, dim, 700, torch.full((700, 1), 1e6))
