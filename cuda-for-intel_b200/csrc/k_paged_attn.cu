@@ -416,10 +416,10 @@ __global__ void __launch_bounds__(W * 32, (PaShape<D, Q8, W>::CTAS)) paged_attn(
                     for (int e = 0; e < 4; e++) o[j][e] *= alpha;
                 m = mn;
             }
-            const float sub = (m == -INFINITY ? 0.0f : m) + (top_v - PA_TOP);
+            const float sub = m == -INFINITY ? 0.0f : m, rise = PA_TOP - top_v;  // added last: a large score would swallow it
             float p[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) p[e] = ex2(s[e] - sub);
+            for (int e = 0; e < 4; e++) p[e] = ex2(s[e] - sub + rise);
             l += (p[0] + p[1]) + (p[2] + p[3]);
             // ---- weighted values ----
             if (!Q8) {
@@ -493,13 +493,15 @@ __global__ void __launch_bounds__(W * 32, (PaShape<D, Q8, W>::CTAS)) paged_attn(
         float* meet = reinterpret_cast<float*>(smem);
         float* mine_o = meet + warp * S::MEET + g * S::MEET_ROW;
         if (Q8) {
+            const float back = ex2(top_v);  // each warp has had scales of its own
+            l *= back;
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     float f[4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) f[i] = o[4 * b + i][e] + o[4 * b + i][e + 2];
+                    for (int i = 0; i < 4; i++) f[i] = (o[4 * b + i][e] + o[4 * b + i][e + 2]) * back;
                     *reinterpret_cast<float4*>(mine_o + 32 * b + 8 * c + 4 * e) = make_float4(f[0], f[1], f[2], f[3]);
                 }
         } else {
@@ -507,7 +509,7 @@ __global__ void __launch_bounds__(W * 32, (PaShape<D, Q8, W>::CTAS)) paged_attn(
             for (int j = 0; j < NT; j++)
                 *reinterpret_cast<float2*>(mine_o + 8 * j + 2 * c) = make_float2(o[j][0] + o[j][2], o[j][1] + o[j][3]);
         }
-        if (c == 0) *reinterpret_cast<float2*>(mine_o + D) = make_float2(m + top_v, l);
+        if (c == 0) *reinterpret_cast<float2*>(mine_o + D) = make_float2(m, l);
         __syncthreads();
         const bool done = t0 == 0 && t1 == n_tiles;
         if (!done) {

@@ -114,3 +114,23 @@ def test_values_of_all_sizes(ty, heads, kv, dim, n):
 def test_values_of_q8_0_past_f16(heads, kv, dim):
     """A block's scale may be any f16, its values then pass f16's range."""
     values_case(Q8, heads, kv, dim, 700, torch.full((700, 1), 1e6))
+
+
+@pytest.mark.parametrize("ty", [F16, Q8])
+@pytest.mark.parametrize("heads,kv,dim", [(14, 2, 64), (12, 2, 128)])
+@pytest.mark.parametrize("n", [5, 600, 9000])
+def test_large_equal_scores(ty, heads, kv, dim, n):
+    """Scores of 2e8 that are all the same: the mean of values whose size changes along the positions, as if they were zero."""
+    page = 16
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(n)
+    k = torch.full((n, kv * dim), 100.0, device=DEV)
+    for grow in (1e6, 1e-6):
+        v = torch.randn(n, kv * dim, generator=gen, device=DEV).clamp(-3, 3) * max(1.0, 1 / grow) * 1e-3 * grow ** torch.linspace(0, 1, n, device=DEV)[:, None]
+        cache, pools, (K, V) = filled(ty, kv, dim, page, k, v)
+        q = torch.full((1, heads * dim), 3e5, device=DEV)
+        table = torch.arange(-(-n // page), dtype=torch.int32, device=DEV)[None].contiguous()
+        got = attention(cache, q, table, torch.tensor([n], dtype=torch.int32, device=DEV), 1.0 / math.sqrt(dim))[0]
+        want = np.repeat(V.mean(0), heads // kv, axis=0)
+        tol = (2 * 2.0 ** -20 + -(-n // 16) * 2.0 ** -23 + n * 2.0 ** -40) * np.abs(V).max()
+        assert np.abs(got - want).max() <= tol, (grow, float(np.abs(got - want).max() / tol))
