@@ -15,8 +15,9 @@
 // and the two halves of its result are added.  The same holds for the weights.  A group of more than 8
 // heads is cut into chunks that read the rows again (from L2).
 //
-// A weight is split at 2^15 times its size: what f16 leaves of it ends at 2^-39 of the largest, and a long tail of small
-// weights stays as large as the sum of them that the result is divided by.
+// A query head is split times the power of two that brings its largest value to 2^14 .. 2^15 (the scores are divided by it again
+// in the exponent), and a weight at 2^15 times its size: what f16 leaves of either ends at 2^-39 of the largest, and a long tail
+// of small weights stays as large as the sum of them that the result is divided by.
 //
 // Q8_0: int8 values are exact in f16, so K enters the MMA as whole numbers, one block of 32 dims at
 // a time, and each block's sum is multiplied by its scale in 32 bits; V's scales are multiplied into the
@@ -342,22 +343,33 @@ __global__ void __launch_bounds__(W * 32, (PaShape<D, Q8, W>::CTAS)) paged_attn(
             for (int e = 0; e < 4; e++) o[j][e] = 0.0f;
 #pragma unroll
         for (int i = 0; i < S::STAGES - 1; i++) fetch(i);
-        uint32_t qf[KK][4];  // in log2 units, split
+        uint32_t qf[KK][4];  // in log2 units over `unit`, split
+        float largest = 0.0f;  // a NaN is passed over
 #pragma unroll
         for (int kk = 0; kk < KK; kk++)
 #pragma unroll
             for (int x = 0; x < 2; x++) {
                 const uint32_t raw = __float_as_uint(qv[kk][x].x);
                 const float2 f = a.q_f16 ? __half22float2(*reinterpret_cast<const __half2*>(&raw)) : qv[kk][x];
-                split(f.x * a.scale_log2, f.y * a.scale_log2, &qf[kk][2 * x], &qf[kk][2 * x + 1]);
+                qv[kk][x] = make_float2(f.x * a.scale_log2, f.y * a.scale_log2);
+                largest = fmaxf(largest, fmaxf(fabsf(qv[kk][x].x), fabsf(qv[kk][x].y)));
             }
+        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+        // 2^(its exponent - 14) and the other way round, both normal: below 2^-111 the largest stays below 2^14
+        const uint32_t exponent = max(__float_as_uint(largest) >> 23, 15u);
+        const float unit = __uint_as_float((exponent - 14) << 23), per_unit = __uint_as_float((268 - exponent) << 23);
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++)
+#pragma unroll
+            for (int x = 0; x < 2; x++) split(qv[kk][x].x * per_unit, qv[kk][x].y * per_unit, &qf[kk][2 * x], &qf[kk][2 * x + 1]);
         for (int i = 0; i < mine; i++) {
             if ((i + S::STAGES - 1) % 32 == 0) ids = load_ids(i + S::STAGES - 1);
             fetch(i + S::STAGES - 1);
             cp_async_wait<S::STAGES - 1>();
             __syncwarp();
             const uint32_t sk = ring + (i % S::STAGES) * S::STAGE, sv = sk + S::ROWS, ss = sk + 2 * S::ROWS;
-            // ---- scores of positions 2c, 2c+1 and 8+2c, 9+2c for head g ----
+            // ---- scores, over `unit`, of positions 2c, 2c+1 and 8+2c, 9+2c for head g ----
             float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             if (!Q8) {
                 float acc[2][4] = {};
@@ -408,7 +420,7 @@ __global__ void __launch_bounds__(W * 32, (PaShape<D, Q8, W>::CTAS)) paged_attn(
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             if (__any_sync(0xffffffffu, mx > m)) {
-                const float mn = fmaxf(m, mx), alpha = m == -INFINITY ? 0.0f : ex2(m - mn);
+                const float mn = fmaxf(m, mx), alpha = m == -INFINITY ? 0.0f : ex2((m - mn) * unit);
                 l *= alpha;
 #pragma unroll
                 for (int j = 0; j < NT; j++)
@@ -419,7 +431,7 @@ __global__ void __launch_bounds__(W * 32, (PaShape<D, Q8, W>::CTAS)) paged_attn(
             const float sub = m == -INFINITY ? 0.0f : m, rise = PA_TOP - top_v;  // added last: a large score would swallow it
             float p[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) p[e] = ex2(s[e] - sub + rise);
+            for (int e = 0; e < 4; e++) p[e] = ex2(fmaf(s[e] - sub, unit, rise));
             l += (p[0] + p[1]) + (p[2] + p[3]);
             // ---- weighted values ----
             if (!Q8) {
@@ -509,7 +521,7 @@ __global__ void __launch_bounds__(W * 32, (PaShape<D, Q8, W>::CTAS)) paged_attn(
             for (int j = 0; j < NT; j++)
                 *reinterpret_cast<float2*>(mine_o + 8 * j + 2 * c) = make_float2(o[j][0] + o[j][2], o[j][1] + o[j][3]);
         }
-        if (c == 0) *reinterpret_cast<float2*>(mine_o + D) = make_float2(m, l);
+        if (c == 0) *reinterpret_cast<float2*>(mine_o + D) = make_float2(m * unit, l);
         __syncthreads();
         const bool done = t0 == 0 && t1 == n_tiles;
         if (!done) {

@@ -70,9 +70,10 @@ CFI_API int cfi_paged_kv_load(const CfiPagedCache *cache, const int64_t *slots, 
  * lies in a page past the length never matters, whatever it holds.
  * q and out: [sequence][head][dim], types 0 F32 or 1 F16, row strides in values (q's a multiple of
  * 8), 16-byte aligned; scale > 0.  Sums and maxima are in 32 bits and the operands of the products with
- * K and V carry 22 bits, a weight (Q8_0: times its scale of V) no bits below 2^-39 of the largest: the results are
- * those of 32-bit arithmetic on the cached values, as long as |q| * scale stays below 45000.  An infinity or a NaN within a
- * sequence's length makes that sequence's results NaN.  Bounds: n_seq 65535, and n_seq * n_kv_head *
+ * K and V carry 22 bits, a query's values no bits below 2^-38 of their head's largest and a weight (Q8_0: times its
+ * scale of V) none below 2^-39 of the largest: the results are those of 32-bit arithmetic on the cached values, as
+ * long as the scores are within the range of f32.
+ * An infinity or a NaN within a sequence's length makes that sequence's results NaN.  Bounds: n_seq 65535, and n_seq * n_kv_head *
  * ceil(n_head / n_kv_head / 8) * (max_pages * page_size + 80) below 2^35.
  */
 CFI_API int cfi_paged_attention(const CfiPagedCache *cache, const void *q, int q_type, long long q_stride, void *out,

@@ -1,5 +1,5 @@
 """The serving operators at the ends of their ranges: one key that outweighs a long flat tail, small and large
-values of Q8_0 blocks.
+values of Q8_0 blocks, small and large queries.
 
 Bounds, as in test_gpu_serve.py: a score is off by at most EPS_S times the sum of its products' magnitudes times
 the scale, a weight by that much twice (numerator and sum) and 2^-20 twice for the exponential.  Three more terms count
@@ -134,3 +134,65 @@ def test_large_equal_scores(ty, heads, kv, dim, n):
         want = np.repeat(V.mean(0), heads // kv, axis=0)
         tol = (2 * 2.0 ** -20 + -(-n // 16) * 2.0 ** -23 + n * 2.0 ** -40) * np.abs(V).max()
         assert np.abs(got - want).max() <= tol, (grow, float(np.abs(got - want).max() / tol))
+
+
+# ---- queries ----
+def queries_case(ty, heads, kv, dim, n, q_size, k_size, seed=0):
+    """q_size and k_size: one number, or one for each dim."""
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(seed + n + dim)
+    page = 16
+    of = lambda x: torch.as_tensor(x, dtype=torch.float32, device=DEV)  # noqa: E731
+    k = (torch.randn(n, kv, dim, generator=gen, device=DEV).clamp(-3, 3) * of(k_size)).reshape(n, -1).contiguous()
+    v = torch.randn(n, kv * dim, generator=gen, device=DEV)
+    cache, pools, (K, V) = filled(ty, kv, dim, page, k, v)
+    q = (torch.randn(1, heads, dim, generator=gen, device=DEV) * of(q_size)).reshape(1, -1).contiguous()
+    table = torch.arange(-(-n // page), dtype=torch.int32, device=DEV)[None].contiguous()
+    lens = torch.tensor([n], dtype=torch.int32, device=DEV)
+    scale = 1.0 / math.sqrt(dim)
+    got = attention(cache, q, table, lens, scale)[0]
+    Q = q.double().cpu().numpy().reshape(heads, dim)
+    g = heads // kv
+    for h in range(kv):
+        qq = Q[h * g:(h + 1) * g]
+        want = attend(qq, K[:, h], V[:, h], scale)
+        S = np.abs(qq) @ np.abs(K[:, h]).T * scale  # of each head its largest
+        tol = (2 * EPS_S * S.max(1, keepdims=True) + 2 * 2.0 ** -20 + -(-n // 16) * 2.0 ** -23) * np.abs(V[:, h]).max()
+        err = np.abs(got[h * g:(h + 1) * g] - want)
+        assert (err <= tol).all(), (h, float((err / tol).max()))
+
+
+@pytest.mark.parametrize("ty", [F16, Q8])
+@pytest.mark.parametrize("heads,kv,dim", [(14, 2, 64), (12, 2, 128)])
+@pytest.mark.parametrize("q_size,k_size", [(1e-2, 1e2), (1e-4, 1e4), (1e-6, 2e4), (1e3, 1e-3), (1e6, 1e-3), (1e30, 1.0), (1e-30, 1.0)])
+def test_queries_of_all_sizes(ty, heads, kv, dim, q_size, k_size):
+    """A query's size is its own matter: 22 bits of each value whatever that is.  (1e30: one key takes all.)"""
+    for n in (3, 1500):
+        if q_size < 1e20:
+            queries_case(ty, heads, kv, dim, n, q_size, k_size)
+        else:  # no rounding of the scores reaches the distance of two of them
+            one_takes_all(ty, heads, kv, dim, n, q_size)
+
+
+def one_takes_all(ty, heads, kv, dim, n, q_size):
+    page = 16
+    k = torch.zeros(n, kv * dim, device=DEV)
+    k[:] = (torch.arange(n, device=DEV) * 0.5 / n)[:, None]
+    k[n // 2] = 2.0
+    v = torch.randn(n, kv * dim, generator=torch.Generator(device=DEV).manual_seed(n), device=DEV)
+    cache, pools, (K, V) = filled(ty, kv, dim, page, k, v)
+    q = torch.full((1, heads * dim), q_size, device=DEV)
+    table = torch.arange(-(-n // page), dtype=torch.int32, device=DEV)[None].contiguous()
+    got = attention(cache, q, table, torch.tensor([n], dtype=torch.int32, device=DEV), 1.0 / math.sqrt(dim))[0]
+    want = np.repeat(V[n // 2], heads // kv, axis=0)
+    assert (np.abs(got - want) <= 2 * 2.0 ** -20 * np.abs(want)).all()
+
+
+@pytest.mark.parametrize("ty", [F16, Q8])
+@pytest.mark.parametrize("heads,kv,dim", [(14, 2, 64), (12, 2, 128)])
+def test_queries_with_outlier_channels(ty, heads, kv, dim):
+    """Large channels of K (a block of 32 of them, as Q8_0 scales them) beside small ones of q, and the reverse."""
+    wide = torch.arange(dim) // 32 == 1
+    for q_size, k_size in ((torch.where(wide, 1e-4, 1.0), torch.where(wide, 1e4, 1.0)),
+                           (torch.where(wide, 1e2, 1e-2), torch.where(wide, 1e-2, 1e2))):
+        queries_case(ty, heads, kv, dim, 1500, q_size, k_size)
