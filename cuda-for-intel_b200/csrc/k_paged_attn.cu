@@ -29,6 +29,7 @@
 // the warps of three CTAs issue in 45 % of the cycles); one of 672, 14/2 heads of 64 in f16, 6.3 us, 5.1 of them on the device:
 // launch, table, one round of loads and the join.
 #include "paged_cache.cuh"
+#include "paged_cut.h"
 #include "sm100_ptx.cuh"
 #include "mma_sync.cuh"
 #include "cfi_kernels.h"
@@ -172,7 +173,7 @@ struct PaCut {
         for (int e = 0; e < PA_KEPT; e++) n += units[e];
         for (int s = lane + 32 * PA_KEPT; s < a.n_seq; s += 32) n += units_of(s) * hc;
         total = __reduce_add_sync(0xffffffffu, n);
-        quota = max((total + ctas - 1) / ctas, PA_FIXED + PA_WARPS);
+        quota = paged_quota(total, ctas, PA_FIXED + PA_WARPS);
     }
 };
 
@@ -238,9 +239,9 @@ __global__ void __launch_bounds__(W * 32, (PaShape<D, Q8, W>::CTAS)) paged_attn(
     } else {
         // ---- this CTA's run ----
         cut.read(a, gridDim.x);
-        if ((int)blockIdx.x > (cut.total - 1) / cut.quota) return;
+        if ((int)blockIdx.x >= paged_runs(cut.total, cut.quota)) return;
         begin = at = blockIdx.x * cut.quota;
-        end = min(begin + cut.quota, cut.total);
+        end = paged_run_end(begin, cut.quota, cut.total);
         auto among = [&](int base, int n) {  // is it one of the 32 sequences from `base` on, this lane's with n units?
             int incl = n;
 #pragma unroll

@@ -1,6 +1,8 @@
 """Refusals of the serving operators (include/cfi_serve.h): arguments outside the documented ones give
 cudaErrorInvalidValue before anything is launched, so none of these needs a GPU."""
 import ctypes as C
+import os
+import subprocess
 
 import pytest
 
@@ -98,3 +100,36 @@ def test_wrappers_raise():
         cfi.paged_kv_store(cache(), P, P, P, 1, src_type=5)
     with pytest.raises(RuntimeError):
         cfi.sample(P, P, P, 1, 0)
+
+
+# ---- the cut of cfi_paged_attention's list into runs (csrc/paged_cut.h), as the kernel computes it ----
+@pytest.fixture(scope="module")
+def cut(tmp_path_factory):
+    d = tmp_path_factory.mktemp("cut")
+    csrc = os.path.join(os.path.dirname(cfi.__file__), "csrc")
+    (d / "cut.cpp").write_text('''#include "paged_cut.h"
+extern "C" int quota(int total, int ctas, int least) { return paged_quota(total, ctas, least); }
+extern "C" int runs(int total, int q) { return paged_runs(total, q); }
+extern "C" int run_end(int begin, int q, int total) { return paged_run_end(begin, q, total); }
+''')
+    # -fwrapv: sums that pass an int wrap, as they do on the device
+    subprocess.run(["g++", "-O1", "-fwrapv", "-shared", "-fPIC", "-I", csrc, str(d / "cut.cpp"), "-o", str(d / "cut.so")], check=True)
+    return C.CDLL(str(d / "cut.so"))
+
+
+@pytest.mark.parametrize("total", [1, 8, 9, 10, 2663, 2664, 2665, 100003, 2**30 + 7, 2**31 - 4000000, 2**31 - 444, 2**31 - 2, 2**31 - 1])
+@pytest.mark.parametrize("ctas", [1, 2, 148, 296, 444])
+def test_runs_cover_the_list(cut, total, ctas):
+    """Every unit is in one run, up to the most that the host accepts."""
+    q = cut.quota(total, ctas, 9)
+    assert q >= 9 and q * ctas >= total and (q == 9 or (q - 1) * ctas < total)
+    n = cut.runs(total, q)
+    assert 1 <= n <= ctas
+    ends = [cut.run_end(b * q, q, total) for b in range(n)]
+    assert ends == [min((b + 1) * q, total) for b in range(n)] and ends[-1] == total and ends[-1] > (n - 1) * q
+
+
+@pytest.mark.parametrize("n_seq,max_pages", [(1, 2**31 - 1), (1, 2**31 - 5), (65535, 32764), (65536, 4)])
+def test_longer_lists_are_refused(n_seq, max_pages):
+    a = [cache(n_kv_head=1), P, 0, 64, P, 0, 64, P, max_pages, P, n_seq, 1, 0.125, None]
+    assert cfi.lib().cfi_paged_attention(*a) == INVALID
