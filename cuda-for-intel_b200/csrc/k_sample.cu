@@ -206,6 +206,10 @@ CFI_DEV float scaled_of(float l, float div) {
     return v == v ? v : -INFINITY;
 }
 
+// The divisor of a row whose largest logit is lmax.  Where its quotient by T passes the largest float, T is below 2^-127 of it and every
+// other logit at least 2^-24 of it away, so that only its equals have weight; so they do by the divisor that makes it 2^100.
+CFI_DEV float held_div(float lmax, float div) { return isinf(lmax / div) && !isinf(lmax) ? fabsf(lmax) * 0x1p-100f : div; }
+
 // The cut of a row.  What stays: key > cut_key, or key == cut_key and index <= cut_idx.  `each` calls its argument
 // with z and index of this thread's elements; of `in_order`, threads and elements are in index order.
 struct SaCut {
@@ -494,7 +498,7 @@ CFI_DEV void sample_row(const SaArgs& a, SaShared& s, float* slice, uint32_t ran
     if (tid < head) z[tid] = __ldcg(src + tid);
     if (tid >= 32 && tid < 32 + n - head - body) z[head + body + tid - 32] = __ldcg(src + head + body + tid - 32);
     const SaRow par(a, row);
-    const float div = par.div, p = par.p, minp = par.minp;
+    const float p = par.p, minp = par.minp;
     const int k = par.k;
     if (body > 0 && !mbar_wait(&s.bar, 0, &s.abort)) {
         cfi_set_error(a.err, 0xfc100);
@@ -502,7 +506,6 @@ CFI_DEV void sample_row(const SaArgs& a, SaShared& s, float* slice, uint32_t ran
     }
     __syncthreads();
 
-    auto scaled = [&](float l) { return scaled_of(l, div); };
     const int run = ((n + SA_THREADS - 1) / SA_THREADS) | 1;  // each thread's run: odd, so that 32 of them meet no bank twice
     const int r0 = min(n, tid * run), r1 = min(n, r0 + run);
     // f(i, z[i]) for this thread's run, SA_AHEAD loads at a time
@@ -544,6 +547,8 @@ CFI_DEV void sample_row(const SaArgs& a, SaShared& s, float* slice, uint32_t ran
     cluster_sync();
     float lmax = lane < SA_CTAS ? *peer(&s.cta_max, lane) : -INFINITY;
     lmax = warp_max(lmax);
+    const float div = held_div(lmax, par.div);
+    auto scaled = [&](float l) { return scaled_of(l, div); };
     const float zmax = scaled(lmax);  // division by a positive number keeps the order
     const bool empty = zmax == -INFINITY;
 
@@ -875,7 +880,7 @@ CFI_DEV void stream_row(const SaArgs& a, SaShared& s, float* slice, int row) {
         whole_row(a, s, 0, &count);
         if (count <= a.spare) return;
     }
-    const float div = par.div, p = par.p, minp = par.minp;
+    const float p = par.p, minp = par.minp;
     const int k = par.k;
     s.cnt[0][tid] = 0;
     s.cnt[1][tid] = 0;
@@ -908,7 +913,7 @@ CFI_DEV void stream_row(const SaArgs& a, SaShared& s, float* slice, int row) {
     if (lane == 0) s.wmax[warp] = mx;
     __syncthreads();
     const float lmax = warp_max(lane < SA_WARPS ? s.wmax[lane] : -INFINITY);
-    const float zmax = scaled_of(lmax, div);
+    const float div = held_div(lmax, par.div), zmax = scaled_of(lmax, div);
     if (zmax == -INFINITY) {
         if (tid == 0) {
             a.token[row] = -1;

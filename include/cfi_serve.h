@@ -105,7 +105,8 @@ CFI_API int cfi_packed_attention(const CfiPackedAttention *a, void *stream);
 /*
  * One token for each of n_rows rows of n_vocab logits (row stride in values), from the uniform
  * number u[row] in [0, 1).  In order:
- *   z = logit / temperature[row]; temperature <= 0 takes the largest logit;
+ *   z = logit / temperature[row] (of any size: where the largest passes f32, it and its equals have all the weight);
+ *     temperature <= 0 takes the largest logit;
  *   top_k[row] > 0 keeps the top_k largest;
  *   top_p[row] < 1 keeps, of those in falling order, the shortest run whose weight reaches top_p of
  *     theirs (a token stays when the weight before it is less);

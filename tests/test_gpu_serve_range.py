@@ -1,5 +1,5 @@
 """The serving operators at the ends of their ranges: one key that outweighs a long flat tail, small and large
-values of Q8_0 blocks, small and large queries.
+values of Q8_0 blocks, small and large queries, logits whose quotient by the temperature overflows.
 
 Bounds, as in test_gpu_serve.py: a score is off by at most EPS_S times the sum of its products' magnitudes times
 the scale, a weight by that much twice (numerator and sum) and 2^-20 twice for the exponential.  Three more terms count
@@ -13,7 +13,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 import cfi_b200 as cfi  # noqa: E402
-from test_gpu_serve import DEV, EPS_S, attend, garbage_pool, pool_rows, stream  # noqa: E402
+from test_gpu_serve import DEV, EPS_S, attend, fits, garbage_pool, pool_rows, sample, stream  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 F16, F32, Q8 = cfi.T_F16, cfi.T_F32, cfi.Q8_0
@@ -196,3 +196,57 @@ def test_queries_with_outlier_channels(ty, heads, kv, dim):
     for q_size, k_size in ((torch.where(wide, 1e-4, 1.0), torch.where(wide, 1e4, 1.0)),
                            (torch.where(wide, 1e2, 1e-2), torch.where(wide, 1e-2, 1e2))):
         queries_case(ty, heads, kv, dim, 1500, q_size, k_size)
+
+
+# ---- sampling ----
+@pytest.mark.parametrize("rows", [6, 80])
+@pytest.mark.parametrize("vocab", [40, 5000, 70000])
+def test_sample_temperature_whose_quotient_overflows(rows, vocab):
+    """logit / temperature may pass the largest float: the largest logits share the weight all the same, whatever their
+    sign, and nothing else has any."""
+    rng = np.random.default_rng(vocab)
+    z = rng.normal(size=(rows, vocab)).astype(np.float32)
+    low = np.finfo(np.float32).min
+    t = np.ones(rows, np.float32)
+    for r in range(rows):
+        kind = r % 6
+        a, b = vocab // 3, vocab // 2
+        if kind == 0:
+            z[r, b], t[r] = 9.0, 1e-39
+            z[r, a] = 8.0
+        elif kind == 1:
+            z[r] -= 20.0
+            z[r, b], t[r] = -1.0, 1e-40
+        elif kind == 2:
+            z[r, [a, b]], t[r] = 9.0, 1e-39
+        elif kind == 3:
+            z[r], t[r] = low, 0.7
+        elif kind == 4:
+            z[r], t[r] = low, 0.7
+            z[r, b] = -3.0
+        else:
+            z[r, b], t[r] = np.finfo(np.float32).max, 0.5
+    u = np.full(rows, 0.75, np.float32)
+    for k, p in ((0, 1.0), (7, 0.9), (0, 0.9)):
+        token, lp = sample(torch.from_numpy(z).to(DEV), u, t, [k] * rows, [p] * rows)
+        for r in range(rows):
+            kind = r % 6
+            a, b = vocab // 3, vocab // 2
+            if kind == 2:
+                assert token[r] == b and abs(lp[r] + math.log(2)) <= 1e-6, (r, k, p)
+            elif kind == 3:
+                count = math.ceil((k or vocab) * np.float64(np.float32(p)) - 1e-6)
+                assert token[r] == int(0.75 * count) and abs(lp[r] + math.log(count)) <= 4e-6 * math.log(count), (r, k, p)
+            else:
+                assert token[r] == b and lp[r] == 0, (r, k, p, token[r])
+
+
+def test_sample_small_temperatures_stay_exact():
+    """Down to where the quotient just holds."""
+    rng = np.random.default_rng(4)
+    z = rng.normal(size=(5, 3000)).astype(np.float32)
+    t = np.array([1e-3, 1e-10, 1e-30, 1e-37, 2e-38], np.float32)
+    u = rng.random(5).astype(np.float32)
+    token, lp = sample(torch.from_numpy(z).to(DEV), u, t)
+    for r in range(5):
+        assert fits(z[r], u[r], token[r], lp[r], t[r])
