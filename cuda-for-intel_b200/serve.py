@@ -32,7 +32,8 @@ class Sequence:
 
 class Server:
     """`model`: a DecodeModel (its weights are used, its own caches are not); `pages` pages of
-    `page_size` positions are shared by all sequences; cache_type cfi.T_F16 or cfi.Q8_0."""
+    `page_size` positions are shared by all sequences; cache_type cfi.T_F16 or cfi.Q8_0.  Each call works on the
+    stream that is torch's current one then, after what the calls before it did on theirs."""
 
     def __init__(self, torch, ctx, model, cache_type=cfi.T_F16, page_size=16, pages=256, seed=0):
         self.t, self.m, self.c = torch, model, model.cfg
@@ -50,7 +51,19 @@ class Server:
         self.free = list(range(pages))[::-1]
         self.gen = torch.Generator(device=self.dev)
         self.gen.manual_seed(seed)
-        self.stream = torch.cuda.current_stream().cuda_stream
+        self.last = torch.cuda.current_stream()  # that of the last call
+        self.stream = self.last.cuda_stream
+
+    def _begin(self, *given):
+        """A call begins: its stream, which waits for the last call's where that was another; what it reads is kept from the
+        allocator until it has."""
+        now = self.t.cuda.current_stream()
+        if now != self.last:
+            now.wait_stream(self.last)
+            self.pools.record_stream(now)
+            self.last, self.stream = now, now.cuda_stream
+        for x in given:
+            x.record_stream(now)
 
     # ---- pages ----
     def _grow(self, seqs, lengths):
@@ -124,6 +137,7 @@ class Server:
     def prefill(self, seqs, upto=None):
         """Runs the sequences' tokens that are not cached yet (of each the first upto[i] at most), all packed,
         after what is; logits of each one's last."""
+        self._begin()
         t, c = self.t, self.c
         ends = [len(s.tokens) if upto is None else min(upto[i], len(s.tokens)) for i, s in enumerate(seqs)]
         if any(e <= s.cached for s, e in zip(seqs, ends)):
@@ -156,6 +170,7 @@ class Server:
 
     def step(self, seqs):
         """One token of each sequence, its last, over its pages; logits."""
+        self._begin()
         t, c = self.t, self.c
         if any(s.cached != len(s.tokens) - 1 for s in seqs):
             raise ValueError("a step runs exactly the last token of each sequence")
@@ -178,6 +193,7 @@ class Server:
 
     def sample(self, seqs, logits):
         """Draws each sequence's next token and appends it; the drawn tokens' log probabilities."""
+        self._begin(logits)
         t, n = self.t, len(seqs)
         f = lambda v: t.tensor(v, dtype=t.float32, device=self.dev)  # noqa: E731
         temperature, top_p, min_p = f([s.temperature for s in seqs]), f([s.top_p for s in seqs]), f([s.min_p for s in seqs])

@@ -104,3 +104,26 @@ def test_generate(model):
     logits = s.prefill([greedy])
     s.sample([greedy], logits)
     assert greedy.tokens[-1] == int(logits.argmax())
+
+
+def test_other_streams_than_the_one_it_was_built_on(model):
+    """Prompts, steps and samples on streams of the caller's give what one stream gives."""
+    ctx, m = model
+    out = []
+    for many in (False, True):
+        s = serve.Server(torch, ctx, m, cfi.Q8_0, 16, 64, seed=9)
+        seqs = [serve.Sequence(tokens(n, n), temperature=0.9, top_k=30) for n in (70, 3)]
+        streams = [torch.cuda.Stream() for _ in range(3)] if many else [torch.cuda.current_stream()]
+        if many:
+            for x in streams:
+                x.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(streams[0]):
+            logits = s.prefill(seqs)
+        for i in range(8):
+            with torch.cuda.stream(streams[(i + 1) % len(streams)]):
+                s.sample(seqs, logits)
+            with torch.cuda.stream(streams[(i + 2) % len(streams)]):
+                logits = s.step(seqs)
+        torch.cuda.synchronize()
+        out.append(([q.tokens for q in seqs], logits.clone()))
+    assert out[0][0] == out[1][0] and torch.equal(out[0][1], out[1][1])
