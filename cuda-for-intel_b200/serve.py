@@ -19,6 +19,10 @@ class OutOfPages(RuntimeError):
     pass
 
 
+class NoToken(RuntimeError):
+    """Logits of which none can be taken: all are -inf or NaN."""
+
+
 class Sequence:
     """One request: its tokens so far, the pages that hold its context, how many positions they hold."""
 
@@ -192,7 +196,8 @@ class Server:
         return logits
 
     def sample(self, seqs, logits):
-        """Draws each sequence's next token and appends it; the drawn tokens' log probabilities."""
+        """Draws each sequence's next token and appends it; the drawn tokens' log probabilities.  NoToken, and no sequence is
+        longer, where one has no logit that can be taken."""
         self._begin(logits)
         t, n = self.t, len(seqs)
         f = lambda v: t.tensor(v, dtype=t.float32, device=self.dev)  # noqa: E731
@@ -202,7 +207,10 @@ class Server:
         token, logprob = t.empty(n, dtype=t.int32, device=self.dev), t.empty(n, device=self.dev)
         cfi.sample(logits.data_ptr(), u.data_ptr(), token.data_ptr(), n, self.c.vocab, temperature.data_ptr(), top_k.data_ptr(),
                    top_p.data_ptr(), min_p.data_ptr(), logprob.data_ptr(), stream=self.stream)
-        for s, x in zip(seqs, token.tolist()):
+        drawn = token.tolist()
+        if min(drawn, default=0) < 0:
+            raise NoToken("no token for the sequences at %s of the batch" % [i for i, x in enumerate(drawn) if x < 0])
+        for s, x in zip(seqs, drawn):
             s.tokens.append(x)
         return logprob
 

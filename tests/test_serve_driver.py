@@ -78,3 +78,18 @@ def test_work_goes_to_the_stream_of_the_call(rig):
     s.sample([serve.Sequence([8])], logits)
     assert len(at.waited_for) == again  # the same stream: nothing to wait for
     assert (logits.data_ptr(), at) in rig.kept  # but these are another's
+
+
+def test_a_row_without_a_token_is_an_error(rig):
+    """-1 (no logit that can be taken) is not appended, nor is anything else of that call: the next step would read the
+    embedding of the last token of the vocabulary."""
+    s = rig.server
+    seqs = [serve.Sequence([1, 2]), serve.Sequence([3])]
+    logits = s.prefill(seqs)
+    rig.drawn[:] = [5, -1]
+    with pytest.raises(serve.NoToken, match="1"):
+        s.sample(seqs, logits)
+    assert [q.tokens for q in seqs] == [[1, 2], [3]]
+    s.sample(seqs[:1], logits[:1])  # the other goes on
+    s.step(seqs[:1])
+    assert seqs[0].tokens == [1, 2, 1]
