@@ -446,6 +446,11 @@ def check(rc, what):
         raise RuntimeError("%s failed with CUDA error %d" % (what, rc))
 
 
+def device_error():
+    """cfi_device_error: reads and clears what the current device's kernels record when a bounded wait runs out (0: none has)."""
+    return lib().cfi_device_error()
+
+
 class GgmlCaller:
     """Launches ggml-cuda kernels the way ggml does (stock grid, block and kernelParams), through
     the substitution C ABI.  Pointers are device addresses (ints); `stream` a cudaStream_t."""

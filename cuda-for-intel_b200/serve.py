@@ -197,7 +197,7 @@ class Server:
 
     def sample(self, seqs, logits):
         """Draws each sequence's next token and appends it; the drawn tokens' log probabilities.  NoToken, and no sequence is
-        longer, where one has no logit that can be taken."""
+        longer, where one has no logit that can be taken; RuntimeError where a kernel since the last call has given up a wait."""
         self._begin(logits)
         t, n = self.t, len(seqs)
         f = lambda v: t.tensor(v, dtype=t.float32, device=self.dev)  # noqa: E731
@@ -208,6 +208,9 @@ class Server:
         cfi.sample(logits.data_ptr(), u.data_ptr(), token.data_ptr(), n, self.c.vocab, temperature.data_ptr(), top_k.data_ptr(),
                    top_p.data_ptr(), min_p.data_ptr(), logprob.data_ptr(), stream=self.stream)
         drawn = token.tolist()
+        error = cfi.device_error()
+        if error:
+            raise RuntimeError("a kernel's wait ran out (0x%x): the logits and what was cached since the last tokens are void" % error)
         if min(drawn, default=0) < 0:
             raise NoToken("no token for the sequences at %s of the batch" % [i for i, x in enumerate(drawn) if x < 0])
         for s, x in zip(seqs, drawn):

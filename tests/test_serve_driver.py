@@ -93,3 +93,17 @@ def test_a_row_without_a_token_is_an_error(rig):
     s.sample(seqs[:1], logits[:1])  # the other goes on
     s.step(seqs[:1])
     assert seqs[0].tokens == [1, 2, 1]
+
+
+def test_a_wait_that_ran_out_is_seen(rig, monkeypatch):
+    """What a kernel records when a bounded wait runs out makes the results void: sample(), which waits for them, raises."""
+    s = rig.server
+    seqs = [serve.Sequence([1, 2])]
+    logits = s.prefill(seqs)
+    words = [0xfb200]
+    monkeypatch.setattr(cfi, "device_error", lambda: words.pop() if words else 0)
+    with pytest.raises(RuntimeError, match="0xfb200"):
+        s.sample(seqs, logits)
+    assert seqs[0].tokens == [1, 2]
+    s.sample(seqs, logits)
+    assert seqs[0].tokens == [1, 2, 1]
