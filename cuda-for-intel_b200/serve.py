@@ -219,9 +219,9 @@ class Server:
 
     def generate(self, seqs, new):
         """Prompts, then `new` tokens of each sequence."""
-        self.sample(seqs, self.prefill(seqs))
-        for _ in range(new - 1):
-            self.sample(seqs, self.step(seqs))
+        logits = self.prefill(seqs)
+        for i in range(new):
+            self.sample(seqs, logits if i == 0 else self.step(seqs))
         return [s.tokens[s.prompt:] for s in seqs]
 
 

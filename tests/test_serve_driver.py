@@ -107,3 +107,10 @@ def test_a_wait_that_ran_out_is_seen(rig, monkeypatch):
     assert seqs[0].tokens == [1, 2]
     s.sample(seqs, logits)
     assert seqs[0].tokens == [1, 2, 1]
+
+
+@pytest.mark.parametrize("new", [0, 1, 3])
+def test_generate_gives_as_many_tokens_as_asked(rig, new):
+    seqs = [serve.Sequence([1, 2]), serve.Sequence([3])]
+    assert rig.server.generate(seqs, new) == [[1] * new] * 2
+    assert [q.cached for q in seqs] == [2 + max(0, new - 1), 1 + max(0, new - 1)]
