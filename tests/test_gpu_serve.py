@@ -320,7 +320,7 @@ def test_packed_attention_group_sizes(heads):
     packed_case(heads, 1, 64, [50, 3, 200], [50, 3, 260])
 
 
-def test_packed_attention_many_sequences():
+def test_packed_attention_hundreds_of_short_sequences():
     rng = np.random.default_rng(5)
     nq = [int(x) for x in rng.integers(0, 40, 300)]
     packed_case(4, 2, 64, nq, nq)
