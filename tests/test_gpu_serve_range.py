@@ -1,5 +1,6 @@
 """The serving operators at the ends of their ranges: one key that outweighs a long flat tail, small and large
-values of Q8_0 blocks, small and large queries, logits whose quotient by the temperature overflows.
+values of Q8_0 blocks, small and large queries, batches past the sequences that a lane keeps, logits whose
+quotient by the temperature overflows.
 
 Bounds, as in test_gpu_serve.py: a score is off by at most EPS_S times the sum of its products' magnitudes times
 the scale, a weight by that much twice (numerator and sum) and 2^-20 twice for the exponential.  Three more terms count
@@ -13,7 +14,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 import cfi_b200 as cfi  # noqa: E402
-from test_gpu_serve import DEV, EPS_S, attend, fits, garbage_pool, pool_rows, sample, stream  # noqa: E402
+from test_gpu_serve import DEV, EPS_S, attend, decode_case, fits, garbage_pool, pool_rows, sample, stream  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 F16, F32, Q8 = cfi.T_F16, cfi.T_F32, cfi.Q8_0
@@ -196,6 +197,19 @@ def test_queries_with_outlier_channels(ty, heads, kv, dim):
     for q_size, k_size in ((torch.where(wide, 1e-4, 1.0), torch.where(wide, 1e4, 1.0)),
                            (torch.where(wide, 1e2, 1e-2), torch.where(wide, 1e-2, 1e2))):
         queries_case(ty, heads, kv, dim, 1500, q_size, k_size)
+
+
+# ---- batches ----
+@pytest.mark.parametrize("ty", [F16, Q8])
+@pytest.mark.parametrize("heads,kv,dim,batch", [(14, 2, 64, 129), (12, 2, 128, 300), (4, 1, 64, 1000)])
+def test_many_sequences(ty, heads, kv, dim, batch):
+    """More sequences than the lanes keep the lengths of, in tables that a CTA takes whole with four warps and in longer ones."""
+    rng = np.random.default_rng(batch)
+    lens = [int(x) for x in rng.integers(-1, 200, batch)]
+    decode_case(ty, heads, kv, dim, 16, lens, F32, F32)[1]()
+    lens[batch - 3] = 3000
+    decode_case(ty, heads, kv, dim, 16, lens, F32, F32)[1]()
+    decode_case(ty, heads, kv, dim, 64, lens[::-1], F16, F16, pad=8)[1]()
 
 
 # ---- sampling ----
