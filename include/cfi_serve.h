@@ -50,7 +50,8 @@ CFI_API size_t cfi_paged_page_bytes(const CfiPagedCache *cache);
  * A slot outside [0, n_pages * page_size) stores nothing.  Two rows with the same slot: which one
  * remains is undefined.
  * Q8_0, per 32 values: d = max|x| / 127, q = x * (1/d) rounded to nearest even, scale f16(d); a block
- * with an infinity or a NaN reads back as NaN and touches no other block. */
+ * with an infinity or a NaN, or whose d passes f16 (8.3e6 and more), has no finite scale and touches no other block: it
+ * reads back as NaN, past f16 alone as NaN or infinities. */
 CFI_API int cfi_paged_kv_store(const CfiPagedCache *cache, const void *k, const void *v, int src_type,
                                long long k_stride, long long v_stride, const int64_t *slots, int n_tokens, void *stream);
 
@@ -73,8 +74,10 @@ CFI_API int cfi_paged_kv_load(const CfiPagedCache *cache, const int64_t *slots, 
  * K and V carry 22 bits, a query's values no bits below 2^-38 of their head's largest and a weight (Q8_0: times its
  * scale of V) none below 2^-39 of the largest: the results are those of 32-bit arithmetic on the cached values, as
  * long as the scores are within the range of f32.
- * An infinity or a NaN within a sequence's length makes that sequence's results NaN.  Bounds: n_seq 65535, and n_seq * n_kv_head *
- * ceil(n_head / n_kv_head / 8) * (max_pages * page_size + 80) below 2^35.
+ * A NaN makes NaN of what the formula takes it into and of nothing else: in q its head's outputs, in a row of K within
+ * the length those of its kv head's query heads, in V the same dims of them.  An infinity there makes of these NaN
+ * or what the formula gives.  Bounds: n_seq 65535, and n_seq * n_kv_head * ceil(n_head / n_kv_head / 8) *
+ * (max_pages * page_size + 80) below 2^35.
  */
 CFI_API int cfi_paged_attention(const CfiPagedCache *cache, const void *q, int q_type, long long q_stride, void *out,
                                 int out_type, long long out_stride, const int32_t *table, int max_pages,

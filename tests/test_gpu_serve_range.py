@@ -199,6 +199,42 @@ def test_queries_with_outlier_channels(ty, heads, kv, dim):
         queries_case(ty, heads, kv, dim, 1500, q_size, k_size)
 
 
+@pytest.mark.parametrize("ty", [F16, Q8])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_bad_queries_and_rows_stay_where_they_are(ty, bad):
+    """A query head of zeros is a mean, one with a NaN or an infinity is NaN, and the other heads and sequences are what they are
+    without it; so are they beside a NaN among another sequence's or another kv head's rows."""
+    heads, kv, dim, page, n = 12, 2, 64, 16, 300
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(3)
+    k, v = (torch.randn(2 * n, kv * dim, generator=gen, device=DEV) for _ in "kv")
+    q = torch.randn(2, heads * dim, generator=gen, device=DEV)
+    q[0, 2 * dim:3 * dim] = 0
+    at = torch.arange(-(-2 * n // page), dtype=torch.int32, device=DEV)
+    table = torch.stack([at[:19], at[18:37]]).contiguous()
+    lens = torch.tensor([n, 294], dtype=torch.int32, device=DEV)
+    cache, pools, (K, V) = filled(ty, kv, dim, page, k, v)
+    want = attention(cache, q, table, lens, 0.125)
+    mean = V[:n, 0].mean(0)
+    assert np.abs(want[0, 2] - mean).max() <= (2 * 2.0 ** -20 + 19 * 2.0 ** -23) * np.abs(V).max()
+    r = q.clone()
+    r[0, 5 * dim + 7] = bad
+    got = attention(cache, r, table, lens, 0.125)
+    assert np.isnan(got[0, 5]).all()
+    rest = np.ones((2, heads), bool)
+    rest[0, 5] = False
+    np.testing.assert_array_equal(got[rest], want[rest])
+    for which in range(2):
+        rows = [k.clone(), v.clone()]
+        rows[which][37, dim + 40] = math.nan  # kv head 1, of the first sequence alone
+        cache, pools, _ = filled(ty, kv, dim, page, *rows)
+        got = attention(cache, q, table, lens, 0.125)
+        reach = slice(0, dim) if which == 0 else slice(32, dim) if ty == Q8 else slice(40, 41)
+        assert np.isnan(got[0, 6:, reach]).all()
+        np.testing.assert_array_equal(got[0, :6], want[0, :6])
+        np.testing.assert_array_equal(got[1], want[1])
+
+
 # ---- batches ----
 @pytest.mark.parametrize("ty", [F16, Q8])
 @pytest.mark.parametrize("heads,kv,dim,batch", [(14, 2, 64, 129), (12, 2, 128, 300), (4, 1, 64, 1000)])
