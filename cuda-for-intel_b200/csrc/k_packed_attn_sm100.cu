@@ -16,6 +16,9 @@
 //     pipe works on one tile while the other is in its softmax;
 //   * warp 9 brings Q and the ring of K and V blocks by TMA.  V rows past the sequence's end are zeroed
 //     in shared memory (the next sequence's rows are there, and 0 x NaN would reach this one).
+// A weight of a key that a row does not see is zero, and zero times a NaN or an infinity is a NaN, in every row of the tile: where
+// a warp's first row has one, each row is looked at, and what is not finite is summed again over the keys that it
+// sees (repair), by its thread, from memory.
 // Where there are few tiles a CTA takes one: A and B are then the same rows over every other block of keys, and are joined at
 // the end by their maxima and sums, through shared memory.
 //
@@ -57,6 +60,8 @@ struct KaArgs {
     int out_f16, causal;
     float scale_log2;
     unsigned int* err;
+    const uint8_t *q, *k, *v;  // f16, for repair()
+    long long q_stride, k_stride, v_stride;
 };
 
 CFI_DEV float ex2(float x) {  // 2^x (PTX ex2.approx; -inf -> +0)
@@ -90,6 +95,15 @@ CFI_DEV uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
+}
+CFI_DEV bool all_finite(const uint4& v) {
+    const float x = fmaf(__uint_as_float(v.x), 0.0f, __uint_as_float(v.y) * 0.0f), y = fmaf(__uint_as_float(v.z), 0.0f, __uint_as_float(v.w) * 0.0f);
+    return x + y == 0.0f;
+}
+CFI_DEV bool all_finite_h2(const uint4& v) {
+    const __half2 *h = reinterpret_cast<const __half2*>(&v), zero = __float2half2_rn(0.0f);
+    const __half2 x = __hfma2(h[0], zero, __hmul2(h[1], zero)), y = __hfma2(h[2], zero, __hmul2(h[3], zero));
+    return __hbeq2(__hadd2(x, y), zero);
 }
 CFI_DEV bool elect_one() {  // true in one lane of a converged warp
     uint32_t r;
@@ -129,10 +143,67 @@ CFI_DEV void find_pair(const KaArgs& a, int span, int index, int* out) {
     __syncwarp();
 }
 
+// One row that is in memory: its pieces of 32 dims that are not finite again, over `keys` keys from k0 on; m and inv as
+// the row's sums ended.  Looking for such rows costs 0.4 of 54 us of sixteen prompts and nothing of one; a document of 16384 tokens
+// takes 24 ms instead of 0.8 with one dim of V all NaN, 65 with the last key's.
+template <int D>
+__device__ __noinline__ void repair(const KaArgs& a, int head, int kvh, int token, int k0, int keys, float m, float inv) {
+    const uint4* q = reinterpret_cast<const uint4*>(a.q + (token * a.q_stride + (long long)head * D) * 2);
+    for (int c = 0; c < D / 32; c++) {
+        const long long at = token * a.out_stride + (long long)head * D + 32 * c;
+        float none = 0.0f;  // but of a NaN or an infinity a NaN
+        for (int i = 0; i < 32; i++)
+            none = fmaf(a.out_f16 ? __half2float(static_cast<const __half*>(a.out)[at + i]) : static_cast<const float*>(a.out)[at + i], 0.0f, none);
+        if (none == 0.0f) continue;
+        float o[32];
+#pragma unroll
+        for (int i = 0; i < 32; i++) o[i] = 0.0f;
+        for (int j = 0; j < keys; j++) {
+            const uint4* k = reinterpret_cast<const uint4*>(a.k + ((k0 + j) * a.k_stride + (long long)kvh * D) * 2);
+            const uint4* v = reinterpret_cast<const uint4*>(a.v + ((k0 + j) * a.v_stride + (long long)kvh * D + 32 * c) * 2);
+            float s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < D / 8; i++) {
+                const uint4 x = __ldg(q + i), y = __ldg(k + i);
+                const __half2 *xh = reinterpret_cast<const __half2*>(&x), *yh = reinterpret_cast<const __half2*>(&y);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float2 f = __half22float2(xh[e]), g = __half22float2(yh[e]);
+                    s = fmaf(f.x, g.x, fmaf(f.y, g.y, s));
+                }
+            }
+            const float p = __half2float(__float2half_rn(ex2(fmaf(s, a.scale_log2, -m))));
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint4 x = __ldg(v + i);
+                const __half2* h = reinterpret_cast<const __half2*>(&x);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float2 f = __half22float2(h[e]);
+                    o[8 * i + 2 * e] = fmaf(p, f.x, o[8 * i + 2 * e]);
+                    o[8 * i + 2 * e + 1] = fmaf(p, f.y, o[8 * i + 2 * e + 1]);
+                }
+            }
+            if ((j & 63) == 63) {  // nothing makes a number of a NaN
+                bool all = true;
+#pragma unroll
+                for (int i = 0; i < 32; i++) all &= o[i] != o[i];
+                if (all) break;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i++)
+            if (a.out_f16)
+                static_cast<__half*>(a.out)[at + i] = __float2half_rn(o[i] * inv);
+            else
+                static_cast<float*>(a.out)[at + i] = o[i] * inv;
+    }
+}
+
 template <int D>
 __global__ void __launch_bounds__(KA_THREADS, 1)
     packed_attn(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
-                const __grid_constant__ CUtensorMap tv, const KaArgs a) {
+                const __grid_constant__ CUtensorMap tv, const __grid_constant__ KaArgs a) {
     constexpr int DB = D / 64;  // 64-value blocks of a row: one 128-byte swizzle atom column each
     constexpr int NS = ka_slots<D>();
     constexpr uint32_t TILE = ka_tile_bytes<D>(), BLK = KA_M * 128;
@@ -458,6 +529,7 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
                 keep = m_used == -INFINITY ? 0.0f : ex2(m_used - m);
                 other = ml.x == -INFINITY ? 0.0f : ex2(ml.x - m);
                 l = l * keep + ml.y * other;
+                m_used = m;
             }
         }
         tc_fence_after();
@@ -473,8 +545,13 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
             auto put = [&](int chunk, int chunks, uint4 v) {
                 *reinterpret_cast<uint4*>(rows + (lane * chunks + (chunk ^ (lane & 7))) * 16) = v;
             };
+            bool look = n_blocks > 0 && valid && l == 0.0f;  // zeros say nothing
             auto store = [&](int chunks, int size, int first) {  // pieces of 16 bytes a row, bytes of a value, first value
                 __syncwarp();
+                if (lane < chunks) {  // the first row's
+                    const uint4 v = *reinterpret_cast<const uint4*>(rows + lane * 16);
+                    look |= size == 2 ? !all_finite_h2(v) : !all_finite(v);
+                }
 #pragma unroll 4
                 for (int i = lane; i < 32 * chunks; i += 32) {
                     const int row = i / chunks, chunk = i % chunks;
@@ -525,6 +602,9 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
                     if (c % HALF == HALF - 1) store(D / 8, 4, 32 * (c - HALF + 1));
                 }
             }
+            // not for a NaN among the scores, which the sum of the weights has too
+            if (__any_sync(0xffffffffu, look) && valid && l - l == 0.0f)
+                repair<D>(a, kvh * a.group + r % a.group, kvh, q0 + t, k0, limit, m_used, inv);
         }
     }
     tc_fence_before();
@@ -580,6 +660,12 @@ template <int D> int launch(const CfiPackedAttention* p, cudaStream_t stream) {
     a.causal = p->causal;
     a.scale_log2 = p->scale * 1.4426950408889634f;
     a.err = cfi_device_error_word();
+    a.q = static_cast<const uint8_t*>(p->q);
+    a.k = static_cast<const uint8_t*>(p->k);
+    a.v = static_cast<const uint8_t*>(p->v);
+    a.q_stride = p->q_stride;
+    a.k_stride = p->k_stride;
+    a.v_stride = p->v_stride;
     // Every sequence adds at most one pair that is not full.  Up to 5/4 pairs an SM a CTA takes a single tile, which halves the
     // chain of the longest; more share the reads of K and V and the CTAs' beginnings and ends.  Single tiles against
     // pairs, us: one prompt of 1024, 12/2 heads of 128, 15 and 22; of 3000 (145 pairs) 39 and 54; of 4096 (196) 67 and

@@ -93,7 +93,8 @@ CFI_API int cfi_paged_attention(const CfiPagedCache *cache, const void *q, int q
  * q, out: [token][head][dim], k, v: [token][kv head][dim]; q, k, v f16, out F32 or F16; row strides
  * in values, multiples of 8, heads contiguous, 16-byte aligned; n_head / n_kv_head at most 128;
  * head_dim 64 or 128; scale > 0.  Products are of f16 values (the softmax weights rounded to f16 too) with
- * 32-bit sums.  A NaN or an infinity in V reaches the queries of its own sequence only.
+ * 32-bit sums.  What a key holds that a query does not see never matters to it, whatever it is; a NaN or an infinity in V reaches
+ * the same dims of the queries that see it (and costs their tiles a slow second pass).
  */
 typedef struct {
     const void *q, *k, *v;

@@ -235,6 +235,57 @@ def test_bad_queries_and_rows_stay_where_they_are(ty, bad):
         np.testing.assert_array_equal(got[1], want[1])
 
 
+# ---- packed prompts ----
+@pytest.mark.parametrize("heads,kv,dim", [(14, 2, 64), (12, 2, 128), (40, 2, 64)])
+@pytest.mark.parametrize("nq,nk", [([1, 40, 300], [1, 40, 300]), ([200, 130, 3], [333, 100, 700]), ([3000, 50], [3000, 800])])
+@pytest.mark.parametrize("ot", [F32, F16])
+def test_packed_attention_bad_values_reach_who_sees_them(heads, kv, dim, nq, nk, ot):
+    """Non-finite values of a key leave the queries that do not see it, and the other dims, as they are; who sees one gets it.
+    A NaN among a key's own numbers makes NaN of all of those, and of nothing else."""
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(heads + sum(nq))
+    g, scale = heads // kv, 1.0 / math.sqrt(dim)
+    q = (torch.randn(sum(nq), heads * dim, generator=gen, device=DEV) * 1.5).half()
+    k, v = (torch.randn(sum(nk), kv * dim, generator=gen, device=DEV).half() for _ in "kv")
+    cq, ck = (np.cumsum([0] + n) for n in (nq, nk))
+    clean_k, clean_v = k.clone(), v.clone()
+    where = {}  # of each sequence: key and dims of V in kv head 0, key of K in kv head 1
+    for s, (n, m) in enumerate(zip(nq, nk)):
+        at = max(0, m - 1 - n // 2)
+        where[s] = at, max(0, m - 1 - n // 3)
+        v[ck[s] + at, 5] = math.nan
+        v[ck[s] + at, 40] = math.inf
+        k[ck[s] + where[s][1], dim + 9] = math.nan
+    out = torch.full((sum(nq), heads * dim), 7.0, dtype=torch.float16 if ot == F16 else torch.float32, device=DEV)
+    du, dk = (torch.from_numpy(c.astype(np.int32)).to(DEV) for c in (cq, ck))
+    cfi.packed_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), du.data_ptr(), dk.data_ptr(), len(nq), sum(nq), sum(nk),
+                         heads, kv, dim, scale, out_type=ot, stream=stream())
+    torch.cuda.synchronize()
+    assert cfi.lib().cfi_device_error() == 0
+    for s, (n, m) in enumerate(zip(nq, nk)):
+        Q = q[cq[s]:cq[s + 1]].double().reshape(n, kv, g, dim).permute(1, 2, 0, 3)
+        K, V = (x[ck[s]:ck[s + 1]].double().reshape(m, kv, dim).permute(1, 0, 2)[:, None] for x in (clean_k, clean_v))
+        got = out[cq[s]:cq[s + 1]].double().reshape(n, kv, g, dim).permute(1, 2, 0, 3)
+        last = torch.arange(n, device=DEV) + (m - n)  # the last key that a query sees
+        x = (Q @ K.transpose(2, 3)) * scale
+        x = x.masked_fill(torch.arange(m, device=DEV)[None] > last[:, None], -math.inf)
+        p = torch.softmax(x, -1)
+        p[:, :, last < 0] = 0
+        want = p @ V
+        S = float((Q.abs() @ K.abs().transpose(2, 3)).max() * scale)
+        tol = (2 * EPS_S * S + 2 * 2.0 ** -20 + 2.0 ** -11) * float(V.abs().max())
+        if ot == F16:
+            tol = tol + 2.0 ** -11 * want.abs() + 2.0 ** -25
+        sees_v, sees_k = last >= where[s][0], last >= where[s][1]
+        near = (got - want).abs() <= tol
+        assert torch.isnan(got[0][:, sees_v][..., 5]).all() and not torch.isfinite(got[0][:, sees_v][..., 40]).any()
+        near[0][:, sees_v, 5] = True
+        near[0][:, sees_v, 40] = True
+        assert torch.isnan(got[1][:, sees_k]).all()
+        near[1][:, sees_k] = True
+        assert near.all(), (s, torch.nonzero(~near)[:4].tolist(), int((~near).sum()))
+
+
 # ---- batches ----
 @pytest.mark.parametrize("ty", [F16, Q8])
 @pytest.mark.parametrize("heads,kv,dim,batch", [(14, 2, 64, 129), (12, 2, 128, 300), (4, 1, 64, 1000)])
