@@ -26,6 +26,7 @@
 #include "../../include/cfi_serve.h"
 #include "sm100_ptx.cuh"
 #include "cfi_kernels.h"
+#include "quotient.h"
 
 #include <stdlib.h>
 #include <string.h>
@@ -458,9 +459,7 @@ CFI_DEV void finish_short(SaCut& cut, int nc, const float* logits, float div, in
     cut.draw(each, sum, upto - sum, total);
 }
 
-// l / T in three forms.  The second, for ordinary T and l only, is Markstein's (Computation of elementary functions on the IBM RISC
-// System/6000, 1990): from the reciprocal rounded to nearest, corrections by the exact remainder end at
-// the quotient rounded to nearest, the first within an ulp of it.  The same value as the division's, without its branch.
+// l / T in three forms.  The last, for ordinary T and l only, gives the same value as the division, without its branch.
 struct SaByOne {
     CFI_DEV float operator()(float l) const { return l; }
 };
@@ -470,10 +469,7 @@ struct SaByDivision {
 };
 struct SaByReciprocal {
     float t, r;
-    CFI_DEV float operator()(float l) const {
-        const float q0 = l * r, q1 = fmaf(fmaf(-q0, t, l), r, q0);
-        return fmaf(fmaf(-q1, t, l), r, q1);
-    }
+    CFI_DEV float operator()(float l) const { return quotient_by(l, t, r); }
 };
 
 // One row, by a cluster: this CTA has the n logits from `base`.

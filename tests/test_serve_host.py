@@ -4,6 +4,7 @@ import ctypes as C
 import os
 import subprocess
 
+import numpy as np
 import pytest
 
 import cfi_b200 as cfi
@@ -133,3 +134,27 @@ def test_runs_cover_the_list(cut, total, ctas):
 def test_longer_lists_are_refused(n_seq, max_pages):
     a = [cache(n_kv_head=1), P, 0, 64, P, 0, 64, P, max_pages, P, n_seq, 1, 0.125, None]
     assert cfi.lib().cfi_paged_attention(*a) == INVALID
+
+
+# ---- the quotient by a temperature (csrc/quotient.h) ----
+@pytest.mark.parametrize("low,high", [(-3, 3), (-59, 59), (0, 1)])
+def test_quotient_is_the_divisions(tmp_path, low, high):
+    """Bit for bit, for temperatures and logits over the powers of two where the kernel takes it: |l| above 2^-60, T between 2^-60
+    and 2^60, |l / T| below 2^13 for the largest logit."""
+    csrc = os.path.join(os.path.dirname(cfi.__file__), "csrc")
+    (tmp_path / "q.cpp").write_text('''#include "quotient.h"
+extern "C" void many(const float *l, const float *t, float *by, float *div, int n) {
+    for (int i = 0; i < n; i++) by[i] = quotient_by(l[i], t[i], 1.0f / t[i]), div[i] = l[i] / t[i];
+}
+''')
+    subprocess.run(["g++", "-O2", "-ffp-contract=off", "-shared", "-fPIC", "-I", csrc, str(tmp_path / "q.cpp"), "-o", str(tmp_path / "q.so")],
+                   check=True)
+    rng, n = np.random.default_rng(low + 100), 1 << 20
+    t = (rng.uniform(1, 2, n) * 2.0 ** rng.integers(low, high, n)).astype(np.float32)
+    t[:4096] = np.nextafter(np.float32(2) ** rng.integers(low + 1, high + 1, 4096).astype(np.float32), np.float32(0))  # all ones
+    l = (rng.normal(size=n) * 2.0 ** np.minimum(rng.integers(-59, 20, n), 12 + np.floor(np.log2(t)))).astype(np.float32)
+    l[np.abs(l) <= 2.0 ** -60] = 1.0
+    by, div = np.empty_like(l), np.empty_like(l)
+    f = C.POINTER(C.c_float)
+    C.CDLL(str(tmp_path / "q.so")).many(*(x.ctypes.data_as(f) for x in (l, t, by, div)), n)
+    np.testing.assert_array_equal(by.view(np.uint32), div.view(np.uint32))
