@@ -26,9 +26,9 @@
 //
 // Bound by the softmax: a block of a tile takes 16384 exponentials, 1024 cycles of an SM's exponential unit, and with
 // the maxima, the fp16 packing and two trips through tensor memory about 2000, half of it beside the other
-// tile's; its MMAs take 512 (heads of 64) or 1024.  One document of 16384 tokens, 12/2 heads of 128: 0.81 ms under the
-// power cap, 1019 TFLOP/s (0.68 ms in short bursts); sixteen prompts of 1 to 2048 tokens 51 us, 620 TFLOP/s (the longest
-// tile's 16 blocks and the CTAs behind it); four chunks after 7000 tokens, 14/2 heads of 64, 81 us, 540 TFLOP/s.
+// tile's; its MMAs take 512 (heads of 64) or 1024.  One document of 16384 tokens, 12/2 heads of 128: 0.82 ms under the
+// power cap, 1003 TFLOP/s (0.68 ms in short bursts); sixteen prompts of 1 to 2048 tokens 54.6 us, 579 TFLOP/s (the longest
+// tile's 16 blocks and the CTAs behind it); four chunks after 7000 tokens, 14/2 heads of 64, 79.5 us, 551 TFLOP/s.
 #include "../../include/cfi_serve.h"
 #include "sm100_ptx.cuh"
 #include "cfi_kernels.h"
@@ -225,7 +225,8 @@ __global__ void __launch_bounds__(KA_THREADS, 1)
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kvh = blockIdx.x % a.n_kv_head;
     pdl_launch_dependents();
-    // all that needs no input: it runs beside the end of the kernel before
+    // all that needs no input: it runs beside the end of the kernel before.  The tensor memory too: 384 x 168 registers leave no other
+    // CTA a place on this SM, so that one of the kernel behind, which may start from here on, cannot take it first
     if (tid == 0) {
         prefetch_tmap(&tq);
         prefetch_tmap(&tk);

@@ -25,8 +25,8 @@
 // that grows, as they are where the maximum does).
 //
 // Measured: 8 sequences of 9000 to 65000 positions, 32/8 heads of 128 in f16, 146 us, 6.2 TB/s; 64 of 16 to 4096, 12/2 heads
-// of 128 in Q8_0, 20.0 us (36 MB; the work of a tile, some 600 instructions of a warp, is what it waits for:
-// the warps of three CTAs issue in 45 % of the cycles); one of 672, 14/2 heads of 64 in f16, 6.3 us, 5.1 of them on the device:
+// of 128 in Q8_0, 20.9 us (36 MB; the work of a tile, some 600 instructions of a warp, is what it waits for:
+// the warps of three CTAs issue in 45 % of the cycles); one of 672, 14/2 heads of 64 in f16, 5.9 us, 5.1 of them on the device:
 // launch, table, one round of loads and the join.
 #include "paged_cache.cuh"
 #include "paged_cut.h"
