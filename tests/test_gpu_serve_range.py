@@ -351,3 +351,75 @@ def test_sample_small_temperatures_stay_exact():
     token, lp = sample(torch.from_numpy(z).to(DEV), u, t)
     for r in range(5):
         assert fits(z[r], u[r], token[r], lp[r], t[r])
+
+
+# ---- graphs ----
+def test_a_captured_step_is_replayed_with_new_inputs():
+    """Rows stored, read back, attended to packed and by single tokens, logits sampled, twice over in one graph: replayed with other
+    rows, slots, tables, lengths and settings it gives what the calls give one after another."""
+    heads, kv, dim, page, pages, n, batch, rows, vocab = 12, 2, 64, 16, 40, 300, 3, 40, 66000
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(11)
+    size = cfi.paged_page_bytes(Q8, page, kv, dim) * pages
+    pools = torch.zeros(2, size, dtype=torch.uint8, device=DEV)
+    cache = cfi.paged_cache(Q8, pools[0].data_ptr(), pools[1].data_ptr(), pages, page, kv, dim)
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device=DEV)  # noqa: E731
+    f32 = lambda *s: torch.zeros(*s, device=DEV)  # noqa: E731
+    x = dict(k=f32(n, kv * dim), v=f32(n, kv * dim), slots=torch.zeros(n, dtype=torch.int64, device=DEV), table=i32(batch, 12),
+             lens=i32(batch), q=f32(batch, heads * dim), pq=torch.zeros(n, heads * dim, dtype=torch.float16, device=DEV), cu=i32(3),
+             z=f32(rows, vocab), t=f32(rows), top_k=i32(rows), top_p=f32(rows), u=f32(rows))
+    y = dict(back=torch.zeros(2, n, kv * dim, dtype=torch.float16, device=DEV), one=f32(batch, heads * dim), many=f32(n, heads * dim),
+             token=i32(rows), logprob=f32(rows))
+    p = lambda t: t.data_ptr()  # noqa: E731
+
+    def step(s):
+        cfi.paged_kv_store(cache, p(x["k"]), p(x["v"]), p(x["slots"]), n, stream=s)
+        cfi.paged_kv_load(cache, p(x["slots"]), p(y["back"][0]), p(y["back"][1]), n, stream=s)
+        cfi.packed_attention(p(x["pq"]), p(y["back"][0]), p(y["back"][1]), p(y["many"]), p(x["cu"]), p(x["cu"]), 2, n, n, heads, kv, dim, 0.125,
+                             stream=s)
+        cfi.paged_attention(cache, p(x["q"]), p(y["one"]), p(x["table"]), p(x["lens"]), batch, heads, 12, 0.125, stream=s)
+        cfi.sample(p(x["z"]), p(x["u"]), p(y["token"]), rows, vocab, p(x["t"]), p(x["top_k"]), p(x["top_p"]), 0, p(y["logprob"]), stream=s)
+
+    def inputs(seed):
+        g = torch.Generator(device=DEV)
+        g.manual_seed(seed)
+        r = np.random.default_rng(seed)
+        for name in ("k", "v", "q", "pq"):
+            x[name].copy_(torch.randn(x[name].shape, generator=g, device=DEV))
+        x["z"].copy_(torch.randn(rows, vocab, generator=g, device=DEV) * 3)
+        x["slots"].copy_(torch.randperm(pages * page, generator=g, device=DEV)[:n])
+        x["table"].copy_(torch.from_numpy(r.integers(0, pages, (batch, 12))))
+        x["lens"].copy_(torch.from_numpy(r.integers(0, 190, batch)))
+        x["cu"].copy_(torch.tensor([0, int(r.integers(0, n)), n]))
+        x["t"].copy_(torch.from_numpy(r.choice([0.0, 0.7, 1.0, 1.3], rows)))
+        # few and many rows with a nucleus of the whole row: both sides of who takes them
+        x["top_k"].copy_(torch.from_numpy(np.where(r.random(rows) < (0.1 if seed % 2 else 0.97), 0, 50)))
+        x["top_p"].copy_(torch.from_numpy(r.choice([0.5, 0.95], rows)))
+        x["u"].copy_(torch.rand(rows, generator=g, device=DEV))
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        inputs(0)
+        step(s.cuda_stream)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            step(s.cuda_stream)
+            step(s.cuda_stream)
+    for seed in range(1, 7):
+        inputs(seed)
+        torch.cuda.synchronize()
+        kept = pools.clone()
+        step(torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        want = {name: t.clone() for name, t in y.items()}
+        pools.copy_(kept)
+        for t in y.values():
+            t.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for name, t in y.items():
+            assert torch.equal(t, want[name]), (seed, name)
+        assert cfi.lib().cfi_device_error() == 0
