@@ -277,15 +277,31 @@ def _prepare_place(s, case, g):
     if own:
         s["held"] = _cfi().page_table(s["table"].data_ptr(), s["cached"].data_ptr(), s["free"].data_ptr(), s["n_free"].data_ptr(),
                                       case["rows"], width, page, pages)
+        s["described"] = _cfi().page_batch(s["rows"].data_ptr(), s["new"].data_ptr(), b, s["lens_out"].data_ptr(),
+                                           s["batch_table"].data_ptr(), s["cu_q"].data_ptr(), s["cu_kv"].data_ptr(), s["slots"].data_ptr(),
+                                           s["positions"].data_ptr(), tokens, s["status"].data_ptr(),
+                                           context=s["context"].data_ptr() if context else 0, max_context=context)
     return s
 
 
 def _bind(s):
-    """The cache's description that a program keeps beside its pools."""
-    if own:
-        c = s["case"]
-        s["cache"] = _cfi().paged_cache(F16 if c["op"] == "rotate" else Q4_1, s["k_pool"].data_ptr(), s["v_pool"].data_ptr(), s["pages"],
-                                        c["page"], c["heads_kv"], c["dim"])
+    """The descriptions of its cache and rows that a program keeps beside their buffers."""
+    if not own:
+        return s
+    cfi, c = _cfi(), s["case"]
+    s["cache"] = cfi.paged_cache(F16 if c["op"] == "rotate" else Q4_1, s["k_pool"].data_ptr(), s["v_pool"].data_ptr(), s["pages"],
+                                 c["page"], c["heads_kv"], c["dim"])
+    if c["op"] == "rotate":
+        size = s["qkv"].element_size()
+        nq, nkv = c["heads"] * c["dim"], c["heads_kv"] * c["dim"]
+        width, q = nq + 2 * nkv, s["qkv"].data_ptr()
+        b = s["bias"].data_ptr() if c["bias"] else 0
+        s["described"] = cfi.norm_rope_rows(
+            q, s["q_out"].data_ptr(), s["pos"].data_ptr(), c["tokens"], c["heads"], c["dim"], k=q + nq * size, v=q + (nq + nkv) * size,
+            n_kv_head=c["heads_kv"], slots=s["slots"].data_ptr(), in_type=c["src"], q_out_type=c["out"], q_bias=b,
+            k_bias=b + 4 * nq if b else 0, v_bias=b + 4 * (nq + nkv) if b else 0, q_norm=s["norm"][0].data_ptr() if c["norm"] else 0,
+            k_norm=s["norm"][1].data_ptr() if c["norm"] else 0, eps=s["eps"], n_rot=c["turned"], freq_base=s["base"], q_stride=width,
+            k_stride=width, v_stride=width)
     return s
 
 
@@ -318,17 +334,7 @@ def _own_decode4(s):
 
 
 def _own_rotate(s):
-    c = s["case"]
-    size = s["qkv"].element_size()
-    nq, nkv = c["heads"] * c["dim"], c["heads_kv"] * c["dim"]
-    width, q = nq + 2 * nkv, s["qkv"].data_ptr()
-    b = s["bias"].data_ptr() if c["bias"] else 0
-    _cfi().norm_rope(q, s["q_out"].data_ptr(), s["pos"].data_ptr(), c["tokens"], c["heads"], c["dim"], k=q + nq * size,
-                     v=q + (nq + nkv) * size, n_kv_head=c["heads_kv"], cache=s["cache"], slots=s["slots"].data_ptr(), in_type=c["src"],
-                     q_out_type=c["out"], q_bias=b, k_bias=b + 4 * nq if b else 0, v_bias=b + 4 * (nq + nkv) if b else 0,
-                     q_norm=s["norm"][0].data_ptr() if c["norm"] else 0, k_norm=s["norm"][1].data_ptr() if c["norm"] else 0,
-                     eps=s["eps"], n_rot=c["turned"], freq_base=s["base"], q_stride=width, k_stride=width, v_stride=width,
-                     stream=s["stream"])
+    _cfi().norm_rope(s["described"], s["cache"], stream=s["stream"])
     return s["q_out"], s["k_pool"], s["v_pool"]
 
 
@@ -339,9 +345,7 @@ def _place_outputs(s):
 
 def _own_place(s):
     cfi, c, st = _cfi(), s["case"], s["stream"]
-    cfi.paged_place(s["held"], s["rows"].data_ptr(), s["new"].data_ptr(), c["batch"], s["lens_out"].data_ptr(), s["batch_table"].data_ptr(),
-                    s["cu_q"].data_ptr(), s["cu_kv"].data_ptr(), s["slots"].data_ptr(), s["positions"].data_ptr(), s["tokens"],
-                    s["status"].data_ptr(), context=s["context"].data_ptr() if c["context"] else 0, max_context=s["n_context"], stream=st)
+    cfi.paged_place(s["held"], s["described"], stream=st)
     cfi.paged_trim(s["held"], s["rows"].data_ptr(), s["before"].data_ptr(), c["batch"], s["status"].data_ptr() + 4, stream=st)
     return _place_outputs(s)
 
