@@ -17,7 +17,7 @@ LIB_PATH = os.path.join(HERE, "lib", "libcfi_b200.so")
 
 # ---- ggml types ----
 T_F32, T_F16 = 0, 1
-Q4_0, Q5_0, Q8_0, Q4_K, Q5_K, Q6_K = 2, 6, 8, 12, 13, 14
+Q4_0, Q4_1, Q5_0, Q8_0, Q4_K, Q5_K, Q6_K = 2, 3, 6, 8, 12, 13, 14
 BLOCK_BYTES = {Q4_0: 18, Q5_0: 22, Q8_0: 34, Q4_K: 144, Q5_K: 176, Q6_K: 210}
 QK = {Q4_0: 32, Q5_0: 32, Q8_0: 32, Q4_K: 256, Q5_K: 256, Q6_K: 256}
 
@@ -147,6 +147,9 @@ def lib():
     L.cfi_paged_kv_load.argtypes = [cp, vp, vp, vp, ll, ll, i, vp]
     L.cfi_paged_attention.argtypes = [cp, vp, i, ll, vp, i, ll, vp, i, vp, i, i, f, vp]
     L.cfi_packed_attention.argtypes = [C.POINTER(PackedAttention), vp]
+    L.cfi_norm_rope.argtypes = [C.POINTER(NormRope), cp, vp]
+    L.cfi_paged_place.argtypes = [C.POINTER(PageTable), C.POINTER(PagedPlace), vp]
+    L.cfi_paged_trim.argtypes = [C.POINTER(PageTable), vp, vp, i, vp, vp]
     L.cfi_sample.argtypes = [vp, ll, i, i, vp, vp, vp, vp, vp, vp, vp, vp]
     _lib = L
     return L
@@ -333,6 +336,31 @@ class PackedAttention(C.Structure):
                 [(n, C.c_longlong) for n in ("q_stride", "k_stride", "v_stride", "out_stride")] +
                 [(n, C.c_int) for n in ("n_seq", "n_q", "n_kv", "n_head", "n_kv_head", "head_dim", "out_type", "causal")] +
                 [("scale", C.c_float)])
+
+
+class NormRope(C.Structure):
+    """CfiNormRope (include/cfi_serve.h)."""
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "k", "v", "q_bias", "k_bias", "v_bias", "q_norm", "k_norm", "freq_factors", "pos",
+                                           "q_out", "k_out", "v_out", "slots")] +
+                [(n, C.c_longlong) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride", "k_out_stride", "v_out_stride")] +
+                [(n, C.c_int) for n in ("n_tokens", "n_head", "n_kv_head", "head_dim", "n_rot", "in_type", "q_out_type", "kv_out_type")] +
+                [(n, C.c_float) for n in ("eps", "freq_base", "freq_scale")])
+
+
+class PageTable(C.Structure):
+    """CfiPageTable (include/cfi_serve.h)."""
+    _fields_ = ([(n, C.c_void_p) for n in ("table", "cached", "free_pages", "n_free")] +
+                [(n, C.c_int) for n in ("n_rows", "max_pages", "page_size", "n_pages")])
+
+
+class PagedPlace(C.Structure):
+    """CfiPagedPlace (include/cfi_serve.h)."""
+    _fields_ = ([(n, C.c_void_p) for n in ("rows", "n_new", "lens", "batch_table", "cu_q", "cu_kv", "positions", "status", "slots",
+                                           "context")] +
+                [(n, C.c_int) for n in ("n_seq", "max_new", "max_context")])
+
+
+PLACED, PLACE_BAD_ROW, PLACE_TOO_LONG, PLACE_NO_ROOM, PLACE_NO_PAGES = range(5)  # what the calls on a page table write as status
 
 
 class Ctx:
@@ -628,7 +656,7 @@ def mmq_skinny_group(ty, xs, y, dsts, nrows, k, ncols, ncols_y=None, stride_row_
 # serving operators (include/cfi_serve.h); pointers are device addresses, strides in values
 # ---------------------------------------------------------------------------------------------
 def paged_cache(ty, k, v, n_pages, page_size, n_kv_head, head_dim):
-    """The description of a paged cache (F16 or Q8_0) whose pools lie at k and v; raises when the
+    """The description of a paged cache (F16, Q8_0 or Q4_1) whose pools lie at k and v; raises when the
     library does not serve such a cache."""
     c = PagedCache(k, v, ty, n_pages, page_size, n_kv_head, head_dim)
     if lib().cfi_paged_page_bytes(C.byref(c)) == 0:
@@ -680,6 +708,52 @@ def packed_attention(q, k, v, out, cu_q, cu_kv, n_seq, n_q, n_kv, n_head, n_kv_h
     rc = lib().cfi_packed_attention(a, stream)
     if rc:
         check(rc, "cfi_packed_attention")
+
+
+def norm_rope_rows(q, q_out, pos, n_tokens, n_head, head_dim, k=0, v=0, n_kv_head=0, slots=0, k_out=0, v_out=0, in_type=T_F32,
+                   q_out_type=T_F32, kv_out_type=T_F32, q_bias=0, k_bias=0, v_bias=0, q_norm=0, k_norm=0, eps=1e-6, n_rot=None,
+                   freq_base=1e6, freq_scale=1.0, freq_factors=0, q_stride=0, k_stride=0, v_stride=0, q_out_stride=0, k_out_stride=0,
+                   v_out_stride=0):
+    """The description of rows of q, k and v for norm_rope (strides 0: packed; n_rot None: whole heads); a program whose buffers
+    stay keeps it."""
+    wq, wk = n_head * head_dim, n_kv_head * head_dim
+    return NormRope(q, k or None, v or None, q_bias or None, k_bias or None, v_bias or None, q_norm or None, k_norm or None,
+                    freq_factors or None, pos or None, q_out, k_out or None, v_out or None, slots or None, q_stride or wq, k_stride or wk,
+                    v_stride or wk, q_out_stride or wq, k_out_stride or wk, v_out_stride or wk, n_tokens, n_head, n_kv_head, head_dim,
+                    head_dim if n_rot is None else n_rot, in_type, q_out_type, kv_out_type, eps, freq_base, freq_scale)
+
+
+def norm_rope(rows, cache=None, stream=0):
+    """cfi_norm_rope: bias, norm and rotation of norm_rope_rows' rows; k and v also into the cache's slots."""
+    rc = lib().cfi_norm_rope(rows, cache, stream)
+    if rc:
+        check(rc, "cfi_norm_rope")
+
+
+def page_table(table, cached, free_pages, n_free, n_rows, max_pages, page_size, n_pages):
+    """The description of a page table on the device: int32 table of n_rows x max_pages, positions held by each row, the stack of
+    free pages and its height."""
+    return PageTable(table, cached, free_pages, n_free, n_rows, max_pages, page_size, n_pages)
+
+
+def page_batch(rows, n_new, n_seq, lens, batch_table, cu_q, cu_kv, slots, positions, max_new, status, context=0, max_context=0):
+    """The description of a batch for paged_place: the int32 rows and new tokens of its sequences and what is written for it
+    (slots and context int64, the others int32)."""
+    return PagedPlace(rows, n_new, lens, batch_table, cu_q, cu_kv, positions, status, slots, context or None, n_seq, max_new, max_context)
+
+
+def paged_place(table, batch, stream=0):
+    """cfi_paged_place: pages, slots, positions and offsets for a page_batch's new tokens."""
+    rc = lib().cfi_paged_place(table, batch, stream)
+    if rc:
+        check(rc, "cfi_paged_place")
+
+
+def paged_trim(table, rows, keep, n_seq, status, stream=0):
+    """cfi_paged_trim: n_seq rows keep their first keep[i] positions; the pages behind go back to the stack."""
+    rc = lib().cfi_paged_trim(table, rows, keep, n_seq, status, stream)
+    if rc:
+        check(rc, "cfi_paged_trim")
 
 
 def sample(logits, u, token, n_rows, n_vocab, temperature=0, top_k=0, top_p=0, min_p=0, logprob=0, row_stride=0, stream=0):

@@ -1,0 +1,236 @@
+// k_norm_rope.cu -- bias, norm of each head and rotation of a product's rows of q and k, bias of v, in one pass, the
+// rows of k and v into the slots of a paged cache (include/cfi_serve.h).
+//
+// Bound by HBM: every row is read once and written once.  D / 8 lanes take a head: lane l the four dims 4 l .. and their four
+// partners n_rot / 2 behind, so that a rotation needs no other lane (the lanes behind n_rot / 8 take eight dims that are not turned).
+//
+// Angles.  A pair's rate in turns, freq_scale freq_base^(-2 i / n_rot) / 2 pi, is a fraction of 2^64; times the position it wraps by
+// whole turns, exactly, and the upper 32 bits are the angle.  (A position of 100000 times a rate in f32 would be off by 4e-3 rad.)
+#include "paged_row.cuh"
+#include "sm100_ptx.cuh"
+#include "cfi_kernels.h"
+
+#include <math.h>
+#include <stdlib.h>
+#include <string.h>
+
+namespace {
+
+constexpr int NR_THREADS = 256, NR_RATES = 64;
+
+struct NrArgs {
+    CfiNormRope r;
+    uint8_t *k_pool, *v_pool;
+    long long n_slots;
+    int page_shift, cache_type;
+    int heads_of_thread;  // heads of one token that a group of lanes takes, `split` apart
+    uint32_t split;
+    union {
+        unsigned long long turn[NR_RATES];  // of 2^64
+        double rate[NR_RATES];              // in turns, where freq_factors divide them
+    };
+};
+
+CFI_DEV float4 f4(uint4 w) { return make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w)); }
+CFI_DEV uint4 ldg128_stream(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+CFI_DEV uint2 ldg64_stream(const void* p) {
+    uint2 v;
+    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
+template <bool IN_F16> CFI_DEV float4 load4(const void* rows, long long at) {
+    if (!IN_F16) return f4(ldg128_stream(static_cast<const float*>(rows) + at));
+    const uint2 w = ldg64_stream(static_cast<const __half*>(rows) + at);
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+    return make_float4(a.x, a.y, b.x, b.y);
+}
+CFI_DEV uint2 halves(float4 x) {
+    const __half2 a = __floats2half2_rn(x.x, x.y), b = __floats2half2_rn(x.z, x.w);
+    return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+CFI_DEV void store4(void* rows, int f16, long long at, float4 x) {
+    if (f16)
+        *reinterpret_cast<uint2*>(static_cast<__half*>(rows) + at) = halves(x);
+    else
+        *reinterpret_cast<float4*>(static_cast<float*>(rows) + at) = x;
+}
+CFI_DEV float4 add4(float4 a, float4 b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
+CFI_DEV float4 mul4(float4 a, float s, float4 b) { return make_float4(a.x * s * b.x, a.y * s * b.y, a.z * s * b.z, a.w * s * b.w); }
+CFI_DEV float dot4(float4 a) { return fmaf(a.x, a.x, fmaf(a.y, a.y, fmaf(a.z, a.z, a.w * a.w))); }
+// (x, y) turned, the products rounded as they are
+CFI_DEV void turn1(float& x, float& y, float c, float s) {
+    const float t = fmaf(x, c, -(y * s));
+    y = fmaf(x, s, y * c);
+    x = t;
+}
+
+template <int D, bool IN_F16> __global__ void __launch_bounds__(NR_THREADS) norm_rope(const __grid_constant__ NrArgs a) {
+    constexpr int G = D / 8;  // lanes of a head
+    __shared__ float4 s_row[NR_THREADS / G][2 * G];  // a row of k, where the cache wants eight dims in a lane
+    const CfiNormRope& r = a.r;
+    const int lane = threadIdx.x % G, group = threadIdx.x / G;
+    const int nk = r.k ? r.n_kv_head : 0, nv = r.v ? r.n_kv_head : 0, heads = r.n_head + nk + nv;
+    const int eighth = r.n_rot / 8;  // lanes that turn
+    const bool turns = lane < eighth;
+    const int d0 = turns ? 4 * lane : 8 * lane, d1 = turns ? 4 * (lane + eighth) : 8 * lane + 4;
+    sm100::pdl_launch_dependents();
+    sm100::pdl_wait();
+    const uint32_t id = blockIdx.x * (NR_THREADS / G) + group;
+    const bool live = id < (uint32_t)r.n_tokens * a.split;
+    const int t = live ? (int)(id / a.split) : r.n_tokens - 1, part = live ? (int)(id % a.split) : 0;
+    float cs[4], sn[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) cs[e] = 1.0f, sn[e] = 0.0f;
+    if (turns) {
+        const int pos = r.pos[t];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            unsigned long long f;
+            if (r.freq_factors) {
+                const double x = a.rate[4 * lane + e] / (double)r.freq_factors[4 * lane + e];
+                f = __double2ull_rn((x - floor(x)) * 18446744073709551616.0);
+            } else {
+                f = a.turn[4 * lane + e];
+            }
+            const int angle = (int)((f * (unsigned long long)(long long)pos) >> 32);
+            sincospif((float)angle * 0x1p-31f, &sn[e], &cs[e]);
+        }
+    }
+    const long long slot = a.k_pool ? r.slots[t] : -1;
+    const bool placed = live && slot >= 0 && slot < a.n_slots;
+    const int off = (int)(slot & ((1 << a.page_shift) - 1));
+    for (int i = 0; i < a.heads_of_thread; i++) {
+        const int u = part + i * (int)a.split;
+        const bool on = live && u < heads;
+        const int kind = u < r.n_head ? 0 : u < r.n_head + nk ? 1 : 2;  // of q, k, v
+        const int h = kind == 0 ? u : kind == 1 ? u - r.n_head : u - r.n_head - nk;
+        const void* rows = kind == 0 ? r.q : kind == 1 ? r.k : r.v;
+        const long long at = (long long)t * (kind == 0 ? r.q_stride : kind == 1 ? r.k_stride : r.v_stride) + h * D;
+        const float *bias = kind == 0 ? r.q_bias : kind == 1 ? r.k_bias : r.v_bias, *norm = kind == 0 ? r.q_norm : kind == 1 ? r.k_norm : nullptr;
+        float4 x0 = make_float4(0.0f, 0.0f, 0.0f, 0.0f), x1 = x0;
+        if (on) {
+            x0 = load4<IN_F16>(rows, at + d0);
+            x1 = load4<IN_F16>(rows, at + d1);
+            if (bias) {
+                x0 = add4(x0, *reinterpret_cast<const float4*>(bias + h * D + d0));
+                x1 = add4(x1, *reinterpret_cast<const float4*>(bias + h * D + d1));
+            }
+        }
+        float ss = dot4(x0) + dot4(x1);
+#pragma unroll
+        for (int o = 1; o < G; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (norm && on) {
+            const float s = rsqrtf(ss / (float)D + r.eps);
+            x0 = mul4(x0, s, *reinterpret_cast<const float4*>(norm + d0));
+            x1 = mul4(x1, s, *reinterpret_cast<const float4*>(norm + d1));
+        }
+        if (kind != 2 && turns) {
+            turn1(x0.x, x1.x, cs[0], sn[0]);
+            turn1(x0.y, x1.y, cs[1], sn[1]);
+            turn1(x0.z, x1.z, cs[2], sn[2]);
+            turn1(x0.w, x1.w, cs[3], sn[3]);
+        }
+        void* out = kind == 0 ? r.q_out : kind == 1 ? r.k_out : r.v_out;
+        if (out && on) {
+            const long long to = (long long)t * (kind == 0 ? r.q_out_stride : kind == 1 ? r.k_out_stride : r.v_out_stride) + h * D;
+            const int f16 = kind == 0 ? r.q_out_type : r.kv_out_type;
+            store4(out, f16, to + d0, x0);
+            store4(out, f16, to + d1, x1);
+        }
+        if (!a.k_pool) continue;
+        const bool put = placed && on && kind != 0;
+        const long long page_head = (slot >> a.page_shift) * r.n_kv_head + h;
+        uint8_t* pool = kind == 2 ? a.v_pool : a.k_pool;
+        if (a.cache_type == CACHE_F16) {
+            if (put) {
+                uint8_t* row = pool + page_head * paged_region_bytes<D, CACHE_F16>(1 << a.page_shift) + (size_t)off * D * 2;
+                *reinterpret_cast<uint2*>(row + d0 * 2) = halves(x0);
+                *reinterpret_cast<uint2*>(row + d1 * 2) = halves(x1);
+            }
+        } else {
+            // eight neighbouring dims in a lane
+            __syncwarp();
+            s_row[group][d0 / 4] = x0;
+            s_row[group][d1 / 4] = x1;
+            __syncwarp();
+            const float4 y0 = s_row[group][2 * lane], y1 = s_row[group][2 * lane + 1];
+            const Row8 w = {{y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w}, {}};
+            if (a.cache_type == CACHE_Q8_0) {
+                put_q8_0<D, false>(w, pool + page_head * paged_region_bytes<D, CACHE_Q8_0>(1 << a.page_shift), a.page_shift, off, lane, put);
+            } else {
+                put_q4_1<D>(w, pool + page_head * paged_region_bytes<D, CACHE_Q4_1>(1 << a.page_shift), off, lane, kind == 2, put);
+            }
+        }
+    }
+}
+
+bool rows_ok(const void* p, long long stride, long long width) { return p && !((uintptr_t)p & 15) && stride % 8 == 0 && stride >= width; }
+bool type_ok(int t) { return t == 0 || t == 1; }
+
+}  // namespace
+
+extern "C" int cfi_norm_rope(const CfiNormRope* r, const CfiPagedCache* c, void* stream) {
+    if (!r || (r->head_dim != 64 && r->head_dim != 128) || r->n_tokens < 0 || r->n_head <= 0 || r->n_head > 65535 || r->n_kv_head < 0 ||
+        r->n_kv_head > 65535 || !type_ok(r->in_type) || !type_ok(r->q_out_type) || !type_ok(r->kv_out_type) || r->n_rot < 0 ||
+        r->n_rot > r->head_dim || r->n_rot % 8 || !(r->eps >= 0.0f) || isinf(r->eps))
+        return (int)cudaErrorInvalidValue;
+    const long long wq = (long long)r->n_head * r->head_dim, wk = (long long)r->n_kv_head * r->head_dim;
+    if (!rows_ok(r->q, r->q_stride, wq) || !rows_ok(r->q_out, r->q_out_stride, wq) || (r->k && !rows_ok(r->k, r->k_stride, wk)) ||
+        (r->v && !rows_ok(r->v, r->v_stride, wk)) || (r->k_out && !rows_ok(r->k_out, r->k_out_stride, wk)) ||
+        (r->v_out && !rows_ok(r->v_out, r->v_out_stride, wk)) || ((r->k || r->v) && r->n_kv_head == 0) || (r->k && !r->k_out && !c) ||
+        (r->v && !r->v_out && !c) || (r->k_out && !r->k) || (r->v_out && !r->v))
+        return (int)cudaErrorInvalidValue;
+    if ((((uintptr_t)r->q_bias | (uintptr_t)r->k_bias | (uintptr_t)r->v_bias | (uintptr_t)r->q_norm | (uintptr_t)r->k_norm) & 15) ||
+        ((uintptr_t)r->freq_factors & 3))
+        return (int)cudaErrorInvalidValue;
+    if (r->n_rot && (!r->pos || ((uintptr_t)r->pos & 3) || !(r->freq_base > 0.0f) || isinf(r->freq_base) || !isfinite(r->freq_scale)))
+        return (int)cudaErrorInvalidValue;
+    if (c && (!cfi_paged_ok(c) || !r->k || !r->v || !r->slots || ((uintptr_t)r->slots & 7) || c->head_dim != r->head_dim ||
+              c->n_kv_head != r->n_kv_head))
+        return (int)cudaErrorInvalidValue;
+    if (r->n_tokens == 0) return 0;
+    NrArgs a = {};
+    a.r = *r;
+    if (c) {
+        a.k_pool = static_cast<uint8_t*>(c->k);
+        a.v_pool = static_cast<uint8_t*>(c->v);
+        a.n_slots = (long long)c->n_pages * c->page_size;
+        a.page_shift = __builtin_ctz((unsigned)c->page_size);
+        a.cache_type = c->type;
+    }
+    if (r->n_rot) {
+        const long double step = powl((long double)r->freq_base, -2.0L / r->n_rot);
+        long double rate = (long double)r->freq_scale / 6.283185307179586476925287L;
+        for (int i = 0; i < r->n_rot / 2; i++, rate *= step) {
+            const long double part = (rate - floorl(rate)) * 18446744073709551616.0L;
+            if (r->freq_factors)
+                a.rate[i] = (double)rate;
+            else
+                a.turn[i] = part < 18446744073709551616.0L ? (unsigned long long)part : 0;
+        }
+    }
+    const int heads = r->n_head + (r->k ? r->n_kv_head : 0) + (r->v ? r->n_kv_head : 0), groups = NR_THREADS / (r->head_dim / 8);
+    a.heads_of_thread = 1;
+    a.split = heads;
+    if ((long long)r->n_tokens * heads > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
+    const uint32_t ctas = ((uint32_t)r->n_tokens * a.split + groups - 1) / groups;
+    const char* ep = getenv("CFI_PDL");
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3(ctas, 1, 1);
+    lc.blockDim = dim3(NR_THREADS, 1, 1);
+    lc.stream = static_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    lc.attrs = at;
+    lc.numAttrs = (ep && strcmp(ep, "0") == 0) ? 0 : 1;
+    const int variant = (r->head_dim == 128) * 2 + r->in_type;
+    return (int)(variant == 0   ? cudaLaunchKernelEx(&lc, norm_rope<64, false>, (const NrArgs)a)
+                 : variant == 1 ? cudaLaunchKernelEx(&lc, norm_rope<64, true>, (const NrArgs)a)
+                 : variant == 2 ? cudaLaunchKernelEx(&lc, norm_rope<128, false>, (const NrArgs)a)
+                                : cudaLaunchKernelEx(&lc, norm_rope<128, true>, (const NrArgs)a));
+}

@@ -1,9 +1,7 @@
-// k_paged_cache.cu -- writing rows of K and V into the pages of a serving cache (quantised to Q8_0
-// where the cache is) and reading them back as f16.  include/cfi_serve.h gives the layout.
-//
-// Per block of 32 values x: d = max|x| / 127, q = rn(x * (1/d)), stored scale f16(d); read back as
-// f16(q * scale).  Four neighbouring threads, 8 values each, make a block.
-#include "paged_cache.cuh"
+// k_paged_cache.cu -- writing rows of K and V into the pages of a serving cache (quantised to Q8_0 or
+// Q4_1 where the cache is, paged_row.cuh) and reading them back as f16.  include/cfi_serve.h gives the layout.
+// Four neighbouring threads, 8 values each, make a block of 32.
+#include "paged_row.cuh"
 #include "sm100_ptx.cuh"
 #include "cfi_kernels.h"
 
@@ -55,27 +53,14 @@ template <int D> struct PcPlace {
         slot = a.slots[t];
     }
     CFI_DEV bool ok(const PcArgs& a) const { return in && slot >= 0 && slot < a.n_slots; }
-    template <bool Q8> CFI_DEV long long region(const PcArgs& a) const {
-        return ((slot >> a.page_shift) * a.n_kv_head + h) * paged_region_bytes<D, Q8>(1 << a.page_shift);
+    template <int TY> CFI_DEV long long region(const PcArgs& a) const {
+        return ((slot >> a.page_shift) * a.n_kv_head + h) * paged_region_bytes<D, TY>(1 << a.page_shift);
     }
     CFI_DEV int off(const PcArgs& a) const { return (int)(slot & ((1 << a.page_shift) - 1)); }
     CFI_DEV long long value(long long stride) const { return (long long)t * stride + h * D + g * 8; }
 };
 
-CFI_DEV __half2 abs_h2(uint32_t w) {
-    w &= 0x7fff7fffu;
-    return *reinterpret_cast<const __half2*>(&w);
-}
-CFI_DEV int to_s8(float x) {  // to the nearest, ties to even; the ends at +-128, a NaN 0
-    int q;
-    asm("cvt.rni.sat.s8.f32 %0, %1;" : "=r"(q) : "f"(x));
-    return q;
-}
-CFI_DEV uint32_t bytes_of(int a, int b, int c, int d) {
-    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
-}
-
-template <int D, bool Q8, bool SRC_F16>
+template <int D, int TY, bool SRC_F16>
 __global__ void __launch_bounds__(PC_THREADS) paged_kv_store(const PcArgs a) {
     sm100::pdl_launch_dependents();
     sm100::pdl_wait();
@@ -96,69 +81,31 @@ __global__ void __launch_bounds__(PC_THREADS) paged_kv_store(const PcArgs a) {
     for (int e = 0; e < PC_STORE_ITEMS; e++)
 #pragma unroll
         for (int kv = 0; kv < 2; kv++) {
-            const bool ok = p[e].ok(a);
-            uint8_t* region = (kv ? a.v : a.k) + p[e].template region<Q8>(a);
-            const int off = p[e].off(a);
-            float x[8];
-            uint4 raw = in[e][kv][0];
+            uint8_t* region = (kv ? a.v : a.k) + p[e].template region<TY>(a);
+            Row8 r;
+            r.h = in[e][kv][0];
             if (SRC_F16) {
-                const __half2* h = reinterpret_cast<const __half2*>(&raw);
+                const __half2* h = reinterpret_cast<const __half2*>(&r.h);
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const float2 f = __half22float2(h[j]);
-                    x[2 * j] = f.x;
-                    x[2 * j + 1] = f.y;
+                    r.x[2 * j] = f.x;
+                    r.x[2 * j + 1] = f.y;
                 }
             } else {
                 const uint4 hi = in[e][kv][SRC_F16 ? 0 : 1];
-                const uint32_t w[8] = {raw.x, raw.y, raw.z, raw.w, hi.x, hi.y, hi.z, hi.w};
+                const uint32_t w[8] = {r.h.x, r.h.y, r.h.z, r.h.w, hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-                for (int j = 0; j < 8; j++) x[j] = __uint_as_float(w[j]);
-                __half2* h = reinterpret_cast<__half2*>(&raw);
+                for (int j = 0; j < 8; j++) r.x[j] = __uint_as_float(w[j]);
+                __half2* h = reinterpret_cast<__half2*>(&r.h);
 #pragma unroll
-                for (int j = 0; j < 4; j++) h[j] = __floats2half2_rn(x[2 * j], x[2 * j + 1]);
+                for (int j = 0; j < 4; j++) h[j] = __floats2half2_rn(r.x[2 * j], r.x[2 * j + 1]);
             }
-            if (!Q8) {
-                if (ok) *reinterpret_cast<uint4*>(region + ((size_t)off * D + p[e].g * 8) * 2) = raw;
-                continue;
-            }
-            float m;  // of a block that has a NaN: NaN, and so its scale
-            if (SRC_F16) {
-                __half2 h = abs_h2(raw.x);
-                h = __hmax2_nan(__hmax2_nan(h, abs_h2(raw.y)), __hmax2_nan(abs_h2(raw.z), abs_h2(raw.w)));
-                h = __hmax2_nan(h, __lowhigh2highlow(h));
-#pragma unroll
-                for (int o = 1; o < 4; o <<= 1) h = __hmax2_nan(h, __shfl_xor_sync(0xffffffffu, h, o));
-                m = __low2float(h);
-            } else {
-                m = 0.0f;
-                uint32_t nan = 0;
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    m = fmaxf(m, fabsf(x[j]));  // drops a NaN
-                    nan |= (uint32_t)(x[j] != x[j]);
-                }
-                if (nan) m = __uint_as_float(0x7fffffffu);
-#pragma unroll
-                for (int o = 1; o < 4; o <<= 1) {
-                    const float other = __shfl_xor_sync(0xffffffffu, m, o);
-                    m = other != other ? other : m != m ? m : fmaxf(m, other);
-                }
-            }
-            const float d = m / 127.0f, id = d > 0.0f ? 1.0f / d : 0.0f;
-            int q[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) q[j] = to_s8(x[j] * id);
-            const uint32_t w[2] = {bytes_of(q[0], q[1], q[2], q[3]), bytes_of(q[4], q[5], q[6], q[7])};
-            if (!ok) continue;
-            *reinterpret_cast<uint2*>(region + (size_t)off * D + p[e].g * 8) = make_uint2(w[0], w[1]);
-            if ((p[e].g & 3) == 0)
-                *reinterpret_cast<uint16_t*>(region + (size_t)(D << a.page_shift) + ((size_t)off * (D / 32) + p[e].g / 4) * 2) =
-                    d != d ? (uint16_t)0x7fff : f2h_bits(d);
+            put_row8<D, TY, SRC_F16>(r, region, a.page_shift, p[e].off(a), p[e].g, kv == 1, p[e].ok(a));
         }
 }
 
-template <int D, bool Q8>
+template <int D, int TY>
 __global__ void __launch_bounds__(PC_THREADS) paged_kv_load(const PcArgs a) {
     sm100::pdl_launch_dependents();
     sm100::pdl_wait();
@@ -175,9 +122,17 @@ __global__ void __launch_bounds__(PC_THREADS) paged_kv_load(const PcArgs a) {
             in[e][kv] = make_uint4(0, 0, 0, 0);
             scale[e][kv] = 0;
             if (!p[e].ok(a)) continue;
-            const uint8_t* region = (kv ? a.v : a.k) + p[e].template region<Q8>(a);
+            const uint8_t* region = (kv ? a.v : a.k) + p[e].template region<TY>(a);
             const int off = p[e].off(a);
-            if (Q8) {
+            if (TY == CACHE_Q4_1) {
+                const int row = off % Q41_TILE, b = p[e].g >> 2, c = p[e].g & 3;
+                const uint8_t* tile = region + Q41<D>::tile_at(off);
+                in[e][kv].x = kv ? *reinterpret_cast<const uint16_t*>(tile + Q41<D>::v_at(row, b, 2 * c)) |
+                                       (uint32_t)*reinterpret_cast<const uint16_t*>(tile + Q41<D>::v_at(row, b, 2 * c + 1)) << 16
+                                 : *reinterpret_cast<const uint32_t*>(tile + Q41<D>::k_at(row, b, c));
+                scale[e][kv] = *reinterpret_cast<const uint16_t*>(tile + Q41<D>::scale_at(row, b)) |
+                               (uint32_t)*reinterpret_cast<const uint16_t*>(tile + Q41<D>::min_at(row, b)) << 16;
+            } else if (TY == CACHE_Q8_0) {
                 const uint2 q = ldg_stream2(region + (size_t)off * D + p[e].g * 8);
                 in[e][kv].x = q.x;
                 in[e][kv].y = q.y;
@@ -192,7 +147,15 @@ __global__ void __launch_bounds__(PC_THREADS) paged_kv_load(const PcArgs a) {
 #pragma unroll
         for (int kv = 0; kv < 2; kv++) {
             uint4 out = in[e][kv];
-            if (Q8) {
+            if (TY == CACHE_Q4_1) {
+                const float d = h2f_bits((uint16_t)scale[e][kv]), m = h2f_bits((uint16_t)(scale[e][kv] >> 16));
+                __half2* o = reinterpret_cast<__half2*>(&out);
+                const uint32_t w = in[e][kv].x;
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    o[j] = __floats2half2_rn(fmaf(d, (float)(w >> (8 * j) & 15), m), fmaf(d, (float)(w >> (8 * j + 4) & 15), m));
+                // a slot outside the pool: zeros
+            } else if (TY == CACHE_Q8_0) {
                 const float d = h2f_bits((uint16_t)scale[e][kv]);
                 __half2* o = reinterpret_cast<__half2*>(&out);
                 const uint32_t w[2] = {in[e][kv].x, in[e][kv].y};
@@ -241,11 +204,14 @@ bool args_of(const CfiPagedCache* c, long long ks, long long vs, const int64_t* 
     return true;
 }
 
+int type_at(const CfiPagedCache* c) { return c->type == CACHE_F16 ? 0 : c->type == CACHE_Q8_0 ? 1 : 2; }
+
 }  // namespace
 
 extern "C" size_t cfi_paged_page_bytes(const CfiPagedCache* c) {
     if (!c || !cfi_paged_shape_ok(c)) return 0;
-    return (size_t)c->n_kv_head * c->page_size * (c->type == 1 ? (size_t)c->head_dim * 2 : (size_t)c->head_dim / 32 * 34);
+    const size_t row = c->type == CACHE_F16 ? (size_t)c->head_dim * 2 : (size_t)c->head_dim / 32 * (c->type == CACHE_Q8_0 ? 34 : 20);
+    return (size_t)c->n_kv_head * c->page_size * row;
 }
 
 extern "C" int cfi_paged_kv_store(const CfiPagedCache* c, const void* k, const void* v, int src_type, long long k_stride,
@@ -258,12 +224,14 @@ extern "C" int cfi_paged_kv_store(const CfiPagedCache* c, const void* k, const v
     if (n_tokens == 0) return 0;
     a.src_k = static_cast<const uint8_t*>(k);
     a.src_v = static_cast<const uint8_t*>(v);
-    static const void* const fns[8] = {
-        (const void*)paged_kv_store<64, false, false>,  (const void*)paged_kv_store<64, false, true>,
-        (const void*)paged_kv_store<64, true, false>,   (const void*)paged_kv_store<64, true, true>,
-        (const void*)paged_kv_store<128, false, false>, (const void*)paged_kv_store<128, false, true>,
-        (const void*)paged_kv_store<128, true, false>,  (const void*)paged_kv_store<128, true, true>};
-    return go(fns[(c->head_dim == 128) * 4 + (c->type == 8) * 2 + src_type], a, PC_STORE_ITEMS, static_cast<cudaStream_t>(stream));
+    static const void* const fns[12] = {
+        (const void*)paged_kv_store<64, CACHE_F16, false>,   (const void*)paged_kv_store<64, CACHE_F16, true>,
+        (const void*)paged_kv_store<64, CACHE_Q8_0, false>,  (const void*)paged_kv_store<64, CACHE_Q8_0, true>,
+        (const void*)paged_kv_store<64, CACHE_Q4_1, false>,  (const void*)paged_kv_store<64, CACHE_Q4_1, true>,
+        (const void*)paged_kv_store<128, CACHE_F16, false>,  (const void*)paged_kv_store<128, CACHE_F16, true>,
+        (const void*)paged_kv_store<128, CACHE_Q8_0, false>, (const void*)paged_kv_store<128, CACHE_Q8_0, true>,
+        (const void*)paged_kv_store<128, CACHE_Q4_1, false>, (const void*)paged_kv_store<128, CACHE_Q4_1, true>};
+    return go(fns[(c->head_dim == 128) * 6 + type_at(c) * 2 + src_type], a, PC_STORE_ITEMS, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int cfi_paged_kv_load(const CfiPagedCache* c, const int64_t* slots, void* k, void* v, long long k_stride,
@@ -275,7 +243,8 @@ extern "C" int cfi_paged_kv_load(const CfiPagedCache* c, const int64_t* slots, v
     if (n_tokens == 0) return 0;
     a.dst_k = static_cast<uint8_t*>(k);
     a.dst_v = static_cast<uint8_t*>(v);
-    static const void* const fns[4] = {(const void*)paged_kv_load<64, false>, (const void*)paged_kv_load<64, true>,
-                                       (const void*)paged_kv_load<128, false>, (const void*)paged_kv_load<128, true>};
-    return go(fns[(c->head_dim == 128) * 2 + (c->type == 8)], a, PC_LOAD_ITEMS, static_cast<cudaStream_t>(stream));
+    static const void* const fns[6] = {
+        (const void*)paged_kv_load<64, CACHE_F16>,  (const void*)paged_kv_load<64, CACHE_Q8_0>,  (const void*)paged_kv_load<64, CACHE_Q4_1>,
+        (const void*)paged_kv_load<128, CACHE_F16>, (const void*)paged_kv_load<128, CACHE_Q8_0>, (const void*)paged_kv_load<128, CACHE_Q4_1>};
+    return go(fns[(c->head_dim == 128) * 3 + type_at(c)], a, PC_LOAD_ITEMS, static_cast<cudaStream_t>(stream));
 }

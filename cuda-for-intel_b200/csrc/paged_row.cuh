@@ -1,0 +1,130 @@
+// paged_row.cuh -- eight values of a row of K or V on their way into a paged cache (paged_cache.cuh).  Four neighbouring
+// lanes, 8 values each, make a block of 32; all lanes of a warp call together.
+//
+// Q8_0: d = max|x| / 127, q = rn(x * (1/d)), stored scale f16(d); read back as f16(q * scale).
+// Q4_1: d = (max - min) / 15, q = floor((x - min) / d + 1/2), stored f16(d) and f16(min), all rounded from the exact values.  The
+// quotient in 32 bits is off by less than 2^-17, d by 2 units of its last place: only a lane whose values come nearer to a border
+// than that (one in a thousand) works them out in 64 bits, where differences and products of f32 values are exact.
+#pragma once
+#include "paged_cache.cuh"
+
+CFI_DEV int to_s8(float x) {  // to the nearest, ties to even; the ends at +-128, a NaN 0
+    int q;
+    asm("cvt.rni.sat.s8.f32 %0, %1;" : "=r"(q) : "f"(x));
+    return q;
+}
+CFI_DEV uint32_t bytes_of(int a, int b, int c, int d) {
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
+// A lane's 8 values, as f32 and as f16.
+struct Row8 {
+    float x[8];
+    uint4 h;
+};
+
+template <bool SRC_F16> CFI_DEV float block_max(const Row8& r) {  // of a block that has a NaN: NaN
+    float m;
+    if (SRC_F16) {
+        __half2 h = abs_h2(r.h.x);
+        h = __hmax2_nan(__hmax2_nan(h, abs_h2(r.h.y)), __hmax2_nan(abs_h2(r.h.z), abs_h2(r.h.w)));
+        h = __hmax2_nan(h, __lowhigh2highlow(h));
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) h = __hmax2_nan(h, __shfl_xor_sync(0xffffffffu, h, o));
+        m = __low2float(h);
+    } else {
+        m = 0.0f;
+        uint32_t nan = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            m = fmaxf(m, fabsf(r.x[j]));  // drops a NaN
+            nan |= (uint32_t)(r.x[j] != r.x[j]);
+        }
+        if (nan) m = __uint_as_float(0x7fffffffu);
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+            const float other = __shfl_xor_sync(0xffffffffu, m, o);
+            m = other != other ? other : m != m ? m : fmaxf(m, other);
+        }
+    }
+    return m;
+}
+
+// Values 8 g .. 8 g + 7 of position `off` of a region; nothing is written where `ok` is false.
+template <int D, bool SRC_F16> CFI_DEV void put_q8_0(const Row8& r, uint8_t* region, int page_shift, int off, int g, bool ok) {
+    const float m = block_max<SRC_F16>(r);
+    const float d = m / 127.0f, id = d > 0.0f ? 1.0f / d : 0.0f;
+    int q[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) q[j] = to_s8(r.x[j] * id);
+    const uint32_t w[2] = {bytes_of(q[0], q[1], q[2], q[3]), bytes_of(q[4], q[5], q[6], q[7])};
+    if (!ok) return;
+    *reinterpret_cast<uint2*>(region + (size_t)off * D + g * 8) = make_uint2(w[0], w[1]);
+    if ((g & 3) == 0)
+        *reinterpret_cast<uint16_t*>(region + (size_t)(D << page_shift) + ((size_t)off * (D / 32) + g / 4) * 2) =
+            d != d ? (uint16_t)0x7fff : f2h_bits(d);
+}
+
+template <int D> CFI_DEV void put_q4_1(const Row8& r, uint8_t* region, int off, int g, bool of_v, bool ok) {
+    float lo = r.x[0], hi = r.x[0], zero = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        lo = fminf(lo, r.x[j]);
+        hi = fmaxf(hi, r.x[j]);
+        zero = fmaf(r.x[j], 0.0f, zero);  // NaN where one is not finite
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        zero += __shfl_xor_sync(0xffffffffu, zero, o);
+    }
+    const float range = hi - lo, inv = 15.0f / range, d32 = range * (1.0f / 15.0f);
+    // slow: d at a border of f16, where it is below its normal numbers, or 32 bits do not hold the quotients
+    const uint32_t below = (__float_as_uint(d32) & 0x1fffu) - 0x0ffcu;
+    bool slow = below <= 8u || !(d32 >= 6.2e-5f && d32 <= 6.0e4f);
+    uint32_t w = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const float t = fmaf(r.x[j] - lo, inv, 0.5f), f = floorf(t);
+        slow |= fabsf(t - f - 0.5f) > 0.49998f;
+        w |= (uint32_t)(int)f << (4 * j);
+    }
+    uint16_t d = f2h_bits(d32);
+    if (slow) {
+        const double wide = (double)hi - (double)lo;
+        d = __half_as_ushort(__double2half(wide / 15.0));
+        w = 0;
+        if (wide > 0.0) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) w |= (uint32_t)(int)floor(((double)r.x[j] - (double)lo) * 15.0 / wide + 0.5) << (4 * j);
+        }
+    }
+    uint16_t m = f2h_bits(lo);
+    if (zero != 0.0f || (d & 0x7c00) == 0x7c00 || (m & 0x7c00) == 0x7c00) {
+        d = m = 0x7fff;
+        w = 0;
+    }
+    if (!ok) return;
+    const int row = off % Q41_TILE, b = g >> 2, c = g & 3;
+    uint8_t* tile = region + Q41<D>::tile_at(off);
+    if (of_v) {
+        *reinterpret_cast<uint16_t*>(tile + Q41<D>::v_at(row, b, 2 * c)) = (uint16_t)w;
+        *reinterpret_cast<uint16_t*>(tile + Q41<D>::v_at(row, b, 2 * c + 1)) = (uint16_t)(w >> 16);
+    } else {
+        *reinterpret_cast<uint32_t*>(tile + Q41<D>::k_at(row, b, c)) = w;
+    }
+    if (c == 0) *reinterpret_cast<uint16_t*>(tile + Q41<D>::scale_at(row, b)) = d;
+    if (c == 1) *reinterpret_cast<uint16_t*>(tile + Q41<D>::min_at(row, b)) = m;
+}
+
+template <int D, int TY, bool SRC_F16>
+CFI_DEV void put_row8(const Row8& r, uint8_t* region, int page_shift, int off, int g, bool of_v, bool ok) {
+    if (TY == CACHE_F16) {
+        if (ok) *reinterpret_cast<uint4*>(region + ((size_t)off * D + g * 8) * 2) = r.h;
+    } else if (TY == CACHE_Q8_0) {
+        put_q8_0<D, SRC_F16>(r, region, page_shift, off, g, ok);
+    } else {
+        put_q4_1<D>(r, region, off, g, of_v, ok);
+    }
+}
