@@ -94,32 +94,10 @@ __global__ void __launch_bounds__(W * 32, (PaShape<D, Q8, W>::CTAS)) paged_attn(
     if (a.whole) {
         seq = blockIdx.x / hc;
         pair = blockIdx.x - seq * hc;
-    } else {
-        // ---- this CTA's run ----
-        cut.read(a, gridDim.x);
-        if ((int)blockIdx.x >= paged_runs(cut.total, cut.quota)) return;
-        begin = at = blockIdx.x * cut.quota;
-        end = paged_run_end(begin, cut.quota, cut.total);
-        auto among = [&](int base, int n) {  // is it one of the 32 sequences from `base` on, this lane's with n units?
-            int incl = n;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int x = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += x;
-            }
-            const uint32_t hit = __ballot_sync(0xffffffffu, seq_start + incl > at);
-            const int l = hit ? __ffs(hit) - 1 : 31;
-            seq = base + l;
-            seq_start += __shfl_sync(0xffffffffu, hit ? incl - n : incl, l);
-            return hit != 0;
-        };
-        bool found = false;
-#pragma unroll
-        for (int e = 0; e < PA_KEPT; e++)
-            if (!found) found = among(32 * e, cut.units[e]);
-        for (int base = 32 * PA_KEPT; !found && base < a.n_seq; base += 32)
-            found = among(base, base + lane < a.n_seq ? cut.units_of(base + lane) * hc : 0);
+    } else if (!cut.find(a, &begin, &end, &seq, &seq_start)) {
+        return;
     }
+    at = begin;
 
     const uint32_t ring = smem_u32(smem) + warp * S::RING;
     PaShared shared[2];  // of the pairs that it goes on with, and leaves unfinished
@@ -416,25 +394,7 @@ __global__ void __launch_bounds__(W * 32, (PaShape<D, Q8, W>::CTAS)) paged_attn(
             seq++;
         }
     }
-    // ---- the results that are parts: the last of a pair's CTAs to come here joins them ----
-    if (a.whole || (shared[0].id < 0 && shared[1].id < 0)) return;
-    if (lane == 0 && warp < 2) {  // one thread for each
-        const PaShared p = warp == 0 ? shared[0] : shared[1];
-        bool last = false;
-        if (p.id >= 0) {
-            __threadfence();  // after a barrier: covers the stores of the whole CTA
-            last = atomicAdd(&a.counters[p.id], 1u) == (unsigned)(p.n - 1);
-            if (last) {
-                __threadfence();
-                a.counters[p.id] = 0u;
-            }
-        }
-        s_last[warp] = last;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int x = 0; x < 2; x++)
-        if (s_last[x]) join_parts<S, D, W * 32>(a, shared[x]);
+    if (!a.whole) join_shared<S, D, W * 32>(a, shared, s_last);
 }
 
 template <int D, bool Q8, int W> int launch(PaArgs& a, long long pairs, long long most_units, cudaStream_t stream) {

@@ -96,6 +96,36 @@ template <int TILE, int FIXED> struct PaCut {
         total = __reduce_add_sync(0xffffffffu, n);
         quota = paged_quota(total, ctas, FIXED + PA_WARPS);
     }
+    // This CTA's run [*begin, *end) and the sequence that it begins in, whose first unit is *seq_start; false where it has none.
+    // Called by whole warps.
+    CFI_DEV bool find(const PaArgs& a, int* begin, int* end, int* seq, int* seq_start) {
+        const int lane = threadIdx.x & 31, hc = a.n_kv_head * a.chunks;
+        read(a, gridDim.x);
+        if ((int)blockIdx.x >= paged_runs(total, quota)) return false;
+        const int at = blockIdx.x * quota;
+        *begin = at;
+        *end = paged_run_end(at, quota, total);
+        auto among = [&](int base, int n) {  // is it one of the 32 sequences from `base` on, this lane's with n units?
+            int incl = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += x;
+            }
+            const uint32_t hit = __ballot_sync(0xffffffffu, *seq_start + incl > at);
+            const int l = hit ? __ffs(hit) - 1 : 31;
+            *seq = base + l;
+            *seq_start += __shfl_sync(0xffffffffu, hit ? incl - n : incl, l);
+            return hit != 0;
+        };
+        bool found = false;
+#pragma unroll
+        for (int e = 0; e < PA_KEPT; e++)
+            if (!found) found = among(32 * e, units[e]);
+        for (int base = 32 * PA_KEPT; !found && base < a.n_seq; base += 32)
+            found = among(base, base + lane < a.n_seq ? units_of(base + lane) * hc : 0);
+        return true;
+    }
 };
 
 // A pair that this CTA has a part of, and what it takes to join all of them.
@@ -139,6 +169,29 @@ template <class S, int D, int THREADS> CFI_DEV void join_parts(const PaArgs& a, 
         }
         write_out(a, p.seq, p.head0 + h, D, d, o, l);
     }
+}
+
+// Behind a CTA's run: the results that are parts are joined by the last of their pair's CTAs to come here.
+template <class S, int D, int THREADS> CFI_DEV void join_shared(const PaArgs& a, const PaShared (&shared)[2], int (&s_last)[2]) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (shared[0].id < 0 && shared[1].id < 0) return;
+    if (lane == 0 && warp < 2) {  // one thread for each
+        const PaShared p = warp == 0 ? shared[0] : shared[1];
+        bool last = false;
+        if (p.id >= 0) {
+            __threadfence();  // after a barrier: covers the stores of the whole CTA
+            last = atomicAdd(&a.counters[p.id], 1u) == (unsigned)(p.n - 1);
+            if (last) {
+                __threadfence();
+                a.counters[p.id] = 0u;
+            }
+        }
+        s_last[warp] = last;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < 2; x++)
+        if (s_last[x]) join_parts<S, D, THREADS>(a, shared[x]);
 }
 
 // The Q4_1 kernel's launch (k_paged_attn_q4.cu), for a checked call.
