@@ -14,8 +14,7 @@
 //   V: two positions meet in a register, so half-words of two rows are first put together by one byte permutation.
 // Which position is which column of the scores is free, as long as the weights go back to the same: column 2 c + e of the n-th eight
 // is position 8 n + 4 e + (c ^ 3 e), so that no two lanes read the same bank of K or of V.
-// The minima of K meet the sums of q over each block in one MMA for 8 positions; those of V are added to
-// the weights' in 32 bits.
+// The minima of K meet the sums of q over each block in one MMA for 8 positions, those of V the weights in one for 16.
 #include "paged_attn.cuh"
 #include "sm100_ptx.cuh"
 #include "cfi_kernels.h"
@@ -78,7 +77,18 @@ CFI_DEV f2 fma2(f2 a, f2 b, f2 c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
     return r;
 }
-CFI_DEV float half_of(uint32_t w, int i) { return h2f_bits((uint16_t)(i ? w >> 16 : w)); }
+CFI_DEV float half_of(uint32_t w, int i) {
+    const __half2 h = *reinterpret_cast<const __half2*>(&w);
+    return i ? __high2float(h) : __low2float(h);
+}
+CFI_DEV void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {  // the sum begins with it
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+CFI_DEV void ldsm_x2_trans(uint32_t a, uint32_t& r0, uint32_t& r1) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(r0), "=r"(r1) : "r"(a));
+}
 // the even and odd nibbles of each half's lower byte as f16 numbers, n 2^-24 and 16 n 2^-24
 CFI_DEV uint32_t low_nibbles(uint32_t w) { return w & 0x000f000fu; }
 CFI_DEV uint32_t high_nibbles(uint32_t w) { return w & 0x00f000f0u; }
@@ -189,12 +199,12 @@ __global__ void __launch_bounds__(W * 32, (P4Shape<D, W>::CTAS)) paged_attn_q4(c
             cp_async_commit();
         };
 
-        // V's scales have been below 2^top_v; weights, l, o and mins have 2^-top_v in them, o 2^-24 (odd dims 2^-20) besides
-        float o[NT][4], m = -INFINITY, top_v = P4_LEAST_V;
-        f2 l = 0, mins[NB];
+        // V's scales have been below 2^top_v; o has 2^-top_v in it, and 2^-24 (odd dims 2^-20)
+        float o[NT][4], mins[4], m = -INFINITY, top_v = P4_LEAST_V, per_top = ex2(-P4_LEAST_V);
+        f2 l = 0;
         __half2 limit_v = __float2half2_rn(ex2(top_v));
 #pragma unroll
-        for (int b = 0; b < NB; b++) mins[b] = 0;
+        for (int e = 0; e < 4; e++) mins[e] = 0.0f;
 #pragma unroll
         for (int j = 0; j < NT; j++)
 #pragma unroll
@@ -265,9 +275,9 @@ __global__ void __launch_bounds__(W * 32, (P4Shape<D, W>::CTAS)) paged_attn_q4(c
                 const uint32_t tile = sk + (n >> 1) * S::TILE;
                 const int row = row_k + 8 * (n & 1);
                 {
-                    float acc[4] = {};
-                    const uint32_t zero[4] = {qs[0], qs[1], 0, 0};
-                    mma_f16f32(acc, zero, lds32(tile + L::NIBBLES + row * L::PARAM_ROW + 4 * (c & (NB - 1))), 0);
+                    float acc[4];
+                    const uint32_t sums2[4] = {qs[0], qs[1], 0, 0};
+                    mma_first(acc, sums2, lds32(tile + L::NIBBLES + row * L::PARAM_ROW + 4 * (c & (NB - 1))), 0);
                     s[n] = mul2(add2(pair2(acc[0], acc[1]), pair2(acc[2], acc[3])), pair2(64.0f / P4_N, 64.0f / P4_N));
                 }
                 uint32_t w[NB], d[2][NB / 2];  // eight dims of each block of the lane's row; scales of columns 2c and 2c+1
@@ -290,8 +300,8 @@ __global__ void __launch_bounds__(W * 32, (P4Shape<D, W>::CTAS)) paged_attn_q4(c
                 }
 #pragma unroll
                 for (int b = 0; b < NB; b++) {
-                    float acc[4] = {};
-                    mma_f16f32(acc, qf[2 * b], low_nibbles(w[b]), high_nibbles(w[b]));
+                    float acc[4];
+                    mma_first(acc, qf[2 * b], low_nibbles(w[b]), high_nibbles(w[b]));
                     mma_f16f32(acc, qf[2 * b + 1], low_nibbles(w[b] >> 8), high_nibbles(w[b] >> 8));
                     s[n] = fma2(add2(pair2(acc[0], acc[1]), pair2(acc[2], acc[3])),
                                 pair2(half_of(d[0][b >> 1], b & 1), half_of(d[1][b >> 1], b & 1)), s[n]);
@@ -317,14 +327,14 @@ __global__ void __launch_bounds__(W * 32, (P4Shape<D, W>::CTAS)) paged_attn_q4(c
                 const f2 alpha2 = pair2(alpha, alpha);
                 l = mul2(l, alpha2);
 #pragma unroll
-                for (int b = 0; b < NB; b++) mins[b] = mul2(mins[b], alpha2);
+                for (int e = 0; e < 4; e++) mins[e] *= alpha;
 #pragma unroll
                 for (int j = 0; j < NT; j++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) o[j][e] *= alpha;
                 m = mn;
             }
-            const float sub = m == -INFINITY ? 0.0f : -m * P4_N, rise = P4_TOP - top_v;  // added last: a large score would swallow it
+            const float sub = m == -INFINITY ? 0.0f : -m * P4_N, rise = P4_TOP;  // added last: a large score would swallow it
             f2 p[4];
 #pragma unroll
             for (int n = 0; n < 4; n++) {
@@ -346,16 +356,11 @@ __global__ void __launch_bounds__(W * 32, (P4Shape<D, W>::CTAS)) paged_attn_q4(c
                     const uint32_t ex = __float_as_uint(fmaxf(__low2float(d), __high2float(d))) >> 23;
                     const float grown = fmaxf(top_v, fminf((float)__reduce_max_sync(0xffffffffu, ex) - 126.0f, P4_MOST_V));
                     const float f = ex2(top_v - grown);
-                    const f2 ff = pair2(f, f);
-                    l = mul2(l, ff);
-#pragma unroll
-                    for (int n = 0; n < 4; n++) p[n] = mul2(p[n], ff);
-#pragma unroll
-                    for (int b = 0; b < NB; b++) mins[b] = mul2(mins[b], ff);
 #pragma unroll
                     for (int j = 0; j < NT; j++)
 #pragma unroll
                         for (int e = 0; e < 4; e++) o[j][e] *= f;
+                    per_top = ex2(-grown);
                     top_v = grown;
                     limit_v = __float2half2_rn(ex2(grown));
                 }
@@ -363,7 +368,22 @@ __global__ void __launch_bounds__(W * 32, (P4Shape<D, W>::CTAS)) paged_attn_q4(c
 #pragma unroll
             for (int t = 0; t < 2; t++) {
                 const uint32_t tile = sv + t * S::TILE;
-                uint32_t w[2][2][NB / 2], dm[2][2][NB];  // of column e of eight n: the lane's dims; scales, then minima
+                {  // minima: column x of a row's scales and minima, of which those from NB on count
+                    uint32_t pf[4], b0, b1;
+#pragma unroll
+                    for (int n = 0; n < 2; n++) split(both(p[2 * t + n]).x, both(p[2 * t + n]).y, &pf[2 * n], &pf[2 * n + 1]);
+                    if (D == 128) {
+                        ldsm_x2_trans(tile + L::NIBBLES + position_of(lane >> 1 & 3, lane & 1, lane >> 3 & 1) * L::PARAM_ROW, b0, b1);
+                    } else {  // rows of four numbers: column g & 3 of the lane's four positions
+                        uint32_t x[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) x[e] = lds16(tile + L::NIBBLES + position_of(c, e & 1, e >> 1) * L::PARAM_ROW + 2 * (g & 3));
+                        b0 = x[0] | x[1] << 16;
+                        b1 = x[2] | x[3] << 16;
+                    }
+                    mma_f16f32(mins, pf, b0, b1);
+                }
+                uint32_t w[2][2][NB / 2], d[2][2][NB / 2];  // of column e of eight n: the lane's dims; scales
 #pragma unroll
                 for (int n = 0; n < 2; n++)
 #pragma unroll
@@ -371,25 +391,24 @@ __global__ void __launch_bounds__(W * 32, (P4Shape<D, W>::CTAS)) paged_attn_q4(c
                         const int row = position_of(c, e, n);
                         const uint32_t q = tile + row * L::ROW + L::v_group(row, g) * (D / 16), r = tile + L::NIBBLES + row * L::PARAM_ROW;
                         if (D == 128) {
-                            const uint2 x = lds64(q);
+                            const uint2 x = lds64(q), y = lds64(r);
                             w[n][e][0] = x.x, w[n][e][NB / 2 - 1] = x.y;
-                            const uint4 y = lds128(r);
-                            dm[n][e][0] = y.x, dm[n][e][1] = y.y, dm[n][e][NB - 2] = y.z, dm[n][e][NB - 1] = y.w;
+                            d[n][e][0] = y.x, d[n][e][NB / 2 - 1] = y.y;
                         } else {
                             w[n][e][0] = lds32(q);
-                            const uint2 y = lds64(r);
-                            dm[n][e][0] = y.x, dm[n][e][1] = y.y;
+                            d[n][e][0] = lds32(r);
                         }
                     }
+                f2 pv[2];
+#pragma unroll
+                for (int n = 0; n < 2; n++) pv[n] = mul2(p[2 * t + n], pair2(per_top, per_top));
 #pragma unroll
                 for (int b = 0; b < NB; b++) {
                     uint32_t pf[4], bw[2][4];
 #pragma unroll
                     for (int n = 0; n < 2; n++) {
-                        const f2 pn = p[2 * t + n];
-                        const float2 x = both(mul2(pn, pair2(half_of(dm[n][0][b >> 1], b & 1), half_of(dm[n][1][b >> 1], b & 1))));
+                        const float2 x = both(mul2(pv[n], pair2(half_of(d[n][0][b >> 1], b & 1), half_of(d[n][1][b >> 1], b & 1))));
                         split(x.x, x.y, &pf[2 * n], &pf[2 * n + 1]);
-                        mins[b] = fma2(pn, pair2(half_of(dm[n][0][(NB + b) >> 1], b & 1), half_of(dm[n][1][(NB + b) >> 1], b & 1)), mins[b]);
                         // dims 32 b + 4 g .. + 3 of two positions: column g of MMA e is dim 32 b + 4 g + e
                         const uint32_t z = __byte_perm(w[n][0][b >> 1], w[n][1][b >> 1], b & 1 ? 0x7632 : 0x5410);
                         bw[n][0] = low_nibbles(z);
@@ -405,16 +424,13 @@ __global__ void __launch_bounds__(W * 32, (P4Shape<D, W>::CTAS)) paged_attn_q4(c
         }
         // ---- the warps meet: [warp][head]: D values, maximum, sum ----
         cp_async_wait<0>();
-        const float back = ex2(top_v);  // each warp has had scales of its own
-        float sum = (both(l).x + both(l).y) * back, low[NB];
+        const float back = ex2(top_v) * P4_N;  // each warp has had scales of its own
+        float sum = both(l).x + both(l).y, low[NB];
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
-        for (int b = 0; b < NB; b++) {
-            low[b] = both(mins[b]).x + both(mins[b]).y;
-            low[b] += __shfl_xor_sync(0xffffffffu, low[b], 1);
-            low[b] += __shfl_xor_sync(0xffffffffu, low[b], 2);
-        }
+        for (int b = 0; b < NB; b++)  // columns 2 c and 2 c + 1 of the minima are this lane's
+            low[b] = __shfl_sync(0xffffffffu, mins[b & 1] + mins[2 + (b & 1)], (lane & ~3) + (NB + b) / 2);
         __syncthreads();  // every warp is done with its stages
         float* meet = reinterpret_cast<float*>(smem);
         float* mine_o = meet + warp * S::MEET + g * S::MEET_ROW;
@@ -425,7 +441,7 @@ __global__ void __launch_bounds__(W * 32, (P4Shape<D, W>::CTAS)) paged_attn_q4(c
                 float f[4];
 #pragma unroll
                 for (int x = 0; x < 4; x++)
-                    f[x] = fmaf(o[4 * b + x][e] + o[4 * b + x][e + 2], x & 1 ? P4_N / 16.0f : P4_N, low[b]) * back;
+                    f[x] = fmaf(o[4 * b + x][e] + o[4 * b + x][e + 2], x & 1 ? back / 16.0f : back, low[b]);
                 *reinterpret_cast<float4*>(mine_o + 32 * b + 8 * c + 4 * e) = make_float4(f[0], f[1], f[2], f[3]);
             }
         if (c == 0) *reinterpret_cast<float2*>(mine_o + D) = make_float2(m * P4_N * unit, sum);
