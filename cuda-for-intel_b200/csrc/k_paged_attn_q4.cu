@@ -7,11 +7,15 @@
 // of the cache: what a tile costs beside its products (maximum, vote, copies) is shared by twice as many.
 //
 // A position and kv head are 160 bytes with heads of 128, which at the memory's rate leaves a warp some 28 instructions: what has to
-// be cheap is making operands of nibbles.  A nibble needs no conversion: the bits 0x000n are the f16 number n 2^-24, and
-// 0x00n0 is 16 n 2^-24, exact subnormals that the MMA multiplies like any others.  One AND (with one shift for every second pair)
-// makes two operands; the powers of two go into q (divided by 16 where the upper nibbles meet it) and into the result.
-//   K: a word of the cache is 8 dims of one position for one lane; dims i and i + 4 of it share a register.
-//   V: two positions meet in a register, so half-words of two rows are first put together by one byte permutation.
+// be cheap is making operands of nibbles.  They need no conversion: the bits 0x00hl of a byte are the f16 number (16 h + l) 2^-24 and
+// 0x000l is l 2^-24, exact subnormals that the MMA multiplies like any others.  A byte goes in twice, whole and without its upper
+// nibble, so that four ANDs and permutations make operands of eight nibbles; where
+//   x l + y h = (x - y/16) l + (y/16) (16 h + l),
+// the weights x, y of q take the first form of K's product, and V's sums are taken apart at the end.
+//   K: a word of the cache is 8 dims of one position for one lane; dims i and i + 4 of it share a register.  A is q, B is K: rows
+//      0-7 of the result and rows 8-15 are added.
+//   V: two positions meet in a register, so half-words of two rows are first put together by one byte permutation.  A is V with
+//      dims as rows, B the weights, which lie as the scores came out; their two parts add up in the same sums.
 // Which position is which column of the scores is free, as long as the weights go back to the same: column 2 c + e of the n-th eight
 // is position 8 n + 4 e + (c ^ 3 e), so that no two lanes read the same bank of K or of V.
 // The minima of K meet the sums of q over each block in one MMA for 8 positions, those of V the weights in one for 16.
@@ -20,6 +24,7 @@
 #include "cfi_kernels.h"
 
 #include <algorithm>
+#include <type_traits>
 #include <math.h>
 #include <stdlib.h>
 #include <string.h>
@@ -38,8 +43,8 @@ using Cut = PaCut<P4_TILE, P4_FIXED>;
 template <int D, int W = PA_WARPS> struct P4Shape {
     static constexpr int TILE = Q41<D>::TILE;
     static constexpr int STAGE = 4 * TILE;  // two tiles of K, two of V
-    static constexpr int STAGES = D == 64 ? 5 : 3;
-    static constexpr int CTAS = W > PA_WARPS ? 1 : 3;  // per SM
+    static constexpr int STAGES = D == 64 ? 5 : W > PA_WARPS ? 4 : 3;
+    static constexpr int CTAS = W > PA_WARPS ? 1 : D == 64 ? 3 : 2;  // per SM
     static constexpr int RING = STAGES * STAGE;        // a warp's
     static constexpr int SMEM = W * RING;
     static constexpr int PART = PA_HEADS * (D + 2);    // floats of a partial result: values, then maximum and sum of each head
@@ -81,28 +86,514 @@ CFI_DEV float half_of(uint32_t w, int i) {
     const __half2 h = *reinterpret_cast<const __half2*>(&w);
     return i ? __high2float(h) : __low2float(h);
 }
+// (x, y) as f16 and what the rounding left, as f16: 22 bits together
+CFI_DEV void split2(f2 x, uint32_t* hi, uint32_t* lo) {
+    const __half2 h = __floats2half2_rn(both(x).x, both(x).y);
+    const float2 f = __half22float2(h);
+    *hi = h2_bits(h);
+    *lo = h2_bits(__floats2half2_rn(both(x).x - f.x, both(x).y - f.y));
+}
 CFI_DEV void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {  // the sum begins with it
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
                  : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
+CFI_DEV void mma_k8(float (&d)[4], const uint32_t (&a)[2], uint32_t b) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%7, %7, %7, %7};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(b), "f"(0.0f));
+}
+CFI_DEV uint32_t turned(uint32_t x) {  // an 8 x 8 of f16: lane (g, c) has row g, columns 2 c and 2 c + 1
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
 CFI_DEV void ldsm_x2_trans(uint32_t a, uint32_t& r0, uint32_t& r1) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(r0), "=r"(r1) : "r"(a));
 }
-// the even and odd nibbles of each half's lower byte as f16 numbers, n 2^-24 and 16 n 2^-24
-CFI_DEV uint32_t low_nibbles(uint32_t w) { return w & 0x000f000fu; }
-CFI_DEV uint32_t high_nibbles(uint32_t w) { return w & 0x00f000f0u; }
+// The lower byte of each half, without and with its upper nibble, as f16 numbers times 2^24; then the upper byte.
+struct Nibbles {
+    uint32_t x0, y0, x1, y1;
+    CFI_DEV explicit Nibbles(uint32_t w) {
+        y0 = w & 0x00ff00ffu;
+        x0 = w & 0x000f000fu;
+        y1 = __byte_perm(w, 0, 0x4341);
+        x1 = y1 & 0x000f000fu;
+    }
+};
 // column 2 c + e of the n-th eight scores
 CFI_DEV int position_of(int c, int e, int n) { return 8 * n + 4 * e + (c ^ (3 * e)); }
 
-template <int D, int W>
+// The largest of V's scales so far: they have been below 2^top; the weights times scales are divided by it.
+struct ScalesTop {
+    float top = P4_LEAST_V, per = 8388608.0f;  // per: 2^-top
+    // Looks at a tile's scales, some a lane; where one passes `top`, raises it and gives what the sums so far have to be multiplied by.
+    template <int D> CFI_DEV bool raise(uint32_t sv, float* by) {
+        const int lane = threadIdx.x & 31;
+        __half2 d = __float2half2_rn(0.0f);
+#pragma unroll
+        for (int x = 0; x < D / 64; x++)
+            d = __hmax2_nan(d, abs_h2(lds32(sv + (lane >> 4) * Q41<D>::TILE + Q41<D>::NIBBLES + (lane & 15) * Q41<D>::PARAM_ROW + 4 * x)));
+        if (!__any_sync(0xffffffffu, !__hblt2(d, limit))) return false;
+        // the exponent of the largest, cut where that is an infinity or a NaN
+        const uint32_t ex = __float_as_uint(fmaxf(__low2float(d), __high2float(d))) >> 23;
+        const float grown = fmaxf(top, fminf((float)__reduce_max_sync(0xffffffffu, ex) - 126.0f, P4_MOST_V));
+        *by = ex2(top - grown);
+        top = grown;
+        per = ex2(-grown);
+        limit = __float2half2_rn(ex2(grown));
+        return true;
+    }
+    __half2 limit = __float2half2_rn(1.1920929e-7f);
+};
+
+// Scales of two rows of blocks 0, 1 and 2, 3
+template <int D> CFI_DEV void scales_of(uint32_t tile, int row, uint32_t (&d)[D / 64]) {
+    const uint32_t p = tile + Q41<D>::NIBBLES + row * Q41<D>::PARAM_ROW;
+    if (D == 128) {
+        const uint2 x = lds64(p);
+        d[0] = x.x, d[D / 64 - 1] = x.y;
+    } else {
+        d[0] = lds32(p);
+    }
+}
+// This lane's eight dims of each block of a row of K
+template <int D> CFI_DEV void dims_of_k(uint32_t tile, int row, uint32_t (&w)[D / 32]) {
+    const int c = threadIdx.x & 3;
+    if (D == 128) {
+        const uint4 x = lds128(tile + row * Q41<D>::ROW + c * 16);
+        w[0] = x.x, w[1] = x.y, w[D / 32 - 2] = x.z, w[D / 32 - 1] = x.w;
+    } else {
+        const uint2 x = lds64(tile + row * Q41<D>::ROW + c * 8);
+        w[0] = x.x, w[1] = x.y;
+    }
+}
+// This lane's four dims of blocks 0, 1 and 2, 3 of a row of V
+template <int D> CFI_DEV void dims_of_v(uint32_t tile, int row, uint32_t (&w)[D / 64]) {
+    const int g = threadIdx.x >> 2 & 7;
+    const uint32_t q = tile + row * Q41<D>::ROW + Q41<D>::v_group(row, g) * (D / 16);
+    if (D == 128) {
+        const uint2 x = lds64(q);
+        w[0] = x.x, w[D / 64 - 1] = x.y;
+    } else {
+        w[0] = lds32(q);
+    }
+}
+// The tile's scales and minima, turned: of number g of a row, positions of columns 2 c and 2 c + 1 of both eights
+template <int D> CFI_DEV void params_turned(uint32_t tile, uint32_t& b0, uint32_t& b1) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    if (D == 128) {
+        ldsm_x2_trans(tile + Q41<D>::NIBBLES + position_of(lane >> 1 & 3, lane & 1, lane >> 3 & 1) * Q41<D>::PARAM_ROW, b0, b1);
+    } else {  // rows of four numbers: g & 3
+        uint32_t x[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = lds16(tile + Q41<D>::NIBBLES + position_of(c, e & 1, e >> 1) * Q41<D>::PARAM_ROW + 2 * (g & 3));
+        b0 = x[0] | x[1] << 16;
+        b1 = x[2] | x[3] << 16;
+    }
+}
+
+// A lane's query values, dims 32 b + 8 c .. + 7 of one head, as MMA operands: in log2 units over `unit`, split; and the sums of
+// the blocks over 2^6 where a row of scales and minima (2 NB numbers, of which a lane has two) has its minima.
+template <int D> struct Queries {
+    static constexpr int NB = D / 32;
+    uint32_t hi[2 * NB][2], lo[2 * NB][2], sum_hi, sum_lo;
+    float unit;
+    CFI_DEV void convert(float (&qv)[NB][8], float scale_log2) {
+        const int c = threadIdx.x & 3;
+        float largest = 0.0f;  // a NaN is passed over
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                qv[b][e] *= scale_log2;
+                largest = fmaxf(largest, fabsf(qv[b][e]));
+            }
+        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+        // 2^(its exponent - 14) and the other way round, both normal: below 2^-111 the largest stays below 2^14
+        const uint32_t exponent = max(__float_as_uint(largest) >> 23, 15u);
+        unit = __uint_as_float((exponent - 14) << 23);
+        const float per_unit = __uint_as_float((268 - exponent) << 23);
+        float sums[NB];
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            sums[b] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                qv[b][e] *= per_unit;
+                sums[b] += qv[b][e];
+            }
+            sums[b] += __shfl_xor_sync(0xffffffffu, sums[b], 1);
+            sums[b] += __shfl_xor_sync(0xffffffffu, sums[b], 2);
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const float y0 = qv[b][2 * k + 1] * 0.0625f, y1 = qv[b][2 * k + 5] * 0.0625f;
+                split(qv[b][2 * k] - y0, qv[b][2 * k + 4] - y1, &hi[2 * b + k][0], &lo[2 * b + k][0]);
+                split(y0, y1, &hi[2 * b + k][1], &lo[2 * b + k][1]);
+            }
+        }
+        const int x = 2 * c - NB;
+        const float s0 = x == 0 ? sums[0] : NB == 4 && x == 2 ? sums[NB - 2] : 0.0f, s1 = x == 0 ? sums[1] : NB == 4 && x == 2 ? sums[NB - 1] : 0.0f;
+        split(s0 * 0.015625f, s1 * 0.015625f, &sum_hi, &sum_lo);
+    }
+};
+
+// ---- five to eight heads ----
+// Scores: A is q (rows 0-7 the heads' f16 values, rows 8-15 the rest), B is K.  A lane has head g, columns 2 c and 2 c + 1.
+template <int D> struct ManyHeads {
+    static constexpr int NB = D / 32;
+    uint32_t qf[2 * NB][4], qs[2];
+    // o has 2^(-top - 24) in it.  Of heads 2 c and 2 c + 1, dims 32 b + 4 g + 2 x and the next one, which has 16 times itself and the first
+    float o[NB][2][4], mins[4], m, unit;
+    f2 l;
+    ScalesTop v;
+    static CFI_DEV int head() { return threadIdx.x >> 2 & 7; }  // whose queries this lane loads
+    CFI_DEV void begin() {
+        m = -INFINITY;
+        l = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) mins[e] = 0.0f;
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[b][0][e] = o[b][1][e] = 0.0f;
+    }
+    CFI_DEV void queries(const Queries<D>& q) {
+#pragma unroll
+        for (int k = 0; k < 2 * NB; k++) qf[k][0] = q.hi[k][0], qf[k][1] = q.lo[k][0], qf[k][2] = q.hi[k][1], qf[k][3] = q.lo[k][1];
+        qs[0] = q.sum_hi, qs[1] = q.sum_lo;
+        unit = q.unit;
+    }
+    CFI_DEV void tile(uint32_t sk, uint32_t sv, int left) {
+        using L = Q41<D>;
+        const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+        // ---- scores, over 2^24 `unit` ----
+        f2 s[4];
+#pragma unroll
+        for (int n = 0; n < 4; n++) {
+            const uint32_t tile = sk + (n >> 1) * L::TILE;
+            const int row = position_of(g >> 1, g & 1, n & 1);
+            float first[4];
+            mma_k8(first, qs, lds32(tile + L::NIBBLES + row * L::PARAM_ROW + 4 * (c & (NB - 1))));
+            s[n] = pair2((first[0] + first[2]) * (64.0f / P4_N), (first[1] + first[3]) * (64.0f / P4_N));
+            uint32_t w[NB], d0[NB / 2], d1[NB / 2];
+            dims_of_k<D>(tile, row, w);
+            scales_of<D>(tile, position_of(c, 0, n & 1), d0);
+            scales_of<D>(tile, position_of(c, 1, n & 1), d1);
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                float acc[4];
+                const Nibbles k(w[b]);
+                mma_first(acc, qf[2 * b], k.x0, k.y0);
+                mma_f16f32(acc, qf[2 * b + 1], k.x1, k.y1);
+                s[n] = fma2(add2(pair2(acc[0], acc[1]), pair2(acc[2], acc[3])),
+                            pair2(half_of(d0[b >> 1], b & 1), half_of(d1[b >> 1], b & 1)), s[n]);
+            }
+        }
+        if (left < P4_TILE) {
+#pragma unroll
+            for (int n = 0; n < 4; n++) {
+                float2 x = both(s[n]);
+                if (16 * (n >> 1) + position_of(c, 0, n & 1) >= left) x.x = -INFINITY;
+                if (16 * (n >> 1) + position_of(c, 1, n & 1) >= left) x.y = -INFINITY;
+                s[n] = pair2(x.x, x.y);
+            }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < 4; n++) mx = fmaxf(mx, fmaxf(both(s[n]).x, both(s[n]).y));
+        if (__any_sync(0xffffffffu, mx > m)) {
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const float mn = fmaxf(m, mx), alpha = m == -INFINITY ? 0.0f : ex2((m - mn) * P4_N * unit);
+            l = mul2(l, pair2(alpha, alpha));
+            const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * c), a1 = __shfl_sync(0xffffffffu, alpha, 8 * c + 4);
+#pragma unroll
+            for (int e = 0; e < 4; e++) mins[e] *= alpha;
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int x = 0; x < 2; x++) o[b][x][0] *= a0, o[b][x][1] *= a1, o[b][x][2] *= a0, o[b][x][3] *= a1;
+            m = mn;
+        }
+        const float sub = m == -INFINITY ? 0.0f : -m * P4_N;  // P4_TOP is added last: a large score would swallow it
+        f2 p[4];
+#pragma unroll
+        for (int n = 0; n < 4; n++) {
+            const float2 x = both(fma2(fma2(s[n], pair2(P4_N, P4_N), pair2(sub, sub)), pair2(unit, unit), pair2(P4_TOP, P4_TOP)));
+            p[n] = pair2(ex2(x.x), ex2(x.y));
+            l = add2(l, p[n]);
+        }
+        // ---- weighted values: A is V with dims as rows, B the weights and then what f16 left of them ----
+        float by;
+        if (v.template raise<D>(sv, &by)) {
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[b][0][e] *= by, o[b][1][e] *= by;
+        }
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const uint32_t tile = sv + t * L::TILE;
+            {  // minima: column x of a row's scales and minima, of which those from NB on count
+                uint32_t pf[4], b0, b1;
+#pragma unroll
+                for (int n = 0; n < 2; n++) split2(p[2 * t + n], &pf[2 * n], &pf[2 * n + 1]);
+                params_turned<D>(tile, b0, b1);
+                mma_f16f32(mins, pf, b0, b1);
+            }
+            uint32_t w[2][2][NB / 2], d[2][2][NB / 2];  // of column 2 c + e of eight n
+            f2 pv[2];
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                pv[n] = mul2(p[2 * t + n], pair2(v.per, v.per));
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    dims_of_v<D>(tile, position_of(c, e, n), w[n][e]);
+                    scales_of<D>(tile, position_of(c, e, n), d[n][e]);
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                uint32_t hi[2], lo[2], z[2];
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    split2(mul2(pv[n], pair2(half_of(d[n][0][b >> 1], b & 1), half_of(d[n][1][b >> 1], b & 1))), &hi[n], &lo[n]);
+                    z[n] = __byte_perm(w[n][0][b >> 1], w[n][1][b >> 1], b & 1 ? 0x7632 : 0x5410);  // dims 32 b + 4 g .. + 3 of two positions
+                }
+                const Nibbles v0(z[0]), v1(z[1]);
+                const uint32_t r0[4] = {v0.x0, v0.y0, v1.x0, v1.y0}, r1[4] = {v0.x1, v0.y1, v1.x1, v1.y1};
+                mma_f16f32(o[b][0], r0, hi[0], hi[1]);
+                mma_f16f32(o[b][1], r1, hi[0], hi[1]);
+                mma_f16f32(o[b][0], r0, lo[0], lo[1]);
+                mma_f16f32(o[b][1], r1, lo[0], lo[1]);
+            }
+        }
+    }
+    // Values, maximum and sum of each head as rows of `row` floats.
+    CFI_DEV void finish(float* meet, int row) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+        const float back = ex2(v.top) * P4_N;  // each warp has had scales of its own
+        float sum = both(l).x + both(l).y;
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const float low = __shfl_sync(0xffffffffu, mins[b & 1] + mins[2 + (b & 1)], 4 * (2 * c + e) + (NB + b) / 2);  // column NB + b
+                float f[4];
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    f[2 * x] = fmaf(o[b][x][e], back, low);
+                    f[2 * x + 1] = fmaf(o[b][x][2 + e] - o[b][x][e], back / 16.0f, low);
+                }
+                *reinterpret_cast<float4*>(meet + (2 * c + e) * row + 32 * b + 4 * g) = make_float4(f[0], f[1], f[2], f[3]);
+            }
+        if (c == 0) *reinterpret_cast<float2*>(meet + g * row + D) = make_float2(m * P4_N * unit, sum);
+    }
+};
+
+// ---- up to four heads ----
+// Both parts of four heads fill the eight columns of one MMA, so that all products take half as many: A is K with positions as rows, B
+// has the heads' f16 values in columns 0-3 and the rest in 4-7, and the two are added when the scores are whole.  A lane then has heads
+// 2 (c & 1) and the next at positions g and g + 8 (in the order above), lanes c and c ^ 2 the same; for V's product it makes f16 values
+// (c < 2) or the rest of its weights, which one 8 x 8 transposition brings to the places that B has them.
+template <int D> struct FewHeads {
+    static constexpr int NB = D / 32;
+    uint32_t qb[2 * NB][2], qs;
+    // o as above; columns 2 c and 2 c + 1, of which those from 4 on are the weights' rest
+    float o[NB][2][4], mins[4], m[2], l[2], unit[2];
+    ScalesTop v;
+    static CFI_DEV int head() { return threadIdx.x >> 2 & 3; }
+    CFI_DEV void begin() {
+        m[0] = m[1] = -INFINITY;
+        l[0] = l[1] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; e++) mins[e] = 0.0f;
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[b][0][e] = o[b][1][e] = 0.0f;
+    }
+    CFI_DEV void queries(const Queries<D>& q) {
+        const int lane = threadIdx.x & 31, c = lane & 3;
+        const bool rest = lane >= 16;
+#pragma unroll
+        for (int k = 0; k < 2 * NB; k++) qb[k][0] = rest ? q.lo[k][0] : q.hi[k][0], qb[k][1] = rest ? q.lo[k][1] : q.hi[k][1];
+        qs = rest ? q.sum_lo : q.sum_hi;
+#pragma unroll
+        for (int x = 0; x < 2; x++) unit[x] = __shfl_sync(0xffffffffu, q.unit, 4 * (2 * (c & 1) + x));
+    }
+    CFI_DEV void tile(uint32_t sk, uint32_t sv, int left) {
+        using L = Q41<D>;
+        const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+        // ---- scores, over 2^24 `unit`: of position g + 8 r of half t, head x ----
+        float s[2][2][2];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const uint32_t tile = sk + t * L::TILE;
+            const int row = position_of(g >> 1, g & 1, 0);  // and 8 behind
+            uint32_t w[2][NB], d[2][NB / 2], low[2];
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                low[r] = lds32(tile + L::NIBBLES + (row + 8 * r) * L::PARAM_ROW + 4 * (c & (NB - 1)));
+                dims_of_k<D>(tile, row + 8 * r, w[r]);
+                scales_of<D>(tile, row + 8 * r, d[r]);
+            }
+            float first[4];
+            mma_k8(first, low, qs);
+#pragma unroll
+            for (int r = 0; r < 2; r++)
+#pragma unroll
+                for (int x = 0; x < 2; x++) s[t][r][x] = first[2 * r + x] * (64.0f / P4_N);
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                float acc[4];
+                const Nibbles k0(w[0][b]), k1(w[1][b]);
+                const uint32_t a0[4] = {k0.x0, k1.x0, k0.y0, k1.y0}, a1[4] = {k0.x1, k1.x1, k0.y1, k1.y1};
+                mma_first(acc, a0, qb[2 * b][0], qb[2 * b][1]);
+                mma_f16f32(acc, a1, qb[2 * b + 1][0], qb[2 * b + 1][1]);
+#pragma unroll
+                for (int r = 0; r < 2; r++) {
+                    const float scale = half_of(d[r][b >> 1], b & 1);
+#pragma unroll
+                    for (int x = 0; x < 2; x++) s[t][r][x] = fmaf(acc[2 * r + x], scale, s[t][r][x]);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 2; r++)
+#pragma unroll
+                for (int x = 0; x < 2; x++) s[t][r][x] += __shfl_xor_sync(0xffffffffu, s[t][r][x], 2);
+        }
+        if (left < P4_TILE) {
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int r = 0; r < 2; r++)
+                    if (16 * t + position_of(g >> 1, g & 1, r) >= left) s[t][r][0] = s[t][r][1] = -INFINITY;
+        }
+        float mx[2];
+#pragma unroll
+        for (int x = 0; x < 2; x++) mx[x] = fmaxf(fmaxf(s[0][0][x], s[0][1][x]), fmaxf(s[1][0][x], s[1][1][x]));
+        if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
+            float alpha[2];
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+#pragma unroll
+                for (int y = 4; y < 32; y <<= 1) mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], y));
+                const float mn = fmaxf(m[x], mx[x]);
+                alpha[x] = m[x] == -INFINITY ? 0.0f : ex2((m[x] - mn) * P4_N * unit[x]);
+                l[x] *= alpha[x];
+                m[x] = mn;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) mins[e] *= alpha[e & 1];
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[b][0][e] *= alpha[e & 1], o[b][1][e] *= alpha[e & 1];
+        }
+        float p[2][2][2];
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            const float sub = m[x] == -INFINITY ? 0.0f : -m[x] * P4_N;  // P4_TOP is added last: a large score would swallow it
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int r = 0; r < 2; r++) {
+                    p[t][r][x] = ex2(fmaf(fmaf(s[t][r][x], P4_N, sub), unit[x], P4_TOP));
+                    l[x] += p[t][r][x];
+                }
+        }
+        // ---- weighted values ----
+        float by;
+        if (v.template raise<D>(sv, &by)) {
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[b][0][e] *= by, o[b][1][e] *= by;
+        }
+        const float rest = c < 2 ? 0.0f : -1.0f;
+        auto part = [&](float x, float y) {  // both heads' f16 values or what these leave, turned
+            const uint32_t h = h2_bits(__floats2half2_rn(x, y));
+            return turned(h2_bits(__floats2half2_rn(fmaf(half_of(h, 0), rest, x), fmaf(half_of(h, 1), rest, y))));
+        };
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const uint32_t tile = sv + t * L::TILE;
+            {  // minima: row x of the scales and minima, of which those from NB on count
+                uint32_t rows[4] = {0, 0, 0, 0};
+                params_turned<D>(tile, rows[0], rows[2]);
+                mma_f16f32(mins, rows, part(p[t][0][0], p[t][0][1]), part(p[t][1][0], p[t][1][1]));
+            }
+            uint32_t w[2][2][NB / 2], d[2][NB / 2];
+            float pv[2][2];
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                scales_of<D>(tile, position_of(g >> 1, g & 1, n), d[n]);
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    dims_of_v<D>(tile, position_of(c, e, n), w[n][e]);
+                    pv[n][e] = p[t][n][e] * v.per;
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                uint32_t wb[2], z[2];
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    const float scale = half_of(d[n][b >> 1], b & 1);
+                    wb[n] = part(pv[n][0] * scale, pv[n][1] * scale);
+                    z[n] = __byte_perm(w[n][0][b >> 1], w[n][1][b >> 1], b & 1 ? 0x7632 : 0x5410);  // dims 32 b + 4 g .. + 3 of two positions
+                }
+                const Nibbles v0(z[0]), v1(z[1]);
+                const uint32_t r0[4] = {v0.x0, v0.y0, v1.x0, v1.y0}, r1[4] = {v0.x1, v0.y1, v1.x1, v1.y1};
+                mma_f16f32(o[b][0], r0, wb[0], wb[1]);
+                mma_f16f32(o[b][1], r1, wb[0], wb[1]);
+            }
+        }
+    }
+    CFI_DEV void finish(float* meet, int row) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+        const float back = ex2(v.top) * P4_N;
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+#pragma unroll
+            for (int y = 4; y < 32; y <<= 1) l[x] += __shfl_xor_sync(0xffffffffu, l[x], y);
+            mins[x] += __shfl_xor_sync(0xffffffffu, mins[x], 2);
+        }
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const float low = __shfl_sync(0xffffffffu, mins[e], 4 * (NB + b) + c);  // row NB + b
+                float f[4];
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const float u = o[b][x][e] + __shfl_xor_sync(0xffffffffu, o[b][x][e], 2),
+                                w = o[b][x][2 + e] + __shfl_xor_sync(0xffffffffu, o[b][x][2 + e], 2);
+                    f[2 * x] = fmaf(u, back, low);
+                    f[2 * x + 1] = fmaf(w - u, back / 16.0f, low);
+                }
+                if (c < 2) *reinterpret_cast<float4*>(meet + (2 * c + e) * row + 32 * b + 4 * g) = make_float4(f[0], f[1], f[2], f[3]);
+            }
+        if (lane < 2) {
+#pragma unroll
+            for (int x = 0; x < 2; x++) *reinterpret_cast<float2*>(meet + (2 * c + x) * row + D) = make_float2(m[x] * P4_N * unit[x], l[x]);
+        }
+    }
+};
+
+template <int D, int W, bool FEW>
 __global__ void __launch_bounds__(W * 32, (P4Shape<D, W>::CTAS)) paged_attn_q4(const PaArgs a) {
     using S = P4Shape<D, W>;
     using L = Q41<D>;
-    constexpr int NB = D / 32, NT = D / 8, KK = D / 16;
+    constexpr int NB = D / 32;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int s_last[2];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, c = lane & 3;
     const int page_size = 1 << a.page_shift, hc = a.n_kv_head * a.chunks;
     pdl_launch_dependents();
     pdl_wait();
@@ -118,7 +609,6 @@ __global__ void __launch_bounds__(W * 32, (P4Shape<D, W>::CTAS)) paged_attn_q4(c
     at = begin;
 
     const uint32_t ring = smem_u32(smem) + warp * S::RING;
-    const int row_k = position_of(g >> 1, g & 1, 0);  // this lane's row of K among eight
     PaShared shared[2];  // of the pairs that it goes on with, and leaves unfinished
     while (at < end) {
         // ---- one (sequence, kv head, chunk): its tiles [t0, t1) of n_tiles ----
@@ -148,13 +638,15 @@ __global__ void __launch_bounds__(W * 32, (P4Shape<D, W>::CTAS)) paged_attn_q4(c
         int id0 = load_id(0, 0), id1 = load_id(0, 1);
 
         // the queries: loaded here, converted when the first tiles are on their way.  Dims 32 b + 8 c .. + 7
+        using Heads = typename std::conditional<FEW, FewHeads<D>, ManyHeads<D>>::type;
+        const int h = Heads::head();
         float qv[NB][8];
 #pragma unroll
         for (int b = 0; b < NB; b++) {
 #pragma unroll
             for (int e = 0; e < 8; e++) qv[b][e] = 0.0f;
-            if (g < nh) {
-                const long long o = seq * a.q_stride + (long long)(head0 + g) * D + 32 * b + 8 * c;
+            if (h < nh) {
+                const long long o = seq * a.q_stride + (long long)(head0 + h) * D + 32 * b + 8 * c;
                 if (a.q_f16) {
                     const uint4 w = *reinterpret_cast<const uint4*>(a.q + o * 2);
                     qv[b][0] = __uint_as_float(w.x), qv[b][1] = __uint_as_float(w.y), qv[b][2] = __uint_as_float(w.z), qv[b][3] = __uint_as_float(w.w);
@@ -166,49 +658,51 @@ __global__ void __launch_bounds__(W * 32, (P4Shape<D, W>::CTAS)) paged_attn_q4(c
             }
         }
 
+        const uint32_t page_bytes = a.n_kv_head * (uint32_t)paged_region_bytes<D, CACHE_Q4_1>(page_size);
+        const uint8_t *k_lane = a.k + kvh * paged_region_bytes<D, CACHE_Q4_1>(page_size) + lane * 16, *v_lane = k_lane + (a.v - a.k);
         auto fetch = [&](int i) {  // tile i of this warp into its stage
             if (i < mine) {
                 const int p0 = (t0 + warp + i * W) * P4_TILE, left = len - p0;
-                const int page0 = __shfl_sync(0xffffffffu, id0, i & 31), page1 = __shfl_sync(0xffffffffu, id1, i & 31);
-                const uint32_t st = ring + (i % S::STAGES) * S::STAGE;
-                auto tile_at = [&](int page, int p) {
-                    return ((long long)page * a.n_kv_head + kvh) * paged_region_bytes<D, CACHE_Q4_1>(page_size) + L::tile_at(p & (page_size - 1));
-                };
-                const long long src0 = tile_at(page0, p0), src1 = tile_at(page1, p0 + Q41_TILE);
-                const int two = left > Q41_TILE ? 16 : 0;  // is there a second half?
-#pragma unroll
-                for (int kv = 0; kv < 2; kv++) {
-                    const uint8_t* pool = kv ? a.v : a.k;
-                    const uint32_t dst = st + kv * 2 * S::TILE;
+                const uint32_t page0 = __shfl_sync(0xffffffffu, id0, i & 31), page1 = __shfl_sync(0xffffffffu, id1, i & 31);
+                const uint32_t st = ring + (i % S::STAGES) * S::STAGE + lane * 16;
+                const uint64_t o0 = (uint64_t)page0 * page_bytes + L::tile_at(p0 & (page_size - 1)),
+                               o1 = (uint64_t)page1 * page_bytes + L::tile_at((p0 + Q41_TILE) & (page_size - 1));
+                // Scales and minima: a chunk a lane, of 4 CH for the four tiles.  Rows past the length get zeros, so that what a page holds
+                // there never matters.
+                constexpr int CH = Q41_TILE * L::PARAM_ROW / 16, ROWS = Q41_TILE / CH, N = 32 / CH;  // of a tile; rows of a chunk; tiles a warp
+                const int n = lane / CH, half = n & 1;
+                const uint64_t op = half ? o1 : o0;
+                const uint32_t to = st + n * (S::TILE - 16 * CH) + L::NIBBLES;  // st counts all lanes before
+                const uint8_t* from = (N == 4 && n >= 2 ? v_lane : k_lane) + op + (L::NIBBLES - 16 * CH * n);
+                if (left >= P4_TILE) {
 #pragma unroll
                     for (int e = 0; e < L::NIBBLES / 512; e++) {
-                        const int o = (e * 32 + lane) * 16;
-                        cp16n(dst + o, pool + src0 + o, 16);
-                        cp16n(dst + S::TILE + o, pool + src1 + o, two);
+                        cp_async16_cg(st + e * 512, k_lane + o0 + e * 512);
+                        cp_async16_cg(st + S::TILE + e * 512, k_lane + o1 + e * 512);
+                        cp_async16_cg(st + 2 * S::TILE + e * 512, v_lane + o0 + e * 512);
+                        cp_async16_cg(st + 3 * S::TILE + e * 512, v_lane + o1 + e * 512);
                     }
-                }
-                // scales and minima, a chunk a lane; rows past the length get zeros, so that what a page holds there never matters
-                constexpr int CH = Q41_TILE * L::PARAM_ROW / 16, ROWS = Q41_TILE / CH;  // chunks of a tile, rows of a chunk
+                    cp_async16_cg(to, from);
+                    if (N == 2) cp_async16_cg(to + 2 * S::TILE, from + (a.v - a.k));
+                } else {
+                    const int two = left > Q41_TILE ? 16 : 0;  // is there a second half?
 #pragma unroll
-                for (int x = 0; x < 4 * CH / 32; x++) {
-                    const int n = (x * 32 + lane) / CH, ch = lane % CH, half = n & 1, kv = n >> 1;  // n: tiles as they lie in the stage
-                    const int bytes = min(max((left - half * Q41_TILE - ch * ROWS) * L::PARAM_ROW, 0), 16);
-                    cp16n(st + n * S::TILE + L::NIBBLES + ch * 16, (kv ? a.v : a.k) + (half ? src1 : src0) + L::NIBBLES + ch * 16, bytes);
+                    for (int e = 0; e < L::NIBBLES / 512; e++) {
+                        cp16n(st + e * 512, k_lane + o0 + e * 512, 16);
+                        cp16n(st + S::TILE + e * 512, k_lane + o1 + e * 512, two);
+                        cp16n(st + 2 * S::TILE + e * 512, v_lane + o0 + e * 512, 16);
+                        cp16n(st + 3 * S::TILE + e * 512, v_lane + o1 + e * 512, two);
+                    }
+                    const int bytes = min(max((left - half * Q41_TILE - lane % CH * ROWS) * L::PARAM_ROW, 0), 16);
+                    cp16n(to, from, bytes);
+                    if (N == 2) cp16n(to + 2 * S::TILE, from + (a.v - a.k), bytes);
                 }
             }
             cp_async_commit();
         };
 
-        // V's scales have been below 2^top_v; o has 2^-top_v in it, and 2^-24 (odd dims 2^-20)
-        float o[NT][4], mins[4], m = -INFINITY, top_v = P4_LEAST_V, per_top = ex2(-P4_LEAST_V);
-        f2 l = 0;
-        __half2 limit_v = __float2half2_rn(ex2(top_v));
-#pragma unroll
-        for (int e = 0; e < 4; e++) mins[e] = 0.0f;
-#pragma unroll
-        for (int j = 0; j < NT; j++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) o[j][e] = 0.0f;
+        Heads heads;
+        heads.begin();
 #pragma unroll
         for (int i = 0; i < S::STAGES - 1; i++) fetch(i);
         if (a.q_f16) {
@@ -222,42 +716,10 @@ __global__ void __launch_bounds__(W * 32, (P4Shape<D, W>::CTAS)) paged_attn_q4(c
                     qv[b][2 * e + 1] = f.y;
                 }
         }
-        float largest = 0.0f;  // a NaN is passed over
-#pragma unroll
-        for (int b = 0; b < NB; b++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                qv[b][e] *= a.scale_log2;
-                largest = fmaxf(largest, fabsf(qv[b][e]));
-            }
-        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-        // 2^(its exponent - 14) and the other way round, both normal: below 2^-111 the largest stays below 2^14
-        const uint32_t exponent = max(__float_as_uint(largest) >> 23, 15u);
-        const float unit = __uint_as_float((exponent - 14) << 23), per_unit = __uint_as_float((268 - exponent) << 23);
-        uint32_t qf[KK][4], qs[2];  // in log2 units over `unit`, split; the sums of the blocks, over 2^6
-        float sums[NB];
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
-            sums[b] = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                qv[b][e] *= per_unit;
-                sums[b] += qv[b][e];
-            }
-            sums[b] += __shfl_xor_sync(0xffffffffu, sums[b], 1);
-            sums[b] += __shfl_xor_sync(0xffffffffu, sums[b], 2);
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                split(qv[b][2 * k], qv[b][2 * k + 4], &qf[2 * b + k][0], &qf[2 * b + k][1]);
-                split(qv[b][2 * k + 1] * 0.0625f, qv[b][2 * k + 5] * 0.0625f, &qf[2 * b + k][2], &qf[2 * b + k][3]);
-            }
-        }
         {
-            // a row of scales and minima is 2 NB f16 numbers: the lane's pair of those are minima of blocks x and x + 1
-            const int x = 2 * c - NB;
-            const float s0 = x == 0 ? sums[0] : NB == 4 && x == 2 ? sums[NB - 2] : 0.0f, s1 = x == 0 ? sums[1] : NB == 4 && x == 2 ? sums[NB - 1] : 0.0f;
-            split(s0 * 0.015625f, s1 * 0.015625f, &qs[0], &qs[1]);
+            Queries<D> q;
+            q.convert(qv, a.scale_log2);
+            heads.queries(q);
         }
         for (int i = 0; i < mine; i++) {
             if ((i + S::STAGES - 1) % 32 == 0) {
@@ -267,184 +729,15 @@ __global__ void __launch_bounds__(W * 32, (P4Shape<D, W>::CTAS)) paged_attn_q4(c
             fetch(i + S::STAGES - 1);
             cp_async_wait<S::STAGES - 1>();
             __syncwarp();
-            const uint32_t sk = ring + (i % S::STAGES) * S::STAGE, sv = sk + 2 * S::TILE;
-            // ---- scores, over 2^24 `unit`, of head g: columns 2c, 2c+1 of four eights ----
-            f2 s[4];
-#pragma unroll
-            for (int n = 0; n < 4; n++) {
-                const uint32_t tile = sk + (n >> 1) * S::TILE;
-                const int row = row_k + 8 * (n & 1);
-                {
-                    float acc[4];
-                    const uint32_t sums2[4] = {qs[0], qs[1], 0, 0};
-                    mma_first(acc, sums2, lds32(tile + L::NIBBLES + row * L::PARAM_ROW + 4 * (c & (NB - 1))), 0);
-                    s[n] = mul2(add2(pair2(acc[0], acc[1]), pair2(acc[2], acc[3])), pair2(64.0f / P4_N, 64.0f / P4_N));
-                }
-                uint32_t w[NB], d[2][NB / 2];  // eight dims of each block of the lane's row; scales of columns 2c and 2c+1
-                if (D == 128) {
-                    const uint4 x = lds128(tile + row * L::ROW + c * 16);
-                    w[0] = x.x, w[1] = x.y, w[NB - 2] = x.z, w[NB - 1] = x.w;
-                } else {
-                    const uint2 x = lds64(tile + row * L::ROW + c * 8);
-                    w[0] = x.x, w[1] = x.y;
-                }
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const uint32_t p = tile + L::NIBBLES + position_of(c, e, n & 1) * L::PARAM_ROW;
-                    if (D == 128) {
-                        const uint2 x = lds64(p);
-                        d[e][0] = x.x, d[e][NB / 2 - 1] = x.y;
-                    } else {
-                        d[e][0] = lds32(p);
-                    }
-                }
-#pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    float acc[4];
-                    mma_first(acc, qf[2 * b], low_nibbles(w[b]), high_nibbles(w[b]));
-                    mma_f16f32(acc, qf[2 * b + 1], low_nibbles(w[b] >> 8), high_nibbles(w[b] >> 8));
-                    s[n] = fma2(add2(pair2(acc[0], acc[1]), pair2(acc[2], acc[3])),
-                                pair2(half_of(d[0][b >> 1], b & 1), half_of(d[1][b >> 1], b & 1)), s[n]);
-                }
-            }
-            const int left = len - (t0 + warp + i * W) * P4_TILE;
-            if (left < P4_TILE) {
-#pragma unroll
-                for (int n = 0; n < 4; n++) {
-                    float2 x = both(s[n]);
-                    if (16 * (n >> 1) + position_of(c, 0, n & 1) >= left) x.x = -INFINITY;
-                    if (16 * (n >> 1) + position_of(c, 1, n & 1) >= left) x.y = -INFINITY;
-                    s[n] = pair2(x.x, x.y);
-                }
-            }
-            float mx = -INFINITY;
-#pragma unroll
-            for (int n = 0; n < 4; n++) mx = fmaxf(mx, fmaxf(both(s[n]).x, both(s[n]).y));
-            if (__any_sync(0xffffffffu, mx > m)) {
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                const float mn = fmaxf(m, mx), alpha = m == -INFINITY ? 0.0f : ex2((m - mn) * P4_N * unit);
-                const f2 alpha2 = pair2(alpha, alpha);
-                l = mul2(l, alpha2);
-#pragma unroll
-                for (int e = 0; e < 4; e++) mins[e] *= alpha;
-#pragma unroll
-                for (int j = 0; j < NT; j++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) o[j][e] *= alpha;
-                m = mn;
-            }
-            const float sub = m == -INFINITY ? 0.0f : -m * P4_N, rise = P4_TOP;  // added last: a large score would swallow it
-            f2 p[4];
-#pragma unroll
-            for (int n = 0; n < 4; n++) {
-                const float2 x = both(fma2(fma2(s[n], pair2(P4_N, P4_N), pair2(sub, sub)), pair2(unit, unit), pair2(rise, rise)));
-                p[n] = pair2(ex2(x.x), ex2(x.y));
-                l = add2(l, p[n]);
-            }
-            // ---- weighted values ----
-            {
-                // a lane looks at some of the tile's scales
-                __half2 d = __float2half2_rn(0.0f);
-#pragma unroll
-                for (int x = 0; x < NB / 2; x++) {
-                    const uint32_t row = sv + (lane >> 4) * S::TILE + L::NIBBLES + (lane & 15) * L::PARAM_ROW;
-                    d = __hmax2_nan(d, abs_h2(lds32(row + 4 * x)));
-                }
-                if (__any_sync(0xffffffffu, !__hblt2(d, limit_v))) {
-                    // the exponent of the largest, cut where that is an infinity or a NaN
-                    const uint32_t ex = __float_as_uint(fmaxf(__low2float(d), __high2float(d))) >> 23;
-                    const float grown = fmaxf(top_v, fminf((float)__reduce_max_sync(0xffffffffu, ex) - 126.0f, P4_MOST_V));
-                    const float f = ex2(top_v - grown);
-#pragma unroll
-                    for (int j = 0; j < NT; j++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) o[j][e] *= f;
-                    per_top = ex2(-grown);
-                    top_v = grown;
-                    limit_v = __float2half2_rn(ex2(grown));
-                }
-            }
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const uint32_t tile = sv + t * S::TILE;
-                {  // minima: column x of a row's scales and minima, of which those from NB on count
-                    uint32_t pf[4], b0, b1;
-#pragma unroll
-                    for (int n = 0; n < 2; n++) split(both(p[2 * t + n]).x, both(p[2 * t + n]).y, &pf[2 * n], &pf[2 * n + 1]);
-                    if (D == 128) {
-                        ldsm_x2_trans(tile + L::NIBBLES + position_of(lane >> 1 & 3, lane & 1, lane >> 3 & 1) * L::PARAM_ROW, b0, b1);
-                    } else {  // rows of four numbers: column g & 3 of the lane's four positions
-                        uint32_t x[4];
-#pragma unroll
-                        for (int e = 0; e < 4; e++) x[e] = lds16(tile + L::NIBBLES + position_of(c, e & 1, e >> 1) * L::PARAM_ROW + 2 * (g & 3));
-                        b0 = x[0] | x[1] << 16;
-                        b1 = x[2] | x[3] << 16;
-                    }
-                    mma_f16f32(mins, pf, b0, b1);
-                }
-                uint32_t w[2][2][NB / 2], d[2][2][NB / 2];  // of column e of eight n: the lane's dims; scales
-#pragma unroll
-                for (int n = 0; n < 2; n++)
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const int row = position_of(c, e, n);
-                        const uint32_t q = tile + row * L::ROW + L::v_group(row, g) * (D / 16), r = tile + L::NIBBLES + row * L::PARAM_ROW;
-                        if (D == 128) {
-                            const uint2 x = lds64(q), y = lds64(r);
-                            w[n][e][0] = x.x, w[n][e][NB / 2 - 1] = x.y;
-                            d[n][e][0] = y.x, d[n][e][NB / 2 - 1] = y.y;
-                        } else {
-                            w[n][e][0] = lds32(q);
-                            d[n][e][0] = lds32(r);
-                        }
-                    }
-                f2 pv[2];
-#pragma unroll
-                for (int n = 0; n < 2; n++) pv[n] = mul2(p[2 * t + n], pair2(per_top, per_top));
-#pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    uint32_t pf[4], bw[2][4];
-#pragma unroll
-                    for (int n = 0; n < 2; n++) {
-                        const float2 x = both(mul2(pv[n], pair2(half_of(d[n][0][b >> 1], b & 1), half_of(d[n][1][b >> 1], b & 1))));
-                        split(x.x, x.y, &pf[2 * n], &pf[2 * n + 1]);
-                        // dims 32 b + 4 g .. + 3 of two positions: column g of MMA e is dim 32 b + 4 g + e
-                        const uint32_t z = __byte_perm(w[n][0][b >> 1], w[n][1][b >> 1], b & 1 ? 0x7632 : 0x5410);
-                        bw[n][0] = low_nibbles(z);
-                        bw[n][1] = high_nibbles(z);
-                        bw[n][2] = low_nibbles(z >> 8);
-                        bw[n][3] = high_nibbles(z >> 8);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; e++) mma_f16f32(o[4 * b + e], pf, bw[0][e], bw[1][e]);
-                }
-            }
+            const uint32_t st = ring + (i % S::STAGES) * S::STAGE;
+            heads.tile(st, st + 2 * S::TILE, len - (t0 + warp + i * W) * P4_TILE);
             __syncwarp();  // the stage is free
         }
         // ---- the warps meet: [warp][head]: D values, maximum, sum ----
         cp_async_wait<0>();
-        const float back = ex2(top_v) * P4_N;  // each warp has had scales of its own
-        float sum = both(l).x + both(l).y, low[NB];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-#pragma unroll
-        for (int b = 0; b < NB; b++)  // columns 2 c and 2 c + 1 of the minima are this lane's
-            low[b] = __shfl_sync(0xffffffffu, mins[b & 1] + mins[2 + (b & 1)], (lane & ~3) + (NB + b) / 2);
         __syncthreads();  // every warp is done with its stages
         float* meet = reinterpret_cast<float*>(smem);
-        float* mine_o = meet + warp * S::MEET + g * S::MEET_ROW;
-#pragma unroll
-        for (int b = 0; b < NB; b++)
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                float f[4];
-#pragma unroll
-                for (int x = 0; x < 4; x++)
-                    f[x] = fmaf(o[4 * b + x][e] + o[4 * b + x][e + 2], x & 1 ? back / 16.0f : back, low[b]);
-                *reinterpret_cast<float4*>(mine_o + 32 * b + 8 * c + 4 * e) = make_float4(f[0], f[1], f[2], f[3]);
-            }
-        if (c == 0) *reinterpret_cast<float2*>(mine_o + D) = make_float2(m * P4_N * unit, sum);
+        heads.finish(meet + warp * S::MEET, S::MEET_ROW);
         __syncthreads();
         const bool done = t0 == 0 && t1 == n_tiles;
         if (!done) {
@@ -483,10 +776,10 @@ __global__ void __launch_bounds__(W * 32, (P4Shape<D, W>::CTAS)) paged_attn_q4(c
     if (!a.whole) join_shared<S, D, W * 32>(a, shared, s_last);
 }
 
-template <int D, int W> int launch(PaArgs& a, long long pairs, long long most_units, cudaStream_t stream) {
+template <int D, int W, bool FEW> int launch(PaArgs& a, long long pairs, long long most_units, cudaStream_t stream) {
     using S = P4Shape<D, W>;
     static CfiPerDeviceOnce once;
-    cfi_once_per_device(once, [] { cudaFuncSetAttribute(paged_attn_q4<D, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM); });
+    cfi_once_per_device(once, [] { cudaFuncSetAttribute(paged_attn_q4<D, W, FEW>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM); });
     long long grid = pairs;
     if (!a.whole) {
         // no CTA has fewer units than this
@@ -509,7 +802,7 @@ template <int D, int W> int launch(PaArgs& a, long long pairs, long long most_un
     at[0].val.programmaticStreamSerializationAllowed = 1;
     lc.attrs = at;
     lc.numAttrs = (ep && strcmp(ep, "0") == 0) ? 0 : 1;
-    return (int)cudaLaunchKernelEx(&lc, paged_attn_q4<D, W>, (const PaArgs)a);
+    return (int)cudaLaunchKernelEx(&lc, paged_attn_q4<D, W, FEW>, (const PaArgs)a);
 }
 
 }  // namespace
@@ -520,6 +813,15 @@ int cfi_paged_attention_q4_1(PaArgs& a, int head_dim, long long pairs, cudaStrea
     const int sms = cfi_sm_count();
     const int w = pairs <= sms ? (positions <= (2 * pairs > sms ? 1536 : 768) ? 8 : 0) : positions <= 768 ? 4 : 0;
     a.whole = w > 0;
-    if (w == 8) return head_dim == 64 ? launch<64, 8>(a, pairs, most_units, stream) : launch<128, 8>(a, pairs, most_units, stream);
-    return head_dim == 64 ? launch<64, PA_WARPS>(a, pairs, most_units, stream) : launch<128, PA_WARPS>(a, pairs, most_units, stream);
+    const int variant = (head_dim == 128) * 4 + (w == 8) * 2 + (a.group <= 4);
+    switch (variant) {
+        case 0: return launch<64, PA_WARPS, false>(a, pairs, most_units, stream);
+        case 1: return launch<64, PA_WARPS, true>(a, pairs, most_units, stream);
+        case 2: return launch<64, 8, false>(a, pairs, most_units, stream);
+        case 3: return launch<64, 8, true>(a, pairs, most_units, stream);
+        case 4: return launch<128, PA_WARPS, false>(a, pairs, most_units, stream);
+        case 5: return launch<128, PA_WARPS, true>(a, pairs, most_units, stream);
+        case 6: return launch<128, 8, false>(a, pairs, most_units, stream);
+        default: return launch<128, 8, true>(a, pairs, most_units, stream);
+    }
 }
