@@ -36,7 +36,7 @@ using namespace sm100;
 constexpr int P4_TILE = 32;         // positions
 constexpr int P4_FIXED = 3;         // what beginning and ending a pair costs, in tiles
 constexpr float P4_TOP = 15.0f;     // log2 of the largest weight as it is split: f16 ends at 65504
-constexpr float P4_LEAST_V = -23.0f, P4_MOST_V = 16.0f;  // f16 scales are below 2^these
+constexpr float P4_LEAST_V = -15.0f, P4_MOST_V = 16.0f;  // f16 has the inverse of 2^the first; scales are below 2^the second
 constexpr float P4_N = 16777216.0f;  // 2^24: nibbles are whole numbers times its inverse
 using Cut = PaCut<P4_TILE, P4_FIXED>;
 
@@ -124,28 +124,41 @@ struct Nibbles {
 // column 2 c + e of the n-th eight scores
 CFI_DEV int position_of(int c, int e, int n) { return 8 * n + 4 * e + (c ^ (3 * e)); }
 
-// The largest of V's scales so far: they have been below 2^top; the weights times scales are divided by it.
+// The largest of V's scales so far: they have been below 2^top, and what the weights are multiplied by is divided by it.
 struct ScalesTop {
-    float top = P4_LEAST_V, per = 8388608.0f;  // per: 2^-top
-    // Looks at a tile's scales, some a lane; where one passes `top`, raises it and gives what the sums so far have to be multiplied by.
-    template <int D> CFI_DEV bool raise(uint32_t sv, float* by) {
-        const int lane = threadIdx.x & 31;
-        __half2 d = __float2half2_rn(0.0f);
-#pragma unroll
-        for (int x = 0; x < D / 64; x++)
-            d = __hmax2_nan(d, abs_h2(lds32(sv + (lane >> 4) * Q41<D>::TILE + Q41<D>::NIBBLES + (lane & 15) * Q41<D>::PARAM_ROW + 4 * x)));
-        if (!__any_sync(0xffffffffu, !__hblt2(d, limit))) return false;
-        // the exponent of the largest, cut where that is an infinity or a NaN
-        const uint32_t ex = __float_as_uint(fmaxf(__low2float(d), __high2float(d))) >> 23;
-        const float grown = fmaxf(top, fminf((float)__reduce_max_sync(0xffffffffu, ex) - 126.0f, P4_MOST_V));
-        *by = ex2(top - grown);
-        top = grown;
-        per = ex2(-grown);
-        limit = __float2half2_rn(ex2(grown));
-        return true;
+    float top, per;  // per: 2^-top
+    __half2 limit, least;  // 2^top; the least scale but 0 that divided by it is a normal f16 number
+    CFI_DEV void set(float t) {
+        top = t;
+        per = ex2(-t);
+        limit = __float2half2_rn(ex2(t));
+        least = __float2half2_rn(ex2(t - 14.0f));
     }
-    __half2 limit = __float2half2_rn(1.1920929e-7f);
+    // Looks at a tile's scales, some a lane.  Where one passes `top`, raises it: `by` is what the sums so far have to be multiplied by, or
+    // 1.  True where a scale is so far below the largest that f16 would not hold it over 2^top.
+    template <int D> CFI_DEV bool look(uint32_t sv, float* by) {
+        const int lane = threadIdx.x & 31;
+        __half2 d[D / 64], most = __float2half2_rn(0.0f);
+#pragma unroll
+        for (int x = 0; x < D / 64; x++) {
+            d[x] = abs_h2(lds32(sv + (lane >> 4) * Q41<D>::TILE + Q41<D>::NIBBLES + (lane & 15) * Q41<D>::PARAM_ROW + 4 * x));
+            most = __hmax2_nan(most, d[x]);
+        }
+        *by = 1.0f;
+        if (__any_sync(0xffffffffu, !__hblt2(most, limit))) {
+            // the exponent of the largest, cut where that is an infinity or a NaN
+            const uint32_t ex = __float_as_uint(fmaxf(__low2float(most), __high2float(most))) >> 23;
+            const float old = top;
+            set(fmaxf(top, fminf((float)__reduce_max_sync(0xffffffffu, ex) - 126.0f, P4_MOST_V)));
+            *by = ex2(old - top);
+        }
+        uint32_t small = 0;
+#pragma unroll
+        for (int x = 0; x < D / 64; x++) small |= __hlt2_mask(d[x], least) & __hne2_mask(d[x], __float2half2_rn(0.0f));
+        return __any_sync(0xffffffffu, small != 0);
+    }
 };
+CFI_DEV __half2 as_h2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
 
 // Scales of two rows of blocks 0, 1 and 2, 3
 template <int D> CFI_DEV void scales_of(uint32_t tile, int row, uint32_t (&d)[D / 64]) {
@@ -252,6 +265,7 @@ template <int D> struct ManyHeads {
     CFI_DEV void begin() {
         m = -INFINITY;
         l = 0;
+        v.set(P4_LEAST_V);
 #pragma unroll
         for (int e = 0; e < 4; e++) mins[e] = 0.0f;
 #pragma unroll
@@ -327,39 +341,59 @@ template <int D> struct ManyHeads {
         }
         // ---- weighted values: A is V with dims as rows, B the weights and then what f16 left of them ----
         float by;
-        if (v.template raise<D>(sv, &by)) {
+        const bool wide = v.template look<D>(sv, &by);
+        if (by != 1.0f) {
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) o[b][0][e] *= by, o[b][1][e] *= by;
         }
+        if (wide)
+            values<true>(sv, p);
+        else
+            values<false>(sv, p);
+    }
+    // Adds the weighted values of a tile.  The weights p, f16 values and the rest, are multiplied by the scales over 2^top in f16: h = hi d
+    // rounded, and what that left (exact in one fused product) with lo d.  WIDE: in 32 bits, where some of these scales are not f16 numbers.
+    template <bool WIDE> CFI_DEV void values(uint32_t sv, const f2 (&p)[4]) {
+        using L = Q41<D>;
+        const int c = threadIdx.x & 3;
 #pragma unroll
         for (int t = 0; t < 2; t++) {
             const uint32_t tile = sv + t * L::TILE;
-            {  // minima: column x of a row's scales and minima, of which those from NB on count
-                uint32_t pf[4], b0, b1;
+            uint32_t pf[4], b0, b1;
 #pragma unroll
-                for (int n = 0; n < 2; n++) split2(p[2 * t + n], &pf[2 * n], &pf[2 * n + 1]);
-                params_turned<D>(tile, b0, b1);
-                mma_f16f32(mins, pf, b0, b1);
-            }
+            for (int n = 0; n < 2; n++) split2(p[2 * t + n], &pf[2 * n], &pf[2 * n + 1]);
+            // minima: column x of a row's scales and minima, of which those from NB on count
+            params_turned<D>(tile, b0, b1);
+            mma_f16f32(mins, pf, b0, b1);
             uint32_t w[2][2][NB / 2], d[2][2][NB / 2];  // of column 2 c + e of eight n
-            f2 pv[2];
+            const __half2 per = __float2half2_rn(v.per);
 #pragma unroll
-            for (int n = 0; n < 2; n++) {
-                pv[n] = mul2(p[2 * t + n], pair2(v.per, v.per));
+            for (int n = 0; n < 2; n++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     dims_of_v<D>(tile, position_of(c, e, n), w[n][e]);
                     scales_of<D>(tile, position_of(c, e, n), d[n][e]);
+                    if (!WIDE) {
+#pragma unroll
+                        for (int x = 0; x < NB / 2; x++) d[n][e][x] = h2_bits(__hmul2(as_h2(d[n][e][x]), per));
+                    }
                 }
-            }
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 uint32_t hi[2], lo[2], z[2];
 #pragma unroll
                 for (int n = 0; n < 2; n++) {
-                    split2(mul2(pv[n], pair2(half_of(d[n][0][b >> 1], b & 1), half_of(d[n][1][b >> 1], b & 1))), &hi[n], &lo[n]);
+                    if (WIDE) {
+                        const f2 scale = pair2(half_of(d[n][0][b >> 1], b & 1) * v.per, half_of(d[n][1][b >> 1], b & 1) * v.per);
+                        split2(mul2(p[2 * t + n], scale), &hi[n], &lo[n]);
+                    } else {
+                        const __half2 scale = as_h2(__byte_perm(d[n][0][b >> 1], d[n][1][b >> 1], b & 1 ? 0x7632 : 0x5410)),
+                                      h = __hmul2(as_h2(pf[2 * n]), scale);
+                        hi[n] = h2_bits(h);
+                        lo[n] = h2_bits(__hfma2(as_h2(pf[2 * n + 1]), scale, __hfma2(as_h2(pf[2 * n]), scale, __hneg2(h))));
+                    }
                     z[n] = __byte_perm(w[n][0][b >> 1], w[n][1][b >> 1], b & 1 ? 0x7632 : 0x5410);  // dims 32 b + 4 g .. + 3 of two positions
                 }
                 const Nibbles v0(z[0]), v1(z[1]);
@@ -410,6 +444,7 @@ template <int D> struct FewHeads {
     CFI_DEV void begin() {
         m[0] = m[1] = -INFINITY;
         l[0] = l[1] = 0.0f;
+        v.set(P4_LEAST_V);
 #pragma unroll
         for (int e = 0; e < 4; e++) mins[e] = 0.0f;
 #pragma unroll
@@ -509,43 +544,63 @@ template <int D> struct FewHeads {
         }
         // ---- weighted values ----
         float by;
-        if (v.template raise<D>(sv, &by)) {
+        const bool wide = v.template look<D>(sv, &by);
+        if (by != 1.0f) {
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) o[b][0][e] *= by, o[b][1][e] *= by;
         }
-        const float rest = c < 2 ? 0.0f : -1.0f;
-        auto part = [&](float x, float y) {  // both heads' f16 values or what these leave, turned
-            const uint32_t h = h2_bits(__floats2half2_rn(x, y));
-            return turned(h2_bits(__floats2half2_rn(fmaf(half_of(h, 0), rest, x), fmaf(half_of(h, 1), rest, y))));
-        };
+        if (wide)
+            values<true>(sv, p);
+        else
+            values<false>(sv, p);
+    }
+    // As above; a lane's two heads at positions g and g + 8.
+    template <bool WIDE> CFI_DEV void values(uint32_t sv, const float (&p)[2][2][2]) {
+        using L = Q41<D>;
+        const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+        const uint32_t rest = c < 2 ? 0u : 0xffffffffu;
 #pragma unroll
         for (int t = 0; t < 2; t++) {
             const uint32_t tile = sv + t * L::TILE;
-            {  // minima: row x of the scales and minima, of which those from NB on count
-                uint32_t rows[4] = {0, 0, 0, 0};
-                params_turned<D>(tile, rows[0], rows[2]);
-                mma_f16f32(mins, rows, part(p[t][0][0], p[t][0][1]), part(p[t][1][0], p[t][1][1]));
+            uint32_t hi[2], lo[2], pt[2], rows[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                split(p[t][n][0], p[t][n][1], &hi[n], &lo[n]);
+                pt[n] = turned(rest ? lo[n] : hi[n]);
             }
+            // minima: row x of the scales and minima, of which those from NB on count
+            params_turned<D>(tile, rows[0], rows[2]);
+            mma_f16f32(mins, rows, pt[0], pt[1]);
             uint32_t w[2][2][NB / 2], d[2][NB / 2];
-            float pv[2][2];
+            const __half2 per = __float2half2_rn(v.per);
 #pragma unroll
             for (int n = 0; n < 2; n++) {
                 scales_of<D>(tile, position_of(g >> 1, g & 1, n), d[n]);
+                if (!WIDE) {
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    dims_of_v<D>(tile, position_of(c, e, n), w[n][e]);
-                    pv[n][e] = p[t][n][e] * v.per;
+                    for (int x = 0; x < NB / 2; x++) d[n][x] = h2_bits(__hmul2(as_h2(d[n][x]), per));
                 }
+#pragma unroll
+                for (int e = 0; e < 2; e++) dims_of_v<D>(tile, position_of(c, e, n), w[n][e]);
             }
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 uint32_t wb[2], z[2];
 #pragma unroll
                 for (int n = 0; n < 2; n++) {
-                    const float scale = half_of(d[n][b >> 1], b & 1);
-                    wb[n] = part(pv[n][0] * scale, pv[n][1] * scale);
+                    if (WIDE) {
+                        const float scale = half_of(d[n][b >> 1], b & 1) * v.per;
+                        uint32_t h, l;
+                        split(p[t][n][0] * scale, p[t][n][1] * scale, &h, &l);
+                        wb[n] = turned(rest ? l : h);
+                    } else {
+                        // with the masked ones 0: hi d rounded; with them whole: what that leaves, and lo d
+                        const __half2 scale = b & 1 ? __high2half2(as_h2(d[n][b >> 1])) : __low2half2(as_h2(d[n][b >> 1]));
+                        const __half2 h = __hmul2(as_h2(hi[n] & rest), scale);
+                        wb[n] = turned(h2_bits(__hfma2(as_h2(lo[n] & rest), scale, __hfma2(as_h2(hi[n]), scale, __hneg2(h)))));
+                    }
                     z[n] = __byte_perm(w[n][0][b >> 1], w[n][1][b >> 1], b & 1 ? 0x7632 : 0x5410);  // dims 32 b + 4 g .. + 3 of two positions
                 }
                 const Nibbles v0(z[0]), v1(z[1]);

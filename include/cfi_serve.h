@@ -84,8 +84,9 @@ CFI_API int cfi_paged_kv_load(const CfiPagedCache *cache, const int64_t *slots, 
  * q and out: [sequence][head][dim], types 0 F32 or 1 F16, row strides in values (q's a multiple of
  * 8), 16-byte aligned; scale > 0.  Sums and maxima are in 32 bits and the operands of the products with
  * K and V carry 22 bits, a query's values no bits below 2^-38 (Q4_1: 2^-34) of their head's largest and a weight (Q8_0 and
- * Q4_1: times its scale of V) none below 2^-39 of the largest: the results are those of 32-bit arithmetic on the cached
- * values, as long as the scores are within the range of f32.  (Q4_1 sums q * scale and minimum apart: in 32 bits each.)
+ * Q4_1: times its scale of V) none below 2^-39 of the largest (Q4_1: scales below 2^-15 count as that): the results are those of
+ * 32-bit arithmetic on the cached values, as long as the scores are within the range of f32.  (Q4_1: of the scaled whole numbers and
+ * the minima, which are summed apart.)
  * A NaN makes NaN of what the formula takes it into and of nothing else: in q its head's outputs, in a row of K within
  * the length those of its kv head's query heads, in V the same dims of them.  An infinity there makes of these NaN
  * or what the formula gives.  Bounds: n_seq 65535, and n_seq * n_kv_head * ceil(n_head / n_kv_head / 8) *

@@ -353,3 +353,42 @@ def test_two_streams_and_a_captured_call():
     a[3][4].copy_(torch.tensor([100, 0, 9], dtype=torch.int32))  # other lengths, read when it runs
     graph.replay()
     a[1]([100, 0, 9])
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(6, 1, 128), (3, 1, 128), (14, 2, 64), (16, 16, 64)])
+def test_scales_far_apart(heads, kv, dim):
+    """Values whose scales lie 2^20 apart, in one tile, between positions and between blocks of a row, and a large one that comes late."""
+    def fill(k, v):
+        v[1::3] *= 2.0 ** -12
+        v[:, 32:64] *= 2.0 ** -10
+        v[-40] *= 2.0 ** 9
+
+    case(heads, kv, dim, 16, [900], fill=fill)[1]()
+
+    def constant(k, v):  # all scales 0 but one, subnormal ones
+        v[:] = 0.25
+        v[7, :32] = torch.arange(32, device=DEV) * 1e-6
+
+    case(heads, kv, dim, 32, [300], fill=constant)[1]()
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(6, 1, 128), (3, 1, 128), (14, 2, 64), (16, 16, 64)])
+def test_small_blocks_beside_large_ones(heads, kv, dim):
+    """A block whose scales are 2^-17 of the others' keeps its own precision: bits of weight times scale end at 2^-39 of the largest,
+    2^-22 of this block's, and a sum of a hundred of them that does not cancel is off by less than 2^-20 of the values.  (The block is
+    kv head 0's: its query heads are looked at.)"""
+    call, check, out, keep = case(heads, kv, dim, 16, [100], fill=lambda k, v: v[:, :32].mul_(2.0 ** -17).add_(2.0 ** -14), amp=0.2)
+    check()
+    V = rows_of(keep[1], 9, kv, 16, dim, True)
+    K = rows_of(keep[0], 9, kv, 16, dim, False)
+    table = keep[3][0].cpu().numpy()
+    pos = np.arange(100)
+    slots = table[pos // 16].astype(np.int64) * 16 + pos % 16
+    q = keep[2].double().cpu().numpy().reshape(heads, dim)
+    got = out.double().cpu().numpy().reshape(heads, dim)
+    for h in range(heads // kv):
+        s = K[slots, h * kv // heads] @ q[h] / math.sqrt(dim)
+        p = np.exp(s - s.max())
+        want = p @ V[slots, h * kv // heads][:, :32] / p.sum()
+        mags = float((np.abs(q[h]) @ (np.abs(K[slots, h * kv // heads]) * 3).T).max() / math.sqrt(dim))
+        assert (np.abs(got[h, :32] - want) <= (2 * EPS_S * mags + 3 * 2.0 ** -20) * 2.0 ** -14 * 2).all()
