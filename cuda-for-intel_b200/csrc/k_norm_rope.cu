@@ -10,6 +10,7 @@
 #include "sm100_ptx.cuh"
 #include "cfi_kernels.h"
 
+#include <algorithm>
 #include <math.h>
 #include <stdlib.h>
 #include <string.h>
@@ -17,6 +18,8 @@
 namespace {
 
 constexpr int NR_THREADS = 256, NR_RATES = 64;
+constexpr int NR_AT_ONCE = 2;  // heads whose loads are in flight together
+constexpr int NR_HEADS = 8, NR_MANY = 8;
 
 struct NrArgs {
     CfiNormRope r;
@@ -68,12 +71,34 @@ CFI_DEV void turn1(float& x, float& y, float c, float s) {
     x = t;
 }
 
-template <int D, bool IN_F16> __global__ void __launch_bounds__(NR_THREADS) norm_rope(const __grid_constant__ NrArgs a) {
+// Head u of a token's heads of q, k and v.
+template <int D> struct Head {
+    int kind, h, f16;  // kind: 0, 1, 2 of q, k, v
+    bool on;
+    const void* rows;
+    void* out;
+    long long stride, out_stride;
+    const float *bias, *norm;
+    CFI_DEV Head(const CfiNormRope& r, int u, bool live) {
+        const int nk = r.k ? r.n_kv_head : 0, nv = r.v ? r.n_kv_head : 0;
+        on = live && u < r.n_head + nk + nv;
+        kind = u < r.n_head ? 0 : u < r.n_head + nk ? 1 : 2;
+        h = kind == 0 ? u : kind == 1 ? u - r.n_head : u - r.n_head - nk;
+        rows = kind == 0 ? r.q : kind == 1 ? r.k : r.v;
+        stride = kind == 0 ? r.q_stride : kind == 1 ? r.k_stride : r.v_stride;
+        bias = kind == 0 ? r.q_bias : kind == 1 ? r.k_bias : r.v_bias;
+        norm = kind == 0 ? r.q_norm : kind == 1 ? r.k_norm : nullptr;
+        out = kind == 0 ? r.q_out : kind == 1 ? r.k_out : r.v_out;
+        out_stride = kind == 0 ? r.q_out_stride : kind == 1 ? r.k_out_stride : r.v_out_stride;
+        f16 = kind == 0 ? r.q_out_type : r.kv_out_type;
+    }
+};
+
+template <int D, bool IN_F16, int AT_ONCE> __global__ void __launch_bounds__(NR_THREADS) norm_rope(const __grid_constant__ NrArgs a) {
     constexpr int G = D / 8;  // lanes of a head
     __shared__ float4 s_row[NR_THREADS / G][2 * G];  // a row of k, where the cache wants eight dims in a lane
     const CfiNormRope& r = a.r;
     const int lane = threadIdx.x % G, group = threadIdx.x / G;
-    const int nk = r.k ? r.n_kv_head : 0, nv = r.v ? r.n_kv_head : 0, heads = r.n_head + nk + nv;
     const int eighth = r.n_rot / 8;  // lanes that turn
     const bool turns = lane < eighth;
     const int d0 = turns ? 4 * lane : 8 * lane, d1 = turns ? 4 * (lane + eighth) : 8 * lane + 4;
@@ -103,66 +128,70 @@ template <int D, bool IN_F16> __global__ void __launch_bounds__(NR_THREADS) norm
     const long long slot = a.k_pool ? r.slots[t] : -1;
     const bool placed = live && slot >= 0 && slot < a.n_slots;
     const int off = (int)(slot & ((1 << a.page_shift) - 1));
-    for (int i = 0; i < a.heads_of_thread; i++) {
-        const int u = part + i * (int)a.split;
-        const bool on = live && u < heads;
-        const int kind = u < r.n_head ? 0 : u < r.n_head + nk ? 1 : 2;  // of q, k, v
-        const int h = kind == 0 ? u : kind == 1 ? u - r.n_head : u - r.n_head - nk;
-        const void* rows = kind == 0 ? r.q : kind == 1 ? r.k : r.v;
-        const long long at = (long long)t * (kind == 0 ? r.q_stride : kind == 1 ? r.k_stride : r.v_stride) + h * D;
-        const float *bias = kind == 0 ? r.q_bias : kind == 1 ? r.k_bias : r.v_bias, *norm = kind == 0 ? r.q_norm : kind == 1 ? r.k_norm : nullptr;
-        float4 x0 = make_float4(0.0f, 0.0f, 0.0f, 0.0f), x1 = x0;
-        if (on) {
-            x0 = load4<IN_F16>(rows, at + d0);
-            x1 = load4<IN_F16>(rows, at + d1);
-            if (bias) {
-                x0 = add4(x0, *reinterpret_cast<const float4*>(bias + h * D + d0));
-                x1 = add4(x1, *reinterpret_cast<const float4*>(bias + h * D + d1));
-            }
-        }
-        float ss = dot4(x0) + dot4(x1);
+    for (int i0 = 0; i0 < a.heads_of_thread; i0 += AT_ONCE) {
+        // all loads first
+        float4 x[AT_ONCE][2];
 #pragma unroll
-        for (int o = 1; o < G; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (norm && on) {
-            const float s = rsqrtf(ss / (float)D + r.eps);
-            x0 = mul4(x0, s, *reinterpret_cast<const float4*>(norm + d0));
-            x1 = mul4(x1, s, *reinterpret_cast<const float4*>(norm + d1));
-        }
-        if (kind != 2 && turns) {
-            turn1(x0.x, x1.x, cs[0], sn[0]);
-            turn1(x0.y, x1.y, cs[1], sn[1]);
-            turn1(x0.z, x1.z, cs[2], sn[2]);
-            turn1(x0.w, x1.w, cs[3], sn[3]);
-        }
-        void* out = kind == 0 ? r.q_out : kind == 1 ? r.k_out : r.v_out;
-        if (out && on) {
-            const long long to = (long long)t * (kind == 0 ? r.q_out_stride : kind == 1 ? r.k_out_stride : r.v_out_stride) + h * D;
-            const int f16 = kind == 0 ? r.q_out_type : r.kv_out_type;
-            store4(out, f16, to + d0, x0);
-            store4(out, f16, to + d1, x1);
-        }
-        if (!a.k_pool) continue;
-        const bool put = placed && on && kind != 0;
-        const long long page_head = (slot >> a.page_shift) * r.n_kv_head + h;
-        uint8_t* pool = kind == 2 ? a.v_pool : a.k_pool;
-        if (a.cache_type == CACHE_F16) {
-            if (put) {
-                uint8_t* row = pool + page_head * paged_region_bytes<D, CACHE_F16>(1 << a.page_shift) + (size_t)off * D * 2;
-                *reinterpret_cast<uint2*>(row + d0 * 2) = halves(x0);
-                *reinterpret_cast<uint2*>(row + d1 * 2) = halves(x1);
+        for (int e = 0; e < AT_ONCE; e++) {
+            const Head<D> w(r, part + (i0 + e) * (int)a.split, live);
+            x[e][0] = x[e][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (w.on) {
+                const long long at = (long long)t * w.stride + w.h * D;
+                x[e][0] = load4<IN_F16>(w.rows, at + d0);
+                x[e][1] = load4<IN_F16>(w.rows, at + d1);
             }
-        } else {
-            // eight neighbouring dims in a lane
-            __syncwarp();
-            s_row[group][d0 / 4] = x0;
-            s_row[group][d1 / 4] = x1;
-            __syncwarp();
-            const float4 y0 = s_row[group][2 * lane], y1 = s_row[group][2 * lane + 1];
-            const Row8 w = {{y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w}, {}};
-            if (a.cache_type == CACHE_Q8_0) {
-                put_q8_0<D, false>(w, pool + page_head * paged_region_bytes<D, CACHE_Q8_0>(1 << a.page_shift), a.page_shift, off, lane, put);
-            } else {
-                put_q4_1<D>(w, pool + page_head * paged_region_bytes<D, CACHE_Q4_1>(1 << a.page_shift), off, lane, kind == 2, put);
+        }
+#pragma unroll
+        for (int e = 0; e < AT_ONCE; e++) {
+            const Head<D> w(r, part + (i0 + e) * (int)a.split, live);
+            float4 x0 = x[e][0], x1 = x[e][1];
+            if (w.bias && w.on) {
+                x0 = add4(x0, *reinterpret_cast<const float4*>(w.bias + w.h * D + d0));
+                x1 = add4(x1, *reinterpret_cast<const float4*>(w.bias + w.h * D + d1));
+            }
+            if (r.q_norm || r.k_norm) {
+                float ss = dot4(x0) + dot4(x1);
+#pragma unroll
+                for (int o = 1; o < G; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                if (w.norm && w.on) {
+                    const float s = rsqrtf(ss / (float)D + r.eps);
+                    x0 = mul4(x0, s, *reinterpret_cast<const float4*>(w.norm + d0));
+                    x1 = mul4(x1, s, *reinterpret_cast<const float4*>(w.norm + d1));
+                }
+            }
+            if (w.kind != 2 && turns) {
+                turn1(x0.x, x1.x, cs[0], sn[0]);
+                turn1(x0.y, x1.y, cs[1], sn[1]);
+                turn1(x0.z, x1.z, cs[2], sn[2]);
+                turn1(x0.w, x1.w, cs[3], sn[3]);
+            }
+            if (w.out && w.on) {
+                const long long to = (long long)t * w.out_stride + w.h * D;
+                store4(w.out, w.f16, to + d0, x0);
+                store4(w.out, w.f16, to + d1, x1);
+            }
+            if (!a.k_pool) continue;
+            const bool put = placed && w.on && w.kind != 0;
+            const long long page_head = (slot >> a.page_shift) * r.n_kv_head + w.h;
+            uint8_t* pool = w.kind == 2 ? a.v_pool : a.k_pool;
+            if (a.cache_type == CACHE_F16) {
+                if (put) {
+                    uint8_t* row = pool + page_head * paged_region_bytes<D, CACHE_F16>(1 << a.page_shift) + (size_t)off * D * 2;
+                    *reinterpret_cast<uint2*>(row + d0 * 2) = halves(x0);
+                    *reinterpret_cast<uint2*>(row + d1 * 2) = halves(x1);
+                }
+            } else if (__any_sync(0xffffffffu, put)) {
+                // eight neighbouring dims in a lane
+                __syncwarp();
+                s_row[group][d0 / 4] = x0;
+                s_row[group][d1 / 4] = x1;
+                __syncwarp();
+                const float4 y0 = s_row[group][2 * lane], y1 = s_row[group][2 * lane + 1];
+                const Row8 y = {{y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w}, {}};
+                if (a.cache_type == CACHE_Q8_0)
+                    put_q8_0<D, false>(y, pool + page_head * paged_region_bytes<D, CACHE_Q8_0>(1 << a.page_shift), a.page_shift, off, lane, put);
+                else
+                    put_q4_1<D>(y, pool + page_head * paged_region_bytes<D, CACHE_Q4_1>(1 << a.page_shift), off, lane, w.kind == 2, put);
             }
         }
     }
@@ -170,6 +199,28 @@ template <int D, bool IN_F16> __global__ void __launch_bounds__(NR_THREADS) norm
 
 bool rows_ok(const void* p, long long stride, long long width) { return p && !((uintptr_t)p & 15) && stride % 8 == 0 && stride >= width; }
 bool type_ok(int t) { return t == 0 || t == 1; }
+
+// The pairs' rates in turns.
+void rates(const CfiNormRope* r, NrArgs* a) {
+    const long double step = powl((long double)r->freq_base, -2.0L / r->n_rot), two64 = 18446744073709551616.0L;
+    long double rate = (long double)r->freq_scale / 6.283185307179586476925287L;
+    if (!r->freq_factors && step < 1.0L && rate >= 0.0L && rate < 1.0L) {  // as is usual: whole numbers all the way
+        unsigned long long turn = (unsigned long long)(rate * two64);
+        const unsigned long long by = (unsigned long long)(step * two64);
+        for (int i = 0; i < r->n_rot / 2; i++) {
+            a->turn[i] = turn;
+            turn = (unsigned long long)(((unsigned __int128)turn * by) >> 64);
+        }
+        return;
+    }
+    for (int i = 0; i < r->n_rot / 2; i++, rate *= step) {
+        const long double part = (rate - floorl(rate)) * two64;
+        if (r->freq_factors)
+            a->rate[i] = (double)rate;
+        else
+            a->turn[i] = part < two64 ? (unsigned long long)part : 0;
+    }
+}
 
 }  // namespace
 
@@ -203,20 +254,13 @@ extern "C" int cfi_norm_rope(const CfiNormRope* r, const CfiPagedCache* c, void*
         a.cache_type = c->type;
     }
     if (r->n_rot) {
-        const long double step = powl((long double)r->freq_base, -2.0L / r->n_rot);
-        long double rate = (long double)r->freq_scale / 6.283185307179586476925287L;
-        for (int i = 0; i < r->n_rot / 2; i++, rate *= step) {
-            const long double part = (rate - floorl(rate)) * 18446744073709551616.0L;
-            if (r->freq_factors)
-                a.rate[i] = (double)rate;
-            else
-                a.turn[i] = part < 18446744073709551616.0L ? (unsigned long long)part : 0;
-        }
+        rates(r, &a);
     }
     const int heads = r->n_head + (r->k ? r->n_kv_head : 0) + (r->v ? r->n_kv_head : 0), groups = NR_THREADS / (r->head_dim / 8);
-    a.heads_of_thread = 1;
-    a.split = heads;
     if ((long long)r->n_tokens * heads > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
+    a.heads_of_thread = 1;
+    if ((long long)r->n_tokens * heads >= NR_MANY * (long long)cfi_sm_count() * groups) a.heads_of_thread = std::min(heads, NR_HEADS);
+    a.split = (heads + a.heads_of_thread - 1) / a.heads_of_thread;
     const uint32_t ctas = ((uint32_t)r->n_tokens * a.split + groups - 1) / groups;
     const char* ep = getenv("CFI_PDL");
     cudaLaunchConfig_t lc = {};
@@ -228,9 +272,10 @@ extern "C" int cfi_norm_rope(const CfiNormRope* r, const CfiPagedCache* c, void*
     at[0].val.programmaticStreamSerializationAllowed = 1;
     lc.attrs = at;
     lc.numAttrs = (ep && strcmp(ep, "0") == 0) ? 0 : 1;
-    const int variant = (r->head_dim == 128) * 2 + r->in_type;
-    return (int)(variant == 0   ? cudaLaunchKernelEx(&lc, norm_rope<64, false>, (const NrArgs)a)
-                 : variant == 1 ? cudaLaunchKernelEx(&lc, norm_rope<64, true>, (const NrArgs)a)
-                 : variant == 2 ? cudaLaunchKernelEx(&lc, norm_rope<128, false>, (const NrArgs)a)
-                                : cudaLaunchKernelEx(&lc, norm_rope<128, true>, (const NrArgs)a));
+    static const void* const fns[8] = {
+        (const void*)norm_rope<64, false, 1>,  (const void*)norm_rope<64, true, 1>,  (const void*)norm_rope<64, false, NR_AT_ONCE>,
+        (const void*)norm_rope<64, true, NR_AT_ONCE>, (const void*)norm_rope<128, false, 1>, (const void*)norm_rope<128, true, 1>,
+        (const void*)norm_rope<128, false, NR_AT_ONCE>, (const void*)norm_rope<128, true, NR_AT_ONCE>};
+    void* args[1] = {&a};
+    return (int)cudaLaunchKernelExC(&lc, fns[(r->head_dim == 128) * 4 + (a.heads_of_thread > 1) * 2 + r->in_type], args);
 }

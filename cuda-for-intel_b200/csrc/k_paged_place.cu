@@ -1,50 +1,57 @@
 // k_paged_place.cu -- page tables, slots, positions and packed offsets of a batch made on the device, and pages given back
 // (include/cfi_serve.h).  Whole numbers only: what a call writes does not depend on any order.
 //
-// A CTA adds up what the sequences hold, get and need (a thread takes some in a row, then one scan over the threads); every
-// element of the lists then finds its sequence by bisection among the sums in shared memory.
+// Every CTA adds up for itself what the sequences hold, get and need (a thread takes some in a row, then one scan over the
+// threads), so that no CTA waits for another; the pages, tokens and positions of the lists are then shared out, and each finds its
+// sequence by bisection among the sums in shared memory.  The state is changed by the last CTA, when all have read it.
+//
+// Bound by latency: rows, lengths, table and lists are read one after the other, a memory round trip each.
 #include "paged_cache.cuh"
 #include "sm100_ptx.cuh"
 #include "cfi_kernels.h"
 
+#include <algorithm>
 #include <stdlib.h>
 #include <string.h>
 
 namespace {
 
-constexpr int PP_THREADS = 1024, PP_SEQS = 8192, PP_ROWS = 65536;
+constexpr int PP_SHARE = 8192;  // elements of a CTA, at least
+constexpr int PP_THREADS = 512, PP_SEQS = 8192, PP_ROWS = 65536;
 
 struct PpArgs {
     CfiPageTable t;
     CfiPagedPlace p;  // of a trim: rows, n_new (what to keep), n_seq, status
     int page_shift;
+    unsigned int* counter;  // CTAs that have read the state; zero between calls
 };
 
-// Sums over the threads of three numbers: those of the threads before this one, and all.
+// Sums over the threads: those of the threads before this one, and all.
 struct Sums {
-    long long q, kv;
-    int pages;
+    long long q, kv;  // new tokens, positions
+    int pages, taken;  // that hold them; of those, new ones
 };
-CFI_DEV Sums operator+(const Sums& a, const Sums& b) { return {a.q + b.q, a.kv + b.kv, a.pages + b.pages}; }
+CFI_DEV Sums operator+(const Sums& a, const Sums& b) { return {a.q + b.q, a.kv + b.kv, a.pages + b.pages, a.taken + b.taken}; }
 CFI_DEV Sums scan(Sums x, Sums* total) {
-    __shared__ Sums s_warp[32];
+    __shared__ Sums s_warp[PP_THREADS / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     Sums incl = x;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const Sums y = {__shfl_up_sync(0xffffffffu, incl.q, o), __shfl_up_sync(0xffffffffu, incl.kv, o), __shfl_up_sync(0xffffffffu, incl.pages, o)};
+        const Sums y = {__shfl_up_sync(0xffffffffu, incl.q, o), __shfl_up_sync(0xffffffffu, incl.kv, o), __shfl_up_sync(0xffffffffu, incl.pages, o),
+                        __shfl_up_sync(0xffffffffu, incl.taken, o)};
         if (lane >= o) incl = incl + y;
     }
     if (lane == 31) s_warp[warp] = incl;
     __syncthreads();
-    Sums before = {0, 0, 0}, all = {0, 0, 0};
+    Sums before = {0, 0, 0, 0}, all = {0, 0, 0, 0};
     for (int w = 0; w < PP_THREADS / 32; w++) {
         if (w == warp) before = all;
         all = all + s_warp[w];
     }
     __syncthreads();
     *total = all;
-    return {before.q + incl.q - x.q, before.kv + incl.kv - x.kv, before.pages + incl.pages - x.pages};
+    return {before.q + incl.q - x.q, before.kv + incl.kv - x.kv, before.pages + incl.pages - x.pages, before.taken + incl.taken - x.taken};
 }
 
 // Marks row r; true where it was marked before or there is no such row.
@@ -63,101 +70,125 @@ CFI_DEV int sequence_of(const int* cu, int n, int i) {
     return lo;
 }
 
+// True in the CTA that is the last to come here: all others have read what they need of the state.
+CFI_DEV bool last_to_read(unsigned int* counter) {
+    __shared__ int s_last;
+    if (gridDim.x == 1) return true;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        __threadfence();
+        s_last = atomicAdd(counter, 1u) == gridDim.x - 1;
+        if (s_last) *counter = 0u;
+    }
+    __syncthreads();
+    return s_last;
+}
+
 __global__ void __launch_bounds__(PP_THREADS) paged_place(const __grid_constant__ PpArgs a) {
     extern __shared__ int smem[];
     const CfiPageTable& t = a.t;
     const CfiPagedPlace& p = a.p;
     const int n = p.n_seq, tid = threadIdx.x, mask = t.page_size - 1;
-    int *cu_q = smem, *cu_kv = cu_q + n + 1, *first = cu_kv + n + 1, *row = first + n;  // first: of the pages taken
+    int *cu_q = smem, *cu_kv = cu_q + n + 1, *cu_pages = cu_kv + n + 1, *first = cu_pages + n + 1, *row = first + n;  // first: of the pages taken
     uint32_t* seen = reinterpret_cast<uint32_t*>(row + n);
     __shared__ int s_why;
     sm100::pdl_launch_dependents();
-    sm100::pdl_wait();
     for (int i = tid; i < (t.n_rows + 31) / 32; i += PP_THREADS) seen[i] = 0;
     if (tid == 0) s_why = 0x7fffffff;
+    sm100::pdl_wait();
     __syncthreads();
     const int each = (n + PP_THREADS - 1) / PP_THREADS, s0 = min(n, tid * each), s1 = min(n, s0 + each);
     const int n_free = min(max(*t.n_free, 0), t.n_pages);
-    Sums mine = {0, 0, 0};
+    Sums mine = {0, 0, 0, 0};
     int why = 0x7fffffff;
     for (int s = s0; s < s1; s++) {
         const int r = p.rows[s], add = p.n_new[s];
+        cu_q[s] = add;
+        row[s] = r;
         if (bad_row(seen, r, t.n_rows) || add < 0) {
             why = min(why, (int)CFI_PLACE_BAD_ROW);
             continue;
         }
-        row[s] = r;
         const int held = t.cached[r];
+        cu_kv[s] = held;
         const long long after = (long long)held + add;
-        if (held < 0) why = min(why, (int)CFI_PLACE_BAD_ROW);
-        else if (after > (long long)t.max_pages << a.page_shift || after > 0x7fffffffLL - mask) why = min(why, (int)CFI_PLACE_TOO_LONG);
-        else mine = mine + Sums{add, after, (int)((after + mask) >> a.page_shift) - ((held + mask) >> a.page_shift)};
+        if (held < 0) {
+            why = min(why, (int)CFI_PLACE_BAD_ROW);
+        } else if (after > (long long)t.max_pages << a.page_shift || after > 0x7fffffffLL - mask) {
+            why = min(why, (int)CFI_PLACE_TOO_LONG);
+        } else {
+            const int pages = (int)((after + mask) >> a.page_shift);
+            mine = mine + Sums{add, after, pages, pages - ((held + mask) >> a.page_shift)};
+        }
     }
     Sums all;
     Sums at = scan(mine, &all);
     if (all.kv > 0x7fffffffLL) why = min(why, (int)CFI_PLACE_TOO_LONG);
     if (all.q > p.max_new || (p.context && all.kv > p.max_context)) why = min(why, (int)CFI_PLACE_NO_ROOM);
-    if (all.pages > n_free) why = min(why, (int)CFI_PLACE_NO_PAGES);
+    if (all.taken > n_free) why = min(why, (int)CFI_PLACE_NO_PAGES);
     if (why != 0x7fffffff) atomicMin(&s_why, why);
     __syncthreads();
-    const bool ok = s_why == 0x7fffffff;
+    const bool ok = s_why == 0x7fffffff, writes = blockIdx.x == 0;
     for (int s = s0; s < s1; s++) {
-        int add = 0, after = 0, need = 0;
-        if (ok) {
-            add = p.n_new[s];
-            const int held = t.cached[row[s]];
-            after = held + add;
-            need = ((after + mask) >> a.page_shift) - ((held + mask) >> a.page_shift);
+        const int add = ok ? cu_q[s] : 0, held = ok ? cu_kv[s] : 0, pages = (held + add + mask) >> a.page_shift;
+        cu_q[s] = ok ? (int)at.q : 0;
+        cu_kv[s] = ok ? (int)at.kv : 0;
+        cu_pages[s] = at.pages;
+        first[s] = at.taken;
+        if (writes) {
+            p.cu_q[s] = cu_q[s];
+            p.cu_kv[s] = cu_kv[s];
+            p.lens[s] = held + add;
         }
-        cu_q[s] = (int)(ok ? at.q : 0);
-        cu_kv[s] = (int)(ok ? at.kv : 0);
-        first[s] = at.pages;
-        p.cu_q[s] = cu_q[s];
-        p.cu_kv[s] = cu_kv[s];
-        p.lens[s] = after;
-        at = at + Sums{add, after, need};
+        at = at + Sums{add, held + add, pages, pages - ((held + mask) >> a.page_shift)};
     }
     if (tid == 0) {
-        p.status[0] = ok ? (int)CFI_PLACED : s_why;
-        p.cu_q[n] = cu_q[n] = ok ? (int)all.q : 0;
-        p.cu_kv[n] = cu_kv[n] = ok ? (int)all.kv : 0;
+        cu_q[n] = ok ? (int)all.q : 0;
+        cu_kv[n] = ok ? (int)all.kv : 0;
+        cu_pages[n] = ok ? all.pages : 0;
+        if (writes) {
+            p.status[0] = ok ? (int)CFI_PLACED : s_why;
+            p.cu_q[n] = cu_q[n];
+            p.cu_kv[n] = cu_kv[n];
+        }
     }
     __syncthreads();
-    // page i of sequence s, which held `old` pages before
-    auto page = [&](int s, int i, int old) {
+    auto held = [&](int s) { return cu_kv[s + 1] - cu_kv[s] - (cu_q[s + 1] - cu_q[s]); };
+    // page i of sequence s
+    auto page = [&](int s, int i) {
+        const int old = (held(s) + mask) >> a.page_shift;
         return i < old ? t.table[(long long)row[s] * t.max_pages + i] : t.free_pages[n_free - 1 - (first[s] + i - old)];
     };
-    auto held = [&](int s) { return cu_kv[s + 1] - cu_kv[s] - (cu_q[s + 1] - cu_q[s]); };
-    for (int s = tid >> 5; ok && s < n; s += PP_THREADS / 32) {
-        const int old = (held(s) + mask) >> a.page_shift, pages = (cu_kv[s + 1] - cu_kv[s] + mask) >> a.page_shift;
-        for (int i = tid & 31; i < pages; i += 32) {
-            const int id = page(s, i, old);
-            p.batch_table[(long long)s * t.max_pages + i] = id;
-            if (i >= old) t.table[(long long)row[s] * t.max_pages + i] = id;
-        }
+    const int all_pages = cu_pages[n], all_q = cu_q[n], all_kv = cu_kv[n];
+    const uint32_t id = blockIdx.x * PP_THREADS + tid, threads = gridDim.x * PP_THREADS;
+    for (uint32_t x = id; x < (uint32_t)all_pages; x += threads) {
+        const int s = sequence_of(cu_pages, n, x), i = x - cu_pages[s], to = page(s, i);
+        p.batch_table[(long long)s * t.max_pages + i] = to;
+        if (i >= (held(s) + mask) >> a.page_shift) t.table[(long long)row[s] * t.max_pages + i] = to;
     }
-    for (int i = tid; i < p.max_new; i += PP_THREADS) {
+    for (uint32_t x = id; x < (uint32_t)p.max_new; x += threads) {
         long long slot = -1;
         int pos = 0;
-        if (i < cu_q[n]) {
-            const int s = sequence_of(cu_q, n, i), h = held(s);
-            pos = h + i - cu_q[s];
-            slot = ((long long)page(s, pos >> a.page_shift, (h + mask) >> a.page_shift) << a.page_shift) + (pos & mask);
+        if (x < (uint32_t)all_q) {
+            const int s = sequence_of(cu_q, n, x);
+            pos = held(s) + x - cu_q[s];
+            slot = ((long long)page(s, pos >> a.page_shift) << a.page_shift) + (pos & mask);
         }
-        p.slots[i] = slot;
-        p.positions[i] = pos;
+        p.slots[x] = slot;
+        p.positions[x] = pos;
     }
-    for (int i = tid; p.context && i < p.max_context; i += PP_THREADS) {
-        long long slot = -1;
-        if (i < cu_kv[n]) {
-            const int s = sequence_of(cu_kv, n, i), pos = i - cu_kv[s];
-            slot = ((long long)page(s, pos >> a.page_shift, (held(s) + mask) >> a.page_shift) << a.page_shift) + (pos & mask);
+    if (p.context) {
+        // 16 lanes to a page
+        for (uint32_t x = id >> 4; x < (uint32_t)all_pages; x += threads >> 4) {
+            const int s = sequence_of(cu_pages, n, x), i = x - cu_pages[s], len = cu_kv[s + 1] - cu_kv[s];
+            const long long slot = (long long)page(s, i) << a.page_shift;
+            for (int j = tid & 15; j <= mask && (i << a.page_shift) + j < len; j += 16) p.context[cu_kv[s] + (i << a.page_shift) + j] = slot + j;
         }
-        p.context[i] = slot;
+        for (uint32_t x = all_kv + id; x < (uint32_t)p.max_context; x += threads) p.context[x] = -1;
     }
-    if (!ok) return;
+    if (!ok || !last_to_read(a.counter)) return;
     for (int s = s0; s < s1; s++) t.cached[row[s]] = cu_kv[s + 1] - cu_kv[s];
-    if (tid == 0) *t.n_free = n_free - all.pages;
+    if (tid == 0) *t.n_free = n_free - all.taken;
 }
 
 __global__ void __launch_bounds__(PP_THREADS) paged_trim(const __grid_constant__ PpArgs a) {
@@ -165,35 +196,36 @@ __global__ void __launch_bounds__(PP_THREADS) paged_trim(const __grid_constant__
     const CfiPageTable& t = a.t;
     const int n = a.p.n_seq, tid = threadIdx.x, mask = t.page_size - 1;
     const int32_t* keep = a.p.n_new;
-    int *first = smem, *from = first + n + 1, *row = from + n;  // of the pages given back; the first such of a row
-    uint32_t* seen = reinterpret_cast<uint32_t*>(row + n);
+    int *first = smem, *from = first + n + 1, *row = from + n, *now = row + n;  // of the pages given back; the first such of a row
+    uint32_t* seen = reinterpret_cast<uint32_t*>(now + n);
     __shared__ int s_why;
     sm100::pdl_launch_dependents();
-    sm100::pdl_wait();
     for (int i = tid; i < (t.n_rows + 31) / 32; i += PP_THREADS) seen[i] = 0;
     if (tid == 0) s_why = 0x7fffffff;
+    sm100::pdl_wait();
     __syncthreads();
     const int each = (n + PP_THREADS - 1) / PP_THREADS, s0 = min(n, tid * each), s1 = min(n, s0 + each);
     const int n_free = min(max(*t.n_free, 0), t.n_pages);
-    Sums mine = {0, 0, 0};
+    Sums mine = {0, 0, 0, 0};
     int why = 0x7fffffff;
     for (int s = s0; s < s1; s++) {
-        const int r = a.p.rows[s];
+        const int r = a.p.rows[s], most = max(keep[s], 0);
         row[s] = r;
         if (bad_row(seen, r, t.n_rows)) {
             why = min(why, (int)CFI_PLACE_BAD_ROW);
             continue;
         }
-        const int held = t.cached[r], now = min(held, max(keep[s], 0));
+        const int held = t.cached[r];
         if (held < 0) {
             why = min(why, (int)CFI_PLACE_BAD_ROW);
         } else if (held > (long long)t.max_pages << a.page_shift || held > 0x7fffffff - mask) {
             why = min(why, (int)CFI_PLACE_TOO_LONG);
         } else {
+            now[s] = min(held, most);
             first[s] = mine.pages;
-            from[s] = (now + mask) >> a.page_shift;
+            from[s] = (now[s] + mask) >> a.page_shift;
             const int gone = ((held + mask) >> a.page_shift) - from[s];
-            mine = mine + Sums{0, gone, gone};
+            mine = mine + Sums{0, gone, gone, 0};
         }
     }
     Sums all;
@@ -201,23 +233,20 @@ __global__ void __launch_bounds__(PP_THREADS) paged_trim(const __grid_constant__
     if (all.kv > t.n_pages - n_free) why = min(why, (int)CFI_PLACE_NO_PAGES);
     if (why != 0x7fffffff) atomicMin(&s_why, why);
     __syncthreads();
-    if (s_why != 0x7fffffff) {
-        if (tid == 0) a.p.status[0] = s_why;
-        return;
+    const bool ok = s_why == 0x7fffffff;
+    if (tid == 0 && blockIdx.x == 0) a.p.status[0] = ok ? (int)CFI_PLACED : s_why;
+    if (ok) {
+        for (int s = s0; s < s1; s++) first[s] += at.pages;
+        if (tid == 0) first[n] = all.pages;
+        __syncthreads();
+        for (uint32_t x = blockIdx.x * PP_THREADS + tid; x < (uint32_t)all.pages; x += gridDim.x * PP_THREADS) {
+            const int s = sequence_of(first, n, x);
+            t.free_pages[n_free + all.pages - 1 - x] = t.table[(long long)row[s] * t.max_pages + from[s] + x - first[s]];
+        }
     }
-    for (int s = s0; s < s1; s++) {
-        first[s] += at.pages;
-        t.cached[row[s]] = min(t.cached[row[s]], max(keep[s], 0));
-    }
-    if (tid == 0) {
-        first[n] = all.pages;
-        *t.n_free = n_free + all.pages;
-        a.p.status[0] = CFI_PLACED;
-    }
-    __syncthreads();
-    for (int s = tid >> 5; s < n; s += PP_THREADS / 32)
-        for (int i = tid & 31; i < first[s + 1] - first[s]; i += 32)
-            t.free_pages[n_free + all.pages - 1 - (first[s] + i)] = t.table[(long long)row[s] * t.max_pages + from[s] + i];
+    if (!last_to_read(a.counter) || !ok) return;
+    for (int s = s0; s < s1; s++) t.cached[row[s]] = now[s];
+    if (tid == 0) *t.n_free = n_free + all.pages;
 }
 
 bool table_ok(const CfiPageTable* t) {
@@ -228,11 +257,18 @@ bool table_ok(const CfiPageTable* t) {
 }
 size_t seen_bytes(const CfiPageTable* t) { return (size_t)(t->n_rows + 31) / 32 * 4; }
 
-int go(const void* fn, PpArgs& a, size_t smem, cudaStream_t stream) {
+// `work`: an upper bound of the elements that are read or written.
+int go(const void* fn, PpArgs& a, size_t smem, long long work, cudaStream_t stream) {
+    const long long ctas = std::min<long long>(cfi_sm_count(), std::max<long long>(1, work / PP_SHARE));
+    if (ctas > 1) {
+        int err = 0;
+        a.counter = static_cast<unsigned int*>(cfi_stream_buffer(CFI_BUF_COUNTERS, 4, stream, &err));
+        if (!a.counter) return err;
+    }
     a.page_shift = __builtin_ctz((unsigned)a.t.page_size);
     const char* ep = getenv("CFI_PDL");
     cudaLaunchConfig_t c = {};
-    c.gridDim = dim3(1, 1, 1);
+    c.gridDim = dim3((unsigned)ctas, 1, 1);
     c.blockDim = dim3(PP_THREADS, 1, 1);
     c.dynamicSmemBytes = smem;
     c.stream = stream;
@@ -244,7 +280,7 @@ int go(const void* fn, PpArgs& a, size_t smem, cudaStream_t stream) {
     void* args[1] = {&a};
     return (int)cudaLaunchKernelExC(&c, fn, args);
 }
-constexpr int PP_SMEM = PP_ROWS / 8 + (4 * PP_SEQS + 2) * 4;
+constexpr int PP_SMEM = PP_ROWS / 8 + (5 * PP_SEQS + 3) * 4;
 void allow_smem() {
     static CfiPerDeviceOnce once;
     cfi_once_per_device(once, [] {
@@ -262,9 +298,10 @@ extern "C" int cfi_paged_place(const CfiPageTable* t, const CfiPagedPlace* p, vo
           (uintptr_t)p->cu_kv | (uintptr_t)p->positions | (uintptr_t)p->status) & 3) ||
         (((uintptr_t)p->slots | (uintptr_t)p->context) & 7))
         return (int)cudaErrorInvalidValue;
-    PpArgs a = {*t, *p, 0};
+    PpArgs a = {*t, *p, 0, nullptr};
     allow_smem();
-    return go((const void*)paged_place, a, (size_t)(4 * p->n_seq + 2) * 4 + seen_bytes(t), static_cast<cudaStream_t>(stream));
+    return go((const void*)paged_place, a, (size_t)(5 * p->n_seq + 3) * 4 + seen_bytes(t),
+              (long long)p->n_seq * t->max_pages + p->max_new + (p->context ? p->max_context : 0), static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int cfi_paged_trim(const CfiPageTable* t, const int32_t* rows, const int32_t* keep, int n_seq, int32_t* status, void* stream) {
@@ -278,5 +315,6 @@ extern "C" int cfi_paged_trim(const CfiPageTable* t, const int32_t* rows, const 
     a.p.n_seq = n_seq;
     a.p.status = status;
     allow_smem();
-    return go((const void*)paged_trim, a, (size_t)(3 * n_seq + 1) * 4 + seen_bytes(t), static_cast<cudaStream_t>(stream));
+    return go((const void*)paged_trim, a, (size_t)(4 * n_seq + 1) * 4 + seen_bytes(t), (long long)n_seq * t->max_pages,
+              static_cast<cudaStream_t>(stream));
 }
