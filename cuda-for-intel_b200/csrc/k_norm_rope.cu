@@ -26,8 +26,9 @@ struct NrArgs {
     uint8_t *k_pool, *v_pool;
     long long n_slots;
     int page_shift, cache_type;
-    int heads_of_thread;  // heads of one token that a group of lanes takes, `split` apart
-    uint32_t split;
+    uint32_t runs;           // of a token's heads: those of q begin at 0, of k and v at begin[1] and begin[2]
+    int begin[3], heads[3];  // heads of a run
+    int most;                // the largest of them
     union {
         unsigned long long turn[NR_RATES];  // of 2^64
         double rate[NR_RATES];              // in turns, where freq_factors divide them
@@ -71,116 +72,106 @@ CFI_DEV void turn1(float& x, float& y, float c, float s) {
     x = t;
 }
 
-// Head u of a token's heads of q, k and v.
-template <int D> struct Head {
-    int kind, h, f16;  // kind: 0, 1, 2 of q, k, v
-    bool on;
-    const void* rows;
-    void* out;
-    long long stride, out_stride;
-    const float *bias, *norm;
-    CFI_DEV Head(const CfiNormRope& r, int u, bool live) {
-        const int nk = r.k ? r.n_kv_head : 0, nv = r.v ? r.n_kv_head : 0;
-        on = live && u < r.n_head + nk + nv;
-        kind = u < r.n_head ? 0 : u < r.n_head + nk ? 1 : 2;
-        h = kind == 0 ? u : kind == 1 ? u - r.n_head : u - r.n_head - nk;
-        rows = kind == 0 ? r.q : kind == 1 ? r.k : r.v;
-        stride = kind == 0 ? r.q_stride : kind == 1 ? r.k_stride : r.v_stride;
-        bias = kind == 0 ? r.q_bias : kind == 1 ? r.k_bias : r.v_bias;
-        norm = kind == 0 ? r.q_norm : kind == 1 ? r.k_norm : nullptr;
-        out = kind == 0 ? r.q_out : kind == 1 ? r.k_out : r.v_out;
-        out_stride = kind == 0 ? r.q_out_stride : kind == 1 ? r.k_out_stride : r.v_out_stride;
-        f16 = kind == 0 ? r.q_out_type : r.kv_out_type;
-    }
-};
-
 template <int D, bool IN_F16, int AT_ONCE> __global__ void __launch_bounds__(NR_THREADS) norm_rope(const __grid_constant__ NrArgs a) {
     constexpr int G = D / 8;  // lanes of a head
-    __shared__ float4 s_row[NR_THREADS / G][2 * G];  // a row of k, where the cache wants eight dims in a lane
+    __shared__ float4 s_row[NR_THREADS / G][2 * G];  // a row of k or v, where the cache wants eight dims in a lane
     const CfiNormRope& r = a.r;
     const int lane = threadIdx.x % G, group = threadIdx.x / G;
     const int eighth = r.n_rot / 8;  // lanes that turn
-    const bool turns = lane < eighth;
-    const int d0 = turns ? 4 * lane : 8 * lane, d1 = turns ? 4 * (lane + eighth) : 8 * lane + 4;
+    const int d0 = lane < eighth ? 4 * lane : 8 * lane, d1 = lane < eighth ? 4 * (lane + eighth) : 8 * lane + 4;
+    // this group's token and run of heads, of q (kind 0), k or v
+    const uint32_t id = blockIdx.x * (NR_THREADS / G) + group;
+    const bool live = id < (uint32_t)r.n_tokens * a.runs;
+    const int t = live ? (int)(id / a.runs) : r.n_tokens - 1, run = live ? (int)(id % a.runs) : 0;
+    const int kind = run < a.begin[1] ? 0 : run < a.begin[2] ? 1 : 2;
+    const int h0 = (run - a.begin[kind]) * a.heads[kind], n = live ? min(a.heads[kind], (kind ? r.n_kv_head : r.n_head) - h0) : 0;
+    const bool turns = lane < eighth && kind != 2;
+    const long long from = (long long)t * (kind == 0 ? r.q_stride : kind == 1 ? r.k_stride : r.v_stride) + h0 * D;
+    const uint8_t* in = static_cast<const uint8_t*>(kind == 0 ? r.q : kind == 1 ? r.k : r.v) + from * (IN_F16 ? 2 : 4);
+    const float* bias = kind == 0 ? r.q_bias : kind == 1 ? r.k_bias : r.v_bias;
+    if (bias) bias += h0 * D;
+    const float* norm = kind == 0 ? r.q_norm : kind == 1 ? r.k_norm : nullptr;
+    const int out_f16 = kind == 0 ? r.q_out_type : r.kv_out_type;
+    uint8_t* out = static_cast<uint8_t*>(kind == 0 ? r.q_out : kind == 1 ? r.k_out : r.v_out);
+    if (out) out += ((long long)t * (kind == 0 ? r.q_out_stride : kind == 1 ? r.k_out_stride : r.v_out_stride) + h0 * D) * (out_f16 ? 2 : 4);
     sm100::pdl_launch_dependents();
     sm100::pdl_wait();
-    const uint32_t id = blockIdx.x * (NR_THREADS / G) + group;
-    const bool live = id < (uint32_t)r.n_tokens * a.split;
-    const int t = live ? (int)(id / a.split) : r.n_tokens - 1, part = live ? (int)(id % a.split) : 0;
-    float cs[4], sn[4];
-#pragma unroll
-    for (int e = 0; e < 4; e++) cs[e] = 1.0f, sn[e] = 0.0f;
-    if (turns) {
-        const int pos = r.pos[t];
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            unsigned long long f;
-            if (r.freq_factors) {
-                const double x = a.rate[4 * lane + e] / (double)r.freq_factors[4 * lane + e];
-                f = __double2ull_rn((x - floor(x)) * 18446744073709551616.0);
-            } else {
-                f = a.turn[4 * lane + e];
-            }
-            const int angle = (int)((f * (unsigned long long)(long long)pos) >> 32);
-            sincospif((float)angle * 0x1p-31f, &sn[e], &cs[e]);
-        }
-    }
-    const long long slot = a.k_pool ? r.slots[t] : -1;
-    const bool placed = live && slot >= 0 && slot < a.n_slots;
+    const long long slot = a.k_pool && kind != 0 ? r.slots[t] : -1;
+    const bool put = live && slot >= 0 && slot < a.n_slots;
     const int off = (int)(slot & ((1 << a.page_shift) - 1));
-    for (int i0 = 0; i0 < a.heads_of_thread; i0 += AT_ONCE) {
+    const long long region_bytes = a.cache_type == CACHE_F16 ? paged_region_bytes<D, CACHE_F16>(1 << a.page_shift)
+                                   : a.cache_type == CACHE_Q8_0 ? paged_region_bytes<D, CACHE_Q8_0>(1 << a.page_shift)
+                                                                : paged_region_bytes<D, CACHE_Q4_1>(1 << a.page_shift);
+    uint8_t* region = (kind == 2 ? a.v_pool : a.k_pool) + ((slot >> a.page_shift) * r.n_kv_head + h0) * region_bytes;
+    float4 w0 = make_float4(0.0f, 0.0f, 0.0f, 0.0f), w1 = w0;
+    if (norm) {
+        w0 = *reinterpret_cast<const float4*>(norm + d0);
+        w1 = *reinterpret_cast<const float4*>(norm + d1);
+    }
+    float cs[4], sn[4];
+    for (int i0 = 0; i0 < a.most; i0 += AT_ONCE) {
         // all loads first
         float4 x[AT_ONCE][2];
 #pragma unroll
         for (int e = 0; e < AT_ONCE; e++) {
-            const Head<D> w(r, part + (i0 + e) * (int)a.split, live);
             x[e][0] = x[e][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (w.on) {
-                const long long at = (long long)t * w.stride + w.h * D;
-                x[e][0] = load4<IN_F16>(w.rows, at + d0);
-                x[e][1] = load4<IN_F16>(w.rows, at + d1);
+            if (i0 + e < n) {
+                x[e][0] = load4<IN_F16>(in, (i0 + e) * D + d0);
+                x[e][1] = load4<IN_F16>(in, (i0 + e) * D + d1);
+            }
+        }
+        if (i0 == 0 && turns) {
+            const int pos = r.pos[t];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                unsigned long long f;
+                if (r.freq_factors) {
+                    const double y = a.rate[4 * lane + e] / (double)r.freq_factors[4 * lane + e];
+                    f = __double2ull_rn((y - floor(y)) * 18446744073709551616.0);
+                } else {
+                    f = a.turn[4 * lane + e];
+                }
+                const int angle = (int)((f * (unsigned long long)(long long)pos) >> 32);
+                sincospif((float)angle * 0x1p-31f, &sn[e], &cs[e]);
             }
         }
 #pragma unroll
         for (int e = 0; e < AT_ONCE; e++) {
-            const Head<D> w(r, part + (i0 + e) * (int)a.split, live);
+            const int h = i0 + e;
+            const bool on = h < n;
             float4 x0 = x[e][0], x1 = x[e][1];
-            if (w.bias && w.on) {
-                x0 = add4(x0, *reinterpret_cast<const float4*>(w.bias + w.h * D + d0));
-                x1 = add4(x1, *reinterpret_cast<const float4*>(w.bias + w.h * D + d1));
+            if (bias && on) {
+                x0 = add4(x0, *reinterpret_cast<const float4*>(bias + h * D + d0));
+                x1 = add4(x1, *reinterpret_cast<const float4*>(bias + h * D + d1));
             }
             if (r.q_norm || r.k_norm) {
                 float ss = dot4(x0) + dot4(x1);
 #pragma unroll
                 for (int o = 1; o < G; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                if (w.norm && w.on) {
+                if (norm && on) {
                     const float s = rsqrtf(ss / (float)D + r.eps);
-                    x0 = mul4(x0, s, *reinterpret_cast<const float4*>(w.norm + d0));
-                    x1 = mul4(x1, s, *reinterpret_cast<const float4*>(w.norm + d1));
+                    x0 = mul4(x0, s, w0);
+                    x1 = mul4(x1, s, w1);
                 }
             }
-            if (w.kind != 2 && turns) {
+            if (turns) {
                 turn1(x0.x, x1.x, cs[0], sn[0]);
                 turn1(x0.y, x1.y, cs[1], sn[1]);
                 turn1(x0.z, x1.z, cs[2], sn[2]);
                 turn1(x0.w, x1.w, cs[3], sn[3]);
             }
-            if (w.out && w.on) {
-                const long long to = (long long)t * w.out_stride + w.h * D;
-                store4(w.out, w.f16, to + d0, x0);
-                store4(w.out, w.f16, to + d1, x1);
+            if (out && on) {
+                store4(out, out_f16, h * D + d0, x0);
+                store4(out, out_f16, h * D + d1, x1);
             }
             if (!a.k_pool) continue;
-            const bool put = placed && w.on && w.kind != 0;
-            const long long page_head = (slot >> a.page_shift) * r.n_kv_head + w.h;
-            uint8_t* pool = w.kind == 2 ? a.v_pool : a.k_pool;
+            uint8_t* to = region + h * region_bytes;
             if (a.cache_type == CACHE_F16) {
-                if (put) {
-                    uint8_t* row = pool + page_head * paged_region_bytes<D, CACHE_F16>(1 << a.page_shift) + (size_t)off * D * 2;
-                    *reinterpret_cast<uint2*>(row + d0 * 2) = halves(x0);
-                    *reinterpret_cast<uint2*>(row + d1 * 2) = halves(x1);
+                if (put && on) {
+                    *reinterpret_cast<uint2*>(to + (off * D + d0) * 2) = halves(x0);
+                    *reinterpret_cast<uint2*>(to + (off * D + d1) * 2) = halves(x1);
                 }
-            } else if (__any_sync(0xffffffffu, put)) {
+            } else if (__any_sync(0xffffffffu, put && on)) {
                 // eight neighbouring dims in a lane
                 __syncwarp();
                 s_row[group][d0 / 4] = x0;
@@ -189,9 +180,9 @@ template <int D, bool IN_F16, int AT_ONCE> __global__ void __launch_bounds__(NR_
                 const float4 y0 = s_row[group][2 * lane], y1 = s_row[group][2 * lane + 1];
                 const Row8 y = {{y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w}, {}};
                 if (a.cache_type == CACHE_Q8_0)
-                    put_q8_0<D, false>(y, pool + page_head * paged_region_bytes<D, CACHE_Q8_0>(1 << a.page_shift), a.page_shift, off, lane, put);
+                    put_q8_0<D, false>(y, to, a.page_shift, off, lane, put && on);
                 else
-                    put_q4_1<D>(y, pool + page_head * paged_region_bytes<D, CACHE_Q4_1>(1 << a.page_shift), off, lane, w.kind == 2, put);
+                    put_q4_1<D>(y, to, off, lane, kind == 2, put && on);
             }
         }
     }
@@ -258,10 +249,16 @@ extern "C" int cfi_norm_rope(const CfiNormRope* r, const CfiPagedCache* c, void*
     }
     const int heads = r->n_head + (r->k ? r->n_kv_head : 0) + (r->v ? r->n_kv_head : 0), groups = NR_THREADS / (r->head_dim / 8);
     if ((long long)r->n_tokens * heads > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
-    a.heads_of_thread = 1;
-    if ((long long)r->n_tokens * heads >= NR_MANY * (long long)cfi_sm_count() * groups) a.heads_of_thread = std::min(heads, NR_HEADS);
-    a.split = (heads + a.heads_of_thread - 1) / a.heads_of_thread;
-    const uint32_t ctas = ((uint32_t)r->n_tokens * a.split + groups - 1) / groups;
+    const bool many = (long long)r->n_tokens * heads >= NR_MANY * (long long)cfi_sm_count() * groups;
+    const int count[3] = {r->n_head, r->k ? r->n_kv_head : 0, r->v ? r->n_kv_head : 0};
+    for (int i = 0; i < 3; i++) {
+        a.begin[i] = (int)a.runs;
+        const int runs = many ? (count[i] + NR_HEADS - 1) / NR_HEADS : count[i];
+        a.heads[i] = runs ? (count[i] + runs - 1) / runs : 0;
+        a.runs += runs;
+        a.most = std::max(a.most, a.heads[i]);
+    }
+    const uint32_t ctas = ((uint32_t)r->n_tokens * a.runs + groups - 1) / groups;
     const char* ep = getenv("CFI_PDL");
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3(ctas, 1, 1);
@@ -277,5 +274,5 @@ extern "C" int cfi_norm_rope(const CfiNormRope* r, const CfiPagedCache* c, void*
         (const void*)norm_rope<64, true, NR_AT_ONCE>, (const void*)norm_rope<128, false, 1>, (const void*)norm_rope<128, true, 1>,
         (const void*)norm_rope<128, false, NR_AT_ONCE>, (const void*)norm_rope<128, true, NR_AT_ONCE>};
     void* args[1] = {&a};
-    return (int)cudaLaunchKernelExC(&lc, fns[(r->head_dim == 128) * 4 + (a.heads_of_thread > 1) * 2 + r->in_type], args);
+    return (int)cudaLaunchKernelExC(&lc, fns[(r->head_dim == 128) * 4 + many * 2 + r->in_type], args);
 }

@@ -16,7 +16,7 @@
 
 namespace {
 
-constexpr int PP_SHARE = 8192;  // elements of a CTA, at least
+constexpr int PP_SHARE = 2048;  // elements of a CTA, at least
 constexpr int PP_THREADS = 512, PP_SEQS = 8192, PP_ROWS = 65536;
 
 struct PpArgs {
@@ -70,18 +70,13 @@ CFI_DEV int sequence_of(const int* cu, int n, int i) {
     return lo;
 }
 
-// True in the CTA that is the last to come here: all others have read what they need of the state.
+// Thread 0 says that its CTA has read the state; true where all others have: this one may change it.
 CFI_DEV bool last_to_read(unsigned int* counter) {
-    __shared__ int s_last;
     if (gridDim.x == 1) return true;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        __threadfence();
-        s_last = atomicAdd(counter, 1u) == gridDim.x - 1;
-        if (s_last) *counter = 0u;
-    }
-    __syncthreads();
-    return s_last;
+    __threadfence();
+    const bool last = atomicAdd(counter, 1u) == gridDim.x - 1;
+    if (last) *counter = 0u;
+    return last;
 }
 
 __global__ void __launch_bounds__(PP_THREADS) paged_place(const __grid_constant__ PpArgs a) {
@@ -91,7 +86,7 @@ __global__ void __launch_bounds__(PP_THREADS) paged_place(const __grid_constant_
     const int n = p.n_seq, tid = threadIdx.x, mask = t.page_size - 1;
     int *cu_q = smem, *cu_kv = cu_q + n + 1, *cu_pages = cu_kv + n + 1, *first = cu_pages + n + 1, *row = first + n;  // first: of the pages taken
     uint32_t* seen = reinterpret_cast<uint32_t*>(row + n);
-    __shared__ int s_why;
+    __shared__ int s_why, s_last;
     sm100::pdl_launch_dependents();
     for (int i = tid; i < (t.n_rows + 31) / 32; i += PP_THREADS) seen[i] = 0;
     if (tid == 0) s_why = 0x7fffffff;
@@ -151,6 +146,7 @@ __global__ void __launch_bounds__(PP_THREADS) paged_place(const __grid_constant_
             p.cu_q[n] = cu_q[n];
             p.cu_kv[n] = cu_kv[n];
         }
+        s_last = ok && last_to_read(a.counter);
     }
     __syncthreads();
     auto held = [&](int s) { return cu_kv[s + 1] - cu_kv[s] - (cu_q[s + 1] - cu_q[s]); };
@@ -159,13 +155,8 @@ __global__ void __launch_bounds__(PP_THREADS) paged_place(const __grid_constant_
         const int old = (held(s) + mask) >> a.page_shift;
         return i < old ? t.table[(long long)row[s] * t.max_pages + i] : t.free_pages[n_free - 1 - (first[s] + i - old)];
     };
-    const int all_pages = cu_pages[n], all_q = cu_q[n], all_kv = cu_kv[n];
+    const int all_pages = cu_pages[n], all_q = cu_q[n], all_kv = cu_kv[n], lane = tid & 31;
     const uint32_t id = blockIdx.x * PP_THREADS + tid, threads = gridDim.x * PP_THREADS;
-    for (uint32_t x = id; x < (uint32_t)all_pages; x += threads) {
-        const int s = sequence_of(cu_pages, n, x), i = x - cu_pages[s], to = page(s, i);
-        p.batch_table[(long long)s * t.max_pages + i] = to;
-        if (i >= (held(s) + mask) >> a.page_shift) t.table[(long long)row[s] * t.max_pages + i] = to;
-    }
     for (uint32_t x = id; x < (uint32_t)p.max_new; x += threads) {
         long long slot = -1;
         int pos = 0;
@@ -177,16 +168,29 @@ __global__ void __launch_bounds__(PP_THREADS) paged_place(const __grid_constant_
         p.slots[x] = slot;
         p.positions[x] = pos;
     }
-    if (p.context) {
-        // 16 lanes to a page
-        for (uint32_t x = id >> 4; x < (uint32_t)all_pages; x += threads >> 4) {
+    // a page to a lane, 32 in a row to a warp, which then writes their positions together
+    for (uint32_t base = id & ~31u; base < (uint32_t)all_pages; base += threads) {
+        const uint32_t x = base + lane;
+        int to = 0, begin = 0, count = 0;  // the page; where in the context its positions go, and how many
+        if (x < (uint32_t)all_pages) {
             const int s = sequence_of(cu_pages, n, x), i = x - cu_pages[s], len = cu_kv[s + 1] - cu_kv[s];
-            const long long slot = (long long)page(s, i) << a.page_shift;
-            for (int j = tid & 15; j <= mask && (i << a.page_shift) + j < len; j += 16) p.context[cu_kv[s] + (i << a.page_shift) + j] = slot + j;
+            to = page(s, i);
+            begin = cu_kv[s] + (i << a.page_shift);
+            count = min(t.page_size, len - (i << a.page_shift));
+            p.batch_table[(long long)s * t.max_pages + i] = to;
+            if (i >= (held(s) + mask) >> a.page_shift) t.table[(long long)row[s] * t.max_pages + i] = to;
         }
-        for (uint32_t x = all_kv + id; x < (uint32_t)p.max_context; x += threads) p.context[x] = -1;
+        if (!p.context) continue;
+        const int lanes = min(t.page_size, 32), at_once = 32 / lanes;  // of a page; pages
+        for (int k = lane / lanes; k < 32; k += at_once) {
+            const long long slot = (long long)__shfl_sync(0xffffffffu, to, k) << a.page_shift;
+            const int b = __shfl_sync(0xffffffffu, begin, k), c = __shfl_sync(0xffffffffu, count, k);
+            for (int j = lane % lanes; j < c; j += lanes) p.context[b + j] = slot + j;
+        }
     }
-    if (!ok || !last_to_read(a.counter)) return;
+    if (p.context)
+        for (uint32_t x = all_kv + id; x < (uint32_t)p.max_context; x += threads) p.context[x] = -1;
+    if (!s_last) return;
     for (int s = s0; s < s1; s++) t.cached[row[s]] = cu_kv[s + 1] - cu_kv[s];
     if (tid == 0) *t.n_free = n_free - all.taken;
 }
@@ -198,7 +202,7 @@ __global__ void __launch_bounds__(PP_THREADS) paged_trim(const __grid_constant__
     const int32_t* keep = a.p.n_new;
     int *first = smem, *from = first + n + 1, *row = from + n, *now = row + n;  // of the pages given back; the first such of a row
     uint32_t* seen = reinterpret_cast<uint32_t*>(now + n);
-    __shared__ int s_why;
+    __shared__ int s_why, s_last;
     sm100::pdl_launch_dependents();
     for (int i = tid; i < (t.n_rows + 31) / 32; i += PP_THREADS) seen[i] = 0;
     if (tid == 0) s_why = 0x7fffffff;
@@ -235,16 +239,18 @@ __global__ void __launch_bounds__(PP_THREADS) paged_trim(const __grid_constant__
     __syncthreads();
     const bool ok = s_why == 0x7fffffff;
     if (tid == 0 && blockIdx.x == 0) a.p.status[0] = ok ? (int)CFI_PLACED : s_why;
-    if (ok) {
-        for (int s = s0; s < s1; s++) first[s] += at.pages;
-        if (tid == 0) first[n] = all.pages;
-        __syncthreads();
-        for (uint32_t x = blockIdx.x * PP_THREADS + tid; x < (uint32_t)all.pages; x += gridDim.x * PP_THREADS) {
-            const int s = sequence_of(first, n, x);
-            t.free_pages[n_free + all.pages - 1 - x] = t.table[(long long)row[s] * t.max_pages + from[s] + x - first[s]];
-        }
+    if (!ok) return;
+    for (int s = s0; s < s1; s++) first[s] += at.pages;
+    if (tid == 0) {
+        first[n] = all.pages;
+        s_last = last_to_read(a.counter);
     }
-    if (!last_to_read(a.counter) || !ok) return;
+    __syncthreads();
+    for (uint32_t x = blockIdx.x * PP_THREADS + tid; x < (uint32_t)all.pages; x += gridDim.x * PP_THREADS) {
+        const int s = sequence_of(first, n, x);
+        t.free_pages[n_free + all.pages - 1 - x] = t.table[(long long)row[s] * t.max_pages + from[s] + x - first[s]];
+    }
+    if (!s_last) return;
     for (int s = s0; s < s1; s++) t.cached[row[s]] = now[s];
     if (tid == 0) *t.n_free = n_free + all.pages;
 }
