@@ -20,12 +20,13 @@ namespace {
 constexpr int NR_THREADS = 256, NR_RATES = 64;
 constexpr int NR_AT_ONCE = 2;  // heads whose loads are in flight together
 constexpr int NR_HEADS = 8, NR_MANY = 8;
+constexpr int NR_CTAS = 4;
 
 struct NrArgs {
     CfiNormRope r;
     uint8_t *k_pool, *v_pool;
     long long n_slots;
-    int page_shift, cache_type;
+    int page_shift;
     uint32_t runs;           // of a token's heads: those of q begin at 0, of k and v at begin[1] and begin[2]
     int begin[3], heads[3];  // heads of a run
     int most;                // the largest of them
@@ -72,9 +73,11 @@ CFI_DEV void turn1(float& x, float& y, float c, float s) {
     x = t;
 }
 
-template <int D, bool IN_F16, int AT_ONCE> __global__ void __launch_bounds__(NR_THREADS) norm_rope(const __grid_constant__ NrArgs a) {
+// TY: of the cache; F16 also where there is none.
+template <int D, bool IN_F16, int TY, int AT_ONCE>
+__global__ void __launch_bounds__(NR_THREADS, TY == CACHE_F16 ? NR_CTAS : 2) norm_rope(const __grid_constant__ NrArgs a) {
     constexpr int G = D / 8;  // lanes of a head
-    __shared__ float4 s_row[NR_THREADS / G][2 * G];  // a row of k or v, where the cache wants eight dims in a lane
+    __shared__ float4 s_row[TY == CACHE_F16 ? 1 : NR_THREADS / G][2 * G];  // a row of k or v, where the cache wants eight dims in a lane
     const CfiNormRope& r = a.r;
     const int lane = threadIdx.x % G, group = threadIdx.x / G;
     const int eighth = r.n_rot / 8;  // lanes that turn
@@ -99,9 +102,7 @@ template <int D, bool IN_F16, int AT_ONCE> __global__ void __launch_bounds__(NR_
     const long long slot = a.k_pool && kind != 0 ? r.slots[t] : -1;
     const bool put = live && slot >= 0 && slot < a.n_slots;
     const int off = (int)(slot & ((1 << a.page_shift) - 1));
-    const long long region_bytes = a.cache_type == CACHE_F16 ? paged_region_bytes<D, CACHE_F16>(1 << a.page_shift)
-                                   : a.cache_type == CACHE_Q8_0 ? paged_region_bytes<D, CACHE_Q8_0>(1 << a.page_shift)
-                                                                : paged_region_bytes<D, CACHE_Q4_1>(1 << a.page_shift);
+    const long long region_bytes = paged_region_bytes<D, TY>(1 << a.page_shift);
     uint8_t* region = (kind == 2 ? a.v_pool : a.k_pool) + ((slot >> a.page_shift) * r.n_kv_head + h0) * region_bytes;
     float4 w0 = make_float4(0.0f, 0.0f, 0.0f, 0.0f), w1 = w0;
     if (norm) {
@@ -166,7 +167,7 @@ template <int D, bool IN_F16, int AT_ONCE> __global__ void __launch_bounds__(NR_
             }
             if (!a.k_pool) continue;
             uint8_t* to = region + h * region_bytes;
-            if (a.cache_type == CACHE_F16) {
+            if (TY == CACHE_F16) {
                 if (put && on) {
                     *reinterpret_cast<uint2*>(to + (off * D + d0) * 2) = halves(x0);
                     *reinterpret_cast<uint2*>(to + (off * D + d1) * 2) = halves(x1);
@@ -179,7 +180,7 @@ template <int D, bool IN_F16, int AT_ONCE> __global__ void __launch_bounds__(NR_
                 __syncwarp();
                 const float4 y0 = s_row[group][2 * lane], y1 = s_row[group][2 * lane + 1];
                 const Row8 y = {{y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w}, {}};
-                if (a.cache_type == CACHE_Q8_0)
+                if (TY == CACHE_Q8_0)
                     put_q8_0<D, false>(y, to, a.page_shift, off, lane, put && on);
                 else
                     put_q4_1<D>(y, to, off, lane, kind == 2, put && on);
@@ -190,6 +191,19 @@ template <int D, bool IN_F16, int AT_ONCE> __global__ void __launch_bounds__(NR_
 
 bool rows_ok(const void* p, long long stride, long long width) { return p && !((uintptr_t)p & 15) && stride % 8 == 0 && stride >= width; }
 bool type_ok(int t) { return t == 0 || t == 1; }
+
+template <int D, bool IN_F16, int TY> const void* kernel(bool many) {
+    return many ? (const void*)norm_rope<D, IN_F16, TY, NR_AT_ONCE> : (const void*)norm_rope<D, IN_F16, TY, 1>;
+}
+template <int D, bool IN_F16> const void* kernel(int ty, bool many) {
+    return ty == CACHE_Q8_0   ? kernel<D, IN_F16, CACHE_Q8_0>(many)
+           : ty == CACHE_Q4_1 ? kernel<D, IN_F16, CACHE_Q4_1>(many)
+                              : kernel<D, IN_F16, CACHE_F16>(many);
+}
+const void* kernel_of(int head_dim, int in_type, int ty, bool many) {
+    if (head_dim == 64) return in_type ? kernel<64, true>(ty, many) : kernel<64, false>(ty, many);
+    return in_type ? kernel<128, true>(ty, many) : kernel<128, false>(ty, many);
+}
 
 // The pairs' rates in turns.
 void rates(const CfiNormRope* r, NrArgs* a) {
@@ -242,7 +256,6 @@ extern "C" int cfi_norm_rope(const CfiNormRope* r, const CfiPagedCache* c, void*
         a.v_pool = static_cast<uint8_t*>(c->v);
         a.n_slots = (long long)c->n_pages * c->page_size;
         a.page_shift = __builtin_ctz((unsigned)c->page_size);
-        a.cache_type = c->type;
     }
     if (r->n_rot) {
         rates(r, &a);
@@ -269,10 +282,6 @@ extern "C" int cfi_norm_rope(const CfiNormRope* r, const CfiPagedCache* c, void*
     at[0].val.programmaticStreamSerializationAllowed = 1;
     lc.attrs = at;
     lc.numAttrs = (ep && strcmp(ep, "0") == 0) ? 0 : 1;
-    static const void* const fns[8] = {
-        (const void*)norm_rope<64, false, 1>,  (const void*)norm_rope<64, true, 1>,  (const void*)norm_rope<64, false, NR_AT_ONCE>,
-        (const void*)norm_rope<64, true, NR_AT_ONCE>, (const void*)norm_rope<128, false, 1>, (const void*)norm_rope<128, true, 1>,
-        (const void*)norm_rope<128, false, NR_AT_ONCE>, (const void*)norm_rope<128, true, NR_AT_ONCE>};
     void* args[1] = {&a};
-    return (int)cudaLaunchKernelExC(&lc, fns[(r->head_dim == 128) * 4 + many * 2 + r->in_type], args);
+    return (int)cudaLaunchKernelExC(&lc, kernel_of(r->head_dim, r->in_type, c ? c->type : CACHE_F16, many), args);
 }
