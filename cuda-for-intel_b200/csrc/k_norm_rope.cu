@@ -32,7 +32,7 @@ struct NrArgs {
     int most;                // the largest of them
     union {
         unsigned long long turn[NR_RATES];  // of 2^64
-        double rate[NR_RATES];              // in turns, where freq_factors divide them
+        float2 rate[NR_RATES];              // in turns, the sum of two, where freq_factors divide them
     };
 };
 
@@ -71,6 +71,14 @@ CFI_DEV void turn1(float& x, float& y, float c, float s) {
     const float t = fmaf(x, c, -(y * s));
     y = fmaf(x, s, y * c);
     x = t;
+}
+
+// A rate in turns over f, as a fraction of 2^64: the quotient digit by digit, 24 bits each, with exact remainders.
+CFI_DEV unsigned long long divided(float2 rate, float f) {
+    const float inv = 1.0f / f, q0 = rate.x * inv;
+    const float r0 = fmaf(-q0, f, rate.x) + rate.y, q1 = r0 * inv, q2 = fmaf(-q1, f, r0) * inv;
+    const float two64 = 18446744073709551616.0f;
+    return __float2ull_rz((q0 - floorf(q0)) * two64) + (unsigned long long)(__float2ll_rn(q1 * two64) + __float2ll_rn(q2 * two64));
 }
 
 // TY: of the cache; F16 also where there is none.
@@ -125,13 +133,7 @@ __global__ void __launch_bounds__(NR_THREADS, TY == CACHE_F16 ? NR_CTAS : 2) nor
             const int pos = r.pos[t];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                unsigned long long f;
-                if (r.freq_factors) {
-                    const double y = a.rate[4 * lane + e] / (double)r.freq_factors[4 * lane + e];
-                    f = __double2ull_rn((y - floor(y)) * 18446744073709551616.0);
-                } else {
-                    f = a.turn[4 * lane + e];
-                }
+                const unsigned long long f = r.freq_factors ? divided(a.rate[4 * lane + e], r.freq_factors[4 * lane + e]) : a.turn[4 * lane + e];
                 const int angle = (int)((f * (unsigned long long)(long long)pos) >> 32);
                 sincospif((float)angle * 0x1p-31f, &sn[e], &cs[e]);
             }
@@ -221,7 +223,7 @@ void rates(const CfiNormRope* r, NrArgs* a) {
     for (int i = 0; i < r->n_rot / 2; i++, rate *= step) {
         const long double part = (rate - floorl(rate)) * two64;
         if (r->freq_factors)
-            a->rate[i] = (double)rate;
+            a->rate[i] = make_float2((float)rate, (float)(rate - (float)rate));
         else
             a->turn[i] = part < two64 ? (unsigned long long)part : 0;
     }
