@@ -14,6 +14,7 @@ namespace {
 // (6.2 TB/s of reads and writes) and 80 us; storing 8192 rows 12.7, 12.7 and 13.8 us (10.3, 5 TB/s, since the maximum of f16
 // rows is taken in f16 and the bytes come from one conversion: it is bound by issue), a step's 48 rows 1.2, 1.5 and 1.9.
 constexpr int PC_THREADS = 256, PC_STORE_ITEMS = 1, PC_LOAD_ITEMS = 2;
+constexpr int PC_Q4_ITEMS = 1;
 
 struct PcArgs {
     uint8_t *k, *v;          // pools
@@ -124,15 +125,7 @@ __global__ void __launch_bounds__(PC_THREADS) paged_kv_load(const PcArgs a) {
             if (!p[e].ok(a)) continue;
             const uint8_t* region = (kv ? a.v : a.k) + p[e].template region<TY>(a);
             const int off = p[e].off(a);
-            if (TY == CACHE_Q4_1) {
-                const int row = off % Q41_TILE, b = p[e].g >> 2, c = p[e].g & 3;
-                const uint8_t* tile = region + Q41<D>::tile_at(off);
-                in[e][kv].x = kv ? *reinterpret_cast<const uint16_t*>(tile + Q41<D>::v_at(row, b, 2 * c)) |
-                                       (uint32_t)*reinterpret_cast<const uint16_t*>(tile + Q41<D>::v_at(row, b, 2 * c + 1)) << 16
-                                 : *reinterpret_cast<const uint32_t*>(tile + Q41<D>::k_at(row, b, c));
-                scale[e][kv] = *reinterpret_cast<const uint16_t*>(tile + Q41<D>::scale_at(row, b)) |
-                               (uint32_t)*reinterpret_cast<const uint16_t*>(tile + Q41<D>::min_at(row, b)) << 16;
-            } else if (TY == CACHE_Q8_0) {
+            if (TY == CACHE_Q8_0) {
                 const uint2 q = ldg_stream2(region + (size_t)off * D + p[e].g * 8);
                 in[e][kv].x = q.x;
                 in[e][kv].y = q.y;
@@ -147,15 +140,7 @@ __global__ void __launch_bounds__(PC_THREADS) paged_kv_load(const PcArgs a) {
 #pragma unroll
         for (int kv = 0; kv < 2; kv++) {
             uint4 out = in[e][kv];
-            if (TY == CACHE_Q4_1) {
-                const float d = h2f_bits((uint16_t)scale[e][kv]), m = h2f_bits((uint16_t)(scale[e][kv] >> 16));
-                __half2* o = reinterpret_cast<__half2*>(&out);
-                const uint32_t w = in[e][kv].x;
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    o[j] = __floats2half2_rn(fmaf(d, (float)(w >> (8 * j) & 15), m), fmaf(d, (float)(w >> (8 * j + 4) & 15), m));
-                // a slot outside the pool: zeros
-            } else if (TY == CACHE_Q8_0) {
+            if (TY == CACHE_Q8_0) {
                 const float d = h2f_bits((uint16_t)scale[e][kv]);
                 __half2* o = reinterpret_cast<__half2*>(&out);
                 const uint32_t w[2] = {in[e][kv].x, in[e][kv].y};
@@ -167,6 +152,66 @@ __global__ void __launch_bounds__(PC_THREADS) paged_kv_load(const PcArgs a) {
             }
             if (p[e].in) *reinterpret_cast<uint4*>((kv ? a.dst_v : a.dst_k) + p[e].value(kv ? a.v_stride : a.k_stride) * 2) = out;
         }
+}
+
+// Q4_1: an item is what lies together in a row, dims 8 c .. 8 c + 7 of all its blocks, of K and of V.
+template <int D> __global__ void __launch_bounds__(PC_THREADS) paged_kv_load_q4_1(const PcArgs a) {
+    using L = Q41<D>;
+    constexpr int NB = D / 32, WORDS = D / 32;  // words of nibbles: block b's dims (V: its first four, then its last four in the upper halves)
+    sm100::pdl_launch_dependents();
+    sm100::pdl_wait();
+    const uint32_t base = blockIdx.x * (PC_THREADS * PC_Q4_ITEMS) + threadIdx.x;
+    uint32_t w[PC_Q4_ITEMS][2][WORDS], m[PC_Q4_ITEMS][2][NB];  // nibbles; scales, then minima
+    long long slot[PC_Q4_ITEMS];
+    uint32_t t[PC_Q4_ITEMS], h[PC_Q4_ITEMS];
+    const int c = threadIdx.x & 3;
+#pragma unroll
+    for (int e = 0; e < PC_Q4_ITEMS; e++) {
+        const uint32_t i = base + e * PC_THREADS, row = (i < a.n_items ? i : a.n_items - 1) / 4;
+        t[e] = row / a.n_kv_head;
+        h[e] = row - t[e] * a.n_kv_head;
+        slot[e] = a.slots[t[e]];
+    }
+#pragma unroll
+    for (int e = 0; e < PC_Q4_ITEMS; e++) {
+        const bool ok = slot[e] >= 0 && slot[e] < a.n_slots;
+        const int off = (int)(slot[e] & ((1 << a.page_shift) - 1)), row = off % Q41_TILE;
+        const long long tile = ((slot[e] >> a.page_shift) * a.n_kv_head + h[e]) * paged_region_bytes<D, CACHE_Q4_1>(1 << a.page_shift) + L::tile_at(off);
+#pragma unroll
+        for (int kv = 0; kv < 2; kv++) {
+            const uint8_t* p = (kv ? a.v : a.k) + tile;
+            const uint8_t *q = p + (kv ? L::v_at(row, 0, 2 * c) : L::k_at(row, 0, c)), *r = p + L::scale_at(row, 0);
+            if (D == 128) {
+                const uint4 x = ok ? ldg_stream(q) : make_uint4(0, 0, 0, 0), y = ok ? *reinterpret_cast<const uint4*>(r) : make_uint4(0, 0, 0, 0);
+                w[e][kv][0] = x.x, w[e][kv][1] = x.y, w[e][kv][WORDS - 2] = x.z, w[e][kv][WORDS - 1] = x.w;
+                m[e][kv][0] = y.x, m[e][kv][1] = y.y, m[e][kv][NB - 2] = y.z, m[e][kv][NB - 1] = y.w;
+            } else {
+                const uint2 x = ok ? ldg_stream2(q) : make_uint2(0, 0), y = ok ? *reinterpret_cast<const uint2*>(r) : make_uint2(0, 0);
+                w[e][kv][0] = x.x, w[e][kv][1] = x.y;
+                m[e][kv][0] = y.x, m[e][kv][1] = y.y;
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < PC_Q4_ITEMS; e++) {
+        if (base + e * PC_THREADS >= a.n_items) continue;
+#pragma unroll
+        for (int kv = 0; kv < 2; kv++) {
+            uint8_t* to = (kv ? a.dst_v : a.dst_k) + ((long long)t[e] * (kv ? a.v_stride : a.k_stride) + h[e] * D + 8 * c) * 2;
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const float d = h2f_bits((uint16_t)(m[e][kv][b >> 1] >> (16 * (b & 1)))), low = h2f_bits((uint16_t)(m[e][kv][(NB + b) >> 1] >> (16 * (b & 1))));
+                // V: the lane's two groups of four dims, NB half-words each
+                const uint32_t x = kv ? __byte_perm(w[e][kv][b >> 1], w[e][kv][WORDS / 2 + (b >> 1)], b & 1 ? 0x7632 : 0x5410) : w[e][kv][b];
+                uint4 out;
+                __half2* o = reinterpret_cast<__half2*>(&out);
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    o[j] = __floats2half2_rn(fmaf(d, (float)(x >> (8 * j) & 15), low), fmaf(d, (float)(x >> (8 * j + 4) & 15), low));
+                *reinterpret_cast<uint4*>(to + 64 * b) = out;
+            }
+        }
+    }
 }
 
 int go(const void* fn, const PcArgs& a, int items, cudaStream_t stream) {
@@ -243,8 +288,12 @@ extern "C" int cfi_paged_kv_load(const CfiPagedCache* c, const int64_t* slots, v
     if (n_tokens == 0) return 0;
     a.dst_k = static_cast<uint8_t*>(k);
     a.dst_v = static_cast<uint8_t*>(v);
-    static const void* const fns[6] = {
-        (const void*)paged_kv_load<64, CACHE_F16>,  (const void*)paged_kv_load<64, CACHE_Q8_0>,  (const void*)paged_kv_load<64, CACHE_Q4_1>,
-        (const void*)paged_kv_load<128, CACHE_F16>, (const void*)paged_kv_load<128, CACHE_Q8_0>, (const void*)paged_kv_load<128, CACHE_Q4_1>};
-    return go(fns[(c->head_dim == 128) * 3 + type_at(c)], a, PC_LOAD_ITEMS, static_cast<cudaStream_t>(stream));
+    if (c->type == CACHE_Q4_1) {
+        a.n_items = a.n_items / (c->head_dim / 8) * 4;
+        return go(c->head_dim == 128 ? (const void*)paged_kv_load_q4_1<128> : (const void*)paged_kv_load_q4_1<64>, a, PC_Q4_ITEMS,
+                  static_cast<cudaStream_t>(stream));
+    }
+    static const void* const fns[4] = {(const void*)paged_kv_load<64, CACHE_F16>, (const void*)paged_kv_load<64, CACHE_Q8_0>,
+                                       (const void*)paged_kv_load<128, CACHE_F16>, (const void*)paged_kv_load<128, CACHE_Q8_0>};
+    return go(fns[(c->head_dim == 128) * 2 + type_at(c)], a, PC_LOAD_ITEMS, static_cast<cudaStream_t>(stream));
 }
