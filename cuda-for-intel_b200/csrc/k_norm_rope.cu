@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(NR_THREADS, TY == CACHE_F16 ? NR_CTAS : 2) nor
                 if (TY == CACHE_Q8_0)
                     put_q8_0<D, false>(y, to, a.page_shift, off, lane, put && on);
                 else
-                    put_q4_1<D>(y, to, off, lane, kind == 2, put && on);
+                    put_q4_1<D, false>(y, to, off, lane, kind == 2, put && on);
             }
         }
     }

@@ -3,8 +3,9 @@
 //
 // Q8_0: d = max|x| / 127, q = rn(x * (1/d)), stored scale f16(d); read back as f16(q * scale).
 // Q4_1: d = (max - min) / 15, q = floor((x - min) / d + 1/2), stored f16(d) and f16(min), all rounded from the exact values.  The
-// quotient in 32 bits is off by less than 2^-17, d by 2 units of its last place: only a lane whose values come nearer to a border
-// than that (one in a thousand) works them out in 64 bits, where differences and products of f32 values are exact.
+// quotient in 32 bits is off by less than 2^-16 (2^-24 of it each by range and difference, 2^-22 by the quotient), d by 2 units of its
+// last place: only a lane whose values come nearer to a border than that (one in a thousand) works them out in 64 bits, where
+// differences and products of f32 values are exact.
 #pragma once
 #include "paged_cache.cuh"
 
@@ -65,31 +66,64 @@ template <int D, bool SRC_F16> CFI_DEV void put_q8_0(const Row8& r, uint8_t* reg
             d != d ? (uint16_t)0x7fff : f2h_bits(d);
 }
 
-template <int D> CFI_DEV void put_q4_1(const Row8& r, uint8_t* region, int off, int g, bool of_v, bool ok) {
-    float lo = r.x[0], hi = r.x[0], zero = 0.0f;
+CFI_DEV float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+CFI_DEV float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// The least and the largest of a block; both NaN where it has one.
+template <bool SRC_F16> CFI_DEV void block_ends(const Row8& r, float* lo, float* hi) {
+    if (SRC_F16) {
+        const __half2 *h = reinterpret_cast<const __half2*>(&r.h);
+        const __half2 a = __hmin2_nan(__hmin2_nan(h[0], h[1]), __hmin2_nan(h[2], h[3])), b = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+        // the negative of the least beside the largest
+        __half2 e = __hmax2_nan(__halves2half2(__hneg(__low2half(a)), __low2half(b)), __halves2half2(__hneg(__high2half(a)), __high2half(b)));
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        lo = fminf(lo, r.x[j]);
-        hi = fmaxf(hi, r.x[j]);
-        zero = fmaf(r.x[j], 0.0f, zero);  // NaN where one is not finite
-    }
+        for (int o = 1; o < 4; o <<= 1) e = __hmax2_nan(e, __shfl_xor_sync(0xffffffffu, e, o));
+        *lo = -__low2float(e);
+        *hi = __high2float(e);
+    } else {
+        float a = r.x[0], b = r.x[0];
 #pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        zero += __shfl_xor_sync(0xffffffffu, zero, o);
+        for (int j = 1; j < 8; j++) {
+            a = min_nan(a, r.x[j]);
+            b = max_nan(b, r.x[j]);
+        }
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+            a = min_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
+            b = max_nan(b, __shfl_xor_sync(0xffffffffu, b, o));
+        }
+        *lo = a;
+        *hi = b;
     }
-    const float range = hi - lo, inv = 15.0f / range, d32 = range * (1.0f / 15.0f);
+}
+
+template <int D, bool SRC_F16> CFI_DEV void put_q4_1(const Row8& r, uint8_t* region, int off, int g, bool of_v, bool ok) {
+    float lo, hi;
+    block_ends<SRC_F16>(r, &lo, &hi);
+    const float range = hi - lo, inv = __fdividef(15.0f, range), d32 = range * (1.0f / 15.0f);
     // slow: d at a border of f16, where it is below its normal numbers, or 32 bits do not hold the quotients
     const uint32_t below = (__float_as_uint(d32) & 0x1fffu) - 0x0ffcu;
     bool slow = below <= 8u || !(d32 >= 6.2e-5f && d32 <= 6.0e4f);
-    uint32_t w = 0;
+    // v + 1.5 * 2^23 is rounded to a whole number, whose last bits are q: with each times 16 and the next, the rest adds up to
+    // a number of its own
+    uint32_t w = 0, rest = 0;
+    float far = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const float t = fmaf(r.x[j] - lo, inv, 0.5f), f = floorf(t);
-        slow |= fabsf(t - f - 0.5f) > 0.49998f;
-        w |= (uint32_t)(int)f << (4 * j);
+    for (int j = 7; j >= 0; j--) {
+        const float v = (r.x[j] - lo) * inv, y = v + 12582912.0f;
+        far = fmaxf(far, fabsf(v - (y - 12582912.0f)));
+        w = w * 16 + __float_as_uint(y);
+        rest = rest * 16 + 0x4b400000u;
     }
+    w -= rest;
+    slow |= far > 0.49998f;
     uint16_t d = f2h_bits(d32);
     if (slow) {
         const double wide = (double)hi - (double)lo;
@@ -101,7 +135,7 @@ template <int D> CFI_DEV void put_q4_1(const Row8& r, uint8_t* region, int off, 
         }
     }
     uint16_t m = f2h_bits(lo);
-    if (zero != 0.0f || (d & 0x7c00) == 0x7c00 || (m & 0x7c00) == 0x7c00) {
+    if ((d & 0x7c00) == 0x7c00 || (m & 0x7c00) == 0x7c00) {
         d = m = 0x7fff;
         w = 0;
     }
@@ -125,6 +159,6 @@ CFI_DEV void put_row8(const Row8& r, uint8_t* region, int page_shift, int off, i
     } else if (TY == CACHE_Q8_0) {
         put_q8_0<D, SRC_F16>(r, region, page_shift, off, g, ok);
     } else {
-        put_q4_1<D>(r, region, off, g, of_v, ok);
+        put_q4_1<D, SRC_F16>(r, region, off, g, of_v, ok);
     }
 }
