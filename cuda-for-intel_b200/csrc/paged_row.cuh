@@ -3,9 +3,10 @@
 //
 // Q8_0: d = max|x| / 127, q = rn(x * (1/d)), stored scale f16(d); read back as f16(q * scale).
 // Q4_1: d = (max - min) / 15, q = floor((x - min) / d + 1/2), stored f16(d) and f16(min), all rounded from the exact values.  The
-// quotient in 32 bits is off by less than 2^-16 (2^-24 of it each by range and difference, 2^-22 by the quotient), d by 2 units of its
-// last place: only a lane whose values come nearer to a border than that (one in a thousand) works them out in 64 bits, where
-// differences and products of f32 values are exact.
+// quotient in 32 bits is off by less than 2^-16 (2^-24 of it each by range and difference, 2^-22 by the quotient): where a value of a
+// warp comes nearer to a border than that, its values are compared with their borders, 30 (x - min) with (2 q + 1) (max - min), as sums of
+// two f32 numbers each (differences of f16 values meet borders exactly).  d is off by 2 units of its last place in 32 bits and worked out
+// in 64 where a border of f16 is nearer.
 #pragma once
 #include "paged_cache.cuh"
 
@@ -108,9 +109,8 @@ template <int D, bool SRC_F16> CFI_DEV void put_q4_1(const Row8& r, uint8_t* reg
     float lo, hi;
     block_ends<SRC_F16>(r, &lo, &hi);
     const float range = hi - lo, inv = __fdividef(15.0f, range), d32 = range * (1.0f / 15.0f);
-    // slow: d at a border of f16, where it is below its normal numbers, or 32 bits do not hold the quotients
-    const uint32_t below = (__float_as_uint(d32) & 0x1fffu) - 0x0ffcu;
-    bool slow = below <= 8u || !(d32 >= 6.2e-5f && d32 <= 6.0e4f);
+    // d at a border of f16; d outside its normal numbers, where 32 bits do not hold the quotients either
+    const bool wide = !(d32 >= 6.2e-5f && d32 <= 6.0e4f), tie = (__float_as_uint(d32) & 0x1fffu) - 0x0ffcu <= 8u;
     // v + 1.5 * 2^23 is rounded to a whole number, whose last bits are q: with each times 16 and the next, the rest adds up to
     // a number of its own
     uint32_t w = 0, rest = 0;
@@ -123,15 +123,27 @@ template <int D, bool SRC_F16> CFI_DEV void put_q4_1(const Row8& r, uint8_t* reg
         rest = rest * 16 + 0x4b400000u;
     }
     w -= rest;
-    slow |= far > 0.49998f;
-    uint16_t d = f2h_bits(d32);
-    if (slow) {
-        const double wide = (double)hi - (double)lo;
-        d = __half_as_ushort(__double2half(wide / 15.0));
+    if (far > 0.49998f && !wide) {  // often, where the values are f16 numbers
+        const float rb = range - hi, range_lo = (hi - (range - rb)) - (lo + rb);  // what the difference was rounded by
         w = 0;
-        if (wide > 0.0) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) w |= (uint32_t)(int)floor(((double)r.x[j] - (double)lo) * 15.0 / wide + 0.5) << (4 * j);
+        for (int j = 0; j < 8; j++) {
+            const float t = r.x[j] - lo, tb = t - r.x[j], t_lo = (r.x[j] - (t - tb)) - (lo + tb);
+            const float v = t * inv, near = (v + 12582912.0f) - 12582912.0f;
+            const float twice = 2.0f * near + (v >= near ? 1.0f : -1.0f), p = twice * range;  // of the border that is next
+            const float over = (fmaf(30.0f, t, -p) - fmaf(twice, range, -p)) + fmaf(30.0f, t_lo, -twice * range_lo);
+            w |= (uint32_t)((int)(twice + (over >= 0.0f ? 1.0f : -1.0f)) >> 1) << (4 * j);
+        }
+    }
+    uint16_t d = f2h_bits(d32);
+    if (wide || tie) {
+        const double exact = (double)hi - (double)lo;
+        d = __half_as_ushort(__double2half(exact / 15.0));
+        if (wide) {
+            w = 0;
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                w |= exact > 0.0 ? (uint32_t)(int)floor(((double)r.x[j] - (double)lo) * 15.0 / exact + 0.5) << (4 * j) : 0;
         }
     }
     uint16_t m = f2h_bits(lo);
