@@ -3,14 +3,18 @@ architecture, Q8_0; random, or those of a GGUF file through decode.load_gguf).
 
 A prompt of any length goes through the stack packed with the others of its batch, one token of each
 running sequence steps together, and tokens are sampled on the device (include/cfi_serve.h): the rows
-of K and V go into the pages of one cache per layer, in f16 or quantised to Q8_0 as they are written;
-a prompt reads its whole context back as f16 rows and attends causally; a step attends over the pages.
+of K and V go into the pages of one cache per layer, in f16 or quantised to Q8_0 or Q4_1 as they are
+written; a prompt reads its whole context back as f16 rows and attends causally; a step attends over the pages.
 Products run through the substituted quantize_mmq_q8_1 and mul_mat_q, norms and rope through rms_norm
-and rope_neox; biases, SwiGLU, residuals and the embedding rows are torch's.
+and rope_neox, or biases, norms of the heads, rope and the cache's rows through one cfi_norm_rope; who owns
+which page is kept on the host or, by cfi_paged_place, on the device; SwiGLU, residuals and the embedding
+rows are torch's.
 
-    python serve.py [--cache f16|q8_0] [--batch 8] [--new 32] [--layers 4] [--file model.gguf]
+    python serve.py [--cache f16|q8_0|q4_1] [--batch 8] [--new 32] [--layers 4] [--file model.gguf] [--fused] [--norms]
+                    [--tables host|device]
 """
 import math
+from types import SimpleNamespace
 
 import cfi_b200 as cfi
 
@@ -29,17 +33,24 @@ class Sequence:
     def __init__(self, tokens, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         self.tokens = [int(t) for t in tokens]
         self.prompt = len(self.tokens)
-        self.pages = []
+        self.pages = []  # where the tables are the host's
+        self.row = None  # of the device's table
         self.cached = 0
         self.temperature, self.top_k, self.top_p, self.min_p = temperature, top_k, top_p, min_p
 
 
 class Server:
     """`model`: a DecodeModel (its weights are used, its own caches are not); `pages` pages of
-    `page_size` positions are shared by all sequences; cache_type cfi.T_F16 or cfi.Q8_0.  Each call works on the
-    stream that is torch's current one then, after what the calls before it did on theirs."""
+    `page_size` positions are shared by all sequences; cache_type cfi.T_F16, cfi.Q8_0 or cfi.Q4_1.  Each call works on the
+    stream that is torch's current one then, after what the calls before it did on theirs.
 
-    def __init__(self, torch, ctx, model, cache_type=cfi.T_F16, page_size=16, pages=256, seed=0):
+    fused: biases, rope and the rows into the cache by one cfi_norm_rope a layer (its angles are right at any position; those of
+    rope_neox are in 32 bits).  None: where the cache is Q4_1 or there are norms.  norms: of each layer the weights (f32, head_dim)
+    that the heads of q and of k are normed with, for models that have them.
+    tables: "host", or "device" for page tables that cfi_paged_place keeps, for up to `rows` sequences at a time."""
+
+    def __init__(self, torch, ctx, model, cache_type=cfi.T_F16, page_size=16, pages=256, seed=0, fused=None, norms=None, tables="host",
+                 rows=64):
         self.t, self.m, self.c = torch, model, model.cfg
         self.dev = model.dev
         self.g = cfi.GgmlCaller(ctx, "all")
@@ -48,11 +59,26 @@ class Server:
         n = cfi.paged_page_bytes(cache_type, page_size, c.n_kv_head, c.head_dim)
         if n == 0:
             raise ValueError("no paged cache of type %d with pages of %d and heads of %d" % (cache_type, page_size, c.head_dim))
+        if norms is not None and (len(norms) != len(model.layers) or fused is False):
+            raise ValueError("norms are two vectors for each layer of a fused server")
+        if tables not in ("host", "device"):
+            raise ValueError("tables are the host's or the device's")
+        self.norms = norms
+        self.fused = cache_type == cfi.Q4_1 or norms is not None if fused is None else fused
         # the pools, [layer][K or V][page]: a program keeps the description of each beside them
         self.pools = torch.zeros(c.layers, 2, pages * n, dtype=torch.uint8, device=self.dev)
         self.caches = [cfi.paged_cache(cache_type, p[0].data_ptr(), p[1].data_ptr(), pages, page_size, c.n_kv_head, c.head_dim)
                        for p in self.pools]
-        self.free = list(range(pages))[::-1]
+        self.free = list(range(pages))[::-1]  # where the tables are the host's
+        self.held = [self.pools]
+        self.on_device = tables == "device"
+        if self.on_device:
+            self.n_free, self.rows = pages, list(range(rows))[::-1]  # of which the host keeps count alone
+            state = dict(table=torch.zeros(rows, pages, dtype=torch.int32, device=self.dev), cached=self._int([0] * rows),
+                         free=self._int(self.free), n_free=self._int([pages]), status=self._int([0]))
+            self.state = SimpleNamespace(**state)
+            self.held += state.values()
+            self.table = cfi.page_table(*(state[x].data_ptr() for x in ("table", "cached", "free", "n_free")), rows, pages, page_size, pages)
         self.gen = torch.Generator(device=self.dev)
         self.gen.manual_seed(seed)
         self.last = torch.cuda.current_stream()  # that of the last call
@@ -64,24 +90,109 @@ class Server:
         now = self.t.cuda.current_stream()
         if now != self.last:
             now.wait_stream(self.last)
-            self.pools.record_stream(now)
+            for x in self.held:
+                x.record_stream(now)
             self.last, self.stream = now, now.cuda_stream
         for x in given:
             x.record_stream(now)
 
     # ---- pages ----
+    def _pages(self, positions):
+        return -(-positions // self.page_size)
+
     def _grow(self, seqs, lengths):
         """Pages for the sequences' positions below `lengths`: all of them, or none are taken."""
-        need = [-(-n // self.page_size) - len(s.pages) for s, n in zip(seqs, lengths)]
+        if self.on_device:
+            need = sum(self._pages(n) - self._pages(s.cached) for s, n in zip(seqs, lengths))
+            if need > self.n_free:
+                raise OutOfPages("%d pages are free" % self.n_free)
+            fresh = [s for s in seqs if s.row is None]
+            if len(fresh) > len(self.rows):
+                raise OutOfPages("%d rows of the page table are free" % len(self.rows))
+            for s in fresh:
+                s.row = self.rows.pop()
+            self.n_free -= need
+            return
+        need = [self._pages(n) - len(s.pages) for s, n in zip(seqs, lengths)]
         if sum(x for x in need if x > 0) > len(self.free):
             raise OutOfPages("%d pages are free" % len(self.free))
         for s, x in zip(seqs, need):
             s.pages += [self.free.pop() for _ in range(x)]
 
+    def _shrink(self, seqs, lengths):
+        """The pages behind the sequences' first lengths[i] positions go back."""
+        lengths = [min(s.cached, max(n, 0)) for s, n in zip(seqs, lengths)]
+        if self.on_device:
+            mine = [(s, n) for s, n in zip(seqs, lengths) if s.row is not None]
+            if mine:
+                rows, keep, status = self._int([s.row for s, _ in mine]), self._int([n for _, n in mine]), self._int([0])
+                cfi.paged_trim(self.table, rows.data_ptr(), keep.data_ptr(), len(mine), status.data_ptr(), stream=self.stream)
+                self.state.status |= status
+            self.n_free += sum(self._pages(s.cached) - self._pages(n) for s, n in mine)
+        else:
+            for s, n in zip(seqs[::-1], lengths[::-1]):
+                while len(s.pages) > self._pages(n):
+                    self.free.append(s.pages.pop())
+        for s, n in zip(seqs, lengths):
+            s.cached = n
+
+    def cut(self, seqs, lengths):
+        """The sequences keep their first lengths[i] tokens and what is cached of them (drafted tokens that were not taken, say): the
+        pages behind go back."""
+        if len({id(s) for s in seqs}) < len(seqs):
+            raise ValueError("a sequence is named twice")
+        self._begin()
+        self._shrink(seqs, lengths)
+        for s, n in zip(seqs, lengths):
+            del s.tokens[max(n, 0):]
+            s.prompt = min(s.prompt, len(s.tokens))
+
     def release(self, seq):
         """The sequence's pages go back; its tokens stay."""
-        self.free += seq.pages[::-1]
-        seq.pages, seq.cached = [], 0
+        if not self.on_device:
+            self.free += seq.pages[::-1]
+            seq.pages, seq.cached = [], 0
+            return
+        self._begin()
+        self._shrink([seq], [0])
+        if seq.row is not None:
+            self.rows.append(seq.row)
+            seq.row = None
+
+    def _placed(self, seqs, ends, with_context):
+        """Where the sequences' tokens from what is cached to `ends` go: slots and positions of the new ones, lengths and pages, and, for
+        prompts, the packed offsets and the slots of whole contexts."""
+        t, n = self.t, len(seqs)
+        self._grow(seqs, ends)
+        p = SimpleNamespace(tokens=sum(e - s.cached for s, e in zip(seqs, ends)), positions=sum(ends), width=max(map(self._pages, ends), default=0))
+        if self.on_device:
+            i32 = lambda k: t.empty(k, dtype=t.int32, device=self.dev)  # noqa: E731
+            p.width = self.pages
+            p.rows, p.new = self._int([s.row for s in seqs]), self._int([e - s.cached for s, e in zip(seqs, ends)])
+            p.lens, p.table, p.cu_q, p.cu_k, p.pos, status = i32(n), i32(n * self.pages), i32(n + 1), i32(n + 1), i32(p.tokens), i32(1)
+            p.slots = t.empty(p.tokens, dtype=t.int64, device=self.dev)
+            p.context = t.empty(p.positions if with_context else 0, dtype=t.int64, device=self.dev)
+            batch = cfi.page_batch(p.rows.data_ptr(), p.new.data_ptr(), n, p.lens.data_ptr(), p.table.data_ptr(), p.cu_q.data_ptr(),
+                                   p.cu_k.data_ptr(), p.slots.data_ptr(), p.pos.data_ptr(), p.tokens, status.data_ptr(),
+                                   context=p.context.data_ptr() if with_context else 0, max_context=p.positions if with_context else 0)
+            cfi.paged_place(self.table, batch, stream=self.stream)
+            self.state.status |= status
+            return p
+        slots, positions, context, cu_q, cu_k = [], [], [], [0], [0]
+        for s, e in zip(seqs, ends):
+            slots += self._slots(s, s.cached, e)
+            positions += range(s.cached, e)
+            cu_q.append(len(slots))
+            if with_context:
+                context += self._slots(s, 0, e)
+                cu_k.append(len(context))
+        p.slots, p.pos = self._int(slots, t.int64), self._int(positions)
+        if with_context:
+            p.cu_q, p.cu_k, p.context = self._int(cu_q), self._int(cu_k), self._int(context, t.int64)
+        else:
+            p.table = self._int([s.pages + [0] * (p.width - len(s.pages)) for s in seqs])
+            p.lens = self._int(ends)
+        return p
 
     def _slots(self, seq, first, end):
         p = self.page_size
@@ -116,23 +227,36 @@ class Server:
         d = b[..., :2].contiguous().view(self.t.float16).float()
         return (b[..., 2:].contiguous().view(self.t.int8).float() * d).reshape(len(tokens), self.c.hidden)
 
-    def _run(self, tokens, positions, new_slots, attend, last):
+    def _rows(self, i, lay, x, placed, q_type):
+        """Layer i's rows of q, and those of k and v in its cache."""
+        t, c = self.t, self.c
+        nq, nkv, n = c.n_head * c.head_dim, c.n_kv_head * c.head_dim, x.shape[0]
+        width = nq + 2 * nkv
+        qkv = self._product(lay["wqkv"], self._norm(x, lay["attn_norm"]), width)
+        if self.fused:
+            out = t.empty(n, nq, dtype=t.float16 if q_type == cfi.T_F16 else t.float32, device=self.dev)
+            at, bias = qkv.data_ptr(), lay["bqkv"].data_ptr()
+            norm = [w.data_ptr() for w in self.norms[i]] if self.norms else [0, 0]
+            cfi.norm_rope(cfi.norm_rope_rows(at, out.data_ptr(), placed.pos.data_ptr(), n, c.n_head, c.head_dim, k=at + 4 * nq, v=at + 4 * (nq + nkv),
+                                             n_kv_head=c.n_kv_head, slots=placed.slots.data_ptr(), q_out_type=q_type, q_bias=bias,
+                                             k_bias=bias + 4 * nq, v_bias=bias + 4 * (nq + nkv), q_norm=norm[0], k_norm=norm[1], eps=c.eps,
+                                             freq_base=c.theta, q_stride=width, k_stride=width, v_stride=width), self.caches[i], stream=self.stream)
+            return out
+        qkv = qkv + lay["bqkv"]
+        q = self._rope(qkv[:, :nq].contiguous(), c.n_head, placed.pos)
+        k = self._rope(qkv[:, nq:nq + nkv].contiguous(), c.n_kv_head, placed.pos)
+        # V is read in place, a slice of the stacked rows
+        cfi.paged_kv_store(self.caches[i], k.data_ptr(), qkv.data_ptr() + 4 * (nq + nkv), placed.slots.data_ptr(), n, v_stride=width,
+                           stream=self.stream)
+        return q.half() if q_type == cfi.T_F16 else q
+
+    def _run(self, tokens, placed, q_type, attend, last):
         """The layers over packed tokens; attend(layer, q) after the layer's rows are stored.  Logits of
         the rows `last`."""
         t, c = self.t, self.c
-        nq, nkv = c.n_head * c.head_dim, c.n_kv_head * c.head_dim
-        width = nq + 2 * nkv
         x = self._embed(tokens)
-        pos = self._int(positions)
-        slots = self._int(new_slots, t.int64)
         for i, lay in enumerate(self.m.layers):
-            qkv = self._product(lay["wqkv"], self._norm(x, lay["attn_norm"]), width) + lay["bqkv"]
-            q = self._rope(qkv[:, :nq].contiguous(), c.n_head, pos)
-            k = self._rope(qkv[:, nq:nq + nkv].contiguous(), c.n_kv_head, pos)
-            # V is read in place, a slice of the stacked rows
-            cfi.paged_kv_store(self.caches[i], k.data_ptr(), qkv.data_ptr() + 4 * (nq + nkv), slots.data_ptr(), len(tokens),
-                               v_stride=width, stream=self.stream)
-            x = x + self._product(lay["wo"], attend(i, q), c.hidden)
+            x = x + self._product(lay["wo"], attend(i, self._rows(i, lay, x, placed, q_type)), c.hidden)
             gu = self._product(lay["wgu"], self._norm(x, lay["ffn_norm"]), 2 * c.ffn)
             x = x + self._product(lay["wd"], t.nn.functional.silu(gu[:, :c.ffn]) * gu[:, c.ffn:], c.hidden)
         x = x[self._int(last, t.int64)].contiguous()
@@ -146,28 +270,22 @@ class Server:
         ends = [len(s.tokens) if upto is None else min(upto[i], len(s.tokens)) for i, s in enumerate(seqs)]
         if any(e <= s.cached for s, e in zip(seqs, ends)):
             raise ValueError("a sequence has no token to run")
-        self._grow(seqs, ends)
-        tokens, positions, new, context, cu_q, cu_k = [], [], [], [], [0], [0]
+        p = self._placed(seqs, ends, True)
+        tokens, last = [], []
         for s, e in zip(seqs, ends):
             tokens += s.tokens[s.cached:e]
-            positions += range(s.cached, e)
-            new += self._slots(s, s.cached, e)
-            context += self._slots(s, 0, e)
-            cu_q.append(len(tokens))
-            cu_k.append(len(context))
-        dq, dk, slots = self._int(cu_q), self._int(cu_k), self._int(context, t.int64)
-        kv = t.empty(2, len(context), c.n_kv_head * c.head_dim, dtype=t.float16, device=self.dev)
+            last.append(len(tokens) - 1)
+        kv = t.empty(2, p.positions, c.n_kv_head * c.head_dim, dtype=t.float16, device=self.dev)
         out = t.empty(len(tokens), c.n_head * c.head_dim, device=self.dev)
 
         def attend(i, q):
-            q16 = q.half()
-            cfi.paged_kv_load(self.caches[i], slots.data_ptr(), kv[0].data_ptr(), kv[1].data_ptr(), len(context), stream=self.stream)
-            cfi.packed_attention(q16.data_ptr(), kv[0].data_ptr(), kv[1].data_ptr(), out.data_ptr(), dq.data_ptr(), dk.data_ptr(),
-                                 len(seqs), len(tokens), len(context), c.n_head, c.n_kv_head, c.head_dim, 1.0 / math.sqrt(c.head_dim),
+            cfi.paged_kv_load(self.caches[i], p.context.data_ptr(), kv[0].data_ptr(), kv[1].data_ptr(), p.positions, stream=self.stream)
+            cfi.packed_attention(q.data_ptr(), kv[0].data_ptr(), kv[1].data_ptr(), out.data_ptr(), p.cu_q.data_ptr(), p.cu_k.data_ptr(),
+                                 len(seqs), len(tokens), p.positions, c.n_head, c.n_kv_head, c.head_dim, 1.0 / math.sqrt(c.head_dim),
                                  stream=self.stream)
             return out
 
-        logits = self._run(tokens, positions, new, attend, [x - 1 for x in cu_q[1:]])
+        logits = self._run(tokens, p, cfi.T_F16, attend, last)
         for s, e in zip(seqs, ends):
             s.cached = e
         return logits
@@ -178,19 +296,15 @@ class Server:
         t, c = self.t, self.c
         if any(s.cached != len(s.tokens) - 1 for s in seqs):
             raise ValueError("a step runs exactly the last token of each sequence")
-        self._grow(seqs, [len(s.tokens) for s in seqs])
-        width = max(len(s.pages) for s in seqs)
-        table = self._int([s.pages + [0] * (width - len(s.pages)) for s in seqs])
-        lens = self._int([len(s.tokens) for s in seqs])
+        p = self._placed(seqs, [len(s.tokens) for s in seqs], False)
         out = t.empty(len(seqs), c.n_head * c.head_dim, device=self.dev)
 
         def attend(i, q):
-            cfi.paged_attention(self.caches[i], q.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(), len(seqs), c.n_head,
-                                width, 1.0 / math.sqrt(c.head_dim), stream=self.stream)
+            cfi.paged_attention(self.caches[i], q.data_ptr(), out.data_ptr(), p.table.data_ptr(), p.lens.data_ptr(), len(seqs), c.n_head,
+                                p.width, 1.0 / math.sqrt(c.head_dim), stream=self.stream)
             return out
 
-        new = [self._slots(s, s.cached, s.cached + 1)[0] for s in seqs]
-        logits = self._run([s.tokens[-1] for s in seqs], [s.cached for s in seqs], new, attend, range(len(seqs)))
+        logits = self._run([s.tokens[-1] for s in seqs], p, cfi.T_F32, attend, range(len(seqs)))
         for s in seqs:
             s.cached += 1
         return logits
@@ -208,6 +322,8 @@ class Server:
         cfi.sample(logits.data_ptr(), u.data_ptr(), token.data_ptr(), n, self.c.vocab, temperature.data_ptr(), top_k.data_ptr(),
                    top_p.data_ptr(), min_p.data_ptr(), logprob.data_ptr(), stream=self.stream)
         drawn = token.tolist()
+        if self.on_device and int(self.state.status):
+            raise RuntimeError("the page table's calls were refused (%d): what was cached since the last tokens is void" % int(self.state.status))
         error = cfi.device_error()
         if error:
             raise RuntimeError("a kernel's wait ran out (0x%x): the logits and what was cached since the last tokens are void" % error)
@@ -234,11 +350,14 @@ def main():
     import decode
 
     ap = argparse.ArgumentParser(description=__doc__.split("\n")[0])
-    ap.add_argument("--cache", choices=("f16", "q8_0"), default="q8_0")
+    ap.add_argument("--cache", choices=("f16", "q8_0", "q4_1"), default="q8_0")
     ap.add_argument("--batch", type=int, default=8)
     ap.add_argument("--new", type=int, default=32)
     ap.add_argument("--layers", type=int, default=4)
     ap.add_argument("--file", help="a qwen2 GGUF file instead of random weights")
+    ap.add_argument("--fused", action="store_true", help="biases, rope and the cache's rows in one kernel")
+    ap.add_argument("--norms", action="store_true", help="norms of the heads of q and k (random weights)")
+    ap.add_argument("--tables", choices=("host", "device"), default="host")
     a = ap.parse_args()
     torch.cuda.set_device(0)
     ctx = cfi.Ctx(0, const_weights=True)
@@ -249,7 +368,9 @@ def main():
     lengths = [int(x) for x in torch.randint(1, 600, (a.batch,), generator=gen)]
     seqs = [Sequence(torch.randint(0, m.cfg.vocab, (n,), generator=gen).tolist(), temperature=0.8, top_k=50, top_p=0.95) for n in lengths]
     pages = sum(-(-(n + a.new) // 16) for n in lengths)
-    s = Server(torch, ctx, m, cfi.Q8_0 if a.cache == "q8_0" else cfi.T_F16, 16, pages)
+    norms = [(1 + 0.1 * torch.randn(2, m.cfg.head_dim, generator=gen)).cuda() for _ in m.layers] if a.norms else None
+    s = Server(torch, ctx, m, dict(f16=cfi.T_F16, q8_0=cfi.Q8_0, q4_1=cfi.Q4_1)[a.cache], 16, pages, fused=True if a.fused else None,
+               norms=norms, tables=a.tables, rows=a.batch)
     begin = time.perf_counter()
     tokens = s.generate(seqs, a.new)
     torch.cuda.synchronize()
