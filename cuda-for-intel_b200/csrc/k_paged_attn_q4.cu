@@ -34,7 +34,10 @@ namespace {
 using namespace sm100;
 
 constexpr int P4_TILE = 32;         // positions
-constexpr int P4_FIXED = 3;         // what beginning and ending a pair costs, in tiles
+// What beginning and ending a pair costs, in tiles: lengths, table, first tiles and the meeting are memory round trips after one
+// another.  Measured with 3, 6, 9 and 12: 64 sequences of 100 to 4000, 32/8 heads of 128, 44.7, 36.9, 33.9 and 34.1 us; 4 of 30000, 12/2
+// heads of 128, 25.7, 22.4, 21.4 and 21.4; 64 of 16 to 4096, 14/2 heads of 64, 11.9, 10.9, 10.9 and 11.4.
+constexpr int P4_FIXED = 9;
 constexpr float P4_TOP = 15.0f;     // log2 of the largest weight as it is split: f16 ends at 65504
 constexpr float P4_LEAST_V = -15.0f, P4_MOST_V = 16.0f;  // f16 has the inverse of 2^the first; scales are below 2^the second
 constexpr float P4_N = 16777216.0f;  // 2^24: nibbles are whole numbers times its inverse
@@ -865,8 +868,13 @@ template <int D, int W, bool FEW> int launch(PaArgs& a, long long pairs, long lo
 int cfi_paged_attention_q4_1(PaArgs& a, int head_dim, long long pairs, cudaStream_t stream) {
     const long long positions = (long long)a.max_pages << a.page_shift;
     const long long most_units = pairs * (P4_FIXED + (positions + P4_TILE - 1) / P4_TILE);
+    // Short tables: a CTA to a pair, which neither reads all lengths nor joins anything; eight warps where an SM has one pair at most, four
+    // otherwise.  Measured against the equal runs (us, lengths from a quarter of the longest; 14/2 heads of 64, 12/2 of 128): one
+    // sequence of 768 5.5 to 7.4 and 7.4 to 9.4, of 2048 10.5 to 7.8 and 14.8 to 9.8; 16 of 1024 6.7 to 8.8 and 9.1 to 11.3, of 2048 10.5
+    // to 9.6 and 14.9 to 11.3; 64 of 2048 10.8 to 11.1 and 15.3 to 15.4; 128 of 512 8.0 to 10.5 and 8.7 to 13.9, of 1024 12.7 to 12.2 and
+    // 14.2 to 17.1; 64 of 2048 with 32/8 heads of 128, four warps, 35.0 to 32.7.
     const int sms = cfi_sm_count();
-    const int w = pairs <= sms ? (positions <= (2 * pairs > sms ? 1536 : 768) ? 8 : 0) : positions <= 768 ? 4 : 0;
+    const int w = pairs <= sms ? (positions <= (2 * pairs > sms ? 2048 : 1280) ? 8 : 0) : positions <= (head_dim == 128 ? 1024 : 768) ? 4 : 0;
     a.whole = w > 0;
     const int variant = (head_dim == 128) * 4 + (w == 8) * 2 + (a.group <= 4);
     switch (variant) {

@@ -179,12 +179,11 @@ template <class S, int D, int THREADS> CFI_DEV void join_shared(const PaArgs& a,
         const PaShared p = warp == 0 ? shared[0] : shared[1];
         bool last = false;
         if (p.id >= 0) {
-            __threadfence();  // after a barrier: covers the stores of the whole CTA
-            last = atomicAdd(&a.counters[p.id], 1u) == (unsigned)(p.n - 1);
-            if (last) {
-                __threadfence();
-                a.counters[p.id] = 0u;
-            }
+            // after a barrier: releases the stores of the whole CTA, and acquires those of the others
+            unsigned int before;
+            asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(a.counters + p.id) : "memory");
+            last = before == (unsigned)(p.n - 1);
+            if (last) a.counters[p.id] = 0u;
         }
         s_last[warp] = last;
     }
