@@ -7,15 +7,18 @@
 // of the cache: what a tile costs beside its products (maximum, vote, copies) is shared by twice as many.
 //
 // A position and kv head are 160 bytes with heads of 128, which at the memory's rate leaves a warp some 28 instructions: what has to
-// be cheap is making operands of nibbles.  They need no conversion: the bits 0x00hl of a byte are the f16 number (16 h + l) 2^-24 and
-// 0x000l is l 2^-24, exact subnormals that the MMA multiplies like any others.  A byte goes in twice, whole and without its upper
-// nibble, so that four ANDs and permutations make operands of eight nibbles; where
+// be cheap is making operands of nibbles.  A byte 16 h + l with 0x64 above it is the f16 number 1024 + 16 h + l; without its upper
+// nibble it is 1024 + l, and one subtraction for two of them takes the 1024 away.  So both go in, where
 //   x l + y h = (x - y/16) l + (y/16) (16 h + l),
-// the weights x, y of q take the first form of K's product, and V's sums are taken apart at the end.
-//   K: a word of the cache is 8 dims of one position for one lane; dims i and i + 4 of it share a register.  A is q, B is K: rows
-//      0-7 of the result and rows 8-15 are added.
+// and V's sums are taken apart at the end.  (The bits 0x00hl alone are 16 h + l times 2^-24, with no instruction more: but an MMA lines
+// its products up by their exponents' fields, cuts them at 24 bits, and subnormal operands lose up to ten of those.)
+//   K, five to eight heads: A is q, B is K: a word of the cache is 8 dims of one position for one lane; dims i and i + 4 of it share a
+//      register.  Rows 0-7 of the result and rows 8-15 are added.
+//   K, up to four heads: whole numbers.  q is four digits of 8 bits, four heads times four digits are the 16 rows of A, and one MMA
+//      of bytes takes a block of 32 dims where f16 needs two; its sums begin at the bits of 1.5 2^23, so that they are read as floats.
 //   V: two positions meet in a register, so half-words of two rows are first put together by one byte permutation.  A is V with
-//      dims as rows, B the weights, which lie as the scores came out; their two parts add up in the same sums.
+//      dims as rows, B the weights, which lie as the scores came out; f16 values and what these leave go one after the other, or, with up to
+//      four heads, in columns 0-3 and 4-7 of the same MMA.
 // Which position is which column of the scores is free, as long as the weights go back to the same: column 2 c + e of the n-th eight
 // is position 8 n + 4 e + (c ^ 3 e), so that no two lanes read the same bank of K or of V.
 // The minima of K meet the sums of q over each block in one MMA for 8 positions, those of V the weights in one for 16.
@@ -24,7 +27,6 @@
 #include "cfi_kernels.h"
 
 #include <algorithm>
-#include <type_traits>
 #include <math.h>
 #include <stdlib.h>
 #include <string.h>
@@ -40,7 +42,6 @@ constexpr int P4_TILE = 32;         // positions
 constexpr int P4_FIXED = 9;
 constexpr float P4_TOP = 15.0f;     // log2 of the largest weight as it is split: f16 ends at 65504
 constexpr float P4_LEAST_V = -15.0f, P4_MOST_V = 16.0f;  // f16 has the inverse of 2^the first; scales are below 2^the second
-constexpr float P4_N = 16777216.0f;  // 2^24: nibbles are whole numbers times its inverse
 using Cut = PaCut<P4_TILE, P4_FIXED>;
 
 template <int D, int W = PA_WARPS> struct P4Shape {
@@ -101,27 +102,42 @@ CFI_DEV void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint3
                  : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
+// Adds the sums of an MMA, rounded.  (An MMA cuts its own result to 24 bits: where it kept the sums of a whole run, all of positive
+// products, they would be short by half a unit for each tile.)
+CFI_DEV void add4(float (&d)[4], const float (&x)[4]) {
+    const float2 a = both(add2(pair2(d[0], d[1]), pair2(x[0], x[1]))), b = both(add2(pair2(d[2], d[3]), pair2(x[2], x[3])));
+    d[0] = a.x, d[1] = a.y, d[2] = b.x, d[3] = b.y;
+}
 CFI_DEV void mma_k8(float (&d)[4], const uint32_t (&a)[2], uint32_t b) {
     asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%7, %7, %7, %7};"
                  : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(b), "f"(0.0f));
 }
-CFI_DEV uint32_t turned(uint32_t x) {  // an 8 x 8 of f16: lane (g, c) has row g, columns 2 c and 2 c + 1
-    uint32_t r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
-    return r;
+// Rows of digits by a block's nibbles; the sums are read as floats, 1.5 2^23 more than they are.
+constexpr float P4_MAGIC = 12582912.0f;
+CFI_DEV void mma_digits(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    int e[4];
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=r"(e[0]), "=r"(e[1]), "=r"(e[2]), "=r"(e[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0x4b400000));
+#pragma unroll
+    for (int i = 0; i < 4; i++) d[i] = __int_as_float(e[i]);
 }
 CFI_DEV void ldsm_x2_trans(uint32_t a, uint32_t& r0, uint32_t& r1) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(r0), "=r"(r1) : "r"(a));
 }
-// The lower byte of each half, without and with its upper nibble, as f16 numbers times 2^24; then the upper byte.
+// The lower byte of each half, without and with its upper nibble, as f16 numbers; then the upper byte.
 struct Nibbles {
     uint32_t x0, y0, x1, y1;
     CFI_DEV explicit Nibbles(uint32_t w) {
-        y0 = w & 0x00ff00ffu;
-        x0 = w & 0x000f000fu;
-        y1 = __byte_perm(w, 0, 0x4341);
-        x1 = y1 & 0x000f000fu;
+        const uint32_t a = __byte_perm(w, 0x64646464u, 0x4240), b = __byte_perm(w, 0x64646464u, 0x4341);
+        x0 = less(a & 0xff0fff0fu);
+        y0 = less(a);
+        x1 = less(b & 0xff0fff0fu);
+        y1 = less(b);
+    }
+    static CFI_DEV uint32_t less(uint32_t w) {
+        return h2_bits(__hsub2(*reinterpret_cast<const __half2*>(&w), __half2half2(__ushort_as_half(0x6400))));
     }
 };
 // column 2 c + e of the n-th eight scores
@@ -209,21 +225,23 @@ template <int D> CFI_DEV void params_turned(uint32_t tile, uint32_t& b0, uint32_
     }
 }
 
-// A lane's query values, dims 32 b + 8 c .. + 7 of one head, as MMA operands: in log2 units over `unit`, split; and the sums of
-// the blocks over 2^6 where a row of scales and minima (2 NB numbers, of which a lane has two) has its minima.
-template <int D> struct Queries {
+// A lane's query values, dims 32 b + 8 c .. + 7 of head g (FEW: g & 3), as MMA operands over `unit`; and the sums of the blocks over 2^6
+// where a row of scales and minima (2 NB numbers, of which a lane has two) has its minima.
+template <int D, bool FEW> struct Queries {
     static constexpr int NB = D / 32;
-    uint32_t hi[2 * NB][2], lo[2 * NB][2], sum_hi, sum_lo;
+    uint32_t a[FEW ? NB : 2 * NB][4], sums[2];
     float unit;
     CFI_DEV void convert(float (&qv)[NB][8], float scale_log2) {
-        const int c = threadIdx.x & 3;
+        const int lane = threadIdx.x & 31, c = lane & 3;
         float largest = 0.0f;  // a NaN is passed over
+        bool odd = false;      // NaN or an infinity among them
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 qv[b][e] *= scale_log2;
                 largest = fmaxf(largest, fabsf(qv[b][e]));
+                odd |= !(fabsf(qv[b][e]) < INFINITY);
             }
         largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
         largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
@@ -231,40 +249,63 @@ template <int D> struct Queries {
         const uint32_t exponent = max(__float_as_uint(largest) >> 23, 15u);
         unit = __uint_as_float((exponent - 14) << 23);
         const float per_unit = __uint_as_float((268 - exponent) << 23);
-        float sums[NB];
+        float sum[NB];
 #pragma unroll
         for (int b = 0; b < NB; b++) {
-            sums[b] = 0.0f;
+            sum[b] = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 qv[b][e] *= per_unit;
-                sums[b] += qv[b][e];
+                sum[b] += qv[b][e];
             }
-            sums[b] += __shfl_xor_sync(0xffffffffu, sums[b], 1);
-            sums[b] += __shfl_xor_sync(0xffffffffu, sums[b], 2);
+            sum[b] += __shfl_xor_sync(0xffffffffu, sum[b], 1);
+            sum[b] += __shfl_xor_sync(0xffffffffu, sum[b], 2);
+            if (FEW) {
+                // digits of q 2^15: rows 0-3 have the first of heads 0-3, rows 4-7 the second, 8-11 the third, 12-15 the last; bytes of a
+                // register are dims 0, 2, 4, 6 of the lane's, or 1, 3, 5, 7
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const float y0 = qv[b][2 * k + 1] * 0.0625f, y1 = qv[b][2 * k + 5] * 0.0625f;
-                split(qv[b][2 * k] - y0, qv[b][2 * k + 4] - y1, &hi[2 * b + k][0], &lo[2 * b + k][0]);
-                split(y0, y1, &hi[2 * b + k][1], &lo[2 * b + k][1]);
+                for (int x = 0; x < 2; x++) {
+                    uint32_t d[4] = {0, 0, 0, 0};  // from the last
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        int v = __float2int_rn(qv[b][2 * e + x] * 32768.0f);
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            d[k] |= (uint32_t)(v & 0xff) << (8 * e);
+                            v = (v - (int)(int8_t)(v & 0xff)) >> 8;
+                        }
+                    }
+                    a[b][2 * x] = lane < 16 ? d[3] : d[2];
+                    a[b][2 * x + 1] = lane < 16 ? d[1] : d[0];
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const float y0 = qv[b][2 * k + 1] * 0.0625f, y1 = qv[b][2 * k + 5] * 0.0625f;
+                    split(qv[b][2 * k] - y0, qv[b][2 * k + 4] - y1, &a[(2 * b + k) % (FEW ? NB : 2 * NB)][0], &a[(2 * b + k) % (FEW ? NB : 2 * NB)][1]);
+                    split(y0, y1, &a[(2 * b + k) % (FEW ? NB : 2 * NB)][2], &a[(2 * b + k) % (FEW ? NB : 2 * NB)][3]);
+                }
             }
         }
+        // a NaN or an infinity has no digits: it reaches the scores by its sum
         const int x = 2 * c - NB;
-        const float s0 = x == 0 ? sums[0] : NB == 4 && x == 2 ? sums[NB - 2] : 0.0f, s1 = x == 0 ? sums[1] : NB == 4 && x == 2 ? sums[NB - 1] : 0.0f;
-        split(s0 * 0.015625f, s1 * 0.015625f, &sum_hi, &sum_lo);
+        float s0 = x == 0 ? sum[0] : NB == 4 && x == 2 ? sum[NB - 2] : 0.0f, s1 = x == 0 ? sum[1] : NB == 4 && x == 2 ? sum[NB - 1] : 0.0f;
+        if (FEW && odd) s0 = s1 = NAN;
+        split(s0 * 0.015625f, s1 * 0.015625f, &sums[0], &sums[1]);
     }
 };
 
-// ---- five to eight heads ----
-// Scores: A is q (rows 0-7 the heads' f16 values, rows 8-15 the rest), B is K.  A lane has head g, columns 2 c and 2 c + 1.
-template <int D> struct ManyHeads {
+// What a warp keeps of up to eight heads (FEW: four).  A lane has the scores of head g (g & 3, lanes g and g + 4 the same) in columns 2 c
+// and 2 c + 1 of a tile's four eights.
+template <int D, bool FEW> struct Heads {
     static constexpr int NB = D / 32;
-    uint32_t qf[2 * NB][4], qs[2];
-    // o has 2^(-top - 24) in it.  Of heads 2 c and 2 c + 1, dims 32 b + 4 g + 2 x and the next one, which has 16 times itself and the first
-    float o[NB][2][4], mins[4], m, unit;
+    Queries<D, FEW> q;
+    // o has 2^-top in it.  Of columns 2 c and 2 c + 1, dims 32 b + 4 g + 2 x and the next one, which has 16 times itself and the first;
+    // a column is a head, or (FEW, from 4 on) what f16 left of a head's weights
+    float o[NB][2][4], mins[4], m;
     f2 l;
     ScalesTop v;
-    static CFI_DEV int head() { return threadIdx.x >> 2 & 7; }  // whose queries this lane loads
+    static CFI_DEV int head() { return threadIdx.x >> 2 & (FEW ? 3 : 7); }  // whose queries this lane loads
     CFI_DEV void begin() {
         m = -INFINITY;
         l = 0;
@@ -276,37 +317,46 @@ template <int D> struct ManyHeads {
 #pragma unroll
             for (int e = 0; e < 4; e++) o[b][0][e] = o[b][1][e] = 0.0f;
     }
-    CFI_DEV void queries(const Queries<D>& q) {
-#pragma unroll
-        for (int k = 0; k < 2 * NB; k++) qf[k][0] = q.hi[k][0], qf[k][1] = q.lo[k][0], qf[k][2] = q.hi[k][1], qf[k][3] = q.lo[k][1];
-        qs[0] = q.sum_hi, qs[1] = q.sum_lo;
-        unit = q.unit;
-    }
     CFI_DEV void tile(uint32_t sk, uint32_t sv, int left) {
         using L = Q41<D>;
         const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-        // ---- scores, over 2^24 `unit` ----
+        // ---- scores, over `unit` ----
         f2 s[4];
 #pragma unroll
         for (int n = 0; n < 4; n++) {
             const uint32_t tile = sk + (n >> 1) * L::TILE;
             const int row = position_of(g >> 1, g & 1, n & 1);
             float first[4];
-            mma_k8(first, qs, lds32(tile + L::NIBBLES + row * L::PARAM_ROW + 4 * (c & (NB - 1))));
-            s[n] = pair2((first[0] + first[2]) * (64.0f / P4_N), (first[1] + first[3]) * (64.0f / P4_N));
+            mma_k8(first, q.sums, lds32(tile + L::NIBBLES + row * L::PARAM_ROW + 4 * (c & (NB - 1))));
+            const f2 low = add2(pair2(first[0], first[1]), pair2(first[2], first[3]));
             uint32_t w[NB], d0[NB / 2], d1[NB / 2];
             dims_of_k<D>(tile, row, w);
             scales_of<D>(tile, position_of(c, 0, n & 1), d0);
             scales_of<D>(tile, position_of(c, 1, n & 1), d1);
+            f2 sum = 0;
 #pragma unroll
             for (int b = 0; b < NB; b++) {
+                const f2 scale = pair2(half_of(d0[b >> 1], b & 1), half_of(d1[b >> 1], b & 1));
                 float acc[4];
-                const Nibbles k(w[b]);
-                mma_first(acc, qf[2 * b], k.x0, k.y0);
-                mma_f16f32(acc, qf[2 * b + 1], k.x1, k.y1);
-                s[n] = fma2(add2(pair2(acc[0], acc[1]), pair2(acc[2], acc[3])),
-                            pair2(half_of(d0[b >> 1], b & 1), half_of(d1[b >> 1], b & 1)), s[n]);
+                if (FEW) {
+                    mma_digits(acc, q.a[b], w[b] & 0x0f0f0f0fu, w[b] >> 4 & 0x0f0f0f0fu);
+                    // 2^16 times rows g and rows g + 8
+                    const f2 upper = fma2(pair2(acc[0], acc[1]), pair2(65536.0f, 65536.0f), pair2(-65536.0f * P4_MAGIC, -65536.0f * P4_MAGIC)),
+                             lower = add2(pair2(acc[2], acc[3]), pair2(-P4_MAGIC, -P4_MAGIC));
+                    sum = fma2(add2(upper, lower), scale, sum);
+                } else {
+                    const Nibbles k(w[b]);
+                    mma_first(acc, q.a[(2 * b) % (FEW ? NB : 2 * NB)], k.x0, k.y0);
+                    mma_f16f32(acc, q.a[(2 * b + 1) % (FEW ? NB : 2 * NB)], k.x1, k.y1);
+                    sum = fma2(add2(pair2(acc[0], acc[1]), pair2(acc[2], acc[3])), scale, sum);
+                }
             }
+            if (FEW) {  // the first digits are 2^8 the second ones', which lanes g and g + 4 have
+                const float by = lane < 16 ? 256.0f / 32768.0f : 1.0f / 32768.0f;
+                sum = mul2(sum, pair2(by, by));
+                sum = add2(sum, pair2(__shfl_xor_sync(0xffffffffu, both(sum).x, 16), __shfl_xor_sync(0xffffffffu, both(sum).y, 16)));
+            }
+            s[n] = fma2(low, pair2(64.0f, 64.0f), sum);
         }
         if (left < P4_TILE) {
 #pragma unroll
@@ -323,9 +373,10 @@ template <int D> struct ManyHeads {
         if (__any_sync(0xffffffffu, mx > m)) {
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const float mn = fmaxf(m, mx), alpha = m == -INFINITY ? 0.0f : ex2((m - mn) * P4_N * unit);
+            const float mn = fmaxf(m, mx), alpha = m == -INFINITY ? 0.0f : ex2((m - mn) * q.unit);
             l = mul2(l, pair2(alpha, alpha));
-            const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * c), a1 = __shfl_sync(0xffffffffu, alpha, 8 * c + 4);
+            const int from = 8 * (FEW ? c & 1 : c);
+            const float a0 = __shfl_sync(0xffffffffu, alpha, from), a1 = __shfl_sync(0xffffffffu, alpha, from + 4);
 #pragma unroll
             for (int e = 0; e < 4; e++) mins[e] *= alpha;
 #pragma unroll
@@ -334,15 +385,15 @@ template <int D> struct ManyHeads {
                 for (int x = 0; x < 2; x++) o[b][x][0] *= a0, o[b][x][1] *= a1, o[b][x][2] *= a0, o[b][x][3] *= a1;
             m = mn;
         }
-        const float sub = m == -INFINITY ? 0.0f : -m * P4_N;  // P4_TOP is added last: a large score would swallow it
+        const float sub = m == -INFINITY ? 0.0f : -m;  // P4_TOP is added last: a large score would swallow it
         f2 p[4];
 #pragma unroll
         for (int n = 0; n < 4; n++) {
-            const float2 x = both(fma2(fma2(s[n], pair2(P4_N, P4_N), pair2(sub, sub)), pair2(unit, unit), pair2(P4_TOP, P4_TOP)));
+            const float2 x = both(fma2(add2(s[n], pair2(sub, sub)), pair2(q.unit, q.unit), pair2(P4_TOP, P4_TOP)));
             p[n] = pair2(ex2(x.x), ex2(x.y));
             l = add2(l, p[n]);
         }
-        // ---- weighted values: A is V with dims as rows, B the weights and then what f16 left of them ----
+        // ---- weighted values: A is V with dims as rows, B the weights ----
         float by;
         const bool wide = v.template look<D>(sv, &by);
         if (by != 1.0f) {
@@ -361,6 +412,7 @@ template <int D> struct ManyHeads {
     template <bool WIDE> CFI_DEV void values(uint32_t sv, const f2 (&p)[4]) {
         using L = Q41<D>;
         const int c = threadIdx.x & 3;
+        const uint32_t rest = (threadIdx.x & 31) < 16 ? 0u : 0xffffffffu;  // FEW: lanes whose column is what f16 left
 #pragma unroll
         for (int t = 0; t < 2; t++) {
             const uint32_t tile = sv + t * L::TILE;
@@ -369,7 +421,9 @@ template <int D> struct ManyHeads {
             for (int n = 0; n < 2; n++) split2(p[2 * t + n], &pf[2 * n], &pf[2 * n + 1]);
             // minima: column x of a row's scales and minima, of which those from NB on count
             params_turned<D>(tile, b0, b1);
-            mma_f16f32(mins, pf, b0, b1);
+            float sums[4];
+            mma_first(sums, pf, b0, b1);
+            add4(mins, sums);
             uint32_t w[2][2][NB / 2], d[2][2][NB / 2];  // of column 2 c + e of eight n
             const __half2 per = __float2half2_rn(v.per);
 #pragma unroll
@@ -391,27 +445,41 @@ template <int D> struct ManyHeads {
                     if (WIDE) {
                         const f2 scale = pair2(half_of(d[n][0][b >> 1], b & 1) * v.per, half_of(d[n][1][b >> 1], b & 1) * v.per);
                         split2(mul2(p[2 * t + n], scale), &hi[n], &lo[n]);
+                        if (FEW) hi[n] = rest ? lo[n] : hi[n];
                     } else {
-                        const __half2 scale = as_h2(__byte_perm(d[n][0][b >> 1], d[n][1][b >> 1], b & 1 ? 0x7632 : 0x5410)),
-                                      h = __hmul2(as_h2(pf[2 * n]), scale);
-                        hi[n] = h2_bits(h);
-                        lo[n] = h2_bits(__hfma2(as_h2(pf[2 * n + 1]), scale, __hfma2(as_h2(pf[2 * n]), scale, __hneg2(h))));
+                        const __half2 scale = as_h2(__byte_perm(d[n][0][b >> 1], d[n][1][b >> 1], b & 1 ? 0x7632 : 0x5410));
+                        if (FEW) {  // with the masked ones 0: hi d rounded; with them whole: what that leaves, and lo d
+                            const __half2 h = __hmul2(as_h2(pf[2 * n] & rest), scale);
+                            hi[n] = h2_bits(__hfma2(as_h2(pf[2 * n + 1] & rest), scale, __hfma2(as_h2(pf[2 * n]), scale, __hneg2(h))));
+                        } else {
+                            const __half2 h = __hmul2(as_h2(pf[2 * n]), scale);
+                            hi[n] = h2_bits(h);
+                            lo[n] = h2_bits(__hfma2(as_h2(pf[2 * n + 1]), scale, __hfma2(as_h2(pf[2 * n]), scale, __hneg2(h))));
+                        }
                     }
                     z[n] = __byte_perm(w[n][0][b >> 1], w[n][1][b >> 1], b & 1 ? 0x7632 : 0x5410);  // dims 32 b + 4 g .. + 3 of two positions
                 }
                 const Nibbles v0(z[0]), v1(z[1]);
                 const uint32_t r0[4] = {v0.x0, v0.y0, v1.x0, v1.y0}, r1[4] = {v0.x1, v0.y1, v1.x1, v1.y1};
-                mma_f16f32(o[b][0], r0, hi[0], hi[1]);
-                mma_f16f32(o[b][1], r1, hi[0], hi[1]);
-                mma_f16f32(o[b][0], r0, lo[0], lo[1]);
-                mma_f16f32(o[b][1], r1, lo[0], lo[1]);
+                float s0[4], s1[4];
+                if (FEW) {
+                    mma_first(s0, r0, hi[0], hi[1]);
+                    mma_first(s1, r1, hi[0], hi[1]);
+                } else {
+                    mma_first(s0, r0, lo[0], lo[1]);
+                    mma_first(s1, r1, lo[0], lo[1]);
+                    mma_f16f32(s0, r0, hi[0], hi[1]);
+                    mma_f16f32(s1, r1, hi[0], hi[1]);
+                }
+                add4(o[b][0], s0);
+                add4(o[b][1], s1);
             }
         }
     }
     // Values, maximum and sum of each head as rows of `row` floats.
     CFI_DEV void finish(float* meet, int row) {
         const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-        const float back = ex2(v.top) * P4_N;  // each warp has had scales of its own
+        const float back = ex2(v.top);  // each warp has had scales of its own
         float sum = both(l).x + both(l).y;
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
@@ -423,224 +491,14 @@ template <int D> struct ManyHeads {
                 float f[4];
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
-                    f[2 * x] = fmaf(o[b][x][e], back, low);
-                    f[2 * x + 1] = fmaf(o[b][x][2 + e] - o[b][x][e], back / 16.0f, low);
-                }
-                *reinterpret_cast<float4*>(meet + (2 * c + e) * row + 32 * b + 4 * g) = make_float4(f[0], f[1], f[2], f[3]);
-            }
-        if (c == 0) *reinterpret_cast<float2*>(meet + g * row + D) = make_float2(m * P4_N * unit, sum);
-    }
-};
-
-// ---- up to four heads ----
-// Both parts of four heads fill the eight columns of one MMA, so that all products take half as many: A is K with positions as rows, B
-// has the heads' f16 values in columns 0-3 and the rest in 4-7, and the two are added when the scores are whole.  A lane then has heads
-// 2 (c & 1) and the next at positions g and g + 8 (in the order above), lanes c and c ^ 2 the same; for V's product it makes f16 values
-// (c < 2) or the rest of its weights, which one 8 x 8 transposition brings to the places that B has them.
-template <int D> struct FewHeads {
-    static constexpr int NB = D / 32;
-    uint32_t qb[2 * NB][2], qs;
-    // o as above; columns 2 c and 2 c + 1, of which those from 4 on are the weights' rest
-    float o[NB][2][4], mins[4], m[2], l[2], unit[2];
-    ScalesTop v;
-    static CFI_DEV int head() { return threadIdx.x >> 2 & 3; }
-    CFI_DEV void begin() {
-        m[0] = m[1] = -INFINITY;
-        l[0] = l[1] = 0.0f;
-        v.set(P4_LEAST_V);
-#pragma unroll
-        for (int e = 0; e < 4; e++) mins[e] = 0.0f;
-#pragma unroll
-        for (int b = 0; b < NB; b++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) o[b][0][e] = o[b][1][e] = 0.0f;
-    }
-    CFI_DEV void queries(const Queries<D>& q) {
-        const int lane = threadIdx.x & 31, c = lane & 3;
-        const bool rest = lane >= 16;
-#pragma unroll
-        for (int k = 0; k < 2 * NB; k++) qb[k][0] = rest ? q.lo[k][0] : q.hi[k][0], qb[k][1] = rest ? q.lo[k][1] : q.hi[k][1];
-        qs = rest ? q.sum_lo : q.sum_hi;
-#pragma unroll
-        for (int x = 0; x < 2; x++) unit[x] = __shfl_sync(0xffffffffu, q.unit, 4 * (2 * (c & 1) + x));
-    }
-    CFI_DEV void tile(uint32_t sk, uint32_t sv, int left) {
-        using L = Q41<D>;
-        const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-        // ---- scores, over 2^24 `unit`: of position g + 8 r of half t, head x ----
-        float s[2][2][2];
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-            const uint32_t tile = sk + t * L::TILE;
-            const int row = position_of(g >> 1, g & 1, 0);  // and 8 behind
-            uint32_t w[2][NB], d[2][NB / 2], low[2];
-#pragma unroll
-            for (int r = 0; r < 2; r++) {
-                low[r] = lds32(tile + L::NIBBLES + (row + 8 * r) * L::PARAM_ROW + 4 * (c & (NB - 1)));
-                dims_of_k<D>(tile, row + 8 * r, w[r]);
-                scales_of<D>(tile, row + 8 * r, d[r]);
-            }
-            float first[4];
-            mma_k8(first, low, qs);
-#pragma unroll
-            for (int r = 0; r < 2; r++)
-#pragma unroll
-                for (int x = 0; x < 2; x++) s[t][r][x] = first[2 * r + x] * (64.0f / P4_N);
-#pragma unroll
-            for (int b = 0; b < NB; b++) {
-                float acc[4];
-                const Nibbles k0(w[0][b]), k1(w[1][b]);
-                const uint32_t a0[4] = {k0.x0, k1.x0, k0.y0, k1.y0}, a1[4] = {k0.x1, k1.x1, k0.y1, k1.y1};
-                mma_first(acc, a0, qb[2 * b][0], qb[2 * b][1]);
-                mma_f16f32(acc, a1, qb[2 * b + 1][0], qb[2 * b + 1][1]);
-#pragma unroll
-                for (int r = 0; r < 2; r++) {
-                    const float scale = half_of(d[r][b >> 1], b & 1);
-#pragma unroll
-                    for (int x = 0; x < 2; x++) s[t][r][x] = fmaf(acc[2 * r + x], scale, s[t][r][x]);
-                }
-            }
-#pragma unroll
-            for (int r = 0; r < 2; r++)
-#pragma unroll
-                for (int x = 0; x < 2; x++) s[t][r][x] += __shfl_xor_sync(0xffffffffu, s[t][r][x], 2);
-        }
-        if (left < P4_TILE) {
-#pragma unroll
-            for (int t = 0; t < 2; t++)
-#pragma unroll
-                for (int r = 0; r < 2; r++)
-                    if (16 * t + position_of(g >> 1, g & 1, r) >= left) s[t][r][0] = s[t][r][1] = -INFINITY;
-        }
-        float mx[2];
-#pragma unroll
-        for (int x = 0; x < 2; x++) mx[x] = fmaxf(fmaxf(s[0][0][x], s[0][1][x]), fmaxf(s[1][0][x], s[1][1][x]));
-        if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
-            float alpha[2];
-#pragma unroll
-            for (int x = 0; x < 2; x++) {
-#pragma unroll
-                for (int y = 4; y < 32; y <<= 1) mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], y));
-                const float mn = fmaxf(m[x], mx[x]);
-                alpha[x] = m[x] == -INFINITY ? 0.0f : ex2((m[x] - mn) * P4_N * unit[x]);
-                l[x] *= alpha[x];
-                m[x] = mn;
-            }
-#pragma unroll
-            for (int e = 0; e < 4; e++) mins[e] *= alpha[e & 1];
-#pragma unroll
-            for (int b = 0; b < NB; b++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) o[b][0][e] *= alpha[e & 1], o[b][1][e] *= alpha[e & 1];
-        }
-        float p[2][2][2];
-#pragma unroll
-        for (int x = 0; x < 2; x++) {
-            const float sub = m[x] == -INFINITY ? 0.0f : -m[x] * P4_N;  // P4_TOP is added last: a large score would swallow it
-#pragma unroll
-            for (int t = 0; t < 2; t++)
-#pragma unroll
-                for (int r = 0; r < 2; r++) {
-                    p[t][r][x] = ex2(fmaf(fmaf(s[t][r][x], P4_N, sub), unit[x], P4_TOP));
-                    l[x] += p[t][r][x];
-                }
-        }
-        // ---- weighted values ----
-        float by;
-        const bool wide = v.template look<D>(sv, &by);
-        if (by != 1.0f) {
-#pragma unroll
-            for (int b = 0; b < NB; b++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) o[b][0][e] *= by, o[b][1][e] *= by;
-        }
-        if (wide)
-            values<true>(sv, p);
-        else
-            values<false>(sv, p);
-    }
-    // As above; a lane's two heads at positions g and g + 8.
-    template <bool WIDE> CFI_DEV void values(uint32_t sv, const float (&p)[2][2][2]) {
-        using L = Q41<D>;
-        const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-        const uint32_t rest = c < 2 ? 0u : 0xffffffffu;
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-            const uint32_t tile = sv + t * L::TILE;
-            uint32_t hi[2], lo[2], pt[2], rows[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int n = 0; n < 2; n++) {
-                split(p[t][n][0], p[t][n][1], &hi[n], &lo[n]);
-                pt[n] = turned(rest ? lo[n] : hi[n]);
-            }
-            // minima: row x of the scales and minima, of which those from NB on count
-            params_turned<D>(tile, rows[0], rows[2]);
-            mma_f16f32(mins, rows, pt[0], pt[1]);
-            uint32_t w[2][2][NB / 2], d[2][NB / 2];
-            const __half2 per = __float2half2_rn(v.per);
-#pragma unroll
-            for (int n = 0; n < 2; n++) {
-                scales_of<D>(tile, position_of(g >> 1, g & 1, n), d[n]);
-                if (!WIDE) {
-#pragma unroll
-                    for (int x = 0; x < NB / 2; x++) d[n][x] = h2_bits(__hmul2(as_h2(d[n][x]), per));
-                }
-#pragma unroll
-                for (int e = 0; e < 2; e++) dims_of_v<D>(tile, position_of(c, e, n), w[n][e]);
-            }
-#pragma unroll
-            for (int b = 0; b < NB; b++) {
-                uint32_t wb[2], z[2];
-#pragma unroll
-                for (int n = 0; n < 2; n++) {
-                    if (WIDE) {
-                        const float scale = half_of(d[n][b >> 1], b & 1) * v.per;
-                        uint32_t h, l;
-                        split(p[t][n][0] * scale, p[t][n][1] * scale, &h, &l);
-                        wb[n] = turned(rest ? l : h);
-                    } else {
-                        // with the masked ones 0: hi d rounded; with them whole: what that leaves, and lo d
-                        const __half2 scale = b & 1 ? __high2half2(as_h2(d[n][b >> 1])) : __low2half2(as_h2(d[n][b >> 1]));
-                        const __half2 h = __hmul2(as_h2(hi[n] & rest), scale);
-                        wb[n] = turned(h2_bits(__hfma2(as_h2(lo[n] & rest), scale, __hfma2(as_h2(hi[n]), scale, __hneg2(h)))));
-                    }
-                    z[n] = __byte_perm(w[n][0][b >> 1], w[n][1][b >> 1], b & 1 ? 0x7632 : 0x5410);  // dims 32 b + 4 g .. + 3 of two positions
-                }
-                const Nibbles v0(z[0]), v1(z[1]);
-                const uint32_t r0[4] = {v0.x0, v0.y0, v1.x0, v1.y0}, r1[4] = {v0.x1, v0.y1, v1.x1, v1.y1};
-                mma_f16f32(o[b][0], r0, wb[0], wb[1]);
-                mma_f16f32(o[b][1], r1, wb[0], wb[1]);
-            }
-        }
-    }
-    CFI_DEV void finish(float* meet, int row) {
-        const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-        const float back = ex2(v.top) * P4_N;
-#pragma unroll
-        for (int x = 0; x < 2; x++) {
-#pragma unroll
-            for (int y = 4; y < 32; y <<= 1) l[x] += __shfl_xor_sync(0xffffffffu, l[x], y);
-            mins[x] += __shfl_xor_sync(0xffffffffu, mins[x], 2);
-        }
-#pragma unroll
-        for (int b = 0; b < NB; b++)
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const float low = __shfl_sync(0xffffffffu, mins[e], 4 * (NB + b) + c);  // row NB + b
-                float f[4];
-#pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    const float u = o[b][x][e] + __shfl_xor_sync(0xffffffffu, o[b][x][e], 2),
-                                w = o[b][x][2 + e] + __shfl_xor_sync(0xffffffffu, o[b][x][2 + e], 2);
+                    float u = o[b][x][e], w = o[b][x][2 + e];
+                    if (FEW) u += __shfl_xor_sync(0xffffffffu, u, 2), w += __shfl_xor_sync(0xffffffffu, w, 2);
                     f[2 * x] = fmaf(u, back, low);
                     f[2 * x + 1] = fmaf(w - u, back / 16.0f, low);
                 }
-                if (c < 2) *reinterpret_cast<float4*>(meet + (2 * c + e) * row + 32 * b + 4 * g) = make_float4(f[0], f[1], f[2], f[3]);
+                if (!FEW || c < 2) *reinterpret_cast<float4*>(meet + (2 * c + e) * row + 32 * b + 4 * g) = make_float4(f[0], f[1], f[2], f[3]);
             }
-        if (lane < 2) {
-#pragma unroll
-            for (int x = 0; x < 2; x++) *reinterpret_cast<float2*>(meet + (2 * c + x) * row + D) = make_float2(m[x] * P4_N * unit[x], l[x]);
-        }
+        if (c == 0 && (!FEW || g < 4)) *reinterpret_cast<float2*>(meet + g * row + D) = make_float2(m * q.unit, sum);
     }
 };
 
@@ -696,8 +554,7 @@ __global__ void __launch_bounds__(W * 32, (P4Shape<D, W>::CTAS)) paged_attn_q4(c
         int id0 = load_id(0, 0), id1 = load_id(0, 1);
 
         // the queries: loaded here, converted when the first tiles are on their way.  Dims 32 b + 8 c .. + 7
-        using Heads = typename std::conditional<FEW, FewHeads<D>, ManyHeads<D>>::type;
-        const int h = Heads::head();
+        const int h = Heads<D, FEW>::head();
         float qv[NB][8];
 #pragma unroll
         for (int b = 0; b < NB; b++) {
@@ -759,7 +616,7 @@ __global__ void __launch_bounds__(W * 32, (P4Shape<D, W>::CTAS)) paged_attn_q4(c
             cp_async_commit();
         };
 
-        Heads heads;
+        Heads<D, FEW> heads;
         heads.begin();
 #pragma unroll
         for (int i = 0; i < S::STAGES - 1; i++) fetch(i);
@@ -774,11 +631,7 @@ __global__ void __launch_bounds__(W * 32, (P4Shape<D, W>::CTAS)) paged_attn_q4(c
                     qv[b][2 * e + 1] = f.y;
                 }
         }
-        {
-            Queries<D> q;
-            q.convert(qv, a.scale_log2);
-            heads.queries(q);
-        }
+        heads.q.convert(qv, a.scale_log2);
         for (int i = 0; i < mine; i++) {
             if ((i + S::STAGES - 1) % 32 == 0) {
                 id0 = load_id(i + S::STAGES - 1, 0);

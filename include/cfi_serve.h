@@ -83,7 +83,7 @@ CFI_API int cfi_paged_kv_load(const CfiPagedCache *cache, const int64_t *slots, 
  * lies in a page past the length never matters, whatever it holds.
  * q and out: [sequence][head][dim], types 0 F32 or 1 F16, row strides in values (q's a multiple of
  * 8), 16-byte aligned; scale > 0.  Sums and maxima are in 32 bits and the operands of the products with
- * K and V carry 22 bits, a query's values no bits below 2^-38 (Q4_1: 2^-34) of their head's largest and a weight (Q8_0 and
+ * K and V carry 22 bits, a query's values no bits below 2^-38 (Q4_1: 2^-30) of their head's largest and a weight (Q8_0 and
  * Q4_1: times its scale of V) none below 2^-39 of the largest (Q4_1: scales below 2^-15 count as that): the results are those of
  * 32-bit arithmetic on the cached values, as long as the scores are within the range of f32.  (Q4_1: of the scaled whole numbers and
  * the minima, which are summed apart.)

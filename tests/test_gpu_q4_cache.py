@@ -392,3 +392,53 @@ def test_small_blocks_beside_large_ones(heads, kv, dim):
         want = p @ V[slots, h * kv // heads][:, :32] / p.sum()
         mags = float((np.abs(q[h]) @ (np.abs(K[slots, h * kv // heads]) * 3).T).max() / math.sqrt(dim))
         assert (np.abs(got[h, :32] - want) <= (2 * EPS_S * mags + 3 * 2.0 ** -20) * 2.0 ** -14 * 2).all()
+
+
+@pytest.mark.parametrize("heads,kv,dim,n", [(8, 8, 64, 33000), (12, 2, 64, 80000), (8, 8, 128, 20000), (16, 2, 128, 60000)])
+def test_long_sums_keep_their_bits(heads, kv, dim, n):
+    """An MMA's result is cut, not rounded, to 24 bits: sums that were kept in one over a sequence would be short by half a unit for each
+    of its hundreds of tiles.  Positive values and equal weights: the mean error of a thousand outputs is that of one cut, half of 2^-23, and
+    what rounding leaves of either sign."""
+    call, check, out, keep = case(heads, kv, dim, 64, [n, n // 2, n], amp=0.0, fill=lambda k, v: v.add_(6.0))
+    torch.cuda.synchronize()
+    pages = keep[1].numel() // (kv * q41.region_bytes(64, dim))
+    V = rows_of(keep[1], pages, kv, 64, dim, True)
+    table = keep[3].cpu().numpy()
+    rel = []
+    for b, m in enumerate((n, n // 2, n)):
+        pos = np.arange(m)
+        want = V[table[b][pos // 64].astype(np.int64) * 64 + pos % 64].mean(0)  # [kv, dim]
+        got = out[b].double().cpu().numpy().reshape(kv, heads // kv, dim)
+        rel.append(got / want[:, None] - 1)
+    rel = np.concatenate([x.reshape(-1) for x in rel])
+    assert abs(rel.mean()) <= 2.0 ** -23 and np.abs(rel).max() <= 2.0 ** -20, (rel.mean() * 2 ** 23, np.abs(rel).max() * 2 ** 23)
+
+
+@pytest.mark.parametrize("heads,kv,dim", SHAPES)
+@pytest.mark.parametrize("amp,offset", [(1.5, 1.0), (0.3, 4.0)])
+def test_as_near_as_32_bits(heads, kv, dim, amp, offset):
+    """Off from 64 bits by no more than four times what the formula on the cached values is in torch's 32 bits: operands of 22 bits are
+    off by up to four units of the 24th."""
+    lens = [672, 1500, 77]
+    call, check, out, keep = case(heads, kv, dim, 16, lens, amp=amp, offset=offset, seed=9)
+    torch.cuda.synchronize()
+    pages = keep[1].numel() // (kv * q41.region_bytes(16, dim))
+    K, V = (torch.from_numpy(rows_of(keep[i], pages, kv, 16, dim, i == 1)).to(DEV) for i in range(2))
+    table = keep[3].cpu().numpy()
+    mine, plain, size = 0.0, 0.0, 0.0
+    for b, n in enumerate(lens):
+        pos = np.arange(n)
+        at = torch.from_numpy(table[b][pos // 16].astype(np.int64) * 16 + pos % 16).to(DEV)
+        k, v = K[at].repeat_interleave(heads // kv, 1).transpose(0, 1), V[at].repeat_interleave(heads // kv, 1).transpose(0, 1)
+        q = keep[2][b].view(heads, 1, dim)
+
+        def formula(t):
+            s = (q.to(t) @ k.to(t).transpose(1, 2)) * (1 / math.sqrt(dim))
+            p = torch.exp(s - s.amax(-1, keepdim=True))
+            return ((p @ v.to(t)) / p.sum(-1, keepdim=True))[:, 0].double()
+
+        want = formula(torch.float64)
+        mine += float((out[b].view(heads, dim).double() - want).pow(2).sum())
+        plain += float((formula(torch.float32) - want).pow(2).sum())
+        size += float(want.pow(2).sum())
+    assert math.sqrt(mine) <= 4 * math.sqrt(plain) + 2.0 ** -24 * math.sqrt(size), (math.sqrt(mine / size), math.sqrt(plain / size))
