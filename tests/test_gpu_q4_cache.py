@@ -417,8 +417,9 @@ def test_long_sums_keep_their_bits(heads, kv, dim, n):
 @pytest.mark.parametrize("heads,kv,dim", SHAPES)
 @pytest.mark.parametrize("amp,offset", [(1.5, 1.0), (0.3, 4.0)])
 def test_as_near_as_32_bits(heads, kv, dim, amp, offset):
-    """Off from 64 bits by no more than four times what the formula on the cached values is in torch's 32 bits: operands of 22 bits are
-    off by up to four units of the 24th."""
+    """Off from 64 bits by no more than twelve times what the formula on the cached values is in torch's 32 bits.  Operands of 22 bits are
+    off by up to four units of the 24th; and the kernel sums a value's parts, scale times whole number and minimum, apart: between -a and
+    a these are up to 2 a and a, three times the value's bound, so that what is rounded is up to three times as large."""
     lens = [672, 1500, 77]
     call, check, out, keep = case(heads, kv, dim, 16, lens, amp=amp, offset=offset, seed=9)
     torch.cuda.synchronize()
@@ -441,4 +442,4 @@ def test_as_near_as_32_bits(heads, kv, dim, amp, offset):
         mine += float((out[b].view(heads, dim).double() - want).pow(2).sum())
         plain += float((formula(torch.float32) - want).pow(2).sum())
         size += float(want.pow(2).sum())
-    assert math.sqrt(mine) <= 4 * math.sqrt(plain) + 2.0 ** -24 * math.sqrt(size), (math.sqrt(mine / size), math.sqrt(plain / size))
+    assert math.sqrt(mine) <= 12 * math.sqrt(plain) + 2.0 ** -24 * math.sqrt(size), (math.sqrt(mine / size), math.sqrt(plain / size))
