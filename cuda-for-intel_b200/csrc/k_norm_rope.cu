@@ -18,9 +18,14 @@
 namespace {
 
 constexpr int NR_THREADS = 256, NR_RATES = 64;
-constexpr int NR_AT_ONCE = 2;  // heads whose loads are in flight together
-constexpr int NR_HEADS = 8, NR_MANY = 8;
-constexpr int NR_CTAS = 4;
+// Few rows: a head to a group of lanes.  Many: a run of up to NR_HEADS heads of one token to a group, which reads its angles once; from
+// NR_MANY heads a group of all SMs' CTAs on.  Measured, a head to a group against runs: 631 rows of 12/2 heads of 128 6.2 to 8.2 us, 300 of
+// 32/8 8.2 to 9.7, 2000 of 12/2 14.4 to 9.8, 1000 of 32/8 20.5 to 12.2.
+constexpr int NR_MANY = 8;
+// Measured, 8191 rows of 32/8 heads of 128 normed, turned and put into f16 pages, 65 us (4.6 TB/s): runs of 4, 8, 16 heads 66, 65, 73;
+// 1, 2, 4 heads' loads together 87, 65, 73; three, four, five CTAs an SM (their registers) 68, 65, 77.  The loads' latency and 190
+// instructions for two heads of a warp share the time.
+constexpr int NR_HEADS = 8, NR_AT_ONCE = 2, NR_CTAS = 4;
 
 struct NrArgs {
     CfiNormRope r;

@@ -22,6 +22,12 @@
 // Which position is which column of the scores is free, as long as the weights go back to the same: column 2 c + e of the n-th eight
 // is position 8 n + 4 e + (c ^ 3 e), so that no two lanes read the same bank of K or of V.
 // The minima of K meet the sums of q over each block in one MMA for 8 positions, those of V the weights in one for 16.
+//
+// Bound by instruction issue: an MMA of 16 x 8 x 16 holds its part of the SM for 8 cycles in which nothing else is issued (measured: 8 + N
+// cycles for one beside N other instructions), and a tile of 32 positions is 36 (five to eight heads: 68) of them and 720 other instructions
+// of a warp, where the memory's rate allows 880 cycles.  Two CTAs an SM with up to 255 registers a thread: with three, 8 to 12 % more
+// instructions, and no faster.  Measured: 8 sequences of 9000 to 65000 positions, 32/8 heads of 128, 71 us, 4.0 TB/s; 8 of 64000
+// 151 us, 4.3 TB/s (64/8 heads 175); 64 of 16 to 4096, 12/2 heads of 128, 15.0 us; one of 672, 14/2 heads of 64, 5.4 us.
 #include "paged_attn.cuh"
 #include "sm100_ptx.cuh"
 #include "cfi_kernels.h"
@@ -37,8 +43,8 @@ using namespace sm100;
 
 constexpr int P4_TILE = 32;         // positions
 // What beginning and ending a pair costs, in tiles: lengths, table, first tiles and the meeting are memory round trips after one
-// another.  Measured with 3, 6, 9 and 12: 64 sequences of 100 to 4000, 32/8 heads of 128, 44.7, 36.9, 33.9 and 34.1 us; 4 of 30000, 12/2
-// heads of 128, 25.7, 22.4, 21.4 and 21.4; 64 of 16 to 4096, 14/2 heads of 64, 11.9, 10.9, 10.9 and 11.4.
+// another.  Measured with 3, 6, 9 and 12: 64 sequences of 100 to 4000, 32/8 heads of 128, 52.8, 43.5, 39.3 and 39.2 us; 4 of 30000, 12/2
+// heads of 128, 26.1, 23.3, 22.6 and 22.5; 64 of 16 to 4096, 14/2 heads of 64, 12.0, 11.1, 11.1 and 11.5.
 constexpr int P4_FIXED = 9;
 constexpr float P4_TOP = 15.0f;     // log2 of the largest weight as it is split: f16 ends at 65504
 constexpr float P4_LEAST_V = -15.0f, P4_MOST_V = 16.0f;  // f16 has the inverse of 2^the first; scales are below 2^the second
@@ -723,11 +729,11 @@ int cfi_paged_attention_q4_1(PaArgs& a, int head_dim, long long pairs, cudaStrea
     const long long most_units = pairs * (P4_FIXED + (positions + P4_TILE - 1) / P4_TILE);
     // Short tables: a CTA to a pair, which neither reads all lengths nor joins anything; eight warps where an SM has one pair at most, four
     // otherwise.  Measured against the equal runs (us, lengths from a quarter of the longest; 14/2 heads of 64, 12/2 of 128): one
-    // sequence of 768 5.5 to 7.4 and 7.4 to 9.4, of 2048 10.5 to 7.8 and 14.8 to 9.8; 16 of 1024 6.7 to 8.8 and 9.1 to 11.3, of 2048 10.5
-    // to 9.6 and 14.9 to 11.3; 64 of 2048 10.8 to 11.1 and 15.3 to 15.4; 128 of 512 8.0 to 10.5 and 8.7 to 13.9, of 1024 12.7 to 12.2 and
-    // 14.2 to 17.1; 64 of 2048 with 32/8 heads of 128, four warps, 35.0 to 32.7.
+    // sequence of 768 5.5 to 7.4 and 7.8 to 9.7, of 1280 7.6 to 7.6 and 11.1 to 9.9, of 2048 10.8 to 7.9 and 15.7 to 10.2; 16 of 1024 6.8 to
+    // 8.9 and 9.6 to 11.6, of 2048 10.9 to 9.9 and 15.8 to 12.3; 64 of 2048 11.2 to 11.3 and 16.4 to 16.4; four warps, 128 of 512 8.3 to 10.8
+    // and 9.7 to 14.5, of 1024 13.6 to 12.5 and 15.8 to 17.8; 64 of 2048 with 32/8 heads of 128 40.7 to 37.8.
     const int sms = cfi_sm_count();
-    const int w = pairs <= sms ? (positions <= (2 * pairs > sms ? 2048 : 1280) ? 8 : 0) : positions <= (head_dim == 128 ? 1024 : 768) ? 4 : 0;
+    const int w = pairs <= sms ? (positions <= (2 * pairs > sms ? 2048 : 1024) ? 8 : 0) : positions <= (head_dim == 128 ? 1024 : 768) ? 4 : 0;
     a.whole = w > 0;
     const int variant = (head_dim == 128) * 4 + (w == 8) * 2 + (a.group <= 4);
     switch (variant) {
