@@ -83,7 +83,7 @@ CFI_DEV unsigned long long divided(float2 rate, float f) {
     const float inv = 1.0f / f, q0 = rate.x * inv;
     const float r0 = fmaf(-q0, f, rate.x) + rate.y, q1 = r0 * inv, q2 = fmaf(-q1, f, r0) * inv;
     const float two64 = 18446744073709551616.0f;
-    return __float2ull_rz((q0 - floorf(q0)) * two64) + (unsigned long long)(__float2ll_rn(q1 * two64) + __float2ll_rn(q2 * two64));
+    return (unsigned long long)(__float2ll_rn((q0 - rintf(q0)) * two64) + __float2ll_rn(q1 * two64) + __float2ll_rn(q2 * two64));
 }
 
 // TY: of the cache; F16 also where there is none.

@@ -52,6 +52,7 @@ def make(tokens, heads, kv, dim, in_type=cfi.T_F32, q_type=cfi.T_F32, kv_type=cf
     g.manual_seed(seed + tokens + heads + dim)
     rand = lambda *s: torch.randn(*s, generator=g, device=DEV)  # noqa: E731
     n_rot = dim if n_rot is None else n_rot
+    base, scale = float(np.float32(base)), float(np.float32(scale))  # as the call takes them
     dt = lambda t: torch.float32 if t == cfi.T_F32 else torch.float16  # noqa: E731
     nq, nkv = heads * dim, kv * dim
     width = nq + 2 * nkv + pad
@@ -139,7 +140,7 @@ def test_many_rows(tokens, heads, kv, dim):
 
 
 @pytest.mark.parametrize("base,scale,ff", [(1e4, 1.0, False), (1e6, 0.25, False), (5e5, 1.0, True), (1e4, 8.0, True), (1.0, 1.0, False),
-                                           (1e4, -1.0, False)])
+                                           (1e4, -1.0, False), (1e4, -1.0, True), (1e4, -0.01, True)])
 def test_angles_of_far_positions(base, scale, ff):
     """The angles' errors do not grow with the positions (a formula in 64 bits is itself off by 2^-53 of the angle)."""
     far = (1 << 24) - 1 if ff else (1 << 31) - 1

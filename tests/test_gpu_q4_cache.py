@@ -443,3 +443,36 @@ def test_as_near_as_32_bits(heads, kv, dim, amp, offset):
         plain += float((formula(torch.float32) - want).pow(2).sum())
         size += float(want.pow(2).sum())
     assert math.sqrt(mine) <= 12 * math.sqrt(plain) + 2.0 ** -24 * math.sqrt(size), (math.sqrt(mine / size), math.sqrt(plain / size))
+
+
+def test_pools_past_31_bits():
+    """Pages at the end of pools of 2.3 GB: rows stored, normed into them, read back and attended to."""
+    kv, dim, page, pages, n = 8, 128, 256, 14200, 300
+    size = cfi.paged_page_bytes(Q, page, kv, dim) * pages
+    assert size > 2 ** 31
+    kp, vp = (torch.empty(size, dtype=torch.uint8, device=DEV) for _ in "kv")
+    cache = cfi.paged_cache(Q, kp.data_ptr(), vp.data_ptr(), pages, page, kv, dim)
+    g = generator(3)
+    k, v = torch.randn(n, kv * dim, generator=g, device=DEV), torch.randn(n, kv * dim, generator=g, device=DEV)
+    table = torch.tensor([[pages - 1, pages - 7]], dtype=torch.int32, device=DEV)
+    pos = torch.arange(n, device=DEV)
+    slots = (table[0].long()[pos // page] * page + pos % page).contiguous()
+    cfi.paged_kv_store(cache, k.data_ptr(), v.data_ptr(), slots.data_ptr(), n, stream=stream())
+    rows = torch.empty(2, n, kv * dim, dtype=torch.float16, device=DEV)
+    cfi.paged_kv_load(cache, slots.data_ptr(), rows[0].data_ptr(), rows[1].data_ptr(), n, stream=stream())
+    q, out, lens = torch.randn(1, kv * dim, generator=g, device=DEV), torch.empty(1, kv * dim, device=DEV), torch.tensor([n], dtype=torch.int32, device=DEV)
+    cfi.paged_attention(cache, q.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(), 1, kv, 2, 0.1, stream=stream())
+    torch.cuda.synchronize()
+    K, V = (torch.from_numpy(q41.quantised(x.double().cpu().numpy().reshape(n, kv, dim))).to(DEV) for x in (k, v))
+    assert torch.equal(rows[0].view(n, kv, dim), K.float().half()) and torch.equal(rows[1].view(n, kv, dim), V.float().half())
+    p = torch.softmax(torch.einsum("hd,nhd->hn", q.double().view(kv, dim), K) * 0.1, -1)
+    want = torch.einsum("hn,nhd->hd", p, V)
+    assert float((out.view(kv, dim) - want).abs().max()) <= 1e-4  # 2^-13: a wrong row is off by tenths
+    kp[-1 << 20:] = 0
+    made = torch.empty(n, kv * dim, device=DEV)
+    cfi.norm_rope(cfi.norm_rope_rows(k.data_ptr(), made.data_ptr(), 0, n, kv, dim, k=k.data_ptr(), v=v.data_ptr(), n_kv_head=kv, n_rot=0,
+                                     slots=slots.data_ptr()), cache, stream=stream())
+    cfi.paged_kv_load(cache, slots.data_ptr(), rows[0].data_ptr(), rows[1].data_ptr(), n, stream=stream())
+    torch.cuda.synchronize()
+    assert torch.equal(rows[0].view(n, kv, dim), K.float().half()) and torch.equal(rows[1].view(n, kv, dim), V.float().half())
+    assert torch.equal(made, k)
