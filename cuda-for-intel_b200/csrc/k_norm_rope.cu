@@ -17,15 +17,19 @@
 
 namespace {
 
-constexpr int NR_THREADS = 256, NR_RATES = 64;
+constexpr int NR_RATES = 64;
 // Few rows: a head to a group of lanes.  Many: a run of up to NR_HEADS heads of one token to a group, which reads its angles once; from
-// NR_MANY heads a group of all SMs' CTAs on.  Measured, a head to a group against runs: 631 rows of 12/2 heads of 128 6.2 to 8.2 us, 300 of
-// 32/8 8.2 to 9.7, 2000 of 12/2 14.4 to 9.8, 1000 of 32/8 20.5 to 12.2.
+// NR_MANY heads a group of all SMs' CTAs on.  Measured, a head to a group against runs: 631 rows of 12/2 heads of 128 5.4 to 6.8 us, 300 of
+// 32/8 6.9 to 7.4, 390 8.4 to 7.7, 700 13.8 to 9.4, 1500 of 12/2 10.5 to 8.1; 1000 of 16/16 of 64 7.9 to 9.0.
 constexpr int NR_MANY = 8;
-// Measured, 8191 rows of 32/8 heads of 128 normed, turned and put into f16 pages, 65 us (4.6 TB/s): runs of 4, 8, 16 heads 66, 65, 73;
-// 1, 2, 4 heads' loads together 87, 65, 73; three, four, five CTAs an SM (their registers) 68, 65, 77.  The loads' latency and 190
-// instructions for two heads of a warp share the time.
-constexpr int NR_HEADS = 8, NR_AT_ONCE = 2, NR_CTAS = 4;
+// Measured, 8191 rows of 32/8 heads of 128 normed, turned and put into f16 pages, 61 us (5.0 TB/s): runs of 4, 8, 12, 16 heads 66, 63, 68, 73
+// (before the last step); 1, 2, 4 heads' loads together 87, 65, 73; blocks of 256, 128, 64, 32 threads 65, 64, 63, 63; 64 and 72 registers
+// (16 and 14 blocks of 64 an SM) 60.7 and 62.2, but 1000 rows 10.0 and 9.4.  Norm weights read for each head and angles
+// turned into sines after all are formed leave the 64 registers nearly unspilled: 63 to 61 us, 631 rows of 12/2 6.1 to 5.3.  The loads' latency
+// and 190 instructions for two heads of a warp share the time.
+constexpr int NR_HEADS = 8, NR_AT_ONCE = 2;
+constexpr int nr_threads(bool many) { return many ? 64 : 256; }
+constexpr int nr_ctas(int ty, bool many) { return (ty == CACHE_F16 ? 1024 : 512) / nr_threads(many); }
 
 struct NrArgs {
     CfiNormRope r;
@@ -87,16 +91,16 @@ CFI_DEV unsigned long long divided(float2 rate, float f) {
 }
 
 // TY: of the cache; F16 also where there is none.
-template <int D, bool IN_F16, int TY, int AT_ONCE>
-__global__ void __launch_bounds__(NR_THREADS, TY == CACHE_F16 ? NR_CTAS : 2) norm_rope(const __grid_constant__ NrArgs a) {
-    constexpr int G = D / 8;  // lanes of a head
-    __shared__ float4 s_row[TY == CACHE_F16 ? 1 : NR_THREADS / G][2 * G];  // a row of k or v, where the cache wants eight dims in a lane
+template <int D, bool IN_F16, int TY, bool MANY>
+__global__ void __launch_bounds__(nr_threads(MANY), nr_ctas(TY, MANY)) norm_rope(const __grid_constant__ NrArgs a) {
+    constexpr int G = D / 8, THREADS = nr_threads(MANY), AT_ONCE = MANY ? NR_AT_ONCE : 1;  // G: lanes of a head
+    __shared__ float4 s_row[TY == CACHE_F16 ? 1 : THREADS / G][2 * G];  // a row of k or v, where the cache wants eight dims in a lane
     const CfiNormRope& r = a.r;
     const int lane = threadIdx.x % G, group = threadIdx.x / G;
     const int eighth = r.n_rot / 8;  // lanes that turn
     const int d0 = lane < eighth ? 4 * lane : 8 * lane, d1 = lane < eighth ? 4 * (lane + eighth) : 8 * lane + 4;
     // this group's token and run of heads, of q (kind 0), k or v
-    const uint32_t id = blockIdx.x * (NR_THREADS / G) + group;
+    const uint32_t id = blockIdx.x * (THREADS / G) + group;
     const bool live = id < (uint32_t)r.n_tokens * a.runs;
     const int t = live ? (int)(id / a.runs) : r.n_tokens - 1, run = live ? (int)(id % a.runs) : 0;
     const int kind = run < a.begin[1] ? 0 : run < a.begin[2] ? 1 : 2;
@@ -117,11 +121,6 @@ __global__ void __launch_bounds__(NR_THREADS, TY == CACHE_F16 ? NR_CTAS : 2) nor
     const int off = (int)(slot & ((1 << a.page_shift) - 1));
     const long long region_bytes = paged_region_bytes<D, TY>(1 << a.page_shift);
     uint8_t* region = (kind == 2 ? a.v_pool : a.k_pool) + ((slot >> a.page_shift) * r.n_kv_head + h0) * region_bytes;
-    float4 w0 = make_float4(0.0f, 0.0f, 0.0f, 0.0f), w1 = w0;
-    if (norm) {
-        w0 = *reinterpret_cast<const float4*>(norm + d0);
-        w1 = *reinterpret_cast<const float4*>(norm + d1);
-    }
     float cs[4], sn[4];
     for (int i0 = 0; i0 < a.most; i0 += AT_ONCE) {
         // all loads first
@@ -139,9 +138,10 @@ __global__ void __launch_bounds__(NR_THREADS, TY == CACHE_F16 ? NR_CTAS : 2) nor
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const unsigned long long f = r.freq_factors ? divided(a.rate[4 * lane + e], r.freq_factors[4 * lane + e]) : a.turn[4 * lane + e];
-                const int angle = (int)((f * (unsigned long long)(long long)pos) >> 32);
-                sincospif((float)angle * 0x1p-31f, &sn[e], &cs[e]);
+                cs[e] = (float)(int)((f * (unsigned long long)(long long)pos) >> 32) * 0x1p-31f;
             }
+#pragma unroll
+            for (int e = 0; e < 4; e++) sincospif(cs[e], &sn[e], &cs[e]);
         }
 #pragma unroll
         for (int e = 0; e < AT_ONCE; e++) {
@@ -158,8 +158,8 @@ __global__ void __launch_bounds__(NR_THREADS, TY == CACHE_F16 ? NR_CTAS : 2) nor
                 for (int o = 1; o < G; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
                 if (norm && on) {
                     const float s = rsqrtf(ss / (float)D + r.eps);
-                    x0 = mul4(x0, s, w0);
-                    x1 = mul4(x1, s, w1);
+                    x0 = mul4(x0, s, *reinterpret_cast<const float4*>(norm + d0));
+                    x1 = mul4(x1, s, *reinterpret_cast<const float4*>(norm + d1));
                 }
             }
             if (turns) {
@@ -200,7 +200,7 @@ bool rows_ok(const void* p, long long stride, long long width) { return p && !((
 bool type_ok(int t) { return t == 0 || t == 1; }
 
 template <int D, bool IN_F16, int TY> const void* kernel(bool many) {
-    return many ? (const void*)norm_rope<D, IN_F16, TY, NR_AT_ONCE> : (const void*)norm_rope<D, IN_F16, TY, 1>;
+    return many ? (const void*)norm_rope<D, IN_F16, TY, true> : (const void*)norm_rope<D, IN_F16, TY, false>;
 }
 template <int D, bool IN_F16> const void* kernel(int ty, bool many) {
     return ty == CACHE_Q8_0   ? kernel<D, IN_F16, CACHE_Q8_0>(many)
@@ -267,9 +267,10 @@ extern "C" int cfi_norm_rope(const CfiNormRope* r, const CfiPagedCache* c, void*
     if (r->n_rot) {
         rates(r, &a);
     }
-    const int heads = r->n_head + (r->k ? r->n_kv_head : 0) + (r->v ? r->n_kv_head : 0), groups = NR_THREADS / (r->head_dim / 8);
+    const int heads = r->n_head + (r->k ? r->n_kv_head : 0) + (r->v ? r->n_kv_head : 0), lanes = r->head_dim / 8;
     if ((long long)r->n_tokens * heads > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
-    const bool many = (long long)r->n_tokens * heads >= NR_MANY * (long long)cfi_sm_count() * groups;
+    const bool many = (long long)r->n_tokens * heads >= NR_MANY * (long long)cfi_sm_count() * (nr_threads(false) / lanes);
+    const int groups = nr_threads(many) / lanes;
     const int count[3] = {r->n_head, r->k ? r->n_kv_head : 0, r->v ? r->n_kv_head : 0};
     for (int i = 0; i < 3; i++) {
         a.begin[i] = (int)a.runs;
@@ -282,7 +283,7 @@ extern "C" int cfi_norm_rope(const CfiNormRope* r, const CfiPagedCache* c, void*
     const char* ep = getenv("CFI_PDL");
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3(ctas, 1, 1);
-    lc.blockDim = dim3(NR_THREADS, 1, 1);
+    lc.blockDim = dim3((unsigned)nr_threads(many), 1, 1);
     lc.stream = static_cast<cudaStream_t>(stream);
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
