@@ -35,6 +35,7 @@ class Sequence:
         self.prompt = len(self.tokens)
         self.pages = []  # where the tables are the host's
         self.row = None  # of the device's table
+        self.placed = 0  # positions that the row may hold: more than are cached where a call did not come to its end
         self.cached = 0
         self.temperature, self.top_k, self.top_p, self.min_p = temperature, top_k, top_p, min_p
 
@@ -103,7 +104,9 @@ class Server:
     def _grow(self, seqs, lengths):
         """Pages for the sequences' positions below `lengths`: all of them, or none are taken."""
         if self.on_device:
-            need = sum(self._pages(n) - self._pages(s.cached) for s, n in zip(seqs, lengths))
+            left = [s for s in seqs if s.placed > s.cached]
+            self._trim(left, [s.cached for s in left])
+            need = sum(self._pages(n) - self._pages(s.placed) for s, n in zip(seqs, lengths))
             if need > self.n_free:
                 raise OutOfPages("%d pages are free" % self.n_free)
             fresh = [s for s in seqs if s.row is None]
@@ -111,7 +114,10 @@ class Server:
                 raise OutOfPages("%d rows of the page table are free" % len(self.rows))
             for s in fresh:
                 s.row = self.rows.pop()
+            # before the device's table has them: what a call that fails from here on leaves behind is cut back by the next
             self.n_free -= need
+            for s, n in zip(seqs, lengths):
+                s.placed = n
             return
         need = [self._pages(n) - len(s.pages) for s, n in zip(seqs, lengths)]
         if sum(x for x in need if x > 0) > len(self.free):
@@ -119,16 +125,23 @@ class Server:
         for s, x in zip(seqs, need):
             s.pages += [self.free.pop() for _ in range(x)]
 
+    def _trim(self, seqs, lengths):
+        """The device's table keeps the sequences' first lengths[i] positions."""
+        if not seqs:
+            return
+        rows, keep, status = self._int([s.row for s in seqs]), self._int(lengths), self._int([0])
+        cfi.paged_trim(self.table, rows.data_ptr(), keep.data_ptr(), len(seqs), status.data_ptr(), stream=self.stream)
+        self.n_free += sum(self._pages(s.placed) - self._pages(n) for s, n in zip(seqs, lengths))
+        for s, n in zip(seqs, lengths):
+            s.placed = n
+        self.state.status |= status
+
     def _shrink(self, seqs, lengths):
         """The pages behind the sequences' first lengths[i] positions go back."""
         lengths = [min(s.cached, max(n, 0)) for s, n in zip(seqs, lengths)]
         if self.on_device:
             mine = [(s, n) for s, n in zip(seqs, lengths) if s.row is not None]
-            if mine:
-                rows, keep, status = self._int([s.row for s, _ in mine]), self._int([n for _, n in mine]), self._int([0])
-                cfi.paged_trim(self.table, rows.data_ptr(), keep.data_ptr(), len(mine), status.data_ptr(), stream=self.stream)
-                self.state.status |= status
-            self.n_free += sum(self._pages(s.cached) - self._pages(n) for s, n in mine)
+            self._trim([s for s, _ in mine], [n for _, n in mine])
         else:
             for s, n in zip(seqs[::-1], lengths[::-1]):
                 while len(s.pages) > self._pages(n):
