@@ -37,6 +37,7 @@ class Sequence:
         self.row = None  # of the device's table
         self.placed = 0  # positions that the row may hold: more than are cached where a call did not come to its end
         self.cached = 0
+        self.sure = 0  # of these, what was there at the last tokens: where the table is the device's
         self.temperature, self.top_k, self.top_p, self.min_p = temperature, top_k, top_p, min_p
 
 
@@ -75,6 +76,7 @@ class Server:
         self.on_device = tables == "device"
         if self.on_device:
             self.n_free, self.rows = pages, list(range(rows))[::-1]  # of which the host keeps count alone
+            self.owner = {}  # the sequence of a row
             state = dict(table=torch.zeros(rows, pages, dtype=torch.int32, device=self.dev), cached=self._int([0] * rows),
                          free=self._int(self.free), n_free=self._int([pages]), status=self._int([0]))
             self.state = SimpleNamespace(**state)
@@ -114,6 +116,7 @@ class Server:
                 raise OutOfPages("%d rows of the page table are free" % len(self.rows))
             for s in fresh:
                 s.row = self.rows.pop()
+                s.sure, self.owner[s.row] = 0, s
             # before the device's table has them: what a call that fails from here on leaves behind is cut back by the next
             self.n_free -= need
             for s, n in zip(seqs, lengths):
@@ -147,7 +150,27 @@ class Server:
                 while len(s.pages) > self._pages(n):
                     self.free.append(s.pages.pop())
         for s, n in zip(seqs, lengths):
-            s.cached = n
+            s.cached, s.sure = n, min(s.sure, n)
+
+    def _told(self):
+        """The page table's status, which is then clear.  Where calls were refused, the sequences have again what they had when it was last
+        clear, and the host's counts are the device's."""
+        status = int(self.state.status)
+        if status == 0:
+            for s in self.owner.values():
+                s.sure = s.cached
+            return 0
+        self.state.status.zero_()
+        held = self.state.cached.tolist()
+        left = [r for r in self.rows if held[r]]  # of sequences that are released
+        if left:
+            rows, keep = self._int(left), self._int([0] * len(left))
+            cfi.paged_trim(self.table, rows.data_ptr(), keep.data_ptr(), len(left), self.state.status.data_ptr(), stream=self.stream)
+        self.n_free = int(self.state.n_free)
+        for r, s in self.owner.items():
+            s.placed = held[r]
+            s.cached = s.sure = min(s.sure, held[r])
+        return status
 
     def cut(self, seqs, lengths):
         """The sequences keep their first lengths[i] tokens and what is cached of them (drafted tokens that were not taken, say): the
@@ -169,6 +192,7 @@ class Server:
         self._begin()
         self._shrink([seq], [0])
         if seq.row is not None:
+            del self.owner[seq.row]
             self.rows.append(seq.row)
             seq.row = None
 
@@ -335,8 +359,9 @@ class Server:
         cfi.sample(logits.data_ptr(), u.data_ptr(), token.data_ptr(), n, self.c.vocab, temperature.data_ptr(), top_k.data_ptr(),
                    top_p.data_ptr(), min_p.data_ptr(), logprob.data_ptr(), stream=self.stream)
         drawn = token.tolist()
-        if self.on_device and int(self.state.status):
-            raise RuntimeError("the page table's calls were refused (%d): what was cached since the last tokens is void" % int(self.state.status))
+        refused = self._told() if self.on_device else 0
+        if refused:
+            raise RuntimeError("the page table's calls were refused (%d): what was cached since the last tokens is void" % refused)
         error = cfi.device_error()
         if error:
             raise RuntimeError("a kernel's wait ran out (0x%x): the logits and what was cached since the last tokens are void" % error)

@@ -200,3 +200,51 @@ def test_a_failed_trim_again(held):
     assert held.attended[-1] == [11] and a.cached == 11
     s.release(a)
     assert free_pages(s) == 8
+
+
+@pytest.mark.parametrize("call", ["step", "prompt"])
+def test_a_refused_place_is_told_once(held, call):
+    """The sample after it raises; the sequences then have what they had at the last tokens, and everything can be done again."""
+    s = held.build(cfi.Q4_1, pages=8, tables="device")
+    a, b = serve.Sequence(list(range(16))), serve.Sequence([1] * 20)
+    s.sample([a], s.prefill([a]))
+    held.refuse[:] = [cfi.PLACE_NO_PAGES]
+    logits = s.step([a]) if call == "step" else s.prefill([b], [18])
+    if call == "prompt":
+        s.prefill([b])  # placed, but at the wrong positions: void
+        s.step([a])  # placed as it should be; nothing says so
+    with pytest.raises(RuntimeError, match="refused"):
+        s.sample([a], logits)
+    assert (a.cached, b.cached, len(a.tokens)) == (16, 0, 17)
+    stored, lengths = run(held, s, lambda: s.prefill([b]), lambda: s.step([a]))
+    assert [x[1] for x in stored] == [list(range(20))] * 2 + [[16]] * 2 and lengths == [[17]] * 2
+    slots = stored[0][0] + stored[2][0]
+    assert len(set(slots)) == 21 and free_pages(s) == 8 - 2 - 2
+    s.sample([a], logits)  # in order again
+    assert len(a.tokens) == 18
+    s.release(a), s.release(b)
+    assert free_pages(s) == 8 and int(s.state.status) == 0
+
+
+@pytest.mark.parametrize("released", [False, True])
+def test_a_refused_trim_is_told_once(held, released):
+    """Its pages go back then, and a row that was given back is empty for the next sequence."""
+    s = held.build(cfi.Q4_1, pages=8, tables="device", rows=2)
+    a, b = serve.Sequence(list(range(40))), serve.Sequence([1])
+    logits = s.prefill([a, b])
+    s.sample([b], logits)
+    held.refuse[:] = [cfi.PLACE_NO_PAGES]
+    s.release(a) if released else s.cut([a], [5])
+    with pytest.raises(RuntimeError, match="refused"):
+        s.sample([b], logits)
+    assert a.cached == (0 if released else 5)
+    if released:
+        assert free_pages(s) == 7
+        a = serve.Sequence([3] * 17)
+        assert run(held, s, lambda: s.prefill([a]))[0][0][1] == list(range(17))
+    else:
+        a.tokens.append(2)
+        assert run(held, s, lambda: s.step([a]))[1][0] == [6]
+    s.sample([b], logits)
+    s.release(a), s.release(b)
+    assert free_pages(s) == 8
