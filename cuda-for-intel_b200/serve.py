@@ -103,9 +103,14 @@ class Server:
     def _pages(self, positions):
         return -(-positions // self.page_size)
 
+    def _once(self, seqs):
+        if len({id(s) for s in seqs}) < len(seqs):
+            raise ValueError("a sequence is named twice")
+
     def _grow(self, seqs, lengths):
         """Pages for the sequences' positions below `lengths`: all of them, or none are taken."""
         if self.on_device:
+            self._once(seqs)
             left = [s for s in seqs if s.placed > s.cached]
             self._trim(left, [s.cached for s in left])
             need = sum(self._pages(n) - self._pages(s.placed) for s, n in zip(seqs, lengths))
@@ -175,8 +180,7 @@ class Server:
     def cut(self, seqs, lengths):
         """The sequences keep their first lengths[i] tokens and what is cached of them (drafted tokens that were not taken, say): the
         pages behind go back."""
-        if len({id(s) for s in seqs}) < len(seqs):
-            raise ValueError("a sequence is named twice")
+        self._once(seqs)
         self._begin()
         self._shrink(seqs, lengths)
         for s, n in zip(seqs, lengths):

@@ -248,3 +248,19 @@ def test_a_refused_trim_is_told_once(held, released):
     s.sample([b], logits)
     s.release(a), s.release(b)
     assert free_pages(s) == 8
+
+
+def test_a_sequence_named_twice(held):
+    """Its row cannot be placed twice in one call of the page table: refused before a page or a row is taken."""
+    s = held.build(cfi.Q4_1, pages=8, tables="device", rows=2)
+    a, b = serve.Sequence(list(range(20))), serve.Sequence([1])
+    with pytest.raises(ValueError, match="twice"):
+        s.prefill([a, b, a])
+    assert a.row is None and len(s.rows) == 2 and free_pages(s) == 8
+    s.prefill([a, b])
+    a.tokens.append(1)
+    with pytest.raises(ValueError, match="twice"):
+        s.step([a, a])
+    assert a.cached == 20
+    assert run(held, s, lambda: s.step([a]))[1][0] == [21]
+    s.sample([a], torch.zeros(1, 64))
