@@ -65,12 +65,16 @@ class Server:
             raise ValueError("norms are two vectors for each layer of a fused server")
         if tables not in ("host", "device"):
             raise ValueError("tables are the host's or the device's")
-        self.norms = norms
+        self.norms = [tuple(pair) for pair in norms] if norms is not None else None
         self.fused = cache_type == cfi.Q4_1 or norms is not None if fused is None else fused
         # the pools, [layer][K or V][page]: a program keeps the description of each beside them
         self.pools = torch.zeros(c.layers, 2, pages * n, dtype=torch.uint8, device=self.dev)
         self.caches = [cfi.paged_cache(cache_type, p[0].data_ptr(), p[1].data_ptr(), pages, page_size, c.n_kv_head, c.head_dim)
                        for p in self.pools]
+        for pair in self.norms or ():  # the kernels are given their addresses
+            if len(pair) != 2 or not all(torch.is_tensor(w) and w.dtype == torch.float32 and w.shape == (c.head_dim,) and w.is_contiguous() and
+                                         w.device == self.pools.device and w.data_ptr() % 16 == 0 for w in pair):
+                raise ValueError("norms are two contiguous f32 vectors of %d on %s for each layer" % (c.head_dim, self.pools.device))
         self.free = list(range(pages))[::-1]  # where the tables are the host's
         self.held = [self.pools]
         self.on_device = tables == "device"

@@ -264,3 +264,19 @@ def test_a_sequence_named_twice(held):
     assert a.cached == 20
     assert run(held, s, lambda: s.step([a]))[1][0] == [21]
     s.sample([a], torch.zeros(1, 64))
+
+
+def test_norms_that_a_kernel_cannot_read(held):
+    """Another type, length, layout or device, or not two of a layer: refused when the server is made, not read by address."""
+    good = torch.ones(64)
+    for bad in (torch.ones(64, dtype=torch.float16), torch.ones(32), torch.ones(128)[::2], torch.ones(64, device="meta"), torch.ones(65)[1:],
+                [1.0] * 64):
+        for pair in ((good, bad), (bad, good)):
+            with pytest.raises(ValueError, match="norms"):
+                held.build(norms=[(good, good), pair])
+    for layer in ((good,), (good, good, good)):
+        with pytest.raises(ValueError, match="norms"):
+            held.build(norms=[layer, (good, good)])
+    s = held.build(norms=[(good, good), torch.ones(2, 64)])
+    s.prefill([serve.Sequence([1, 2])])
+    assert len(held.stored) == 2
