@@ -47,7 +47,7 @@ constexpr int P4_TILE = 32;         // positions
 // heads of 128, 26.1, 23.3, 22.6 and 22.5; 64 of 16 to 4096, 14/2 heads of 64, 12.0, 11.1, 11.1 and 11.5.
 constexpr int P4_FIXED = 9;
 constexpr float P4_TOP = 15.0f;     // log2 of the largest weight as it is split: f16 ends at 65504
-constexpr float P4_LEAST_V = -15.0f, P4_MOST_V = 16.0f;  // f16 has the inverse of 2^the first; scales are below 2^the second
+constexpr float P4_LEAST_V = -15.0f;  // f16 has the inverse of 2^this
 using Cut = PaCut<P4_TILE, P4_FIXED>;
 
 template <int D, int W = PA_WARPS> struct P4Shape {
@@ -149,6 +149,8 @@ struct Nibbles {
 // column 2 c + e of the n-th eight scores
 CFI_DEV int position_of(int c, int e, int n) { return 8 * n + 4 * e + (c ^ (3 * e)); }
 
+CFI_DEV __half2 as_h2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
+
 // The largest of V's scales so far: they have been below 2^top, and what the weights are multiplied by is divided by it.
 struct ScalesTop {
     float top, per;  // per: 2^-top
@@ -171,10 +173,14 @@ struct ScalesTop {
         }
         *by = 1.0f;
         if (__any_sync(0xffffffffu, !__hblt2(most, limit))) {
-            // the exponent of the largest, cut where that is an infinity or a NaN
+            // the exponent of the largest finite one: an infinity or a NaN spoils its own dims and says nothing of the others
+            most = __float2half2_rn(0.0f);
+#pragma unroll
+            for (int x = 0; x < D / 64; x++)
+                most = __hmax2(most, as_h2(h2_bits(d[x]) & __hlt2_mask(d[x], __half2half2(__ushort_as_half(0x7c00)))));
             const uint32_t ex = __float_as_uint(fmaxf(__low2float(most), __high2float(most))) >> 23;
             const float old = top;
-            set(fmaxf(top, fminf((float)__reduce_max_sync(0xffffffffu, ex) - 126.0f, P4_MOST_V)));
+            set(fmaxf(top, (float)__reduce_max_sync(0xffffffffu, ex) - 126.0f));
             *by = ex2(old - top);
         }
         uint32_t small = 0;
@@ -183,8 +189,6 @@ struct ScalesTop {
         return __any_sync(0xffffffffu, small != 0);
     }
 };
-CFI_DEV __half2 as_h2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
-
 // Scales of two rows of blocks 0, 1 and 2, 3
 template <int D> CFI_DEV void scales_of(uint32_t tile, int row, uint32_t (&d)[D / 64]) {
     const uint32_t p = tile + Q41<D>::NIBBLES + row * Q41<D>::PARAM_ROW;

@@ -1,0 +1,89 @@
+"""Serving operators (include/cfi_serve.h) where a bad value lies beside good ones, against 64 bits.
+
+Bounds of the attention, as in test_gpu_q4_cache.py: a score is off by EPS_S = 2^-20 of the sum of the magnitudes that are added for it, a
+weight by twice that and 2^-20, an output by this times the largest magnitude of V's parts."""
+import math
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+import cfi_b200 as cfi  # noqa: E402
+import q41_pages as q41  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+EPS_S = 2.0 ** -20
+DEV = "cuda"
+
+
+def stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def q8_values(pool, pages, kv, page, dim):
+    """Every slot of a Q8_0 pool in 64 bits: [slot, head, dim]."""
+    x = pool.cpu().numpy().reshape(pages, kv, page * dim // 16 * 17)
+    q = x[..., :page * dim].view(np.int8).reshape(pages, kv, page, dim).astype(np.float64)
+    d = np.ascontiguousarray(x[..., page * dim:]).view(np.float16).astype(np.float64).reshape(pages, kv, page, dim // 32)
+    with np.errstate(invalid="ignore"):
+        v = q * np.repeat(d, 32, axis=3)
+    return v.transpose(0, 2, 1, 3).reshape(pages * page, kv, dim)
+
+
+# ---- what a bad block of V leaves the other dims ----
+@pytest.mark.parametrize("ty", [cfi.Q4_1])
+@pytest.mark.parametrize("heads,kv,dim,blocks", [(3, 1, 64, [1]), (16, 2, 64, [0]), (6, 2, 128, [1]), (6, 2, 128, [0, 1]),
+                                                 (7, 1, 128, [0, 1, 3]), (12, 2, 128, [2, 3])])
+@pytest.mark.parametrize("at", [0, 70])
+@pytest.mark.parametrize("bad", [float("nan"), 1e7])
+def test_bad_blocks_of_v_cost_the_other_dims_nothing(ty, heads, kv, dim, blocks, at, bad):
+    """Ordinary values of 1e-4 beside blocks whose scales are not finite (1e7 / 127 passes f16, and is an infinity in Q8_0's pages):
+    the dims of other blocks are as near to the formula as without it.  (Small queries: the scores' part of the bound is small too.)"""
+    page, lens = 16, [80, 3000]
+    g = torch.Generator(device=DEV)
+    g.manual_seed(heads + dim + at)
+    pages = sum(-(-n // page) for n in lens)
+    n = cfi.paged_page_bytes(ty, page, kv, dim) * pages
+    pools = torch.zeros(2, n, dtype=torch.uint8, device=DEV)
+    cache = cfi.paged_cache(ty, pools[0].data_ptr(), pools[1].data_ptr(), pages, page, kv, dim)
+    width = max(-(-n // page) for n in lens)
+    order = torch.randperm(pages, generator=g, device=DEV)
+    table = torch.zeros(2, width, dtype=torch.int32, device=DEV)
+    own = (order[:-(-lens[0] // page)], order[-(-lens[0] // page):])
+    slots = []
+    for b in range(2):
+        table[b, :len(own[b])] = own[b]
+        pos = torch.arange(lens[b], device=DEV)
+        slots.append(own[b][pos // page] * page + pos % page)
+    k, v = (torch.randn(sum(lens), kv * dim, generator=g, device=DEV) for _ in "kv")
+    v *= 1e-4
+    for i in blocks:  # of kv head 0, of both sequences
+        v[at, 32 * i + 5] = v[80 + at, 32 * i + 5] = bad
+    all_slots = torch.cat(slots).contiguous()
+    cfi.paged_kv_store(cache, k.data_ptr(), v.data_ptr(), all_slots.data_ptr(), sum(lens), stream=stream())
+    q = torch.randn(2, heads * dim, generator=g, device=DEV) * 0.02
+    out, dl = torch.empty(2, heads * dim, device=DEV), torch.tensor(lens, dtype=torch.int32, device=DEV)
+    scale = 1 / math.sqrt(dim)
+    cfi.paged_attention(cache, q.data_ptr(), out.data_ptr(), table.data_ptr(), dl.data_ptr(), 2, heads, width, scale, stream=stream())
+    torch.cuda.synchronize()
+    if ty == cfi.Q4_1:
+        K, V = (q41.values(pools[i].cpu().numpy(), pages, kv, page, dim, i == 1) for i in range(2))
+    else:
+        K, V = (q8_values(pools[i], pages, kv, page, dim) for i in range(2))
+    got, qq = out.double().cpu().numpy().reshape(2, heads, dim), q.double().cpu().numpy().reshape(2, heads, dim)
+    spoilt = np.concatenate([np.arange(32 * i, 32 * i + 32) for i in blocks])
+    clean = np.setdiff1d(np.arange(dim), spoilt)
+    for b in range(2):
+        sl = slots[b].cpu().numpy()
+        for h in range(heads):
+            kk, vv = K[sl, h * kv // heads], V[sl, h * kv // heads]
+            dims = clean if h * kv // heads == 0 else np.arange(dim)
+            assert np.isfinite(got[b, h, spoilt]).any() == (h * kv // heads != 0)
+            s = kk @ qq[b, h] * scale
+            p = np.exp(s - s.max())
+            want = p @ vv[:, dims] / p.sum()
+            ends = lambda x: np.repeat(np.abs(x.reshape(len(x), -1, 32)).max(2) * 3, 32, axis=1)  # noqa: E731
+            mags = float((np.abs(qq[b, h]) @ ends(kk).T).max() * scale)
+            tol = (2 * EPS_S * mags + 2 * 2.0 ** -20) * 3 * np.abs(vv[:, dims]).max()
+            err = np.abs(got[b, h][dims] - want).max()
+            assert err <= tol, (b, h, err / tol)
