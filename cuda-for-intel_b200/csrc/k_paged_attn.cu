@@ -43,7 +43,7 @@ using namespace sm100;
 
 constexpr int PA_TILE = 16;        // positions; a page is a multiple of it
 constexpr float PA_TOP = 15.0f;    // log2 of the largest weight as it is split: f16 ends at 65504
-constexpr float PA_LEAST_V = -23.0f, PA_MOST_V = 16.0f;  // f16 scales are below 2^these
+constexpr float PA_LEAST_V = -23.0f;  // log2 of what V's scales are taken to be below at first
 constexpr int PA_FIXED = 5;        // what beginning and ending a pair costs, in tiles
 using Cut = PaCut<PA_TILE, PA_FIXED>;
 
@@ -297,9 +297,9 @@ __global__ void __launch_bounds__(W * 32, (PaShape<D, Q8, W>::CTAS)) paged_attn(
                 // a lane looks at two of the tile's scales
                 const __half2 d = abs_h2(lds32(ss + S::SCALES + (lane * 4 & (D - 1))));
                 if (__any_sync(0xffffffffu, !__hblt2(d, limit_v))) {
-                    // the exponent of the largest, cut where that is an infinity or a NaN
-                    const uint32_t exponent = __float_as_uint(fmaxf(__low2float(d), __high2float(d))) >> 23;
-                    const float grown = fmaxf(top_v, fminf((float)__reduce_max_sync(0xffffffffu, exponent) - 126.0f, PA_MOST_V));
+                    // the exponent of the largest finite one: an infinity or a NaN spoils its own dims and says nothing of the others
+                    const float lo = __low2float(d), hi = __high2float(d), finite = fmaxf(lo < INFINITY ? lo : 0.0f, hi < INFINITY ? hi : 0.0f);
+                    const float grown = fmaxf(top_v, (float)__reduce_max_sync(0xffffffffu, __float_as_uint(finite) >> 23) - 126.0f);
                     const float f = ex2(top_v - grown);
                     l *= f;
 #pragma unroll

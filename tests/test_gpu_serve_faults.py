@@ -31,7 +31,7 @@ def q8_values(pool, pages, kv, page, dim):
 
 
 # ---- what a bad block of V leaves the other dims ----
-@pytest.mark.parametrize("ty", [cfi.Q4_1])
+@pytest.mark.parametrize("ty", [cfi.Q4_1, cfi.Q8_0])
 @pytest.mark.parametrize("heads,kv,dim,blocks", [(3, 1, 64, [1]), (16, 2, 64, [0]), (6, 2, 128, [1]), (6, 2, 128, [0, 1]),
                                                  (7, 1, 128, [0, 1, 3]), (12, 2, 128, [2, 3])])
 @pytest.mark.parametrize("at", [0, 70])
