@@ -6,7 +6,7 @@
 // quotient in 32 bits is off by less than 2^-16 (2^-24 of it each by range and difference, 2^-22 by the quotient): where a value of a
 // warp comes nearer to a border than that, its values are compared with their borders, 30 (x - min) with (2 q + 1) (max - min), as sums of
 // two f32 numbers each (differences of f16 values meet borders exactly).  d is off by 2 units of its last place in 32 bits and worked out
-// in 64 where a border of f16 is nearer.
+// in 64 (a difference that 64 bits do not hold as the sum of two) where a border of f16 is nearer.
 #pragma once
 #include "paged_cache.cuh"
 
@@ -105,6 +105,15 @@ template <bool SRC_F16> CFI_DEV void block_ends(const Row8& r, float* lo, float*
     }
 }
 
+// a - b, and what that was rounded by
+struct Apart {
+    double x, rest;
+};
+CFI_DEV Apart apart(double a, double b) {
+    const double x = a - b, back = x - a;
+    return {x, (a - (x - back)) - (b + back)};
+}
+
 template <int D, bool SRC_F16> CFI_DEV void put_q4_1(const Row8& r, uint8_t* region, int off, int g, bool of_v, bool ok) {
     float lo, hi;
     block_ends<SRC_F16>(r, &lo, &hi);
@@ -137,13 +146,20 @@ template <int D, bool SRC_F16> CFI_DEV void put_q4_1(const Row8& r, uint8_t* reg
     }
     uint16_t d = f2h_bits(d32);
     if (wide || tie) {
-        const double exact = (double)hi - (double)lo;
-        d = __half_as_ushort(__double2half(exact / 15.0));
+        const Apart all = apart(hi, lo);
+        double d64 = all.x / 15.0;
+        // exactly so: what the difference was rounded by decides where d lies on a border
+        if (all.rest != 0.0 && fma(-15.0, d64, all.x) == 0.0) d64 = __longlong_as_double(__double_as_longlong(d64) + (all.rest > 0.0 ? 1 : -1));
+        d = __half_as_ushort(__double2half(d64));
         if (wide) {
             w = 0;
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                w |= exact > 0.0 ? (uint32_t)(int)floor(((double)r.x[j] - (double)lo) * 15.0 / exact + 0.5) << (4 * j) : 0;
+            for (int j = 0; j < 8; j++) {
+                const Apart t = apart(r.x[j], lo);
+                const double v = t.x * 15.0 / all.x, near = rint(v), twice = 2.0 * near + (v >= near ? 1.0 : -1.0), p = twice * all.x;
+                const double over = (fma(30.0, t.x, -p) - fma(twice, all.x, -p)) + fma(30.0, t.rest, -twice * all.rest);
+                w |= all.x > 0.0 ? (uint32_t)((int)(twice + (over >= 0.0 ? 1.0 : -1.0)) >> 1) << (4 * j) : 0;
+            }
         }
     }
     uint16_t m = f2h_bits(lo);

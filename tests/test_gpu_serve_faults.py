@@ -1,8 +1,10 @@
-"""Serving operators (include/cfi_serve.h) where a bad value lies beside good ones, against 64 bits.
+"""Serving operators (include/cfi_serve.h) where a bad value lies beside good ones and where values meet borders, against 64 bits and
+fractions.
 
 Bounds of the attention, as in test_gpu_q4_cache.py: a score is off by EPS_S = 2^-20 of the sum of the magnitudes that are added for it, a
 weight by twice that and 2^-20, an output by this times the largest magnitude of V's parts."""
 import math
+from fractions import Fraction
 
 import numpy as np
 import pytest
@@ -87,3 +89,45 @@ def test_bad_blocks_of_v_cost_the_other_dims_nothing(ty, heads, kv, dim, blocks,
             tol = (2 * EPS_S * mags + 2 * 2.0 ** -20) * 3 * np.abs(vv[:, dims]).max()
             err = np.abs(got[b, h][dims] - want).max()
             assert err <= tol, (b, h, err / tol)
+
+
+# ---- Q4_1 values on borders, beside a minimum far below them ----
+def exactly(block):
+    """Scale (f16), minimum (f16) and whole numbers of a block, from fractions."""
+    if abs(block.min()) >= 65520:
+        return math.nan, math.nan, [0] * 32
+    x = [Fraction(float(v)) for v in block]
+    lo, wide = min(x), max(x) - min(x)
+    exact = wide / 15
+    near = np.float16(float(exact))
+    around = [np.nextafter(near, np.float16(-np.inf)), near, np.nextafter(near, np.float16(np.inf))]
+    d = min(around, key=lambda c: (abs(Fraction(float(c)) - exact), int(np.float16(c).view(np.uint16)) & 1))
+    return float(d), float(np.float16(block.min())), [int((v - lo) * 15 / wide + Fraction(1, 2)) if wide else 0 for v in x]
+
+
+def test_scales_and_values_on_borders():
+    """Scale and quotients are rounded from their exact values: a minimum that only just is not zero decides where the rest lies on a border,
+    with scales among f16's normal numbers, below them and large."""
+    blocks = []
+    for low in (2.0 ** -100, 2.0 ** -60, 2.0 ** -40, 2.0 ** -30, 1e-38):
+        for sign in (-1, 0, 1):
+            for step in (1 + 2.0 ** -11, 1 + 3 * 2.0 ** -11, 2.0 ** -15, 2.0 ** -17 * 1.5, 2.0 ** -20, 2.0 ** -24 * 2.5, 700.0 + 0.25, 61000.0, 5.0):
+                b = [(i + 0.5) * step for i in range(15)] + [i * step for i in range(1, 16)] + [15 * step]
+                blocks.append([sign * low] + b)
+    x = np.array(blocks, dtype=np.float32)
+    assert x.shape[1] == 32
+    rng = np.random.default_rng(1)
+    x = np.concatenate([x, -x, rng.permuted(x, axis=1)])
+    x = np.concatenate([x, np.zeros((-len(x) % 4, 32), dtype=np.float32)])
+    n, page = len(x) // 4, 16
+    pages = -(-n // page)
+    rows = torch.from_numpy(x.reshape(n, 128)).to(DEV)
+    pools = torch.zeros(2, cfi.paged_page_bytes(cfi.Q4_1, page, 1, 128) * pages, dtype=torch.uint8, device=DEV)
+    cache = cfi.paged_cache(cfi.Q4_1, pools[0].data_ptr(), pools[1].data_ptr(), pages, page, 1, 128)
+    slots = torch.arange(n, device=DEV)
+    cfi.paged_kv_store(cache, rows.data_ptr(), rows.data_ptr(), slots.data_ptr(), n, stream=stream())
+    torch.cuda.synchronize()
+    want = np.array([[q * d + m for q in qs] for d, m, qs in map(exactly, x)]).reshape(n, 128)
+    for i in range(2):
+        got = q41.values(pools[i].cpu().numpy(), pages, 1, page, 128, i == 1)[:n, 0]
+        np.testing.assert_array_equal(got, want)
