@@ -104,8 +104,9 @@ CFI_API int cfi_paged_attention(const CfiPagedCache *cache, const void *q, int q
  *   for i < n_rot / 2: (x[i], x[i + n_rot/2]) turned by the angle
  *     pos[t] * freq_scale * freq_base^(-2 i / n_rot) / freq_factors[i]    (freq_factors NULL: ones);
  *   what lies at n_rot and behind is not turned.
- * The angle is formed modulo a turn in 64 bits: it is off by 1e-7 rad at most at any position (with freq_factors, and positions
- * below 2^24).
+ * The angle is formed modulo a turn in 64 bits and rounded once to 32.  With theta the pair's angle at position 1, up to 2^24 rad, it is
+ * off, before its sine and cosine, by 1e-7 rad and |pos| * max(1, |theta|) * 2^-53 rad at most; with freq_factors, which are part of
+ * theta, by 1e-7 rad and |pos| * max(1, |theta|) * 2^-45 rad.
  * q_out, k_out and v_out get the rows (F32 or F16); with `cache` the rows of k and v also go to its slots, as
  * cfi_paged_kv_store would put them there (from 32 bits).  A slot outside the pool stores nothing.
  * q: n_head heads, k and v: n_kv_head; in_type, q_out_type, kv_out_type 0 F32 or 1 F16; biases and norms F32;

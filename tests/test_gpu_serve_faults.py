@@ -1,9 +1,10 @@
-"""Serving operators (include/cfi_serve.h) where a bad value lies beside good ones and where values meet borders, against 64 bits and
-fractions.
+"""Serving operators (include/cfi_serve.h) where a bad value lies beside good ones, where values meet borders, and angles to their bound,
+against 64 bits and more.
 
 Bounds of the attention, as in test_gpu_q4_cache.py: a score is off by EPS_S = 2^-20 of the sum of the magnitudes that are added for it, a
 weight by twice that and 2^-20, an output by this times the largest magnitude of V's parts."""
 import math
+from decimal import Decimal, localcontext
 from fractions import Fraction
 
 import numpy as np
@@ -131,3 +132,43 @@ def test_scales_and_values_on_borders():
     for i in range(2):
         got = q41.values(pools[i].cpu().numpy(), pages, 1, page, 128, i == 1)[:n, 0]
         np.testing.assert_array_equal(got, want)
+
+
+# ---- angles ----
+PI = Decimal("3.14159265358979323846264338327950288419716939937510582097494459230781640628620899862803")
+
+
+@pytest.mark.parametrize("base,scale,lo,hi", [(1e4, 1.0, 1.0, 4.0), (1e4, 8.0, 1.0, 4.0), (1e4, 1.0, 0.05, 0.2), (5e5, 8.0, 0.05, 0.2),
+                                              (1e4, -1.0, 0.5, 1.0), (1e6, 1.0, None, None), (1e4, 8.0, None, None), (0.5, 1.0, None, None),
+                                              (1e4, 300.0, None, None), (1.01, 1.0, None, None)])
+def test_angles_to_their_bound(base, scale, lo, hi):
+    """Pairs of (1, 0) come out as cosine and sine, which are off by a unit of the last place, 2^-23 of themselves: together by 2^-23 rad."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(int(base) + int(scale))
+    n, dim = 60, 128
+    far = (1 << 31) - 1
+    pos = torch.randint(1 << 23, 1 << 24, (n,), generator=g, device=DEV).to(torch.int32)
+    pos[::3] = torch.randint(far // 2, far, (n // 3,), generator=g, device=DEV).to(torch.int32)
+    pos[:5] = torch.tensor([0, 1, far, -far, 4097])
+    rows = torch.zeros(n, dim, device=DEV)
+    rows[:, :dim // 2] = 1.0
+    ff = (lo + (hi - lo) * torch.rand(dim // 2, generator=g, device=DEV)).float() if lo else None
+    out = torch.empty(n, dim, device=DEV)
+    cfi.norm_rope(cfi.norm_rope_rows(rows.data_ptr(), out.data_ptr(), pos.data_ptr(), n, 1, dim, freq_base=base, freq_scale=scale,
+                                     freq_factors=ff.data_ptr() if lo else 0), stream=stream())
+    torch.cuda.synchronize()
+    got, pos = out.double().cpu().numpy(), pos.tolist()
+    factors = ff.double().cpu().tolist() if lo else [1.0] * (dim // 2)
+    worst = 0.0
+    with localcontext() as c:
+        c.prec = 60
+        b, s = Decimal(float(np.float32(base))), Decimal(float(np.float32(scale)))
+        for i in range(dim // 2):
+            rate = s * (b.ln() * Decimal(-2 * i) / dim).exp() / Decimal(factors[i])
+            for t in range(n):
+                angle = rate * pos[t]
+                a = float(angle - (angle / (2 * PI)).to_integral_value() * 2 * PI)
+                err = abs(got[t, i + dim // 2] * math.cos(a) - got[t, i] * math.sin(a))
+                bound = 1e-7 + abs(pos[t]) * max(1.0, abs(float(rate))) * 2.0 ** (-45 if lo else -53)
+                worst = max(worst, err / (bound + 2.0 ** -23))
+    assert worst <= 1.0, worst
