@@ -1,5 +1,5 @@
-"""Serving operators (include/cfi_serve.h) where a bad value lies beside good ones, where values meet borders, and angles to their bound,
-against 64 bits and more.
+"""Serving operators (include/cfi_serve.h) where a bad value lies beside good ones, where values meet borders, angles to their bound, and
+in other company, against 64 bits and more.
 
 Bounds of the attention, as in test_gpu_q4_cache.py: a score is off by EPS_S = 2^-20 of the sum of the magnitudes that are added for it, a
 weight by twice that and 2^-20, an output by this times the largest magnitude of V's parts."""
@@ -13,6 +13,7 @@ import pytest
 torch = pytest.importorskip("torch")
 import cfi_b200 as cfi  # noqa: E402
 import q41_pages as q41  # noqa: E402
+import test_gpu_q4_cache as q4  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 EPS_S = 2.0 ** -20
@@ -172,3 +173,142 @@ def test_angles_to_their_bound(base, scale, lo, hi):
                 bound = 1e-7 + abs(pos[t]) * max(1.0, abs(float(rate))) * 2.0 ** (-45 if lo else -53)
                 worst = max(worst, err / (bound + 2.0 ** -23))
     assert worst <= 1.0, worst
+
+
+# ---- what earlier tests leave open ----
+@pytest.mark.parametrize("heads,kv,dim", [(12, 2, 128), (14, 2, 64), (8, 2, 128)])
+def test_a_sequence_alone_and_in_company(heads, kv, dim):
+    """Q4_1: the batch cuts a sequence in other places than it alone is cut; both results are within the bound of the formula."""
+    lens = [2500, 1, 300, 4096, 77]
+    call, check, out, keep = q4.case(heads, kv, dim, 16, lens)
+    check()
+    kp, vp, q, table, dl = keep
+    pages, width = kp.numel() // cfi.paged_page_bytes(cfi.Q4_1, 16, kv, dim), table.shape[1]
+    cache = cfi.paged_cache(cfi.Q4_1, kp.data_ptr(), vp.data_ptr(), pages, 16, kv, dim)
+    K, V = (q41.values(x.cpu().numpy(), pages, kv, 16, dim, i) for i, x in enumerate((kp, vp)))
+    alone = torch.empty(1, heads * dim, device=DEV)
+    for b, n in enumerate(lens):
+        own, cut = table[b:b + 1].contiguous(), dl[b:b + 1].clone()
+        for w in (width, -(-n // 16)):
+            t = own[:, :w].contiguous()
+            alone.fill_(7.0)
+            cfi.paged_attention(cache, q[b:b + 1].contiguous().data_ptr(), alone.data_ptr(), t.data_ptr(), cut.data_ptr(), 1, heads, w,
+                                1 / math.sqrt(dim), stream=stream())
+            torch.cuda.synchronize()
+            pos = np.arange(n)
+            sl = own[0].cpu().numpy()[pos // 16].astype(np.int64) * 16 + pos % 16
+            ends = lambda x: np.repeat(np.abs(x.reshape(len(x), kv, -1, 32)).max(3) * 3, 32, axis=2)  # noqa: E731
+            qq = np.abs(q[b].double().cpu().numpy().reshape(kv, -1, dim))
+            mags = float(np.einsum("hgd,nhd->hgn", qq, ends(K[sl])).max()) / math.sqrt(dim)
+            tol = 2 * (2 * EPS_S * mags + 2 * 2.0 ** -20) * ends(V[sl]).max()
+            assert float((alone[0] - out[b]).abs().max()) <= tol
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(14, 2, 64), (12, 2, 128), (32, 8, 128), (9, 3, 64)])
+def test_blocks_without_offsets_are_as_near_as_32_bits(heads, kv, dim):
+    """Q4_1 blocks whose minimum is zero have one part only: off from 64 bits by no more than four times what torch's 32 bits are, since
+    operands of 22 bits are off by up to four units of the 24th."""
+    def fill(k, v):
+        for x in (k, v):
+            x.abs_()
+            x[:, ::32] = 0
+
+    lens = [672, 1500, 77]
+    call, check, out, keep = q4.case(heads, kv, dim, 16, lens, offset=0.0, fill=fill, seed=9)
+    check()
+    pages = keep[1].numel() // (kv * q41.region_bytes(16, dim))
+    K, V = (torch.from_numpy(q41.values(keep[i].cpu().numpy(), pages, kv, 16, dim, i == 1)).to(DEV) for i in range(2))
+    table = keep[3].cpu().numpy()
+    mine, plain, size = 0.0, 0.0, 0.0
+    for b, n in enumerate(lens):
+        pos = np.arange(n)
+        at = torch.from_numpy(table[b][pos // 16].astype(np.int64) * 16 + pos % 16).to(DEV)
+        k, v = K[at].repeat_interleave(heads // kv, 1).transpose(0, 1), V[at].repeat_interleave(heads // kv, 1).transpose(0, 1)
+        q = keep[2][b].view(heads, 1, dim)
+
+        def formula(t):
+            s = (q.to(t) @ k.to(t).transpose(1, 2)) * (1 / math.sqrt(dim))
+            p = torch.exp(s - s.amax(-1, keepdim=True))
+            return ((p @ v.to(t)) / p.sum(-1, keepdim=True))[:, 0].double()
+
+        want = formula(torch.float64)
+        mine += float((out[b].view(heads, dim).double() - want).pow(2).sum())
+        plain += float((formula(torch.float32) - want).pow(2).sum())
+        size += float(want.pow(2).sum())
+    assert math.sqrt(mine) <= 4 * math.sqrt(plain) + 2.0 ** -24 * math.sqrt(size), (math.sqrt(mine / size), math.sqrt(plain / size))
+
+
+@pytest.mark.parametrize("ty", [cfi.T_F16, cfi.Q8_0, cfi.Q4_1])
+def test_rows_in_the_cache_do_not_depend_on_what_was_there(ty):
+    """cfi_norm_rope writes whole rows: over garbage, over zeros and without rows out beside them the cached values are the same, and slots
+    that are not named keep theirs."""
+    from test_gpu_norm_rope import make
+    heads, kv, dim, page, tokens = 12, 2, 128, 16, 90
+    x = make(tokens, heads, kv, dim)
+    pages = 8
+    n = cfi.paged_page_bytes(ty, page, kv, dim) * pages
+    slots = torch.randperm(pages * page, device=DEV)[:tokens].contiguous()
+    others = torch.tensor(np.setdiff1d(np.arange(pages * page), slots.cpu().numpy()), device=DEV)
+    back = []
+    garbage = torch.randint(0, 256, (2, n), device=DEV, dtype=torch.int32).to(torch.uint8)
+    for pools, kw in ((garbage, {}), (torch.zeros_like(garbage), {}), (garbage.clone(), dict(k_out=0, v_out=0))):
+        pools = pools.clone()
+        cache = cfi.paged_cache(ty, pools[0].data_ptr(), pools[1].data_ptr(), pages, page, kv, dim)
+
+        def read(at):
+            rows = torch.empty(2, len(at), kv * dim, dtype=torch.float16, device=DEV)
+            cfi.paged_kv_load(cache, at.data_ptr(), rows[0].data_ptr(), rows[1].data_ptr(), len(at), stream=stream())
+            torch.cuda.synchronize()
+            return rows.view(torch.int16)
+
+        before = read(others)
+        cfi.norm_rope(x["describe"](slots=slots.data_ptr(), **kw), cache, stream=stream())
+        back.append(read(slots))
+        assert torch.equal(read(others), before)
+    assert torch.equal(back[0], back[1]) and torch.equal(back[0], back[2])
+
+
+# ---- the driver after a call that failed ----
+@pytest.mark.parametrize("tables", ["host", "device"])
+def test_a_server_goes_on_after_a_failed_call(monkeypatch, tables):
+    """A prompt and a step that raise in the second layer, and again: the same bits as if they had not."""
+    import decode
+    import serve
+    ctx = cfi.Ctx(0)
+    cfg = decode.Config(hidden=256, layers=2, n_head=4, n_kv_head=2, head_dim=64, ffn=512, vocab=1024, prompt=8, n_ctx=16)
+    m = decode.DecodeModel(torch, ctx, "cuda", cfg, fused=1)
+    out = []
+    for broken in (False, True):
+        fail = []
+
+        def once(real, name):
+            def call(*a, **k):
+                if fail and fail[0] == name:
+                    fail.pop(0)
+                    if not fail or fail[0] != name:
+                        raise MemoryError(name)
+                return real(*a, **k)
+            return call
+
+        for name in ("paged_attention", "packed_attention"):
+            monkeypatch.setattr(cfi, name, once(getattr(cfi, name), name))
+        s = serve.Server(torch, ctx, m, cfi.Q4_1, 16, 20, tables=tables)
+        a, b = serve.Sequence([i * 7 % 1024 for i in range(48)]), serve.Sequence([5, 6, 7])
+        got = []
+        for call, name in ((lambda: s.prefill([a, b]), "packed_attention"), (lambda: s.step([a, b]), "paged_attention"),
+                           (lambda: s.step([b, a]), "paged_attention")):
+            if broken:
+                fail[:] = [name] * 2  # the second layer's
+                with pytest.raises(MemoryError):
+                    call()
+            got.append(call())
+            a.tokens.append(11), b.tokens.append(12)
+        if tables == "device":
+            assert int(s.state.status) == 0 and s.state.cached[[a.row, b.row]].tolist() == [50, 5]
+        s.cut([a], [20])
+        s.release(a), s.release(b)
+        assert (s.n_free if tables == "device" else len(s.free)) == 20
+        monkeypatch.undo()
+        out.append(got)
+    assert all(torch.equal(x, y) for x, y in zip(*out))
+    ctx.close()
