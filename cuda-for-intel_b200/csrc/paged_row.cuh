@@ -6,7 +6,8 @@
 // quotient in 32 bits is off by less than 2^-16 (2^-24 of it each by range and difference, 2^-22 by the quotient): where a value of a
 // warp comes nearer to a border than that, its values are compared with their borders, 30 (x - min) with (2 q + 1) (max - min), as sums of
 // two f32 numbers each (differences of f16 values meet borders exactly).  d is off by 2 units of its last place in 32 bits and worked out
-// in 64 (a difference that 64 bits do not hold as the sum of two) where a border of f16 is nearer.
+// in 64 (a difference that 64 bits do not hold as the sum of two) where a border of f16 is nearer or d is no normal f16 number; the
+// quotients only where a block's range is below 1.5e-35 or above 9e5.
 #pragma once
 #include "paged_cache.cuh"
 
@@ -118,8 +119,10 @@ template <int D, bool SRC_F16> CFI_DEV void put_q4_1(const Row8& r, uint8_t* reg
     float lo, hi;
     block_ends<SRC_F16>(r, &lo, &hi);
     const float range = hi - lo, inv = __fdividef(15.0f, range), d32 = range * (1.0f / 15.0f);
-    // d at a border of f16; d outside its normal numbers, where 32 bits do not hold the quotients either
-    const bool wide = !(d32 >= 6.2e-5f && d32 <= 6.0e4f), tie = (__float_as_uint(d32) & 0x1fffu) - 0x0ffcu <= 8u;
+    // where 32 bits do not hold the quotients (f16 values are not that near to one another); where d is outside f16's normal numbers or at a border
+    // of them.  Blocks of one value, whose q and d are 0, need neither: rows of zeros are common, and so are a warp's lanes without a row.
+    const bool wide = !(d32 <= 6.0e4f) || (!SRC_F16 && d32 < 1e-36f && range != 0.0f),
+               tie = !(d32 >= 6.2e-5f && d32 <= 6.0e4f) ? range != 0.0f : (__float_as_uint(d32) & 0x1fffu) - 0x0ffcu <= 8u;
     // v + 1.5 * 2^23 is rounded to a whole number, whose last bits are q: with each times 16 and the next, the rest adds up to
     // a number of its own
     uint32_t w = 0, rest = 0;
@@ -145,7 +148,7 @@ template <int D, bool SRC_F16> CFI_DEV void put_q4_1(const Row8& r, uint8_t* reg
         }
     }
     uint16_t d = f2h_bits(d32);
-    if (wide || tie) {
+    if (tie) {
         const Apart all = apart(hi, lo);
         double d64 = all.x / 15.0;
         // exactly so: what the difference was rounded by decides where d lies on a border
@@ -162,6 +165,7 @@ template <int D, bool SRC_F16> CFI_DEV void put_q4_1(const Row8& r, uint8_t* reg
             }
         }
     }
+    if (range == 0.0f) w = 0;
     uint16_t m = f2h_bits(lo);
     if ((d & 0x7c00) == 0x7c00 || (m & 0x7c00) == 0x7c00) {
         d = m = 0x7fff;

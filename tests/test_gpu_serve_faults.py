@@ -96,11 +96,11 @@ def test_bad_blocks_of_v_cost_the_other_dims_nothing(ty, heads, kv, dim, blocks,
 # ---- Q4_1 values on borders, beside a minimum far below them ----
 def exactly(block):
     """Scale (f16), minimum (f16) and whole numbers of a block, from fractions."""
-    if abs(block.min()) >= 65520:
-        return math.nan, math.nan, [0] * 32
     x = [Fraction(float(v)) for v in block]
     lo, wide = min(x), max(x) - min(x)
     exact = wide / 15
+    if abs(lo) >= 65520 or exact >= 65520:  # past f16
+        return math.nan, math.nan, [0] * 32
     near = np.float16(float(exact))
     around = [np.nextafter(near, np.float16(-np.inf)), near, np.nextafter(near, np.float16(np.inf))]
     d = min(around, key=lambda c: (abs(Fraction(float(c)) - exact), int(np.float16(c).view(np.uint16)) & 1))
@@ -133,6 +133,42 @@ def test_scales_and_values_on_borders():
     for i in range(2):
         got = q41.values(pools[i].cpu().numpy(), pages, 1, page, 128, i == 1)[:n, 0]
         np.testing.assert_array_equal(got, want)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.float16])
+def test_whole_numbers_of_blocks_of_all_sizes(dt):
+    """From f32's least numbers to where a scale passes f16: a block's whole numbers are the exact quotients', values next to borders and blocks
+    of one value among them, and scale and minimum the exact ones'."""
+    rng = np.random.default_rng(3)
+    blocks = []
+    for k in range(-148, 17) if dt == torch.float32 else range(-24, 12):
+        for offset in (0.0, 1.0, -7.3):
+            step = np.ldexp(1 + rng.random(), k)
+            at = rng.integers(1, 16, 32) - 0.5
+            at[:2] = 0, 15
+            b = ((at + offset) * step).astype(np.float32)
+            b[2:] = np.where(rng.random(30) < 0.5, b[2:], np.nextafter(b[2:], np.float32(rng.choice([-1, 1]) * 1e38)))
+            blocks.append(b)
+        blocks.append(np.full(32, np.float32(step)))
+    x = np.array(blocks, dtype=np.float32)
+    x = x.astype(np.float16).astype(np.float32) if dt == torch.float16 else x
+    x = np.concatenate([x, np.zeros((-len(x) % 4, 32), dtype=np.float32)])
+    n, page = len(x) // 4, 16
+    pages = -(-n // page)
+    rows = torch.from_numpy(x.reshape(n, 128)).to(DEV).to(dt)
+    pools = torch.zeros(2, cfi.paged_page_bytes(cfi.Q4_1, page, 1, 128) * pages, dtype=torch.uint8, device=DEV)
+    cache = cfi.paged_cache(cfi.Q4_1, pools[0].data_ptr(), pools[1].data_ptr(), pages, page, 1, 128)
+    slots = torch.arange(n, device=DEV)
+    cfi.paged_kv_store(cache, rows.data_ptr(), rows.data_ptr(), slots.data_ptr(), n, src_type=int(dt == torch.float16), stream=stream())
+    torch.cuda.synchronize()
+    parts = [exactly(b) for b in x]
+    q = np.array([p[2] for p in parts]).reshape(n, 128)
+    want = np.array([[i * d + m for i in qs] for d, m, qs in parts]).reshape(n, 128)
+    for i in range(2):
+        np.testing.assert_array_equal(q41.values(pools[i].cpu().numpy(), pages, 1, page, 128, i == 1)[:n, 0], want)
+        bare = pools[i].cpu().numpy().reshape(pages, 1280).copy()  # scales of 1 and minima of 0
+        bare[:, 1024:].view(np.uint16).reshape(pages, 16, 2, 4)[:] = np.array([0x3c00, 0], dtype=np.uint16)[None, None, :, None]
+        np.testing.assert_array_equal(q41.values(bare.reshape(-1), pages, 1, page, 128, i == 1)[:n, 0], q)
 
 
 # ---- angles ----
