@@ -20,9 +20,17 @@ namespace {
 
 constexpr int NR_RATES = 64;
 // Few rows: a head to a group of lanes.  Many: a run of up to NR_HEADS heads of one token to a group, which reads its angles once; from
-// NR_MANY heads a group of all SMs' CTAs on.  Measured, a head to a group against runs: 631 rows of 12/2 heads of 128 5.4 to 6.8 us, 300 of
-// 32/8 6.9 to 7.4, 390 8.4 to 7.7, 700 13.8 to 9.4, 1500 of 12/2 10.5 to 8.1; 1000 of 16/16 of 64 7.9 to 9.0.
-constexpr int NR_MANY = 8;
+// nr_many() heads a group of all SMs' CTAs on.  Measured (us), a head to a group against runs, at 5, 7, 9 and 12 such heads:
+//   12/2 heads of 128, f16 6.0 to 6.1, 7.1 to 7.0, 9.1 to 7.5, 11.7 to 7.6; Q8_0 6.3 to 4.6, 8.2 to 6.0, 9.7 to 6.0, 12.5 to 8.8; Q4_1 7.7 to
+//      5.5, 9.9 to 5.6, 12.1 to 8.7, 15.4 to 9.4;
+//   32/8 of 128, f16 6.0 to 5.4, 7.8 to 6.3, 9.4 to 7.7, 11.9 to 8.4; Q8_0 6.3 to 7.4, 8.1 to 8.4, 9.8 to 8.6, 12.6 to 9.0; Q4_1 6.8 to 8.1, 9.0
+//      to 8.7, 11.3 to 9.1, 14.7 to 9.3;
+//   14/2 of 64, f16 5.0 to 7.0, 6.3 to 7.9, 7.6 to 5.7, 9.4 to 8.5; Q8_0 6.0 to 6.8, 7.9 to 7.0, 9.0 to 7.0, 11.7 to 11.2; Q4_1 7.3 to 6.4, 9.6 to
+//      6.5, 11.9 to 6.7, 15.0 to 11.7;
+//   16/16 of 64, f16 4.5 to 5.4, 5.4 to 6.2, 6.5 to 7.6, 8.0 to 8.4; Q8_0 5.2 to 8.5, 6.5 to 9.1, 7.8 to 9.4, 9.8 to 9.7; Q4_1 6.4 to 8.7, 8.2 to
+//      9.1, 10.1 to 9.4, 12.9 to 9.5.
+// Where they cross is a matter of how full the last wave of CTAs is: no limit is right for all, and these cost 3.2 us at most.
+constexpr int nr_many(int head_dim) { return head_dim == 128 ? 7 : 8; }
 // Measured, 8191 rows of 32/8 heads of 128 normed, turned and put into f16 pages, 61 us (5.0 TB/s): runs of 4, 8, 12, 16 heads 66, 63, 68, 73
 // (before the last step); 1, 2, 4 heads' loads together 87, 65, 73; blocks of 256, 128, 64, 32 threads 65, 64, 63, 63; 64 and 72 registers
 // (16 and 14 blocks of 64 an SM) 60.7 and 62.2, but 1000 rows 10.0 and 9.4.  Norm weights read for each head and angles
@@ -272,7 +280,7 @@ extern "C" int cfi_norm_rope(const CfiNormRope* r, const CfiPagedCache* c, void*
     }
     const int heads = r->n_head + (r->k ? r->n_kv_head : 0) + (r->v ? r->n_kv_head : 0), lanes = r->head_dim / 8;
     if ((long long)r->n_tokens * heads > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
-    const bool many = (long long)r->n_tokens * heads >= NR_MANY * (long long)cfi_sm_count() * (nr_threads(false) / lanes);
+    const bool many = (long long)r->n_tokens * heads >= nr_many(r->head_dim) * (long long)cfi_sm_count() * (nr_threads(false) / lanes);
     const int groups = nr_threads(many) / lanes;
     const int count[3] = {r->n_head, r->k ? r->n_kv_head : 0, r->v ? r->n_kv_head : 0};
     for (int i = 0; i < 3; i++) {
