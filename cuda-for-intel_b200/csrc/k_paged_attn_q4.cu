@@ -23,10 +23,11 @@
 // is position 8 n + 4 e + (c ^ 3 e), so that no two lanes read the same bank of K or of V.
 // The minima of K meet the sums of q over each block in one MMA for 8 positions, those of V the weights in one for 16.
 //
-// Bound by instruction issue: an MMA of 16 x 8 x 16 holds its part of the SM for 8 cycles in which nothing else is issued (measured: 8 + N
-// cycles for one beside N other instructions), and a tile of 32 positions is 38 (five to eight heads: 70) of them and 720 other instructions
-// of a warp, where the memory's rate allows 880 cycles.  Two CTAs an SM with up to 255 registers a thread: with three, 8 to 12 % more
-// instructions, and no faster.  Measured: 8 sequences of 9000 to 65000 positions, 32/8 heads of 128, 71 us, 4.0 TB/s; 8 of 64000
+// Bound by instruction issue and by chains that two warps a scheduler do not cover.  An MMA of 16 x 8 x 16 holds its part of the SM for 8 cycles in
+// which nothing else is issued (measured: 8 + N cycles for one beside N other instructions), and a tile of 32 positions is 38 (five to eight heads:
+// 70) of them and 720 other instructions of a warp, 1020 cycles where the memory's rate allows 880: of the 71 us below, that is 50.  The others are
+// idle, a fifth to a quarter of the cycles, between an MMA, its sums, the maximum, the weights and the next MMA.  Two CTAs an SM with up to 255
+// registers a thread: with three, 8 to 12 % more instructions, and no faster.  Measured: 8 sequences of 9000 to 65000 positions, 32/8 heads of 128, 71 us, 4.0 TB/s; 8 of 64000
 // 151 us, 4.3 TB/s (64/8 heads 175); 64 of 16 to 4096, 12/2 heads of 128, 15.0 us; one of 672, 14/2 heads of 64, 5.4 us.
 #include "paged_attn.cuh"
 #include "sm100_ptx.cuh"

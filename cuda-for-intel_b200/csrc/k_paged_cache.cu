@@ -14,8 +14,9 @@ namespace {
 // (6.2 TB/s of reads and writes) and 80 us; storing 8192 rows 12.7, 12.7 and 13.8 us (10.3, 5 TB/s, since the maximum of f16
 // rows is taken in f16 and the bytes come from one conversion: it is bound by issue), a step's 48 rows 1.2, 1.5 and 1.9.
 constexpr int PC_THREADS = 256, PC_STORE_ITEMS = 1, PC_LOAD_ITEMS = 2;
-// Q4_1: reading back 65537 rows 52 us (6.7 TB/s of reads and writes), storing 8192 f16 rows 21: bound by issue, 390 instructions of a
-// warp for 8 values of K and of V a lane.  With two items a thread 73.3 us become 72.4, and a step's 48 rows 3.6 become 4.3.
+// Q4_1: reading back 65537 rows 52 us (6.7 TB/s of reads and writes), storing 8192 f16 rows 21 (17 from L2): bound by issue, 390 instructions of a
+// warp for 8 values of K and of V a lane; of f16 values one of a warp is nearly always near a border, so that
+// both ways of paged_row.cuh are gone.  With two items a thread 73.3 us become 72.4, and a step's 48 rows 3.6 become 4.3.
 constexpr int PC_Q4_ITEMS = 1;
 
 struct PcArgs {

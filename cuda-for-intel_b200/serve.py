@@ -47,9 +47,11 @@ class Server:
     stream that is torch's current one then, after what the calls before it did on theirs.
 
     fused: biases, rope and the rows into the cache by one cfi_norm_rope a layer (its angles are right at any position; those of
-    rope_neox are in 32 bits).  None: where the cache is Q4_1 or there are norms.  norms: of each layer the weights (f32, head_dim)
-    that the heads of q and of k are normed with, for models that have them.
-    tables: "host", or "device" for page tables that cfi_paged_place keeps, for up to `rows` sequences at a time."""
+    rope_neox are in 32 bits).  None: where the cache is Q4_1 or there are norms.  norms: of each layer the weights (f32, head_dim,
+    on the model's device) that the heads of q and of k are normed with, for models that have them.
+    tables: "host", or "device" for page tables that cfi_paged_place keeps, for up to `rows` sequences at a time; a step's attention is then given
+    a table as wide as the pool, for which it is cut as for long sequences (one of 768 takes 7.4 us instead of 5.5).
+    A call that raises leaves what was cached before it; it can be made again."""
 
     def __init__(self, torch, ctx, model, cache_type=cfi.T_F16, page_size=16, pages=256, seed=0, fused=None, norms=None, tables="host",
                  rows=64):
@@ -182,8 +184,7 @@ class Server:
         return status
 
     def cut(self, seqs, lengths):
-        """The sequences keep their first lengths[i] tokens and what is cached of them (drafted tokens that were not taken, say): the
-        pages behind go back."""
+        """The sequences keep their first lengths[i] tokens and what is cached of them: the pages behind go back."""
         self._once(seqs)
         self._begin()
         self._shrink(seqs, lengths)

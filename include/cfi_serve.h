@@ -9,7 +9,8 @@
  * `stream` is a cudaStream_t, and each function returns 0 or a CUDA error code: cudaErrorInvalidValue,
  * before anything is launched, for arguments outside what is documented here.  Nothing is
  * allocated but per-stream scratch, which grows outside stream capture only (run the largest
- * call once before capturing).  Lengths, page tables, slots and sampling settings are read from
+ * call once before capturing).  A captured graph keeps the scratch of the stream that it was captured on: graphs that were captured on
+ * one stream, and what else runs on that stream, do not run at the same time.  Lengths, page tables, slots and sampling settings are read from
  * device memory by the kernels: a captured graph can be replayed with new ones.
  *
  * Types are ggml's ids: 0 F32, 1 F16, 3 Q4_1, 8 Q8_0.
@@ -86,7 +87,7 @@ CFI_API int cfi_paged_kv_load(const CfiPagedCache *cache, const int64_t *slots, 
  * K and V carry 22 bits, a query's values no bits below 2^-38 (Q4_1: 2^-30) of their head's largest and a weight (Q8_0 and
  * Q4_1: times its scale of V) none below 2^-39 of the largest (Q4_1: scales below 2^-15 count as that): the results are those of
  * 32-bit arithmetic on the cached values, as long as the scores are within the range of f32.  (Q4_1: of the scaled whole numbers and
- * the minima, which are summed apart.)
+ * the minima, which are summed apart; the minima of K meet the sums of a query's values over each block, of which 22 bits are kept.)
  * A NaN makes NaN of what the formula takes it into and of nothing else: in q its head's outputs, in a row of K within
  * the length those of its kv head's query heads, in V the same dims of them.  An infinity there makes of these NaN
  * or what the formula gives.  Bounds: n_seq 65535, and n_seq * n_kv_head * ceil(n_head / n_kv_head / 8) *
